@@ -115,7 +115,7 @@ def _quantised(x):
     floor = amax.clamp_min(2.0 ** -24)
     bad = ~torch.isfinite(x).all(-1, keepdim=True)
     scale = torch.where(bad, torch.full_like(amax, math.nan), floor / 448.0)
-    code = torch.where(bad, torch.zeros_like(x), (x * (448.0 / floor)).clamp(-448.0, 448.0))
+    code = torch.where(bad, torch.zeros_like(x), (x * torch.div(torch.full_like(floor, 448.0), floor)).clamp(-448.0, 448.0))
     return code.to(torch.float8_e4m3fn), scale.squeeze(-1)
 
 
