@@ -31,7 +31,8 @@ EXPORTED = [
     "cfb_wide_create", "cfb_wide_run", "cfb_wide_error", "cfb_wide_info", "cfb_wide_destroy",
     "cfb_ring_write", "cfb_ring_gather", "cfb_tree_gdn_verify", "cfb_vae_workspace", "cfb_vae_create",
     "cfb_vae_plan_workspace", "cfb_vae_plan_build", "cfb_tree_attn_merge", "cfb_tree_verify_workspace",
-    "cfb_tree_verify_greedy", "cfb_tree_gdn_factor",
+    "cfb_tree_verify_greedy", "cfb_tree_gdn_factor", "cfb_kv_write", "cfb_kv_read", "cfb_paged_attn_workspace",
+    "cfb_paged_attn", "cfb_gdn_step", "cfb_gdn_chunk_workspace", "cfb_gdn_chunk",
 ]
 ABI_VERSION = 5
 XROWS, XFLOATS = 64, 18          # CFB_XROWS, CFB_XFLOATS: the merged-list exchange rows
@@ -96,6 +97,24 @@ class VaeSide(C.Structure):
                 ("layer", C.POINTER(VaeLayer)), ("out_proj", Linear)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
+                ("scale_page_stride", C.c_int64), ("scale_head_stride", C.c_int64), ("scale_slot_stride", C.c_int64),
+                ("pages", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int), ("dtype", C.c_int)]
+
+
+class GdnArgs(C.Structure):
+    _fields_ = [("A_log", C.c_void_p), ("A_log_dtype", C.c_int), ("dt_bias", C.c_void_p), ("dt_bias_dtype", C.c_int),
+                ("a", C.c_void_p), ("a_dtype", C.c_int), ("a_stride", C.c_int64),
+                ("b", C.c_void_p), ("b_dtype", C.c_int), ("b_stride", C.c_int64),
+                ("q", C.c_void_p), ("q_stride", C.c_int64), ("k", C.c_void_p), ("k_stride", C.c_int64),
+                ("v", C.c_void_p), ("v_stride", C.c_int64), ("o", C.c_void_p), ("o_stride", C.c_int64),
+                ("dtype", C.c_int), ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("slot_stride", C.c_int64),
+                ("slots", C.c_int), ("init_slot", C.c_void_p), ("out_slot", C.c_void_p), ("scale", C.c_float),
+                ("H", C.c_int), ("HV", C.c_int), ("K", C.c_int), ("V", C.c_int)]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -146,6 +165,16 @@ def _declare(lib):
     lib.cfb_tree_verify_workspace.restype = sz
     lib.cfb_tree_verify_greedy.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp,
                                            sz, vp, vp]
+    lib.cfb_kv_write.argtypes = [C.POINTER(KvCache), vp, i64, i64, vp, i64, i64, i32, vp, i32, vp]
+    lib.cfb_kv_read.argtypes = [C.POINTER(KvCache), vp, i32, vp, i64, i64, vp, i64, i64, i32, vp]
+    lib.cfb_paged_attn_workspace.argtypes = [i32, i32, i32]
+    lib.cfb_paged_attn_workspace.restype = sz
+    lib.cfb_paged_attn.argtypes = [vp, i64, i64, C.POINTER(KvCache), vp, i64, i32, vp, vp, vp, i64, i64, vp, C.c_float,
+                                   i32, i32, i32, i32, i32, vp, sz, vp]
+    lib.cfb_gdn_step.argtypes = [C.POINTER(GdnArgs), i32, vp]
+    lib.cfb_gdn_chunk_workspace.argtypes = [i32, i32, i32]
+    lib.cfb_gdn_chunk_workspace.restype = sz
+    lib.cfb_gdn_chunk.argtypes = [C.POINTER(GdnArgs), vp, i32, i32, vp, sz, vp]
     return lib
 
 

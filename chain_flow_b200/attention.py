@@ -1,0 +1,77 @@
+"""Attention of a step's new tokens over a paged key/value cache, with its log-sum-exp, on
+cfb_paged_attn (cfb_attn.cu): prompt chunks and single tokens (causal), and the prefix half of a
+tree step, whose outputs ``tree.tree_attn_merge`` joins with the tree's own part."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .kv_cache import HEAD_DIMS, PagedKVCache
+
+_DT = {torch.float16: 1, torch.bfloat16: 2}
+
+
+class PagedAttention:
+    """Owns the workspace of calls with ``heads`` query heads over ``kv_heads`` kv heads of
+    ``head_dim``; a call allocates only outputs it is not given. Calls share the workspace: order
+    them on one stream."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, device=None):
+        self.lib = _lib.load()
+        if heads <= 0 or kv_heads <= 0 or heads % kv_heads or heads // kv_heads > 128 or head_dim not in HEAD_DIMS:
+            raise _lib.CfbError(f"PagedAttention: heads must be a multiple (up to 128) of kv_heads and head_dim one of "
+                                f"{HEAD_DIMS}, got {heads} / {kv_heads} / {head_dim}")
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.ws_bytes = int(self.lib.cfb_paged_attn_workspace(heads, kv_heads, head_dim))
+        self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
+        self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+
+    def __call__(self, query, cache: PagedKVCache, page_table, kv_len, cu_q, *, scale: float | None = None,
+                 causal: bool = True, out=None, lse=None, stream=None):
+        """(out [T, heads, head_dim], lse fp32 [heads, T], natural log). Request b owns the query rows
+        [cu_q[b], cu_q[b + 1]) and the first kv_len[b] positions of the pages page_table[b]; with
+        ``causal`` its new tokens are the last of those positions and see up to themselves, without
+        it they see all of them. Rows that see nothing get 0 and -inf. query fp16 or bf16 (the
+        cache's dtype, or either over an e4m3 cache), page_table int32 [B, width], kv_len int32 [B],
+        cu_q int32 [B + 1], all on the GPU: nothing is read back. scale defaults to
+        head_dim ** -0.5. Rows outside every request are left as they are (given buffers) or
+        undefined (new ones)."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self(query, cache, page_table, kv_len, cu_q, scale=scale, causal=causal, out=out, lse=lse)
+        for t, n in ((query, "query"), (page_table, "page_table"), (kv_len, "kv_len"), (cu_q, "cu_q")):
+            _lib.require_cuda(t, n)
+            if t.device != cache.device:
+                raise _lib.CfbError(f"{n} is on {t.device}, the cache on {cache.device}")
+        if query.dim() != 3 or query.shape[1] != self.heads or query.shape[2] != self.head_dim:
+            raise _lib.CfbError(f"query: expected [T, {self.heads}, {self.head_dim}], got {list(query.shape)}")
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
+            raise _lib.CfbError("PagedAttention: the cache has other kv heads or another head dim")
+        dt = _DT.get(query.dtype)
+        if dt is None or (cache.k_scale is None and query.dtype != cache.dtype):
+            raise _lib.CfbError("PagedAttention: query must be fp16 or bf16, the cache's own dtype unless it is e4m3")
+        B = kv_len.numel()
+        if page_table.dim() != 2 or page_table.shape[0] != B or kv_len.dim() != 1 or cu_q.dim() != 1 or cu_q.numel() != B + 1:
+            raise _lib.CfbError("PagedAttention: page_table [B, width], kv_len [B] and cu_q [B + 1] disagree")
+        if page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+            page_table = page_table.to(torch.int32).contiguous()
+        kv_len, cu_q = kv_len.to(torch.int32).contiguous(), cu_q.to(torch.int32).contiguous()
+        if query.stride(2) != 1:
+            raise _lib.CfbError("query needs a contiguous head dim")
+        T = query.shape[0]
+        if out is None:
+            out = torch.empty(T, self.heads, self.head_dim, dtype=query.dtype, device=query.device)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(2) != 1:
+            raise _lib.CfbError("out must have the query's shape, dtype and device, and a contiguous head dim")
+        if lse is None:
+            lse = torch.empty(self.heads, T, dtype=torch.float32, device=query.device)
+        elif tuple(lse.shape) != (self.heads, T) or lse.dtype != torch.float32 or lse.device != query.device \
+                or not lse.is_contiguous():
+            raise _lib.CfbError(f"lse must be contiguous fp32 [{self.heads}, {T}] on the query's device")
+        _lib.check(self.lib.cfb_paged_attn(
+            query.data_ptr(), query.stride(0), query.stride(1), cache.desc, page_table.data_ptr(), page_table.stride(0),
+            page_table.shape[1], kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+            lse.data_ptr(), float(self.head_dim ** -0.5 if scale is None else scale), T, B, self.heads, int(causal), dt,
+            self.ws_ptr, self.ws_bytes, _lib.stream_ptr()), "cfb_paged_attn")
+        return out, lse

@@ -5,7 +5,9 @@
 independent trees in one launch. ``make_tree`` builds the seeded BFS parent arrays the
 benchmarks use (parent < child, bounded depth and branching). ``gdn_verify`` is the in-engine
 variant of the reference's vLLM patch (gate from the model's raw parameters, slot-addressed
-states, a path-parallel walk of each row's ancestor chain; cfb_tree_gdn_verify).
+states, a path-parallel walk of each row's ancestor chain; cfb_tree_gdn_verify). ``ChunkedGdn`` and
+``gdn_step`` run the same recurrence without a tree, over prompts and single tokens (cfb_gdn_chunk,
+cfb_gdn_step).
 """
 from __future__ import annotations
 
@@ -155,3 +157,97 @@ def gdn_factor(A_log, dt_bias, a, b, q, k, v, o, state, chain, depth, init_slot,
         v.data_ptr(), o.data_ptr(), _DTYPE_CODE[q.dtype], state.data_ptr(), state.stride(0), ch.data_ptr(),
         ch.stride(0), dp.data_ptr(), isl.data_ptr(), rs.data_ptr(), rc.data_ptr(), rs.numel(), int(n_max),
         float(scale), H, HV, K, V, _lib.stream_ptr()), "cfb_tree_gdn_factor")
+
+
+def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B):
+    """(cfb_gdn_args, the converted index tensors, which the caller keeps until the launch)."""
+    T = q.shape[0]
+    H, K = q.shape[1], q.shape[2]
+    HV, V = v.shape[1], v.shape[2]
+    out_state = state if out_state is None else out_state
+    for t, n, shape in ((q, "q", (T, H, K)), (k, "k", (T, H, K)), (v, "v", (T, HV, V)), (o, "o", (T, HV, V)),
+                        (a, "a", (T, HV)), (b, "b", (T, HV)), (A_log, "A_log", (HV,)), (dt_bias, "dt_bias", (HV,)),
+                        (state, "state", (state.shape[0], HV, V, K)), (out_state, "out_state", tuple(state.shape)),
+                        (init_slot, "init_slot", (B,)), (out_slot, "out_slot", (B,))):
+        _lib.require_cuda(t, n)
+        if t.device != q.device:
+            raise _lib.CfbError(f"{what}: {n} is on {t.device}, q on {q.device}")
+        if tuple(t.shape) != shape:
+            raise _lib.CfbError(f"{what}: {n} must be {list(shape)}, got {list(t.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, o)):
+        raise _lib.CfbError(f"{what}: q, k, v, o must share one dtype, fp16 or bf16")
+    for t in (A_log, dt_bias, a, b):
+        if t.dtype not in _DTYPE_CODE:
+            raise _lib.CfbError(f"{what}: a, b, A_log and dt_bias must be fp32, fp16 or bf16")
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
+        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+            raise _lib.CfbError(f"{what}: {n} needs contiguous heads (any token stride)")
+    if HV > 1 and any(t.stride(-1) != 1 for t in (a, b, A_log, dt_bias)):
+        raise _lib.CfbError(f"{what}: a, b, A_log and dt_bias need contiguous heads")
+    for t, n in ((state, "state"), (out_state, "out_state")):
+        if t.dtype != torch.float32 or t.stride(3) != 1 or t.stride(2) != K or (HV > 1 and t.stride(1) != V * K) \
+                or t.stride(0) != state.stride(0):
+            raise _lib.CfbError(f"{what}: {n} must be fp32 [slots, HV, V, K] with contiguous slots (one slot stride)")
+    init, to = (t.to(torch.int32).contiguous() for t in (init_slot, out_slot))
+    args = _lib.GdnArgs(
+        A_log.data_ptr(), _DTYPE_CODE[A_log.dtype], dt_bias.data_ptr(), _DTYPE_CODE[dt_bias.dtype],
+        a.data_ptr(), _DTYPE_CODE[a.dtype], a.stride(0), b.data_ptr(), _DTYPE_CODE[b.dtype], b.stride(0),
+        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), o.data_ptr(), o.stride(0),
+        _DTYPE_CODE[q.dtype], state.data_ptr(), out_state.data_ptr(), state.stride(0), state.shape[0], init.data_ptr(),
+        to.data_ptr(), float(scale), H, HV, K, V)
+    return args, (init, to)
+
+
+def gdn_step(A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, *, scale: float, out_state=None,
+             stream=None) -> None:
+    """One token of the gated delta rule for each of B requests (cfb_gdn_step): row b walks from
+    ``state[init_slot[b]]`` (negative: zeros), writes ``o[b]`` and ``out_state[out_slot[b]]``
+    (default: ``state`` itself; negative: not kept). q, k [B, H, 128], v, o [B, HV, V] fp16 or bf16
+    with contiguous heads; a, b [B, HV] and A_log, dt_bias [HV] fp32 / fp16 / bf16; state fp32
+    [slots, HV, V, 128]."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return gdn_step(A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale=scale, out_state=out_state)
+    lib = _lib.load()
+    B = q.shape[0]
+    args, keep = _sequence_args("gdn_step", A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B)
+    _lib.check(lib.cfb_gdn_step(C.byref(args), B, _lib.stream_ptr()), "cfb_gdn_step")
+
+
+class ChunkedGdn:
+    """The gated delta rule over whole sequences (cfb_gdn_chunk) for calls of up to ``max_tokens``
+    tokens of up to ``max_requests`` requests and ``value_heads`` value heads. Owns the workspace,
+    so a call allocates nothing; calls share it, so order them on one stream."""
+
+    def __init__(self, max_tokens: int, max_requests: int, value_heads: int, device=None):
+        self.lib = _lib.load()
+        if max_tokens < 0 or max_requests <= 0 or value_heads <= 0:
+            raise _lib.CfbError("ChunkedGdn: max_requests and value_heads must be positive, max_tokens not negative")
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.max_tokens, self.max_requests, self.value_heads = max_tokens, max_requests, value_heads
+        self.ws_bytes = int(self.lib.cfb_gdn_chunk_workspace(max_tokens, max_requests, value_heads))
+        self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
+        self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+
+    def __call__(self, A_log, dt_bias, a, b, q, k, v, o, state, cu_seqlens, init_slot, out_slot, *, scale: float,
+                 out_state=None, stream=None) -> None:
+        """Request b's tokens are the rows [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [B + 1], on the
+        GPU), walked from ``state[init_slot[b]]``; arguments otherwise as ``gdn_step``. Rows of no
+        request are not written."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self(A_log, dt_bias, a, b, q, k, v, o, state, cu_seqlens, init_slot, out_slot, scale=scale,
+                            out_state=out_state)
+        _lib.require_cuda(cu_seqlens, "cu_seqlens")
+        B = cu_seqlens.numel() - 1
+        if cu_seqlens.dim() != 1 or B < 0 or cu_seqlens.device != q.device:
+            raise _lib.CfbError("ChunkedGdn: cu_seqlens must be 1-D [requests + 1] on q's device")
+        T, HV = q.shape[0], v.shape[1]
+        if T > self.max_tokens or B > self.max_requests or HV > self.value_heads:
+            raise _lib.CfbError(f"ChunkedGdn: {T} tokens / {B} requests / {HV} value heads exceed this object's "
+                                f"{self.max_tokens} / {self.max_requests} / {self.value_heads}")
+        args, keep = _sequence_args("ChunkedGdn", A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale,
+                                    out_state, B)
+        cu = cu_seqlens.to(torch.int32).contiguous()
+        _lib.check(self.lib.cfb_gdn_chunk(C.byref(args), cu.data_ptr(), T, B, self.ws_ptr, self.ws_bytes,
+                                          _lib.stream_ptr()), "cfb_gdn_chunk")

@@ -384,6 +384,100 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
                                   int32_t* accepted_len, int32_t* row_argmax, void* ws,
                                   size_t ws_bytes, int* err, void* stream);
 
+/* ---- the target model's side of a step: paged cache, attention over it, gated delta rule --------
+ * The key/value cache of one full-attention layer: rows of `dim` elements in pages of page_size
+ * slots, kept as fp16 (dtype 1), bf16 (2) or e4m3 (3). Row (slot, kv head h) of a flat slot =
+ * page * page_size + offset is at page * page_stride + h * head_stride + offset * slot_stride
+ * elements of k and of v; its fp32 scale (dtype 3 only) at page * scale_page_stride +
+ * h * scale_head_stride + offset * scale_slot_stride of k_scale and of v_scale. k and v: 16-byte
+ * aligned, strides multiples of 16 bytes. Supported: dim in {64, 128, 256}. */
+typedef struct cfb_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;              /* dtype 3 only, else NULL */
+  float* v_scale;
+  int64_t page_stride, head_stride, slot_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
+  int pages, page_size, kv_heads, dim;
+  int dtype;
+} cfb_kv_cache;
+
+/* Write the rows of T tokens (key, value [T, kv_heads, dim] of `dtype` 1 or 2, strides in elements,
+ * rows 16-byte aligned) to the slots slots[t] (int64; negative or past the pool: the token is
+ * skipped; the slots of a call are distinct). A 16-bit cache takes rows of its own dtype unchanged.
+ * An e4m3 cache takes, per row x, with m = max(max |x|, 2^-24):
+ *   scale = m / 448,  code = e4m3(x * (448 / m))  (round to nearest even, |code| <= 448),
+ * and for a row that holds a NaN or an infinity scale = NaN and codes 0: it reads back as NaN.
+ * cfb_kv_read writes the rows of T slots to key, value [T, kv_heads, dim] of `dtype` 0 (fp32), 1 or
+ * 2: code * scale (the stored element of a 16-bit cache) rounded once; a negative slot or one past
+ * the pool reads as 0. */
+cfb_status cfb_kv_write(const cfb_kv_cache* c, const void* key, int64_t sk_t, int64_t sk_h,
+                        const void* value, int64_t sv_t, int64_t sv_h, int dtype,
+                        const int64_t* slots, int T, void* stream);
+cfb_status cfb_kv_read(const cfb_kv_cache* c, const int64_t* slots, int T, void* key, int64_t sk_t,
+                       int64_t sk_h, void* value, int64_t sv_t, int64_t sv_h, int dtype, void* stream);
+
+/* Attention of new tokens over a paged cache, for B requests in one launch. Request b owns the
+ * query rows [cu_q[b], cu_q[b + 1]) (int32 [B + 1], non-decreasing, within [0, T]), n of them, and
+ * the first L = kv_len[b] (int32) positions of its pages page_table[b * table_stride + j] (int32,
+ * `table_width` entries a request). Query row i of it, head h (kv head h / (H / kv_heads)):
+ *   s_j = scale * q[i, h] . k_j over the allowed positions j: all j < L, or with `causal`
+ *         j <= L - n + i (the request's own new tokens are its last n positions);
+ *   o[i, h] = softmax(s) v,   lse[h * T + i] = log sum_j exp(s_j)   (natural log; lse may be NULL).
+ * A row with no allowed position gets o = 0 and lse = -inf. Positions that are not allowed have no
+ * influence, whatever they hold. A page index outside [0, pages) is never dereferenced: its
+ * positions' scores are NaN; L is capped at table_width * page_size, and a request whose L is over
+ * that gets NaN. q, o [T, H, dim] of `dtype` 1 or 2 (the cache's own, or any of the two over an
+ * e4m3 cache), strides in elements, rows 16-byte aligned; q rows outside every request are not read
+ * and their o and lse not written. ws: cfb_paged_attn_workspace(H, c) bytes, 256-byte aligned,
+ * for calls ordered on one stream; it needs no initialisation. Supported: H a multiple of kv_heads,
+ * H / kv_heads <= 128. */
+size_t cfb_paged_attn_workspace(int H, int kv_heads, int dim);
+cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, const cfb_kv_cache* c,
+                          const int32_t* page_table, int64_t table_stride, int table_width,
+                          const int32_t* kv_len, const int32_t* cu_q, void* o, int64_t so_t,
+                          int64_t so_h, float* lse, float scale, int T, int B, int H, int causal,
+                          int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* The gated delta rule of cfb_tree_gdn_verify without a tree: request b's tokens are the rows
+ * t = cu[b] .. cu[b + 1] - 1 (int32 [B + 1], non-decreasing, within [0, T]), walked in order from
+ * state_in[init_slot[b]] (a negative slot: zeros; one >= slots: NaN):
+ *   S <- S * exp(-exp(A_log[hv]) * softplus(a[t, hv] + dt_bias[hv]))
+ *   S <- S + sigmoid(b[t, hv]) * (v[t, hv] - S kn) (x) kn,   o[t, hv] = S qn,
+ * and state_out[out_slot[b]] = the last S (negative or >= slots: not kept; a request without tokens
+ * copies its state). q, k [T, H, K] and v, o [T, HV, V] of dtype 1 or 2, a and b [T, HV]: inner
+ * dims contiguous, the given token strides in elements (q, k, v, o rows 16-byte aligned). State
+ * slots fp32 [HV, V, K], state_in and state_out with the same slot_stride in floats and the same
+ * number of slots; they may be the same array. The out slots of a call are distinct, and no
+ * request reads another's out slot. Other arguments as cfb_tree_gdn_verify. Supported: K == 128, V
+ * a multiple of 32, HV a multiple of H.
+ * cfb_gdn_step: one token per request (row t = b of B rows). cfb_gdn_chunk: any lengths; ws:
+ * cfb_gdn_chunk_workspace(T, B, HV) bytes, 256-byte aligned, for calls ordered on one stream; it
+ * needs no initialisation. */
+typedef struct cfb_gdn_args {
+  const void* A_log; int A_log_dtype;
+  const void* dt_bias; int dt_bias_dtype;
+  const void* a; int a_dtype; int64_t a_stride;
+  const void* b; int b_dtype; int64_t b_stride;
+  const void* q; int64_t q_stride;
+  const void* k; int64_t k_stride;
+  const void* v; int64_t v_stride;
+  void* o; int64_t o_stride;
+  int dtype;
+  const float* state_in;
+  float* state_out;
+  int64_t slot_stride;
+  int slots;
+  const int32_t* init_slot;
+  const int32_t* out_slot;
+  float scale;
+  int H, HV, K, V;
+} cfb_gdn_args;
+cfb_status cfb_gdn_step(const cfb_gdn_args* g, int B, void* stream);
+size_t cfb_gdn_chunk_workspace(int T, int B, int HV);
+cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, int T, int B, void* ws,
+                         size_t ws_bytes, void* stream);
+
 /* ---- the per-request context ring -------------------------------------------------------------
  * The window of the last C target hidden states each request's draft is conditioned on
  * (reference FlowDrafterProposer._init_ring / _ring_write / _ring_gather,

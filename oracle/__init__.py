@@ -18,11 +18,12 @@ against ``tests/golden/ring.npz`` (``tests/golden/make_ring_golden.py``: the ref
 from .flow import (FlowConfig, layer_norm, mha, flow_block, expert_velocity, integrate,
                    path_residual, markov_bias)
 from .beam import beam_chains, beam_tree, head_logprobs, twopass_candidates, twopass_logprobs
-from .gdn import tree_gdn_scan, path_gdn_output, tree_gdn_verify, tree_gdn_factor
+from .gdn import tree_gdn_scan, path_gdn_output, tree_gdn_verify, tree_gdn_factor, gdn_sequence
 from .ring import ring_write, ring_gather
 from .vae import vae_encode, vae_decode, predict_hidden_vae
 from .tree_attn import tree_attn_merge, attention_over
 from .tree_verify import tree_verify_greedy
+from .paged import kv_quantise, kv_values, paged_attention
 
 __all__ = [
     "FlowConfig", "layer_norm", "mha", "flow_block", "expert_velocity", "integrate",
@@ -30,4 +31,5 @@ __all__ = [
     "twopass_logprobs",
     "tree_gdn_scan", "path_gdn_output", "tree_gdn_verify", "tree_gdn_factor", "ring_write", "ring_gather",
     "vae_encode", "vae_decode", "predict_hidden_vae", "tree_attn_merge", "attention_over", "tree_verify_greedy",
+    "gdn_sequence", "kv_quantise", "kv_values", "paged_attention",
 ]

@@ -168,3 +168,27 @@ def tree_gdn_factor(A_log, dt_bias, a, b, q, k, v, state, chain, depth, init_slo
                     acc = acc + w[t][j] * (kn[m, h] @ qn[t, h]) * u[m]
                 o[t, hv] = acc
     return o
+
+
+def gdn_sequence(A_log, dt_bias, a, b, q, k, v, state, cu, init_slot, out_slot, scale):
+    """The gated delta rule of tree_gdn_verify along whole sequences, in 64 bits: request r's tokens
+    cu[r] .. cu[r + 1] walked in order from state[init_slot[r]] (negative: zeros). Returns
+    (o [T, HV, V], new state): state with out_slot[r] (unless negative) set to request r's last S."""
+    q, k, v, a, b, A_log, dt_bias = (t.double() for t in (q, k, v, a, b, A_log, dt_bias))
+    rep = v.shape[1] // q.shape[1]
+    kn = (k * torch.rsqrt((k * k).sum(-1, keepdim=True) + 1e-6)).repeat_interleave(rep, 1)
+    qn = (q * torch.rsqrt((q * q).sum(-1, keepdim=True) + 1e-6) * scale).repeat_interleave(rep, 1)
+    decay = torch.exp(-A_log.exp() * torch.nn.functional.softplus(a + dt_bias))
+    beta = torch.sigmoid(b)
+    o = torch.zeros(v.shape, dtype=torch.float64)
+    new = state.double().clone()
+    for r in range(len(init_slot)):
+        S = state[int(init_slot[r])].double().clone() if int(init_slot[r]) >= 0 else torch.zeros_like(new[0])
+        for t in range(int(cu[r]), int(cu[r + 1])):
+            S = S * decay[t][:, None, None]
+            u = (v[t] - torch.einsum("hvk,hk->hv", S, kn[t])) * beta[t][:, None]
+            S = S + u[:, :, None] * kn[t][:, None, :]
+            o[t] = torch.einsum("hvk,hk->hv", S, qn[t])
+        if int(out_slot[r]) >= 0:
+            new[int(out_slot[r])] = S
+    return o, new
