@@ -3,6 +3,8 @@ cfb_paged_attn (cfb_attn.cu): prompt chunks and single tokens (causal), and the 
 tree step, whose outputs ``tree.tree_attn_merge`` joins with the tree's own part."""
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from . import _lib
@@ -26,6 +28,15 @@ class PagedAttention:
         self.ws_bytes = int(self.lib.cfb_paged_attn_workspace(heads, kv_heads, head_dim))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+
+    def check(self) -> None:
+        """Raises if a device-side wait of the last call expired (its outputs are then invalid). Waits
+        for the GPU."""
+        err = C.c_int(0)
+        torch.cuda.synchronize(self.device)
+        _lib.check(self.lib.cfb_paged_attn_error(self.ws_ptr, C.byref(err)), "cfb_paged_attn_error")
+        if err.value:
+            raise _lib.CfbError(f"PagedAttention: device error {err.value} (a bounded wait expired); outputs are invalid")
 
     def __call__(self, query, cache: PagedKVCache, page_table, kv_len, cu_q, *, scale: float | None = None,
                  causal: bool = True, out=None, lse=None, stream=None):

@@ -5,10 +5,14 @@
 // j (j < L, or j <= L - n + i):
 //   s_j = scale q_i . k_j,  m = max s_j,  l = sum exp(s_j - m),  o_i = sum exp(s_j - m) v_j / l,
 //   lse_i = m + log l.
-// One warp per (query row, head), lanes over the head dim, positions one by one with the running
-// maximum and sum; positions that are not allowed are never read.
+// Over an e4m3 cache k_j = ks_j kc_j and v_j = vs_j vc_j (codes and scales), and
+//   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
+//   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
+// so the weights stay at most 1, whatever the scales, and the codes enter the products exactly.
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
+#include <cstdlib>
+#include <type_traits>
 
 #include "cfb_types.cuh"
 
@@ -16,7 +20,23 @@ using namespace cfb;
 
 namespace {
 
-constexpr int kWarps = 8;
+// ---- the split ------------------------------------------------------------------------------------
+// The query rows of one kv head of a request (its n tokens x rep heads, token-major) are cut into
+// tiles of kM = 128 rows, the allowed positions of a tile into units of kKeys = 64. A piece of work
+// is (request, kv head, row tile); the units of all pieces, laid end to end, are dealt to the CTAs in
+// equal contiguous shares, so one long context and a thousand short ones both keep every SM busy. A
+// piece cut by a share's end leaves partial results (unnormalised o, m, l, fp32) in the workspace,
+// which attn_join_kernel adds up in unit order; a share holds at most two such pieces (its first and
+// its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
+// the same call gives the same bits.
+constexpr int kM = 128, kKeys = 64;
+constexpr int kSoftWarps = 4, kLoadWarps = 8;
+constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
+constexpr int kMmaWarp = kSoftWarps;
+constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int kScaleStages = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum has grown by 2^8
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -27,95 +47,791 @@ struct AttnArgs {
   void* o; long long so_t, so_h;
   float* lse;
   float scale;
-  int T, B, H, causal;
+  int T, B, H, causal, rep;
+  struct Desc* desc;                      // [grid]
+  float* part;                            // [grid][2][kM][dim + 2]
 };
 
-template <typename C, int E>
-CFB_DEV void load_elems(const C* p, float (&x)[E]) {
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    if constexpr (sizeof(C) == 1) x[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(p[i], __NV_E4M3)));
-    else x[i] = to_float(p[i]);
-  }
+struct Desc {                             // a piece that begins in this CTA's share and runs past its end
+  int last;                               // the last CTA that holds a part of it; -1: no such piece
+  int kh, t0, rows, row0;                 // kv head, first token row of the request, valid rows, first row of the tile
+  int err;
+  long long units;                        // all units of the launch
+};
+
+CFB_DEV long long share(long long units, int cta, int grid) { return units * cta / grid; }
+
+struct Request { int t0, n, L; bool over; };
+CFB_DEV Request request(const AttnArgs& A, int b) {
+  Request r;
+  r.t0 = min(max(A.cu_q[b], 0), A.T);
+  r.n = min(max(A.cu_q[b + 1], r.t0), A.T) - r.t0;
+  const long long cap = (long long)A.width * A.c.page_size;
+  const int len = max(A.kv_len[b], 0);
+  r.over = len > cap;
+  r.L = r.over ? (int)cap : len;
+  return r;
+}
+CFB_DEV int row_limit(const AttnArgs& A, const Request& r, int tok) {      // positions that token `tok` may see
+  return A.causal ? max(min(r.L - r.n + tok + 1, r.L), 0) : r.L;
+}
+CFB_DEV int tiles_of(const AttnArgs& A, const Request& r) { return (r.n * A.rep + kM - 1) / kM; }
+CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
+  const int last = (min((tile + 1) * kM, r.n * A.rep) - 1) / A.rep;
+  return max(1, (row_limit(A, r, last) + kKeys - 1) / kKeys);
+}
+CFB_DEV int head_units(const AttnArgs& A, const Request& r) {
+  const int tiles = tiles_of(A, r);
+  int u = 0;
+  for (int t = 0; t < tiles; ++t) u += units_of(A, r, t);
+  return u;
 }
 
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kWarps * 32) attn_rows_kernel(const AttnArgs A) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long task = (long long)blockIdx.x * kWarps + threadIdx.x / 32;
-  if (task >= (long long)A.T * A.H) return;
-  const int t = (int)(task / A.H), h = (int)(task - (long long)t * A.H);
-  // the request that owns row t: the last b with cu_q[b] <= t
-  int lo = 0, hi = A.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (A.cu_q[mid] <= t) lo = mid; else hi = mid;
+// A share, piece by piece; every warp of the CTA walks it alike.
+struct Walk {
+  long long u, end;
+  int b, kh, tile, tiles, units, first;   // units of the piece; first unit of it in this share
+  Request r;
+  CFB_DEV void start(const AttnArgs& A, long long from, long long to, int req, long long rest, int per_head) {
+    u = from; end = to; b = req;
+    if (u >= end) return;
+    r = request(A, b);
+    tiles = tiles_of(A, r);
+    kh = (int)(rest / per_head);
+    first = (int)(rest - (long long)kh * per_head);
+    tile = 0;
+    for (;;) {
+      units = units_of(A, r, tile);
+      if (first < units) break;
+      first -= units;
+      ++tile;
+    }
   }
-  const int first = A.cu_q[lo], end = A.cu_q[lo + 1];
-  if (t < first || t >= end) return;
-  const long long cap = (long long)A.width * A.c.page_size;
-  long long L = max(A.kv_len[lo], 0);
-  const bool over = L > cap;
-  L = over ? cap : L;
-  const long long stop = A.causal ? min(L, L - (end - first) + (t - first) + 1) : L;
-  const int kh = h / (A.H / A.c.kv_heads);
-  float q[E], acc[E];
-  load_elems(static_cast<const T*>(A.q) + t * A.sq_t + h * A.sq_h + lane * E, q);
-#pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (long long j = 0; j < stop; ++j) {
-    const int page = A.table[lo * A.st + j / A.c.page_size];
-    const int off = (int)(j % A.c.page_size);
-    float s = __int_as_float(0x7fc00000), vs = 1.f;
-    float v[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = 0.f;
-    if (page >= 0 && page < A.c.pages) {
-      const long long row = page * A.c.page_stride + kh * A.c.head_stride + off * A.c.slot_stride + lane * E;
-      float k[E];
-      load_elems(static_cast<const C*>(A.c.k) + row, k);
-      load_elems(static_cast<const C*>(A.c.v) + row, v);
-      s = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(q[i], k[i], s);
-#pragma unroll
-      for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= A.scale;
-      if constexpr (sizeof(C) == 1) {
-        const long long sc = page * A.c.scale_page_stride + kh * A.c.scale_head_stride + off * A.c.scale_slot_stride;
-        s *= A.c.k_scale[sc];
-        vs = A.c.v_scale[sc];
+  CFB_DEV bool done() const { return u >= end; }
+  CFB_DEV int stop() const { return (int)min((long long)units, first + (end - u)); }   // first unit past this share's part
+  CFB_DEV void next(const AttnArgs& A) {
+    u += stop() - first;
+    if (u >= end) return;
+    first = 0;
+    if (++tile == tiles) {
+      tile = 0;
+      if (++kh == A.c.kv_heads) {
+        kh = 0;
+        do {
+          r = request(A, ++b);
+          tiles = tiles_of(A, r);
+        } while (tiles == 0);
       }
     }
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - top), p = s == -INFINITY ? 0.f : expf(s - top);
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = acc[i] * keep + p * vs * v[i];
-    m = top;
+    units = units_of(A, r, tile);
   }
-  if (over) l = __int_as_float(0x7fc00000);
-  T* o = static_cast<T*>(A.o) + t * A.so_t + h * A.so_h + lane * E;
+};
+
+// ---- shared and tensor memory ------------------------------------------------------------------------
+// Q, K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed
+// with row & 7. Q and K are read K-major (the head dim is summed over), V MN-major (the positions
+// are), from the same image.
+template <int D>
+struct Layout {
+  static constexpr uint32_t kQ = kM * D * 2, kTile = kKeys * D * 2;
+  static constexpr uint32_t kQSlab = kM * 128, kKSlab = kKeys * 128;
+  static constexpr uint32_t off_q = 0, off_k = kQ, off_v = kQ + 2 * kTile, off_scale = kQ + 4 * kTile;
+  static constexpr uint32_t bytes = off_scale + kScaleStages * kKeys * 16 + 1024;
+  static constexpr uint32_t s_col = 0, p_col = 2 * kKeys, o_col = 3 * kKeys + (D == 256 ? 64 : 0);   // TMEM columns
+  static constexpr uint32_t cols = D == 64 ? 256 : 512;
+};
+
+struct Bars {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_free, sc_full[kScaleStages], drain;
+};
+
+CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 #pragma unroll
-  for (int i = 0; i < E; ++i) o[i] = from_float<T>(l == 0.f ? 0.f : acc[i] / l);
-  if (A.lse && lane == 0) A.lse[(long long)h * A.T + t] = l == 0.f ? -INFINITY : m + logf(l);
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+CFB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+CFB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+CFB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] . B[smem], 16-bit A (two elements a column) and B
+CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %4, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t}"
+      :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// MN-major 128-byte-swizzled operand: 64-element slabs `slab` bytes apart, 8-row groups 1024 bytes apart
+CFB_DEV uint64_t mn_desc(uint32_t saddr, uint32_t slab) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+template <typename T>
+CFB_DEV constexpr uint32_t type_bits() {          // operand formats of the instruction descriptor
+  return sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+}
+CFB_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {     // 16 bytes, zeros past `bytes`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+CFB_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> CFB_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+CFB_DEV void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+CFB_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T, typename C>
-void launch(const AttnArgs& A, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((long long)A.T * A.H + kWarps - 1) / kWarps);
-  if (A.c.dim == 64) attn_rows_kernel<T, C, 64><<<grid, kWarps * 32, 0, st>>>(A);
-  else if (A.c.dim == 128) attn_rows_kernel<T, C, 128><<<grid, kWarps * 32, 0, st>>>(A);
-  else attn_rows_kernel<T, C, 256><<<grid, kWarps * 32, 0, st>>>(A);
+// Where the row of position j lies; -1 if its page is none of the pool's.
+CFB_DEV long long row_offset(const AttnArgs& A, int b, int kh, int j, long long* scale_off) {
+  const int p = (unsigned)j / (unsigned)A.c.page_size, off = j - p * A.c.page_size;
+  const int page = __ldg(A.table + (long long)b * A.st + p);
+  if (page < 0 || page >= A.c.pages) return -1;
+  if (scale_off)
+    *scale_off = (long long)page * A.c.scale_page_stride + kh * A.c.scale_head_stride + off * A.c.scale_slot_stride;
+  return (long long)page * A.c.page_stride + kh * A.c.head_stride + off * A.c.slot_stride;
+}
+
+// eight e4m3 codes -> eight elements of T (exact: both types hold every e4m3 value)
+template <typename T> CFB_DEV uint4 widen8(uint32_t lo, uint32_t hi);
+template <> CFB_DEV uint4 widen8<__half>(uint32_t lo, uint32_t hi) {
+  uint4 r;
+  const auto two = [](uint32_t w) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
+    return (uint32_t)h.x | (uint32_t)h.y << 16;
+  };
+  r.x = two(lo & 0xffff); r.y = two(lo >> 16); r.z = two(hi & 0xffff); r.w = two(hi >> 16);
+  return r;
+}
+// bf16: the code's exponent and mantissa bits, moved to bf16's places, read as value * 2^-120 (e4m3's
+// bias is 7, bf16's 127; subnormals come out as subnormals), and one exact product undoes that.
+template <> CFB_DEV uint4 widen8<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
+  uint4 r;
+  const auto two = [](uint32_t b0, uint32_t b1) {
+    const uint32_t w = b0 | b1 << 16;
+    const uint32_t x = (w & 0x00800080u) << 8 | (w & 0x007f007fu) << 4;
+    const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80));   // 2^120
+    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), up);
+    return *reinterpret_cast<const uint32_t*>(&y);
+  };
+  r.x = two(lo & 0xff, lo >> 8 & 0xff); r.y = two(lo >> 16 & 0xff, lo >> 24);
+  r.z = two(hi & 0xff, hi >> 8 & 0xff); r.w = two(hi >> 16 & 0xff, hi >> 24);
+  return r;
+}
+
+// ---- the kernel -----------------------------------------------------------------------------------
+// One CTA per SM, 13 warps. Warps 5-12 load: per piece the Q tile, per unit a K and a V tile (two
+// stages each) with 16-byte copies, rows found through the page table, positions past the end filled
+// with zeros; e4m3 rows come through registers, where they are widened. Warp 4 issues the tensor
+// work: S(i) = Q K(i)^T into one of two fp32 tiles in tensor memory, then O += P(i-1) V(i-1) with P
+// read from tensor memory, so the softmax of a unit runs beside the next unit's product. Warps 0-3
+// are the softmax, a thread a row: the row's 64 scores come from tensor memory, the maximum is kept
+// in the thread, the weights go back to tensor memory in the operands' type (the one rounding of the
+// weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of the unrounded fp32 values). O is
+// rescaled only when the row's maximum has grown by more than 2^8 since the last time: weights are
+// then at most 2^8, far inside both types, and most units touch O not at all.
+template <typename T, bool QUANT, int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
+  using Lay = Layout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Bars bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ long long sh_sum[kThreads / 32];
+  __shared__ long long sh_rest, sh_total;
+  __shared__ int sh_req, sh_per;
+  __shared__ int dead;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grid = gridDim.x, cta = blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.k_full[i], kLoadWarps); mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_full[i], kLoadWarps); mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], kSoftWarps); mbar_init(&bar.pv_done[i], 1);
+    }
+    mbar_init(&bar.o_free, kSoftWarps);
+    for (int i = 0; i < kScaleStages; ++i) mbar_init(&bar.sc_full[i], kKeys / 32);
+    mbar_init(&bar.drain, 1);
+    fence_mbar_init();
+    dead = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
+
+  // where this CTA's share begins: the running sum of the requests' units
+  long long total = 0;
+  for (int b0 = 0; b0 < A.B; b0 += kThreads) {
+    long long mine = 0;
+    if (b0 + (int)threadIdx.x < A.B) mine = (long long)head_units(A, request(A, b0 + threadIdx.x)) * A.c.kv_heads;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+    if (lane == 0) sh_sum[warp] = mine;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 32; ++w) total += sh_sum[w];
+    __syncthreads();
+  }
+  const long long from = share(total, cta, grid), to = share(total, cta + 1, grid);
+  if (threadIdx.x == 0) {
+    sh_total = total;
+    A.desc[cta].last = -1;
+    A.desc[cta].err = 0;
+  }
+  if (from < to) {
+    long long before = 0;
+    for (int b0 = 0; b0 < A.B && before <= from; b0 += kThreads) {
+      int per = 0;
+      if (b0 + (int)threadIdx.x < A.B) per = head_units(A, request(A, b0 + threadIdx.x));
+      const long long mine = (long long)per * A.c.kv_heads;
+      long long run = mine;                                   // inclusive scan over the warp
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, run, off);
+        if (lane >= off) run += y;
+      }
+      if (lane == 31) sh_sum[warp] = run;
+      __syncthreads();
+      long long all = 0;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w == warp) run += before + all;
+        all += sh_sum[w];
+      }
+      if (from >= run - mine && from < run) {
+        sh_req = b0 + threadIdx.x;
+        sh_rest = from - (run - mine);
+        sh_per = per;
+      }
+      before += all;
+      __syncthreads();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  Walk w;
+  w.start(A, from, to, sh_req, sh_rest, sh_per);
+
+  // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait.
+  const auto wait = [&](uint64_t* b, uint32_t parity) {
+    bool ok = mbar_wait(b, parity);
+    if (!ok) *reinterpret_cast<volatile int*>(&dead) = 1;
+    ok = ok && *reinterpret_cast<volatile int*>(&dead) == 0;
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+
+  if (warp < kSoftWarps) {
+    // ---------------------------------------------------------------- softmax: thread = row
+    const uint32_t tw = tmem + ((uint32_t)(warp * 32) << 16);
+    const int r = threadIdx.x;
+    const float c2 = A.scale * kLog2e;
+    uint32_t g = 0, pieces = 0;                               // units and pieces so far
+    for (; !w.done(); w.next(A), ++pieces) {
+      const int stop = w.stop(), first = w.first;
+      const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
+      const bool valid = r < rows;
+      const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
+      const int lim = valid ? row_limit(A, w.r, tok) : 0;
+      const bool warp_live = warp * 32 < rows;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int i = first; i < stop; ++i, ++g) {
+        const int s = g & 1;
+        if (!(ok = wait(&bar.s_full[s], (g >> 1) & 1))) break;
+        if (warp_live) {
+          tc_fence_after();
+          float x[kKeys];
+          tmem_ld32(tw + Lay::s_col + s * kKeys, x);
+          tmem_ld32(tw + Lay::s_col + s * kKeys + 32, x + 32);
+          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys;
+          if (QUANT) ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1);
+          tmem_wait_ld();
+          if (!ok) break;
+          const int j0 = i * kKeys;
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e) {
+            if constexpr (QUANT) {
+              const float2 f = *reinterpret_cast<const float2*>(sc + e);
+              x[e] = fmaf(x[e], f.x, f.y);
+            } else {
+              x[e] *= c2;
+            }
+          }
+          if (__any_sync(0xffffffffu, lim < j0 + kKeys)) {
+#pragma unroll
+            for (int e = 0; e < kKeys; ++e)
+              if (j0 + e >= lim) x[e] = -INFINITY;
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          // P's buffer is free once the product that read it two units ago is done
+          if (i - first >= 2 && !(ok = wait(&bar.pv_done[s], ((g >> 1) + 1) & 1))) break;
+          if (m == -INFINITY) {
+            // nothing seen yet: o is zero (or not begun), l is zero, any m will do
+            m = high;
+          }
+          if (__any_sync(0xffffffffu, high > m + kRescaleAt) && i > first) {
+            const float up = high > m + kRescaleAt ? high : m;
+            const float keep = m == -INFINITY ? 1.f : exp2_approx(m - up);
+            if (!(ok = wait(&bar.pv_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
+            tc_fence_after();
+            l *= keep;
+            m = up;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+              float o[32];
+              uint32_t u[32];
+              tmem_ld32(tw + Lay::o_col + d, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * keep);
+              tmem_st32(tw + Lay::o_col + d, u);
+            }
+          }
+          const float mm = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t p[kKeys / 2];
+#pragma unroll
+          for (int e = 0; e < kKeys; e += 2) {
+            const float a = exp2_approx(x[e] - mm), b = exp2_approx(x[e + 1] - mm);
+            if constexpr (QUANT) {
+              sum[e & 3] = fmaf(a, sc[e].z, sum[e & 3]);
+              sum[(e + 1) & 3] = fmaf(b, sc[e + 1].z, sum[(e + 1) & 3]);
+            } else {
+              sum[e & 3] += a;
+              sum[(e + 1) & 3] += b;
+            }
+            p[e / 2] = pack16<T>(a, b);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st32(tw + Lay::p_col + s * (kKeys / 2), p);
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[s]);
+      }
+      if (!ok) break;
+      // the last product of the piece
+      const uint32_t gl = g - 1;
+      if (!wait(&bar.pv_done[gl & 1], (gl >> 1) & 1)) break;
+      tc_fence_after();
+      if (warp_live) {
+        const bool whole = first == 0 && stop == w.units;
+        if (w.r.over) l = __int_as_float(0x7fc00000);
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        T* out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
+        float* part = A.part + ((long long)cta * 2 + (first == 0)) * kM * (D + 2) + (long long)r * (D + 2);
+        float bad = 0.f;                                      // turns NaN where an element is not finite
+#pragma unroll 1
+        for (int d = 0; d < D; d += 32) {
+          float o[32];
+          tmem_ld32(tw + Lay::o_col + d, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) bad = fmaf(o[e], 0.f, bad);
+          if (valid && whole) {
+            uint4* dst = reinterpret_cast<uint4*>(out + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float* y = o + 8 * e;
+              dst[e] = l == 0.f ? make_uint4(0, 0, 0, 0)
+                                : make_uint4(pack16<T>(y[0] * inv, y[1] * inv), pack16<T>(y[2] * inv, y[3] * inv),
+                                             pack16<T>(y[4] * inv, y[5] * inv), pack16<T>(y[6] * inv, y[7] * inv));
+            }
+          } else if (valid) {
+            float2* dst = reinterpret_cast<float2*>(part + d);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dst[e] = make_float2(o[2 * e], o[2 * e + 1]);
+          }
+          __syncwarp();
+        }
+        if (valid) {
+          if (!whole) {
+            part[D] = m;
+            part[D + 1] = l;
+          } else if (A.lse) {
+            A.lse[(long long)head * A.T + w.r.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+          }
+        }
+        if constexpr (!QUANT) {
+          // A value that is not finite at a position that this row may not see has met a weight of 0 in
+          // the product. Only a causal row's last units can hold one; such a row is taken again from
+          // its own positions alone, with m and l as they are.
+          unsigned again = __ballot_sync(0xffffffffu, A.causal && valid && bad != 0.f && l == l && lim < stop * kKeys);
+          while (again) {
+            const int src = __ffs(again) - 1;
+            again &= again - 1;
+            const int row = warp * 32 + src, RR = w.tile * kM + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
+            const int li = __shfl_sync(0xffffffffu, lim, src);
+            const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
+            constexpr int E = D / 32;
+            const T* qp = static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h + lane * E;
+            float q[E], acc[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) { q[e] = to_float(qp[e]); acc[e] = 0.f; }
+            for (int j = first * kKeys; j < li; ++j) {
+              const long long off = row_offset(A, w.b, w.kh, j, nullptr);
+              if (off < 0) continue;                          // its score is NaN: l is too, and this row is not here
+              const T* kp = static_cast<const T*>(A.c.k) + off + lane * E;
+              const T* vp = static_cast<const T*>(A.c.v) + off + lane * E;
+              float s = 0.f;
+#pragma unroll
+              for (int e = 0; e < E; ++e) s = fmaf(q[e], to_float(kp[e]), s);
+#pragma unroll
+              for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+              const float p = exp2_approx(s * c2 - mr);
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(vp[e]), acc[e]);
+            }
+            T* op = static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h + lane * E;
+            float* pp = A.part + ((long long)cta * 2 + (first == 0)) * kM * (D + 2) + (long long)row * (D + 2) + lane * E;
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              if (whole) op[e] = from_float<T>(acc[e] * ir);
+              else pp[e] = acc[e];
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.o_free);
+      if (threadIdx.x == 0 && first == 0 && stop < w.units) {  // begins here, ends elsewhere
+        const long long end = w.u + w.units;                   // w.u: its first unit
+        int last = cta + 1;
+        while (share(total, last + 1, grid) < end) ++last;
+        Desc d;
+        d.last = last; d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * kM; d.err = 0; d.units = total;
+        A.desc[cta] = d;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- tensor work
+    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | type_bits<T>();
+    constexpr uint32_t idesc_o = tc_idesc(kM, D) | type_bits<T>() | (1u << 16);      // B is MN-major
+    uint32_t g = 0, pieces = 0;
+    bool ok = true;
+    const auto pv = [&](uint32_t u, bool fresh) {              // O (+)= P(u) V(u)
+      const int s = u & 1;
+      if (!wait(&bar.v_full[s], (u >> 1) & 1) || !wait(&bar.p_full[s], (u >> 1) & 1)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k)
+        mma_ts_warp(tmem + Lay::o_col, tmem + Lay::p_col + s * (kKeys / 2) + k * 8,
+                    mn_desc(base + Lay::off_v + s * Lay::kTile + k * 2048, Lay::kKSlab), idesc_o, !(fresh && k == 0));
+      tc_commit_warp(&bar.v_empty[s]);
+      tc_commit_warp(&bar.pv_done[s]);
+      return true;
+    };
+    for (; ok && !w.done(); w.next(A), ++pieces) {
+      const int count = w.stop() - w.first;
+      for (int i = 0; i < count; ++i, ++g) {
+        const int s = g & 1;
+        if (!(ok = wait(&bar.k_full[s], (g >> 1) & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_f16_warp(tmem + Lay::s_col + s * kKeys,
+                          sw128_desc(base + Lay::off_q + (k / 4) * Lay::kQSlab + (k % 4) * 32),
+                          sw128_desc(base + Lay::off_k + s * Lay::kTile + (k / 4) * Lay::kKSlab + (k % 4) * 32), idesc_s, k > 0);
+        tc_commit_warp(&bar.k_empty[s]);
+        tc_commit_warp(&bar.s_full[s]);
+        if (i > 0) {
+          // the piece's first product overwrites O: the last piece's must have been read
+          if (i == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
+          if (!(ok = pv(g - 1, i == 1))) break;
+        }
+      }
+      if (!ok) break;
+      if (count == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
+      ok = pv(g - 1, count == 1);
+    }
+    tc_commit_warp(&bar.drain);                                // everything issued has completed
+    mbar_wait(&bar.drain, 0);
+  } else {
+    // ---------------------------------------------------------------- loads
+    const int lt = threadIdx.x - (kMmaWarp + 1) * 32, lw = lt >> 5;
+    constexpr int kElem = QUANT ? 1 : 2;                       // stored bytes an element
+    constexpr int kLanesRow = D * kElem / 16;                  // lanes a row of 16-byte pieces
+    constexpr int kRowsPass = 32 / kLanesRow;                  // rows a warp's access covers
+    constexpr int kPasses = kKeys / (kLoadWarps * kRowsPass);
+    static_assert(kPasses >= 1, "a tile has a pass for every warp");
+    const int sub = lane / kLanesRow, piece = lane % kLanesRow;
+    // lane x of a warp (x < kPasses * kRowsPass) finds the row of position x % kRowsPass + ... of its warp
+    constexpr int kOwn = kPasses * kRowsPass;                  // positions a warp loads of a unit
+    static_assert(kOwn <= 32, "a lane a position");
+    const auto position = [&](int x) { return (x / kRowsPass) * (kLoadWarps * kRowsPass) + lw * kRowsPass + x % kRowsPass; };
+    const auto load_q = [&](const Walk& w) {
+      constexpr int kLanesQ = D / 8, kRowsQ = 32 / kLanesQ;
+      const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
+      const int qs = lane / kLanesQ, qc = lane % kLanesQ;
+#pragma unroll 4
+      for (int x = 0; x < kM / (kLoadWarps * kRowsQ); ++x) {
+        const int r = x * (kLoadWarps * kRowsQ) + lw * kRowsQ + qs;
+        const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
+        const bool in = r < rows;
+        const T* src = static_cast<const T*>(A.q) + (in ? (long long)(w.r.t0 + tok) * A.sq_t + head * A.sq_h + qc * 8 : 0);
+        cp_async16(base + Lay::off_q + (qc >> 3) * Lay::kQSlab + r * 128 + (((qc & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
+      }
+    };
+    uint32_t g = 0, fulls = 0;                                 // units; groups (K(0), V(0), K(1), ...) announced
+    const auto announce = [&] {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive((fulls & 1) ? &bar.v_full[(fulls >> 1) & 1] : &bar.k_full[(fulls >> 1) & 1]);
+      ++fulls;
+    };
+    bool ok = true;
+    if constexpr (!QUANT) {
+      // cp.async groups in flight: up to three tiles
+      for (; ok && !w.done(); w.next(A)) {
+        const int stop = w.stop();
+        const int lim_max = row_limit(A, w.r, w.r.n - 1);
+        for (int i = w.first; i < stop; ++i, ++g) {
+          const int s = g & 1;
+          long long off = -1;
+          const int mine = i * kKeys + position(lane % kOwn);
+          const bool there = mine < lim_max;
+          if (there) off = row_offset(A, w.b, w.kh, mine, nullptr);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (g >= 2 && !(ok = wait(kv ? &bar.v_empty[s] : &bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
+            const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + s * Lay::kTile + (piece >> 3) * Lay::kKSlab;
+            const T* src = static_cast<const T*>(kv ? A.c.v : A.c.k);
+#pragma unroll
+            for (int x = 0; x < kPasses; ++x) {
+              const int r = position(x * kRowsPass + sub);
+              const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+              const bool in = i * kKeys + r < lim_max;
+              const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+              if (in && o < 0 && kv == 0) {                    // no such page: its scores are NaN
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(at), "r"(0x7fff7fff) : "memory");
+              } else {
+                cp_async16(at, src + (in && o >= 0 ? o + piece * 8 : 0), in && o >= 0 ? 16 : 0);
+              }
+            }
+            if (kv == 0 && i == w.first) {                     // the piece's Q rides with its first K
+              if (g > 0) {                                     // once the last piece's products are done with theirs
+                cp_async_wait<0>();
+                while (fulls < 2 * g) announce();
+                if (!(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;
+              }
+              load_q(w);
+            }
+            cp_async_commit();
+            // V(g) waits for the product of V(g - 2), which is issued after that of K(g - 1): of the groups
+            // before V(g) only two may be unannounced
+            if (g * 2 + kv - fulls >= 2) {
+              cp_async_wait<2>();
+              announce();
+            }
+          }
+          if (!ok) break;
+        }
+      }
+      cp_async_wait<0>();
+      while (ok && fulls < 2 * g) announce();
+    } else {
+      // A unit's codes go through registers: the loads of the next unit are issued before this one's are
+      // widened and stored.
+      uint4 kr[kPasses], vr[kPasses];
+      float2 sc = make_float2(0.f, 0.f);
+      int pos = 0, lim = 0;
+      unsigned none = 0;                                       // bit x: pass x's row has no page
+      const auto fetch = [&](const Walk& w, int i) {
+        lim = row_limit(A, w.r, w.r.n - 1);
+        pos = i * kKeys;
+        long long off = -1;
+        const int mine = pos + position(lane % kOwn);
+        if (mine < lim) off = row_offset(A, w.b, w.kh, mine, nullptr);
+        none = 0;
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+          kr[x] = vr[x] = make_uint4(0, 0, 0, 0);
+          if (o >= 0) {
+            kr[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.k) + o) + piece);
+            vr[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.v) + o) + piece);
+          }
+        }
+        if (lt < kKeys) {                                      // a lane a position: its scales
+          sc = make_float2(0.f, 1.f);
+          if (pos + lt < lim) {
+            long long so = 0;
+            if (row_offset(A, w.b, w.kh, pos + lt, &so) >= 0) sc = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+            else sc.x = __int_as_float(0x7fc00000);            // no such page: its scores are NaN
+          }
+        }
+      };
+      const auto put = [&](uint32_t dst, const uint4* regs) {
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+          const int r = position(x * kRowsPass + sub);
+          const uint4 a = widen8<T>(regs[x].x, regs[x].y), b = widen8<T>(regs[x].z, regs[x].w);
+          const int c0 = piece * 2;                            // 16-byte pieces of the widened row
+          const uint32_t row = dst + (c0 >> 3) * Lay::kKSlab + r * 128;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + (((c0 & 7) ^ (r & 7)) << 4)), "r"(a.x), "r"(a.y),
+                       "r"(a.z), "r"(a.w) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)), "r"(b.x), "r"(b.y),
+                       "r"(b.z), "r"(b.w) : "memory");
+        }
+      };
+      if (!w.done()) fetch(w, w.first);
+      for (; ok && !w.done();) {
+        const int stop = w.stop(), first = w.first;
+        const Walk here = w;
+        w.next(A);
+        for (int i = first; i < stop; ++i, ++g) {
+          const int s = g & 1;
+          if (g >= 2 && !(ok = wait(&bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
+          put(base + Lay::off_k + s * Lay::kTile, kr);
+          if (lt < kKeys) {
+            // a scale of NaN reaches the row through its score; where the row may not see the position,
+            // its weight of 0 meets a finite factor
+            reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
+                make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
+          }
+          if (i == first) {
+            if (g > 0 && !(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;
+            load_q(here);
+            cp_async_commit();
+            cp_async_wait<0>();
+          }
+          announce();
+          if (g >= 2 && !(ok = wait(&bar.v_empty[s], ((g >> 1) + 1) & 1))) break;
+          put(base + Lay::off_v + s * Lay::kTile, vr);
+          announce();
+          if (i + 1 < stop) fetch(here, i + 1);
+          else if (!w.done()) fetch(w, w.first);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && dead) A.desc[cta].err = DEV_TIMEOUT_FULL;
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Lay::cols);
+  }
+}
+
+// ---- the pieces that were cut --------------------------------------------------------------------
+// o = sum_i 2^(m_i - m) o_i / l,  l = sum_i 2^(m_i - m) l_i,  m = max m_i over the parts in unit order.
+// A warp per row of a cut piece; CTA x takes the piece that begins in share x.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs A) {
+  const int grid = gridDim.x, cta = blockIdx.x;
+  const Desc d = A.desc[cta];
+  const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + threadIdx.x / 32;
+  if (d.last < 0 || r >= d.rows) return;
+  const auto part_of = [&](int c) { return A.part + ((long long)c * 2 + (c == cta)) * kM * (D + 2) + (long long)r * (D + 2); };
+  const auto holds = [&](int c) { return c == cta || share(d.units, c, grid) < share(d.units, c + 1, grid); };
+  float m = -INFINITY;
+  for (int c = cta + lane; c <= d.last; c += 32)
+    if (holds(c)) m = fmaxf(m, part_of(c)[D]);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float mm = m == -INFINITY ? 0.f : m;
+  constexpr int E = D / 32;
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int c = cta; c <= d.last; ++c) {
+    if (!holds(c)) continue;
+    const float* p = part_of(c);
+    const float w = exp2_approx(p[D] - mm);
+    l = fmaf(w, p[D + 1], l);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p + e * 32 + lane * 2);
+      acc[e] = fmaf(w, x.x, acc[e]);
+      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+    }
+  }
+  const int R = d.row0 + r, tok = R / A.rep, head = d.kh * A.rep + R - tok * A.rep;
+  T* out = static_cast<T*>(A.o) + (long long)(d.t0 + tok) * A.so_t + head * A.so_h;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e * 32 + lane * 2) = l == 0.f ? 0u : pack16<T>(acc[e] / l, acc[e + 1] / l);
+  if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+}
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      sms <= 0) {
+    cudaGetLastError();
+    return 148;
+  }
+  return sms;
+}
+size_t desc_bytes(int grid) { return ((size_t)grid * sizeof(Desc) + 255) / 256 * 256; }
+
+template <typename T, bool QUANT, int D>
+cfb_status launch(const AttnArgs& A, int grid, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, QUANT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)Layout<D>::bytes);
+  if (e != cudaSuccess) return cfb_launch_status("attn_kernel attribute");
+  attn_kernel<T, QUANT, D><<<grid, kThreads, Layout<D>::bytes, st>>>(A);
+  if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;
+  const int rows = (int)min((long long)kM, (long long)A.T * A.rep);
+  attn_join_kernel<T, D><<<dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, st>>>(A);
+  return cfb_launch_status("attn_join_kernel");
+}
+template <typename T, bool QUANT>
+cfb_status launch_dim(const AttnArgs& A, int grid, cudaStream_t st) {
+  if (A.c.dim == 64) return launch<T, QUANT, 64>(A, grid, st);
+  if (A.c.dim == 128) return launch<T, QUANT, 128>(A, grid, st);
+  return launch<T, QUANT, 256>(A, grid, st);
 }
 
 }  // namespace
 
 extern "C" size_t cfb_paged_attn_workspace(int H, int kv_heads, int dim) {
-  (void)H; (void)kv_heads; (void)dim;
-  return 256;
+  if (H <= 0 || kv_heads <= 0 || dim <= 0) return 0;
+  const int grid = sm_count();
+  return desc_bytes(grid) + (size_t)grid * 2 * kM * (dim + 2) * sizeof(float);
+}
+
+extern "C" cfb_status cfb_paged_attn_error(const void* ws, int* device_error) {
+  if (!ws || !device_error) return CFB_ERR_INVALID_ARG;
+  *device_error = 0;
+  const int grid = sm_count();
+  Desc* d = static_cast<Desc*>(malloc(grid * sizeof(Desc)));
+  if (!d) return CFB_ERR_CUDA;
+  const cudaError_t e = cudaMemcpy(d, ws, grid * sizeof(Desc), cudaMemcpyDeviceToHost);
+  for (int i = 0; e == cudaSuccess && i < grid; ++i)
+    if (d[i].err) *device_error = d[i].err;
+  free(d);
+  return e == cudaSuccess ? CFB_OK : cfb_launch_status("cfb_paged_attn_error");
 }
 
 extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, const cfb_kv_cache* c,
@@ -127,15 +843,19 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   if (T < 0 || B < 0 || H <= 0 || table_width < 0 || table_stride < table_width) return CFB_ERR_INVALID_ARG;
   if ((dtype != DT_F16 && dtype != DT_BF16) || (c->dtype != DT_E4M3 && c->dtype != dtype)) return CFB_ERR_UNSUPPORTED;
   if (H % c->kv_heads || H / c->kv_heads > 128) return CFB_ERR_UNSUPPORTED;
+  if ((long long)T * (H / c->kv_heads) > 0x7fffffffll - kM || (long long)table_width * c->page_size > 0x7fffffffll - kKeys)
+    return CFB_ERR_UNSUPPORTED;
   if (T == 0 || B == 0) return CFB_OK;
   if (!q || !o || !kv_len || !cu_q || (table_width && !page_table) || !ws) return CFB_ERR_INVALID_ARG;
   if (!rows_aligned(q, 2, sq_t, sq_h) || !rows_aligned(o, 2, so_t, so_h)) return CFB_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_paged_attn_workspace(H, c->kv_heads, c->dim))
     return CFB_ERR_WORKSPACE;
+  const int grid = sm_count();
   const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-                   T, B, H, causal};
+                   T, B, H, causal, H / c->kv_heads, static_cast<Desc*>(ws),
+                   reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == DT_F16) c->dtype == DT_E4M3 ? launch<__half, uint8_t>(A, st) : launch<__half, __half>(A, st);
-  else c->dtype == DT_E4M3 ? launch<__nv_bfloat16, uint8_t>(A, st) : launch<__nv_bfloat16, __nv_bfloat16>(A, st);
-  return cfb_launch_status("attn_rows_kernel");
+  const bool quant = c->dtype == DT_E4M3;
+  if (dtype == DT_F16) return quant ? launch_dim<__half, true>(A, grid, st) : launch_dim<__half, false>(A, grid, st);
+  return quant ? launch_dim<__nv_bfloat16, true>(A, grid, st) : launch_dim<__nv_bfloat16, false>(A, grid, st);
 }

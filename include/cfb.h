@@ -389,7 +389,8 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * slots, kept as fp16 (dtype 1), bf16 (2) or e4m3 (3). Row (slot, kv head h) of a flat slot =
  * page * page_size + offset is at page * page_stride + h * head_stride + offset * slot_stride
  * elements of k and of v; its fp32 scale (dtype 3 only) at page * scale_page_stride +
- * h * scale_head_stride + offset * scale_slot_stride of k_scale and of v_scale. k and v: 16-byte
+ * h * scale_head_stride + offset * scale_slot_stride of k_scale and of v_scale (positive, or NaN
+ * for a row that reads as NaN; codes finite). k and v: 16-byte
  * aligned, strides multiples of 16 bytes. Supported: dim in {64, 128, 256}. */
 typedef struct cfb_kv_cache {
   void* k;
@@ -438,6 +439,9 @@ cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, const cfb_k
                           const int32_t* kv_len, const int32_t* cu_q, void* o, int64_t so_t,
                           int64_t so_h, float* lse, float scale, int T, int B, int H, int causal,
                           int dtype, void* ws, size_t ws_bytes, void* stream);
+/* Synchronous: the device error word of the last cfb_paged_attn call with this workspace: 0 if it
+ * completed, else a bounded device-side wait expired and its outputs are invalid. */
+cfb_status cfb_paged_attn_error(const void* ws, int* device_error);
 
 /* The gated delta rule of cfb_tree_gdn_verify without a tree: request b's tokens are the rows
  * t = cu[b] .. cu[b + 1] - 1 (int32 [B + 1], non-decreasing, within [0, T]), walked in order from

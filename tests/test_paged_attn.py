@@ -128,7 +128,7 @@ def test_long_contexts(dtype, quant, news, lens, H, HKV, D, page):
     attn = PagedAttention(H, HKV, D)
     got = attn(*case)
     again = attn(*case)
-    torch.cuda.synchronize()
+    attn.check()
     _check(got, _want(*case, True), dtype)
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
 
