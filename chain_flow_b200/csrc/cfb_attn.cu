@@ -191,14 +191,19 @@ CFB_DEV constexpr uint32_t type_bits() {          // operand formats of the inst
 CFB_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {     // 16 bytes, zeros past `bytes`
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-CFB_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> CFB_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+// one arrival on `bar` when every earlier cp.async of this thread has landed
+CFB_DEV void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
 CFB_DEV void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 CFB_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// What the key rows of a page outside the pool read: NaN in both 16-bit types.
+__device__ const uint4 kNanRow[1] = {{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}};
 
 // Where the row of position j lies; -1 if its page is none of the pool's.
 CFB_DEV long long row_offset(const AttnArgs& A, int b, int kh, int j, long long* scale_off) {
@@ -265,8 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], kLoadWarps); mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], kLoadWarps); mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.k_full[i], kLoadThreads); mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_full[i], kLoadThreads); mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], kSoftWarps); mbar_init(&bar.pv_done[i], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
@@ -536,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
     const auto pv = [&](uint32_t u, bool fresh) {              // O (+)= P(u) V(u)
       const int s = u & 1;
       if (!wait(&bar.v_full[s], (u >> 1) & 1) || !wait(&bar.p_full[s], (u >> 1) & 1)) return false;
+      fence_async_shared();
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
@@ -550,6 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       for (int i = 0; i < count; ++i, ++g) {
         const int s = g & 1;
         if (!(ok = wait(&bar.k_full[s], (g >> 1) & 1))) break;
+        fence_async_shared();                                  // the copies are the generic proxy's
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
@@ -596,139 +603,147 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
         cp_async16(base + Lay::off_q + (qc >> 3) * Lay::kQSlab + r * 128 + (((qc & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
       }
     };
-    uint32_t g = 0, fulls = 0;                                 // units; groups (K(0), V(0), K(1), ...) announced
-    const auto announce = [&] {
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive((fulls & 1) ? &bar.v_full[(fulls >> 1) & 1] : &bar.k_full[(fulls >> 1) & 1]);
-      ++fulls;
-    };
+    uint32_t g = 0;                                            // units so far
     bool ok = true;
+    // The stages come free in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)), and
+    // that is the order they are filled in.
     if constexpr (!QUANT) {
-      // cp.async groups in flight: up to three tiles
-      for (; ok && !w.done(); w.next(A)) {
+      // A thread's copies arrive on the stage's barrier by themselves when they land, so the loads run as
+      // far ahead as the stages allow. The next unit's page is looked up a unit early.
+      const auto find = [&](const Walk& w, int i) {
+        const int j = i * kKeys + position(lane % kOwn);
+        return j < row_limit(A, w.r, w.r.n - 1) ? row_offset(A, w.b, w.kh, j, nullptr) : -2ll;
+      };
+      const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
+        const uint32_t dst = base + tile + (piece >> 3) * Lay::kKSlab;
+        const T* src = static_cast<const T*>(pool);
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+          const int r = position(x * kRowsPass + sub);
+          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+          const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+          // -1: no such page, its scores are NaN; -2: past the end, zeros
+          const bool nan_row = key && o == -1;
+          cp_async16(at, o >= 0 ? static_cast<const void*>(src + o + piece * 8) : static_cast<const void*>(kNanRow),
+                     o >= 0 || nan_row ? 16 : 0);
+        }
+        cp_async_arrive(full);
+      };
+      long long off = w.done() ? -2 : find(w, w.first), v_off = -2;
+      while (ok && !w.done()) {
         const int stop = w.stop();
-        const int lim_max = row_limit(A, w.r, w.r.n - 1);
         for (int i = w.first; i < stop; ++i, ++g) {
           const int s = g & 1;
-          long long off = -1;
-          const int mine = i * kKeys + position(lane % kOwn);
-          const bool there = mine < lim_max;
-          if (there) off = row_offset(A, w.b, w.kh, mine, nullptr);
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            if (g >= 2 && !(ok = wait(kv ? &bar.v_empty[s] : &bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
-            const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + s * Lay::kTile + (piece >> 3) * Lay::kKSlab;
-            const T* src = static_cast<const T*>(kv ? A.c.v : A.c.k);
-#pragma unroll
-            for (int x = 0; x < kPasses; ++x) {
-              const int r = position(x * kRowsPass + sub);
-              const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-              const bool in = i * kKeys + r < lim_max;
-              const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-              if (in && o < 0 && kv == 0) {                    // no such page: its scores are NaN
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(at), "r"(0x7fff7fff) : "memory");
-              } else {
-                cp_async16(at, src + (in && o >= 0 ? o + piece * 8 : 0), in && o >= 0 ? 16 : 0);
-              }
-            }
-            if (kv == 0 && i == w.first) {                     // the piece's Q rides with its first K
-              if (g > 0) {                                     // once the last piece's products are done with theirs
-                cp_async_wait<0>();
-                while (fulls < 2 * g) announce();
-                if (!(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;
-              }
-              load_q(w);
-            }
-            cp_async_commit();
-            // V(g) waits for the product of V(g - 2), which is issued after that of K(g - 1): of the groups
-            // before V(g) only two may be unannounced
-            if (g * 2 + kv - fulls >= 2) {
-              cp_async_wait<2>();
-              announce();
-            }
+          if (g >= 2 && !(ok = wait(&bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
+          if (i == w.first) {                                  // the piece's Q rides with its first K,
+            if (g > 0 && !(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;   // when the last one's is done with
+            load_q(w);
           }
-          if (!ok) break;
+          fill(A.c.k, Lay::off_k + s * Lay::kTile, off, &bar.k_full[s], true);
+          if (g > 0) {
+            if (g >= 3 && !(ok = wait(&bar.v_empty[s ^ 1], (((g - 1) >> 1) + 1) & 1))) break;
+            fill(A.c.v, Lay::off_v + (s ^ 1) * Lay::kTile, v_off, &bar.v_full[s ^ 1], false);
+          }
+          v_off = off;
+          if (i + 1 < stop) off = find(w, i + 1);
         }
+        if (!ok) break;
+        w.next(A);
+        if (!w.done()) off = find(w, w.first);
       }
-      cp_async_wait<0>();
-      while (ok && fulls < 2 * g) announce();
+      if (ok && g > 0) {
+        const int s = (g - 1) & 1;
+        if (g >= 3) ok = wait(&bar.v_empty[s], (((g - 1) >> 1) + 1) & 1);
+        if (ok) fill(A.c.v, Lay::off_v + s * Lay::kTile, v_off, &bar.v_full[s], false);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-      // A unit's codes go through registers: the loads of the next unit are issued before this one's are
-      // widened and stored.
-      uint4 kr[kPasses], vr[kPasses];
-      float2 sc = make_float2(0.f, 0.f);
-      int pos = 0, lim = 0;
-      unsigned none = 0;                                       // bit x: pass x's row has no page
-      const auto fetch = [&](const Walk& w, int i) {
-        lim = row_limit(A, w.r, w.r.n - 1);
-        pos = i * kKeys;
+      // A unit's codes go through registers, two units in flight: each set is refilled as soon as its
+      // tile is stored.
+      struct Set {
+        uint4 k[kPasses], v[kPasses];
+        float2 sc;
+      } set[2];
+      Walk f = w;                                              // the unit to be fetched next
+      int fi = f.first;
+      const auto fetch = [&](Set& z) {
+        if (f.done()) return;
+        const int lim = row_limit(A, f.r, f.r.n - 1), pos = fi * kKeys;
         long long off = -1;
         const int mine = pos + position(lane % kOwn);
-        if (mine < lim) off = row_offset(A, w.b, w.kh, mine, nullptr);
-        none = 0;
+        if (mine < lim) off = row_offset(A, f.b, f.kh, mine, nullptr);
+        z.sc = make_float2(0.f, 1.f);
+        if (lt < kKeys && pos + lt < lim) {                    // a lane a position: its scales
+          long long so = 0;
+          if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0) z.sc = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+          else z.sc.x = __int_as_float(0x7fc00000);            // no such page: its scores are NaN
+        }
 #pragma unroll
         for (int x = 0; x < kPasses; ++x) {
           const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-          kr[x] = vr[x] = make_uint4(0, 0, 0, 0);
+          z.k[x] = z.v[x] = make_uint4(0, 0, 0, 0);
           if (o >= 0) {
-            kr[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.k) + o) + piece);
-            vr[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.v) + o) + piece);
+            z.k[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.k) + o) + piece);
+            z.v[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.v) + o) + piece);
           }
         }
-        if (lt < kKeys) {                                      // a lane a position: its scales
-          sc = make_float2(0.f, 1.f);
-          if (pos + lt < lim) {
-            long long so = 0;
-            if (row_offset(A, w.b, w.kh, pos + lt, &so) >= 0) sc = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
-            else sc.x = __int_as_float(0x7fc00000);            // no such page: its scores are NaN
-          }
+        if (++fi == f.stop()) {
+          f.next(A);
+          fi = f.first;
         }
       };
-      const auto put = [&](uint32_t dst, const uint4* regs) {
+      const auto put = [&](uint32_t tile, const uint4* regs) {
 #pragma unroll
         for (int x = 0; x < kPasses; ++x) {
           const int r = position(x * kRowsPass + sub);
           const uint4 a = widen8<T>(regs[x].x, regs[x].y), b = widen8<T>(regs[x].z, regs[x].w);
           const int c0 = piece * 2;                            // 16-byte pieces of the widened row
-          const uint32_t row = dst + (c0 >> 3) * Lay::kKSlab + r * 128;
+          const uint32_t row = base + tile + (c0 >> 3) * Lay::kKSlab + r * 128;
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + (((c0 & 7) ^ (r & 7)) << 4)), "r"(a.x), "r"(a.y),
                        "r"(a.z), "r"(a.w) : "memory");
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)), "r"(b.x), "r"(b.y),
                        "r"(b.z), "r"(b.w) : "memory");
         }
       };
-      if (!w.done()) fetch(w, w.first);
-      for (; ok && !w.done();) {
-        const int stop = w.stop(), first = w.first;
-        const Walk here = w;
-        w.next(A);
-        for (int i = first; i < stop; ++i, ++g) {
-          const int s = g & 1;
-          if (g >= 2 && !(ok = wait(&bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
-          put(base + Lay::off_k + s * Lay::kTile, kr);
-          if (lt < kKeys) {
-            // a scale of NaN reaches the row through its score; where the row may not see the position,
-            // its weight of 0 meets a finite factor
-            reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
-                make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
-          }
-          if (i == first) {
-            if (g > 0 && !(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;
-            load_q(here);
-            cp_async_commit();
-            cp_async_wait<0>();
-          }
-          announce();
-          if (g >= 2 && !(ok = wait(&bar.v_empty[s], ((g >> 1) + 1) & 1))) break;
-          put(base + Lay::off_v + s * Lay::kTile, vr);
-          announce();
-          if (i + 1 < stop) fetch(here, i + 1);
-          else if (!w.done()) fetch(w, w.first);
+      int i = w.first, stop = w.done() ? 0 : w.stop();
+      const auto unit = [&](Set& z) {                          // stores the unit `i` of the walk and fetches two ahead
+        const int s = g & 1;
+        if (g >= 2 && !wait(&bar.k_empty[s], ((g >> 1) + 1) & 1)) return false;
+        put(Lay::off_k + s * Lay::kTile, z.k);
+        if (lt < kKeys) {
+          // a scale of NaN reaches the row through its score; where the row may not see the position,
+          // its weight of 0 meets a finite factor
+          reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
+              make_float4(z.sc.x * (A.scale * kLog2e), log2f(z.sc.y), z.sc.y > 0.f ? 1.f / z.sc.y : 1.f, 0.f);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
         }
+        if (i == w.first) {
+          if (g > 0 && !wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1)) return false;
+          load_q(w);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        fence_async_shared();
+        mbar_arrive(&bar.k_full[s]);
+        if (g >= 2 && !wait(&bar.v_empty[s], ((g >> 1) + 1) & 1)) return false;
+        put(Lay::off_v + s * Lay::kTile, z.v);
+        fence_async_shared();
+        mbar_arrive(&bar.v_full[s]);
+        fetch(z);
+        ++g;
+        if (++i == stop) {
+          w.next(A);
+          if (!w.done()) { i = w.first; stop = w.stop(); }
+        }
+        return true;
+      };
+      fetch(set[0]);
+      fetch(set[1]);
+      while (!w.done()) {
+        if (!unit(set[0]) || w.done()) break;
+        if (!unit(set[1])) break;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   }
   tc_fence_before();
