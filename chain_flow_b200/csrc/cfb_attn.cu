@@ -30,12 +30,13 @@ namespace {
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
 constexpr int kM = 128, kKeys = 64;
-constexpr int kSoftWarps = 4, kLoadWarps = 8;
+constexpr int kSoftWarps = 8, kLoadWarps = 8;
+constexpr int kHalf = kKeys / 2;           // positions of a unit a softmax thread takes
 constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
 constexpr int kMmaWarp = kSoftWarps;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kScaleStages = 4;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum has grown by 2^8
 
 struct AttnArgs {
@@ -49,17 +50,19 @@ struct AttnArgs {
   float scale;
   int T, B, H, causal, rep;
   struct Desc* desc;                      // [grid]
-  float* part;                            // [grid][2][kM][dim + 2]
+  float* part;                            // [grid][2][kM][dim + 4]
 };
 
 struct Desc {                             // a piece that begins in this CTA's share and runs past its end
   int last;                               // the last CTA that holds a part of it; -1: no such piece
   int kh, t0, rows, row0;                 // kv head, first token row of the request, valid rows, first row of the tile
   int err;
-  long long units;                        // all units of the launch
+  long long each;                         // the deal: units a CTA, and how many CTAs have one more
+  int extra;
 };
 
-CFB_DEV long long share(long long units, int cta, int grid) { return units * cta / grid; }
+// first unit of CTA `cta`'s share
+CFB_DEV long long share(long long each, int extra, int cta) { return each * cta + min(cta, extra); }
 
 struct Request { int t0, n, L; bool over; };
 CFB_DEV Request request(const AttnArgs& A, int b) {
@@ -131,6 +134,7 @@ struct Walk {
 // Q, K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed
 // with row & 7. Q and K are read K-major (the head dim is summed over), V MN-major (the positions
 // are), from the same image.
+template <int D> constexpr int kPart = D + 4;   // floats of a row's partial result: o, m, l (rows 16-byte aligned)
 template <int D>
 struct Layout {
   static constexpr uint32_t kQ = kM * D * 2, kTile = kKeys * D * 2;
@@ -141,9 +145,11 @@ struct Layout {
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
 
+// full: a stage's tile has landed. s_done / o_done: the product S(i) / O += P(i) V(i) has completed, so
+// S may be read and K's stage refilled / O is up to date and P's and V's are free. p_full: P(i) is
+// written (and S(i) read). o_free: the piece's O has been read.
 struct Bars {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], pv_done[2], o_free, sc_full[kScaleStages], drain;
+  uint64_t k_full[2], v_full[2], s_done[2], p_full[2], o_done[2], o_free, sc_full[kScaleStages], swap[4], drain;
 };
 
 CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
@@ -171,14 +177,42 @@ CFB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 // D[tmem] (+)= A[tmem] . B[smem], 16-bit A (two elements a column) and B
-CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// over 64 positions: four products of 16 in one statement, by one elected lane (one election and one
+// statement for four take less issue time than four)
+CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "setp.ne.b32 q, %4, 0;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t}"
-      :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %8, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %9, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %10, %3, 1;\n\t}"
+      :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "r"(tmem_a + 16), "r"(tmem_a + 24),
+         "l"(b + 128), "l"(b + 256), "l"(b + 384)
+      : "memory");
+}
+// D[tmem] (+)= A[smem] . B[smem]^T over a 64-column slab of both
+CFB_DEV void mma_ss4_warp(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %4, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %8, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %9, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %10, %3, 1;\n\t}"
+      :: "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b + 2), "l"(b + 4),
+         "l"(b + 6)
+      : "memory");
 }
 // MN-major 128-byte-swizzled operand: 64-element slabs `slab` bytes apart, 8-row groups 1024 bytes apart
 CFB_DEV uint64_t mn_desc(uint32_t saddr, uint32_t slab) {
@@ -230,15 +264,14 @@ template <> CFB_DEV uint4 widen8<__half>(uint32_t lo, uint32_t hi) {
 // bias is 7, bf16's 127; subnormals come out as subnormals), and one exact product undoes that.
 template <> CFB_DEV uint4 widen8<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
   uint4 r;
-  const auto two = [](uint32_t b0, uint32_t b1) {
-    const uint32_t w = b0 | b1 << 16;
-    const uint32_t x = (w & 0x00800080u) << 8 | (w & 0x007f007fu) << 4;
+  const auto two = [](uint32_t w, uint32_t pick) {
+    const uint32_t t = __byte_perm(w, 0, pick);                // each half: code << 8
+    const uint32_t x = (t & 0x80008000u) | (t >> 4 & 0x07f007f0u);
     const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80));   // 2^120
     const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), up);
     return *reinterpret_cast<const uint32_t*>(&y);
   };
-  r.x = two(lo & 0xff, lo >> 8 & 0xff); r.y = two(lo >> 16 & 0xff, lo >> 24);
-  r.z = two(hi & 0xff, hi >> 8 & 0xff); r.w = two(hi >> 16 & 0xff, hi >> 24);
+  r.x = two(lo, 0x1404); r.y = two(lo, 0x3424); r.z = two(hi, 0x1404); r.w = two(hi, 0x3424);
   return r;
 }
 
@@ -260,9 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
   __shared__ long long sh_sum[kThreads / 32];
-  __shared__ long long sh_rest, sh_total;
+  __shared__ long long sh_rest;
   __shared__ int sh_req, sh_per;
   __shared__ int dead;
+  __shared__ float sh_swap[2][2 * kM];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,23 +304,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], kLoadThreads); mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], kLoadThreads); mbar_init(&bar.v_empty[i], 1);
-      mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], kSoftWarps); mbar_init(&bar.pv_done[i], 1);
+      mbar_init(&bar.k_full[i], kLoadThreads); mbar_init(&bar.v_full[i], kLoadThreads);
+      mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps); mbar_init(&bar.o_done[i], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
     for (int i = 0; i < kScaleStages; ++i) mbar_init(&bar.sc_full[i], kKeys / 32);
+    for (int i = 0; i < 4; ++i) mbar_init(&bar.swap[i], 2);
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
     dead = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
 
-  // where this CTA's share begins: the running sum of the requests' units
+  // where this CTA's share begins: the running sum of the requests' units (kept in registers while the
+  // requests are no more than the threads)
   long long total = 0;
+  int per = 0;
   for (int b0 = 0; b0 < A.B; b0 += kThreads) {
-    long long mine = 0;
-    if (b0 + (int)threadIdx.x < A.B) mine = (long long)head_units(A, request(A, b0 + threadIdx.x)) * A.c.kv_heads;
+    per = b0 + (int)threadIdx.x < A.B ? head_units(A, request(A, b0 + threadIdx.x)) : 0;
+    long long mine = (long long)per * A.c.kv_heads;
 #pragma unroll
     for (int off = 16; off; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
     if (lane == 0) sh_sum[warp] = mine;
@@ -294,17 +330,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
     for (int w = 0; w < kThreads / 32; ++w) total += sh_sum[w];
     __syncthreads();
   }
-  const long long from = share(total, cta, grid), to = share(total, cta + 1, grid);
+  const long long each = total / grid;
+  const int extra = (int)(total - each * grid);
+  const long long from = share(each, extra, cta), to = share(each, extra, cta + 1);
   if (threadIdx.x == 0) {
-    sh_total = total;
     A.desc[cta].last = -1;
     A.desc[cta].err = 0;
   }
   if (from < to) {
     long long before = 0;
     for (int b0 = 0; b0 < A.B && before <= from; b0 += kThreads) {
-      int per = 0;
-      if (b0 + (int)threadIdx.x < A.B) per = head_units(A, request(A, b0 + threadIdx.x));
+      if (A.B > kThreads) per = b0 + (int)threadIdx.x < A.B ? head_units(A, request(A, b0 + threadIdx.x)) : 0;
       const long long mine = (long long)per * A.c.kv_heads;
       long long run = mine;                                   // inclusive scan over the warp
 #pragma unroll
@@ -335,44 +371,64 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
   Walk w;
   w.start(A, from, to, sh_req, sh_rest, sh_per);
 
-  // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait.
+  // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait
+  // that is not over at once.
   const auto wait = [&](uint64_t* b, uint32_t parity) {
-    bool ok = mbar_wait(b, parity);
-    if (!ok) *reinterpret_cast<volatile int*>(&dead) = 1;
-    ok = ok && *reinterpret_cast<volatile int*>(&dead) == 0;
+    if (__all_sync(0xffffffffu, mbar_test_wait(b, parity))) return true;
+    volatile int* const d = &dead;
+    bool ok = true;
+    const unsigned long long t0 = globaltimer();
+    for (unsigned it = 1; !mbar_try_wait(b, parity); ++it)
+      if (it % kPollsPerCheck == 0) {
+        if (wait_expired(t0, kWaitBudgetNs)) *d = 1;
+        if (*d != 0) {
+          ok = false;
+          break;
+        }
+      }
     return __all_sync(0xffffffffu, ok) != 0;
   };
 
   if (warp < kSoftWarps) {
-    // ---------------------------------------------------------------- softmax: thread = row
-    const uint32_t tw = tmem + ((uint32_t)(warp * 32) << 16);
-    const int r = threadIdx.x;
+    // ---------------------------------------------------------------- softmax: two threads a row
+    const int half = warp >> 2, pair = warp & 3;               // warps w and w + 4 share 32 rows
+    const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
+    const int r = pair * 32 + lane;
     const float c2 = A.scale * kLog2e;
-    uint32_t g = 0, pieces = 0;                               // units and pieces so far
-    for (; !w.done(); w.next(A), ++pieces) {
+    uint32_t g = 0, turns = 0;                                 // units, exchanges so far
+    const auto exchange = [&](float mine, float* other) {      // the row's other thread's value
+      float* const slot = sh_swap[turns & 1];
+      slot[half * kM + r] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.swap[pair]);
+      if (!wait(&bar.swap[pair], turns & 1)) return false;
+      ++turns;
+      *other = slot[(half ^ 1) * kM + r];
+      return true;
+    };
+    for (; !w.done(); w.next(A)) {
       const int stop = w.stop(), first = w.first;
       const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
       const bool valid = r < rows;
       const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
       const int lim = valid ? row_limit(A, w.r, tok) : 0;
-      const bool warp_live = warp * 32 < rows;
+      const bool warp_live = pair * 32 < rows;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int i = first; i < stop; ++i, ++g) {
         const int s = g & 1;
-        if (!(ok = wait(&bar.s_full[s], (g >> 1) & 1))) break;
+        if (!(ok = wait(&bar.s_done[s], (g >> 1) & 1))) break;
         if (warp_live) {
           tc_fence_after();
-          float x[kKeys];
-          tmem_ld32(tw + Lay::s_col + s * kKeys, x);
-          tmem_ld32(tw + Lay::s_col + s * kKeys + 32, x + 32);
-          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys;
+          float x[kHalf];
+          tmem_ld32(tw + Lay::s_col + s * kKeys + half * kHalf, x);
+          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys + half * kHalf;
           if (QUANT) ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1);
           tmem_wait_ld();
           if (!ok) break;
-          const int j0 = i * kKeys;
+          const int j0 = i * kKeys + half * kHalf;
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) {
+          for (int e = 0; e < kHalf; ++e) {
             if constexpr (QUANT) {
               const float2 f = *reinterpret_cast<const float2*>(sc + e);
               x[e] = fmaf(x[e], f.x, f.y);
@@ -380,30 +436,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
               x[e] *= c2;
             }
           }
-          if (__any_sync(0xffffffffu, lim < j0 + kKeys)) {
+          if (__any_sync(0xffffffffu, lim < j0 + kHalf)) {
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e)
+            for (int e = 0; e < kHalf; ++e)
               if (j0 + e >= lim) x[e] = -INFINITY;
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
-          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          for (int e = 0; e < kHalf; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          float other;
+          if (!(ok = exchange(high, &other))) break;
+          high = fmaxf(high, other);
           // P's buffer is free once the product that read it two units ago is done
-          if (i - first >= 2 && !(ok = wait(&bar.pv_done[s], ((g >> 1) + 1) & 1))) break;
-          if (m == -INFINITY) {
-            // nothing seen yet: o is zero (or not begun), l is zero, any m will do
-            m = high;
-          }
-          if (__any_sync(0xffffffffu, high > m + kRescaleAt) && i > first) {
+          if (i - first >= 2 && !(ok = wait(&bar.o_done[s], ((g >> 1) + 1) & 1))) break;
+          if (m == -INFINITY) m = high;                        // nothing seen yet: o is zero (or not begun), l is zero
+          if (__any_sync(0xffffffffu, high > m + kRescaleAt)) {
             const float up = high > m + kRescaleAt ? high : m;
             const float keep = m == -INFINITY ? 1.f : exp2_approx(m - up);
-            if (!(ok = wait(&bar.pv_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
+            if (!(ok = wait(&bar.o_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
             tc_fence_after();
             l *= keep;
             m = up;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
+            for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
               float o[32];
               uint32_t u[32];
               tmem_ld32(tw + Lay::o_col + d, o);
@@ -415,9 +471,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
           }
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t p[kKeys / 2];
+          uint32_t p[kHalf / 2];
 #pragma unroll
-          for (int e = 0; e < kKeys; e += 2) {
+          for (int e = 0; e < kHalf; e += 2) {
             const float a = exp2_approx(x[e] - mm), b = exp2_approx(x[e + 1] - mm);
             if constexpr (QUANT) {
               sum[e & 3] = fmaf(a, sc[e].z, sum[e & 3]);
@@ -429,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
             p[e / 2] = pack16<T>(a, b);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st32(tw + Lay::p_col + s * (kKeys / 2), p);
+          tmem_st16(tw + Lay::p_col + s * (kKeys / 2) + half * (kHalf / 2), p);
           tmem_wait_st();
           tc_fence_before();
         }
@@ -439,22 +495,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       if (!ok) break;
       // the last product of the piece
       const uint32_t gl = g - 1;
-      if (!wait(&bar.pv_done[gl & 1], (gl >> 1) & 1)) break;
+      if (!wait(&bar.o_done[gl & 1], (gl >> 1) & 1)) break;
       tc_fence_after();
       if (warp_live) {
         const bool whole = first == 0 && stop == w.units;
+        float other;
+        if (!exchange(l, &other)) break;
+        l += other;
         if (w.r.over) l = __int_as_float(0x7fc00000);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         T* out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
-        float* part = A.part + ((long long)cta * 2 + (first == 0)) * kM * (D + 2) + (long long)r * (D + 2);
-        float bad = 0.f;                                      // turns NaN where an element is not finite
-#pragma unroll 1
-        for (int d = 0; d < D; d += 32) {
+        float* part = A.part + (((long long)cta * 2 + (first == 0)) * kM + r) * kPart<D>;
+        float bad[4] = {0.f, 0.f, 0.f, 0.f};                   // turn NaN where an element is not finite
+#pragma unroll
+        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
           float o[32];
           tmem_ld32(tw + Lay::o_col + d, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) bad = fmaf(o[e], 0.f, bad);
+          for (int e = 0; e < 32; ++e) bad[e & 3] = fmaf(o[e], 0.f, bad[e & 3]);
           if (valid && whole) {
             uint4* dst = reinterpret_cast<uint4*>(out + d);
 #pragma unroll
@@ -465,29 +524,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
                                              pack16<T>(y[4] * inv, y[5] * inv), pack16<T>(y[6] * inv, y[7] * inv));
             }
           } else if (valid) {
-            float2* dst = reinterpret_cast<float2*>(part + d);
+            float4* dst = reinterpret_cast<float4*>(part + d);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dst[e] = make_float2(o[2 * e], o[2 * e + 1]);
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
           __syncwarp();
         }
-        if (valid) {
+        if (valid && half == 0) {
           if (!whole) {
             part[D] = m;
             part[D + 1] = l;
           } else if (A.lse) {
-            A.lse[(long long)head * A.T + w.r.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+            A.lse[(long long)head * A.T + w.r.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
           }
         }
         if constexpr (!QUANT) {
           // A value that is not finite at a position that this row may not see has met a weight of 0 in
           // the product. Only a causal row's last units can hold one; such a row is taken again from
           // its own positions alone, with m and l as they are.
-          unsigned again = __ballot_sync(0xffffffffu, A.causal && valid && bad != 0.f && l == l && lim < stop * kKeys);
+          const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
+          unsigned again = __ballot_sync(0xffffffffu, A.causal && valid && worst != 0.f && l == l && lim < stop * kKeys);
           while (again) {
             const int src = __ffs(again) - 1;
             again &= again - 1;
-            const int row = warp * 32 + src, RR = w.tile * kM + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
+            const int row = pair * 32 + src, RR = w.tile * kM + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
             const int li = __shfl_sync(0xffffffffu, lim, src);
             const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
             constexpr int E = D / 32;
@@ -510,12 +570,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
               for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(vp[e]), acc[e]);
             }
             T* op = static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h + lane * E;
-            float* pp = A.part + ((long long)cta * 2 + (first == 0)) * kM * (D + 2) + (long long)row * (D + 2) + lane * E;
+            float* pp = A.part + (((long long)cta * 2 + (first == 0)) * kM + row) * kPart<D> + lane * E;
             __syncwarp();
+            if (lane >> 4 == half) {                           // this warp's half of the row
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              if (whole) op[e] = from_float<T>(acc[e] * ir);
-              else pp[e] = acc[e];
+              for (int e = 0; e < E; ++e) {
+                if (whole) op[e] = from_float<T>(acc[e] * ir);
+                else pp[e] = acc[e];
+              }
             }
           }
         }
@@ -525,10 +587,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       if (lane == 0) mbar_arrive(&bar.o_free);
       if (threadIdx.x == 0 && first == 0 && stop < w.units) {  // begins here, ends elsewhere
         const long long end = w.u + w.units;                   // w.u: its first unit
-        int last = cta + 1;
-        while (share(total, last + 1, grid) < end) ++last;
         Desc d;
-        d.last = last; d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * kM; d.err = 0; d.units = total;
+        d.last = cta + 1;
+        while (share(each, extra, d.last + 1) < end) ++d.last;
+        d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * kM; d.err = 0; d.each = each; d.extra = extra;
         A.desc[cta] = d;
       }
     }
@@ -543,12 +605,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       if (!wait(&bar.v_full[s], (u >> 1) & 1) || !wait(&bar.p_full[s], (u >> 1) & 1)) return false;
       fence_async_shared();
       tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts_warp(tmem + Lay::o_col, tmem + Lay::p_col + s * (kKeys / 2) + k * 8,
-                    mn_desc(base + Lay::off_v + s * Lay::kTile + k * 2048, Lay::kKSlab), idesc_o, !(fresh && k == 0));
-      tc_commit_warp(&bar.v_empty[s]);
-      tc_commit_warp(&bar.pv_done[s]);
+      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::p_col + s * (kKeys / 2), mn_desc(base + Lay::off_v + s * Lay::kTile, Lay::kKSlab),
+                   idesc_o, !fresh);
+      tc_commit_warp(&bar.o_done[s]);
       return true;
     };
     for (; ok && !w.done(); w.next(A), ++pieces) {
@@ -559,12 +618,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
         fence_async_shared();                                  // the copies are the generic proxy's
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma_f16_warp(tmem + Lay::s_col + s * kKeys,
-                          sw128_desc(base + Lay::off_q + (k / 4) * Lay::kQSlab + (k % 4) * 32),
-                          sw128_desc(base + Lay::off_k + s * Lay::kTile + (k / 4) * Lay::kKSlab + (k % 4) * 32), idesc_s, k > 0);
-        tc_commit_warp(&bar.k_empty[s]);
-        tc_commit_warp(&bar.s_full[s]);
+        for (int k = 0; k < D / 64; ++k)
+          mma_ss4_warp(tmem + Lay::s_col + s * kKeys, sw128_desc(base + Lay::off_q + k * Lay::kQSlab),
+                       sw128_desc(base + Lay::off_k + s * Lay::kTile + k * Lay::kKSlab), idesc_s, k > 0);
+        tc_commit_warp(&bar.s_done[s]);
         if (i > 0) {
           // the piece's first product overwrites O: the last piece's must have been read
           if (i == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
@@ -634,14 +691,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
         const int stop = w.stop();
         for (int i = w.first; i < stop; ++i, ++g) {
           const int s = g & 1;
-          if (g >= 2 && !(ok = wait(&bar.k_empty[s], ((g >> 1) + 1) & 1))) break;
+          if (g >= 2 && !(ok = wait(&bar.s_done[s], ((g >> 1) + 1) & 1))) break;
           if (i == w.first) {                                  // the piece's Q rides with its first K,
-            if (g > 0 && !(ok = wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1))) break;   // when the last one's is done with
+            if (g > 0 && !(ok = wait(&bar.s_done[s ^ 1], ((g - 1) >> 1) & 1))) break;   // when the last one's is done with
             load_q(w);
           }
           fill(A.c.k, Lay::off_k + s * Lay::kTile, off, &bar.k_full[s], true);
           if (g > 0) {
-            if (g >= 3 && !(ok = wait(&bar.v_empty[s ^ 1], (((g - 1) >> 1) + 1) & 1))) break;
+            if (g >= 3 && !(ok = wait(&bar.o_done[s ^ 1], (((g - 1) >> 1) + 1) & 1))) break;
             fill(A.c.v, Lay::off_v + (s ^ 1) * Lay::kTile, v_off, &bar.v_full[s ^ 1], false);
           }
           v_off = off;
@@ -653,43 +710,42 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       }
       if (ok && g > 0) {
         const int s = (g - 1) & 1;
-        if (g >= 3) ok = wait(&bar.v_empty[s], (((g - 1) >> 1) + 1) & 1);
+        if (g >= 3) ok = wait(&bar.o_done[s], (((g - 1) >> 1) + 1) & 1);
         if (ok) fill(A.c.v, Lay::off_v + s * Lay::kTile, v_off, &bar.v_full[s], false);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-      // A unit's codes go through registers, two units in flight: each set is refilled as soon as its
-      // tile is stored.
-      struct Set {
-        uint4 k[kPasses], v[kPasses];
-        float2 sc;
-      } set[2];
-      Walk f = w;                                              // the unit to be fetched next
+      // A tile's codes go through registers: each is refilled with the next unit's as soon as it is
+      // stored, so one to two tiles are in flight. Pages and scales are looked up a unit before that.
+      uint4 kr[kPasses], vr[kPasses];
+      Walk f = w;                                              // the unit to be looked up next
       int fi = f.first;
-      const auto fetch = [&](Set& z) {
+      long long off = -1;                                      // the looked-up unit's rows (a lane's) and scales
+      float2 sc_next = make_float2(0.f, 1.f), sc = sc_next;
+      const auto look = [&] {
+        off = -1;
+        sc_next = make_float2(0.f, 1.f);
         if (f.done()) return;
         const int lim = row_limit(A, f.r, f.r.n - 1), pos = fi * kKeys;
-        long long off = -1;
         const int mine = pos + position(lane % kOwn);
         if (mine < lim) off = row_offset(A, f.b, f.kh, mine, nullptr);
-        z.sc = make_float2(0.f, 1.f);
         if (lt < kKeys && pos + lt < lim) {                    // a lane a position: its scales
           long long so = 0;
-          if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0) z.sc = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
-          else z.sc.x = __int_as_float(0x7fc00000);            // no such page: its scores are NaN
-        }
-#pragma unroll
-        for (int x = 0; x < kPasses; ++x) {
-          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-          z.k[x] = z.v[x] = make_uint4(0, 0, 0, 0);
-          if (o >= 0) {
-            z.k[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.k) + o) + piece);
-            z.v[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.c.v) + o) + piece);
-          }
+          if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0)
+            sc_next = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+          else sc_next.x = __int_as_float(0x7fc00000);         // no such page: its scores are NaN
         }
         if (++fi == f.stop()) {
           f.next(A);
           fi = f.first;
+        }
+      };
+      const auto fetch = [&](const void* pool, uint4* regs) {
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+          regs[x] = make_uint4(0, 0, 0, 0);
+          if (o >= 0) regs[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + o) + piece);
         }
       };
       const auto put = [&](uint32_t tile, const uint4* regs) {
@@ -705,43 +761,42 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
                        "r"(b.z), "r"(b.w) : "memory");
         }
       };
-      int i = w.first, stop = w.done() ? 0 : w.stop();
-      const auto unit = [&](Set& z) {                          // stores the unit `i` of the walk and fetches two ahead
-        const int s = g & 1;
-        if (g >= 2 && !wait(&bar.k_empty[s], ((g >> 1) + 1) & 1)) return false;
-        put(Lay::off_k + s * Lay::kTile, z.k);
-        if (lt < kKeys) {
-          // a scale of NaN reaches the row through its score; where the row may not see the position,
-          // its weight of 0 meets a finite factor
-          reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
-              make_float4(z.sc.x * (A.scale * kLog2e), log2f(z.sc.y), z.sc.y > 0.f ? 1.f / z.sc.y : 1.f, 0.f);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
+      look();
+      fetch(A.c.k, kr);
+      fetch(A.c.v, vr);
+      sc = sc_next;
+      look();
+      for (; ok && !w.done(); w.next(A)) {
+        const int stop = w.stop();
+        for (int i = w.first; i < stop; ++i, ++g) {
+          const int s = g & 1;
+          if (g >= 2 && !(ok = wait(&bar.s_done[s], ((g >> 1) + 1) & 1))) break;
+          put(Lay::off_k + s * Lay::kTile, kr);
+          fetch(A.c.k, kr);
+          if (lt < kKeys) {
+            // a scale of NaN reaches the row through its score; where the row may not see the position,
+            // its weight of 0 meets a finite factor
+            reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
+                make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
+          }
+          if (i == w.first) {
+            if (g > 0 && !(ok = wait(&bar.s_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
+            load_q(w);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+          }
+          fence_async_shared();
+          mbar_arrive(&bar.k_full[s]);
+          if (g >= 2 && !(ok = wait(&bar.o_done[s], ((g >> 1) + 1) & 1))) break;
+          put(Lay::off_v + s * Lay::kTile, vr);
+          fence_async_shared();
+          mbar_arrive(&bar.v_full[s]);
+          fetch(A.c.v, vr);
+          sc = sc_next;
+          look();
         }
-        if (i == w.first) {
-          if (g > 0 && !wait(&bar.k_empty[s ^ 1], ((g - 1) >> 1) & 1)) return false;
-          load_q(w);
-          asm volatile("cp.async.wait_all;" ::: "memory");
-        }
-        fence_async_shared();
-        mbar_arrive(&bar.k_full[s]);
-        if (g >= 2 && !wait(&bar.v_empty[s], ((g >> 1) + 1) & 1)) return false;
-        put(Lay::off_v + s * Lay::kTile, z.v);
-        fence_async_shared();
-        mbar_arrive(&bar.v_full[s]);
-        fetch(z);
-        ++g;
-        if (++i == stop) {
-          w.next(A);
-          if (!w.done()) { i = w.first; stop = w.stop(); }
-        }
-        return true;
-      };
-      fetch(set[0]);
-      fetch(set[1]);
-      while (!w.done()) {
-        if (!unit(set[0]) || w.done()) break;
-        if (!unit(set[1])) break;
+        if (!ok) break;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
@@ -766,37 +821,62 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
   const Desc d = A.desc[cta];
   const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + threadIdx.x / 32;
   if (d.last < 0 || r >= d.rows) return;
-  const auto part_of = [&](int c) { return A.part + ((long long)c * 2 + (c == cta)) * kM * (D + 2) + (long long)r * (D + 2); };
-  const auto holds = [&](int c) { return c == cta || share(d.units, c, grid) < share(d.units, c + 1, grid); };
+  // the parts: this CTA's second one, then the first one of every later CTA that has a share
+  const int last = d.each > 0 ? d.last : min(d.last, d.extra - 1);
+  const auto part_of = [&](int c) { return A.part + (((long long)c * 2 + (c == cta)) * kM + r) * kPart<D>; };
   float m = -INFINITY;
-  for (int c = cta + lane; c <= d.last; c += 32)
-    if (holds(c)) m = fmaxf(m, part_of(c)[D]);
+  for (int c = cta + lane; c <= last; c += 32) m = fmaxf(m, part_of(c)[D]);
 #pragma unroll
   for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float mm = m == -INFINITY ? 0.f : m;
-  constexpr int E = D / 32;
+  constexpr int E = D / 32, V = E < 4 ? E : 4;                 // elements a lane; of one access
   float acc[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int c = cta; c <= d.last; ++c) {
-    if (!holds(c)) continue;
-    const float* p = part_of(c);
-    const float w = exp2_approx(p[D] - mm);
-    l = fmaf(w, p[D + 1], l);
+  for (int c0 = cta; c0 <= last; c0 += 32) {
+    float wl = 0.f, ll = 0.f;
+    if (c0 + lane <= last) {
+      const float* p = part_of(c0 + lane);
+      wl = exp2_approx(p[D] - mm);
+      ll = p[D + 1];
+    }
+    const int n = min(32, last + 1 - c0);
+    constexpr int kBatch = 8;                                  // parts whose loads are in flight together
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+      float x[kBatch][E];
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p + e * 32 + lane * 2);
-      acc[e] = fmaf(w, x.x, acc[e]);
-      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+      for (int i = 0; i < kBatch; ++i) {
+        const float* p = part_of(min(c0 + i0 + i, last)) + lane * V;
+#pragma unroll
+        for (int e = 0; e < E; e += V) {
+          if constexpr (V == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(p + e * 32);
+            x[i][e] = y.x; x[i][e + 1] = y.y; x[i][e + 2] = y.z; x[i][e + 3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(p + e * 32);
+            x[i][e] = y.x; x[i][e + 1] = y.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float w = __shfl_sync(0xffffffffu, wl, i0 + i);
+        const float lp = __shfl_sync(0xffffffffu, ll, i0 + i);
+        if (i0 + i >= n) break;
+        l = fmaf(w, lp, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[i][e], acc[e]);
+      }
     }
   }
   const int R = d.row0 + r, tok = R / A.rep, head = d.kh * A.rep + R - tok * A.rep;
   T* out = static_cast<T*>(A.o) + (long long)(d.t0 + tok) * A.so_t + head * A.so_h;
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(out + e * 32 + lane * 2) = l == 0.f ? 0u : pack16<T>(acc[e] / l, acc[e + 1] / l);
-  if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+  for (int e = 0; e < E; e += V)
+#pragma unroll
+    for (int x = 0; x < V; x += 2)
+      *reinterpret_cast<uint32_t*>(out + e * 32 + lane * V + x) = l == 0.f ? 0u : pack16<T>(acc[e + x] / l, acc[e + x + 1] / l);
+  if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 int sm_count() {
@@ -833,7 +913,7 @@ cfb_status launch_dim(const AttnArgs& A, int grid, cudaStream_t st) {
 extern "C" size_t cfb_paged_attn_workspace(int H, int kv_heads, int dim) {
   if (H <= 0 || kv_heads <= 0 || dim <= 0) return 0;
   const int grid = sm_count();
-  return desc_bytes(grid) + (size_t)grid * 2 * kM * (dim + 2) * sizeof(float);
+  return desc_bytes(grid) + (size_t)grid * 2 * kM * (dim + 4) * sizeof(float);
 }
 
 extern "C" cfb_status cfb_paged_attn_error(const void* ws, int* device_error) {
