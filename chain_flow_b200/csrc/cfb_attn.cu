@@ -30,8 +30,7 @@ namespace {
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
 constexpr int kM = 128, kKeys = 64;
-constexpr int kSoftWarps = 8, kLoadWarps = 8;
-constexpr int kHalf = kKeys / 2;           // positions of a unit a softmax thread takes
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
 constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
 constexpr int kMmaWarp = kSoftWarps;
 constexpr int kLoadThreads = kLoadWarps * 32;
@@ -97,10 +96,9 @@ struct Walk {
   Request r;
   CFB_DEV void start(const AttnArgs& A, long long from, long long to, int req, long long rest, int per_head) {
     u = from; end = to; b = req;
-    if (u >= end) return;
     r = request(A, b);
     tiles = tiles_of(A, r);
-    kh = (int)(rest / per_head);
+    kh = (int)(rest <= 0x7fffffff ? (unsigned)rest / (unsigned)per_head : rest / per_head);
     first = (int)(rest - (long long)kh * per_head);
     tile = 0;
     for (;;) {
@@ -132,8 +130,11 @@ struct Walk {
 
 // ---- shared and tensor memory ------------------------------------------------------------------------
 // Q, K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed
-// with row & 7. Q and K are read K-major (the head dim is summed over), V MN-major (the positions
-// are), from the same image.
+// with row & 7. K is read K-major (the head dim is summed over), V MN-major (the positions are), from
+// the same image. Q moves on to tensor memory: as the first operand of S = Q K^T it would be read from
+// shared memory again with every unit, and a 128 x 64 product of 16 reads 4 KB of it in its 32 cycles,
+// the whole shared-memory bandwidth. Tensor memory columns: two units' S (fp32), each overwritten by
+// its P (16-bit), then Q, then O.
 template <int D> constexpr int kPart = D + 4;   // floats of a row's partial result: o, m, l (rows 16-byte aligned)
 template <int D>
 struct Layout {
@@ -141,15 +142,17 @@ struct Layout {
   static constexpr uint32_t kQSlab = kM * 128, kKSlab = kKeys * 128;
   static constexpr uint32_t off_q = 0, off_k = kQ, off_v = kQ + 2 * kTile, off_scale = kQ + 4 * kTile;
   static constexpr uint32_t bytes = off_scale + kScaleStages * kKeys * 16 + 1024;
-  static constexpr uint32_t s_col = 0, p_col = 2 * kKeys, o_col = 3 * kKeys + (D == 256 ? 64 : 0);   // TMEM columns
+  static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
 
-// full: a stage's tile has landed. s_done / o_done: the product S(i) / O += P(i) V(i) has completed, so
-// S may be read and K's stage refilled / O is up to date and P's and V's are free. p_full: P(i) is
-// written (and S(i) read). o_free: the piece's O has been read.
+// full: a tile has landed. q_ready: Q is in tensor memory (and its staging free). s_done / o_done: the
+// product S(i) / O += P(i) V(i) has completed, so S may be read and K's stage refilled / O is up to
+// date and V's stage free. p_full: P(i) is written (and S(i) read). m_set: the rows' maximum after unit
+// i is in shared memory. o_free: the piece's O has been read.
 struct Bars {
-  uint64_t k_full[2], v_full[2], s_done[2], p_full[2], o_done[2], o_free, sc_full[kScaleStages], swap[4], drain;
+  uint64_t q_full, q_ready, k_full[2], v_full[2], s_done[2], p_full[2], o_done[2], o_free, sc_full[kScaleStages],
+      m_set[2][4], swap[4], drain;
 };
 
 CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
@@ -185,9 +188,9 @@ CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 // D[tmem] (+)= A[tmem] . B[smem], 16-bit A (two elements a column) and B
-// over 64 positions: four products of 16 in one statement, by one elected lane (one election and one
-// statement for four take less issue time than four)
-CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// over 64 of the summed dim: four products of 16 in one statement, by one elected lane (one election and
+// one statement for four take less issue time than four), B's descriptor advancing by `step`
+CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t step, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
@@ -197,21 +200,7 @@ CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t
       "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %9, %3, 1;\n\t"
       "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %10, %3, 1;\n\t}"
       :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "r"(tmem_a + 16), "r"(tmem_a + 24),
-         "l"(b + 128), "l"(b + 256), "l"(b + 384)
-      : "memory");
-}
-// D[tmem] (+)= A[smem] . B[smem]^T over a 64-column slab of both
-CFB_DEV void mma_ss4_warp(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "setp.ne.b32 q, %4, 0;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %5, %8, %3, 1;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %6, %9, %3, 1;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %7, %10, %3, 1;\n\t}"
-      :: "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b + 2), "l"(b + 4),
-         "l"(b + 6)
+         "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step)
       : "memory");
 }
 // MN-major 128-byte-swizzled operand: 64-element slabs `slab` bytes apart, 8-row groups 1024 bytes apart
@@ -276,13 +265,13 @@ template <> CFB_DEV uint4 widen8<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------
-// One CTA per SM, 13 warps. Warps 5-12 load: per piece the Q tile, per unit a K and a V tile (two
+// One CTA per SM, 13 warps. Warps 9-12 load: per piece the Q tile, per unit a K and a V tile (two
 // stages each) with 16-byte copies, rows found through the page table, positions past the end filled
-// with zeros; e4m3 rows come through registers, where they are widened. Warp 4 issues the tensor
+// with zeros; e4m3 rows come through registers, where they are widened. Warp 8 issues the tensor
 // work: S(i) = Q K(i)^T into one of two fp32 tiles in tensor memory, then O += P(i-1) V(i-1) with P
-// read from tensor memory, so the softmax of a unit runs beside the next unit's product. Warps 0-3
-// are the softmax, a thread a row: the row's 64 scores come from tensor memory, the maximum is kept
-// in the thread, the weights go back to tensor memory in the operands' type (the one rounding of the
+// read from tensor memory, so the softmax of a unit runs beside the next unit's product. Warps 0-7
+// are the softmax, a thread a row, units alternating between two groups: the row's 64 scores come from
+// tensor memory, and the weights go back there in the operands' type (the one rounding of the
 // weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of the unrounded fp32 values). O is
 // rescaled only when the row's maximum has grown by more than 2^8 since the last time: weights are
 // then at most 2^8, far inside both types, and most units touch O not at all.
@@ -292,20 +281,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ long long sh_sum[kThreads / 32];
-  __shared__ long long sh_rest;
-  __shared__ int sh_req, sh_per;
   __shared__ int dead;
-  __shared__ float sh_swap[2][2 * kM];
+  __shared__ float sh_m[2][kM];
+  __shared__ float2 sh_swap[2 * kM];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grid = gridDim.x, cta = blockIdx.x;
 
   if (threadIdx.x == 0) {
+    mbar_init(&bar.q_full, kLoadThreads);
+    mbar_init(&bar.q_ready, kSoftWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.k_full[i], kLoadThreads); mbar_init(&bar.v_full[i], kLoadThreads);
-      mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps); mbar_init(&bar.o_done[i], 1);
+      mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps / 2); mbar_init(&bar.o_done[i], 1);
+      for (int j = 0; j < 4; ++j) mbar_init(&bar.m_set[i][j], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
     for (int i = 0; i < kScaleStages; ++i) mbar_init(&bar.sc_full[i], kKeys / 32);
@@ -313,63 +303,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
     dead = 0;
-  }
-  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
-
-  // where this CTA's share begins: the running sum of the requests' units (kept in registers while the
-  // requests are no more than the threads)
-  long long total = 0;
-  int per = 0;
-  for (int b0 = 0; b0 < A.B; b0 += kThreads) {
-    per = b0 + (int)threadIdx.x < A.B ? head_units(A, request(A, b0 + threadIdx.x)) : 0;
-    long long mine = (long long)per * A.c.kv_heads;
-#pragma unroll
-    for (int off = 16; off; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
-    if (lane == 0) sh_sum[warp] = mine;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) total += sh_sum[w];
-    __syncthreads();
-  }
-  const long long each = total / grid;
-  const int extra = (int)(total - each * grid);
-  const long long from = share(each, extra, cta), to = share(each, extra, cta + 1);
-  if (threadIdx.x == 0) {
     A.desc[cta].last = -1;
     A.desc[cta].err = 0;
   }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
+
+  // Where this CTA's share begins: the running sum of the requests' units, by every warp for itself, a
+  // lane a request.
+  long long total = 0;
+  int per = 0;
+  for (int b0 = 0; b0 < A.B; b0 += 32) {
+    per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
+    long long sum = (long long)per * A.c.kv_heads;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    total += sum;
+  }
+  const long long each = total <= 0x7fffffff ? (long long)((unsigned)total / (unsigned)grid) : total / grid;
+  const int extra = (int)(total - each * grid);
+  const long long from = share(each, extra, cta), to = share(each, extra, cta + 1);
+  Walk w;
+  w.u = w.end = 0;
   if (from < to) {
     long long before = 0;
-    for (int b0 = 0; b0 < A.B && before <= from; b0 += kThreads) {
-      if (A.B > kThreads) per = b0 + (int)threadIdx.x < A.B ? head_units(A, request(A, b0 + threadIdx.x)) : 0;
+    for (int b0 = 0;; b0 += 32) {
+      if (A.B > 32) per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
       const long long mine = (long long)per * A.c.kv_heads;
-      long long run = mine;                                   // inclusive scan over the warp
+      long long run = mine;                                    // inclusive scan
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, run, off);
         if (lane >= off) run += y;
       }
-      if (lane == 31) sh_sum[warp] = run;
-      __syncthreads();
-      long long all = 0;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w == warp) run += before + all;
-        all += sh_sum[w];
+      const unsigned here = __ballot_sync(0xffffffffu, from < before + run);
+      if (here) {                                              // the first request whose units reach past `from`
+        const int x = __ffs(here) - 1;
+        w.start(A, from, to, b0 + x, from - before - __shfl_sync(0xffffffffu, run - mine, x), __shfl_sync(0xffffffffu, per, x));
+        break;
       }
-      if (from >= run - mine && from < run) {
-        sh_req = b0 + threadIdx.x;
-        sh_rest = from - (run - mine);
-        sh_per = per;
-      }
-      before += all;
-      __syncthreads();
+      before += __shfl_sync(0xffffffffu, run, 31);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  Walk w;
-  w.start(A, from, to, sh_req, sh_rest, sh_per);
 
   // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait
   // that is not over at once.
@@ -390,45 +368,64 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
   };
 
   if (warp < kSoftWarps) {
-    // ---------------------------------------------------------------- softmax: two threads a row
+    // ---------------------------------------------------------------- softmax: a thread a row
+    // Two groups of four warps take the units in turn, so that two units' softmax run side by side. The
+    // row's maximum passes from unit to unit through shared memory; each group keeps its own sum.
     const int half = warp >> 2, pair = warp & 3;               // warps w and w + 4 share 32 rows
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
     const int r = pair * 32 + lane;
     const float c2 = A.scale * kLog2e;
-    uint32_t g = 0, turns = 0;                                 // units, exchanges so far
-    const auto exchange = [&](float mine, float* other) {      // the row's other thread's value
-      float* const slot = sh_swap[turns & 1];
-      slot[half * kM + r] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.swap[pair]);
-      if (!wait(&bar.swap[pair], turns & 1)) return false;
-      ++turns;
-      *other = slot[(half ^ 1) * kM + r];
-      return true;
-    };
-    for (; !w.done(); w.next(A)) {
+    uint32_t g0 = 0, pieces = 0, swaps = 0;                    // units and pieces before this one; exchanges of sums
+    for (; !w.done(); g0 += w.stop() - w.first, w.next(A), ++pieces) {
       const int stop = w.stop(), first = w.first;
       const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
       const bool valid = r < rows;
       const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
       const int lim = valid ? row_limit(A, w.r, tok) : 0;
       const bool warp_live = pair * 32 < rows;
-      float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int i = first; i < stop; ++i, ++g) {
+      // Q from its staging to tensor memory, a half of the head dim a group
+      if (!wait(&bar.q_full, pieces & 1)) break;
+      if (warp_live) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < (D == 64 ? 1 : D / 128); ++c) {
+          constexpr int kCols = D == 64 ? 16 : 32, kPieces = kCols / 4;
+          const int piece0 = half * (D / 16) + c * 8;          // 16-byte pieces of the row
+          uint32_t u[kCols];
+#pragma unroll
+          for (int e = 0; e < kPieces; ++e) {
+            const int pc = piece0 + e;
+            const uint4 y = *reinterpret_cast<const uint4*>(sm + Lay::off_q + (pc >> 3) * Lay::kQSlab + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
+            u[4 * e] = y.x; u[4 * e + 1] = y.y; u[4 * e + 2] = y.z; u[4 * e + 3] = y.w;
+          }
+          if constexpr (kCols == 32) tmem_st32(tw + Lay::q_col + piece0 * 4, u);
+          else tmem_st16(tw + Lay::q_col + piece0 * 4, u);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.q_ready);
+
+      float m = -INFINITY, l = 0.f;                            // this group's: l in units of 2^m
+      for (int i = first; i < stop; ++i) {
+        const uint32_t g = g0 + (i - first);
         const int s = g & 1;
+        if (s != half) continue;
         if (!(ok = wait(&bar.s_done[s], (g >> 1) & 1))) break;
         if (warp_live) {
           tc_fence_after();
-          float x[kHalf];
-          tmem_ld32(tw + Lay::s_col + s * kKeys + half * kHalf, x);
-          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys + half * kHalf;
+          float x[kKeys];
+          tmem_ld32(tw + Lay::s_col + s * kKeys, x);
+          tmem_ld32(tw + Lay::s_col + s * kKeys + 32, x + 32);
+          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys;
           if (QUANT) ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1);
           tmem_wait_ld();
           if (!ok) break;
-          const int j0 = i * kKeys + half * kHalf;
+          const int j0 = i * kKeys;
 #pragma unroll
-          for (int e = 0; e < kHalf; ++e) {
+          for (int e = 0; e < kKeys; ++e) {
             if constexpr (QUANT) {
               const float2 f = *reinterpret_cast<const float2*>(sc + e);
               x[e] = fmaf(x[e], f.x, f.y);
@@ -436,72 +433,87 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
               x[e] *= c2;
             }
           }
-          if (__any_sync(0xffffffffu, lim < j0 + kHalf)) {
+          if (__any_sync(0xffffffffu, lim < j0 + kKeys)) {
 #pragma unroll
-            for (int e = 0; e < kHalf; ++e)
+            for (int e = 0; e < kKeys; ++e)
               if (j0 + e >= lim) x[e] = -INFINITY;
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < kHalf; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
-          float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          float other;
-          if (!(ok = exchange(high, &other))) break;
-          high = fmaxf(high, other);
-          // P's buffer is free once the product that read it two units ago is done
-          if (i - first >= 2 && !(ok = wait(&bar.o_done[s], ((g >> 1) + 1) & 1))) break;
-          if (m == -INFINITY) m = high;                        // nothing seen yet: o is zero (or not begun), l is zero
-          if (__any_sync(0xffffffffu, high > m + kRescaleAt)) {
-            const float up = high > m + kRescaleAt ? high : m;
-            const float keep = m == -INFINITY ? 1.f : exp2_approx(m - up);
+          for (int e = 0; e < kKeys; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          float now = -INFINITY;                               // the maximum the weights so far are relative to
+          if (i > first) {
+            if (!(ok = wait(&bar.m_set[s ^ 1][pair], ((g - 1) >> 1) & 1))) break;
+            now = sh_m[s ^ 1][r];
+          }
+          const float before = now;
+          if (now == -INFINITY || high > now + kRescaleAt) now = high;
+          sh_m[s][r] = now;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
+          // (o is zero, or not begun, while nothing has been seen)
+          const float keep = before == -INFINITY ? 1.f : exp2_approx(before - now);
+          if (__any_sync(0xffffffffu, keep != 1.f)) {
             if (!(ok = wait(&bar.o_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
             tc_fence_after();
-            l *= keep;
-            m = up;
 #pragma unroll 1
-            for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
-              float o[32];
-              uint32_t u[32];
-              tmem_ld32(tw + Lay::o_col + d, o);
-              tmem_wait_ld();
+            for (int d = 0; d < D; d += 16) {
+              float o[16];
+              uint32_t u[16];
+              tmem_ld16(tw + Lay::o_col + d, o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * keep);
-              tmem_st32(tw + Lay::o_col + d, u);
+              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * keep);
+              tmem_st16(tw + Lay::o_col + d, u);
             }
           }
+          l *= m == -INFINITY ? 1.f : exp2_approx(m - now);
+          m = now;
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t p[kHalf / 2];
 #pragma unroll
-          for (int e = 0; e < kHalf; e += 2) {
-            const float a = exp2_approx(x[e] - mm), b = exp2_approx(x[e + 1] - mm);
-            if constexpr (QUANT) {
-              sum[e & 3] = fmaf(a, sc[e].z, sum[e & 3]);
-              sum[(e + 1) & 3] = fmaf(b, sc[e + 1].z, sum[(e + 1) & 3]);
-            } else {
-              sum[e & 3] += a;
-              sum[(e + 1) & 3] += b;
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float a = exp2_approx(x[32 * c + e] - mm), b = exp2_approx(x[32 * c + e + 1] - mm);
+              if constexpr (QUANT) {
+                sum[e & 3] = fmaf(a, sc[32 * c + e].z, sum[e & 3]);
+                sum[(e + 1) & 3] = fmaf(b, sc[32 * c + e + 1].z, sum[(e + 1) & 3]);
+              } else {
+                sum[e & 3] += a;
+                sum[(e + 1) & 3] += b;
+              }
+              p[e / 2] = pack16<T>(a, b);
             }
-            p[e / 2] = pack16<T>(a, b);
+            tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st16(tw + Lay::p_col + s * (kKeys / 2) + half * (kHalf / 2), p);
           tmem_wait_st();
           tc_fence_before();
+        } else {
+          if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_full[s]);
       }
       if (!ok) break;
       // the last product of the piece
-      const uint32_t gl = g - 1;
+      const uint32_t gl = g0 + (stop - first) - 1;
       if (!wait(&bar.o_done[gl & 1], (gl >> 1) & 1)) break;
       tc_fence_after();
       if (warp_live) {
         const bool whole = first == 0 && stop == w.units;
-        float other;
-        if (!exchange(l, &other)) break;
-        l += other;
+        // the two groups' sums, relative to the later maximum
+        sh_swap[half * kM + r] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.swap[pair]);
+        if (!wait(&bar.swap[pair], swaps++ & 1)) break;
+        const float2 other = sh_swap[(half ^ 1) * kM + r];
+        const float top = fmaxf(m, other.x);
+        const auto to_top = [&](float mm, float ll) { return mm == top || mm == -INFINITY ? ll : ll * exp2_approx(mm - top); };
+        l = to_top(m, l) + to_top(other.x, other.y);
+        m = top;
         if (w.r.over) l = __int_as_float(0x7fc00000);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         T* out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
@@ -605,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       if (!wait(&bar.v_full[s], (u >> 1) & 1) || !wait(&bar.p_full[s], (u >> 1) & 1)) return false;
       fence_async_shared();
       tc_fence_after();
-      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::p_col + s * (kKeys / 2), mn_desc(base + Lay::off_v + s * Lay::kTile, Lay::kKSlab),
+      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_desc(base + Lay::off_v + s * Lay::kTile, Lay::kKSlab), 128,
                    idesc_o, !fresh);
       tc_commit_warp(&bar.o_done[s]);
       return true;
@@ -614,13 +626,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       const int count = w.stop() - w.first;
       for (int i = 0; i < count; ++i, ++g) {
         const int s = g & 1;
+        if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
         if (!(ok = wait(&bar.k_full[s], (g >> 1) & 1))) break;
         fence_async_shared();                                  // the copies are the generic proxy's
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 64; ++k)
-          mma_ss4_warp(tmem + Lay::s_col + s * kKeys, sw128_desc(base + Lay::off_q + k * Lay::kQSlab),
-                       sw128_desc(base + Lay::off_k + s * Lay::kTile + k * Lay::kKSlab), idesc_s, k > 0);
+          mma_ts4_warp(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + k * 32,
+                       sw128_desc(base + Lay::off_k + s * Lay::kTile + k * Lay::kKSlab), 2, idesc_s, k > 0);
         tc_commit_warp(&bar.s_done[s]);
         if (i > 0) {
           // the piece's first product overwrites O: the last piece's must have been read
@@ -660,8 +673,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
         cp_async16(base + Lay::off_q + (qc >> 3) * Lay::kQSlab + r * 128 + (((qc & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
       }
     };
-    uint32_t g = 0;                                            // units so far
+    uint32_t g = 0, pieces = 0;                                // units and pieces so far
     bool ok = true;
+    const auto stage_q = [&](const Walk& w) {                  // once the last piece's Q has moved on
+      if (pieces > 0 && !wait(&bar.q_ready, (pieces - 1) & 1)) return false;
+      load_q(w);
+      cp_async_arrive(&bar.q_full);
+      ++pieces;
+      return true;
+    };
     // The stages come free in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)), and
     // that is the order they are filled in.
     if constexpr (!QUANT) {
@@ -692,10 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
         for (int i = w.first; i < stop; ++i, ++g) {
           const int s = g & 1;
           if (g >= 2 && !(ok = wait(&bar.s_done[s], ((g >> 1) + 1) & 1))) break;
-          if (i == w.first) {                                  // the piece's Q rides with its first K,
-            if (g > 0 && !(ok = wait(&bar.s_done[s ^ 1], ((g - 1) >> 1) & 1))) break;   // when the last one's is done with
-            load_q(w);
-          }
+          if (i == w.first && !(ok = stage_q(w))) break;
           fill(A.c.k, Lay::off_k + s * Lay::kTile, off, &bar.k_full[s], true);
           if (g > 0) {
             if (g >= 3 && !(ok = wait(&bar.o_done[s ^ 1], (((g - 1) >> 1) + 1) & 1))) break;
@@ -781,11 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
           }
-          if (i == w.first) {
-            if (g > 0 && !(ok = wait(&bar.s_done[s ^ 1], ((g - 1) >> 1) & 1))) break;
-            load_q(w);
-            asm volatile("cp.async.wait_all;" ::: "memory");
-          }
+          if (i == w.first && !(ok = stage_q(w))) break;
           fence_async_shared();
           mbar_arrive(&bar.k_full[s]);
           if (g >= 2 && !(ok = wait(&bar.o_done[s], ((g >> 1) + 1) & 1))) break;
