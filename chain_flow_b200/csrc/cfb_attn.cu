@@ -9,9 +9,13 @@
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
 // so the weights stay at most 1, whatever the scales, and the codes enter the products exactly.
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp8.h>
+#include <algorithm>
 #include <cstdlib>
+#include <numeric>
 #include <type_traits>
 
 #include "cfb_types.cuh"
@@ -30,13 +34,19 @@ namespace {
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
 constexpr int kM = 128, kKeys = 64;
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + 1 + kLoadWarps) * 32;
-constexpr int kMmaWarp = kSoftWarps;
-constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4, kLoadThreads = kLoadWarps * 32;
 constexpr int kScaleStages = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum has grown by 2^8
+
+// How the cache's rows come in: 16-bit or e4m3, by TMA where boxes of 8 rows or more tile both the pages
+// and the units (gcd(page size, 64) >= 8), else row by row.
+enum Source : int { TMA16 = 0, ROWS16 = 1, TMA8 = 2, ROWS8 = 3 };
+__host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
+__host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
+// warps 0-7 softmax, 8 products, then: TMA16 one that issues the copies; ROWS16 four that copy; TMA8 four
+// that widen and one that issues the copies; ROWS8 four that copy and widen
+constexpr int threads_of(int src) { return (kSoftWarps + 1 + (src == TMA16 ? 1 : src == TMA8 ? kLoadWarps + 1 : kLoadWarps)) * 32; }
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -48,6 +58,7 @@ struct AttnArgs {
   float* lse;
   float scale;
   int T, B, H, causal, rep;
+  int box;                                // rows of a TMA box
   struct Desc* desc;                      // [grid]
   float* part;                            // [grid][2][kM][dim + 4]
 };
@@ -129,32 +140,42 @@ struct Walk {
 };
 
 // ---- shared and tensor memory ------------------------------------------------------------------------
-// Q, K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed
-// with row & 7. K is read K-major (the head dim is summed over), V MN-major (the positions are), from
-// the same image. Q moves on to tensor memory: as the first operand of S = Q K^T it would be read from
+// K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed with
+// row & 7. K is read K-major (the head dim is summed over), V MN-major (the positions are), from the
+// same image. Q lies in tensor memory: as the first operand of S = Q K^T it would be read from
 // shared memory again with every unit, and a 128 x 64 product of 16 reads 4 KB of it in its 32 cycles,
 // the whole shared-memory bandwidth. Tensor memory columns: two units' S (fp32), each overwritten by
 // its P (16-bit), then Q, then O.
 template <int D> constexpr int kPart = D + 4;   // floats of a row's partial result: o, m, l (rows 16-byte aligned)
-template <int D>
+template <int D, int SRC>
 struct Layout {
-  static constexpr uint32_t kQ = kM * D * 2, kTile = kKeys * D * 2;
-  static constexpr uint32_t kQSlab = kM * 128, kKSlab = kKeys * 128;
-  static constexpr uint32_t off_q = 0, off_k = kQ, off_v = kQ + 2 * kTile, off_scale = kQ + 4 * kTile;
-  static constexpr uint32_t bytes = off_scale + kScaleStages * kKeys * 16 + 1024;
+  // stages of K and of V; an e4m3 unit's codes land in stages of their own
+  static constexpr int kStages = SRC == TMA16 ? (D == 256 ? 3 : 4) : 2, kRaw = SRC == TMA8 ? (D == 256 ? 4 : 8) : 0;
+  static constexpr uint32_t kTile = kKeys * D * 2, kSlab = kKeys * 128, kRawTile = kKeys * D;
+  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_raw = 2 * kStages * kTile;
+  static constexpr uint32_t off_scale = off_raw + kRaw * kRawTile;
+  static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kKeys * 16 : 0) + 1024;
   static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
 
-// full: a tile has landed. q_ready: Q is in tensor memory (and its staging free). s_done / o_done: the
-// product S(i) / O += P(i) V(i) has completed, so S may be read and K's stage refilled / O is up to
-// date and V's stage free. p_full: P(i) is written (and S(i) read). m_set: the rows' maximum after unit
-// i is in shared memory. o_free: the piece's O has been read.
+// full / empty: a stage's tile has landed / its product has read it. q_ready: Q is in tensor memory.
+// s_done / o_done: the product S(i) / O += P(i) V(i) has completed. p_full: P(i) is written (and S(i)
+// read). m_set: the rows' maximum after unit i is in shared memory. o_free: the piece's O has been read.
 struct Bars {
-  uint64_t q_full, q_ready, k_full[2], v_full[2], s_done[2], p_full[2], o_done[2], o_free, sc_full[kScaleStages],
-      m_set[2][4], swap[4], drain;
+  uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], s_done[2], p_full[2], o_done[2], o_free,
+      sc_full[kScaleStages], raw_full[8], raw_empty[8], m_set[2][4], swap[4], drain;
 };
 
+CFB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+CFB_DEV void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t r[32];
   asm volatile(
@@ -265,19 +286,21 @@ template <> CFB_DEV uint4 widen8<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------
-// One CTA per SM, 13 warps. Warps 9-12 load: per piece the Q tile, per unit a K and a V tile (two
-// stages each) with 16-byte copies, rows found through the page table, positions past the end filled
-// with zeros; e4m3 rows come through registers, where they are widened. Warp 8 issues the tensor
-// work: S(i) = Q K(i)^T into one of two fp32 tiles in tensor memory, then O += P(i-1) V(i-1) with P
-// read from tensor memory, so the softmax of a unit runs beside the next unit's product. Warps 0-7
-// are the softmax, a thread a row, units alternating between two groups: the row's 64 scores come from
-// tensor memory, and the weights go back there in the operands' type (the one rounding of the
-// weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of the unrounded fp32 values). O is
-// rescaled only when the row's maximum has grown by more than 2^8 since the last time: weights are
-// then at most 2^8, far inside both types, and most units touch O not at all.
-template <typename T, bool QUANT, int D>
-__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
-  using Lay = Layout<D>;
+// One CTA per SM. The loading warps (Source) fill, per unit, a K and a V tile: pages are found through
+// the page table a unit early, positions past the end are zeros where it matters (V), and e4m3 codes
+// are widened on the way. Warp 8 issues the tensor work: S(i) = Q K(i)^T into one of two fp32 tiles in
+// tensor memory, then O += P(i-1) V(i-1) with P read from tensor memory, so the softmax of a unit runs
+// beside the next unit's product. Warps 0-7 are the softmax, a thread a row, units alternating between
+// two groups: the row's 64 scores come from tensor memory, and the weights go back there in the
+// operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of
+// the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^8 since
+// the last time: weights are then at most 2^8, far inside both types, and most units touch O not at all.
+template <typename T, int D, int SRC>
+__global__ void __launch_bounds__(threads_of(SRC), 1)
+attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using Lay = Layout<D, SRC>;
+  constexpr bool QUANT = is_e4m3(SRC);
+  constexpr int kSt = Lay::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
@@ -290,10 +313,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
   const int grid = gridDim.x, cta = blockIdx.x;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bar.q_full, kLoadThreads);
     mbar_init(&bar.q_ready, kSoftWarps);
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(&bar.k_full[i], SRC == TMA16 ? 1 : kLoadThreads); mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_full[i], SRC == TMA16 ? 1 : kLoadThreads); mbar_init(&bar.v_empty[i], 1);
+    }
+    for (int i = 0; i < Lay::kRaw; ++i) { mbar_init(&bar.raw_full[i], 1); mbar_init(&bar.raw_empty[i], kLoadWarps); }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], kLoadThreads); mbar_init(&bar.v_full[i], kLoadThreads);
       mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps / 2); mbar_init(&bar.o_done[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&bar.m_set[i][j], 1);
     }
@@ -375,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
     const int r = pair * 32 + lane;
     const float c2 = A.scale * kLog2e;
-    uint32_t g0 = 0, pieces = 0, swaps = 0;                    // units and pieces before this one; exchanges of sums
-    for (; !w.done(); g0 += w.stop() - w.first, w.next(A), ++pieces) {
+    uint32_t g0 = 0, swaps = 0;                                // units before this piece; exchanges of sums
+    for (; !w.done(); g0 += w.stop() - w.first, w.next(A)) {
       const int stop = w.stop(), first = w.first;
       const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
       const bool valid = r < rows;
@@ -384,23 +410,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
       const int lim = valid ? row_limit(A, w.r, tok) : 0;
       const bool warp_live = pair * 32 < rows;
       bool ok = true;
-      // Q from its staging to tensor memory, a half of the head dim a group
-      if (!wait(&bar.q_full, pieces & 1)) break;
+      // Q to tensor memory, a half of the head dim a group
       if (warp_live) {
-        tc_fence_after();
+        constexpr int kCols = D == 64 ? 16 : 32, kPieces = kCols / 4, kRounds = D == 256 ? 2 : 1;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (long long)(w.r.t0 + (valid ? tok : 0)) * A.sq_t +
+                                                          (valid ? head : 0) * A.sq_h + half * (D / 2));
+        uint32_t u[kRounds][kCols];
 #pragma unroll
-        for (int c = 0; c < (D == 64 ? 1 : D / 128); ++c) {
-          constexpr int kCols = D == 64 ? 16 : 32, kPieces = kCols / 4;
-          const int piece0 = half * (D / 16) + c * 8;          // 16-byte pieces of the row
-          uint32_t u[kCols];
+        for (int e = 0; e < kRounds * kPieces; ++e) {
+          const uint4 y = valid ? __ldg(src + e) : make_uint4(0, 0, 0, 0);
+          uint32_t* z = u[e / kPieces] + 4 * (e % kPieces);
+          z[0] = y.x; z[1] = y.y; z[2] = y.z; z[3] = y.w;
+        }
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < kPieces; ++e) {
-            const int pc = piece0 + e;
-            const uint4 y = *reinterpret_cast<const uint4*>(sm + Lay::off_q + (pc >> 3) * Lay::kQSlab + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
-            u[4 * e] = y.x; u[4 * e + 1] = y.y; u[4 * e + 2] = y.z; u[4 * e + 3] = y.w;
-          }
-          if constexpr (kCols == 32) tmem_st32(tw + Lay::q_col + piece0 * 4, u);
-          else tmem_st16(tw + Lay::q_col + piece0 * 4, u);
+        for (int c = 0; c < kRounds; ++c) {
+          if constexpr (kCols == 32) tmem_st32(tw + Lay::q_col + half * (D / 4) + c * 32, u[c]);
+          else tmem_st16(tw + Lay::q_col + half * (D / 4), u[c]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -612,206 +638,272 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const AttnArgs A) {
     constexpr uint32_t idesc_o = tc_idesc(kM, D) | type_bits<T>() | (1u << 16);      // B is MN-major
     uint32_t g = 0, pieces = 0;
     bool ok = true;
-    const auto pv = [&](uint32_t u, bool fresh) {              // O (+)= P(u) V(u)
-      const int s = u & 1;
-      if (!wait(&bar.v_full[s], (u >> 1) & 1) || !wait(&bar.p_full[s], (u >> 1) & 1)) return false;
-      fence_async_shared();
+    const auto pv = [&](uint32_t u, int i, bool fresh) {       // O (+)= P(u) V(u), u the piece's unit i
+      const int s = u & 1, st = u % kSt;
+      if (!wait(&bar.v_full[st], (u / kSt) & 1)) return false;
+      const uint32_t v = base + Lay::off_v + st * Lay::kTile;
+      if constexpr (SRC == TMA16) {
+        // rows past the end hold what the pages or the last tile left there: 0 x NaN must not happen
+        const int rows = row_limit(A, w.r, w.r.n - 1) - i * kKeys;
+        if (rows < kKeys) {
+          for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) st_shared16(v + c * Lay::kSlab + x * 16, 0, 0, 0, 0);
+          fence_async_shared();
+          __syncwarp();
+        }
+      }
+      if (!wait(&bar.p_full[s], (u >> 1) & 1)) return false;
+      if constexpr (SRC != TMA16) fence_async_shared();        // the tile was stored by threads
       tc_fence_after();
-      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_desc(base + Lay::off_v + s * Lay::kTile, Lay::kKSlab), 128,
-                   idesc_o, !fresh);
+      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_desc(v, Lay::kSlab), 128, idesc_o, !fresh);
+      tc_commit_warp(&bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
       return true;
     };
     for (; ok && !w.done(); w.next(A), ++pieces) {
       const int count = w.stop() - w.first;
       for (int i = 0; i < count; ++i, ++g) {
-        const int s = g & 1;
+        const int s = g & 1, st = g % kSt;
         if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
-        if (!(ok = wait(&bar.k_full[s], (g >> 1) & 1))) break;
-        fence_async_shared();                                  // the copies are the generic proxy's
+        if (!(ok = wait(&bar.k_full[st], (g / kSt) & 1))) break;
+        if constexpr (SRC != TMA16) fence_async_shared();
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 64; ++k)
           mma_ts4_warp(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + k * 32,
-                       sw128_desc(base + Lay::off_k + s * Lay::kTile + k * Lay::kKSlab), 2, idesc_s, k > 0);
+                       sw128_desc(base + Lay::off_k + st * Lay::kTile + k * Lay::kSlab), 2, idesc_s, k > 0);
         tc_commit_warp(&bar.s_done[s]);
+        tc_commit_warp(&bar.k_empty[st]);
         if (i > 0) {
           // the piece's first product overwrites O: the last piece's must have been read
           if (i == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
-          if (!(ok = pv(g - 1, i == 1))) break;
+          if (!(ok = pv(g - 1, w.first + i - 1, i == 1))) break;
         }
       }
       if (!ok) break;
       if (count == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
-      ok = pv(g - 1, count == 1);
+      ok = pv(g - 1, w.first + count - 1, count == 1);
     }
     tc_commit_warp(&bar.drain);                                // everything issued has completed
     mbar_wait(&bar.drain, 0);
   } else {
     // ---------------------------------------------------------------- loads
     const int lt = threadIdx.x - (kMmaWarp + 1) * 32, lw = lt >> 5;
-    constexpr int kElem = QUANT ? 1 : 2;                       // stored bytes an element
-    constexpr int kLanesRow = D * kElem / 16;                  // lanes a row of 16-byte pieces
-    constexpr int kRowsPass = 32 / kLanesRow;                  // rows a warp's access covers
-    constexpr int kPasses = kKeys / (kLoadWarps * kRowsPass);
-    static_assert(kPasses >= 1, "a tile has a pass for every warp");
-    const int sub = lane / kLanesRow, piece = lane % kLanesRow;
-    // lane x of a warp (x < kPasses * kRowsPass) finds the row of position x % kRowsPass + ... of its warp
-    constexpr int kOwn = kPasses * kRowsPass;                  // positions a warp loads of a unit
-    static_assert(kOwn <= 32, "a lane a position");
-    const auto position = [&](int x) { return (x / kRowsPass) * (kLoadWarps * kRowsPass) + lw * kRowsPass + x % kRowsPass; };
-    const auto load_q = [&](const Walk& w) {
-      constexpr int kLanesQ = D / 8, kRowsQ = 32 / kLanesQ;
-      const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
-      const int qs = lane / kLanesQ, qc = lane % kLanesQ;
-#pragma unroll 4
-      for (int x = 0; x < kM / (kLoadWarps * kRowsQ); ++x) {
-        const int r = x * (kLoadWarps * kRowsQ) + lw * kRowsQ + qs;
-        const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
-        const bool in = r < rows;
-        const T* src = static_cast<const T*>(A.q) + (in ? (long long)(w.r.t0 + tok) * A.sq_t + head * A.sq_h + qc * 8 : 0);
-        cp_async16(base + Lay::off_q + (qc >> 3) * Lay::kQSlab + r * 128 + (((qc & 7) ^ (r & 7)) << 4), src, in ? 16 : 0);
-      }
-    };
-    uint32_t g = 0, pieces = 0;                                // units and pieces so far
+    uint32_t g = 0;                                            // units so far
     bool ok = true;
-    const auto stage_q = [&](const Walk& w) {                  // once the last piece's Q has moved on
-      if (pieces > 0 && !wait(&bar.q_ready, (pieces - 1) & 1)) return false;
-      load_q(w);
-      cp_async_arrive(&bar.q_full);
-      ++pieces;
-      return true;
-    };
-    // The stages come free in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)), and
-    // that is the order they are filled in.
-    if constexpr (!QUANT) {
-      // A thread's copies arrive on the stage's barrier by themselves when they land, so the loads run as
-      // far ahead as the stages allow. The next unit's page is looked up a unit early.
-      const auto find = [&](const Walk& w, int i) {
-        const int j = i * kKeys + position(lane % kOwn);
-        return j < row_limit(A, w.r, w.r.n - 1) ? row_offset(A, w.b, w.kh, j, nullptr) : -2ll;
-      };
-      const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
-        const uint32_t dst = base + tile + (piece >> 3) * Lay::kKSlab;
-        const T* src = static_cast<const T*>(pool);
-#pragma unroll
-        for (int x = 0; x < kPasses; ++x) {
-          const int r = position(x * kRowsPass + sub);
-          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-          const uint32_t at = dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-          // -1: no such page, its scores are NaN; -2: past the end, zeros
-          const bool nan_row = key && o == -1;
-          cp_async16(at, o >= 0 ? static_cast<const void*>(src + o + piece * 8) : static_cast<const void*>(kNanRow),
-                     o >= 0 || nan_row ? 16 : 0);
+    const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
+    const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
+    if (is_tma(SRC) && lw == (SRC == TMA16 ? 0 : kLoadWarps)) {
+      // -------- the warp that issues TMA copies: a lane a box of A.box rows (and, for 16-bit rows, of 64
+      // columns), whose page it looks up
+      constexpr int kCols = SRC == TMA16 ? D / 64 : 1;         // boxes side by side
+      const int box = A.box, bx = lane / kCols, col = lane % kCols;
+      const bool mine = lane < (kKeys / box) * kCols;
+      const uint32_t bytes = box * (SRC == TMA16 ? 128 : D);
+      int page = -1, off = 0;
+      bool need = false;
+      const auto look = [&](const Walk& w, int i) {
+        const int j = i * kKeys + bx * box;
+        need = mine && j < row_limit(A, w.r, w.r.n - 1);
+        page = -1;
+        if (need) {
+          const int p = (unsigned)j / (unsigned)A.c.page_size;
+          off = j - p * A.c.page_size;
+          page = __ldg(A.table + (long long)w.b * A.st + p);
+          if (page >= A.c.pages) page = -1;
         }
-        cp_async_arrive(full);
       };
-      long long off = w.done() ? -2 : find(w, w.first), v_off = -2;
-      while (ok && !w.done()) {
-        const int stop = w.stop();
-        for (int i = w.first; i < stop; ++i, ++g) {
-          const int s = g & 1;
-          if (g >= 2 && !(ok = wait(&bar.s_done[s], ((g >> 1) + 1) & 1))) break;
-          if (i == w.first && !(ok = stage_q(w))) break;
-          fill(A.c.k, Lay::off_k + s * Lay::kTile, off, &bar.k_full[s], true);
-          if (g > 0) {
-            if (g >= 3 && !(ok = wait(&bar.o_done[s ^ 1], (((g - 1) >> 1) + 1) & 1))) break;
-            fill(A.c.v, Lay::off_v + (s ^ 1) * Lay::kTile, v_off, &bar.v_full[s ^ 1], false);
+      const auto issue = [&](const CUtensorMap* map, uint32_t stage, uint64_t* full, int kh, bool key) {
+        const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
+        if constexpr (SRC == TMA16) {
+          const uint32_t dst = base + stage + col * Lay::kSlab + bx * box * 128;
+          const bool lost = need && page < 0;                  // no such page: its scores are NaN
+          if (lost) {
+            const uint32_t fill = key ? 0x7fff7fffu : 0u;
+            for (int x = 0; x < box * 8; ++x) st_shared16(dst + x * 16, fill, fill, fill, fill);
+            fence_async_shared();
           }
-          v_off = off;
-          if (i + 1 < stop) off = find(w, i + 1);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
+          __syncwarp();
+          if (need && page >= 0) tma_load_4d(dst, map, col * 64, off, kh, page, full);
+        } else {
+          if (need && page < 0)                                // no such page (its scales are NaN)
+            for (uint32_t x = 0; x < bytes; x += 16) st_shared16(base + stage + bx * bytes + x, 0, 0, 0, 0);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
+          __syncwarp();
+          if (need && page >= 0) tma_load_4d(base + stage + bx * bytes, map, 0, off, kh, page, full);
+        }
+      };
+      if (!w.done()) look(w, w.first);
+      while (ok && !w.done()) {
+        const int stop = w.stop(), kh = w.kh;
+        for (int i = w.first; i < stop; ++i, ++g) {
+          if constexpr (SRC == TMA16) {
+            if (!(ok = k_free())) break;
+            issue(&k_map, Lay::off_k + (g % kSt) * Lay::kTile, &bar.k_full[g % kSt], kh, true);
+            if (!(ok = v_free(g))) break;
+            issue(&v_map, Lay::off_v + (g % kSt) * Lay::kTile, &bar.v_full[g % kSt], kh, false);
+          } else {
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              const uint32_t u = 2 * g + kv, st = u % Lay::kRaw;
+              if (u >= Lay::kRaw && !(ok = wait(&bar.raw_empty[st], (u / Lay::kRaw - 1) & 1))) break;
+              issue(kv ? &v_map : &k_map, Lay::off_raw + st * Lay::kRawTile, &bar.raw_full[st], kh, kv == 0);
+            }
+            if (!ok) break;
+          }
+          if (i + 1 < stop) look(w, i + 1);
         }
         if (!ok) break;
         w.next(A);
-        if (!w.done()) off = find(w, w.first);
+        if (!w.done()) look(w, w.first);
       }
-      if (ok && g > 0) {
-        const int s = (g - 1) & 1;
-        if (g >= 3) ok = wait(&bar.o_done[s], (((g - 1) >> 1) + 1) & 1);
-        if (ok) fill(A.c.v, Lay::off_v + s * Lay::kTile, v_off, &bar.v_full[s], false);
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-    } else {
-      // A tile's codes go through registers: each is refilled with the next unit's as soon as it is
-      // stored, so one to two tiles are in flight. Pages and scales are looked up a unit before that.
-      uint4 kr[kPasses], vr[kPasses];
-      Walk f = w;                                              // the unit to be looked up next
-      int fi = f.first;
-      long long off = -1;                                      // the looked-up unit's rows (a lane's) and scales
-      float2 sc_next = make_float2(0.f, 1.f), sc = sc_next;
-      const auto look = [&] {
-        off = -1;
-        sc_next = make_float2(0.f, 1.f);
-        if (f.done()) return;
-        const int lim = row_limit(A, f.r, f.r.n - 1), pos = fi * kKeys;
-        const int mine = pos + position(lane % kOwn);
-        if (mine < lim) off = row_offset(A, f.b, f.kh, mine, nullptr);
-        if (lt < kKeys && pos + lt < lim) {                    // a lane a position: its scales
-          long long so = 0;
-          if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0)
-            sc_next = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
-          else sc_next.x = __int_as_float(0x7fc00000);         // no such page: its scores are NaN
-        }
-        if (++fi == f.stop()) {
-          f.next(A);
-          fi = f.first;
-        }
+    } else if constexpr (SRC != TMA16) {
+      // -------- the warps that copy rows, or widen codes, into the tiles
+      constexpr int kElem = QUANT ? 1 : 2;                     // stored bytes an element
+      constexpr int kLanesRow = D * kElem / 16;                // lanes a row of 16-byte pieces
+      constexpr int kRowsPass = 32 / kLanesRow;                // rows a warp's access covers
+      constexpr int kPasses = kKeys / (kLoadWarps * kRowsPass);
+      constexpr int kOwn = kPasses * kRowsPass;                // positions a warp handles of a unit
+      static_assert(kPasses >= 1 && kOwn <= 32, "a lane a position, a pass for every warp");
+      const int sub = lane / kLanesRow, piece = lane % kLanesRow;
+      const auto position = [&](int x) { return (x / kRowsPass) * (kLoadWarps * kRowsPass) + lw * kRowsPass + x % kRowsPass; };
+      const auto find = [&](const Walk& w, int i) {            // the row of this lane's position; -1 no such page, -2 past the end
+        const int j = i * kKeys + position(lane % kOwn);
+        return j < row_limit(A, w.r, w.r.n - 1) ? row_offset(A, w.b, w.kh, j, nullptr) : -2ll;
       };
-      const auto fetch = [&](const void* pool, uint4* regs) {
+      if constexpr (SRC == ROWS16) {
+        // A thread's copies arrive on the stage's barrier by themselves when they land. Stages come free
+        // in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)): they are filled so.
+        const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
+          const uint32_t dst = base + tile + (piece >> 3) * Lay::kSlab;
+          const T* src = static_cast<const T*>(pool);
 #pragma unroll
-        for (int x = 0; x < kPasses; ++x) {
-          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-          regs[x] = make_uint4(0, 0, 0, 0);
-          if (o >= 0) regs[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + o) + piece);
-        }
-      };
-      const auto put = [&](uint32_t tile, const uint4* regs) {
-#pragma unroll
-        for (int x = 0; x < kPasses; ++x) {
-          const int r = position(x * kRowsPass + sub);
-          const uint4 a = widen8<T>(regs[x].x, regs[x].y), b = widen8<T>(regs[x].z, regs[x].w);
-          const int c0 = piece * 2;                            // 16-byte pieces of the widened row
-          const uint32_t row = base + tile + (c0 >> 3) * Lay::kKSlab + r * 128;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + (((c0 & 7) ^ (r & 7)) << 4)), "r"(a.x), "r"(a.y),
-                       "r"(a.z), "r"(a.w) : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4)), "r"(b.x), "r"(b.y),
-                       "r"(b.z), "r"(b.w) : "memory");
-        }
-      };
-      look();
-      fetch(A.c.k, kr);
-      fetch(A.c.v, vr);
-      sc = sc_next;
-      look();
-      for (; ok && !w.done(); w.next(A)) {
-        const int stop = w.stop();
-        for (int i = w.first; i < stop; ++i, ++g) {
-          const int s = g & 1;
-          if (g >= 2 && !(ok = wait(&bar.s_done[s], ((g >> 1) + 1) & 1))) break;
-          put(Lay::off_k + s * Lay::kTile, kr);
-          fetch(A.c.k, kr);
-          if (lt < kKeys) {
-            // a scale of NaN reaches the row through its score; where the row may not see the position,
-            // its weight of 0 meets a finite factor
-            reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
-                make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
+          for (int x = 0; x < kPasses; ++x) {
+            const int r = position(x * kRowsPass + sub);
+            const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+            const bool nan_row = key && o == -1;
+            cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
+                       o >= 0 ? static_cast<const void*>(src + o + piece * 8) : static_cast<const void*>(kNanRow),
+                       o >= 0 || nan_row ? 16 : 0);
           }
-          if (i == w.first && !(ok = stage_q(w))) break;
-          fence_async_shared();
-          mbar_arrive(&bar.k_full[s]);
-          if (g >= 2 && !(ok = wait(&bar.o_done[s], ((g >> 1) + 1) & 1))) break;
-          put(Lay::off_v + s * Lay::kTile, vr);
-          fence_async_shared();
-          mbar_arrive(&bar.v_full[s]);
-          fetch(A.c.v, vr);
-          sc = sc_next;
-          look();
+          cp_async_arrive(full);
+        };
+        long long off = w.done() ? -2 : find(w, w.first), v_off = -2;
+        const auto fill_v = [&](uint32_t u) {
+          if (!v_free(u)) return false;
+          fill(A.c.v, Lay::off_v + (u % kSt) * Lay::kTile, v_off, &bar.v_full[u % kSt], false);
+          return true;
+        };
+        while (ok && !w.done()) {
+          const int stop = w.stop();
+          for (int i = w.first; i < stop; ++i, ++g) {
+            if (!(ok = k_free())) break;
+            fill(A.c.k, Lay::off_k + (g % kSt) * Lay::kTile, off, &bar.k_full[g % kSt], true);
+            if (g > 0 && !(ok = fill_v(g - 1))) break;
+            v_off = off;
+            if (i + 1 < stop) off = find(w, i + 1);
+          }
+          if (!ok) break;
+          w.next(A);
+          if (!w.done()) off = find(w, w.first);
         }
-        if (!ok) break;
+        if (ok && g > 0) fill_v(g - 1);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+        // Codes come from their stages (TMA8) or through registers, each refilled with the next unit's
+        // as soon as it is stored (ROWS8). Scales are looked up a unit early.
+        const auto put = [&](uint32_t tile, int x, const uint4& y) {       // pass x's codes, widened
+          const int r = position(x * kRowsPass + sub);
+          const uint4 a = widen8<T>(y.x, y.y), b = widen8<T>(y.z, y.w);
+          const int c0 = piece * 2;                            // 16-byte pieces of the widened row
+          const uint32_t row = base + tile + (c0 >> 3) * Lay::kSlab + r * 128;
+          st_shared16(row + (((c0 & 7) ^ (r & 7)) << 4), a.x, a.y, a.z, a.w);
+          st_shared16(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4), b.x, b.y, b.z, b.w);
+        };
+        Walk f = w;                                            // the unit to be looked up next
+        int fi = f.first;
+        long long off = -1;
+        float2 sc_next = make_float2(0.f, 1.f);
+        const auto look = [&] {
+          off = -1;
+          sc_next = make_float2(0.f, 1.f);
+          if (f.done()) return;
+          const int lim = row_limit(A, f.r, f.r.n - 1), pos = fi * kKeys;
+          if (SRC == ROWS8) off = find(f, fi);
+          if (lt < kKeys && pos + lt < lim) {                  // a lane a position
+            long long so = 0;
+            if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0)
+              sc_next = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+            else sc_next.x = __int_as_float(0x7fc00000);       // no such page: its scores are NaN
+          }
+          if (++fi == f.stop()) {
+            f.next(A);
+            fi = f.first;
+          }
+        };
+        uint4 kr[SRC == ROWS8 ? kPasses : 1], vr[SRC == ROWS8 ? kPasses : 1];
+        const auto fetch = [&](const void* pool, uint4* regs) {
+#pragma unroll
+          for (int x = 0; x < kPasses; ++x) {
+            const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+            regs[x] = make_uint4(0, 0, 0, 0);
+            if (o >= 0) regs[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + o) + piece);
+          }
+        };
+        // one tile of the unit: wait for its stage, store it widened, announce it
+        const auto tile = [&](uint32_t at, uint64_t* full, uint32_t u, int rows, uint4* regs) {
+          if constexpr (SRC == ROWS8) {
+#pragma unroll
+            for (int x = 0; x < kPasses; ++x) put(at, x, regs[x]);
+          } else {
+            const uint32_t st = u % Lay::kRaw;
+            if (!wait(&bar.raw_full[st], (u / Lay::kRaw) & 1)) return false;
+            const uint8_t* raw = sm + Lay::off_raw + st * Lay::kRawTile;
+#pragma unroll
+            for (int x = 0; x < kPasses; ++x) {
+              const int r = position(x * kRowsPass + sub);
+              uint4 y = reinterpret_cast<const uint4*>(raw)[r * kLanesRow + piece];
+              if (r >= rows) y = make_uint4(0, 0, 0, 0);       // past the end: what the stage held before
+              put(at, x, y);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.raw_empty[st]);
+          }
+          fence_async_shared();
+          mbar_arrive(full);
+          return true;
+        };
+        look();
+        if (SRC == ROWS8) { fetch(A.c.k, kr); fetch(A.c.v, vr); }
+        float2 sc = sc_next;
+        look();
+        for (; ok && !w.done(); w.next(A)) {
+          const int stop = w.stop(), lim = row_limit(A, w.r, w.r.n - 1);
+          for (int i = w.first; i < stop; ++i, ++g) {
+            if (!(ok = k_free())) break;
+            if (lt < kKeys) {
+              // a scale of NaN reaches the row through its score; where the row may not see the position,
+              // its weight of 0 meets a finite factor
+              reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
+                  make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
+            }
+            if (!(ok = tile(Lay::off_k + (g % kSt) * Lay::kTile, &bar.k_full[g % kSt], 2 * g, lim - i * kKeys, kr))) break;
+            if (SRC == ROWS8) fetch(A.c.k, kr);
+            if (!(ok = v_free(g))) break;
+            if (!(ok = tile(Lay::off_v + (g % kSt) * Lay::kTile, &bar.v_full[g % kSt], 2 * g + 1, lim - i * kKeys, vr))) break;
+            if (SRC == ROWS8) fetch(A.c.v, vr);
+            sc = sc_next;
+            look();
+          }
+          if (!ok) break;
+        }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   }
   tc_fence_before();
@@ -903,22 +995,57 @@ int sm_count() {
 }
 size_t desc_bytes(int grid) { return ((size_t)grid * sizeof(Desc) + 255) / 256 * 256; }
 
-template <typename T, bool QUANT, int D>
-cfb_status launch(const AttnArgs& A, int grid, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, QUANT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)Layout<D>::bytes);
-  if (e != cudaSuccess) return cfb_launch_status("attn_kernel attribute");
-  attn_kernel<T, QUANT, D><<<grid, kThreads, Layout<D>::bytes, st>>>(A);
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// The pool as [page][kv head][slot][dim], read in boxes of `rows` slots: 64 columns of 16-bit rows, whole
+// rows of codes. False where a tensor map cannot describe it (rows are then copied one by one).
+bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
+  const bool codes = c.dtype == DT_E4M3;
+  const cuuint64_t size = codes ? 1 : 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * size, (cuuint64_t)c.head_stride * size, (cuuint64_t)c.page_stride * size};
+  const cuuint32_t box[4] = {(cuuint32_t)(codes ? c.dim : 64), (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const auto encode = encoder();
+  return encode && encode(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box,
+                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, int SRC>
+cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
+  if (cudaFuncSetAttribute(attn_kernel<T, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<D, SRC>::bytes) != cudaSuccess)
+    return cfb_launch_status("attn_kernel attribute");
+  attn_kernel<T, D, SRC><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
   if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;
-  const int rows = (int)min((long long)kM, (long long)A.T * A.rep);
+  const int rows = (int)std::min((long long)kM, (long long)A.T * A.rep);
   attn_join_kernel<T, D><<<dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, st>>>(A);
   return cfb_launch_status("attn_join_kernel");
 }
-template <typename T, bool QUANT>
-cfb_status launch_dim(const AttnArgs& A, int grid, cudaStream_t st) {
-  if (A.c.dim == 64) return launch<T, QUANT, 64>(A, grid, st);
-  if (A.c.dim == 128) return launch<T, QUANT, 128>(A, grid, st);
-  return launch<T, QUANT, 256>(A, grid, st);
+template <typename T, int D>
+cfb_status launch_source(const AttnArgs& A, int src, const CUtensorMap* maps, int grid, cudaStream_t st) {
+  switch (src) {
+    case TMA16: return launch<T, D, TMA16>(A, maps, grid, st);
+    case ROWS16: return launch<T, D, ROWS16>(A, maps, grid, st);
+    case TMA8: return launch<T, D, TMA8>(A, maps, grid, st);
+    default: return launch<T, D, ROWS8>(A, maps, grid, st);
+  }
+}
+template <typename T>
+cfb_status launch_dim(const AttnArgs& A, int src, const CUtensorMap* maps, int grid, cudaStream_t st) {
+  if (A.c.dim == 64) return launch_source<T, 64>(A, src, maps, grid, st);
+  if (A.c.dim == 128) return launch_source<T, 128>(A, src, maps, grid, st);
+  return launch_source<T, 256>(A, src, maps, grid, st);
 }
 
 }  // namespace
@@ -959,11 +1086,13 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_paged_attn_workspace(H, c->kv_heads, c->dim))
     return CFB_ERR_WORKSPACE;
   const int grid = sm_count();
-  const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-                   T, B, H, causal, H / c->kv_heads, static_cast<Desc*>(ws),
-                   reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
+  AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
+             T, B, H, causal, H / c->kv_heads, std::gcd(c->page_size, kKeys), static_cast<Desc*>(ws),
+             reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
+  CUtensorMap maps[2] = {};
+  const bool tma = A.box >= 8 && pool_map(&maps[0], *c, c->k, A.box) && pool_map(&maps[1], *c, c->v, A.box);
+  const int src = c->dtype == DT_E4M3 ? (tma ? TMA8 : ROWS8) : (tma ? TMA16 : ROWS16);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool quant = c->dtype == DT_E4M3;
-  if (dtype == DT_F16) return quant ? launch_dim<__half, true>(A, grid, st) : launch_dim<__half, false>(A, grid, st);
-  return quant ? launch_dim<__nv_bfloat16, true>(A, grid, st) : launch_dim<__nv_bfloat16, false>(A, grid, st);
+  if (dtype == DT_F16) return launch_dim<__half>(A, src, maps, grid, st);
+  return launch_dim<__nv_bfloat16>(A, src, maps, grid, st);
 }
