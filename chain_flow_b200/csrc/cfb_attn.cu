@@ -36,6 +36,7 @@ namespace {
 constexpr int kM = 128, kKeys = 64;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4, kLoadThreads = kLoadWarps * 32;
 constexpr int kScaleStages = 4;
+constexpr uint32_t kScaleBytes = kKeys * 12;   // a unit's scales: [64] (k's with the softmax's, log2 v's), [64] 1 / v's
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum has grown by 2^8
 
@@ -44,9 +45,9 @@ constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum
 enum Source : int { TMA16 = 0, ROWS16 = 1, TMA8 = 2, ROWS8 = 3 };
 __host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
 __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
-// warps 0-7 softmax, 8 products, then: TMA16 one that issues the copies; ROWS16 four that copy; TMA8 four
-// that widen and one that issues the copies; ROWS8 four that copy and widen
-constexpr int threads_of(int src) { return (kSoftWarps + 1 + (src == TMA16 ? 1 : src == TMA8 ? kLoadWarps + 1 : kLoadWarps)) * 32; }
+// warps 0-7 softmax, 8 products, then: TMA16 two that issue the copies of K and of V; ROWS16 four that copy;
+// TMA8 four that widen and two that issue the copies; ROWS8 four that copy and widen
+constexpr int threads_of(int src) { return (kSoftWarps + 1 + (src == TMA16 ? 2 : src == TMA8 ? kLoadWarps + 2 : kLoadWarps)) * 32; }
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -59,6 +60,7 @@ struct AttnArgs {
   float scale;
   int T, B, H, causal, rep;
   int box;                                // rows of a TMA box
+  uint32_t slab, group;                   // bytes between a tile's 64-column slabs and its 8-row groups
   struct Desc* desc;                      // [grid]
   float* part;                            // [grid][2][kM][dim + 4]
 };
@@ -140,8 +142,9 @@ struct Walk {
 };
 
 // ---- shared and tensor memory ------------------------------------------------------------------------
-// K and V tiles are 128-byte-swizzled: [64-column slab][row][128 B], a row's 16-byte pieces XORed with
-// row & 7. K is read K-major (the head dim is summed over), V MN-major (the positions are), from the
+// K and V tiles are 128-byte-swizzled: groups of 8 rows of 64 columns (128 B), a row's 16-byte pieces
+// XORed with row & 7, as [slab of 64 columns][group] or, where the pages are no multiple of a unit,
+// [group][slab], so that one TMA box of 8 rows brings all their columns. K is read K-major (the head dim is summed over), V MN-major (the positions are), from the
 // same image. Q lies in tensor memory: as the first operand of S = Q K^T it would be read from
 // shared memory again with every unit, and a 128 x 64 product of 16 reads 4 KB of it in its 32 cycles,
 // the whole shared-memory bandwidth. Tensor memory columns: two units' S (fp32), each overwritten by
@@ -151,10 +154,10 @@ template <int D, int SRC>
 struct Layout {
   // stages of K and of V; an e4m3 unit's codes land in stages of their own
   static constexpr int kStages = SRC == TMA16 ? (D == 256 ? 3 : 4) : 2, kRaw = SRC == TMA8 ? (D == 256 ? 4 : 8) : 0;
-  static constexpr uint32_t kTile = kKeys * D * 2, kSlab = kKeys * 128, kRawTile = kKeys * D;
+  static constexpr uint32_t kTile = kKeys * D * 2, kRawTile = kKeys * D;
   static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_raw = 2 * kStages * kTile;
   static constexpr uint32_t off_scale = off_raw + kRaw * kRawTile;
-  static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kKeys * 16 : 0) + 1024;
+  static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kScaleBytes : 0) + 1024;
   static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
@@ -171,6 +174,12 @@ CFB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+CFB_DEV void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int u, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u), "r"(smem_u32(bar))
       : "memory");
 }
 CFB_DEV void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -224,9 +233,14 @@ CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t
          "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step)
       : "memory");
 }
-// MN-major 128-byte-swizzled operand: 64-element slabs `slab` bytes apart, 8-row groups 1024 bytes apart
-CFB_DEV uint64_t mn_desc(uint32_t saddr, uint32_t slab) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// 128-byte-swizzled operands: K-major, 8-row groups `group` bytes apart; MN-major, 64-element slabs `slab`
+// and 8-row groups `group` bytes apart
+CFB_DEV uint64_t k_major(uint32_t saddr, uint32_t group) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+CFB_DEV uint64_t mn_major(uint32_t saddr, uint32_t slab, uint32_t group) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
 }
 template <typename T>
 CFB_DEV constexpr uint32_t type_bits() {          // operand formats of the instruction descriptor
@@ -445,18 +459,20 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           float x[kKeys];
           tmem_ld32(tw + Lay::s_col + s * kKeys, x);
           tmem_ld32(tw + Lay::s_col + s * kKeys + 32, x + 32);
-          const float4* sc = reinterpret_cast<const float4*>(sm + Lay::off_scale) + (g % kScaleStages) * kKeys;
+          const float4* const sc = reinterpret_cast<const float4*>(sm + Lay::off_scale + (g % kScaleStages) * kScaleBytes);
           if (QUANT) ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1);
           tmem_wait_ld();
           if (!ok) break;
           const int j0 = i * kKeys;
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) {
+          for (int e = 0; e < kKeys; e += 2) {
             if constexpr (QUANT) {
-              const float2 f = *reinterpret_cast<const float2*>(sc + e);
+              const float4 f = sc[e / 2];
               x[e] = fmaf(x[e], f.x, f.y);
+              x[e + 1] = fmaf(x[e + 1], f.z, f.w);
             } else {
               x[e] *= c2;
+              x[e + 1] *= c2;
             }
           }
           if (__any_sync(0xffffffffu, lim < j0 + kKeys)) {
@@ -501,16 +517,22 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           for (int c = 0; c < 2; ++c) {
             uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float a = exp2_approx(x[32 * c + e] - mm), b = exp2_approx(x[32 * c + e + 1] - mm);
+            for (int e = 0; e < 32; e += 4) {
+              float y[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
               if constexpr (QUANT) {
-                sum[e & 3] = fmaf(a, sc[32 * c + e].z, sum[e & 3]);
-                sum[(e + 1) & 3] = fmaf(b, sc[32 * c + e + 1].z, sum[(e + 1) & 3]);
+                const float4 f = sc[kKeys / 2 + 8 * c + e / 4];
+                sum[0] = fmaf(y[0], f.x, sum[0]);
+                sum[1] = fmaf(y[1], f.y, sum[1]);
+                sum[2] = fmaf(y[2], f.z, sum[2]);
+                sum[3] = fmaf(y[3], f.w, sum[3]);
               } else {
-                sum[e & 3] += a;
-                sum[(e + 1) & 3] += b;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) sum[z] += y[z];
               }
-              p[e / 2] = pack16<T>(a, b);
+              p[e / 2] = pack16<T>(y[0], y[1]);
+              p[e / 2 + 1] = pack16<T>(y[2], y[3]);
             }
             tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
           }
@@ -648,7 +670,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         if (rows < kKeys) {
           for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) st_shared16(v + c * Lay::kSlab + x * 16, 0, 0, 0, 0);
+            for (int c = 0; c < D / 64; ++c) st_shared16(v + c * A.slab + (x >> 6) * A.group + (x & 63) * 16, 0, 0, 0, 0);
           fence_async_shared();
           __syncwarp();
         }
@@ -656,7 +678,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       if (!wait(&bar.p_full[s], (u >> 1) & 1)) return false;
       if constexpr (SRC != TMA16) fence_async_shared();        // the tile was stored by threads
       tc_fence_after();
-      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_desc(v, Lay::kSlab), 128, idesc_o, !fresh);
+      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major(v, A.slab, A.group), A.group >> 3, idesc_o, !fresh);
       tc_commit_warp(&bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
       return true;
@@ -672,7 +694,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
 #pragma unroll
         for (int k = 0; k < D / 64; ++k)
           mma_ts4_warp(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + k * 32,
-                       sw128_desc(base + Lay::off_k + st * Lay::kTile + k * Lay::kSlab), 2, idesc_s, k > 0);
+                       k_major(base + Lay::off_k + st * Lay::kTile + k * A.slab, A.group), 2, idesc_s, k > 0);
         tc_commit_warp(&bar.s_done[s]);
         tc_commit_warp(&bar.k_empty[st]);
         if (i > 0) {
@@ -694,18 +716,17 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
     bool ok = true;
     const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
     const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
-    if (is_tma(SRC) && lw == (SRC == TMA16 ? 0 : kLoadWarps)) {
-      // -------- the warp that issues TMA copies: a lane a box of A.box rows (and, for 16-bit rows, of 64
-      // columns), whose page it looks up
-      constexpr int kCols = SRC == TMA16 ? D / 64 : 1;         // boxes side by side
-      const int box = A.box, bx = lane / kCols, col = lane % kCols;
-      const bool mine = lane < (kKeys / box) * kCols;
-      const uint32_t bytes = box * (SRC == TMA16 ? 128 : D);
+    if (is_tma(SRC) && lw >= (SRC == TMA16 ? 0 : kLoadWarps)) {
+      // -------- the two warps that issue TMA copies, of K and of V: a lane a box, whose page it looks up
+      const int kv = lw - (SRC == TMA16 ? 0 : kLoadWarps);
+      const CUtensorMap* const map = kv ? &v_map : &k_map;
+      const int box = A.box;
+      const uint32_t bytes = box * D * (SRC == TMA16 ? 2 : 1);
       int page = -1, off = 0;
       bool need = false;
       const auto look = [&](const Walk& w, int i) {
-        const int j = i * kKeys + bx * box;
-        need = mine && j < row_limit(A, w.r, w.r.n - 1);
+        const int j = i * kKeys + lane * box;
+        need = lane * box < kKeys && j < row_limit(A, w.r, w.r.n - 1);
         page = -1;
         if (need) {
           const int p = (unsigned)j / (unsigned)A.c.page_size;
@@ -714,46 +735,33 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           if (page >= A.c.pages) page = -1;
         }
       };
-      const auto issue = [&](const CUtensorMap* map, uint32_t stage, uint64_t* full, int kh, bool key) {
+      const auto issue = [&](uint32_t stage, uint64_t* full, int kh) {
         const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
-        if constexpr (SRC == TMA16) {
-          const uint32_t dst = base + stage + col * Lay::kSlab + bx * box * 128;
-          const bool lost = need && page < 0;                  // no such page: its scores are NaN
-          if (lost) {
-            const uint32_t fill = key ? 0x7fff7fffu : 0u;
-            for (int x = 0; x < box * 8; ++x) st_shared16(dst + x * 16, fill, fill, fill, fill);
-            fence_async_shared();
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
-          __syncwarp();
-          if (need && page >= 0) tma_load_4d(dst, map, col * 64, off, kh, page, full);
-        } else {
-          if (need && page < 0)                                // no such page (its scales are NaN)
-            for (uint32_t x = 0; x < bytes; x += 16) st_shared16(base + stage + bx * bytes + x, 0, 0, 0, 0);
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
-          __syncwarp();
-          if (need && page >= 0) tma_load_4d(base + stage + bx * bytes, map, 0, off, kh, page, full);
+        const uint32_t dst = base + stage + lane * bytes;
+        if (need && page < 0) {                                // no such page: its scores are NaN
+          const uint32_t fill = SRC == TMA16 && kv == 0 ? 0x7fff7fffu : 0u;
+          for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
+          if (SRC == TMA16) fence_async_shared();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
+        __syncwarp();
+        if (need && page >= 0) {
+          if constexpr (SRC == TMA16) tma_load_5d(dst, map, 0, off, 0, kh, page, full);
+          else tma_load_4d(dst, map, 0, off, kh, page, full);
         }
       };
       if (!w.done()) look(w, w.first);
       while (ok && !w.done()) {
-        const int stop = w.stop(), kh = w.kh;
+        const int stop = w.stop();
         for (int i = w.first; i < stop; ++i, ++g) {
           if constexpr (SRC == TMA16) {
-            if (!(ok = k_free())) break;
-            issue(&k_map, Lay::off_k + (g % kSt) * Lay::kTile, &bar.k_full[g % kSt], kh, true);
-            if (!(ok = v_free(g))) break;
-            issue(&v_map, Lay::off_v + (g % kSt) * Lay::kTile, &bar.v_full[g % kSt], kh, false);
+            if (!(ok = kv ? v_free(g) : k_free())) break;
+            issue((kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile, kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt], w.kh);
           } else {
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-              const uint32_t u = 2 * g + kv, st = u % Lay::kRaw;
-              if (u >= Lay::kRaw && !(ok = wait(&bar.raw_empty[st], (u / Lay::kRaw - 1) & 1))) break;
-              issue(kv ? &v_map : &k_map, Lay::off_raw + st * Lay::kRawTile, &bar.raw_full[st], kh, kv == 0);
-            }
-            if (!ok) break;
+            const uint32_t u = 2 * g + kv, st = u % Lay::kRaw;
+            if (u >= Lay::kRaw && !(ok = wait(&bar.raw_empty[st], (u / Lay::kRaw - 1) & 1))) break;
+            issue(Lay::off_raw + st * Lay::kRawTile, &bar.raw_full[st], w.kh);
           }
           if (i + 1 < stop) look(w, i + 1);
         }
@@ -779,14 +787,14 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         // A thread's copies arrive on the stage's barrier by themselves when they land. Stages come free
         // in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)): they are filled so.
         const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
-          const uint32_t dst = base + tile + (piece >> 3) * Lay::kSlab;
+          const uint32_t dst = base + tile + (piece >> 3) * A.slab;
           const T* src = static_cast<const T*>(pool);
 #pragma unroll
           for (int x = 0; x < kPasses; ++x) {
             const int r = position(x * kRowsPass + sub);
             const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
             const bool nan_row = key && o == -1;
-            cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
+            cp_async16(dst + (r >> 3) * A.group + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4),
                        o >= 0 ? static_cast<const void*>(src + o + piece * 8) : static_cast<const void*>(kNanRow),
                        o >= 0 || nan_row ? 16 : 0);
           }
@@ -820,7 +828,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           const int r = position(x * kRowsPass + sub);
           const uint4 a = widen8<T>(y.x, y.y), b = widen8<T>(y.z, y.w);
           const int c0 = piece * 2;                            // 16-byte pieces of the widened row
-          const uint32_t row = base + tile + (c0 >> 3) * Lay::kSlab + r * 128;
+          const uint32_t row = base + tile + (c0 >> 3) * A.slab + (r >> 3) * A.group + (r & 7) * 128;
           st_shared16(row + (((c0 & 7) ^ (r & 7)) << 4), a.x, a.y, a.z, a.w);
           st_shared16(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4), b.x, b.y, b.z, b.w);
         };
@@ -863,15 +871,17 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
             const uint32_t st = u % Lay::kRaw;
             if (!wait(&bar.raw_full[st], (u / Lay::kRaw) & 1)) return false;
             const uint8_t* raw = sm + Lay::off_raw + st * Lay::kRawTile;
+            uint4 y[kPasses];
 #pragma unroll
             for (int x = 0; x < kPasses; ++x) {
               const int r = position(x * kRowsPass + sub);
-              uint4 y = reinterpret_cast<const uint4*>(raw)[r * kLanesRow + piece];
-              if (r >= rows) y = make_uint4(0, 0, 0, 0);       // past the end: what the stage held before
-              put(at, x, y);
+              y[x] = reinterpret_cast<const uint4*>(raw)[r * kLanesRow + piece];
+              if (r >= rows) y[x] = make_uint4(0, 0, 0, 0);    // past the end: what the stage held before
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.raw_empty[st]);
+#pragma unroll
+            for (int x = 0; x < kPasses; ++x) put(at, x, y[x]);
           }
           fence_async_shared();
           mbar_arrive(full);
@@ -888,8 +898,9 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
             if (lt < kKeys) {
               // a scale of NaN reaches the row through its score; where the row may not see the position,
               // its weight of 0 meets a finite factor
-              reinterpret_cast<float4*>(sm + Lay::off_scale)[(g % kScaleStages) * kKeys + lt] =
-                  make_float4(sc.x * (A.scale * kLog2e), log2f(sc.y), sc.y > 0.f ? 1.f / sc.y : 1.f, 0.f);
+              uint8_t* const at = sm + Lay::off_scale + (g % kScaleStages) * kScaleBytes;
+              reinterpret_cast<float2*>(at)[lt] = make_float2(sc.x * (A.scale * kLog2e), log2f(sc.y));
+              reinterpret_cast<float*>(at + kKeys * 8)[lt] = sc.y > 0.f ? 1.f / sc.y : 1.f;
               __syncwarp();
               if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
             }
@@ -1008,18 +1019,25 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// The pool as [page][kv head][slot][dim], read in boxes of `rows` slots: 64 columns of 16-bit rows, whole
-// rows of codes. False where a tensor map cannot describe it (rows are then copied one by one).
+// The pool as [page][kv head][slot][dim], read in boxes of `rows` slots: of 16-bit rows all 64-column slabs
+// at once, of codes whole rows. False where a tensor map cannot describe it (rows are then copied one
+// by one).
 bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
-  const bool codes = c.dtype == DT_E4M3;
-  const cuuint64_t size = codes ? 1 : 2;
-  const cuuint64_t dims[4] = {(cuuint64_t)c.dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * size, (cuuint64_t)c.head_stride * size, (cuuint64_t)c.page_stride * size};
-  const cuuint32_t box[4] = {(cuuint32_t)(codes ? c.dim : 64), (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint64_t dim = c.dim, slots = c.page_size, heads = c.kv_heads, pages = c.pages;
+  const cuuint64_t slot = c.slot_stride, head = c.head_stride, page = c.page_stride;
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1}, r = rows;
   const auto encode = encoder();
-  return encode && encode(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box,
-                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  if (!encode) return false;
+  if (c.dtype == DT_E4M3) {
+    const cuuint64_t dims[4] = {dim, slots, heads, pages}, strides[3] = {slot, head, page};
+    const cuuint32_t box[4] = {(cuuint32_t)c.dim, r, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
+  const cuuint64_t dims[5] = {64, slots, dim / 64, heads, pages}, strides[4] = {slot * 2, 128, head * 2, page * 2};
+  const cuuint32_t box[5] = {64, r, (cuuint32_t)(c.dim / 64), 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D, int SRC>
@@ -1086,11 +1104,15 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_paged_attn_workspace(H, c->kv_heads, c->dim))
     return CFB_ERR_WORKSPACE;
   const int grid = sm_count();
-  AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-             T, B, H, causal, H / c->kv_heads, std::gcd(c->page_size, kKeys), static_cast<Desc*>(ws),
-             reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
+  // Boxes: a whole unit where pages hold whole units; else of 8 rows for 16-bit rows (the tile is then
+  // [group][slab]) and as many rows as divide both a page and a unit for codes.
+  const int fit = std::gcd(c->page_size, kKeys), box = c->dtype != DT_E4M3 && fit < kKeys ? std::min(fit, 8) : fit;
+  const bool grouped = c->dtype != DT_E4M3 && box == 8;
+  const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
+                   T, B, H, causal, H / c->kv_heads, box, grouped ? 1024u : kKeys * 128u, grouped ? c->dim / 64 * 1024u : 1024u,
+                   static_cast<Desc*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
   CUtensorMap maps[2] = {};
-  const bool tma = A.box >= 8 && pool_map(&maps[0], *c, c->k, A.box) && pool_map(&maps[1], *c, c->v, A.box);
+  const bool tma = box >= 8 && pool_map(&maps[0], *c, c->k, box) && pool_map(&maps[1], *c, c->v, box);
   const int src = c->dtype == DT_E4M3 ? (tma ? TMA8 : ROWS8) : (tma ? TMA16 : ROWS16);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == DT_F16) return launch_dim<__half>(A, src, maps, grid, st);
