@@ -7,6 +7,7 @@ impossible, or no CUDA device is visible when a kernel is requested, the call ra
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -115,6 +116,10 @@ class GdnArgs(C.Structure):
                 ("H", C.c_int), ("HV", C.c_int), ("K", C.c_int), ("V", C.c_int)]
 
 
+# a cfb_gdn_args from its fields in order: packing takes a third of the time of filling a ctypes structure
+PACK_GDN_ARGS = struct.Struct("@" + "".join(
+    {C.c_void_p: "P", C.c_int: "i", C.c_int64: "q", C.c_float: "f"}[t] for _, t in GdnArgs._fields_) + "0P").pack
+
 _lock = threading.Lock()
 _lib = None
 
@@ -172,10 +177,11 @@ def _declare(lib):
     lib.cfb_paged_attn.argtypes = [vp, i64, i64, C.POINTER(KvCache), vp, i64, i32, vp, vp, vp, i64, i64, vp, C.c_float,
                                    i32, i32, i32, i32, i32, vp, sz, vp]
     lib.cfb_paged_attn_error.argtypes = [vp, C.POINTER(i32)]
-    lib.cfb_gdn_step.argtypes = [C.POINTER(GdnArgs), i32, vp]
+    # cfb_gdn_args as a GdnArgs by reference or as its packed bytes (PACK_GDN_ARGS)
+    lib.cfb_gdn_step.argtypes = [vp, i32, vp]
     lib.cfb_gdn_chunk_workspace.argtypes = [i32, i32, i32]
     lib.cfb_gdn_chunk_workspace.restype = sz
-    lib.cfb_gdn_chunk.argtypes = [C.POINTER(GdnArgs), vp, i32, i32, vp, sz, vp]
+    lib.cfb_gdn_chunk.argtypes = [vp, vp, i32, i32, vp, sz, vp]
     return lib
 
 
@@ -204,10 +210,18 @@ def check(status: int, what: str) -> None:
 
 def stream_ptr(stream=None) -> int:
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # the raw handle: building a torch.cuda.Stream takes as long as a small launch
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def require_cuda(t, name: str) -> None:
     if not t.is_cuda:
         raise CfbError(f"{name} must be a CUDA tensor: the chain_flow_b200 engine has no CPU path")
+
+
+def int32(t):
+    """t as a contiguous int32 tensor (itself if it is one)."""
+    import torch
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()

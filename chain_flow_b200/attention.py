@@ -24,10 +24,23 @@ class PagedAttention:
             raise _lib.CfbError(f"PagedAttention: heads must be a multiple (up to 128) of kv_heads and head_dim one of "
                                 f"{HEAD_DIMS}, got {heads} / {kv_heads} / {head_dim}")
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.heads, self.kv_heads, self.head_dim, self.scale = heads, kv_heads, head_dim, head_dim ** -0.5
         self.ws_bytes = int(self.lib.cfb_paged_attn_workspace(heads, kv_heads, head_dim))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+
+    def _refuse(self, query, cache, page_table, kv_len, cu_q):
+        for t, n in ((query, "query"), (page_table, "page_table"), (kv_len, "kv_len"), (cu_q, "cu_q")):
+            _lib.require_cuda(t, n)
+            if t.device != cache.device:
+                raise _lib.CfbError(f"{n} is on {t.device}, the cache on {cache.device}")
+        if query.dim() != 3 or query.shape[1] != self.heads or query.shape[2] != self.head_dim or query.stride(2) != 1:
+            raise _lib.CfbError(f"query: expected [T, {self.heads}, {self.head_dim}] with a contiguous head dim, got {list(query.shape)}")
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
+            raise _lib.CfbError("PagedAttention: the cache has other kv heads or another head dim")
+        if query.dtype not in _DT or (cache.k_scale is None and query.dtype != cache.dtype):
+            raise _lib.CfbError("PagedAttention: query must be fp16 or bf16, the cache's own dtype unless it is e4m3")
+        raise _lib.CfbError("PagedAttention: page_table [B, width], kv_len [B] and cu_q [B + 1] disagree")
 
     def check(self) -> None:
         """Raises if a device-side wait of the last call expired (its outputs are then invalid). Waits
@@ -51,38 +64,30 @@ class PagedAttention:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self(query, cache, page_table, kv_len, cu_q, scale=scale, causal=causal, out=out, lse=lse)
-        for t, n in ((query, "query"), (page_table, "page_table"), (kv_len, "kv_len"), (cu_q, "cu_q")):
-            _lib.require_cuda(t, n)
-            if t.device != cache.device:
-                raise _lib.CfbError(f"{n} is on {t.device}, the cache on {cache.device}")
-        if query.dim() != 3 or query.shape[1] != self.heads or query.shape[2] != self.head_dim:
-            raise _lib.CfbError(f"query: expected [T, {self.heads}, {self.head_dim}], got {list(query.shape)}")
-        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
-            raise _lib.CfbError("PagedAttention: the cache has other kv heads or another head dim")
-        dt = _DT.get(query.dtype)
-        if dt is None or (cache.k_scale is None and query.dtype != cache.dtype):
-            raise _lib.CfbError("PagedAttention: query must be fp16 or bf16, the cache's own dtype unless it is e4m3")
-        B = kv_len.numel()
-        if page_table.dim() != 2 or page_table.shape[0] != B or kv_len.dim() != 1 or cu_q.dim() != 1 or cu_q.numel() != B + 1:
-            raise _lib.CfbError("PagedAttention: page_table [B, width], kv_len [B] and cu_q [B + 1] disagree")
+        B, shape, dev, dtype = kv_len.shape[0] if kv_len.dim() else -1, query.shape, cache._dev, query.dtype
+        dt, sq = _DT.get(dtype), query.stride()
+        if (len(shape) != 3 or shape[1] != self.heads or shape[2] != self.head_dim or sq[2] != 1 or dt is None
+                or (cache.k_scale is None and dtype != cache.dtype)
+                or cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim
+                or page_table.dim() != 2 or page_table.shape[0] != B or kv_len.dim() != 1 or cu_q.shape != (B + 1,)
+                or any(t.get_device() != dev for t in (query, page_table, kv_len, cu_q))):
+            self._refuse(query, cache, page_table, kv_len, cu_q)
         if page_table.dtype != torch.int32 or page_table.stride(1) != 1:
             page_table = page_table.to(torch.int32).contiguous()
-        kv_len, cu_q = kv_len.to(torch.int32).contiguous(), cu_q.to(torch.int32).contiguous()
-        if query.stride(2) != 1:
-            raise _lib.CfbError("query needs a contiguous head dim")
-        T = query.shape[0]
+        kv_len, cu_q = _lib.int32(kv_len), _lib.int32(cu_q)
+        T = shape[0]
         if out is None:
-            out = torch.empty(T, self.heads, self.head_dim, dtype=query.dtype, device=query.device)
-        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(2) != 1:
+            out = torch.empty(shape, dtype=dtype, device=cache.device)
+        elif out.shape != shape or out.dtype != dtype or out.get_device() != dev or out.stride(2) != 1:
             raise _lib.CfbError("out must have the query's shape, dtype and device, and a contiguous head dim")
         if lse is None:
-            lse = torch.empty(self.heads, T, dtype=torch.float32, device=query.device)
-        elif tuple(lse.shape) != (self.heads, T) or lse.dtype != torch.float32 or lse.device != query.device \
-                or not lse.is_contiguous():
+            lse = torch.empty((self.heads, T), dtype=torch.float32, device=cache.device)
+        elif lse.shape != (self.heads, T) or lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous():
             raise _lib.CfbError(f"lse must be contiguous fp32 [{self.heads}, {T}] on the query's device")
+        so, st = out.stride(), page_table.stride()
         _lib.check(self.lib.cfb_paged_attn(
-            query.data_ptr(), query.stride(0), query.stride(1), cache.desc, page_table.data_ptr(), page_table.stride(0),
-            page_table.shape[1], kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-            lse.data_ptr(), float(self.head_dim ** -0.5 if scale is None else scale), T, B, self.heads, int(causal), dt,
-            self.ws_ptr, self.ws_bytes, _lib.stream_ptr()), "cfb_paged_attn")
+            query.data_ptr(), sq[0], sq[1], cache.desc, page_table.data_ptr(), max(st[0], page_table.shape[1]),
+            page_table.shape[1], kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),
+            self.scale if scale is None else scale, T, B, self.heads, causal, dt, self.ws_ptr, self.ws_bytes,
+            _lib.stream_ptr()), "cfb_paged_attn")
         return out, lse

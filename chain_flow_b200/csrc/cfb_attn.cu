@@ -62,7 +62,7 @@ struct AttnArgs {
   int box;                                // rows of a TMA box
   uint32_t slab, group;                   // bytes between a tile's 64-column slabs and its 8-row groups
   struct Desc* desc;                      // [grid]
-  float* part;                            // [grid][2][kM][dim + 4]
+  float* part;                            // part_row
 };
 
 struct Desc {                             // a piece that begins in this CTA's share and runs past its end
@@ -149,7 +149,13 @@ struct Walk {
 // shared memory again with every unit, and a 128 x 64 product of 16 reads 4 KB of it in its 32 cycles,
 // the whole shared-memory bandwidth. Tensor memory columns: two units' S (fp32), each overwritten by
 // its P (16-bit), then Q, then O.
-template <int D> constexpr int kPart = D + 4;   // floats of a row's partial result: o, m, l (rows 16-byte aligned)
+// The partial results: rows of kPart floats (o, m, l), eight rows of a CTA side by side and then the CTAs,
+// so that the few rows of a decode step lie together however many CTAs share them.
+template <int D> constexpr int kPart = D + 4;
+template <int D>
+CFB_DEV float* part_row(float* part, int grid, int cta, int which, int row) {
+  return part + ((((long long)(row >> 3) * 2 + which) * grid + cta) * 8 + (row & 7)) * kPart<D>;
+}
 template <int D, int SRC>
 struct Layout {
   // stages of K and of V; an e4m3 unit's codes land in stages of their own
@@ -347,6 +353,10 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
     A.desc[cta].err = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
+  if (is_tma(SRC) && threadIdx.x == blockDim.x - 1) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
+  }
 
   // Where this CTA's share begins: the running sum of the requests' units, by every warp for itself, a
   // lane a request.
@@ -565,7 +575,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         if (w.r.over) l = __int_as_float(0x7fc00000);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         T* out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
-        float* part = A.part + (((long long)cta * 2 + (first == 0)) * kM + r) * kPart<D>;
+        float* const part = part_row<D>(A.part, grid, cta, first == 0, r);
         float bad[4] = {0.f, 0.f, 0.f, 0.f};                   // turn NaN where an element is not finite
 #pragma unroll
         for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
@@ -630,7 +640,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
               for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(vp[e]), acc[e]);
             }
             T* op = static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h + lane * E;
-            float* pp = A.part + (((long long)cta * 2 + (first == 0)) * kM + row) * kPart<D> + lane * E;
+            float* const pp = part_row<D>(A.part, grid, cta, first == 0, row) + lane * E;
             __syncwarp();
             if (lane >> 4 == half) {                           // this warp's half of the row
 #pragma unroll
@@ -928,70 +938,103 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
 
 // ---- the pieces that were cut --------------------------------------------------------------------
 // o = sum_i 2^(m_i - m) o_i / l,  l = sum_i 2^(m_i - m) l_i,  m = max m_i over the parts in unit order.
-// A warp per row of a cut piece; CTA x takes the piece that begins in share x.
-constexpr int kJoinWarps = 8;
+// CTA x takes the piece that begins in share x, WARPS warps a row: 8 where a piece has many parts (few
+// pieces, as in a step of a few decodes), else 1. A warp takes every WARPS-th part, kBatch of them at a
+// time with all their loads in flight together: the kernel is a chain of memory latencies, so it is
+// made short.
+constexpr int kJoinWarps = 8, kBatch = 8;
 
-template <typename T, int D>
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs A) {
-  const int grid = gridDim.x, cta = blockIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");           // launched before the parts are complete
+  const int grid = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Desc d = A.desc[cta];
-  const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + threadIdx.x / 32;
-  if (d.last < 0 || r >= d.rows) return;
+  const int r = blockIdx.y * (kJoinWarps / WARPS) + warp / WARPS;
+  if (d.last < 0 || r >= d.rows) return;                       // (WARPS == 8: the whole CTA alike)
   // the parts: this CTA's second one, then the first one of every later CTA that has a share
   const int last = d.each > 0 ? d.last : min(d.last, d.extra - 1);
-  const auto part_of = [&](int c) { return A.part + (((long long)c * 2 + (c == cta)) * kM + r) * kPart<D>; };
-  float m = -INFINITY;
-  for (int c = cta + lane; c <= last; c += 32) m = fmaxf(m, part_of(c)[D]);
-#pragma unroll
-  for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float mm = m == -INFINITY ? 0.f : m;
   constexpr int E = D / 32, V = E < 4 ? E : 4;                 // elements a lane; of one access
-  float acc[E], l = 0.f;
+  float acc[E], l = 0.f, m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int c0 = cta; c0 <= last; c0 += 32) {
-    float wl = 0.f, ll = 0.f;
-    if (c0 + lane <= last) {
-      const float* p = part_of(c0 + lane);
-      wl = exp2_approx(p[D] - mm);
-      ll = p[D + 1];
-    }
-    const int n = min(32, last + 1 - c0);
-    constexpr int kBatch = 8;                                  // parts whose loads are in flight together
-    for (int i0 = 0; i0 < n; i0 += kBatch) {
-      float x[kBatch][E];
+  const int first = cta + (WARPS > 1 ? warp : 0);
+  for (int c0 = first; c0 <= last; c0 += kBatch * WARPS) {
+    float x[kBatch][E], pm[kBatch], pl[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const float* p = part_of(min(c0 + i0 + i, last)) + lane * V;
+    for (int i = 0; i < kBatch; ++i) {
+      const int c = c0 + i * WARPS;
+      pm[i] = -INFINITY;
+      pl[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+      if (c <= last) {
+        const float* p = part_row<D>(A.part, grid, c, c == cta, r);
+        pm[i] = p[D];
+        pl[i] = p[D + 1];
 #pragma unroll
         for (int e = 0; e < E; e += V) {
           if constexpr (V == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(p + e * 32);
+            const float4 y = *reinterpret_cast<const float4*>(p + lane * V + e * 32);
             x[i][e] = y.x; x[i][e + 1] = y.y; x[i][e + 2] = y.z; x[i][e + 3] = y.w;
           } else {
-            const float2 y = *reinterpret_cast<const float2*>(p + e * 32);
+            const float2 y = *reinterpret_cast<const float2*>(p + lane * V + e * 32);
             x[i][e] = y.x; x[i][e + 1] = y.y;
           }
         }
       }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const float w = __shfl_sync(0xffffffffu, wl, i0 + i);
-        const float lp = __shfl_sync(0xffffffffu, ll, i0 + i);
-        if (i0 + i >= n) break;
-        l = fmaf(w, lp, l);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[i][e], acc[e]);
-      }
     }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, pm[i]);
+    const float mm = top == -INFINITY ? 0.f : top, keep = exp2_approx(m - mm);
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float w = exp2_approx(pm[i] - mm);
+      // a part with nothing in it has m = -inf, and l = 0 or (scores of NaN only) NaN
+      l += pm[i] == -INFINITY ? pl[i] : w * pl[i];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[i][e], acc[e]);
+    }
+    m = top;
+  }
+  if constexpr (WARPS > 1) {
+    __shared__ float sh_acc[WARPS][D], sh_m[WARPS], sh_l[WARPS];
+#pragma unroll
+    for (int e = 0; e < E; e += V)
+#pragma unroll
+      for (int z = 0; z < V; ++z) sh_acc[warp][lane * V + e * 32 + z] = acc[e + z];
+    if (lane == 0) { sh_m[warp] = m; sh_l[warp] = l; }
+    __syncthreads();
+    if (warp > 0) return;
+    float top = sh_m[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) top = fmaxf(top, sh_m[i]);
+    const float mm = top == -INFINITY ? 0.f : top;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      const float w = exp2_approx(sh_m[i] - mm);
+      l += sh_m[i] == -INFINITY ? sh_l[i] : w * sh_l[i];
+#pragma unroll
+      for (int e = 0; e < E; e += V)
+#pragma unroll
+        for (int z = 0; z < V; ++z) acc[e + z] = fmaf(w, sh_acc[i][lane * V + e * 32 + z], acc[e + z]);
+    }
+    m = top;
   }
   const int R = d.row0 + r, tok = R / A.rep, head = d.kh * A.rep + R - tok * A.rep;
   T* out = static_cast<T*>(A.o) + (long long)(d.t0 + tok) * A.so_t + head * A.so_h;
+  const float inv = 1.f / l;
 #pragma unroll
   for (int e = 0; e < E; e += V)
 #pragma unroll
-    for (int x = 0; x < V; x += 2)
-      *reinterpret_cast<uint32_t*>(out + e * 32 + lane * V + x) = l == 0.f ? 0u : pack16<T>(acc[e + x] / l, acc[e + x + 1] / l);
+    for (int z = 0; z < V; z += 2)
+      *reinterpret_cast<uint32_t*>(out + e * 32 + lane * V + z) = l == 0.f ? 0u : pack16<T>(acc[e + z] * inv, acc[e + z + 1] * inv);
   if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -1046,8 +1089,20 @@ cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStre
     return cfb_launch_status("attn_kernel attribute");
   attn_kernel<T, D, SRC><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
   if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;
-  const int rows = (int)std::min((long long)kM, (long long)A.T * A.rep);
-  attn_join_kernel<T, D><<<dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, st>>>(A);
+  const long long rows = std::min((long long)kM, (long long)A.T * A.rep);
+  // pieces: at least a row tile a kv head and request that has tokens; parts of one: the CTAs over those
+  const long long pieces = (long long)A.c.kv_heads * std::max((long long)std::min(A.B, A.T), ((long long)A.T * A.rep + kM - 1) / kM);
+  const bool many = grid > 8 * pieces;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, (unsigned)(many ? rows : (rows + kJoinWarps - 1) / kJoinWarps));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, many ? attn_join_kernel<T, D, kJoinWarps> : attn_join_kernel<T, D, 1>, A);
   return cfb_launch_status("attn_join_kernel");
 }
 template <typename T, int D>

@@ -76,6 +76,7 @@ def tree_gated_delta_scan(query, key, value, g, beta, parent, depth, initial_sta
 
 
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_HALVES = (torch.float16, torch.bfloat16)
 
 
 def ancestor_chains(parent: torch.Tensor, max_depth: int):
@@ -159,12 +160,12 @@ def gdn_factor(A_log, dt_bias, a, b, q, k, v, o, state, chain, depth, init_slot,
         float(scale), H, HV, K, V, _lib.stream_ptr()), "cfb_tree_gdn_factor")
 
 
-def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B):
-    """(cfb_gdn_args, the converted index tensors, which the caller keeps until the launch)."""
-    T = q.shape[0]
-    H, K = q.shape[1], q.shape[2]
+def _refuse_sequence(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, out_state, B):
+    """Raises with what is wrong with the arguments that _sequence_args does not take."""
+    if q.dim() != 3 or v.dim() != 3 or state.dim() != 4:
+        raise _lib.CfbError(f"{what}: q must be [T, H, K], v [T, HV, V] and state [slots, HV, V, K]")
+    T, H, K = q.shape
     HV, V = v.shape[1], v.shape[2]
-    out_state = state if out_state is None else out_state
     for t, n, shape in ((q, "q", (T, H, K)), (k, "k", (T, H, K)), (v, "v", (T, HV, V)), (o, "o", (T, HV, V)),
                         (a, "a", (T, HV)), (b, "b", (T, HV)), (A_log, "A_log", (HV,)), (dt_bias, "dt_bias", (HV,)),
                         (state, "state", (state.shape[0], HV, V, K)), (out_state, "out_state", tuple(state.shape)),
@@ -176,26 +177,47 @@ def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out
             raise _lib.CfbError(f"{what}: {n} must be {list(shape)}, got {list(t.shape)}")
     if q.dtype not in (torch.float16, torch.bfloat16) or any(t.dtype != q.dtype for t in (k, v, o)):
         raise _lib.CfbError(f"{what}: q, k, v, o must share one dtype, fp16 or bf16")
-    for t in (A_log, dt_bias, a, b):
-        if t.dtype not in _DTYPE_CODE:
-            raise _lib.CfbError(f"{what}: a, b, A_log and dt_bias must be fp32, fp16 or bf16")
-    for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
-        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-            raise _lib.CfbError(f"{what}: {n} needs contiguous heads (any token stride)")
-    if HV > 1 and any(t.stride(-1) != 1 for t in (a, b, A_log, dt_bias)):
-        raise _lib.CfbError(f"{what}: a, b, A_log and dt_bias need contiguous heads")
-    for t, n in ((state, "state"), (out_state, "out_state")):
-        if t.dtype != torch.float32 or t.stride(3) != 1 or t.stride(2) != K or (HV > 1 and t.stride(1) != V * K) \
-                or t.stride(0) != state.stride(0):
-            raise _lib.CfbError(f"{what}: {n} must be fp32 [slots, HV, V, K] with contiguous slots (one slot stride)")
-    init, to = (t.to(torch.int32).contiguous() for t in (init_slot, out_slot))
-    args = _lib.GdnArgs(
-        A_log.data_ptr(), _DTYPE_CODE[A_log.dtype], dt_bias.data_ptr(), _DTYPE_CODE[dt_bias.dtype],
-        a.data_ptr(), _DTYPE_CODE[a.dtype], a.stride(0), b.data_ptr(), _DTYPE_CODE[b.dtype], b.stride(0),
-        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), o.data_ptr(), o.stride(0),
-        _DTYPE_CODE[q.dtype], state.data_ptr(), out_state.data_ptr(), state.stride(0), state.shape[0], init.data_ptr(),
-        to.data_ptr(), float(scale), H, HV, K, V)
-    return args, (init, to)
+    if any(t.dtype not in _DTYPE_CODE for t in (A_log, dt_bias, a, b)):
+        raise _lib.CfbError(f"{what}: a, b, A_log and dt_bias must be fp32, fp16 or bf16")
+    raise _lib.CfbError(f"{what}: q, k, v, o need contiguous heads (any token stride), a, b, A_log, dt_bias too, and state "
+                        "and out_state must be fp32 with contiguous slots and one slot stride")
+
+
+def _heads_strides(t):
+    """The token stride of a [T, heads, dim] tensor with contiguous heads, else None."""
+    st = t.stride()
+    return st[0] if st[2] == 1 and (st[1] == t.shape[2] or t.shape[1] == 1) else None
+
+
+def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B):
+    """(the packed cfb_gdn_args, the converted index tensors, which the caller keeps until the launch)."""
+    out_state = state if out_state is None else out_state
+    qs, vs, ss, dev, dt = q.shape, v.shape, state.shape, q.get_device(), q.dtype
+    good = len(qs) == 3 and len(vs) == 3 and len(ss) == 4 and dev >= 0 and dt in _HALVES
+    if good:
+        T, H, K = qs
+        HV, V = vs[1], vs[2]
+        gates = (T, HV)
+        sq, sk, sv, so = _heads_strides(q), _heads_strides(k), _heads_strides(v), _heads_strides(o)
+        sa, sb, s_in, s_out = a.stride(), b.stride(), state.stride(), out_state.stride()
+        c_A, c_d, c_a, c_b = (_DTYPE_CODE.get(t.dtype) for t in (A_log, dt_bias, a, b))
+        good = (k.shape == qs and vs[0] == T and o.shape == vs and a.shape == gates and b.shape == gates
+                and A_log.shape == (HV,) and dt_bias.shape == (HV,) and ss[1:] == (HV, V, K) and out_state.shape == ss
+                and init_slot.shape == (B,) and out_slot.shape == (B,)
+                and k.dtype == dt and v.dtype == dt and o.dtype == dt
+                and state.dtype == torch.float32 and out_state.dtype == torch.float32
+                and None not in (sq, sk, sv, so, c_A, c_d, c_a, c_b)
+                and (HV == 1 or (sa[1] == 1 and sb[1] == 1 and A_log.stride(0) == 1 and dt_bias.stride(0) == 1))
+                and s_in[3] == 1 and s_in[2] == K and (HV == 1 or s_in[1] == V * K) and s_out[2:] == s_in[2:]
+                and (HV == 1 or s_out[1] == s_in[1]) and s_out[0] == s_in[0]
+                and all(t.get_device() == dev for t in (k, v, o, a, b, A_log, dt_bias, state, out_state, init_slot, out_slot)))
+    if not good:
+        _refuse_sequence(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, out_state, B)
+    init, to = _lib.int32(init_slot), _lib.int32(out_slot)
+    return _lib.PACK_GDN_ARGS(
+        A_log.data_ptr(), c_A, dt_bias.data_ptr(), c_d, a.data_ptr(), c_a, sa[0], b.data_ptr(), c_b, sb[0], q.data_ptr(), sq,
+        k.data_ptr(), sk, v.data_ptr(), sv, o.data_ptr(), so, _DTYPE_CODE[dt], state.data_ptr(), out_state.data_ptr(), s_in[0],
+        ss[0], init.data_ptr(), to.data_ptr(), scale, H, HV, K, V), (init, to)
 
 
 def gdn_step(A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, *, scale: float, out_state=None,
@@ -211,7 +233,7 @@ def gdn_step(A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, *, sc
     lib = _lib.load()
     B = q.shape[0]
     args, keep = _sequence_args("gdn_step", A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B)
-    _lib.check(lib.cfb_gdn_step(C.byref(args), B, _lib.stream_ptr()), "cfb_gdn_step")
+    _lib.check(lib.cfb_gdn_step(args, B, _lib.stream_ptr()), "cfb_gdn_step")
 
 
 class ChunkedGdn:
@@ -240,14 +262,14 @@ class ChunkedGdn:
                             out_state=out_state)
         _lib.require_cuda(cu_seqlens, "cu_seqlens")
         B = cu_seqlens.numel() - 1
-        if cu_seqlens.dim() != 1 or B < 0 or cu_seqlens.device != q.device:
-            raise _lib.CfbError("ChunkedGdn: cu_seqlens must be 1-D [requests + 1] on q's device")
+        if cu_seqlens.dim() != 1 or B < 0 or cu_seqlens.get_device() != q.get_device() or q.dim() != 3 or v.dim() != 3:
+            raise _lib.CfbError("ChunkedGdn: cu_seqlens must be 1-D [requests + 1] on q's device, q [T, H, K], v [T, HV, V]")
         T, HV = q.shape[0], v.shape[1]
         if T > self.max_tokens or B > self.max_requests or HV > self.value_heads:
             raise _lib.CfbError(f"ChunkedGdn: {T} tokens / {B} requests / {HV} value heads exceed this object's "
                                 f"{self.max_tokens} / {self.max_requests} / {self.value_heads}")
         args, keep = _sequence_args("ChunkedGdn", A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale,
                                     out_state, B)
-        cu = cu_seqlens.to(torch.int32).contiguous()
-        _lib.check(self.lib.cfb_gdn_chunk(C.byref(args), cu.data_ptr(), T, B, self.ws_ptr, self.ws_bytes,
+        cu = _lib.int32(cu_seqlens)
+        _lib.check(self.lib.cfb_gdn_chunk(args, cu.data_ptr(), T, B, self.ws_ptr, self.ws_bytes,
                                           _lib.stream_ptr()), "cfb_gdn_chunk")

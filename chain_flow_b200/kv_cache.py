@@ -13,16 +13,6 @@ _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3f
 HEAD_DIMS = (64, 128, 256)
 
 
-def _rows(t, name: str, tokens: int, heads: int, dim: int, device) -> None:
-    _lib.require_cuda(t, name)
-    if t.device != device:
-        raise _lib.CfbError(f"{name} is on {t.device}, the cache on {device}")
-    if tuple(t.shape) != (tokens, heads, dim):
-        raise _lib.CfbError(f"{name}: expected [{tokens}, {heads}, {dim}], got {list(t.shape)}")
-    if t.stride(2) != 1:
-        raise _lib.CfbError(f"{name} needs a contiguous head dim")
-
-
 class PagedKVCache:
     """Keys and values of one layer in ``pages`` pages of ``page_size`` slots. A token's flat slot is
     ``page * page_size + offset``. ``dtype``: fp16 or bf16 (rows are kept as they are), or
@@ -79,7 +69,7 @@ class PagedKVCache:
                     raise _lib.CfbError("PagedKVCache: scales must be fp32 [pages, kv_heads, page_size] with one set of strides")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self._dev = k.dtype, k.device, k.get_device()
         ss = k_scale.stride() if quant else (0, 0, 0)
         self._desc = _lib.KvCache(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if quant else None, v_scale.data_ptr() if quant else None,
@@ -88,10 +78,18 @@ class PagedKVCache:
         self.desc = C.byref(self._desc)
 
     def _slots(self, slots):
-        _lib.require_cuda(slots, "slots")
-        if slots.dim() != 1 or slots.is_floating_point():
-            raise _lib.CfbError("slots must be a 1-D integer tensor")
-        return slots.to(torch.int64).contiguous()
+        if slots.dim() != 1 or slots.is_floating_point() or slots.get_device() != self._dev:
+            _lib.require_cuda(slots, "slots")
+            raise _lib.CfbError("slots must be a 1-D integer tensor on the cache's device")
+        return slots if slots.dtype == torch.int64 and slots.is_contiguous() else slots.to(torch.int64).contiguous()
+
+    def _refuse_rows(self, t, name: str, tokens: int):
+        _lib.require_cuda(t, name)
+        if t.get_device() != self._dev:
+            raise _lib.CfbError(f"{name} is on {t.device}, the cache on {self.device}")
+        if tuple(t.shape) != (tokens, self.kv_heads, self.head_dim):
+            raise _lib.CfbError(f"{name}: expected [{tokens}, {self.kv_heads}, {self.head_dim}], got {list(t.shape)}")
+        raise _lib.CfbError(f"{name} needs a contiguous head dim")
 
     def write(self, key, value, slots, stream=None) -> None:
         """Rows key, value [T, kv_heads, head_dim] (fp16 or bf16; a 16-bit cache takes its own dtype)
@@ -101,15 +99,17 @@ class PagedKVCache:
             with torch.cuda.stream(stream):
                 return self.write(key, value, slots)
         slots = self._slots(slots)
-        T = slots.numel()
-        for t, n in ((key, "key"), (value, "value")):
-            _rows(t, n, T, self.kv_heads, self.head_dim, self.device)
-        dt = _DT.get(key.dtype)
-        if dt not in (1, 2) or value.dtype != key.dtype or (self.k_scale is None and key.dtype != self.dtype):
+        T = slots.shape[0]
+        shape, sk, sv = (T, self.kv_heads, self.head_dim), key.stride(), value.stride()
+        for t, n, st in ((key, "key", sk), (value, "value", sv)):
+            if t.shape != shape or st[2] != 1 or t.get_device() != self._dev:
+                self._refuse_rows(t, n, T)
+        dtype = key.dtype
+        dt = _DT.get(dtype)
+        if dt not in (1, 2) or value.dtype != dtype or (self.k_scale is None and dtype != self.dtype):
             raise _lib.CfbError("PagedKVCache.write: key and value must share fp16 or bf16, the cache's own unless it is e4m3")
-        _lib.check(self.lib.cfb_kv_write(
-            self.desc, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            dt, slots.data_ptr(), T, _lib.stream_ptr()), "cfb_kv_write")
+        _lib.check(self.lib.cfb_kv_write(self.desc, key.data_ptr(), sk[0], sk[1], value.data_ptr(), sv[0], sv[1], dt,
+                                         slots.data_ptr(), T, _lib.stream_ptr()), "cfb_kv_write")
 
     def read(self, slots, dtype=None, stream=None):
         """(key, value) [T, kv_heads, head_dim] of the flat slots [T] in fp32, fp16 or bf16 (default:
@@ -122,9 +122,8 @@ class PagedKVCache:
             dtype = self.dtype if self.k_scale is None else torch.float16
         if _DT.get(dtype) not in (0, 1, 2):
             raise _lib.CfbError("PagedKVCache.read: dtype must be fp32, fp16 or bf16")
-        T = slots.numel()
-        key, value = torch.empty(2, T, self.kv_heads, self.head_dim, dtype=dtype, device=self.device).unbind(0)
-        _lib.check(self.lib.cfb_kv_read(
-            self.desc, slots.data_ptr(), T, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
-            value.stride(0), value.stride(1), _DT[dtype], _lib.stream_ptr()), "cfb_kv_read")
+        T, D = slots.shape[0], self.head_dim
+        key, value = torch.empty(2, T, self.kv_heads, D, dtype=dtype, device=self.device).unbind(0)
+        _lib.check(self.lib.cfb_kv_read(self.desc, slots.data_ptr(), T, key.data_ptr(), self.kv_heads * D, D, value.data_ptr(),
+                                        self.kv_heads * D, D, _DT[dtype], _lib.stream_ptr()), "cfb_kv_read")
         return key, value
