@@ -33,7 +33,7 @@ EXPORTED = [
     "cfb_ring_write", "cfb_ring_gather", "cfb_tree_gdn_verify", "cfb_vae_workspace", "cfb_vae_create",
     "cfb_vae_plan_workspace", "cfb_vae_plan_build", "cfb_tree_attn_merge", "cfb_tree_verify_workspace",
     "cfb_tree_verify_greedy", "cfb_tree_gdn_factor", "cfb_kv_write", "cfb_kv_read", "cfb_paged_attn_workspace",
-    "cfb_paged_attn", "cfb_paged_attn_error", "cfb_gdn_step", "cfb_gdn_chunk_workspace", "cfb_gdn_chunk",
+    "cfb_paged_attn", "cfb_paged_attn_error", "cfb_gdn_step", "cfb_gdn_chunk_workspace", "cfb_gdn_chunk", "cfb_gdn_chunk_error",
 ]
 ABI_VERSION = 5
 XROWS, XFLOATS = 64, 18          # CFB_XROWS, CFB_XFLOATS: the merged-list exchange rows
@@ -182,6 +182,7 @@ def _declare(lib):
     lib.cfb_gdn_chunk_workspace.argtypes = [i32, i32, i32]
     lib.cfb_gdn_chunk_workspace.restype = sz
     lib.cfb_gdn_chunk.argtypes = [vp, vp, i32, i32, vp, sz, vp]
+    lib.cfb_gdn_chunk_error.argtypes = [vp, C.POINTER(i32)]
     return lib
 
 

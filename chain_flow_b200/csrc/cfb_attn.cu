@@ -9,9 +9,7 @@
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
 // so the weights stay at most 1, whatever the scales, and the codes enter the products exactly.
-#include <cuda.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 #include <cuda_fp8.h>
 #include <algorithm>
 #include <cstdlib>
@@ -176,18 +174,6 @@ struct Bars {
       sc_full[kScaleStages], raw_full[8], raw_empty[8], m_set[2][4], swap[4], drain;
 };
 
-CFB_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-CFB_DEV void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, int u, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u), "r"(smem_u32(bar))
-      : "memory");
-}
 CFB_DEV void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -354,8 +340,8 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
   }
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, Lay::cols);
   if (is_tma(SRC) && threadIdx.x == blockDim.x - 1) {
-    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
+    prefetch_map(&k_map);
+    prefetch_map(&v_map);
   }
 
   // Where this CTA's share begins: the running sum of the requests' units, by every warp for itself, a
@@ -1049,19 +1035,6 @@ int sm_count() {
 }
 size_t desc_bytes(int grid) { return ((size_t)grid * sizeof(Desc) + 255) / 256 * 256; }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      f = nullptr;
-    }
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
-  return fn;
-}
-
 // The pool as [page][kv head][slot][dim], read in boxes of `rows` slots: of 16-bit rows all 64-column slabs
 // at once, of codes whole rows. False where a tensor map cannot describe it (rows are then copied one
 // by one).
@@ -1069,7 +1042,7 @@ bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
   const cuuint64_t dim = c.dim, slots = c.page_size, heads = c.kv_heads, pages = c.pages;
   const cuuint64_t slot = c.slot_stride, head = c.head_stride, page = c.page_stride;
   const cuuint32_t step[5] = {1, 1, 1, 1, 1}, r = rows;
-  const auto encode = encoder();
+  const auto encode = tensor_map_encoder();
   if (!encode) return false;
   if (c.dtype == DT_E4M3) {
     const cuuint64_t dims[4] = {dim, slots, heads, pages}, strides[3] = {slot, head, page};

@@ -167,17 +167,19 @@ constexpr int kPairs = kBlocks * (kBlocks + 1) / 2;            // lower-triangul
 // float4 (two neighbours' hi, their lo) a lane for each lower-triangular block, then per token beta,
 // beta e^G r, e^{G_C-G} r, e^G scale rq, then e^{G_C}.
 constexpr int kFragFloats = kPairs * 32 * 4;
-constexpr int kPrepFloats = 2 * kFragFloats + 4 * kC + 4;
+constexpr int kPrepFloats = 2 * kFragFloats + 4 * kC + 4;      // (over bf16 P's lo terms are left out)
+template <typename T>
+struct Prep {
+  static constexpr int kP = std::is_same<T, __half>::value ? 4 : 2;          // floats of P a lane and block
+  static constexpr int kVec = kFragFloats + kPairs * 32 * kP, kFloats = kVec + 4 * kC + 4;
+};
 constexpr int kRowHalves = kK + 8;                             // padded row of a staged K or Q tile
 
-CFB_DEV float tf32(float x) {
-  uint32_t y;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
-  return __uint_as_float(y);
-}
+// x = hi + lo, both of 11 bits (tf32): hi is x cut off, lo the remainder rounded. Integer operations: a
+// conversion instruction takes eight cycles a warp, and a chunk splits 128 values a lane.
 CFB_DEV void split(float x, float& hi, float& lo) {
-  hi = tf32(x);
-  lo = tf32(x - hi);
+  hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+  lo = __uint_as_float((__float_as_uint(x - hi) + 0x1000u) & 0xffffe000u);
 }
 CFB_DEV void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -227,27 +229,31 @@ CFB_DEV bool chunk_of(const int32_t* cu, int total, int B, int x, int* b, int* t
   return *t0 >= first && *n > 0;
 }
 
-// One CTA of two warps per (chunk, value head): warp 0 forms K K^T and T, warp 1 Q K^T and P. Rows of
-// tokens that the chunk does not have are zeros with beta = 0 and no decay.
+// One CTA of two warps per (chunk, value head): warp 0 forms K K^T, A and T, warp 1 Q K^T and P, both in
+// their accumulators (P's are already in the order that the scan reads). The norms are diagonals of
+// K K^T and Q Q^T. Rows of tokens that the chunk does not have are zeros with beta = 0 and no decay.
 template <typename T>
-__global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, float* ws) {
+__global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, float* ws, int* err) {
   __shared__ __align__(16) T sk[kC][kRowHalves];
   __shared__ __align__(16) T sq[kC][kRowHalves];
   __shared__ __align__(16) float sa[kC][kC + 4];               // A, then T
-  __shared__ float sp[kC][kC + 1];                             // q . k
-  __shared__ double sG[kC];
-  __shared__ float sr[kC], srq[kC];
+  __shared__ float2 sG[kC];                                    // G log2(e) as a sum of two floats
+  __shared__ float sd[2][kC];                                  // reciprocal norms of k, of q
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hv = blockIdx.y, h = hv / (g.HV / g.H);
   int b, t0, n;
+  if (blockIdx.x == 0 && hv == 0 && threadIdx.x == 0) *err = 0;
   if (!chunk_of(cu, total, B, blockIdx.x, &b, &t0, &n)) return;
-  for (int x = threadIdx.x; x < kC * 16 * 2; x += 64) {
-    const int row = (x >> 4) % kC, c = x & 15;
-    const bool is_q = x >= kC * 16;
-    const T* src = is_q ? static_cast<const T*>(g.q) + (long long)(t0 + row) * g.q_stride : static_cast<const T*>(g.k) + (long long)(t0 + row) * g.k_stride;
-    uint4 y = make_uint4(0, 0, 0, 0);
-    if (row < n) y = __ldg(reinterpret_cast<const uint4*>(src + (long long)h * kK) + c);
-    *reinterpret_cast<uint4*>(is_q ? &sq[row][c * 8] : &sk[row][c * 8]) = y;
+  {
+    const T* k = static_cast<const T*>(g.k) + (long long)t0 * g.k_stride + (long long)h * kK;
+    const T* q = static_cast<const T*>(g.q) + (long long)t0 * g.q_stride + (long long)h * kK;
+#pragma unroll
+    for (int x = 0; x < kC * 16 / 64; ++x) {
+      const int row = x * 4 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+      const bool in = row < n;
+      cp_async16z(smem_u32(&sk[row][c * 8]), k + (in ? (long long)row * g.k_stride : 0) + c * 8, in);
+      cp_async16z(smem_u32(&sq[row][c * 8]), q + (in ? (long long)row * g.q_stride : 0) + c * 8, in);
+    }
   }
   float beta = 0.f, decay = 0.f;
   if (lane < n) {
@@ -257,81 +263,78 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
     beta = sigmoid(load_coded(g.b, g.b_dtype, (long long)(t0 + lane) * g.b_stride + hv));
   }
   // G by token (a decay of e^-1e6 is 0 all the same; sums and differences stay numbers)
-  double G = decay < -1e6f ? -1e6 : (double)decay;
+  double G = (decay < -1e6f ? -1e6 : (double)decay) * 1.4426950408889634;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const double y = __shfl_up_sync(0xffffffffu, G, off);
     if (lane >= off) G += y;
   }
-  const double G_end = __shfl_sync(0xffffffffu, G, 31);
+  // differences of G from two floats each: the sum of 32 decays in 48 bits
+  const float2 G2 = make_float2((float)G, (float)(G - (double)(float)G));
+  const float2 G_end = make_float2(__shfl_sync(0xffffffffu, G2.x, 31), __shfl_sync(0xffffffffu, G2.y, 31));
+  const auto decay_between = [](float2 to, float2 from) { return exp2f((to.x - from.x) + (to.y - from.y)); };
+  if (warp == 0) sG[lane] = G2;
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  // norms: warp 0 of k, warp 1 of q, a lane a row
-  {
-    const T* row = warp ? sq[lane] : sk[lane];
-    float sum = 0.f;
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      const uint4 y = *reinterpret_cast<const uint4*>(row + 8 * c);
-      const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack16<T>(ys[e]);
-        sum = fmaf(f.x, f.x, sum);
-        sum = fmaf(f.y, f.y, sum);
-      }
-    }
-    (warp ? srq : sr)[lane] = rsqrtf(sum + kNormEps);
-    if (warp == 0) sG[lane] = G;
-  }
-  // X K^T, X = K (warp 0) or Q (warp 1)
+  // X K^T, X = K (warp 0) or Q (warp 1): blocks on and below the diagonal
   const int gid = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
-    float acc[kBlocks][4] = {};
-    const uint32_t a_at = smem_u32(&(warp ? sq : sk)[mt * 16 + (lane & 15)][(lane >> 4) * 8]);
-    const uint32_t b_at = smem_u32(&sk[lane][0]);
+  float acc[2][kBlocks][4] = {};
+  {
+    const uint32_t a_at = smem_u32(&(warp ? sq : sk)[lane & 15][(lane >> 4) * 8]), b_at = smem_u32(&sk[lane][0]);
+    float dq[2][2][4] = {};                                    // Q Q^T's diagonal blocks (warp 1)
 #pragma unroll
     for (int k = 0; k < kK / 16; ++k) {
-      uint32_t a[4], b0[4], b1[4];
-      ldmatrix4(a, a_at + k * 32);
+      uint32_t a[2][4], b0[4], b1[4];
+      ldmatrix4(a[0], a_at + k * 32);
+      ldmatrix4(a[1], a_at + 16 * kRowHalves * 2 + k * 32);
       ldmatrix4(b0, b_at + k * 32);
       ldmatrix4(b1, b_at + k * 32 + 16);
 #pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt) mma_16<T>(acc[nt], a, b0[nt], b1[nt]);
-    }
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-    for (int nt = 0; nt < kBlocks; ++nt)
+        for (int nt = 0; nt < 2 * mt + 2; ++nt) mma_16<T>(acc[mt][nt], a[mt], b0[nt], b1[nt]);
+      if (warp) {
+        // a's fragments hold Q's own rows as the second operand too: rows 0-7 in a[0], a[2], 8-15 in a[1], a[3]
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = mt * 16 + gid + (e >> 1) * 8, j = nt * 8 + 2 * t + (e & 1);
-        if (warp) sp[i][j] = acc[nt][e];
-        else sa[i][j] = acc[nt][e];
+        for (int mt = 0; mt < 2; ++mt) {
+          mma_16<T>(dq[mt][0], a[mt], a[mt][0], a[mt][2]);
+          mma_16<T>(dq[mt][1], a[mt], a[mt][1], a[mt][3]);
+        }
       }
+    }
+    // the diagonals: row gid of a block is column 2t (+ 1) in lane t = gid / 2
+    if (t == gid >> 1) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const float even = warp ? dq[mt][z][2 * z] : acc[mt][2 * mt + z][2 * z];
+          const float odd = warp ? dq[mt][z][2 * z + 1] : acc[mt][2 * mt + z][2 * z + 1];
+          sd[warp][mt * 16 + z * 8 + gid] = rsqrtf((gid & 1 ? odd : even) + kNormEps);
+        }
+    }
   }
   __syncthreads();
+  const float* const rk = sd[0];
   float* const out = ws + ((long long)blockIdx.x * g.HV + hv) * kPrepFloats;
-  const auto put = [&](float4* dst, auto value) {              // the lower-triangular blocks, as the scan reads them
-#pragma unroll
-    for (int nt = 0; nt < kBlocks; ++nt)
-#pragma unroll
-      for (int jb = 0; jb <= nt; ++jb) {
-        const int i = nt * 8 + gid, j = jb * 8 + 2 * t;
-        float4 f;
-        split(j <= i ? value(i, j) : 0.f, f.x, f.z);
-        split(j + 1 <= i ? value(i, j + 1) : 0.f, f.y, f.w);
-        dst[(nt * (nt + 1) / 2 + jb) * 32 + lane] = f;
-      }
-  };
   if (warp == 0) {
-    // A, a lane a column; then T column by column: x_i = [i = j] - sum_{m<i} A_im x_m
-    const double Gj = sG[lane];
-    const float rj = sr[lane];
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      const float bi = __shfl_sync(0xffffffffu, beta, i);
-      sa[i][lane] = lane < i ? bi * sr[i] * rj * expf((float)(sG[i] - Gj)) * sa[i][lane] : 0.f;
-    }
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int i = mt * 16 + z * 8 + gid;
+        const float f = __shfl_sync(0xffffffffu, beta, i) * rk[i];
+        const float2 Gi = sG[i];
+#pragma unroll
+        for (int nt = 0; nt <= 2 * mt + z; ++nt) {
+          const int j = nt * 8 + 2 * t;
+          const float2 x = make_float2(j < i ? f * rk[j] * decay_between(Gi, sG[j]) * acc[mt][nt][2 * z] : 0.f,
+                                       j + 1 < i ? f * rk[j + 1] * decay_between(Gi, sG[j + 1]) * acc[mt][nt][2 * z + 1] : 0.f);
+          *reinterpret_cast<float2*>(&sa[i][j]) = x;
+        }
+      }
     __syncwarp();
+    // T column by column, a lane a column: x_i = [i = j] - sum_{m<i} A_im x_m
     float x[kC];
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
@@ -350,77 +353,232 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
 #pragma unroll
     for (int i = 0; i < kC; ++i) sa[i][lane] = x[i];
     __syncwarp();
-    put(reinterpret_cast<float4*>(out), [&](int i, int j) { return sa[i][j]; });
+    float4* const tf = reinterpret_cast<float4*>(out) + lane;
+#pragma unroll
+    for (int nt = 0; nt < kBlocks; ++nt)
+#pragma unroll
+      for (int jb = 0; jb <= nt; ++jb) {
+        const float2 y = *reinterpret_cast<const float2*>(&sa[nt * 8 + gid][jb * 8 + 2 * t]);
+        float4 f;
+        split(y.x, f.x, f.z);
+        split(y.y, f.y, f.w);
+        tf[(nt * (nt + 1) / 2 + jb) * 32] = f;
+      }
   } else {
-    put(reinterpret_cast<float4*>(out + kFragFloats),
-        [&](int i, int j) { return g.scale * srq[i] * sr[j] * expf((float)(sG[i] - sG[j])) * sp[i][j]; });
-    float* const v = out + 2 * kFragFloats;
-    const float eG = expf((float)G);
+    const float* const rq = sd[1];
+    float* const pf = out + kFragFloats + lane * Prep<T>::kP;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int nt = 2 * mt + z, i = nt * 8 + gid;
+        const float f = g.scale * rq[i];
+        const float2 Gi = sG[i];
+#pragma unroll
+        for (int jb = 0; jb <= nt; ++jb) {
+          const int j = jb * 8 + 2 * t;
+          const float x = j <= i ? f * rk[j] * decay_between(Gi, sG[j]) * acc[mt][jb][2 * z] : 0.f;
+          const float y = j + 1 <= i ? f * rk[j + 1] * decay_between(Gi, sG[j + 1]) * acc[mt][jb][2 * z + 1] : 0.f;
+          float* const dst = pf + (nt * (nt + 1) / 2 + jb) * 32 * Prep<T>::kP;
+          float4 w;
+          split(x, w.x, w.z);
+          split(y, w.y, w.w);
+          if constexpr (Prep<T>::kP == 4) *reinterpret_cast<float4*>(dst) = w;
+          else *reinterpret_cast<float2*>(dst) = make_float2(w.x, w.y);
+        }
+      }
+    float* const v = out + Prep<T>::kVec;
+    const float eG = exp2f(G2.x + G2.y);
     v[lane] = beta;
-    v[kC + lane] = beta * eG * sr[lane];
-    v[2 * kC + lane] = expf((float)(G_end - G)) * sr[lane];
-    v[3 * kC + lane] = eG * g.scale * srq[lane];
-    if (lane == 0) v[4 * kC] = expf((float)G_end);
+    v[kC + lane] = beta * eG * rk[lane];
+    v[2 * kC + lane] = decay_between(G_end, G2) * rk[lane];
+    v[3 * kC + lane] = eG * g.scale * rq[lane];
+    if (lane < 4) v[4 * kC + lane] = exp2f(G_end.x + G_end.y);
   }
 }
 
-// One CTA per (32 value rows, value head, request): 2 * KS warps, a warp 16 value rows and 128 / KS of
-// the state's columns. KS = 2 halves the longest chain of a chunk at the price of an exchange of the
-// partial sums of S k and S q; it is taken where KS = 1 would leave SM quarters without a warp.
-constexpr int kScanRows = 32, kScanStages = 3;
-struct ScanStage {
-  static constexpr int kKV = kC * kRowHalves * 2, kVPitch = kScanRows * 2 + 16;
-  static constexpr int off_q = kKV, off_v = 2 * kKV, off_prep = off_v + kC * kVPitch, bytes = off_prep + kPrepFloats * 4;
+// One CTA per (32 value rows, value head, request), two value tiles of 16 rows, nine warps, so that every
+// quarter of the SM has a warp of the first two kinds:
+//   0-3  the state: warp 2 vt + ks holds tile vt's rows and half ks of the columns. A chunk is S k (the two
+//        halves exchange partial sums), U and the update, nothing else;
+//   4-7  the outputs, a chunk behind, warp 4 + 2 vt + x tile vt's of half x of the tokens: S, as it was before
+//        the chunk, and U reach them through shared memory (two buffers), so that S q and P U are off the
+//        chain that bounds the kernel;
+//   8    one lane issues the copies of the chunks to come: K and Q as [64 columns][32 tokens] 128-byte-
+//        swizzled boxes, V as a plain box, T, P and the vectors in one piece. (The same copies by 16-byte
+//        cp.async kept a warp busy for longer than a chunk takes.)
+constexpr int kScanStages = 3, kTiles = 2, kStateWarps = 2 * kTiles, kOutWarps = 2 * kTiles, kScanRows = 16 * kTiles;
+constexpr int kScanThreads = (kStateWarps + kOutWarps + 1) * 32;
+constexpr int kHandThreads = 4 * 32;                           // a tile's two state and two output warps
+template <typename T>
+struct Scan {
+  static constexpr int kKV = kC * kK * 2, kV = kC * kScanRows * 2, kPrep = Prep<T>::kFloats * 4;
+  static constexpr int off_q = kKV, off_v = 2 * kKV, off_prep = off_v + kV;
+  static constexpr int stage = (off_prep + kPrep + 1023) / 1024 * 1024, off_swap = kScanStages * stage;
+  static constexpr int kSwap = kBlocks * 2 * 32 * 8;           // one warp's partial sums of S k
+  // what a tile's output warp reads: S ([16 blocks][lane] of four), U ([4 blocks][lane]), the first tokens lost
+  static constexpr int off_hand = off_swap + 2 * kStateWarps * kSwap, off_u = 16 * 512, off_lost = off_u + kBlocks * 512;
+  static constexpr int kHand = off_lost + 256;
+  static constexpr int bytes = off_hand + 2 * kTiles * kHand + 1024;
+  static constexpr int tx = 2 * kKV + kV + kPrep;
 };
-static_assert(ScanStage::off_prep % 16 == 0 && ScanStage::bytes % 16 == 0 && kPrepFloats % 4 == 0, "16-byte copies");
+CFB_DEV void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
+CFB_DEV void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
 
-template <typename T, int KS>
-__global__ void __launch_bounds__(64 * KS) gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float* ws) {
-  constexpr int NJ = 16 / KS;                                  // 8-column blocks of the state a warp holds
+// An accumulator as the first operand of the next product: the summed index is permuted, 2t and 2t + 1 for
+// t and t + 4, and the second operand is read so.
+CFB_DEV void operand(const float (&s)[4], float (&hi)[4], float (&lo)[4]) {
+  split(s[0], hi[0], lo[0]);
+  split(s[2], hi[1], lo[1]);
+  split(s[1], hi[2], lo[2]);
+  split(s[3], hi[3], lo[3]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads)
+gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float* ws, int* err,
+                const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                const __grid_constant__ CUtensorMap v_map) {
+  using Lay = Scan<T>;
+  constexpr int NJ = 8;                                        // 8-column blocks of the state a warp holds
   constexpr bool kFine = std::is_same<T, __half>::value;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float2 sx[KS == 2 ? 2 : 1][2][kBlocks][2][32];    // partial sums that the two halves exchange
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kScanStages], empty[kScanStages];
+  __shared__ int dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
-  const int vt = warp / KS, ks = warp % KS;                    // value tile, column half
   const int hv = blockIdx.y, b = blockIdx.z, h = hv / (g.HV / g.H), v0 = blockIdx.x * kScanRows;
   const int first = min(max(cu[b], 0), total), end = min(max(cu[b + 1], first), total);
   const int chunks = (end - first + kC - 1) / kC;
-  const float* const prep = ws + ((long long)(first / kC + b) * g.HV + hv) * kPrepFloats;
-  const uint32_t sm = smem_u32(smem);
-
-  const auto load = [&](int c) {
-    const uint32_t at = sm + (c % kScanStages) * ScanStage::bytes;
-    const int t0 = first + c * kC, n = min(kC, end - t0);
-    const T* k = static_cast<const T*>(g.k) + (long long)t0 * g.k_stride + (long long)h * kK;
-    const T* q = static_cast<const T*>(g.q) + (long long)t0 * g.q_stride + (long long)h * kK;
-    const T* v = static_cast<const T*>(g.v) + (long long)t0 * g.v_stride + (long long)hv * g.V + v0;
-    for (int x = threadIdx.x; x < kC * 16; x += 64 * KS) {
-      const int row = x >> 4, p = x & 15;
-      const bool in = row < n;
-      cp_async16z(at + row * (kRowHalves * 2) + p * 16, k + (in ? (long long)row * g.k_stride : 0) + p * 8, in);
-      cp_async16z(at + ScanStage::off_q + row * (kRowHalves * 2) + p * 16, q + (in ? (long long)row * g.q_stride : 0) + p * 8, in);
+  const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (sm - smem_u32(smem_raw));
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kScanStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kStateWarps + kOutWarps);
     }
-    for (int x = threadIdx.x; x < kC * kScanRows / 8; x += 64 * KS) {
-      const int row = x / (kScanRows / 8), p = x % (kScanRows / 8);
-      const bool in = row < n;
-      cp_async16z(at + ScanStage::off_v + row * ScanStage::kVPitch + p * 16, v + (in ? (long long)row * g.v_stride : 0) + p * 8, in);
-    }
-    const float* src = prep + (long long)c * g.HV * kPrepFloats;
-    for (int x = threadIdx.x; x < kPrepFloats / 4; x += 64 * KS) cp_async16z(at + ScanStage::off_prep + x * 16, src + x * 4, true);
-  };
-
-#pragma unroll
-  for (int c = 0; c < kScanStages - 1; ++c) {
-    if (c < chunks) load(c);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    fence_mbar_init();
+    dead = 0;
   }
-  // the state: lane (gid, t) holds rows gid and gid + 8, columns 2t and 2t + 1 of every 8-column block
+  __syncthreads();
+  // A wait that outlasts its limit marks the CTA dead: from then on nothing waits, the chunks run through
+  // to the end on whatever is there (so that the barriers between warps still meet), and the state is set
+  // to NaN.
+  volatile int* const is_dead = &dead;
+  const auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_test_wait(bar, parity)) return;
+    if (*is_dead == 0 && !mbar_wait(bar, parity)) *is_dead = 1;
+  };
+  // barriers of a tile: the state warps' exchange; S and U handed over; a hand-over buffer free again
+  const int tile = (warp % kStateWarps) / 2;
+  const int swap_bar = 1 + tile * 5, hand_bar = swap_bar + 1, free_bar = swap_bar + 3;       // (+ chunk & 1)
+  const auto hand_at = [&](int c) { return smem + Lay::off_hand + ((c & 1) * kTiles + tile) * Lay::kHand; };
+  // token `lane`'s row of a K or Q tile, 8-column block x: 128-byte rows of half the columns, 16-byte pieces
+  // XORed with token & 7
+  const auto block = [&](uint32_t at, int x) { return at + lane * 128 + (x >> 3) * (kC * 128) + (((x & 7) ^ (lane & 7)) << 4); };
+
+  if (warp == kStateWarps + kOutWarps) {
+    // ------------------------------------------------------------ copies
+    if (lane == 0) {
+      prefetch_map(&q_map);
+      prefetch_map(&k_map);
+      prefetch_map(&v_map);
+      const float* const prep = ws + ((long long)(first / kC + b) * g.HV + hv) * kPrepFloats;
+      for (int c = 0; c < chunks; ++c) {
+        const int st = c % kScanStages;
+        if (c >= kScanStages) wait(&empty[st], (c / kScanStages - 1) & 1);
+        if (*is_dead) break;
+        const uint32_t at = sm + st * Lay::stage;
+        mbar_arrive_expect_tx(&full[st], Lay::tx);
+        tma_load_4d(at, &k_map, 0, first + c * kC, 0, h, &full[st]);
+        tma_load_3d(at + Lay::off_v, &v_map, v0, first + c * kC, hv, &full[st]);
+        bulk_g2s(smem + st * Lay::stage + Lay::off_prep, prep + (long long)c * g.HV * kPrepFloats, Lay::kPrep, &full[st]);
+        tma_load_4d(at + Lay::off_q, &q_map, 0, first + c * kC, 0, h, &full[st]);
+      }
+    }
+    return;
+  }
+
+  if (warp >= kStateWarps) {
+    // ------------------------------------------------------------ outputs: o = e^G scale rq (S q) + P U
+    for (int c = 0; c < chunks; ++c) {
+      wait(&full[c % kScanStages], (c / kScanStages) & 1);
+      const uint8_t* const st = smem + (c % kScanStages) * Lay::stage;
+      const uint32_t q_at = sm + (c % kScanStages) * Lay::stage + Lay::off_q;
+      const float* const pf = reinterpret_cast<const float*>(st + Lay::off_prep) + kFragFloats + lane * Prep<T>::kP;
+      const float* const vec = reinterpret_cast<const float*>(st + Lay::off_prep) + Prep<T>::kVec;
+      const uint8_t* const hand = hand_at(c);
+      bar_sync(hand_bar + (c & 1), kHandThreads);
+      float O[2][4] = {}, hi[kBlocks][4], lo[kBlocks][4];
+      const int n0 = 2 * (warp & 1);                           // this warp's token blocks: n0, n0 + 1
+#pragma unroll 4
+      for (int j = 0; j < 16; ++j) {
+        const float4 s4 = reinterpret_cast<const float4*>(hand)[j * 32 + lane];
+        const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
+        uint32_t qw[4];
+        ldmatrix4(qw, block(q_at, j));
+        operand(sj, hi[0], lo[0]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float2 q2 = unpack16<T>(n0 ? qw[2 + x] : qw[x]);
+          mma_tf32(O[x], hi[0], q2.x, q2.y);
+          if (kFine) mma_tf32(O[x], lo[0], q2.x, q2.y);
+        }
+      }
+      const int2 lost = reinterpret_cast<const int2*>(hand + Lay::off_lost)[lane];
+#pragma unroll
+      for (int jb = 0; jb < kBlocks; ++jb) {
+        const float4 u4 = reinterpret_cast<const float4*>(hand + Lay::off_u)[jb * 32 + lane];
+        const float u[4] = {u4.x, u4.y, u4.z, u4.w};
+        operand(u, hi[jb], lo[jb]);
+      }
+      bar_arrive(free_bar + (c & 1), kHandThreads);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int nt = n0 + x;
+        const float2 f = *reinterpret_cast<const float2*>(vec + 3 * kC + nt * 8 + 2 * t);
+        O[x][0] *= f.x; O[x][1] *= f.y; O[x][2] *= f.x; O[x][3] *= f.y;
+#pragma unroll
+        for (int jb = 0; jb < kBlocks; ++jb) {
+          if (jb > nt) break;
+          const float* const p = pf + (nt * (nt + 1) / 2 + jb) * 32 * Prep<T>::kP;
+          if constexpr (kFine) {
+            const float4 w = *reinterpret_cast<const float4*>(p);
+            mma_tf32(O[x], hi[jb], w.z, w.w);
+            mma_tf32(O[x], lo[jb], w.x, w.y);
+            mma_tf32(O[x], hi[jb], w.x, w.y);
+          } else {
+            const float2 w = *reinterpret_cast<const float2*>(p);
+            mma_tf32(O[x], hi[jb], w.x, w.y);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (nt * 8 + 2 * t + (e & 1) >= (e < 2 ? lost.x : lost.y)) O[x][e] = __int_as_float(0x7fc00000);
+        // rows to tokens: lane (gid, t) then holds token gid, value rows 2t and 2t + 1
+        const int tok = first + c * kC + nt * 8 + gid;
+        const uint32_t a = transpose8(pack16<T>(O[x][0], O[x][1])), bb = transpose8(pack16<T>(O[x][2], O[x][3]));
+        if (tok < end) {
+          T* out = static_cast<T*>(g.o) + (long long)tok * g.o_stride + (long long)hv * g.V + v0 + tile * 16 + 2 * t;
+          *reinterpret_cast<uint32_t*>(out) = a;
+          *reinterpret_cast<uint32_t*>(out + 8) = bb;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[c % kScanStages]);
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- state: lane (gid, t) holds rows gid and
+  // gid + 8, columns 2t and 2t + 1 of every 8-column block
+  const int ks = warp & 1;
   float S[NJ][4];
+  const long long state_at = ((long long)hv * g.V + v0 + tile * 16 + gid) * kK + ks * NJ * 8 + 2 * t;
   {
     const int from = g.init_slot[b];
     const float fill = from < 0 ? 0.f : __int_as_float(0x7fc00000);
     const bool read = from >= 0 && from < g.slots;
-    const float* src = g.state_in + (read ? from * g.slot_stride : 0) + ((long long)hv * g.V + v0 + vt * 16 + gid) * kK + ks * NJ * 8 + 2 * t;
+    const float* src = g.state_in + (read ? from * g.slot_stride : 0) + state_at;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float2 x = make_float2(fill, fill), y = x;
@@ -431,148 +589,112 @@ __global__ void __launch_bounds__(64 * KS) gdn_scan_kernel(const cfb_gdn_args g,
       S[j][0] = x.x; S[j][1] = x.y; S[j][2] = y.x; S[j][3] = y.y;
     }
   }
-  // an accumulator as the first operand of the next product (see above)
-  const auto operand = [](const float (&s)[4], float (&hi)[4], float (&lo)[4]) {
-    split(s[0], hi[0], lo[0]);
-    split(s[2], hi[1], lo[1]);
-    split(s[1], hi[2], lo[2]);
-    split(s[3], hi[3], lo[3]);
-  };
-
   for (int c = 0; c < chunks; ++c) {
-    asm volatile("cp.async.wait_group %0;" :: "n"(kScanStages - 2) : "memory");
-    __syncthreads();
-    if (c + kScanStages - 1 < chunks) load(c + kScanStages - 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    const uint32_t at = sm + (c % kScanStages) * ScanStage::bytes;
-    const uint8_t* const st = smem + (c % kScanStages) * ScanStage::bytes;
-    const float4* const tf = reinterpret_cast<const float4*>(st + ScanStage::off_prep) + lane;
-    const float4* const pf = tf + kFragFloats / 4;
-    const float* const vec = reinterpret_cast<const float*>(st + ScanStage::off_prep) + 2 * kFragFloats;
+    uint8_t* const hand = hand_at(c);
+    if (c >= 2) bar_sync(free_bar + (c & 1), kHandThreads);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      reinterpret_cast<float4*>(hand)[(ks * NJ + j) * 32 + lane] = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
+    wait(&full[c % kScanStages], (c / kScanStages) & 1);
+    const uint32_t at = sm + (c % kScanStages) * Lay::stage;
+    uint8_t* const st = smem + (c % kScanStages) * Lay::stage;
+    const float4* const tf = reinterpret_cast<const float4*>(st + Lay::off_prep) + lane;
+    const float* const vec = reinterpret_cast<const float*>(st + Lay::off_prep) + Prep<T>::kVec;
+    const int live = end - first - c * kC;                     // tokens of the chunk, if fewer than kC
+    if (live < kC) {
+      // the boxes hold the next request's rows there: keys whose zero weights must not meet a NaN (every
+      // warp zeroes all of them for itself)
+      for (int x = live * 8 + lane; x < kC * 8; x += 32) {
+        *reinterpret_cast<uint4*>(st + x * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(st + kC * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+    }
 
-    // S k and S q of the chunk's tokens
-    float R[kBlocks][4] = {}, Rl[kBlocks][4] = {}, O[kBlocks][4] = {};
-    const uint32_t row_at = at + lane * (kRowHalves * 2) + ks * NJ * 16;
+    // S k of the chunk's tokens
+    float R[kBlocks][4] = {}, Rl[kBlocks][4] = {};
+    uint32_t kw[2][4];                                         // a block ahead
+    ldmatrix4(kw[0], block(at, ks * NJ));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float hi[4], lo[4];
       operand(S[j], hi, lo);
-      uint32_t kw[4], qw[4];
-      ldmatrix4(kw, row_at + j * 16);
-      ldmatrix4(qw, row_at + ScanStage::off_q + j * 16);
+      if (j + 1 < NJ) ldmatrix4(kw[(j + 1) & 1], block(at, ks * NJ + j + 1));
 #pragma unroll
       for (int nt = 0; nt < kBlocks; ++nt) {
-        const float2 k2 = unpack16<T>(kw[nt]), q2 = unpack16<T>(qw[nt]);
+        const float2 k2 = unpack16<T>(kw[j & 1][nt]);
         mma_tf32(R[nt], hi, k2.x, k2.y);
         mma_tf32(Rl[nt], lo, k2.x, k2.y);
-        mma_tf32(O[nt], hi, q2.x, q2.y);
-        if (kFine) mma_tf32(O[nt], lo, q2.x, q2.y);
       }
     }
+    // what the next steps read, ahead of them
+    uint32_t vw[kBlocks / 2][4];
 #pragma unroll
-    for (int nt = 0; nt < kBlocks; ++nt)
+    for (int nt = 0; nt < kBlocks; nt += 2)
+      ldmatrix4_t(vw[nt / 2], at + Lay::off_v + (nt * 8 + (lane & 7) + (lane & 16 ? 8 : 0)) * (kScanRows * 2) + tile * 32 + (lane & 8 ? 16 : 0));
+    float2 bt[kBlocks], be[kBlocks], eg[kBlocks];
+    float4 tw[kPairs];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) R[nt][e] += Rl[nt][e];
-    // With two column halves: both need all of S k; of S q each takes two blocks of tokens to finish.
-    constexpr int kOut = kBlocks / KS;                         // token blocks whose outputs this warp writes
-    const int o0 = ks * kOut;
-    if constexpr (KS == 2) {
+    for (int nt = 0; nt < kBlocks; ++nt) {
+      bt[nt] = *reinterpret_cast<const float2*>(vec + nt * 8 + 2 * t);
+      be[nt] = *reinterpret_cast<const float2*>(vec + kC + nt * 8 + 2 * t);
+      eg[nt] = *reinterpret_cast<const float2*>(vec + 2 * kC + nt * 8 + 2 * t);
+    }
+#pragma unroll
+    for (int x = 0; x < kPairs; ++x) tw[x] = tf[x * 32];
+    const float dec = vec[4 * kC];
+    // both halves need all of S k (two buffers in turn: the next chunk's barrier comes between a value's
+    // reading and its overwriting)
+    {
+      using Sums = float2[kBlocks][2][32];
+      uint8_t* const swap = smem + Lay::off_swap + ((c & 1) * kTiles + tile) * 2 * Lay::kSwap;
+      Sums& mine = *reinterpret_cast<Sums*>(swap + ks * Lay::kSwap);
+      Sums& theirs = *reinterpret_cast<Sums*>(swap + (ks ^ 1) * Lay::kSwap);
 #pragma unroll
       for (int nt = 0; nt < kBlocks; ++nt) {
-        sx[vt][ks][nt][0][lane] = make_float2(R[nt][0], R[nt][1]);
-        sx[vt][ks][nt][1][lane] = make_float2(R[nt][2], R[nt][3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) R[nt][e] += Rl[nt][e];
+        mine[nt][0][lane] = make_float2(R[nt][0], R[nt][1]);
+        mine[nt][1][lane] = make_float2(R[nt][2], R[nt][3]);
       }
-      __syncthreads();
+      bar_sync(swap_bar, 64);
 #pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt) {
-        const float2 x = sx[vt][ks ^ 1][nt][0][lane], y = sx[vt][ks ^ 1][nt][1][lane];
-        // in one order, so that both halves go on with the same bits
-        const float mine[4] = {R[nt][0], R[nt][1], R[nt][2], R[nt][3]}, other[4] = {x.x, x.y, y.x, y.y};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) R[nt][e] = ks ? other[e] + mine[e] : mine[e] + other[e];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int x = 0; x < kOut; ++x) {
-        const int nt = (ks ^ 1) * kOut + x;
-        float give[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) give[e] = ks ? O[x][e] : O[kOut + x][e];
-        sx[vt][ks][nt][0][lane] = make_float2(give[0], give[1]);
-        sx[vt][ks][nt][1][lane] = make_float2(give[2], give[3]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int x = 0; x < kOut; ++x) {
-        const float2 u = sx[vt][ks ^ 1][o0 + x][0][lane], y = sx[vt][ks ^ 1][o0 + x][1][lane];
-        const float add[4] = {u.x, u.y, y.x, y.y};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[x][e] = (ks ? O[kOut + x][e] : O[x][e]) + add[e];
+      for (int nt = 0; nt < kBlocks; ++nt) {                   // (a + b is b + a: both halves go on with the same bits)
+        const float2 x = theirs[nt][0][lane], y = theirs[nt][1][lane];
+        R[nt][0] += x.x; R[nt][1] += x.y; R[nt][2] += y.x; R[nt][3] += y.y;
       }
     }
 
     // beta (v - e^G r (S k)), value rows by tokens like the accumulators
     float hi[kBlocks][4], lo[kBlocks][4];
-    float odd = 0.f;                                           // turns NaN where something is not finite
+    float odd[kBlocks];                                        // turns NaN where something is not finite
 #pragma unroll
-    for (int nt = 0; nt < kBlocks; nt += 2) {
-      uint32_t vw[4];
-      ldmatrix4_t(vw, at + ScanStage::off_v + (nt * 8 + (lane & 7) + (lane & 16 ? 8 : 0)) * ScanStage::kVPitch + vt * 32 + (lane & 8 ? 16 : 0));
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const float2 bt = *reinterpret_cast<const float2*>(vec + (nt + z) * 8 + 2 * t);
-        const float2 be = *reinterpret_cast<const float2*>(vec + kC + (nt + z) * 8 + 2 * t);
-        const float2 va = unpack16<T>(vw[2 * z]), vb = unpack16<T>(vw[2 * z + 1]);
-        float (&r)[4] = R[nt + z];
-        r[0] = fmaf(-be.x, r[0], bt.x * va.x);
-        r[1] = fmaf(-be.y, r[1], bt.y * va.y);
-        r[2] = fmaf(-be.x, r[2], bt.x * vb.x);
-        r[3] = fmaf(-be.y, r[3], bt.y * vb.y);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd = fmaf(r[e], 0.f, odd);
+    for (int nt = 0; nt < kBlocks; ++nt) {
+      const float2 va = unpack16<T>(vw[nt / 2][2 * (nt & 1)]), vb = unpack16<T>(vw[nt / 2][2 * (nt & 1) + 1]);
+      float (&r)[4] = R[nt];
+      r[0] = fmaf(-be[nt].x, r[0], bt[nt].x * va.x);
+      r[1] = fmaf(-be[nt].y, r[1], bt[nt].y * va.y);
+      r[2] = fmaf(-be[nt].x, r[2], bt[nt].x * vb.x);
+      r[3] = fmaf(-be[nt].y, r[3], bt[nt].y * vb.y);
+      if (live < kC) {                                         // rows of no token (v there is the next request's)
+        const int tok = nt * 8 + 2 * t;
+        if (tok >= live) r[0] = r[2] = 0.f;
+        if (tok + 1 >= live) r[1] = r[3] = 0.f;
       }
+      odd[nt] = fmaf(r[0], 0.f, r[1] * 0.f) + fmaf(r[2], 0.f, r[3] * 0.f);
     }
     // A value that is not finite reaches its own row from its token on, and nothing else: the products
     // below would carry it, through their zeros, to tokens before it. It is taken out of them, and
     // what it reaches is set to NaN afterwards.
     int lost[2] = {kC, kC};                                    // rows gid, gid + 8: the first such token
-    const bool any_lost = __any_sync(0xffffffffu, odd != 0.f);
-    if (any_lost) {
-#pragma unroll
-      for (int nt = kBlocks - 1; nt >= 0; --nt)
-#pragma unroll
-        for (int e = 3; e >= 0; --e)
-          if (!isfinite(R[nt][e])) {
-            R[nt][e] = 0.f;
-            lost[e >> 1] = min(lost[e >> 1], nt * 8 + 2 * t + (e & 1));
-          }
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        lost[z] = min(lost[z], __shfl_xor_sync(0xffffffffu, lost[z], 1));
-        lost[z] = min(lost[z], __shfl_xor_sync(0xffffffffu, lost[z], 2));
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < kBlocks; ++nt) operand(R[nt], hi[nt], lo[nt]);
-
-    // U = T (...)
-    float U[kBlocks][4] = {};
-#pragma unroll
-    for (int jb = 0; jb < kBlocks; ++jb)
-#pragma unroll
-      for (int nt = jb; nt < kBlocks; ++nt) {
-        const float4 f = tf[(nt * (nt + 1) / 2 + jb) * 32];
-        mma_tf32(U[nt], hi[jb], f.z, f.w);
-        mma_tf32(U[nt], lo[jb], f.x, f.y);
-        mma_tf32(U[nt], hi[jb], f.x, f.y);
-      }
-    if (any_lost) {
+    const bool any_lost = __any_sync(0xffffffffu, (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f);
+    const auto take_out = [&](float (&x)[kBlocks][4]) {
 #pragma unroll
       for (int nt = 0; nt < kBlocks; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!isfinite(U[nt][e])) {                           // (T's own entries, or an overflow)
-            U[nt][e] = 0.f;
+          if (!isfinite(x[nt][e])) {
+            x[nt][e] = 0.f;
             lost[e >> 1] = min(lost[e >> 1], nt * 8 + 2 * t + (e & 1));
           }
 #pragma unroll
@@ -580,62 +702,68 @@ __global__ void __launch_bounds__(64 * KS) gdn_scan_kernel(const cfb_gdn_args g,
         lost[z] = min(lost[z], __shfl_xor_sync(0xffffffffu, lost[z], 1));
         lost[z] = min(lost[z], __shfl_xor_sync(0xffffffffu, lost[z], 2));
       }
-    }
+    };
+    if (any_lost) take_out(R);
+#pragma unroll
+    for (int nt = 0; nt < kBlocks; ++nt) operand(R[nt], hi[nt], lo[nt]);
 
-    // o = e^G scale rq (S q) + P U
+    // U = T (...)
+    float U[kBlocks][4] = {}, Ul[kBlocks][4] = {}, Um[kBlocks][4] = {};
 #pragma unroll
-    for (int jb = 0; jb < kBlocks; ++jb) operand(U[jb], hi[jb], lo[jb]);
+    for (int jb = 0; jb < kBlocks; ++jb)
 #pragma unroll
-    for (int x = 0; x < kOut; ++x) {
-      const int nt = o0 + x;
-      const float2 f = *reinterpret_cast<const float2*>(vec + 3 * kC + nt * 8 + 2 * t);
-      O[x][0] *= f.x; O[x][1] *= f.y; O[x][2] *= f.x; O[x][3] *= f.y;
-#pragma unroll
-      for (int jb = 0; jb < kBlocks; ++jb) {
-        if (jb > nt) break;
-        const float4 p = pf[(nt * (nt + 1) / 2 + jb) * 32];
-        if (kFine) {
-          mma_tf32(O[x], hi[jb], p.z, p.w);
-          mma_tf32(O[x], lo[jb], p.x, p.y);
-        }
-        mma_tf32(O[x], hi[jb], p.x, p.y);
+      for (int nt = jb; nt < kBlocks; ++nt) {
+        const float4 f = tw[nt * (nt + 1) / 2 + jb];
+        mma_tf32(U[nt], hi[jb], f.x, f.y);
+        mma_tf32(Ul[nt], lo[jb], f.x, f.y);
+        mma_tf32(Um[nt], hi[jb], f.z, f.w);
       }
-      if (any_lost) {
+    uint32_t kt[2][4];
+    ldmatrix4_t(kt[0], block(at, ks * NJ));
+    ldmatrix4_t(kt[1], block(at, ks * NJ + 1));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (nt * 8 + 2 * t + (e & 1) >= lost[e >> 1]) O[x][e] = __int_as_float(0x7fc00000);
-      }
-      // rows to tokens: lane (gid, t) then holds token gid, value rows 2t and 2t + 1
-      const int tok = first + c * kC + nt * 8 + gid;
-      const uint32_t a = transpose8(pack16<T>(O[x][0], O[x][1])), bb = transpose8(pack16<T>(O[x][2], O[x][3]));
-      if (tok < end) {
-        T* out = static_cast<T*>(g.o) + (long long)tok * g.o_stride + (long long)hv * g.V + v0 + vt * 16 + 2 * t;
-        *reinterpret_cast<uint32_t*>(out) = a;
-        *reinterpret_cast<uint32_t*>(out + 8) = bb;
-      }
+    for (int nt = 0; nt < kBlocks; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) U[nt][e] += Ul[nt][e] + Um[nt][e];
+    if (any_lost) take_out(U);                                 // (T's own entries, or an overflow)
+    if (ks == 0) {
+#pragma unroll
+      for (int nt = 0; nt < kBlocks; ++nt)
+        reinterpret_cast<float4*>(hand + Lay::off_u)[nt * 32 + lane] = make_float4(U[nt][0], U[nt][1], U[nt][2], U[nt][3]);
+      reinterpret_cast<int2*>(hand + Lay::off_lost)[lane] = make_int2(lost[0], lost[1]);
     }
+    bar_arrive(hand_bar + (c & 1), kHandThreads);
 
     // S = e^{G_C} S + (e^{G_C-G} r U) K
 #pragma unroll
     for (int nt = 0; nt < kBlocks; ++nt) {
-      const float2 f = *reinterpret_cast<const float2*>(vec + 2 * kC + nt * 8 + 2 * t);
-      U[nt][0] *= f.x; U[nt][1] *= f.y; U[nt][2] *= f.x; U[nt][3] *= f.y;
+      U[nt][0] *= eg[nt].x; U[nt][1] *= eg[nt].y; U[nt][2] *= eg[nt].x; U[nt][3] *= eg[nt].y;
       operand(U[nt], hi[nt], lo[nt]);
     }
-    const float dec = vec[4 * kC];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      uint32_t kw[4];
-      ldmatrix4_t(kw, row_at + j * 16);
-      float acc[4] = {}, accl[4] = {};
+    for (int j = 0; j < NJ; j += 2) {                          // four sums side by side cover a product's latency
+      float acc[2][4] = {}, accl[2][4] = {};
+      uint32_t now[2][4];
 #pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt) {
-        const float2 k2 = unpack16<T>(kw[nt]);
-        mma_tf32(acc, hi[nt], k2.x, k2.y);
-        mma_tf32(accl, lo[nt], k2.x, k2.y);
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) now[z][e] = kt[z][e];
+      if (j + 2 < NJ) {
+        ldmatrix4_t(kt[0], block(at, ks * NJ + j + 2));
+        ldmatrix4_t(kt[1], block(at, ks * NJ + j + 3));
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) S[j][e] = fmaf(S[j][e], dec, acc[e] + accl[e]);
+      for (int nt = 0; nt < kBlocks; ++nt)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const float2 k2 = unpack16<T>(now[z][nt]);
+          mma_tf32(acc[z], hi[nt], k2.x, k2.y);
+          mma_tf32(accl[z], lo[nt], k2.x, k2.y);
+        }
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[j + z][e] = fmaf(S[j + z][e], dec, acc[z][e] + accl[z][e]);
     }
     if (any_lost) {
 #pragma unroll
@@ -644,11 +772,21 @@ __global__ void __launch_bounds__(64 * KS) gdn_scan_kernel(const cfb_gdn_args g,
         for (int e = 0; e < 4; ++e)
           if (lost[e >> 1] < kC) S[j][e] = __int_as_float(0x7fc00000);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[c % kScanStages]);
   }
-
+  // (hand-over buffers that the output warps have freed and nobody will wait for)
+  for (int c = max(chunks, 2); c < chunks + 2; ++c) bar_sync(free_bar + (c & 1), kHandThreads);
+  if (*is_dead) {
+    if (lane == 0) *err = DEV_TIMEOUT_FULL;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[j][e] = __int_as_float(0x7fc00000);
+  }
   const int to = g.out_slot[b];
   if (to >= 0 && to < g.slots) {
-    float* dst = g.state_out + to * g.slot_stride + ((long long)hv * g.V + v0 + vt * 16 + gid) * kK + ks * NJ * 8 + 2 * t;
+    float* dst = g.state_out + to * g.slot_stride + state_at;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(S[j][0], S[j][1]);
@@ -681,27 +819,47 @@ void launch_walk(const cfb_gdn_args& g, const int32_t* cu, int total, int B, cud
   else gdn_walk_kernel<__nv_bfloat16><<<grid, kStepThreads, 0, st>>>(g, cu, total);
 }
 
+constexpr size_t kErrBytes = 256;                              // the device error word, at the workspace's start
 int chunk_slots(int T, int B) { return T / kC + B; }
 
-template <typename T, int KS>
-cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, cudaStream_t st) {
-  constexpr int bytes = kScanStages * ScanStage::bytes;
-  if (cudaFuncSetAttribute(gdn_scan_kernel<T, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+// q or k [T, H, 128] as [head][half][token][64 columns], v [T, HV, V] as [head][token][columns]
+bool key_map(CUtensorMap* map, const void* base, int64_t stride, int total, int heads) {
+  const cuuint64_t dims[4] = {64, (cuuint64_t)total, 2, (cuuint64_t)heads}, strides[3] = {(cuuint64_t)stride * 2, 128, 256};
+  const cuuint32_t box[4] = {64, kC, 2, 1}, step[4] = {1, 1, 1, 1};
+  return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool value_map(CUtensorMap* map, const void* base, int64_t stride, int total, int heads, int V) {
+  const cuuint64_t dims[3] = {(cuuint64_t)V, (cuuint64_t)total, (cuuint64_t)heads}, strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)V * 2};
+  const cuuint32_t box[3] = {kScanRows, kC, 1}, step[3] = {1, 1, 1};
+  return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, int* err, cudaStream_t st) {
+  if (cudaFuncSetAttribute(gdn_scan_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Scan<T>::bytes) != cudaSuccess)
     return cfb_launch_status("gdn_scan_kernel attribute");
+  CUtensorMap q, k, v;
+  if (!tensor_map_encoder()) return cfb_launch_status("cuTensorMapEncodeTiled");
+  if (!key_map(&q, g.q, g.q_stride, total, g.H) || !key_map(&k, g.k, g.k_stride, total, g.H) ||
+      !value_map(&v, g.v, g.v_stride, total, g.HV, g.V))
+    return CFB_ERR_INVALID_ARG;
   const dim3 grid((unsigned)(g.V / kScanRows), (unsigned)g.HV, (unsigned)B);
-  gdn_scan_kernel<T, KS><<<grid, 64 * KS, bytes, st>>>(g, cu, total, ws);
+  gdn_scan_kernel<T><<<grid, kScanThreads, Scan<T>::bytes, st>>>(g, cu, total, ws, err, q, k, v);
   return cfb_launch_status("gdn_scan_kernel");
 }
 template <typename T>
-cfb_status launch_chunks(const cfb_gdn_args& g, const int32_t* cu, int total, int B, float* ws, cudaStream_t st) {
-  gdn_prep_kernel<T><<<dim3((unsigned)chunk_slots(total, B), (unsigned)g.HV), 64, 0, st>>>(g, cu, total, B, ws);
+cfb_status launch_chunks(const cfb_gdn_args& g, const int32_t* cu, int total, int B, float* ws, int* err, cudaStream_t st) {
+  if (total == 0) {                                            // states only
+    launch_walk(g, cu, total, B, st);
+    return cfb_launch_status("gdn_walk_kernel");
+  }
+  gdn_prep_kernel<T><<<dim3((unsigned)chunk_slots(total, B), (unsigned)g.HV), 64, 0, st>>>(g, cu, total, B, ws, err);
   if (const cfb_status s = cfb_launch_status("gdn_prep_kernel")) return s;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return cfb_launch_status("cudaDeviceGetAttribute");
-  // KS = 1 has two warps a CTA for an SM's four quarters
-  const bool wide = (long long)(g.V / kScanRows) * g.HV * B * 2 <= 4ll * sms;
-  return wide ? launch_scan<T, 2>(g, cu, total, B, ws, st) : launch_scan<T, 1>(g, cu, total, B, ws, st);
+  return launch_scan<T>(g, cu, total, B, ws, err, st);
 }
 
 }  // namespace
@@ -715,7 +873,7 @@ extern "C" cfb_status cfb_gdn_step(const cfb_gdn_args* g, int B, void* stream) {
 
 extern "C" size_t cfb_gdn_chunk_workspace(int T, int B, int HV) {
   if (T < 0 || B <= 0 || HV <= 0) return 0;
-  return (size_t)chunk_slots(T, B) * HV * kPrepFloats * sizeof(float);
+  return kErrBytes + (size_t)chunk_slots(T, B) * HV * kPrepFloats * sizeof(float);
 }
 
 extern "C" cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, int T, int B, void* ws, size_t ws_bytes,
@@ -725,7 +883,14 @@ extern "C" cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, in
   if (T < 0 || !cu || !ws) return CFB_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_gdn_chunk_workspace(T, B, g->HV)) return CFB_ERR_WORKSPACE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* const prep = static_cast<float*>(ws);
-  if (g->dtype == DT_F16) return launch_chunks<__half>(*g, cu, T, B, prep, st);
-  return launch_chunks<__nv_bfloat16>(*g, cu, T, B, prep, st);
+  int* const err = static_cast<int*>(ws);
+  float* const prep = reinterpret_cast<float*>(static_cast<char*>(ws) + kErrBytes);
+  if (g->dtype == DT_F16) return launch_chunks<__half>(*g, cu, T, B, prep, err, st);
+  return launch_chunks<__nv_bfloat16>(*g, cu, T, B, prep, err, st);
+}
+
+extern "C" cfb_status cfb_gdn_chunk_error(const void* ws, int* device_error) {
+  if (!ws || !device_error) return CFB_ERR_INVALID_ARG;
+  if (cudaMemcpy(device_error, ws, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return cfb_launch_status("cfb_gdn_chunk_error");
+  return CFB_OK;
 }

@@ -251,6 +251,15 @@ class ChunkedGdn:
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
 
+    def check(self) -> None:
+        """Raises if a device-side wait of the last call (with tokens) expired (its outputs are then
+        invalid, its states NaN). Waits for the GPU."""
+        err = C.c_int(0)
+        torch.cuda.synchronize(self.device)
+        _lib.check(self.lib.cfb_gdn_chunk_error(self.ws_ptr, C.byref(err)), "cfb_gdn_chunk_error")
+        if err.value:
+            raise _lib.CfbError(f"ChunkedGdn: device error {err.value} (a bounded wait expired); outputs are invalid")
+
     def __call__(self, A_log, dt_bias, a, b, q, k, v, o, state, cu_seqlens, init_slot, out_slot, *, scale: float,
                  out_state=None, stream=None) -> None:
         """Request b's tokens are the rows [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [B + 1], on the

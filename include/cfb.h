@@ -481,6 +481,9 @@ cfb_status cfb_gdn_step(const cfb_gdn_args* g, int B, void* stream);
 size_t cfb_gdn_chunk_workspace(int T, int B, int HV);
 cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, int T, int B, void* ws,
                          size_t ws_bytes, void* stream);
+/* Synchronous: the device error word of the last cfb_gdn_chunk call with T > 0 and this workspace: 0
+ * if it completed, else a bounded device-side wait expired; its outputs are invalid (states NaN). */
+cfb_status cfb_gdn_chunk_error(const void* ws, int* device_error);
 
 /* ---- the per-request context ring -------------------------------------------------------------
  * The window of the last C target hidden states each request's draft is conditioned on
