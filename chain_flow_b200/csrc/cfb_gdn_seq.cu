@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
 //   8    one lane issues the copies of the chunks to come: K and Q as [64 columns][32 tokens] 128-byte-
 //        swizzled boxes, V as a plain box, T, P and the vectors in one piece. (The same copies by 16-byte
 //        cp.async kept a warp busy for longer than a chunk takes.)
-constexpr int kScanStages = 3, kTiles = 2, kStateWarps = 2 * kTiles, kOutWarps = 2 * kTiles, kScanRows = 16 * kTiles;
+constexpr int kScanStages = 4, kTiles = 2, kStateWarps = 2 * kTiles, kOutWarps = 2 * kTiles, kScanRows = 16 * kTiles;
 constexpr int kScanThreads = (kStateWarps + kOutWarps + 1) * 32;
 constexpr int kHandThreads = 4 * 32;                           // a tile's two state and two output warps
 template <typename T>
@@ -611,22 +611,6 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
       __syncwarp();
     }
 
-    // S k of the chunk's tokens
-    float R[kBlocks][4] = {}, Rl[kBlocks][4] = {};
-    uint32_t kw[2][4];                                         // a block ahead
-    ldmatrix4(kw[0], block(at, ks * NJ));
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      float hi[4], lo[4];
-      operand(S[j], hi, lo);
-      if (j + 1 < NJ) ldmatrix4(kw[(j + 1) & 1], block(at, ks * NJ + j + 1));
-#pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt) {
-        const float2 k2 = unpack16<T>(kw[j & 1][nt]);
-        mma_tf32(R[nt], hi, k2.x, k2.y);
-        mma_tf32(Rl[nt], lo, k2.x, k2.y);
-      }
-    }
     // what the next steps read, ahead of them
     uint32_t vw[kBlocks / 2][4];
 #pragma unroll
@@ -643,6 +627,23 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
 #pragma unroll
     for (int x = 0; x < kPairs; ++x) tw[x] = tf[x * 32];
     const float dec = vec[4 * kC];
+
+    // S k of the chunk's tokens
+    float R[kBlocks][4] = {}, Rl[kBlocks][4] = {};
+    uint32_t kw[2][4];                                         // a block ahead
+    ldmatrix4(kw[0], block(at, ks * NJ));
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float hi[4], lo[4];
+      operand(S[j], hi, lo);
+      if (j + 1 < NJ) ldmatrix4(kw[(j + 1) & 1], block(at, ks * NJ + j + 1));
+#pragma unroll
+      for (int nt = 0; nt < kBlocks; ++nt) {
+        const float2 k2 = unpack16<T>(kw[j & 1][nt]);
+        mma_tf32(R[nt], hi, k2.x, k2.y);
+        mma_tf32(Rl[nt], lo, k2.x, k2.y);
+      }
+    }
     // both halves need all of S k (two buffers in turn: the next chunk's barrier comes between a value's
     // reading and its overwriting)
     {
