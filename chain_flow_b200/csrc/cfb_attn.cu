@@ -1024,14 +1024,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
   if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// CTAs of a launch (without a device, as in a size computed on the host alone: a B200's)
 int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      sms <= 0) {
-    cudaGetLastError();
-    return 148;
-  }
-  return sms;
+  const int n = device_sms();
+  return n > 0 ? n : 148;
 }
 size_t desc_bytes(int grid) { return ((size_t)grid * sizeof(Desc) + 255) / 256 * 256; }
 
@@ -1058,7 +1054,7 @@ bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
 
 template <typename T, int D, int SRC>
 cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
-  if (cudaFuncSetAttribute(attn_kernel<T, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<D, SRC>::bytes) != cudaSuccess)
+  if (allow_smem<attn_kernel<T, D, SRC>>((int)Layout<D, SRC>::bytes) != cudaSuccess)
     return cfb_launch_status("attn_kernel attribute");
   attn_kernel<T, D, SRC><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
   if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;

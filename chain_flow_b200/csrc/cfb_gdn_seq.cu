@@ -841,7 +841,7 @@ bool value_map(CUtensorMap* map, const void* base, int64_t stride, int total, in
 
 template <typename T>
 cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, int* err, cudaStream_t st) {
-  if (cudaFuncSetAttribute(gdn_scan_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Scan<T>::bytes) != cudaSuccess)
+  if (allow_smem<gdn_scan_kernel<T>>(Scan<T>::bytes) != cudaSuccess)
     return cfb_launch_status("gdn_scan_kernel attribute");
   CUtensorMap q, k, v;
   if (!tensor_map_encoder()) return cfb_launch_status("cuTensorMapEncodeTiled");

@@ -9,10 +9,13 @@
 // row's elements are each rounded once, to nearest even.
 //
 // Bound: HBM (a step's rows) or launch latency (a decode step's). A row is independent of every
-// other, so a group of D / 8 lanes holds one row in registers, 8 elements (16 bytes) a lane: one
-// pass over the data, one shuffle reduction of log2(D / 8) steps for the maximum, one store.
+// other, so a group of D / 8 lanes holds a row in registers, 8 elements a lane: one pass over the data,
+// one shuffle reduction for the maximum, one store. A group takes kRows rows, neighbours in the order
+// [token][k or v][head], and has all their loads in flight before the first is used; a row's data is
+// loaded beside its slot, not after it.
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "cfb_types.cuh"
 
@@ -20,7 +23,8 @@ using namespace cfb;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kRows = 4;
 constexpr float kFloor = 5.9604644775390625e-8f;      // 2^-24
 constexpr float kMaxCode = 448.f;
 
@@ -45,123 +49,141 @@ __device__ __forceinline__ bool locate(const cfb_kv_cache& c, long long slot, in
   return true;
 }
 
-// row index r over [T][k or v][kv_heads]
-__device__ __forceinline__ void row_of(const cfb_kv_cache& c, long long r, long long* t, int* which, int* h) {
-  const long long per = 2ll * c.kv_heads;
-  *t = r / per;
-  const int x = (int)(r - *t * per);
-  *which = x >= c.kv_heads;
-  *h = x - *which * c.kv_heads;
+// row r over [T][k or v][kv_heads]
+__device__ __forceinline__ void row_of(const cfb_kv_cache& c, unsigned r, long long* t, int* which, int* h) {
+  const unsigned per = 2u * (unsigned)c.kv_heads, q = r / per, x = r - q * per;
+  *t = q;
+  *which = x >= (unsigned)c.kv_heads;
+  *h = (int)x - *which * c.kv_heads;
 }
 
 template <typename T, int D, bool QUANT>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const cfb_kv_cache c, const Rows in, const int64_t* slots,
-                                                            long long rows) {
+                                                            unsigned rows) {
   constexpr int kLanes = D / 8;                        // lanes a row
-  const long long r = (long long)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const unsigned r0 = (blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes) * kRows;
   const int lane = threadIdx.x % kLanes;
-  // whole warps stay for the shuffles
-  long long t = 0;
-  int which = 0, h = 0;
-  const bool live = r < rows;
-  if (live) row_of(c, r, &t, &which, &h);
-  long long row = 0, sc = 0;
-  const bool put = live && locate(c, slots[t], h, &row, &sc);
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (put) {
-    const T* src = which ? static_cast<const T*>(in.v) + t * in.sv_t + h * in.sv_h
-                         : static_cast<const T*>(in.k) + t * in.sk_t + h * in.sk_h;
-    w = __ldg(reinterpret_cast<const uint4*>(src) + lane);
+  uint4 w[kRows];
+  long long slot[kRows];
+  int which[kRows], h[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    w[i] = make_uint4(0, 0, 0, 0);
+    slot[i] = -1;
+    which[i] = h[i] = 0;
+    if (r0 + i < rows) {
+      long long t;
+      row_of(c, r0 + i, &t, &which[i], &h[i]);
+      slot[i] = __ldg(slots + t);
+      const T* src = which[i] ? static_cast<const T*>(in.v) + t * in.sv_t + h[i] * in.sv_h
+                              : static_cast<const T*>(in.k) + t * in.sk_t + h[i] * in.sk_h;
+      w[i] = __ldg(reinterpret_cast<const uint4*>(src) + lane);
+    }
   }
-  if constexpr (!QUANT) {
-    if (put) reinterpret_cast<uint4*>(static_cast<T*>(which ? c.v : c.k) + row)[lane] = w;
-  } else {
-    float x[8];
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack16<T>(ws[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+  for (int i = 0; i < kRows; ++i) {
+    long long row = 0, sc = 0;
+    const bool put = locate(c, slot[i], h[i], &row, &sc);
+    if constexpr (!QUANT) {
+      if (put) reinterpret_cast<uint4*>(static_cast<T*>(which[i] ? c.v : c.k) + row)[lane] = w[i];
+    } else {
+      float x[8];
+      const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      float m = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack16<T>(ws[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+        m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+        bad |= !isfinite(f.x) || !isfinite(f.y);
+      }
+      if (bad) m = INFINITY;                           // fmaxf drops NaN: an infinity carries it
+#pragma unroll
+      for (int off = kLanes / 2; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off, kLanes));
+      bad = isinf(m);
+      m = fmaxf(m, kFloor);
+      const float inv = kMaxCode / m;
+      uint2 q = make_uint2(0, 0);
+      if (!bad) {
+        uint32_t p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p[e] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * e] * inv, x[2 * e + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        q = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+      }
+      if (put) {
+        reinterpret_cast<uint2*>(static_cast<uint8_t*>(which[i] ? c.v : c.k) + row)[lane] = q;
+        if (lane == 0) (which[i] ? c.v_scale : c.k_scale)[sc] = bad ? __int_as_float(0x7fc00000) : m / kMaxCode;
+      }
     }
-    float m = 0.f;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = fmaxf(m, fabsf(x[i]));
-      bad |= !isfinite(x[i]);
-    }
-    if (bad) m = INFINITY;                             // fmaxf drops NaN: an infinity carries it
-#pragma unroll
-    for (int off = kLanes / 2; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off, kLanes));
-    if (!put) return;
-    bad = isinf(m);
-    m = fmaxf(m, kFloor);
-    const float inv = kMaxCode / m;
-    uint2 q = make_uint2(0, 0);
-    if (!bad) {
-      uint32_t p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        p[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      q = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
-    }
-    reinterpret_cast<uint2*>(static_cast<uint8_t*>(which ? c.v : c.k) + row)[lane] = q;
-    if (lane == 0) (which ? c.v_scale : c.k_scale)[sc] = bad ? __int_as_float(0x7fc00000) : m / kMaxCode;
   }
 }
 
 // C: stored type (uint8_t = e4m3), T: type read
 template <typename C, typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const cfb_kv_cache c, const int64_t* slots, const Rows out,
-                                                           long long rows) {
+                                                           unsigned rows) {
   constexpr int kLanes = D / 8;
-  const long long r = (long long)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  using Word = typename std::conditional<sizeof(C) == 1, uint2, uint4>::type;
+  const unsigned r0 = (blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes) * kRows;
   const int lane = threadIdx.x % kLanes;
-  if (r >= rows) return;
-  long long t, row, sc;
-  int which, h;
-  row_of(c, r, &t, &which, &h);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (locate(c, slots[t], h, &row, &sc)) {
-    const C* src = static_cast<const C*>(which ? c.v : c.k) + row;
-    if constexpr (sizeof(C) == 1) {
-      const float s = (which ? c.v_scale : c.k_scale)[sc];
-      const uint2 w = reinterpret_cast<const uint2*>(src)[lane];
-      const uint32_t ws[2] = {w.x, w.y};
+  Word w[kRows];
+  float scale[kRows];
+  T* dst[kRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 f = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(ws[i / 2] >> (16 * (i & 1))), __NV_E4M3));
-        x[2 * i] = __low2float(f) * s;
-        x[2 * i + 1] = __high2float(f) * s;
-      }
-    } else {
-      const uint4 w = reinterpret_cast<const uint4*>(src)[lane];
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack16<C>(ws[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-      }
+  for (int i = 0; i < kRows; ++i) {
+    w[i] = Word{};
+    scale[i] = 0.f;
+    dst[i] = nullptr;
+    if (r0 + i >= rows) continue;
+    long long t, row, sc;
+    int which, h;
+    row_of(c, r0 + i, &t, &which, &h);
+    dst[i] = which ? static_cast<T*>(out.v) + t * out.sv_t + h * out.sv_h : static_cast<T*>(out.k) + t * out.sk_t + h * out.sk_h;
+    if (locate(c, __ldg(slots + t), h, &row, &sc)) {
+      w[i] = __ldg(reinterpret_cast<const Word*>(static_cast<const C*>(which ? c.v : c.k) + row) + lane);
+      if constexpr (sizeof(C) == 1) scale[i] = __ldg((which ? c.v_scale : c.k_scale) + sc);
     }
   }
-  T* dst = which ? static_cast<T*>(out.v) + t * out.sv_t + h * out.sv_h : static_cast<T*>(out.k) + t * out.sk_t + h * out.sk_h;
-  if constexpr (sizeof(T) == 4) {
-    float4* d = reinterpret_cast<float4*>(dst) + 2 * lane;
-    d[0] = make_float4(x[0], x[1], x[2], x[3]);
-    d[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    reinterpret_cast<uint4*>(dst)[lane] =
-        make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    if (!dst[i]) continue;
+    float x[8];
+    if constexpr (sizeof(C) == 1) {
+      const uint32_t ws[2] = {w[i].x, w[i].y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __half2 f = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(ws[e / 2] >> (16 * (e & 1))), __NV_E4M3));
+        x[2 * e] = __low2float(f) * scale[i];
+        x[2 * e + 1] = __high2float(f) * scale[i];
+      }
+    } else {
+      const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack16<C>(ws[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+    }
+    if constexpr (sizeof(T) == 4) {
+      float4* d = reinterpret_cast<float4*>(dst[i]) + 2 * lane;
+      d[0] = make_float4(x[0], x[1], x[2], x[3]);
+      d[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      reinterpret_cast<uint4*>(dst[i])[lane] =
+          make_uint4(pack16<T>(x[0], x[1]), pack16<T>(x[2], x[3]), pack16<T>(x[4], x[5]), pack16<T>(x[6], x[7]));
+    }
   }
 }
 
 template <typename T, bool QUANT>
 void launch_write(const cfb_kv_cache& c, const Rows& in, const int64_t* slots, long long rows, cudaStream_t st) {
   const auto go = [&](auto kernel, int lanes) {
-    const long long per = kThreads / lanes;
-    kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, st>>>(c, in, slots, rows);
+    const long long per = kThreads / lanes * kRows;
+    kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, st>>>(c, in, slots, (unsigned)rows);
   };
   if (c.dim == 64) go(kv_write_kernel<T, 64, QUANT>, 8);
   else if (c.dim == 128) go(kv_write_kernel<T, 128, QUANT>, 16);
@@ -171,8 +193,8 @@ void launch_write(const cfb_kv_cache& c, const Rows& in, const int64_t* slots, l
 template <typename C, typename T>
 void launch_read(const cfb_kv_cache& c, const int64_t* slots, const Rows& out, long long rows, cudaStream_t st) {
   const auto go = [&](auto kernel, int lanes) {
-    const long long per = kThreads / lanes;
-    kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, st>>>(c, slots, out, rows);
+    const long long per = kThreads / lanes * kRows;
+    kernel<<<(unsigned)((rows + per - 1) / per), kThreads, 0, st>>>(c, slots, out, (unsigned)rows);
   };
   if (c.dim == 64) go(kv_read_kernel<C, T, 64>, 8);
   else if (c.dim == 128) go(kv_read_kernel<C, T, 128>, 16);

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/cfb.h"
@@ -84,6 +85,33 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
+// host: the current device's SMs (0 where there is none: no launch will follow), and a kernel's dynamic
+// shared memory allowed on it, both asked of the runtime once a device
+inline int device_sms() {
+  static std::atomic<int> sms[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 64 && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 64) sms[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+template <auto Kernel>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
 // host: base and row strides (in elements of `size` bytes) keep every row 16-byte aligned
 inline bool rows_aligned(const void* p, int size, int64_t s0, int64_t s1) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (s0 * size) % 16 == 0 && (s1 * size) % 16 == 0;
