@@ -8,7 +8,12 @@
 // Over an e4m3 cache k_j = ks_j kc_j and v_j = vs_j vc_j (codes and scales), and
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
-// so the weights stay at most 1, whatever the scales, and the codes enter the products exactly.
+// so the weights stay at most 1, whatever the scales. The codes go into the products as they are, on the
+// 8-bit tensor path, and the other operand is cut into e4m3 pieces of 4 bits each: x = x1 + x2 (+ x3), two
+// pieces over bf16 (8 bits) and three over fp16 (11). A query row is first brought to a largest element of
+// 128 to 256 by a power of two, and the weights to at most 2^8.5, so that what e4m3's smallest step (2^-9)
+// loses of a small element is 2^-17 of the largest. (Widening the codes to 16 bits instead took three times
+// as long: the widened tiles' way through shared memory, not the conversion, was the bound.)
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
 #include <algorithm>
@@ -32,20 +37,25 @@ namespace {
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
 constexpr int kM = 128, kKeys = 64;
-constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4, kLoadThreads = kLoadWarps * 32;
+constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4;
 constexpr int kScaleStages = 4;
 constexpr uint32_t kScaleBytes = kKeys * 12;   // a unit's scales: [64] (k's with the softmax's, log2 v's), [64] 1 / v's
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kRescaleAt = 8.f;         // o is rescaled only when the maximum has grown by 2^8
+// Weights are 2^(x - m). m is set to the maximum less kLift, and moved again (o rescaled) only when the
+// maximum has grown by 2^kSlack since: over 16-bit rows weights are then at most 2^8, far inside both
+// types; over e4m3 between 2^6.5 and 2^8.5, e4m3's upper end.
+template <bool E4M3> constexpr float kLift = E4M3 ? 6.5f : 0.f;
+template <bool E4M3> constexpr float kSlack = E4M3 ? 2.f : 8.f;
 
 // How the cache's rows come in: 16-bit or e4m3, by TMA where boxes of 8 rows or more tile both the pages
 // and the units (gcd(page size, 64) >= 8), else row by row.
 enum Source : int { TMA16 = 0, ROWS16 = 1, TMA8 = 2, ROWS8 = 3 };
 __host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
 __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
-// warps 0-7 softmax, 8 products, then: TMA16 two that issue the copies of K and of V; ROWS16 four that copy;
-// TMA8 four that widen and two that issue the copies; ROWS8 four that copy and widen
-constexpr int threads_of(int src) { return (kSoftWarps + 1 + (src == TMA16 ? 2 : src == TMA8 ? kLoadWarps + 2 : kLoadWarps)) * 32; }
+// warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V or four that copy rows, and
+// over e4m3 one that brings the scales
+__host__ __device__ constexpr int load_warps(int src) { return is_tma(src) ? 2 : 4; }
+__host__ __device__ constexpr int threads_of(int src) { return (9 + load_warps(src) + (is_e4m3(src) ? 1 : 0)) * 32; }
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -156,22 +166,25 @@ CFB_DEV float* part_row(float* part, int grid, int cta, int which, int row) {
 }
 template <int D, int SRC>
 struct Layout {
-  // stages of K and of V; an e4m3 unit's codes land in stages of their own
-  static constexpr int kStages = SRC == TMA16 ? (D == 256 ? 3 : 4) : 2, kRaw = SRC == TMA8 ? (D == 256 ? 4 : 8) : 0;
-  static constexpr uint32_t kTile = kKeys * D * 2, kRawTile = kKeys * D;
-  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_raw = 2 * kStages * kTile;
-  static constexpr uint32_t off_scale = off_raw + kRaw * kRawTile;
+  static constexpr int kElem = is_e4m3(SRC) ? 1 : 2;                       // stored bytes an element
+  static constexpr int kRowB = D * kElem < 128 ? 64 : 128, kSlabs = D * kElem / kRowB;   // a slab's row
+  static constexpr int kStages = SRC == TMA16 && D == 256 ? 3 : SRC == ROWS16 ? 2 : 4;
+  static constexpr uint32_t kTile = kKeys * D * kElem;
+  // a third piece of Q over e4m3 that tensor memory has no room for (D = 256) lies in shared memory
+  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_q3 = 2 * kStages * kTile;
+  static constexpr uint32_t off_scale = off_q3 + (is_e4m3(SRC) && D == 256 ? kM * D : 0);
   static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kScaleBytes : 0) + 1024;
   static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
 
-// full / empty: a stage's tile has landed / its product has read it. q_ready: Q is in tensor memory.
-// s_done / o_done: the product S(i) / O += P(i) V(i) has completed. p_full: P(i) is written (and S(i)
-// read). m_set: the rows' maximum after unit i is in shared memory. o_free: the piece's O has been read.
+// full / empty: a stage's tile has landed / its product has read it (sc: a unit's scales). q_ready: Q is in
+// tensor memory. s_done / o_done: the product S(i) / O += P(i) V(i) has completed. p_full: P(i) is written
+// (and S(i) read). m_set: the rows' maximum after unit i is in shared memory. o_free: the piece's O has
+// been read.
 struct Bars {
   uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], s_done[2], p_full[2], o_done[2], o_free,
-      sc_full[kScaleStages], raw_full[8], raw_empty[8], m_set[2][4], swap[4], drain;
+      sc_full[kScaleStages], sc_empty[kScaleStages], m_set[2][4], swap[4], drain;
 };
 
 CFB_DEV void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -202,6 +215,10 @@ CFB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+CFB_DEV void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -209,30 +226,49 @@ CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// D[tmem] (+)= A[tmem] . B[smem], 16-bit A (two elements a column) and B
-// over 64 of the summed dim: four products of 16 in one statement, by one elected lane (one election and
-// one statement for four take less issue time than four), B's descriptor advancing by `step`
-CFB_DEV void mma_ts4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t step, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] . B[smem] over N steps of 32 bytes of the summed dim in one statement, by one elected
+// lane (one election and one statement for four take less issue time than four), B's descriptor advancing
+// by `step`. F8: e4m3, else 16-bit operands.
+template <int N, bool F8>
+CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t step, uint32_t idesc, uint32_t accumulate) {
+#define CFB_TS4(KIND)                                                                                                        \
+  asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%1], %2, %3, q;\n\t"                                       \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %8, %3, 1;\n\t"                                       \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%6], %9, %3, 1;\n\t"                                       \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%7], %10, %3, 1;\n\t}"                                     \
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "r"(tmem_a + 16),            \
+                  "r"(tmem_a + 24), "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step) : "memory")
+#define CFB_TS2(KIND)                                                                                                        \
+  asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%1], %2, %3, q;\n\t"                                       \
+               "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %6, %3, 1;\n\t}"                                      \
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "l"(b + step) : "memory")
+  static_assert(N == 4 || (N == 2 && F8), "steps");
+  if constexpr (!F8) CFB_TS4("f16");
+  else if constexpr (N == 4) CFB_TS4("f8f6f4");
+  else CFB_TS2("f8f6f4");
+#undef CFB_TS4
+#undef CFB_TS2
+}
+// D[tmem] += A[smem] . B[smem], e4m3, over four steps of 32 columns (128-byte rows of both)
+CFB_DEV void mma_ss4_f8_warp(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "setp.ne.b32 q, %4, 0;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%5], %8, %3, 1;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%6], %9, %3, 1;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%7], %10, %3, 1;\n\t}"
-      :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "r"(tmem_a + 16), "r"(tmem_a + 24),
-         "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step)
-      : "memory");
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %4, %7, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %5, %8, %3, 1;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %6, %9, %3, 1;\n\t}"
+      :: "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b + 2), "l"(b + 4), "l"(b + 6) : "memory");
 }
-// 128-byte-swizzled operands: K-major, 8-row groups `group` bytes apart; MN-major, 64-element slabs `slab`
-// and 8-row groups `group` bytes apart
-CFB_DEV uint64_t k_major(uint32_t saddr, uint32_t group) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// swizzled operands of rows of 128 bytes, or of 64: K-major, 8-row groups `group` bytes apart; MN-major, slabs
+// of a row's elements `slab` and 8-row groups `group` bytes apart
+template <int ROWB> CFB_DEV constexpr uint64_t swizzle_bits() { return (1ull << 46) | (ROWB == 128 ? 2ull << 61 : 4ull << 61); }
+template <int ROWB> CFB_DEV uint64_t k_major(uint32_t saddr, uint32_t group) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(group >> 4) << 32) | swizzle_bits<ROWB>();
 }
-CFB_DEV uint64_t mn_major(uint32_t saddr, uint32_t slab, uint32_t group) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
+template <int ROWB> CFB_DEV uint64_t mn_major(uint32_t saddr, uint32_t slab, uint32_t group) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | swizzle_bits<ROWB>();
 }
 template <typename T>
 CFB_DEV constexpr uint32_t type_bits() {          // operand formats of the instruction descriptor
@@ -265,31 +301,24 @@ CFB_DEV long long row_offset(const AttnArgs& A, int b, int kh, int j, long long*
   return (long long)page * A.c.page_stride + kh * A.c.head_stride + off * A.c.slot_stride;
 }
 
-// eight e4m3 codes -> eight elements of T (exact: both types hold every e4m3 value)
-template <typename T> CFB_DEV uint4 widen8(uint32_t lo, uint32_t hi);
-template <> CFB_DEV uint4 widen8<__half>(uint32_t lo, uint32_t hi) {
-  uint4 r;
-  const auto two = [](uint32_t w) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
-    return (uint32_t)h.x | (uint32_t)h.y << 16;
-  };
-  r.x = two(lo & 0xffff); r.y = two(lo >> 16); r.z = two(hi & 0xffff); r.w = two(hi >> 16);
-  return r;
+// Four values as e4m3: the leading piece, and what it leaves. The piece is the value rounded to 4 bits by an
+// integer addition, which the conversion then takes as it is (it rounds only below e4m3's normal range,
+// by at most half its smallest step).
+CFB_DEV uint32_t e4m3_of(const float (&x)[4]) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
 }
-// bf16: the code's exponent and mantissa bits, moved to bf16's places, read as value * 2^-120 (e4m3's
-// bias is 7, bf16's 127; subnormals come out as subnormals), and one exact product undoes that.
-template <> CFB_DEV uint4 widen8<__nv_bfloat16>(uint32_t lo, uint32_t hi) {
-  uint4 r;
-  const auto two = [](uint32_t w, uint32_t pick) {
-    const uint32_t t = __byte_perm(w, 0, pick);                // each half: code << 8
-    const uint32_t x = (t & 0x80008000u) | (t >> 4 & 0x07f007f0u);
-    const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80));   // 2^120
-    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), up);
-    return *reinterpret_cast<const uint32_t*>(&y);
-  };
-  r.x = two(lo, 0x1404); r.y = two(lo, 0x3424); r.z = two(hi, 0x1404); r.w = two(hi, 0x3424);
-  return r;
+CFB_DEV uint32_t take_piece(float (&x)[4]) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i] = __uint_as_float((__float_as_uint(x[i]) + 0x00080000u) & 0xfff00000u);
+    x[i] -= y[i];
+  }
+  return e4m3_of(y);
 }
+template <typename T> constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
 
 // ---- the kernel -----------------------------------------------------------------------------------
 // One CTA per SM. The loading warps (Source) fill, per unit, a K and a V tile: pages are found through
@@ -321,16 +350,15 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_ready, kSoftWarps);
     for (int i = 0; i < kSt; ++i) {
-      mbar_init(&bar.k_full[i], SRC == TMA16 ? 1 : kLoadThreads); mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], SRC == TMA16 ? 1 : kLoadThreads); mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.k_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], 1);
     }
-    for (int i = 0; i < Lay::kRaw; ++i) { mbar_init(&bar.raw_full[i], 1); mbar_init(&bar.raw_empty[i], kLoadWarps); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps / 2); mbar_init(&bar.o_done[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&bar.m_set[i][j], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
-    for (int i = 0; i < kScaleStages; ++i) mbar_init(&bar.sc_full[i], kKeys / 32);
+    for (int i = 0; i < kScaleStages; ++i) { mbar_init(&bar.sc_full[i], 1); mbar_init(&bar.sc_empty[i], kSoftWarps / 2); }
     for (int i = 0; i < 4; ++i) mbar_init(&bar.swap[i], 2);
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
@@ -421,22 +449,74 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       const bool warp_live = pair * 32 < rows;
       bool ok = true;
       // Q to tensor memory, a half of the head dim a group
+      float rowf = c2;                                         // the softmax's scale, with the row's own over e4m3
       if (warp_live) {
-        constexpr int kCols = D == 64 ? 16 : 32, kPieces = kCols / 4, kRounds = D == 256 ? 2 : 1;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (long long)(w.r.t0 + (valid ? tok : 0)) * A.sq_t +
-                                                          (valid ? head : 0) * A.sq_h + half * (D / 2));
-        uint32_t u[kRounds][kCols];
+        const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (long long)(w.r.t0 + (valid ? tok : 0)) * A.sq_t +
+                                                                (valid ? head : 0) * A.sq_h);
+        const auto load = [&](int e) { return valid ? __ldg(src + e) : make_uint4(0, 0, 0, 0); };
+        constexpr int kRounds = D == 256 ? 2 : 1, kWords = D == 64 ? 16 : 32;        // 32-bit words of a round
+        if constexpr (!QUANT) {
+          uint32_t u[kRounds][kWords];
 #pragma unroll
-        for (int e = 0; e < kRounds * kPieces; ++e) {
-          const uint4 y = valid ? __ldg(src + e) : make_uint4(0, 0, 0, 0);
-          uint32_t* z = u[e / kPieces] + 4 * (e % kPieces);
-          z[0] = y.x; z[1] = y.y; z[2] = y.z; z[3] = y.w;
-        }
-        __syncwarp();
+          for (int e = 0; e < kRounds * kWords / 4; ++e) {
+            const uint4 y = load(half * (D / 16) + e);
+            uint32_t* z = u[e / (kWords / 4)] + 4 * (e % (kWords / 4));
+            z[0] = y.x; z[1] = y.y; z[2] = y.z; z[3] = y.w;
+          }
+          __syncwarp();
 #pragma unroll
-        for (int c = 0; c < kRounds; ++c) {
-          if constexpr (kCols == 32) tmem_st32(tw + Lay::q_col + half * (D / 4) + c * 32, u[c]);
-          else tmem_st16(tw + Lay::q_col + half * (D / 4), u[c]);
+          for (int c = 0; c < kRounds; ++c) {
+            if constexpr (kWords == 32) tmem_st32(tw + Lay::q_col + half * (D / 4) + c * 32, u[c]);
+            else tmem_st16(tw + Lay::q_col + half * (D / 4), u[c]);
+          }
+        } else {
+          // the row's largest magnitude (patterns order like integers; what is not finite is largest)
+          constexpr uint32_t kMag = 0x7fff7fffu, kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+          uint32_t top = 0;
+#pragma unroll 8
+          for (int e = 0; e < D / 8; ++e) {
+            const uint4 y = load(e);
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(y.x & kMag, y.y & kMag), __vmaxu2(y.z & kMag, y.w & kMag)));
+          }
+          top = max(top & 0xffffu, top >> 16);
+          // 2^(7 - exponent): the largest element lands in [128, 256)
+          const int e2 = min(max((int)(__float_as_uint(unpack16<T>(top).x) >> 23) - 127, -100), 127);
+          const float up = __uint_as_float((uint32_t)(127 + 7 - e2) << 23);
+          rowf = top >= kInf ? __int_as_float(0x7fc00000) : c2 * __uint_as_float((uint32_t)(127 + e2 - 7) << 23);
+          // 64 elements a round: 16 words of each piece (32 elements, 8 words where D = 64)
+          constexpr int kOct = D == 64 ? 4 : 8;                // 16-byte loads of a round
+#pragma unroll
+          for (int c = 0; c < (D == 64 ? 1 : D / 128); ++c) {
+            uint32_t piece[kPieces<T>][2 * kOct];
+#pragma unroll
+            for (int e = 0; e < kOct; ++e) {
+              const uint4 y = load(half * (D / 16) + c * kOct + e);
+              const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float2 f = unpack16<T>(ys[2 * z]), g = unpack16<T>(ys[2 * z + 1]);
+                float x[4] = {f.x * up, f.y * up, g.x * up, g.y * up};
+#pragma unroll
+                for (int n = 0; n < kPieces<T> - 1; ++n) piece[n][2 * e + z] = take_piece(x);
+                piece[kPieces<T> - 1][2 * e + z] = e4m3_of(x);
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < kPieces<T>; ++n) {
+              const uint32_t col = tw + Lay::q_col + n * (D / 4) + half * (D / 8) + c * 16;
+              if constexpr (D == 64) tmem_st8(col, piece[n]);
+              else if (D < 256 || n < 2) tmem_st16(col, piece[n]);
+              else {
+                // the third piece of D = 256: 128-byte-swizzled rows in shared memory, one slab a group
+                const uint32_t at = base + Lay::off_q3 + half * (kM * 128) + r * 128;
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  st_shared16(at + (((c * 4 + z) ^ (r & 7)) << 4), piece[n][4 * z], piece[n][4 * z + 1], piece[n][4 * z + 2], piece[n][4 * z + 3]);
+              }
+            }
+          }
+          if (D == 256 && kPieces<T> == 3) fence_async_shared();
         }
         tmem_wait_st();
         tc_fence_before();
@@ -464,8 +544,8 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           for (int e = 0; e < kKeys; e += 2) {
             if constexpr (QUANT) {
               const float4 f = sc[e / 2];
-              x[e] = fmaf(x[e], f.x, f.y);
-              x[e + 1] = fmaf(x[e + 1], f.z, f.w);
+              x[e] = fmaf(x[e] * rowf, f.x, f.y);
+              x[e + 1] = fmaf(x[e + 1] * rowf, f.z, f.w);
             } else {
               x[e] *= c2;
               x[e + 1] *= c2;
@@ -486,7 +566,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
             now = sh_m[s ^ 1][r];
           }
           const float before = now;
-          if (now == -INFINITY || high > now + kRescaleAt) now = high;
+          if (now == -INFINITY || high > now + (kLift<QUANT> + kSlack<QUANT>)) now = high - kLift<QUANT>;
           sh_m[s][r] = now;
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
@@ -509,6 +589,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           m = now;
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pieces[QUANT ? kPieces<T> : 1][QUANT ? 16 : 1];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t p[16];
@@ -523,14 +604,21 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
                 sum[1] = fmaf(y[1], f.y, sum[1]);
                 sum[2] = fmaf(y[2], f.z, sum[2]);
                 sum[3] = fmaf(y[3], f.w, sum[3]);
+#pragma unroll
+                for (int n = 0; n < kPieces<T> - 1; ++n) pieces[n][8 * c + e / 4] = take_piece(y);
+                pieces[kPieces<T> - 1][8 * c + e / 4] = e4m3_of(y);
               } else {
 #pragma unroll
                 for (int z = 0; z < 4; ++z) sum[z] += y[z];
+                p[e / 2] = pack16<T>(y[0], y[1]);
+                p[e / 2 + 1] = pack16<T>(y[2], y[3]);
               }
-              p[e / 2] = pack16<T>(y[0], y[1]);
-              p[e / 2 + 1] = pack16<T>(y[2], y[3]);
             }
-            tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
+            if constexpr (!QUANT) tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
+          }
+          if constexpr (QUANT) {
+#pragma unroll
+            for (int n = 0; n < kPieces<T>; ++n) tmem_st16(tw + Lay::s_col + s * kKeys + n * 16, pieces[n]);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
@@ -539,7 +627,10 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_full[s]);
+        if (lane == 0) {
+          mbar_arrive(&bar.p_full[s]);
+          if (QUANT) mbar_arrive(&bar.sc_empty[g % kScaleStages]);
+        }
       }
       if (!ok) break;
       // the last product of the piece
@@ -652,29 +743,40 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- tensor work
-    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | type_bits<T>();
-    constexpr uint32_t idesc_o = tc_idesc(kM, D) | type_bits<T>() | (1u << 16);      // B is MN-major
+    // operand formats: 16-bit types, or e4m3 (0); the second product's B is MN-major
+    constexpr uint32_t kTypes = QUANT ? 0u : type_bits<T>();
+    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | kTypes, idesc_o = tc_idesc(kM, D) | kTypes | (1u << 16);
+    constexpr int kRowB = Lay::kRowB;
     uint32_t g = 0, pieces = 0;
     bool ok = true;
     const auto pv = [&](uint32_t u, int i, bool fresh) {       // O (+)= P(u) V(u), u the piece's unit i
       const int s = u & 1, st = u % kSt;
       if (!wait(&bar.v_full[st], (u / kSt) & 1)) return false;
       const uint32_t v = base + Lay::off_v + st * Lay::kTile;
-      if constexpr (SRC == TMA16) {
+      if constexpr (is_tma(SRC)) {
         // rows past the end hold what the pages or the last tile left there: 0 x NaN must not happen
         const int rows = row_limit(A, w.r, w.r.n - 1) - i * kKeys;
         if (rows < kKeys) {
-          for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
+          constexpr int kRowP = kRowB / 16;                    // 16-byte pieces of a slab's row
+          for (int x = max(rows, 0) * kRowP + lane; x < kKeys * kRowP; x += 32)
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) st_shared16(v + c * A.slab + (x >> 6) * A.group + (x & 63) * 16, 0, 0, 0, 0);
+            for (int c = 0; c < Lay::kSlabs; ++c)
+              st_shared16(v + c * A.slab + x / (8 * kRowP) * A.group + x % (8 * kRowP) * 16, 0, 0, 0, 0);
           fence_async_shared();
           __syncwarp();
         }
       }
       if (!wait(&bar.p_full[s], (u >> 1) & 1)) return false;
-      if constexpr (SRC != TMA16) fence_async_shared();        // the tile was stored by threads
+      if constexpr (!is_tma(SRC)) fence_async_shared();        // the tile was stored by threads
       tc_fence_after();
-      mma_ts4_warp(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major(v, A.slab, A.group), A.group >> 3, idesc_o, !fresh);
+      const uint64_t desc = mn_major<kRowB>(v, A.slab, A.group);
+      if constexpr (!QUANT) {                                  // four steps of 16 positions
+        mma_ts_warp<4, false>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, desc, A.group >> 3, idesc_o, !fresh);
+      } else {                                                 // each piece of P: two steps of 32
+#pragma unroll
+        for (int n = 0; n < kPieces<T>; ++n)
+          mma_ts_warp<2, true>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys + n * 16, desc, A.group >> 2, idesc_o, n > 0 || !fresh);
+      }
       tc_commit_warp(&bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
       return true;
@@ -685,12 +787,19 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         const int s = g & 1, st = g % kSt;
         if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
         if (!(ok = wait(&bar.k_full[st], (g / kSt) & 1))) break;
-        if constexpr (SRC != TMA16) fence_async_shared();
+        if constexpr (!is_tma(SRC)) fence_async_shared();
         tc_fence_after();
+        const uint32_t k_at = base + Lay::off_k + st * Lay::kTile;
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k)
-          mma_ts4_warp(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + k * 32,
-                       k_major(base + Lay::off_k + st * Lay::kTile + k * A.slab, A.group), 2, idesc_s, k > 0);
+        for (int n = 0; n < (QUANT ? kPieces<T> : 1); ++n)
+#pragma unroll
+          for (int k = 0; k < Lay::kSlabs; ++k) {
+            const uint64_t desc = k_major<kRowB>(k_at + k * A.slab, A.group);
+            if (QUANT && D == 256 && n == 2)
+              mma_ss4_f8_warp(tmem + Lay::s_col + s * kKeys, k_major<128>(base + Lay::off_q3 + k * (kM * 128), 1024), desc, idesc_s);
+            else
+              mma_ts_warp<kRowB / 32, QUANT>(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + n * (D / 4) + k * 32, desc, 2, idesc_s, n + k > 0);
+          }
         tc_commit_warp(&bar.s_done[s]);
         tc_commit_warp(&bar.k_empty[st]);
         if (i > 0) {
@@ -707,17 +816,54 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
     mbar_wait(&bar.drain, 0);
   } else {
     // ---------------------------------------------------------------- loads
-    const int lt = threadIdx.x - (kMmaWarp + 1) * 32, lw = lt >> 5;
+    const int lw = warp - kMmaWarp - 1;
     uint32_t g = 0;                                            // units so far
     bool ok = true;
     const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
     const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
-    if (is_tma(SRC) && lw >= (SRC == TMA16 ? 0 : kLoadWarps)) {
+    if (QUANT && lw == load_warps(SRC)) {
+      // -------- the scales, two positions a lane, looked up a unit early
+      float2 sc[2];
+      const auto look = [&](const Walk& w, int i) {
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int j = i * kKeys + z * 32 + lane;
+          sc[z] = make_float2(0.f, 1.f);
+          if (j < row_limit(A, w.r, w.r.n - 1)) {
+            long long so = 0;
+            if (row_offset(A, w.b, w.kh, j, &so) >= 0) sc[z] = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+            else sc[z].x = __int_as_float(0x7fc00000);         // no such page: its scores are NaN
+          }
+        }
+      };
+      if (!w.done()) look(w, w.first);
+      while (ok && !w.done()) {
+        const int stop = w.stop();
+        for (int i = w.first; i < stop; ++i, ++g) {
+          const uint32_t st = g % kScaleStages;
+          if (g >= kScaleStages && !(ok = wait(&bar.sc_empty[st], (g / kScaleStages - 1) & 1))) break;
+          uint8_t* const at = sm + Lay::off_scale + st * kScaleBytes;
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            // a scale of NaN reaches the row through its score; where the row may not see the position, its
+            // weight of 0 meets a finite factor
+            reinterpret_cast<float2*>(at)[z * 32 + lane] = make_float2(sc[z].x, log2f(sc[z].y));
+            reinterpret_cast<float*>(at + kKeys * 8)[z * 32 + lane] = sc[z].y > 0.f ? 1.f / sc[z].y : 1.f;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.sc_full[st]);
+          if (i + 1 < stop) look(w, i + 1);
+        }
+        if (!ok) break;
+        w.next(A);
+        if (!w.done()) look(w, w.first);
+      }
+    } else if constexpr (is_tma(SRC)) {
       // -------- the two warps that issue TMA copies, of K and of V: a lane a box, whose page it looks up
-      const int kv = lw - (SRC == TMA16 ? 0 : kLoadWarps);
+      const int kv = lw;
       const CUtensorMap* const map = kv ? &v_map : &k_map;
       const int box = A.box;
-      const uint32_t bytes = box * D * (SRC == TMA16 ? 2 : 1);
+      const uint32_t bytes = box * D * Lay::kElem;
       int page = -1, off = 0;
       bool need = false;
       const auto look = [&](const Walk& w, int i) {
@@ -731,47 +877,38 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           if (page >= A.c.pages) page = -1;
         }
       };
-      const auto issue = [&](uint32_t stage, uint64_t* full, int kh) {
-        const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
-        const uint32_t dst = base + stage + lane * bytes;
-        if (need && page < 0) {                                // no such page: its scores are NaN
-          const uint32_t fill = SRC == TMA16 && kv == 0 ? 0x7fff7fffu : 0u;
-          for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
-          if (SRC == TMA16) fence_async_shared();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
-        __syncwarp();
-        if (need && page >= 0) {
-          if constexpr (SRC == TMA16) tma_load_5d(dst, map, 0, off, 0, kh, page, full);
-          else tma_load_4d(dst, map, 0, off, kh, page, full);
-        }
-      };
       if (!w.done()) look(w, w.first);
       while (ok && !w.done()) {
         const int stop = w.stop();
         for (int i = w.first; i < stop; ++i, ++g) {
-          if constexpr (SRC == TMA16) {
-            if (!(ok = kv ? v_free(g) : k_free())) break;
-            issue((kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile, kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt], w.kh);
-          } else {
-            const uint32_t u = 2 * g + kv, st = u % Lay::kRaw;
-            if (u >= Lay::kRaw && !(ok = wait(&bar.raw_empty[st], (u / Lay::kRaw - 1) & 1))) break;
-            issue(Lay::off_raw + st * Lay::kRawTile, &bar.raw_full[st], w.kh);
+          if (!(ok = kv ? v_free(g) : k_free())) break;
+          const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile + lane * bytes;
+          uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
+          const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
+          if (need && page < 0) {                              // no such page: its scores are NaN (over e4m3 by its scales)
+            const uint32_t fill = !QUANT && kv == 0 ? 0x7fff7fffu : 0u;
+            for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
+            fence_async_shared();
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
+          __syncwarp();
+          if (need && page >= 0) tma_load_5d(dst, map, 0, off, 0, w.kh, page, full);
           if (i + 1 < stop) look(w, i + 1);
         }
         if (!ok) break;
         w.next(A);
         if (!w.done()) look(w, w.first);
       }
-    } else if constexpr (SRC != TMA16) {
-      // -------- the warps that copy rows, or widen codes, into the tiles
-      constexpr int kElem = QUANT ? 1 : 2;                     // stored bytes an element
-      constexpr int kLanesRow = D * kElem / 16;                // lanes a row of 16-byte pieces
+    } else {
+      // -------- the warps that copy rows. A thread's copies arrive on the stage's barrier by themselves when
+      // they land. Stages come free in the order K(g + 1), V(g) (the products are issued S(g - 1),
+      // O(g - 2)): they are filled so.
+      constexpr int kLanesRow = D * Lay::kElem / 16;           // lanes a row of 16-byte pieces
       constexpr int kRowsPass = 32 / kLanesRow;                // rows a warp's access covers
       constexpr int kPasses = kKeys / (kLoadWarps * kRowsPass);
       constexpr int kOwn = kPasses * kRowsPass;                // positions a warp handles of a unit
+      constexpr int kRowP = Lay::kRowB / 16;                   // pieces of a slab's row
       static_assert(kPasses >= 1 && kOwn <= 32, "a lane a position, a pass for every warp");
       const int sub = lane / kLanesRow, piece = lane % kLanesRow;
       const auto position = [&](int x) { return (x / kRowsPass) * (kLoadWarps * kRowsPass) + lw * kRowsPass + x % kRowsPass; };
@@ -779,138 +916,42 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         const int j = i * kKeys + position(lane % kOwn);
         return j < row_limit(A, w.r, w.r.n - 1) ? row_offset(A, w.b, w.kh, j, nullptr) : -2ll;
       };
-      if constexpr (SRC == ROWS16) {
-        // A thread's copies arrive on the stage's barrier by themselves when they land. Stages come free
-        // in the order K(g + 1), V(g) (the products are issued S(g - 1), O(g - 2)): they are filled so.
-        const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
-          const uint32_t dst = base + tile + (piece >> 3) * A.slab;
-          const T* src = static_cast<const T*>(pool);
+      const auto fill = [&](const void* pool, uint32_t tile, long long off, uint64_t* full, bool key) {
+        const uint32_t dst = base + tile + piece / kRowP * A.slab;
+        const uint8_t* src = static_cast<const uint8_t*>(pool);
 #pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const int r = position(x * kRowsPass + sub);
-            const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-            const bool nan_row = key && o == -1;
-            cp_async16(dst + (r >> 3) * A.group + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4),
-                       o >= 0 ? static_cast<const void*>(src + o + piece * 8) : static_cast<const void*>(kNanRow),
-                       o >= 0 || nan_row ? 16 : 0);
-          }
-          cp_async_arrive(full);
-        };
-        long long off = w.done() ? -2 : find(w, w.first), v_off = -2;
-        const auto fill_v = [&](uint32_t u) {
-          if (!v_free(u)) return false;
-          fill(A.c.v, Lay::off_v + (u % kSt) * Lay::kTile, v_off, &bar.v_full[u % kSt], false);
-          return true;
-        };
-        while (ok && !w.done()) {
-          const int stop = w.stop();
-          for (int i = w.first; i < stop; ++i, ++g) {
-            if (!(ok = k_free())) break;
-            fill(A.c.k, Lay::off_k + (g % kSt) * Lay::kTile, off, &bar.k_full[g % kSt], true);
-            if (g > 0 && !(ok = fill_v(g - 1))) break;
-            v_off = off;
-            if (i + 1 < stop) off = find(w, i + 1);
-          }
-          if (!ok) break;
-          w.next(A);
-          if (!w.done()) off = find(w, w.first);
-        }
-        if (ok && g > 0) fill_v(g - 1);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      } else {
-        // Codes come from their stages (TMA8) or through registers, each refilled with the next unit's
-        // as soon as it is stored (ROWS8). Scales are looked up a unit early.
-        const auto put = [&](uint32_t tile, int x, const uint4& y) {       // pass x's codes, widened
+        for (int x = 0; x < kPasses; ++x) {
           const int r = position(x * kRowsPass + sub);
-          const uint4 a = widen8<T>(y.x, y.y), b = widen8<T>(y.z, y.w);
-          const int c0 = piece * 2;                            // 16-byte pieces of the widened row
-          const uint32_t row = base + tile + (c0 >> 3) * A.slab + (r >> 3) * A.group + (r & 7) * 128;
-          st_shared16(row + (((c0 & 7) ^ (r & 7)) << 4), a.x, a.y, a.z, a.w);
-          st_shared16(row + ((((c0 + 1) & 7) ^ (r & 7)) << 4), b.x, b.y, b.z, b.w);
-        };
-        Walk f = w;                                            // the unit to be looked up next
-        int fi = f.first;
-        long long off = -1;
-        float2 sc_next = make_float2(0.f, 1.f);
-        const auto look = [&] {
-          off = -1;
-          sc_next = make_float2(0.f, 1.f);
-          if (f.done()) return;
-          const int lim = row_limit(A, f.r, f.r.n - 1), pos = fi * kKeys;
-          if (SRC == ROWS8) off = find(f, fi);
-          if (lt < kKeys && pos + lt < lim) {                  // a lane a position
-            long long so = 0;
-            if (row_offset(A, f.b, f.kh, pos + lt, &so) >= 0)
-              sc_next = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
-            else sc_next.x = __int_as_float(0x7fc00000);       // no such page: its scores are NaN
-          }
-          if (++fi == f.stop()) {
-            f.next(A);
-            fi = f.first;
-          }
-        };
-        uint4 kr[SRC == ROWS8 ? kPasses : 1], vr[SRC == ROWS8 ? kPasses : 1];
-        const auto fetch = [&](const void* pool, uint4* regs) {
-#pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
-            regs[x] = make_uint4(0, 0, 0, 0);
-            if (o >= 0) regs[x] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + o) + piece);
-          }
-        };
-        // one tile of the unit: wait for its stage, store it widened, announce it
-        const auto tile = [&](uint32_t at, uint64_t* full, uint32_t u, int rows, uint4* regs) {
-          if constexpr (SRC == ROWS8) {
-#pragma unroll
-            for (int x = 0; x < kPasses; ++x) put(at, x, regs[x]);
-          } else {
-            const uint32_t st = u % Lay::kRaw;
-            if (!wait(&bar.raw_full[st], (u / Lay::kRaw) & 1)) return false;
-            const uint8_t* raw = sm + Lay::off_raw + st * Lay::kRawTile;
-            uint4 y[kPasses];
-#pragma unroll
-            for (int x = 0; x < kPasses; ++x) {
-              const int r = position(x * kRowsPass + sub);
-              y[x] = reinterpret_cast<const uint4*>(raw)[r * kLanesRow + piece];
-              if (r >= rows) y[x] = make_uint4(0, 0, 0, 0);    // past the end: what the stage held before
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.raw_empty[st]);
-#pragma unroll
-            for (int x = 0; x < kPasses; ++x) put(at, x, y[x]);
-          }
-          fence_async_shared();
-          mbar_arrive(full);
-          return true;
-        };
-        look();
-        if (SRC == ROWS8) { fetch(A.c.k, kr); fetch(A.c.v, vr); }
-        float2 sc = sc_next;
-        look();
-        for (; ok && !w.done(); w.next(A)) {
-          const int stop = w.stop(), lim = row_limit(A, w.r, w.r.n - 1);
-          for (int i = w.first; i < stop; ++i, ++g) {
-            if (!(ok = k_free())) break;
-            if (lt < kKeys) {
-              // a scale of NaN reaches the row through its score; where the row may not see the position,
-              // its weight of 0 meets a finite factor
-              uint8_t* const at = sm + Lay::off_scale + (g % kScaleStages) * kScaleBytes;
-              reinterpret_cast<float2*>(at)[lt] = make_float2(sc.x * (A.scale * kLog2e), log2f(sc.y));
-              reinterpret_cast<float*>(at + kKeys * 8)[lt] = sc.y > 0.f ? 1.f / sc.y : 1.f;
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bar.sc_full[g % kScaleStages]);
-            }
-            if (!(ok = tile(Lay::off_k + (g % kSt) * Lay::kTile, &bar.k_full[g % kSt], 2 * g, lim - i * kKeys, kr))) break;
-            if (SRC == ROWS8) fetch(A.c.k, kr);
-            if (!(ok = v_free(g))) break;
-            if (!(ok = tile(Lay::off_v + (g % kSt) * Lay::kTile, &bar.v_full[g % kSt], 2 * g + 1, lim - i * kKeys, vr))) break;
-            if (SRC == ROWS8) fetch(A.c.v, vr);
-            sc = sc_next;
-            look();
-          }
-          if (!ok) break;
+          const long long o = __shfl_sync(0xffffffffu, off, x * kRowsPass + sub);
+          const bool nan_row = !QUANT && key && o == -1;
+          const int swz = Lay::kRowB == 128 ? (piece % kRowP) ^ (r & 7) : (piece % kRowP) ^ (r >> 1 & 3);
+          cp_async16(dst + (r >> 3) * A.group + (r & 7) * Lay::kRowB + (swz << 4),
+                     o >= 0 ? static_cast<const void*>(src + o * Lay::kElem + piece * 16) : static_cast<const void*>(kNanRow),
+                     o >= 0 || nan_row ? 16 : 0);
         }
+        cp_async_arrive(full);
+      };
+      long long off = w.done() ? -2 : find(w, w.first), v_off = -2;
+      const auto fill_v = [&](uint32_t u) {
+        if (!v_free(u)) return false;
+        fill(A.c.v, Lay::off_v + (u % kSt) * Lay::kTile, v_off, &bar.v_full[u % kSt], false);
+        return true;
+      };
+      while (ok && !w.done()) {
+        const int stop = w.stop();
+        for (int i = w.first; i < stop; ++i, ++g) {
+          if (!(ok = k_free())) break;
+          fill(A.c.k, Lay::off_k + (g % kSt) * Lay::kTile, off, &bar.k_full[g % kSt], true);
+          if (g > 0 && !(ok = fill_v(g - 1))) break;
+          v_off = off;
+          if (i + 1 < stop) off = find(w, i + 1);
+        }
+        if (!ok) break;
+        w.next(A);
+        if (!w.done()) off = find(w, w.first);
       }
+      if (ok && g > 0) fill_v(g - 1);
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   }
   tc_fence_before();
@@ -1031,25 +1072,19 @@ int sm_count() {
 }
 size_t desc_bytes(int grid) { return ((size_t)grid * sizeof(Desc) + 255) / 256 * 256; }
 
-// The pool as [page][kv head][slot][dim], read in boxes of `rows` slots: of 16-bit rows all 64-column slabs
-// at once, of codes whole rows. False where a tensor map cannot describe it (rows are then copied one
-// by one).
+// The pool as [page][kv head][slot][dim], read in boxes of `rows` slots and all their columns, as slabs of 128
+// bytes (64 where a row has no more). False where a tensor map cannot describe it (rows are then copied
+// one by one).
 bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
-  const cuuint64_t dim = c.dim, slots = c.page_size, heads = c.kv_heads, pages = c.pages;
-  const cuuint64_t slot = c.slot_stride, head = c.head_stride, page = c.page_stride;
-  const cuuint32_t step[5] = {1, 1, 1, 1, 1}, r = rows;
+  const bool codes = c.dtype == DT_E4M3;
+  const cuuint64_t size = codes ? 1 : 2, row = c.dim * size < 128 ? 64 : 128, slabs = c.dim * size / row;
+  const cuuint64_t dims[5] = {row / size, (cuuint64_t)c.page_size, slabs, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)c.slot_stride * size, row, (cuuint64_t)c.head_stride * size, (cuuint64_t)c.page_stride * size};
+  const cuuint32_t box[5] = {(cuuint32_t)(row / size), (cuuint32_t)rows, (cuuint32_t)slabs, 1, 1}, step[5] = {1, 1, 1, 1, 1};
   const auto encode = tensor_map_encoder();
-  if (!encode) return false;
-  if (c.dtype == DT_E4M3) {
-    const cuuint64_t dims[4] = {dim, slots, heads, pages}, strides[3] = {slot, head, page};
-    const cuuint32_t box[4] = {(cuuint32_t)c.dim, r, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  }
-  const cuuint64_t dims[5] = {64, slots, dim / 64, heads, pages}, strides[4] = {slot * 2, 128, head * 2, page * 2};
-  const cuuint32_t box[5] = {64, r, (cuuint32_t)(c.dim / 64), 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode && encode(map, codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, base, dims, strides, box,
+                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D, int SRC>
@@ -1128,12 +1163,12 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_paged_attn_workspace(H, c->kv_heads, c->dim))
     return CFB_ERR_WORKSPACE;
   const int grid = sm_count();
-  // Boxes: a whole unit where pages hold whole units; else of 8 rows for 16-bit rows (the tile is then
-  // [group][slab]) and as many rows as divide both a page and a unit for codes.
-  const int fit = std::gcd(c->page_size, kKeys), box = c->dtype != DT_E4M3 && fit < kKeys ? std::min(fit, 8) : fit;
-  const bool grouped = c->dtype != DT_E4M3 && box == 8;
+  // Boxes: a whole unit where pages hold whole units, else of 8 rows (the tile is then [group][slab]).
+  const int fit = std::gcd(c->page_size, kKeys), box = fit < kKeys ? std::min(fit, 8) : fit;
+  const uint32_t row = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) < 128 ? 64 : 128, slabs = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) / row;
+  const bool grouped = box == 8;
   const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-                   T, B, H, causal, H / c->kv_heads, box, grouped ? 1024u : kKeys * 128u, grouped ? c->dim / 64 * 1024u : 1024u,
+                   T, B, H, causal, H / c->kv_heads, box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
                    static_cast<Desc*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
   CUtensorMap maps[2] = {};
   const bool tma = box >= 8 && pool_map(&maps[0], *c, c->k, box) && pool_map(&maps[1], *c, c->v, box);
