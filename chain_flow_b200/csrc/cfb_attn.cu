@@ -39,6 +39,10 @@ namespace {
 constexpr int kM = 128, kKeys = 64;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4;
 constexpr int kScaleStages = 4;
+// A softmax thread holds a row; memory wants a warp's access to run along rows. 64 bytes of 32 rows at a time
+// are turned in a buffer of the warp's own (row by row, a warp's access touched 32 lines: a piece's Q and O
+// took 12000 and 5000 cycles so at 128 columns).
+constexpr int kTurnPitch = 80;
 constexpr uint32_t kScaleBytes = kKeys * 12;   // a unit's scales: [64] (k's with the softmax's, log2 v's), [64] 1 / v's
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Weights are 2^(x - m). m is set to the maximum less kLift, and moved again (o rescaled) only when the
@@ -110,12 +114,14 @@ CFB_DEV int head_units(const AttnArgs& A, const Request& r) {
   return u;
 }
 
-// A share, piece by piece; every warp of the CTA walks it alike.
+// A share, piece by piece; every warp of the CTA walks it alike. What runs once a piece or less is kept out of
+// line, here and below: the kernel's roles run side by side, and their code has to share the instruction
+// cache (inlined everywhere, a quarter of all warp cycles went by without an instruction to issue).
 struct Walk {
   long long u, end;
   int b, kh, tile, tiles, units, first;   // units of the piece; first unit of it in this share
   Request r;
-  CFB_DEV void start(const AttnArgs& A, long long from, long long to, int req, long long rest, int per_head) {
+  __device__ __noinline__ void start(const AttnArgs& A, long long from, long long to, int req, long long rest, int per_head) {
     u = from; end = to; b = req;
     r = request(A, b);
     tiles = tiles_of(A, r);
@@ -131,7 +137,7 @@ struct Walk {
   }
   CFB_DEV bool done() const { return u >= end; }
   CFB_DEV int stop() const { return (int)min((long long)units, first + (end - u)); }   // first unit past this share's part
-  CFB_DEV void next(const AttnArgs& A) {
+  __device__ __noinline__ void next(const AttnArgs& A) {
     u += stop() - first;
     if (u >= end) return;
     first = 0;
@@ -172,7 +178,8 @@ struct Layout {
   static constexpr uint32_t kTile = kKeys * D * kElem;
   // a third piece of Q over e4m3 that tensor memory has no room for (D = 256) lies in shared memory
   static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_q3 = 2 * kStages * kTile;
-  static constexpr uint32_t off_scale = off_q3 + (is_e4m3(SRC) && D == 256 ? kM * D : 0);
+  static constexpr uint32_t off_turn = off_q3 + (is_e4m3(SRC) && D == 256 ? kM * D : 0);
+  static constexpr uint32_t off_scale = off_turn + kSoftWarps * 32 * kTurnPitch;
   static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kScaleBytes : 0) + 1024;
   static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
@@ -228,8 +235,8 @@ CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 // D[tmem] (+)= A[tmem] . B[smem] over N steps of 32 bytes of the summed dim in one statement, by one elected
 // lane (one election and one statement for four take less issue time than four), B's descriptor advancing
-// by `step`. F8: e4m3, else 16-bit operands.
-template <int N, bool F8>
+// by `step` and A by ASTEP columns. F8: e4m3, else 16-bit operands.
+template <int N, bool F8, int ASTEP = 8>
 CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t step, uint32_t idesc, uint32_t accumulate) {
 #define CFB_TS4(KIND)                                                                                                        \
   asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
@@ -237,13 +244,13 @@ CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t 
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %8, %3, 1;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%6], %9, %3, 1;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%7], %10, %3, 1;\n\t}"                                     \
-               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "r"(tmem_a + 16),            \
-                  "r"(tmem_a + 24), "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step) : "memory")
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + ASTEP),                           \
+                  "r"(tmem_a + 2 * ASTEP), "r"(tmem_a + 3 * ASTEP), "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step) : "memory")
 #define CFB_TS2(KIND)                                                                                                        \
   asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%1], %2, %3, q;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %6, %3, 1;\n\t}"                                      \
-               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "l"(b + step) : "memory")
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + ASTEP), "l"(b + step) : "memory")
   static_assert(N == 4 || (N == 2 && F8), "steps");
   if constexpr (!F8) CFB_TS4("f16");
   else if constexpr (N == 4) CFB_TS4("f8f6f4");
@@ -320,6 +327,55 @@ CFB_DEV uint32_t take_piece(float (&x)[4]) {
 }
 template <typename T> constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
 
+// The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not.
+__device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int* dead) {
+  bool ok = true;
+  const unsigned long long t0 = globaltimer();
+  for (unsigned it = 1; !mbar_try_wait(b, parity); ++it)
+    if (it % kPollsPerCheck == 0) {
+      if (wait_expired(t0, kWaitBudgetNs)) *dead = 1;
+      if (*dead != 0) {
+        ok = false;
+        break;
+      }
+    }
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// One row's o over positions [from, to) of its own, from its m (and, into the output, divided by its sum):
+// the columns [half * D / 2, ...) of it. For 16-bit rows whose product met a value that is not finite.
+template <typename T, int D>
+__device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T* q, int from, int to, float m, float inv, int half,
+                                       T* out, float* part) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  float x[E], acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) { x[e] = to_float(q[lane * E + e]); acc[e] = 0.f; }
+  for (int j = from; j < to; ++j) {
+    const long long off = row_offset(A, b, kh, j, nullptr);
+    if (off < 0) continue;                                     // its score is NaN: so is l, and this row is not here
+    const T* k = static_cast<const T*>(A.c.k) + off + lane * E;
+    const T* v = static_cast<const T*>(A.c.v) + off + lane * E;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s = fmaf(x[e], to_float(k[e]), s);
+#pragma unroll
+    for (int z = 16; z; z >>= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
+    const float p = exp2_approx(s * (A.scale * kLog2e) - m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(v[e]), acc[e]);
+  }
+  __syncwarp();
+  if (lane >> 4 == half) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (out) out[lane * E + e] = from_float<T>(acc[e] * inv);
+      else part[lane * E + e] = acc[e];
+    }
+  }
+}
+
 // ---- the kernel -----------------------------------------------------------------------------------
 // One CTA per SM. The loading warps (Source) fill, per unit, a K and a V tile: pages are found through
 // the page table a unit early, positions past the end are zeros where it matters (V), and e4m3 codes
@@ -332,7 +388,7 @@ template <typename T> constexpr int kPieces = std::is_same<T, __half>::value ? 3
 // the last time: weights are then at most 2^8, far inside both types, and most units touch O not at all.
 template <typename T, int D, int SRC>
 __global__ void __launch_bounds__(threads_of(SRC), 1)
-attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using Lay = Layout<D, SRC>;
   constexpr bool QUANT = is_e4m3(SRC);
   constexpr int kSt = Lay::kStages;
@@ -416,19 +472,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
   // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait
   // that is not over at once.
   const auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (__all_sync(0xffffffffu, mbar_test_wait(b, parity))) return true;
-    volatile int* const d = &dead;
-    bool ok = true;
-    const unsigned long long t0 = globaltimer();
-    for (unsigned it = 1; !mbar_try_wait(b, parity); ++it)
-      if (it % kPollsPerCheck == 0) {
-        if (wait_expired(t0, kWaitBudgetNs)) *d = 1;
-        if (*d != 0) {
-          ok = false;
-          break;
-        }
-      }
-    return __all_sync(0xffffffffu, ok) != 0;
+    return __all_sync(0xffffffffu, mbar_test_wait(b, parity)) || wait_on(b, parity, &dead);
   };
 
   if (warp < kSoftWarps) {
@@ -439,7 +483,18 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
     const int r = pair * 32 + lane;
     const float c2 = A.scale * kLog2e;
-    uint32_t g0 = 0, swaps = 0;                                // units before this piece; exchanges of sums
+    uint32_t g0 = 0, swaps = 0;                                // units before this piece; exchanges of the two groups
+    uint8_t* const turn = sm + Lay::off_turn + warp * (32 * kTurnPitch);
+    uint8_t* const turn_row = turn + lane * kTurnPitch;                              // this lane's row
+    uint8_t* const turn_at = turn + (lane >> 2) * kTurnPitch + (lane & 3) * 16;      // its piece of row lane / 4, then every 8th
+    const auto exchange = [&](float2 mine, float2* other) {    // with the row's thread of the other group
+      sh_swap[half * kM + r] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.swap[pair]);
+      if (!wait(&bar.swap[pair], swaps++ & 1)) return false;
+      *other = sh_swap[(half ^ 1) * kM + r];
+      return true;
+    };
     for (; !w.done(); g0 += w.stop() - w.first, w.next(A)) {
       const int stop = w.stop(), first = w.first;
       const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
@@ -451,68 +506,78 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       // Q to tensor memory, a half of the head dim a group
       float rowf = c2;                                         // the softmax's scale, with the row's own over e4m3
       if (warp_live) {
-        const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (long long)(w.r.t0 + (valid ? tok : 0)) * A.sq_t +
-                                                                (valid ? head : 0) * A.sq_h);
-        const auto load = [&](int e) { return valid ? __ldg(src + e) : make_uint4(0, 0, 0, 0); };
-        constexpr int kRounds = D == 256 ? 2 : 1, kWords = D == 64 ? 16 : 32;        // 32-bit words of a round
-        if constexpr (!QUANT) {
-          uint32_t u[kRounds][kWords];
+        const long long q_off = valid ? (long long)(w.r.t0 + tok) * A.sq_t + head * A.sq_h + half * (D / 2) : -1;
+        constexpr int kChunks = D / 64;                        // 32 elements of this group's half each
+        // the warp's rows, all loads in flight, then turned 64 bytes a row at a time: y[c] of this lane's row
+        uint4 y[kChunks][4];
 #pragma unroll
-          for (int e = 0; e < kRounds * kWords / 4; ++e) {
-            const uint4 y = load(half * (D / 16) + e);
-            uint32_t* z = u[e / (kWords / 4)] + 4 * (e % (kWords / 4));
-            z[0] = y.x; z[1] = y.y; z[2] = y.z; z[3] = y.w;
+        for (int x = 0; x < 4; ++x) {
+          const long long o = __shfl_sync(0xffffffffu, q_off, x * 8 + (lane >> 2));
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (o < 0 ? 0 : o)) + (lane & 3);
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            y[c][x] = make_uint4(0, 0, 0, 0);
+            if (o >= 0) y[c][x] = __ldg(src + c * 4);
           }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(turn_at + x * 8 * kTurnPitch) = y[c][x];
           __syncwarp();
 #pragma unroll
-          for (int c = 0; c < kRounds; ++c) {
-            if constexpr (kWords == 32) tmem_st32(tw + Lay::q_col + half * (D / 4) + c * 32, u[c]);
-            else tmem_st16(tw + Lay::q_col + half * (D / 4), u[c]);
+          for (int x = 0; x < 4; ++x) y[c][x] = *reinterpret_cast<const uint4*>(turn_row + x * 16);
+          __syncwarp();
+        }
+        if constexpr (!QUANT) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t u[16];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) { u[4 * x] = y[c][x].x; u[4 * x + 1] = y[c][x].y; u[4 * x + 2] = y[c][x].z; u[4 * x + 3] = y[c][x].w; }
+            tmem_st16(tw + Lay::q_col + half * (D / 4) + c * 16, u);
           }
         } else {
           // the row's largest magnitude (patterns order like integers; what is not finite is largest)
           constexpr uint32_t kMag = 0x7fff7fffu, kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
           uint32_t top = 0;
-#pragma unroll 8
-          for (int e = 0; e < D / 8; ++e) {
-            const uint4 y = load(e);
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(y.x & kMag, y.y & kMag), __vmaxu2(y.z & kMag, y.w & kMag)));
-          }
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              top = __vmaxu2(top, __vmaxu2(__vmaxu2(y[c][x].x & kMag, y[c][x].y & kMag), __vmaxu2(y[c][x].z & kMag, y[c][x].w & kMag)));
           top = max(top & 0xffffu, top >> 16);
+          float2 other;
+          if (!exchange(make_float2(__uint_as_float(top), 0.f), &other)) break;
+          top = max(top, __float_as_uint(other.x));
           // 2^(7 - exponent): the largest element lands in [128, 256)
           const int e2 = min(max((int)(__float_as_uint(unpack16<T>(top).x) >> 23) - 127, -100), 127);
           const float up = __uint_as_float((uint32_t)(127 + 7 - e2) << 23);
           rowf = top >= kInf ? __int_as_float(0x7fc00000) : c2 * __uint_as_float((uint32_t)(127 + e2 - 7) << 23);
-          // 64 elements a round: 16 words of each piece (32 elements, 8 words where D = 64)
-          constexpr int kOct = D == 64 ? 4 : 8;                // 16-byte loads of a round
 #pragma unroll
-          for (int c = 0; c < (D == 64 ? 1 : D / 128); ++c) {
-            uint32_t piece[kPieces<T>][2 * kOct];
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t piece[kPieces<T>][8];
 #pragma unroll
-            for (int e = 0; e < kOct; ++e) {
-              const uint4 y = load(half * (D / 16) + c * kOct + e);
-              const uint32_t ys[4] = {y.x, y.y, y.z, y.w};
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t ys[4] = {y[c][x].x, y[c][x].y, y[c][x].z, y[c][x].w};
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
-                const float2 f = unpack16<T>(ys[2 * z]), g = unpack16<T>(ys[2 * z + 1]);
-                float x[4] = {f.x * up, f.y * up, g.x * up, g.y * up};
+                const float2 f = unpack16<T>(ys[2 * z]), h = unpack16<T>(ys[2 * z + 1]);
+                float v[4] = {f.x * up, f.y * up, h.x * up, h.y * up};
 #pragma unroll
-                for (int n = 0; n < kPieces<T> - 1; ++n) piece[n][2 * e + z] = take_piece(x);
-                piece[kPieces<T> - 1][2 * e + z] = e4m3_of(x);
+                for (int n = 0; n < kPieces<T> - 1; ++n) piece[n][2 * x + z] = take_piece(v);
+                piece[kPieces<T> - 1][2 * x + z] = e4m3_of(v);
               }
             }
-            __syncwarp();
 #pragma unroll
             for (int n = 0; n < kPieces<T>; ++n) {
-              const uint32_t col = tw + Lay::q_col + n * (D / 4) + half * (D / 8) + c * 16;
-              if constexpr (D == 64) tmem_st8(col, piece[n]);
-              else if (D < 256 || n < 2) tmem_st16(col, piece[n]);
+              if (D < 256 || n < 2) tmem_st8(tw + Lay::q_col + n * (D / 4) + half * (D / 8) + c * 8, piece[n]);
               else {
                 // the third piece of D = 256: 128-byte-swizzled rows in shared memory, one slab a group
                 const uint32_t at = base + Lay::off_q3 + half * (kM * 128) + r * 128;
 #pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  st_shared16(at + (((c * 4 + z) ^ (r & 7)) << 4), piece[n][4 * z], piece[n][4 * z + 1], piece[n][4 * z + 2], piece[n][4 * z + 3]);
+                for (int z = 0; z < 2; ++z)
+                  st_shared16(at + (((c * 2 + z) ^ (r & 7)) << 4), piece[n][4 * z], piece[n][4 * z + 1], piece[n][4 * z + 2], piece[n][4 * z + 3]);
               }
             }
           }
@@ -524,6 +589,15 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.q_ready);
 
+      // the next tile's Q (of the same heads and request, the common case), into L2 by the time it is wanted
+      if (w.tile + 1 < w.tiles && valid && w.u + (stop - first) < w.end) {
+        const int next = R + kM, nt = next / A.rep;
+        if (nt < w.r.n) {
+          const T* p = static_cast<const T*>(A.q) + (long long)(w.r.t0 + nt) * A.sq_t + (w.kh * A.rep + next - nt * A.rep) * A.sq_h + half * (D / 2);
+#pragma unroll
+          for (int z = 0; z < (D >= 128 ? D / 128 : 1); ++z) asm volatile("prefetch.global.L2 [%0];" :: "l"(p + z * 64));
+        }
+      }
       float m = -INFINITY, l = 0.f;                            // this group's: l in units of 2^m
       for (int i = first; i < stop; ++i) {
         const uint32_t g = g0 + (i - first);
@@ -532,34 +606,41 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
         if (!(ok = wait(&bar.s_done[s], (g >> 1) & 1))) break;
         if (warp_live) {
           tc_fence_after();
-          float x[kKeys];
-          tmem_ld32(tw + Lay::s_col + s * kKeys, x);
-          tmem_ld32(tw + Lay::s_col + s * kKeys + 32, x + 32);
           const float4* const sc = reinterpret_cast<const float4*>(sm + Lay::off_scale + (g % kScaleStages) * kScaleBytes);
-          if (QUANT) ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1);
-          tmem_wait_ld();
-          if (!ok) break;
           const int j0 = i * kKeys;
+          const bool masked = __any_sync(0xffffffffu, lim < j0 + kKeys);
+          if (QUANT && !(ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1))) break;
+          // the scaled scores of the columns from 32 c on
+          const auto scores = [&](int c, float* x) {
+            tmem_ld32(tw + Lay::s_col + s * kKeys + 32 * c, x);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < kKeys; e += 2) {
-            if constexpr (QUANT) {
-              const float4 f = sc[e / 2];
-              x[e] = fmaf(x[e] * rowf, f.x, f.y);
-              x[e + 1] = fmaf(x[e + 1] * rowf, f.z, f.w);
-            } else {
-              x[e] *= c2;
-              x[e + 1] *= c2;
+            for (int e = 0; e < 32; e += 2) {
+              if constexpr (QUANT) {
+                const float4 f = sc[16 * c + e / 2];
+                x[e] = fmaf(x[e] * rowf, f.x, f.y);
+                x[e + 1] = fmaf(x[e + 1] * rowf, f.z, f.w);
+              } else {
+                x[e] *= c2;
+                x[e + 1] *= c2;
+              }
             }
-          }
-          if (__any_sync(0xffffffffu, lim < j0 + kKeys)) {
+            if (masked) {
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e)
-              if (j0 + e >= lim) x[e] = -INFINITY;
-          }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              for (int e = 0; e < 32; ++e)
+                if (j0 + 32 * c + e >= lim) x[e] = -INFINITY;
+            }
+          };
+          const auto top_of = [](const float* x, float high) {
+            float top[4] = {high, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
-          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+            return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          };
+          float x[kKeys];
+          scores(0, x);
+          scores(1, x + 32);
+          const float high = top_of(x + 32, top_of(x, -INFINITY));
           float now = -INFINITY;                               // the maximum the weights so far are relative to
           if (i > first) {
             if (!(ok = wait(&bar.m_set[s ^ 1][pair], ((g - 1) >> 1) & 1))) break;
@@ -589,36 +670,45 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
           m = now;
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pieces[QUANT ? kPieces<T> : 1][QUANT ? 16 : 1];
+          if constexpr (!QUANT) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[16];
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float y[4];
+              for (int e = 0; e < 32; e += 4) {
+                float y[4];
 #pragma unroll
-              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
-              if constexpr (QUANT) {
+                for (int z = 0; z < 4; ++z) {
+                  y[z] = exp2_approx(x[32 * c + e + z] - mm);
+                  sum[z] += y[z];
+                }
+                p[e / 2] = pack16<T>(y[0], y[1]);
+                p[e / 2 + 1] = pack16<T>(y[2], y[3]);
+              }
+              tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
+            }
+          } else {
+            // 32 positions are one step of the product: their pieces go where their scores were
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pieces[kPieces<T>][8];
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                float y[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
                 const float4 f = sc[kKeys / 2 + 8 * c + e / 4];
                 sum[0] = fmaf(y[0], f.x, sum[0]);
                 sum[1] = fmaf(y[1], f.y, sum[1]);
                 sum[2] = fmaf(y[2], f.z, sum[2]);
                 sum[3] = fmaf(y[3], f.w, sum[3]);
 #pragma unroll
-                for (int n = 0; n < kPieces<T> - 1; ++n) pieces[n][8 * c + e / 4] = take_piece(y);
-                pieces[kPieces<T> - 1][8 * c + e / 4] = e4m3_of(y);
-              } else {
-#pragma unroll
-                for (int z = 0; z < 4; ++z) sum[z] += y[z];
-                p[e / 2] = pack16<T>(y[0], y[1]);
-                p[e / 2 + 1] = pack16<T>(y[2], y[3]);
+                for (int n = 0; n < kPieces<T> - 1; ++n) pieces[n][e / 4] = take_piece(y);
+                pieces[kPieces<T> - 1][e / 4] = e4m3_of(y);
               }
-            }
-            if constexpr (!QUANT) tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
-          }
-          if constexpr (QUANT) {
 #pragma unroll
-            for (int n = 0; n < kPieces<T>; ++n) tmem_st16(tw + Lay::s_col + s * kKeys + n * 16, pieces[n]);
+              for (int n = 0; n < kPieces<T>; ++n) tmem_st8(tw + Lay::s_col + s * kKeys + 32 * c + n * 8, pieces[n]);
+            }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
@@ -640,42 +730,60 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       if (warp_live) {
         const bool whole = first == 0 && stop == w.units;
         // the two groups' sums, relative to the later maximum
-        sh_swap[half * kM + r] = make_float2(m, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.swap[pair]);
-        if (!wait(&bar.swap[pair], swaps++ & 1)) break;
-        const float2 other = sh_swap[(half ^ 1) * kM + r];
+        float2 other;
+        if (!exchange(make_float2(m, l), &other)) break;
         const float top = fmaxf(m, other.x);
         const auto to_top = [&](float mm, float ll) { return mm == top || mm == -INFINITY ? ll : ll * exp2_approx(mm - top); };
         l = to_top(m, l) + to_top(other.x, other.y);
         m = top;
         if (w.r.over) l = __int_as_float(0x7fc00000);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        T* out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
         float* const part = part_row<D>(A.part, grid, cta, first == 0, r);
+        const long long o_off = (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
         float bad[4] = {0.f, 0.f, 0.f, 0.f};                   // turn NaN where an element is not finite
-#pragma unroll
+#pragma unroll 1
         for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
           float o[32];
           tmem_ld32(tw + Lay::o_col + d, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) bad[e & 3] = fmaf(o[e], 0.f, bad[e & 3]);
-          if (valid && whole) {
-            uint4* dst = reinterpret_cast<uint4*>(out + d);
+          for (int e = 0; e < 32; ++e)
+            if constexpr (!QUANT) bad[e & 3] = fmaf(o[e], 0.f, bad[e & 3]);
+          if (whole) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float* y = o + 8 * e;
-              dst[e] = l == 0.f ? make_uint4(0, 0, 0, 0)
-                                : make_uint4(pack16<T>(y[0] * inv, y[1] * inv), pack16<T>(y[2] * inv, y[3] * inv),
-                                             pack16<T>(y[4] * inv, y[5] * inv), pack16<T>(y[6] * inv, y[7] * inv));
+              *reinterpret_cast<uint4*>(turn_row + e * 16) =
+                  l == 0.f ? make_uint4(0, 0, 0, 0)
+                           : make_uint4(pack16<T>(y[0] * inv, y[1] * inv), pack16<T>(y[2] * inv, y[3] * inv),
+                                        pack16<T>(y[4] * inv, y[5] * inv), pack16<T>(y[6] * inv, y[7] * inv));
             }
-          } else if (valid) {
-            float4* dst = reinterpret_cast<float4*>(part + d);
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int x = 0; x < 4; ++x) {
+              const int row = x * 8 + (lane >> 2);
+              const long long off = __shfl_sync(0xffffffffu, o_off, row);
+              if (pair * 32 + row < rows)
+                *(reinterpret_cast<uint4*>(static_cast<T*>(A.o) + off + d) + (lane & 3)) = *reinterpret_cast<const uint4*>(turn_at + x * 8 * kTurnPitch);
+            }
+            __syncwarp();
+          } else {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {                      // 16 columns a turn
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<float4*>(turn_row + e * 16) = make_float4(o[16 * z + 4 * e], o[16 * z + 4 * e + 1], o[16 * z + 4 * e + 2], o[16 * z + 4 * e + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int row = x * 8 + (lane >> 2);
+                if (pair * 32 + row < rows)
+                  *(reinterpret_cast<float4*>(part_row<D>(A.part, grid, cta, first == 0, pair * 32 + row) + d + 16 * z) + (lane & 3)) =
+                      *reinterpret_cast<const float4*>(turn_at + x * 8 * kTurnPitch);
+              }
+              __syncwarp();
+            }
           }
-          __syncwarp();
         }
         if (valid && half == 0) {
           if (!whole) {
@@ -697,35 +805,9 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
             const int row = pair * 32 + src, RR = w.tile * kM + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
             const int li = __shfl_sync(0xffffffffu, lim, src);
             const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
-            constexpr int E = D / 32;
-            const T* qp = static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h + lane * E;
-            float q[E], acc[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) { q[e] = to_float(qp[e]); acc[e] = 0.f; }
-            for (int j = first * kKeys; j < li; ++j) {
-              const long long off = row_offset(A, w.b, w.kh, j, nullptr);
-              if (off < 0) continue;                          // its score is NaN: l is too, and this row is not here
-              const T* kp = static_cast<const T*>(A.c.k) + off + lane * E;
-              const T* vp = static_cast<const T*>(A.c.v) + off + lane * E;
-              float s = 0.f;
-#pragma unroll
-              for (int e = 0; e < E; ++e) s = fmaf(q[e], to_float(kp[e]), s);
-#pragma unroll
-              for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-              const float p = exp2_approx(s * c2 - mr);
-#pragma unroll
-              for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(vp[e]), acc[e]);
-            }
-            T* op = static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h + lane * E;
-            float* const pp = part_row<D>(A.part, grid, cta, first == 0, row) + lane * E;
-            __syncwarp();
-            if (lane >> 4 == half) {                           // this warp's half of the row
-#pragma unroll
-              for (int e = 0; e < E; ++e) {
-                if (whole) op[e] = from_float<T>(acc[e] * ir);
-                else pp[e] = acc[e];
-              }
-            }
+            row_again<T, D>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
+                            half, whole ? static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h : nullptr,
+                            part_row<D>(A.part, grid, cta, first == 0, row));
           }
         }
         tc_fence_before();
@@ -775,7 +857,7 @@ attn_kernel(const AttnArgs A, const __grid_constant__ CUtensorMap k_map, const _
       } else {                                                 // each piece of P: two steps of 32
 #pragma unroll
         for (int n = 0; n < kPieces<T>; ++n)
-          mma_ts_warp<2, true>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys + n * 16, desc, A.group >> 2, idesc_o, n > 0 || !fresh);
+          mma_ts_warp<2, true, 32>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys + n * 8, desc, A.group >> 2, idesc_o, n > 0 || !fresh);
       }
       tc_commit_warp(&bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
