@@ -8,12 +8,13 @@
 // Over an e4m3 cache k_j = ks_j kc_j and v_j = vs_j vc_j (codes and scales), and
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
-// so the weights stay at most 1, whatever the scales. The codes go into the products as they are, on the
-// 8-bit tensor path, and the other operand is cut into e4m3 pieces of 4 bits each: x = x1 + x2 (+ x3), two
-// pieces over bf16 (8 bits) and three over fp16 (11). A query row is first brought to a largest element of
-// 128 to 256 by a power of two, and the weights to at most 2^8.5, so that what e4m3's smallest step (2^-9)
-// loses of a small element is 2^-17 of the largest. (Widening the codes to 16 bits instead took three times
-// as long: the widened tiles' way through shared memory, not the conversion, was the bound.)
+// so the weights stay at most 1, whatever the scales. Scores are formed on the 8-bit tensor path: keys as
+// the codes they are, the query in e4m3 pieces of 4 bits, q = q1 + q2 (+ q3), two over bf16 (8 bits) and
+// three over fp16 (11); a query row is first brought to a largest element of 128 to 256 by a power of two, so
+// that what e4m3's smallest step (2^-9) loses of a small element is 2^-17 of the largest. Value codes are
+// widened to 16 bits (exactly) on their way and meet 16-bit weights. (Both other ways were built: keys
+// widened too spend shared memory's bandwidth, 350 us for 48 decodes of the shape below against 170; weights in
+// pieces spend the conversion unit's, a warp instruction in 16 cycles, 440 us for five prompts.)
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
 #include <algorithm>
@@ -45,21 +46,17 @@ constexpr int kScaleStages = 4;
 constexpr int kTurnPitch = 80;
 constexpr uint32_t kScaleBytes = kKeys * 12;   // a unit's scales: [64] (k's with the softmax's, log2 v's), [64] 1 / v's
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Weights are 2^(x - m). m is set to the maximum less kLift, and moved again (o rescaled) only when the
-// maximum has grown by 2^kSlack since: over 16-bit rows weights are then at most 2^8, far inside both
-// types; over e4m3 between 2^6.5 and 2^8.5, e4m3's upper end.
-template <bool E4M3> constexpr float kLift = E4M3 ? 6.5f : 0.f;
-template <bool E4M3> constexpr float kSlack = E4M3 ? 2.f : 8.f;
+constexpr float kSlack = 8.f;             // o is rescaled only when the maximum has grown by 2^8
 
 // How the cache's rows come in: 16-bit or e4m3, by TMA where boxes of 8 rows or more tile both the pages
 // and the units (gcd(page size, 64) >= 8), else row by row.
 enum Source : int { TMA16 = 0, ROWS16 = 1, TMA8 = 2, ROWS8 = 3 };
 __host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
 __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
-// warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V or four that copy rows, and
-// over e4m3 one that brings the scales
-__host__ __device__ constexpr int load_warps(int src) { return is_tma(src) ? 2 : 4; }
-__host__ __device__ constexpr int threads_of(int src) { return (9 + load_warps(src) + (is_e4m3(src) ? 1 : 0)) * 32; }
+// warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V (over e4m3 one: registers) or
+// four that copy rows, and over e4m3 four that widen V and bring the scales
+__host__ __device__ constexpr int load_warps(int src) { return src == TMA16 ? 2 : src == TMA8 ? 1 : 4; }
+__host__ __device__ constexpr int threads_of(int src) { return (9 + load_warps(src) + (is_e4m3(src) ? 4 : 0)) * 32; }
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -174,10 +171,12 @@ template <int D, int SRC>
 struct Layout {
   static constexpr int kElem = is_e4m3(SRC) ? 1 : 2;                       // stored bytes an element
   static constexpr int kRowB = D * kElem < 128 ? 64 : 128, kSlabs = D * kElem / kRowB;   // a slab's row
-  static constexpr int kStages = SRC == TMA16 && D == 256 ? 3 : SRC == ROWS16 ? 2 : 4;
+  static constexpr int kStages = SRC == ROWS16 ? 2 : D == 256 ? 3 : 4;
   static constexpr uint32_t kTile = kKeys * D * kElem;
-  // a third piece of Q over e4m3 that tensor memory has no room for (D = 256) lies in shared memory
-  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_q3 = 2 * kStages * kTile;
+  // over e4m3: two stages of V widened, [64-column slab][row]; a third piece of Q that tensor memory has no
+  // room for (D = 256)
+  static constexpr uint32_t kWide = kKeys * D * 2;
+  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_w = 2 * kStages * kTile, off_q3 = off_w + (is_e4m3(SRC) ? 2 * kWide : 0);
   static constexpr uint32_t off_turn = off_q3 + (is_e4m3(SRC) && D == 256 ? kM * D : 0);
   static constexpr uint32_t off_scale = off_turn + kSoftWarps * 32 * kTurnPitch;
   static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kScaleBytes : 0) + 1024;
@@ -185,12 +184,13 @@ struct Layout {
   static constexpr uint32_t cols = D == 64 ? 256 : 512;
 };
 
-// full / empty: a stage's tile has landed / its product has read it (sc: a unit's scales). q_ready: Q is in
+// full / empty: a stage's tile has landed / its product has read it (sc: a unit's scales; w: V widened, the
+// codes' stage then free). q_ready: Q is in
 // tensor memory. s_done / o_done: the product S(i) / O += P(i) V(i) has completed. p_full: P(i) is written
 // (and S(i) read). m_set: the rows' maximum after unit i is in shared memory. o_free: the piece's O has
 // been read.
 struct Bars {
-  uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], s_done[2], p_full[2], o_done[2], o_free,
+  uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], w_full[2], w_empty[2], s_done[2], p_full[2], o_done[2], o_free,
       sc_full[kScaleStages], sc_empty[kScaleStages], m_set[2][4], swap[4], drain;
 };
 
@@ -235,8 +235,8 @@ CFB_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
 }
 // D[tmem] (+)= A[tmem] . B[smem] over N steps of 32 bytes of the summed dim in one statement, by one elected
 // lane (one election and one statement for four take less issue time than four), B's descriptor advancing
-// by `step` and A by ASTEP columns. F8: e4m3, else 16-bit operands.
-template <int N, bool F8, int ASTEP = 8>
+// by `step`. F8: e4m3, else 16-bit operands.
+template <int N, bool F8>
 CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t step, uint32_t idesc, uint32_t accumulate) {
 #define CFB_TS4(KIND)                                                                                                        \
   asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
@@ -244,13 +244,13 @@ CFB_DEV void mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t 
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %8, %3, 1;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%6], %9, %3, 1;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%7], %10, %3, 1;\n\t}"                                     \
-               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + ASTEP),                           \
-                  "r"(tmem_a + 2 * ASTEP), "r"(tmem_a + 3 * ASTEP), "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step) : "memory")
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8),                           \
+                  "r"(tmem_a + 16), "r"(tmem_a + 24), "l"(b + step), "l"(b + 2 * step), "l"(b + 3 * step) : "memory")
 #define CFB_TS2(KIND)                                                                                                        \
   asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %4, 0;\n\t"                           \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%1], %2, %3, q;\n\t"                                       \
                "@p tcgen05.mma.cta_group::1.kind::" KIND " [%0], [%5], %6, %3, 1;\n\t}"                                      \
-               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + ASTEP), "l"(b + step) : "memory")
+               :: "r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(tmem_a + 8), "l"(b + step) : "memory")
   static_assert(N == 4 || (N == 2 && F8), "steps");
   if constexpr (!F8) CFB_TS4("f16");
   else if constexpr (N == 4) CFB_TS4("f8f6f4");
@@ -306,6 +306,26 @@ CFB_DEV long long row_offset(const AttnArgs& A, int b, int kh, int j, long long*
   if (scale_off)
     *scale_off = (long long)page * A.c.scale_page_stride + kh * A.c.scale_head_stride + off * A.c.scale_slot_stride;
   return (long long)page * A.c.page_stride + kh * A.c.head_stride + off * A.c.slot_stride;
+}
+
+// eight e4m3 codes -> eight elements of T, exactly: exponent and mantissa bits moved to T's places are the value
+// times 2^(7 - T's bias) (subnormals come out as subnormals), and a product by the inverse undoes that
+template <typename T>
+CFB_DEV uint4 widen8(uint32_t lo, uint32_t hi) {
+  const auto two = [](uint32_t w, uint32_t pick) {
+    const uint32_t t = __byte_perm(w, 0, pick);                // each half: code << 8
+    if constexpr (std::is_same<T, __half>::value) {
+      const uint32_t x = (t & 0x80008000u) | (t >> 1 & 0x3f803f80u);
+      const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(256.f));
+      return *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      const uint32_t x = (t & 0x80008000u) | (t >> 4 & 0x07f007f0u);
+      const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                       __halves2bfloat162(__ushort_as_bfloat16(0x7b80), __ushort_as_bfloat16(0x7b80)));   // 2^120
+      return *reinterpret_cast<const uint32_t*>(&y);
+    }
+  };
+  return make_uint4(two(lo, 0x1404), two(lo, 0x3424), two(hi, 0x1404), two(hi, 0x3424));
 }
 
 // Four values as e4m3: the leading piece, and what it leaves. The piece is the value rounded to 4 bits by an
@@ -407,14 +427,15 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     mbar_init(&bar.q_ready, kSoftWarps);
     for (int i = 0; i < kSt; ++i) {
       mbar_init(&bar.k_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], QUANT ? 4 : 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.w_full[i], 4 * 32); mbar_init(&bar.w_empty[i], 1);
       mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps / 2); mbar_init(&bar.o_done[i], 1);
       for (int j = 0; j < 4; ++j) mbar_init(&bar.m_set[i][j], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
-    for (int i = 0; i < kScaleStages; ++i) { mbar_init(&bar.sc_full[i], 1); mbar_init(&bar.sc_empty[i], kSoftWarps / 2); }
+    for (int i = 0; i < kScaleStages; ++i) { mbar_init(&bar.sc_full[i], kKeys / 32); mbar_init(&bar.sc_empty[i], kSoftWarps / 2); }
     for (int i = 0; i < 4; ++i) mbar_init(&bar.swap[i], 2);
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
@@ -647,7 +668,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             now = sh_m[s ^ 1][r];
           }
           const float before = now;
-          if (now == -INFINITY || high > now + (kLift<QUANT> + kSlack<QUANT>)) now = high - kLift<QUANT>;
+          if (now == -INFINITY || high > now + kSlack) now = high;
           sh_m[s][r] = now;
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
@@ -670,45 +691,28 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           m = now;
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (!QUANT) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t p[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float y[4];
+            for (int e = 0; e < 32; e += 4) {
+              float y[4];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  y[z] = exp2_approx(x[32 * c + e + z] - mm);
-                  sum[z] += y[z];
-                }
-                p[e / 2] = pack16<T>(y[0], y[1]);
-                p[e / 2 + 1] = pack16<T>(y[2], y[3]);
-              }
-              tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
-            }
-          } else {
-            // 32 positions are one step of the product: their pieces go where their scores were
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t pieces[kPieces<T>][8];
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float y[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
+              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
+              if constexpr (QUANT) {
                 const float4 f = sc[kKeys / 2 + 8 * c + e / 4];
                 sum[0] = fmaf(y[0], f.x, sum[0]);
                 sum[1] = fmaf(y[1], f.y, sum[1]);
                 sum[2] = fmaf(y[2], f.z, sum[2]);
                 sum[3] = fmaf(y[3], f.w, sum[3]);
+              } else {
 #pragma unroll
-                for (int n = 0; n < kPieces<T> - 1; ++n) pieces[n][e / 4] = take_piece(y);
-                pieces[kPieces<T> - 1][e / 4] = e4m3_of(y);
+                for (int z = 0; z < 4; ++z) sum[z] += y[z];
               }
-#pragma unroll
-              for (int n = 0; n < kPieces<T>; ++n) tmem_st8(tw + Lay::s_col + s * kKeys + 32 * c + n * 8, pieces[n]);
+              p[e / 2] = pack16<T>(y[0], y[1]);
+              p[e / 2 + 1] = pack16<T>(y[2], y[3]);
             }
+            tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
@@ -825,41 +829,33 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- tensor work
-    // operand formats: 16-bit types, or e4m3 (0); the second product's B is MN-major
-    constexpr uint32_t kTypes = QUANT ? 0u : type_bits<T>();
-    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | kTypes, idesc_o = tc_idesc(kM, D) | kTypes | (1u << 16);
+    // operand formats: 16-bit types, or e4m3 (0) for the scores; the second product's B is MN-major
+    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | (QUANT ? 0u : type_bits<T>()), idesc_o = tc_idesc(kM, D) | type_bits<T>() | (1u << 16);
     constexpr int kRowB = Lay::kRowB;
     uint32_t g = 0, pieces = 0;
     bool ok = true;
     const auto pv = [&](uint32_t u, int i, bool fresh) {       // O (+)= P(u) V(u), u the piece's unit i
-      const int s = u & 1, st = u % kSt;
-      if (!wait(&bar.v_full[st], (u / kSt) & 1)) return false;
-      const uint32_t v = base + Lay::off_v + st * Lay::kTile;
-      if constexpr (is_tma(SRC)) {
+      const int s = u & 1, st = QUANT ? s : u % kSt;
+      uint64_t* const full = QUANT ? &bar.w_full[s] : &bar.v_full[st];
+      if (!wait(full, (QUANT ? u >> 1 : u / kSt) & 1)) return false;
+      const uint32_t v = QUANT ? base + Lay::off_w + s * Lay::kWide : base + Lay::off_v + st * Lay::kTile;
+      if constexpr (SRC == TMA16) {
         // rows past the end hold what the pages or the last tile left there: 0 x NaN must not happen
         const int rows = row_limit(A, w.r, w.r.n - 1) - i * kKeys;
         if (rows < kKeys) {
-          constexpr int kRowP = kRowB / 16;                    // 16-byte pieces of a slab's row
-          for (int x = max(rows, 0) * kRowP + lane; x < kKeys * kRowP; x += 32)
+          for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
 #pragma unroll
-            for (int c = 0; c < Lay::kSlabs; ++c)
-              st_shared16(v + c * A.slab + x / (8 * kRowP) * A.group + x % (8 * kRowP) * 16, 0, 0, 0, 0);
+            for (int c = 0; c < Lay::kSlabs; ++c) st_shared16(v + c * A.slab + (x >> 6) * A.group + (x & 63) * 16, 0, 0, 0, 0);
           fence_async_shared();
           __syncwarp();
         }
       }
       if (!wait(&bar.p_full[s], (u >> 1) & 1)) return false;
-      if constexpr (!is_tma(SRC)) fence_async_shared();        // the tile was stored by threads
+      if constexpr (SRC == ROWS16) fence_async_shared();       // the tile was stored by threads
       tc_fence_after();
-      const uint64_t desc = mn_major<kRowB>(v, A.slab, A.group);
-      if constexpr (!QUANT) {                                  // four steps of 16 positions
-        mma_ts_warp<4, false>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, desc, A.group >> 3, idesc_o, !fresh);
-      } else {                                                 // each piece of P: two steps of 32
-#pragma unroll
-        for (int n = 0; n < kPieces<T>; ++n)
-          mma_ts_warp<2, true, 32>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys + n * 8, desc, A.group >> 2, idesc_o, n > 0 || !fresh);
-      }
-      tc_commit_warp(&bar.v_empty[st]);
+      const uint32_t slab = QUANT ? kKeys * 128u : A.slab, group = QUANT ? 1024u : A.group;
+      mma_ts_warp<4, false>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major<128>(v, slab, group), group >> 3, idesc_o, !fresh);
+      tc_commit_warp(QUANT ? &bar.w_empty[s] : &bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
       return true;
     };
@@ -903,47 +899,70 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     bool ok = true;
     const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
     const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
-    if (QUANT && lw == load_warps(SRC)) {
-      // -------- the scales, two positions a lane, looked up a unit early
-      float2 sc[2];
+    if (QUANT && lw >= load_warps(SRC)) {
+      // -------- V's codes to 16 bits, and (the first two warps, a lane a position) the scales, looked up a unit
+      // early
+      const int cw = lw - load_warps(SRC), ct = cw * 32 + lane;
+      float2 sc = make_float2(0.f, 1.f);
       const auto look = [&](const Walk& w, int i) {
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int j = i * kKeys + z * 32 + lane;
-          sc[z] = make_float2(0.f, 1.f);
-          if (j < row_limit(A, w.r, w.r.n - 1)) {
-            long long so = 0;
-            if (row_offset(A, w.b, w.kh, j, &so) >= 0) sc[z] = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
-            else sc[z].x = __int_as_float(0x7fc00000);         // no such page: its scores are NaN
-          }
+        sc = make_float2(0.f, 1.f);
+        const int j = i * kKeys + ct;
+        if (ct < kKeys && j < row_limit(A, w.r, w.r.n - 1)) {
+          long long so = 0;
+          if (row_offset(A, w.b, w.kh, j, &so) >= 0) sc = make_float2(__ldg(A.c.k_scale + so), __ldg(A.c.v_scale + so));
+          else sc.x = __int_as_float(0x7fc00000);              // no such page: its scores are NaN
         }
       };
+      constexpr int kRowP = D / 16, kPasses = kKeys * kRowP / 128;                   // 16-code pieces of a row; of a lane
       if (!w.done()) look(w, w.first);
       while (ok && !w.done()) {
-        const int stop = w.stop();
+        const int stop = w.stop(), lim = row_limit(A, w.r, w.r.n - 1);
         for (int i = w.first; i < stop; ++i, ++g) {
-          const uint32_t st = g % kScaleStages;
-          if (g >= kScaleStages && !(ok = wait(&bar.sc_empty[st], (g / kScaleStages - 1) & 1))) break;
-          uint8_t* const at = sm + Lay::off_scale + st * kScaleBytes;
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
+          const uint32_t ss = g % kScaleStages, st = g % kSt, ws = g & 1;
+          if (cw < kKeys / 32) {
+            if (g >= kScaleStages && !(ok = wait(&bar.sc_empty[ss], (g / kScaleStages - 1) & 1))) break;
             // a scale of NaN reaches the row through its score; where the row may not see the position, its
             // weight of 0 meets a finite factor
-            reinterpret_cast<float2*>(at)[z * 32 + lane] = make_float2(sc[z].x, log2f(sc[z].y));
-            reinterpret_cast<float*>(at + kKeys * 8)[z * 32 + lane] = sc[z].y > 0.f ? 1.f / sc[z].y : 1.f;
+            uint8_t* const at = sm + Lay::off_scale + ss * kScaleBytes;
+            reinterpret_cast<float2*>(at)[ct] = make_float2(sc.x, log2f(sc.y));
+            reinterpret_cast<float*>(at + kKeys * 8)[ct] = sc.y > 0.f ? 1.f / sc.y : 1.f;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.sc_full[ss]);
+            if (i + 1 < stop) look(w, i + 1);
+          }
+          if (!(ok = wait(&bar.v_full[st], (g / kSt) & 1))) break;
+          uint4 y[kPasses];
+          const uint8_t* const raw = sm + Lay::off_v + st * Lay::kTile;
+#pragma unroll
+          for (int x = 0; x < kPasses; ++x) {
+            const int z = x * 128 + ct, r = z / kRowP, p = z % kRowP;
+            constexpr int kSlabP = Lay::kRowB / 16;
+            const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
+            y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
+            if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);       // past the end: whatever the page holds
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.sc_full[st]);
-          if (i + 1 < stop) look(w, i + 1);
+          if (lane == 0) mbar_arrive(&bar.v_empty[st]);
+          if (g >= 2 && !(ok = wait(&bar.w_empty[ws], ((g >> 1) + 1) & 1))) break;
+#pragma unroll
+          for (int x = 0; x < kPasses; ++x) {
+            const int z = x * 128 + ct, r = z / kRowP, p = z % kRowP;
+            const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
+            const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
+            const int c0 = (p & 3) * 2, odd = p >> 2 & 1;      // (lanes of odd slabs store their halves in the other order: no two on a bank)
+            const uint4 u = odd ? b : a, v = odd ? a : b;
+            st_shared16(row + (((c0 + odd) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+            st_shared16(row + (((c0 + 1 - odd) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+          }
+          fence_async_shared();
+          mbar_arrive(&bar.w_full[ws]);
         }
         if (!ok) break;
         w.next(A);
         if (!w.done()) look(w, w.first);
       }
     } else if constexpr (is_tma(SRC)) {
-      // -------- the two warps that issue TMA copies, of K and of V: a lane a box, whose page it looks up
-      const int kv = lw;
-      const CUtensorMap* const map = kv ? &v_map : &k_map;
+      // -------- the warps that issue TMA copies: a lane a box, whose page it looks up
       const int box = A.box;
       const uint32_t bytes = box * D * Lay::kElem;
       int page = -1, off = 0;
@@ -963,19 +982,24 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       while (ok && !w.done()) {
         const int stop = w.stop();
         for (int i = w.first; i < stop; ++i, ++g) {
-          if (!(ok = kv ? v_free(g) : k_free())) break;
-          const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile + lane * bytes;
-          uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
           const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
-          if (need && page < 0) {                              // no such page: its scores are NaN (over e4m3 by its scales)
-            const uint32_t fill = !QUANT && kv == 0 ? 0x7fff7fffu : 0u;
-            for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
-            fence_async_shared();
+#pragma unroll
+          for (int z = 0; z < (SRC == TMA16 ? 1 : 2); ++z) {
+            const int kv = SRC == TMA16 ? lw : z;
+            if (!(ok = kv ? v_free(g) : k_free())) break;
+            const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile + lane * bytes;
+            uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
+            if (need && page < 0) {                            // no such page: its scores are NaN (over e4m3 by its scales)
+              const uint32_t fill = !QUANT && kv == 0 ? 0x7fff7fffu : 0u;
+              for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
+              fence_async_shared();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
+            __syncwarp();
+            if (need && page >= 0) tma_load_5d(dst, kv ? &v_map : &k_map, 0, off, 0, w.kh, page, full);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
-          __syncwarp();
-          if (need && page >= 0) tma_load_5d(dst, map, 0, off, 0, w.kh, page, full);
+          if (!ok) break;
           if (i + 1 < stop) look(w, i + 1);
         }
         if (!ok) break;
