@@ -107,6 +107,7 @@ CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
 CFB_DEV int head_units(const AttnArgs& A, const Request& r) {
   const int tiles = tiles_of(A, r);
   int u = 0;
+#pragma unroll 1
   for (int t = 0; t < tiles; ++t) u += units_of(A, r, t);
   return u;
 }
@@ -125,6 +126,7 @@ struct Walk {
     kh = (int)(rest <= 0x7fffffff ? (unsigned)rest / (unsigned)per_head : rest / per_head);
     first = (int)(rest - (long long)kh * per_head);
     tile = 0;
+#pragma unroll 1
     for (;;) {
       units = units_of(A, r, tile);
       if (first < units) break;
@@ -351,6 +353,7 @@ template <typename T> constexpr int kPieces = std::is_same<T, __half>::value ? 3
 __device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int* dead) {
   bool ok = true;
   const unsigned long long t0 = globaltimer();
+#pragma unroll 1
   for (unsigned it = 1; !mbar_try_wait(b, parity); ++it)
     if (it % kPollsPerCheck == 0) {
       if (wait_expired(t0, kWaitBudgetNs)) *dead = 1;
@@ -372,6 +375,7 @@ __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T
   float x[E], acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { x[e] = to_float(q[lane * E + e]); acc[e] = 0.f; }
+#pragma unroll 1
   for (int j = from; j < to; ++j) {
     const long long off = row_offset(A, b, kh, j, nullptr);
     if (off < 0) continue;                                     // its score is NaN: so is l, and this row is not here
@@ -453,6 +457,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   // lane a request.
   long long total = 0;
   int per = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < A.B; b0 += 32) {
     per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
     long long sum = (long long)per * A.c.kv_heads;
@@ -467,6 +472,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   w.u = w.end = 0;
   if (from < to) {
     long long before = 0;
+#pragma unroll 1
     for (int b0 = 0;; b0 += 32) {
       if (A.B > 32) per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
       const long long mine = (long long)per * A.c.kv_heads;
@@ -516,6 +522,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       *other = sh_swap[(half ^ 1) * kM + r];
       return true;
     };
+#pragma unroll 1
     for (; !w.done(); g0 += w.stop() - w.first, w.next(A)) {
       const int stop = w.stop(), first = w.first;
       const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
@@ -620,6 +627,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         }
       }
       float m = -INFINITY, l = 0.f;                            // this group's: l in units of 2^m
+#pragma unroll 1
       for (int i = first; i < stop; ++i) {
         const uint32_t g = g0 + (i - first);
         const int s = g & 1;
@@ -803,6 +811,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           // its own positions alone, with m and l as they are.
           const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
           unsigned again = __ballot_sync(0xffffffffu, A.causal && valid && worst != 0.f && l == l && lim < stop * kKeys);
+#pragma unroll 1
           while (again) {
             const int src = __ffs(again) - 1;
             again &= again - 1;
@@ -822,6 +831,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         const long long end = w.u + w.units;                   // w.u: its first unit
         Desc d;
         d.last = cta + 1;
+#pragma unroll 1
         while (share(each, extra, d.last + 1) < end) ++d.last;
         d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * kM; d.err = 0; d.each = each; d.extra = extra;
         A.desc[cta] = d;
@@ -843,6 +853,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         // rows past the end hold what the pages or the last tile left there: 0 x NaN must not happen
         const int rows = row_limit(A, w.r, w.r.n - 1) - i * kKeys;
         if (rows < kKeys) {
+#pragma unroll 1
           for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
 #pragma unroll
             for (int c = 0; c < Lay::kSlabs; ++c) st_shared16(v + c * A.slab + (x >> 6) * A.group + (x & 63) * 16, 0, 0, 0, 0);
@@ -859,8 +870,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       tc_commit_warp(&bar.o_done[s]);
       return true;
     };
+#pragma unroll 1
     for (; ok && !w.done(); w.next(A), ++pieces) {
       const int count = w.stop() - w.first;
+#pragma unroll 1
       for (int i = 0; i < count; ++i, ++g) {
         const int s = g & 1, st = g % kSt;
         if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
@@ -915,8 +928,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       };
       constexpr int kRowP = D / 16, kPasses = kKeys * kRowP / 128;                   // 16-code pieces of a row; of a lane
       if (!w.done()) look(w, w.first);
+#pragma unroll 1
       while (ok && !w.done()) {
         const int stop = w.stop(), lim = row_limit(A, w.r, w.r.n - 1);
+#pragma unroll 1
         for (int i = w.first; i < stop; ++i, ++g) {
           const uint32_t ss = g % kScaleStages, st = g % kSt, ws = g & 1;
           if (cw < kKeys / 32) {
@@ -979,8 +994,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         }
       };
       if (!w.done()) look(w, w.first);
+#pragma unroll 1
       while (ok && !w.done()) {
         const int stop = w.stop();
+#pragma unroll 1
         for (int i = w.first; i < stop; ++i, ++g) {
           const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
 #pragma unroll
@@ -991,6 +1008,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
             if (need && page < 0) {                            // no such page: its scores are NaN (over e4m3 by its scales)
               const uint32_t fill = !QUANT && kv == 0 ? 0x7fff7fffu : 0u;
+#pragma unroll 1
               for (uint32_t x = 0; x < bytes; x += 16) st_shared16(dst + x, fill, fill, fill, fill);
               fence_async_shared();
             }
@@ -1043,8 +1061,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         fill(A.c.v, Lay::off_v + (u % kSt) * Lay::kTile, v_off, &bar.v_full[u % kSt], false);
         return true;
       };
+#pragma unroll 1
       while (ok && !w.done()) {
         const int stop = w.stop();
+#pragma unroll 1
         for (int i = w.first; i < stop; ++i, ++g) {
           if (!(ok = k_free())) break;
           fill(A.c.k, Lay::off_k + (g % kSt) * Lay::kTile, off, &bar.k_full[g % kSt], true);
@@ -1091,6 +1111,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   const int first = cta + (WARPS > 1 ? warp : 0);
+#pragma unroll 1
   for (int c0 = first; c0 <= last; c0 += kBatch * WARPS) {
     float x[kBatch][E], pm[kBatch], pl[kBatch];
 #pragma unroll
