@@ -37,7 +37,7 @@ namespace {
 // which attn_join_kernel adds up in unit order; a share holds at most two such pieces (its first and
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
-constexpr int kM = 128, kKeys = 64;
+constexpr int kM = 128, kKeys = 64, kFewRows = 32;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4;
 constexpr int kScaleStages = 4;
 // A softmax thread holds a row; memory wants a warp's access to run along rows. 64 bytes of 32 rows at a time
@@ -68,6 +68,7 @@ struct AttnArgs {
   float* lse;
   float scale;
   int T, B, H, causal, rep;
+  int m;                                  // rows of a row tile
   int box;                                // rows of a TMA box
   uint32_t slab, group;                   // bytes between a tile's 64-column slabs and its 8-row groups
   struct Desc* desc;                      // [grid]
@@ -99,16 +100,31 @@ CFB_DEV Request request(const AttnArgs& A, int b) {
 CFB_DEV int row_limit(const AttnArgs& A, const Request& r, int tok) {      // positions that token `tok` may see
   return A.causal ? max(min(r.L - r.n + tok + 1, r.L), 0) : r.L;
 }
-CFB_DEV int tiles_of(const AttnArgs& A, const Request& r) { return (r.n * A.rep + kM - 1) / kM; }
+CFB_DEV int tiles_of(const AttnArgs& A, const Request& r) { return (r.n * A.rep + A.m - 1) / A.m; }
 CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
-  const int last = (min((tile + 1) * kM, r.n * A.rep) - 1) / A.rep;
+  const int last = (min((tile + 1) * A.m, r.n * A.rep) - 1) / A.rep;
   return max(1, (row_limit(A, r, last) + kKeys - 1) / kKeys);
 }
-CFB_DEV int head_units(const AttnArgs& A, const Request& r) {
+// A kv head's units of request b (0 past the last), for the warp's 32 requests at once: a lane each where all have
+// one tile, else a request at a time with a lane a tile (one prompt of 1500 tokens has 47).
+__device__ __noinline__ int head_units(const AttnArgs& A, int b) {
+  const int lane = threadIdx.x & 31;
+  Request r = {0, 0, 0, false};
+  if (b < A.B) r = request(A, b);
   const int tiles = tiles_of(A, r);
-  int u = 0;
+  unsigned longer = __ballot_sync(0xffffffffu, tiles > 1);
+  int u = tiles == 1 ? units_of(A, r, 0) : 0;
 #pragma unroll 1
-  for (int t = 0; t < tiles; ++t) u += units_of(A, r, t);
+  for (; longer; longer &= longer - 1) {
+    const int x = __ffs(longer) - 1;
+    const Request y = {0, __shfl_sync(0xffffffffu, r.n, x), __shfl_sync(0xffffffffu, r.L, x), false};
+    const int n = tiles_of(A, y);
+    int sum = 0;
+#pragma unroll 1
+    for (int t = lane; t < n; t += 32) sum += units_of(A, y, t);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == x) u = sum;
+  }
   return u;
 }
 
@@ -125,13 +141,26 @@ struct Walk {
     tiles = tiles_of(A, r);
     kh = (int)(rest <= 0x7fffffff ? (unsigned)rest / (unsigned)per_head : rest / per_head);
     first = (int)(rest - (long long)kh * per_head);
-    tile = 0;
+    // the tile that holds it: 32 at a time, a lane a tile
+    const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (;;) {
-      units = units_of(A, r, tile);
-      if (first < units) break;
-      first -= units;
-      ++tile;
+    for (tile = 0;; tile += 32) {
+      const int mine = tile + lane < tiles ? units_of(A, r, tile + lane) : 0;
+      int run = mine;
+#pragma unroll 1
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, run, off);
+        if (lane >= off) run += y;
+      }
+      const unsigned here = __ballot_sync(0xffffffffu, first < run);
+      if (here) {
+        const int x = __ffs(here) - 1;
+        tile += x;
+        units = __shfl_sync(0xffffffffu, mine, x);
+        first -= __shfl_sync(0xffffffffu, run - mine, x);
+        break;
+      }
+      first -= __shfl_sync(0xffffffffu, run, 31);
     }
   }
   CFB_DEV bool done() const { return u >= end; }
@@ -192,7 +221,7 @@ struct Layout {
 // (and S(i) read). m_set: the rows' maximum after unit i is in shared memory. o_free: the piece's O has
 // been read.
 struct Bars {
-  uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], w_full[2], w_empty[2], s_done[2], p_full[2], o_done[2], o_free,
+  uint64_t q_ready, k_full[4], k_empty[4], v_full[4], v_empty[4], w_full[2], w_empty[2], s_done[2], p_full[2], o_done[2], o_free, meet,
       sc_full[kScaleStages], sc_empty[kScaleStages], m_set[2][4], swap[4], drain;
 };
 
@@ -214,16 +243,6 @@ CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
 }
 CFB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 CFB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-CFB_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 CFB_DEV void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
@@ -349,6 +368,23 @@ CFB_DEV uint32_t take_piece(float (&x)[4]) {
 }
 template <typename T> constexpr int kPieces = std::is_same<T, __half>::value ? 3 : 2;
 
+// eight elements of a query row, times `up`, in pieces
+template <typename T> struct QPieces { uint32_t w[kPieces<T>][2]; };
+template <typename T>
+__device__ __noinline__ QPieces<T> query_pieces(uint4 q, float up) {
+  QPieces<T> p;
+  const uint32_t y[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    const float2 f = unpack16<T>(y[2 * z]), h = unpack16<T>(y[2 * z + 1]);
+    float v[4] = {f.x * up, f.y * up, h.x * up, h.y * up};
+#pragma unroll
+    for (int n = 0; n < kPieces<T> - 1; ++n) p.w[n][z] = take_piece(v);
+    p.w[kPieces<T> - 1][z] = e4m3_of(v);
+  }
+  return p;
+}
+
 // The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not.
 __device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int* dead) {
   bool ok = true;
@@ -410,18 +446,20 @@ __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T
 // operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of
 // the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^8 since
 // the last time: weights are then at most 2^8, far inside both types, and most units touch O not at all.
-template <typename T, int D, int SRC>
+template <typename T, int D, int SRC, int M>
 __global__ void __launch_bounds__(threads_of(SRC), 1)
 attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using Lay = Layout<D, SRC>;
   constexpr bool QUANT = is_e4m3(SRC);
+  constexpr bool SPREAD = M < kM;
+  constexpr int kCols = kKeys / (kM / M);                      // a unit's columns of a softmax thread
   constexpr int kSt = Lay::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   __shared__ float sh_m[2][kM];
-  __shared__ float2 sh_swap[2 * kM];
+  __shared__ float2 sh_swap[2 * kM];                           // [group][lane of tensor memory]: its maximum and sum
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,19 +467,25 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_ready, kSoftWarps);
+#pragma unroll 1
     for (int i = 0; i < kSt; ++i) {
       mbar_init(&bar.k_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.k_empty[i], 1);
       mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], QUANT ? 4 : 1);
     }
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.w_full[i], 4 * 32); mbar_init(&bar.w_empty[i], 1);
       mbar_init(&bar.s_done[i], 1); mbar_init(&bar.p_full[i], kSoftWarps / 2); mbar_init(&bar.o_done[i], 1);
+#pragma unroll 1
       for (int j = 0; j < 4; ++j) mbar_init(&bar.m_set[i][j], 1);
     }
     mbar_init(&bar.o_free, kSoftWarps);
+#pragma unroll 1
     for (int i = 0; i < kScaleStages; ++i) { mbar_init(&bar.sc_full[i], kKeys / 32); mbar_init(&bar.sc_empty[i], kSoftWarps / 2); }
+#pragma unroll 1
     for (int i = 0; i < 4; ++i) mbar_init(&bar.swap[i], 2);
     mbar_init(&bar.drain, 1);
+    mbar_init(&bar.meet, kSoftWarps);
     fence_mbar_init();
     dead = 0;
     A.desc[cta].last = -1;
@@ -459,7 +503,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   int per = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < A.B; b0 += 32) {
-    per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
+    per = head_units(A, b0 + lane);
     long long sum = (long long)per * A.c.kv_heads;
 #pragma unroll
     for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -474,7 +518,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     long long before = 0;
 #pragma unroll 1
     for (int b0 = 0;; b0 += 32) {
-      if (A.B > 32) per = b0 + lane < A.B ? head_units(A, request(A, b0 + lane)) : 0;
+      if (A.B > 32) per = head_units(A, b0 + lane);
       const long long mine = (long long)per * A.c.kv_heads;
       long long run = mine;                                    // inclusive scan
 #pragma unroll
@@ -508,9 +552,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     // row's maximum passes from unit to unit through shared memory; each group keeps its own sum.
     const int half = warp >> 2, pair = warp & 3;               // warps w and w + 4 share 32 rows
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
-    const int r = pair * 32 + lane;
+    const int r = pair * 32 + lane, tr = SPREAD ? lane : r;    // lane of tensor memory, row of the tile
+    const int col0 = SPREAD ? pair * kCols : 0;
     const float c2 = A.scale * kLog2e;
-    uint32_t g0 = 0, swaps = 0;                                // units before this piece; exchanges of the two groups
+    uint32_t g0 = 0, swaps = 0, meets = 0;                     // units before this piece; exchanges of the two groups, of all eight warps
     uint8_t* const turn = sm + Lay::off_turn + warp * (32 * kTurnPitch);
     uint8_t* const turn_row = turn + lane * kTurnPitch;                              // this lane's row
     uint8_t* const turn_at = turn + (lane >> 2) * kTurnPitch + (lane & 3) * 16;      // its piece of row lane / 4, then every 8th
@@ -522,14 +567,19 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       *other = sh_swap[(half ^ 1) * kM + r];
       return true;
     };
+    const auto meet = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.meet);
+      return wait(&bar.meet, meets++ & 1);
+    };
 #pragma unroll 1
     for (; !w.done(); g0 += w.stop() - w.first, w.next(A)) {
       const int stop = w.stop(), first = w.first;
-      const int rows = min(kM, w.r.n * A.rep - w.tile * kM);
-      const bool valid = r < rows;
-      const int R = w.tile * kM + r, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
+      const int rows = min(M, w.r.n * A.rep - w.tile * M);
+      const bool valid = tr < rows;
+      const int R = w.tile * M + tr, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
       const int lim = valid ? row_limit(A, w.r, tok) : 0;
-      const bool warp_live = pair * 32 < rows;
+      const bool warp_live = SPREAD || pair * 32 < rows;
       bool ok = true;
       // Q to tensor memory, a half of the head dim a group
       float rowf = c2;                                         // the softmax's scale, with the row's own over e4m3
@@ -587,14 +637,11 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             uint32_t piece[kPieces<T>][8];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const uint32_t ys[4] = {y[c][x].x, y[c][x].y, y[c][x].z, y[c][x].w};
+              const QPieces<T> z = query_pieces<T>(y[c][x], up);
 #pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const float2 f = unpack16<T>(ys[2 * z]), h = unpack16<T>(ys[2 * z + 1]);
-                float v[4] = {f.x * up, f.y * up, h.x * up, h.y * up};
-#pragma unroll
-                for (int n = 0; n < kPieces<T> - 1; ++n) piece[n][2 * x + z] = take_piece(v);
-                piece[kPieces<T> - 1][2 * x + z] = e4m3_of(v);
+              for (int n = 0; n < kPieces<T>; ++n) {
+                piece[n][2 * x] = z.w[n][0];
+                piece[n][2 * x + 1] = z.w[n][1];
               }
             }
 #pragma unroll
@@ -619,7 +666,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 
       // the next tile's Q (of the same heads and request, the common case), into L2 by the time it is wanted
       if (w.tile + 1 < w.tiles && valid && w.u + (stop - first) < w.end) {
-        const int next = R + kM, nt = next / A.rep;
+        const int next = R + M, nt = next / A.rep;
         if (nt < w.r.n) {
           const T* p = static_cast<const T*>(A.q) + (long long)(w.r.t0 + nt) * A.sq_t + (w.kh * A.rep + next - nt * A.rep) * A.sq_h + half * (D / 2);
 #pragma unroll
@@ -637,16 +684,19 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           tc_fence_after();
           const float4* const sc = reinterpret_cast<const float4*>(sm + Lay::off_scale + (g % kScaleStages) * kScaleBytes);
           const int j0 = i * kKeys;
-          const bool masked = __any_sync(0xffffffffu, lim < j0 + kKeys);
+          const bool masked = __any_sync(0xffffffffu, lim < j0 + col0 + kCols);
           if (QUANT && !(ok = wait(&bar.sc_full[g % kScaleStages], (g / kScaleStages) & 1))) break;
-          // the scaled scores of the columns from 32 c on
-          const auto scores = [&](int c, float* x) {
-            tmem_ld32(tw + Lay::s_col + s * kKeys + 32 * c, x);
+          // the scaled scores of this thread's columns
+          float x[kCols];
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32) {
+            if constexpr (SPREAD) tmem_ld16(tw + Lay::s_col + s * kKeys + col0, x);
+            else tmem_ld32(tw + Lay::s_col + s * kKeys + c, x + c);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
+            for (int e = c; e < c + 32 && e < kCols; e += 2) {
               if constexpr (QUANT) {
-                const float4 f = sc[16 * c + e / 2];
+                const float4 f = sc[(col0 + e) / 2];
                 x[e] = fmaf(x[e] * rowf, f.x, f.y);
                 x[e + 1] = fmaf(x[e + 1] * rowf, f.z, f.w);
               } else {
@@ -654,22 +704,16 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
                 x[e + 1] *= c2;
               }
             }
-            if (masked) {
+          }
+          if (masked) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (j0 + 32 * c + e >= lim) x[e] = -INFINITY;
-            }
-          };
-          const auto top_of = [](const float* x, float high) {
-            float top[4] = {high, -INFINITY, -INFINITY, -INFINITY};
+            for (int e = 0; e < kCols; ++e)
+              if (j0 + col0 + e >= lim) x[e] = -INFINITY;
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
-            return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          };
-          float x[kKeys];
-          scores(0, x);
-          scores(1, x + 32);
-          const float high = top_of(x + 32, top_of(x, -INFINITY));
+          for (int e = 0; e < kCols; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
           float now = -INFINITY;                               // the maximum the weights so far are relative to
           if (i > first) {
             if (!(ok = wait(&bar.m_set[s ^ 1][pair], ((g - 1) >> 1) & 1))) break;
@@ -700,15 +744,15 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           const float mm = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < kCols; c += 32) {
             uint32_t p[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 32 && e < kCols; e += 4) {
               float y[4];
 #pragma unroll
-              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[32 * c + e + z] - mm);
+              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[c + e + z] - mm);
               if constexpr (QUANT) {
-                const float4 f = sc[kKeys / 2 + 8 * c + e / 4];
+                const float4 f = sc[kKeys / 2 + (col0 + c + e) / 4];
                 sum[0] = fmaf(y[0], f.x, sum[0]);
                 sum[1] = fmaf(y[1], f.y, sum[1]);
                 sum[2] = fmaf(y[2], f.z, sum[2]);
@@ -720,7 +764,16 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               p[e / 2] = pack16<T>(y[0], y[1]);
               p[e / 2 + 1] = pack16<T>(y[2], y[3]);
             }
-            tmem_st16(tw + Lay::s_col + s * kKeys + c * 16, p);
+            if constexpr (SPREAD) {                            // the other lanes' columns have no weight here
+              const uint32_t none[8] = {};
+              const uint32_t at = tw + Lay::s_col + s * kKeys;
+              tmem_st8(at + 8 * pair, p);
+              tmem_st8(at + 8 * (pair ^ 1), none);
+              tmem_st8(at + 8 * (pair ^ 2), none);
+              tmem_st8(at + 8 * (pair ^ 3), none);
+            } else {
+              tmem_st16(tw + Lay::s_col + s * kKeys + c / 2, p);
+            }
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
@@ -741,63 +794,104 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       tc_fence_after();
       if (warp_live) {
         const bool whole = first == 0 && stop == w.units;
-        // the two groups' sums, relative to the later maximum
-        float2 other;
-        if (!exchange(make_float2(m, l), &other)) break;
-        const float top = fmaxf(m, other.x);
-        const auto to_top = [&](float mm, float ll) { return mm == top || mm == -INFINITY ? ll : ll * exp2_approx(mm - top); };
-        l = to_top(m, l) + to_top(other.x, other.y);
-        m = top;
+        // the groups' sums (SPREAD: of all the row's lanes) relative to the latest maximum, which this lane's
+        // O then meets by `mine`
+        float mine = 1.f;
+        if constexpr (SPREAD) {
+          sh_swap[half * kM + r] = make_float2(m, l);
+          if (!meet()) break;
+          float lane_m = -INFINITY, top = -INFINITY;
+#pragma unroll
+          for (int z = 0; z < kSoftWarps; ++z) top = fmaxf(top, sh_swap[z * 32 + lane].x);
+          lane_m = fmaxf(m, sh_swap[(half ^ 1) * kM + r].x);
+          l = 0.f;
+#pragma unroll
+          for (int z = 0; z < kSoftWarps; ++z) {
+            const float2 y = sh_swap[z * 32 + lane];
+            l += y.x == -INFINITY ? y.y : y.y * exp2_approx(y.x - top);
+          }
+          mine = lane_m == -INFINITY ? 1.f : exp2_approx(lane_m - top);
+          m = top;
+        } else {
+          float2 other;
+          if (!exchange(make_float2(m, l), &other)) break;
+          const float top = fmaxf(m, other.x);
+          const auto to_top = [&](float mm, float ll) { return mm == top || mm == -INFINITY ? ll : ll * exp2_approx(mm - top); };
+          l = to_top(m, l) + to_top(other.x, other.y);
+          m = top;
+        }
         if (w.r.over) l = __int_as_float(0x7fc00000);
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        float* const part = part_row<D>(A.part, grid, cta, first == 0, r);
+        float* const part = part_row<D>(A.part, grid, cta, first == 0, tr);
         const long long o_off = (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
         float bad[4] = {0.f, 0.f, 0.f, 0.f};                   // turn NaN where an element is not finite
+        const auto put = [&](float4 y, float row_inv, float row_l, long long off, int row, int d) {      // four columns of a row
+          if (whole)
+            *reinterpret_cast<uint2*>(static_cast<T*>(A.o) + off + d) =
+                row_l == 0.f ? make_uint2(0, 0) : make_uint2(pack16<T>(y.x * row_inv, y.y * row_inv), pack16<T>(y.z * row_inv, y.w * row_inv));
+          else
+            *reinterpret_cast<float4*>(part_row<D>(A.part, grid, cta, first == 0, row) + d) = y;
+        };
+        if constexpr (SPREAD) {
+          // The row's four lanes are added up through the warps' buffers, 64 columns at a time (16 where there are
+          // more than 8 rows): warp `pair` then takes a quarter of the rows, four columns a lane.
+          const int per_row = rows <= 8 ? 16 : 4, pitch = per_row * 16 + 16;                // 16-byte pieces; bytes
+          const int row = (pair * 32 + lane) / per_row, piece = lane % per_row;
+          const long long off = __shfl_sync(0xffffffffu, o_off, row);
+          const float row_inv = __shfl_sync(0xffffffffu, inv, row), row_l = __shfl_sync(0xffffffffu, l, row);
+          uint8_t* const mine4 = turn + lane * pitch;
+          const uint8_t* const from4 = turn - pair * (32 * kTurnPitch) + row * pitch + piece * 16;
 #pragma unroll 1
-        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
-          float o[32];
-          tmem_ld32(tw + Lay::o_col + d, o);
-          tmem_wait_ld();
+          for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 4 * per_row) {
+#pragma unroll 1
+            for (int x = 0; x < 4 * per_row && d + x < (half + 1) * (D / 2); x += 16) {
+              float o[16];
+              tmem_ld16(tw + Lay::o_col + d + x, o);
+              tmem_wait_ld();
+              if (lane < rows) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if constexpr (!QUANT) bad[e & 3] = fmaf(o[e], 0.f, bad[e & 3]);
-          if (whole) {
+                for (int e = 0; e < 4; ++e)
+                  *reinterpret_cast<float4*>(mine4 + x * 4 + e * 16) = make_float4(o[4 * e] * mine, o[4 * e + 1] * mine, o[4 * e + 2] * mine, o[4 * e + 3] * mine);
+              }
+            }
+            if (!(ok = meet())) break;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < rows && d + piece * 4 < (half + 1) * (D / 2)) {
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                const float4 v = *reinterpret_cast<const float4*>(from4 + z * (32 * kTurnPitch));
+                y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+              }
+              if constexpr (!QUANT) bad[0] = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, bad[0]))));
+              put(y, row_inv, row_l, off, row, d + piece * 4);
+            }
+            if (!(ok = meet())) break;
+          }
+          if (!ok) break;
+        } else {
+#pragma unroll 1
+          for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
+            float o[16];
+            tmem_ld16(tw + Lay::o_col + d, o);
+            tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float* y = o + 8 * e;
-              *reinterpret_cast<uint4*>(turn_row + e * 16) =
-                  l == 0.f ? make_uint4(0, 0, 0, 0)
-                           : make_uint4(pack16<T>(y[0] * inv, y[1] * inv), pack16<T>(y[2] * inv, y[3] * inv),
-                                        pack16<T>(y[4] * inv, y[5] * inv), pack16<T>(y[6] * inv, y[7] * inv));
+              if constexpr (!QUANT) bad[e] = fmaf(o[4 * e], 0.f, fmaf(o[4 * e + 1], 0.f, fmaf(o[4 * e + 2], 0.f, fmaf(o[4 * e + 3], 0.f, bad[e]))));
+              *reinterpret_cast<float4*>(turn_row + e * 16) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
             __syncwarp();
-#pragma unroll
+#pragma unroll 1
             for (int x = 0; x < 4; ++x) {
               const int row = x * 8 + (lane >> 2);
               const long long off = __shfl_sync(0xffffffffu, o_off, row);
+              const float row_inv = __shfl_sync(0xffffffffu, inv, row), row_l = __shfl_sync(0xffffffffu, l, row);
               if (pair * 32 + row < rows)
-                *(reinterpret_cast<uint4*>(static_cast<T*>(A.o) + off + d) + (lane & 3)) = *reinterpret_cast<const uint4*>(turn_at + x * 8 * kTurnPitch);
+                put(*reinterpret_cast<const float4*>(turn_at + x * 8 * kTurnPitch), row_inv, row_l, off, pair * 32 + row, d + (lane & 3) * 4);
             }
             __syncwarp();
-          } else {
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {                      // 16 columns a turn
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<float4*>(turn_row + e * 16) = make_float4(o[16 * z + 4 * e], o[16 * z + 4 * e + 1], o[16 * z + 4 * e + 2], o[16 * z + 4 * e + 3]);
-              __syncwarp();
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const int row = x * 8 + (lane >> 2);
-                if (pair * 32 + row < rows)
-                  *(reinterpret_cast<float4*>(part_row<D>(A.part, grid, cta, first == 0, pair * 32 + row) + d + 16 * z) + (lane & 3)) =
-                      *reinterpret_cast<const float4*>(turn_at + x * 8 * kTurnPitch);
-              }
-              __syncwarp();
-            }
           }
         }
-        if (valid && half == 0) {
+        if (valid && half == 0 && (!SPREAD || pair == 0)) {
           if (!whole) {
             part[D] = m;
             part[D + 1] = l;
@@ -809,14 +903,23 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           // A value that is not finite at a position that this row may not see has met a weight of 0 in
           // the product. Only a causal row's last units can hold one; such a row is taken again from
           // its own positions alone, with m and l as they are.
+          // (SPREAD: a position's weight is 0 in three of a row's lanes, so any such value does this.)
           const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
-          unsigned again = __ballot_sync(0xffffffffu, A.causal && valid && worst != 0.f && l == l && lim < stop * kKeys);
+          const int seen = min(lim, stop * kKeys);             // where its positions here end
+          unsigned again = __ballot_sync(0xffffffffu, worst != 0.f);
+          const unsigned take = __ballot_sync(0xffffffffu, valid && l == l && (SPREAD || (A.causal && lim < stop * kKeys)));
+          if constexpr (SPREAD) {                              // from the lanes that added a row up to the row's own
+            const int per_row = rows <= 8 ? 16 : 4, base_row = pair * 32 / per_row;
+            again = __ballot_sync(0xffffffffu, lane >= base_row && lane < base_row + 32 / per_row &&
+                                                   (again >> ((lane - base_row) * per_row & 31) & ((1u << per_row) - 1)) != 0);
+          }
+          again &= take;
 #pragma unroll 1
           while (again) {
             const int src = __ffs(again) - 1;
             again &= again - 1;
-            const int row = pair * 32 + src, RR = w.tile * kM + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
-            const int li = __shfl_sync(0xffffffffu, lim, src);
+            const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
+            const int li = __shfl_sync(0xffffffffu, seen, src);
             const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
             row_again<T, D>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
                             half, whole ? static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h : nullptr,
@@ -833,7 +936,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         d.last = cta + 1;
 #pragma unroll 1
         while (share(each, extra, d.last + 1) < end) ++d.last;
-        d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * kM; d.err = 0; d.each = each; d.extra = extra;
+        d.kh = w.kh; d.t0 = w.r.t0; d.rows = rows; d.row0 = w.tile * M; d.err = 0; d.each = each; d.extra = extra;
         A.desc[cta] = d;
       }
     }
@@ -874,34 +977,35 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     for (; ok && !w.done(); w.next(A), ++pieces) {
       const int count = w.stop() - w.first;
 #pragma unroll 1
-      for (int i = 0; i < count; ++i, ++g) {
-        const int s = g & 1, st = g % kSt;
-        if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
-        if (!(ok = wait(&bar.k_full[st], (g / kSt) & 1))) break;
-        if constexpr (!is_tma(SRC)) fence_async_shared();
-        tc_fence_after();
-        const uint32_t k_at = base + Lay::off_k + st * Lay::kTile;
-#pragma unroll
-        for (int n = 0; n < (QUANT ? kPieces<T> : 1); ++n)
-#pragma unroll
-          for (int k = 0; k < Lay::kSlabs; ++k) {
-            const uint64_t desc = k_major<kRowB>(k_at + k * A.slab, A.group);
-            if (QUANT && D == 256 && n == 2)
-              mma_ss4_f8_warp(tmem + Lay::s_col + s * kKeys, k_major<128>(base + Lay::off_q3 + k * (kM * 128), 1024), desc, idesc_s);
-            else
-              mma_ts_warp<kRowB / 32, QUANT>(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + n * (D / 4) + k * 32, desc, 2, idesc_s, n + k > 0);
-          }
-        tc_commit_warp(&bar.s_done[s]);
-        tc_commit_warp(&bar.k_empty[st]);
+      for (int i = 0; i <= count; ++i) {                       // S(i), then O(i - 1)
+        if (i < count) {
+          const uint32_t u = g + i;
+          const int s = u & 1, st = u % kSt;
+          if (i == 0 && !(ok = wait(&bar.q_ready, pieces & 1))) break;
+          if (!(ok = wait(&bar.k_full[st], (u / kSt) & 1))) break;
+          if constexpr (!is_tma(SRC)) fence_async_shared();
+          tc_fence_after();
+          const uint32_t k_at = base + Lay::off_k + st * Lay::kTile;
+#pragma unroll 1
+          for (int n = 0; n < (QUANT ? kPieces<T> : 1); ++n)
+#pragma unroll 1
+            for (int k = 0; k < Lay::kSlabs; ++k) {
+              const uint64_t desc = k_major<kRowB>(k_at + k * A.slab, A.group);
+              if (QUANT && D == 256 && n == 2)
+                mma_ss4_f8_warp(tmem + Lay::s_col + s * kKeys, k_major<128>(base + Lay::off_q3 + k * (kM * 128), 1024), desc, idesc_s);
+              else
+                mma_ts_warp<kRowB / 32, QUANT>(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + n * (D / 4) + k * 32, desc, 2, idesc_s, n + k > 0);
+            }
+          tc_commit_warp(&bar.s_done[s]);
+          tc_commit_warp(&bar.k_empty[st]);
+        }
         if (i > 0) {
           // the piece's first product overwrites O: the last piece's must have been read
           if (i == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
-          if (!(ok = pv(g - 1, w.first + i - 1, i == 1))) break;
+          if (!(ok = pv(g + i - 1, w.first + i - 1, i == 1))) break;
         }
       }
-      if (!ok) break;
-      if (count == 1 && pieces > 0 && !(ok = wait(&bar.o_free, (pieces - 1) & 1))) break;
-      ok = pv(g - 1, w.first + count - 1, count == 1);
+      g += count;
     }
     tc_commit_warp(&bar.drain);                                // everything issued has completed
     mbar_wait(&bar.drain, 0);
@@ -926,7 +1030,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           else sc.x = __int_as_float(0x7fc00000);              // no such page: its scores are NaN
         }
       };
-      constexpr int kRowP = D / 16, kPasses = kKeys * kRowP / 128;                   // 16-code pieces of a row; of a lane
+      constexpr int kRowP = D / 16, kPasses = kKeys * kRowP / 128, kBatch = kPasses < 4 ? kPasses : 4;    // 16-code pieces of a row; of a lane; in flight
       if (!w.done()) look(w, w.first);
 #pragma unroll 1
       while (ok && !w.done()) {
@@ -946,29 +1050,35 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             if (i + 1 < stop) look(w, i + 1);
           }
           if (!(ok = wait(&bar.v_full[st], (g / kSt) & 1))) break;
-          uint4 y[kPasses];
           const uint8_t* const raw = sm + Lay::off_v + st * Lay::kTile;
+#pragma unroll 1
+          for (int x0 = 0; x0 < kPasses; x0 += kBatch) {
+            uint4 y[kBatch];
 #pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const int z = x * 128 + ct, r = z / kRowP, p = z % kRowP;
-            constexpr int kSlabP = Lay::kRowB / 16;
-            const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
-            y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
-            if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);       // past the end: whatever the page holds
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.v_empty[st]);
-          if (g >= 2 && !(ok = wait(&bar.w_empty[ws], ((g >> 1) + 1) & 1))) break;
+            for (int x = 0; x < kBatch; ++x) {
+              const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
+              constexpr int kSlabP = Lay::kRowB / 16;
+              const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
+              y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
+              if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);     // past the end: whatever the page holds
+            }
+            if (x0 + kBatch >= kPasses) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar.v_empty[st]);
+            }
+            if (x0 == 0 && g >= 2 && !(ok = wait(&bar.w_empty[ws], ((g >> 1) + 1) & 1))) break;
 #pragma unroll
-          for (int x = 0; x < kPasses; ++x) {
-            const int z = x * 128 + ct, r = z / kRowP, p = z % kRowP;
-            const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
-            const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
-            const int c0 = (p & 3) * 2, odd = p >> 2 & 1;      // (lanes of odd slabs store their halves in the other order: no two on a bank)
-            const uint4 u = odd ? b : a, v = odd ? a : b;
-            st_shared16(row + (((c0 + odd) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
-            st_shared16(row + (((c0 + 1 - odd) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+            for (int x = 0; x < kBatch; ++x) {
+              const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
+              const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
+              const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
+              const int c0 = (p & 3) * 2, odd = p >> 2 & 1;    // (lanes of odd slabs store their halves in the other order: no two on a bank)
+              const uint4 u = odd ? b : a, v = odd ? a : b;
+              st_shared16(row + (((c0 + odd) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+              st_shared16(row + (((c0 + 1 - odd) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+            }
           }
+          if (!ok) break;
           fence_async_shared();
           mbar_arrive(&bar.w_full[ws]);
         }
@@ -1214,15 +1324,15 @@ bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int SRC>
+template <typename T, int D, int SRC, int M>
 cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
-  if (allow_smem<attn_kernel<T, D, SRC>>((int)Layout<D, SRC>::bytes) != cudaSuccess)
+  if (allow_smem<attn_kernel<T, D, SRC, M>>((int)Layout<D, SRC>::bytes) != cudaSuccess)
     return cfb_launch_status("attn_kernel attribute");
-  attn_kernel<T, D, SRC><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
+  attn_kernel<T, D, SRC, M><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
   if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;
-  const long long rows = std::min((long long)kM, (long long)A.T * A.rep);
+  const long long rows = std::min((long long)M, (long long)A.T * A.rep);
   // pieces: at least a row tile a kv head and request that has tokens; parts of one: the CTAs over those
-  const long long pieces = (long long)A.c.kv_heads * std::max((long long)std::min(A.B, A.T), ((long long)A.T * A.rep + kM - 1) / kM);
+  const long long pieces = (long long)A.c.kv_heads * std::max((long long)std::min(A.B, A.T), ((long long)A.T * A.rep + M - 1) / M);
   const bool many = grid > 8 * pieces;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1236,13 +1346,17 @@ cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStre
   cudaLaunchKernelEx(&cfg, many ? attn_join_kernel<T, D, kJoinWarps> : attn_join_kernel<T, D, 1>, A);
   return cfb_launch_status("attn_join_kernel");
 }
+template <typename T, int D, int SRC>
+cfb_status launch_rows(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
+  return A.m == kM ? launch<T, D, SRC, kM>(A, maps, grid, st) : launch<T, D, SRC, kFewRows>(A, maps, grid, st);
+}
 template <typename T, int D>
 cfb_status launch_source(const AttnArgs& A, int src, const CUtensorMap* maps, int grid, cudaStream_t st) {
   switch (src) {
-    case TMA16: return launch<T, D, TMA16>(A, maps, grid, st);
-    case ROWS16: return launch<T, D, ROWS16>(A, maps, grid, st);
-    case TMA8: return launch<T, D, TMA8>(A, maps, grid, st);
-    default: return launch<T, D, ROWS8>(A, maps, grid, st);
+    case TMA16: return launch_rows<T, D, TMA16>(A, maps, grid, st);
+    case ROWS16: return launch_rows<T, D, ROWS16>(A, maps, grid, st);
+    case TMA8: return launch_rows<T, D, TMA8>(A, maps, grid, st);
+    default: return launch_rows<T, D, ROWS8>(A, maps, grid, st);
   }
 }
 template <typename T>
@@ -1294,8 +1408,9 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   const int fit = std::gcd(c->page_size, kKeys), box = fit < kKeys ? std::min(fit, 8) : fit;
   const uint32_t row = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) < 128 ? 64 : 128, slabs = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) / row;
   const bool grouped = box == 8;
+  const int rep = H / c->kv_heads, m = (long long)T * rep <= (long long)kFewRows * B ? kFewRows : kM;
   const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-                   T, B, H, causal, H / c->kv_heads, box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
+                   T, B, H, causal, rep, m, box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
                    static_cast<Desc*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
   CUtensorMap maps[2] = {};
   const bool tma = box >= 8 && pool_map(&maps[0], *c, c->k, box) && pool_map(&maps[1], *c, c->v, box);
