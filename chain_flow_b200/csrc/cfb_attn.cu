@@ -37,7 +37,8 @@ namespace {
 // which attn_join_kernel adds up in unit order; a share holds at most two such pieces (its first and
 // its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
 // the same call gives the same bits.
-constexpr int kM = 128, kKeys = 64, kFewRows = 32;
+constexpr int kM = 128, kKeys = 64;
+__host__ __device__ constexpr int few_rows(bool e4m3) { return e4m3 ? 8 : 32; }
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4;
 constexpr int kScaleStages = 4;
 // A softmax thread holds a row; memory wants a warp's access to run along rows. 64 bytes of 32 rows at a time
@@ -46,7 +47,6 @@ constexpr int kScaleStages = 4;
 constexpr int kTurnPitch = 80;
 constexpr uint32_t kScaleBytes = kKeys * 12;   // a unit's scales: [64] (k's with the softmax's, log2 v's), [64] 1 / v's
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.f;             // o is rescaled only when the maximum has grown by 2^8
 
 // How the cache's rows come in: 16-bit or e4m3, by TMA where boxes of 8 rows or more tile both the pages
 // and the units (gcd(page size, 64) >= 8), else row by row.
@@ -56,7 +56,15 @@ __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
 // warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V (over e4m3 one: registers) or
 // four that copy rows, and over e4m3 four that widen V and bring the scales
 __host__ __device__ constexpr int load_warps(int src) { return src == TMA16 ? 2 : src == TMA8 ? 1 : 4; }
-__host__ __device__ constexpr int threads_of(int src) { return (9 + load_warps(src) + (is_e4m3(src) ? 4 : 0)) * 32; }
+__host__ __device__ constexpr int code_warps(int src, int m) { return !is_e4m3(src) ? 0 : m == kM ? 4 : kKeys / 32; }
+__host__ __device__ constexpr int threads_of(int src, int m) { return (9 + load_warps(src) + code_warps(src, m)) * 32; }
+
+// division of 0 <= n < 2^31 by a fixed d: with 2^k >= 2^31 d, mul = ceil(2^k / d) < 2^32 is above 2^k / d by
+// less than 1, so (n mul) >> k is floor(n / d)
+struct Divisor {
+  uint32_t mul; int k;
+  CFB_DEV int of(int n) const { return (int)(((unsigned long long)(unsigned)n * mul) >> k); }
+};
 
 struct AttnArgs {
   const void* q; long long sq_t, sq_h;
@@ -69,6 +77,7 @@ struct AttnArgs {
   float scale;
   int T, B, H, causal, rep;
   int m;                                  // rows of a row tile
+  Divisor by_rep, by_page;
   int box;                                // rows of a TMA box
   uint32_t slab, group;                   // bytes between a tile's 64-column slabs and its 8-row groups
   struct Desc* desc;                      // [grid]
@@ -102,7 +111,7 @@ CFB_DEV int row_limit(const AttnArgs& A, const Request& r, int tok) {      // po
 }
 CFB_DEV int tiles_of(const AttnArgs& A, const Request& r) { return (r.n * A.rep + A.m - 1) / A.m; }
 CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
-  const int last = (min((tile + 1) * A.m, r.n * A.rep) - 1) / A.rep;
+  const int last = A.by_rep.of(min((tile + 1) * A.m, r.n * A.rep) - 1);
   return max(1, (row_limit(A, r, last) + kKeys - 1) / kKeys);
 }
 // A kv head's units of request b (0 past the last), for the warp's 32 requests at once: a lane each where all have
@@ -198,17 +207,18 @@ template <int D>
 CFB_DEV float* part_row(float* part, int grid, int cta, int which, int row) {
   return part + ((((long long)(row >> 3) * 2 + which) * grid + cta) * 8 + (row & 7)) * kPart<D>;
 }
-template <int D, int SRC>
+template <int D, int SRC, int M>
 struct Layout {
+  static constexpr bool kWiden = is_e4m3(SRC) && M == kM;                   // V's codes to 16 bits
   static constexpr int kElem = is_e4m3(SRC) ? 1 : 2;                       // stored bytes an element
   static constexpr int kRowB = D * kElem < 128 ? 64 : 128, kSlabs = D * kElem / kRowB;   // a slab's row
-  static constexpr int kStages = SRC == ROWS16 ? 2 : D == 256 ? 3 : 4;
+  static constexpr int kStages = SRC == ROWS16 ? 2 : D == 256 && (kWiden || !is_e4m3(SRC)) ? 3 : 4;
   static constexpr uint32_t kTile = kKeys * D * kElem;
   // over e4m3: two stages of V widened, [64-column slab][row]; a third piece of Q that tensor memory has no
   // room for (D = 256)
   static constexpr uint32_t kWide = kKeys * D * 2;
-  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_w = 2 * kStages * kTile, off_q3 = off_w + (is_e4m3(SRC) ? 2 * kWide : 0);
-  static constexpr uint32_t off_turn = off_q3 + (is_e4m3(SRC) && D == 256 ? kM * D : 0);
+  static constexpr uint32_t off_k = 0, off_v = kStages * kTile, off_w = 2 * kStages * kTile, off_q3 = off_w + (kWiden ? 2 * kWide : 0);
+  static constexpr uint32_t off_turn = off_q3 + (kWiden && D == 256 ? kM * D : 0);
   static constexpr uint32_t off_scale = off_turn + kSoftWarps * 32 * kTurnPitch;
   static constexpr uint32_t bytes = off_scale + (is_e4m3(SRC) ? kScaleStages * kScaleBytes : 0) + 1024;
   static constexpr uint32_t s_col = 0, q_col = 2 * kKeys, o_col = D == 64 ? 192 : 256;
@@ -243,6 +253,9 @@ CFB_DEV void tmem_ld32(uint32_t taddr, float* v) {
 }
 CFB_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 CFB_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+CFB_DEV void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 CFB_DEV void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
@@ -321,7 +334,7 @@ __device__ const uint4 kNanRow[1] = {{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7
 
 // Where the row of position j lies; -1 if its page is none of the pool's.
 CFB_DEV long long row_offset(const AttnArgs& A, int b, int kh, int j, long long* scale_off) {
-  const int p = (unsigned)j / (unsigned)A.c.page_size, off = j - p * A.c.page_size;
+  const int p = A.by_page.of(j), off = j - p * A.c.page_size;
   const int page = __ldg(A.table + (long long)b * A.st + p);
   if (page < 0 || page >= A.c.pages) return -1;
   if (scale_off)
@@ -383,6 +396,29 @@ __device__ __noinline__ QPieces<T> query_pieces(uint4 q, float up) {
     p.w[kPieces<T> - 1][z] = e4m3_of(v);
   }
   return p;
+}
+
+// piece n of four values (zero past the last)
+template <typename T>
+CFB_DEV uint32_t piece_of(float (&v)[4], int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y = v[i];
+#pragma unroll
+    for (int k = 0; k < kPieces<T> - 1; ++k) {
+      const float lead = __uint_as_float((__float_as_uint(v[i]) + 0x00080000u) & 0xfff00000u);
+      if (k < n) v[i] -= lead;
+      y = k < n ? v[i] : lead;
+    }
+    v[i] = n < kPieces<T> ? (n == kPieces<T> - 1 ? v[i] : y) : 0.f;
+  }
+  return e4m3_of(v);
+}
+template <typename T>
+__device__ __noinline__ uint2 query_piece(uint4 q, float up, int n) {
+  const float2 a = unpack16<T>(q.x), b = unpack16<T>(q.y), c = unpack16<T>(q.z), d = unpack16<T>(q.w);
+  float v[4] = {a.x * up, a.y * up, b.x * up, b.y * up}, w[4] = {c.x * up, c.y * up, d.x * up, d.y * up};
+  return make_uint2(piece_of<T>(v, n), piece_of<T>(w, n));
 }
 
 // The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not.
@@ -447,12 +483,15 @@ __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T
 // the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^8 since
 // the last time: weights are then at most 2^8, far inside both types, and most units touch O not at all.
 template <typename T, int D, int SRC, int M>
-__global__ void __launch_bounds__(threads_of(SRC), 1)
+__global__ void __launch_bounds__(threads_of(SRC, M), 1)
 attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
-  using Lay = Layout<D, SRC>;
+  using Lay = Layout<D, SRC, M>;
   constexpr bool QUANT = is_e4m3(SRC);
   constexpr bool SPREAD = M < kM;
-  constexpr int kCols = kKeys / (kM / M);                      // a unit's columns of a softmax thread
+  constexpr bool PIECES = QUANT && SPREAD, WIDEN = QUANT && !SPREAD;
+  constexpr int kCols = SPREAD ? kKeys / 4 : kKeys;            // a unit's columns of a softmax thread
+  // the weights are at most 2^(kLift + kSlack), and o is rescaled only when the maximum has grown by 2^kSlack
+  constexpr float kLift = PIECES ? 6.5f : 0.f, kSlack = PIECES ? 2.f : 8.f;
   constexpr int kSt = Lay::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
@@ -470,7 +509,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 #pragma unroll 1
     for (int i = 0; i < kSt; ++i) {
       mbar_init(&bar.k_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], QUANT ? 4 : 1);
+      mbar_init(&bar.v_full[i], is_tma(SRC) ? 1 : kLoadWarps * 32); mbar_init(&bar.v_empty[i], WIDEN ? 4 : 1);
     }
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
@@ -552,7 +591,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     // row's maximum passes from unit to unit through shared memory; each group keeps its own sum.
     const int half = warp >> 2, pair = warp & 3;               // warps w and w + 4 share 32 rows
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
-    const int r = pair * 32 + lane, tr = SPREAD ? lane : r;    // lane of tensor memory, row of the tile
+    const int r = pair * 32 + lane, tr = PIECES ? lane & 7 : SPREAD ? lane : r;    // lane of tensor memory, row of the tile
     const int col0 = SPREAD ? pair * kCols : 0;
     const float c2 = A.scale * kLog2e;
     uint32_t g0 = 0, swaps = 0, meets = 0;                     // units before this piece; exchanges of the two groups, of all eight warps
@@ -577,7 +616,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       const int stop = w.stop(), first = w.first;
       const int rows = min(M, w.r.n * A.rep - w.tile * M);
       const bool valid = tr < rows;
-      const int R = w.tile * M + tr, tok = R / A.rep, head = w.kh * A.rep + R - tok * A.rep;
+      const int R = w.tile * M + tr, tok = A.by_rep.of(R), head = w.kh * A.rep + R - tok * A.rep;
       const int lim = valid ? row_limit(A, w.r, tok) : 0;
       const bool warp_live = SPREAD || pair * 32 < rows;
       bool ok = true;
@@ -634,6 +673,16 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           rowf = top >= kInf ? __int_as_float(0x7fc00000) : c2 * __uint_as_float((uint32_t)(127 + e2 - 7) << 23);
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
+            if constexpr (PIECES) {                            // this lane's piece alone
+              uint32_t piece[8];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint2 z = query_piece<T>(y[c][x], up, lane >> 3);
+                piece[2 * x] = z.x;
+                piece[2 * x + 1] = z.y;
+              }
+              tmem_st8(tw + Lay::q_col + half * (D / 8) + c * 8, piece);
+            } else {
             uint32_t piece[kPieces<T>][8];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -656,7 +705,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               }
             }
           }
-          if (D == 256 && kPieces<T> == 3) fence_async_shared();
+          }
+          if (WIDEN && D == 256 && kPieces<T> == 3) fence_async_shared();
         }
         tmem_wait_st();
         tc_fence_before();
@@ -666,7 +716,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 
       // the next tile's Q (of the same heads and request, the common case), into L2 by the time it is wanted
       if (w.tile + 1 < w.tiles && valid && w.u + (stop - first) < w.end) {
-        const int next = R + M, nt = next / A.rep;
+        const int next = R + M, nt = A.by_rep.of(next);
         if (nt < w.r.n) {
           const T* p = static_cast<const T*>(A.q) + (long long)(w.r.t0 + nt) * A.sq_t + (w.kh * A.rep + next - nt * A.rep) * A.sq_h + half * (D / 2);
 #pragma unroll
@@ -693,6 +743,12 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             if constexpr (SPREAD) tmem_ld16(tw + Lay::s_col + s * kKeys + col0, x);
             else tmem_ld32(tw + Lay::s_col + s * kKeys + c, x + c);
             tmem_wait_ld();
+            if constexpr (PIECES) {                            // the products of the query's pieces, added up alike in every lane
+#pragma unroll
+              for (int e = 0; e < kCols; ++e) x[e] += __shfl_xor_sync(0xffffffffu, x[e], 8);
+#pragma unroll
+              for (int e = 0; e < kCols; ++e) x[e] += __shfl_xor_sync(0xffffffffu, x[e], 16);
+            }
 #pragma unroll
             for (int e = c; e < c + 32 && e < kCols; e += 2) {
               if constexpr (QUANT) {
@@ -720,7 +776,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             now = sh_m[s ^ 1][r];
           }
           const float before = now;
-          if (now == -INFINITY || high > now + kSlack) now = high;
+          if (now == -INFINITY || high > now + (kLift + kSlack)) now = high - kLift;
           sh_m[s][r] = now;
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar.m_set[s][pair]);
@@ -761,10 +817,21 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 #pragma unroll
                 for (int z = 0; z < 4; ++z) sum[z] += y[z];
               }
-              p[e / 2] = pack16<T>(y[0], y[1]);
-              p[e / 2 + 1] = pack16<T>(y[2], y[3]);
+              if constexpr (PIECES) {
+                p[e / 4] = piece_of<T>(y, lane >> 3);
+              } else {
+                p[e / 2] = pack16<T>(y[0], y[1]);
+                p[e / 2 + 1] = pack16<T>(y[2], y[3]);
+              }
             }
-            if constexpr (SPREAD) {                            // the other lanes' columns have no weight here
+            if constexpr (PIECES) {                            // (as below, a code a column)
+              const uint32_t none[4] = {};
+              const uint32_t at = tw + Lay::s_col + s * kKeys;
+              tmem_st4(at + 4 * pair, p);
+              tmem_st4(at + 4 * (pair ^ 1), none);
+              tmem_st4(at + 4 * (pair ^ 2), none);
+              tmem_st4(at + 4 * (pair ^ 3), none);
+            } else if constexpr (SPREAD) {                            // the other lanes' columns have no weight here
               const uint32_t none[8] = {};
               const uint32_t at = tw + Lay::s_col + s * kKeys;
               tmem_st8(at + 8 * pair, p);
@@ -848,6 +915,12 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               float o[16];
               tmem_ld16(tw + Lay::o_col + d + x, o);
               tmem_wait_ld();
+              if constexpr (PIECES) {                          // the products of the weights' pieces
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 8);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 16);
+              }
               if (lane < rows) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -891,7 +964,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             __syncwarp();
           }
         }
-        if (valid && half == 0 && (!SPREAD || pair == 0)) {
+        if (valid && half == 0 && (!SPREAD || r < M)) {
           if (!whole) {
             part[D] = m;
             part[D + 1] = l;
@@ -918,7 +991,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           while (again) {
             const int src = __ffs(again) - 1;
             again &= again - 1;
-            const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = RR / A.rep, hd = w.kh * A.rep + RR - tk * A.rep;
+            const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = A.by_rep.of(RR), hd = w.kh * A.rep + RR - tk * A.rep;
             const int li = __shfl_sync(0xffffffffu, seen, src);
             const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
             row_again<T, D>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
@@ -943,33 +1016,38 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- tensor work
     // operand formats: 16-bit types, or e4m3 (0) for the scores; the second product's B is MN-major
-    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | (QUANT ? 0u : type_bits<T>()), idesc_o = tc_idesc(kM, D) | type_bits<T>() | (1u << 16);
+    constexpr uint32_t idesc_s = tc_idesc(kM, kKeys) | (QUANT ? 0u : type_bits<T>()), idesc_o = tc_idesc(kM, D) | (PIECES ? 0u : type_bits<T>()) | (1u << 16);
     constexpr int kRowB = Lay::kRowB;
     uint32_t g = 0, pieces = 0;
     bool ok = true;
     const auto pv = [&](uint32_t u, int i, bool fresh) {       // O (+)= P(u) V(u), u the piece's unit i
-      const int s = u & 1, st = QUANT ? s : u % kSt;
-      uint64_t* const full = QUANT ? &bar.w_full[s] : &bar.v_full[st];
-      if (!wait(full, (QUANT ? u >> 1 : u / kSt) & 1)) return false;
-      const uint32_t v = QUANT ? base + Lay::off_w + s * Lay::kWide : base + Lay::off_v + st * Lay::kTile;
-      if constexpr (SRC == TMA16) {
+      const int s = u & 1, st = WIDEN ? s : u % kSt;
+      uint64_t* const full = WIDEN ? &bar.w_full[s] : &bar.v_full[st];
+      if (!wait(full, (WIDEN ? u >> 1 : u / kSt) & 1)) return false;
+      const uint32_t v = WIDEN ? base + Lay::off_w + s * Lay::kWide : base + Lay::off_v + st * Lay::kTile;
+      if constexpr (is_tma(SRC) && !WIDEN) {
         // rows past the end hold what the pages or the last tile left there: 0 x NaN must not happen
         const int rows = row_limit(A, w.r, w.r.n - 1) - i * kKeys;
         if (rows < kKeys) {
+          constexpr int kRowP = kRowB / 16;                    // 16-byte pieces of a slab's row
 #pragma unroll 1
-          for (int x = max(rows, 0) * 8 + lane; x < kKeys * 8; x += 32)
+          for (int x = max(rows, 0) * kRowP + lane; x < kKeys * kRowP; x += 32)
 #pragma unroll
-            for (int c = 0; c < Lay::kSlabs; ++c) st_shared16(v + c * A.slab + (x >> 6) * A.group + (x & 63) * 16, 0, 0, 0, 0);
+            for (int c = 0; c < Lay::kSlabs; ++c) st_shared16(v + c * A.slab + x / (8 * kRowP) * A.group + x % (8 * kRowP) * 16, 0, 0, 0, 0);
           fence_async_shared();
           __syncwarp();
         }
       }
       if (!wait(&bar.p_full[s], (u >> 1) & 1)) return false;
-      if constexpr (SRC == ROWS16) fence_async_shared();       // the tile was stored by threads
+      if constexpr (!is_tma(SRC) && !WIDEN) fence_async_shared();                          // the tile was stored by threads
       tc_fence_after();
-      const uint32_t slab = QUANT ? kKeys * 128u : A.slab, group = QUANT ? 1024u : A.group;
-      mma_ts_warp<4, false>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major<128>(v, slab, group), group >> 3, idesc_o, !fresh);
-      tc_commit_warp(QUANT ? &bar.w_empty[s] : &bar.v_empty[st]);
+      if constexpr (PIECES) {                                  // two steps of 32 positions
+        mma_ts_warp<2, true>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major<kRowB>(v, A.slab, A.group), A.group >> 2, idesc_o, !fresh);
+      } else {                                                 // four steps of 16
+        const uint32_t slab = WIDEN ? kKeys * 128u : A.slab, group = WIDEN ? 1024u : A.group;
+        mma_ts_warp<4, false>(tmem + Lay::o_col, tmem + Lay::s_col + s * kKeys, mn_major<128>(v, slab, group), group >> 3, idesc_o, !fresh);
+      }
+      tc_commit_warp(WIDEN ? &bar.w_empty[s] : &bar.v_empty[st]);
       tc_commit_warp(&bar.o_done[s]);
       return true;
     };
@@ -987,11 +1065,11 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           tc_fence_after();
           const uint32_t k_at = base + Lay::off_k + st * Lay::kTile;
 #pragma unroll 1
-          for (int n = 0; n < (QUANT ? kPieces<T> : 1); ++n)
+          for (int n = 0; n < (WIDEN ? kPieces<T> : 1); ++n)
 #pragma unroll 1
             for (int k = 0; k < Lay::kSlabs; ++k) {
               const uint64_t desc = k_major<kRowB>(k_at + k * A.slab, A.group);
-              if (QUANT && D == 256 && n == 2)
+              if (WIDEN && D == 256 && n == 2)
                 mma_ss4_f8_warp(tmem + Lay::s_col + s * kKeys, k_major<128>(base + Lay::off_q3 + k * (kM * 128), 1024), desc, idesc_s);
               else
                 mma_ts_warp<kRowB / 32, QUANT>(tmem + Lay::s_col + s * kKeys, tmem + Lay::q_col + n * (D / 4) + k * 32, desc, 2, idesc_s, n + k > 0);
@@ -1049,6 +1127,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             if (lane == 0) mbar_arrive(&bar.sc_full[ss]);
             if (i + 1 < stop) look(w, i + 1);
           }
+          if constexpr (WIDEN) {
           if (!(ok = wait(&bar.v_full[st], (g / kSt) & 1))) break;
           const uint8_t* const raw = sm + Lay::off_v + st * Lay::kTile;
 #pragma unroll 1
@@ -1081,6 +1160,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           if (!ok) break;
           fence_async_shared();
           mbar_arrive(&bar.w_full[ws]);
+          }
         }
         if (!ok) break;
         w.next(A);
@@ -1097,7 +1177,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         need = lane * box < kKeys && j < row_limit(A, w.r, w.r.n - 1);
         page = -1;
         if (need) {
-          const int p = (unsigned)j / (unsigned)A.c.page_size;
+          const int p = A.by_page.of(j);
           off = j - p * A.c.page_size;
           page = __ldg(A.table + (long long)w.b * A.st + p);
           if (page >= A.c.pages) page = -1;
@@ -1291,7 +1371,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
     }
     m = top;
   }
-  const int R = d.row0 + r, tok = R / A.rep, head = d.kh * A.rep + R - tok * A.rep;
+  const int R = d.row0 + r, tok = A.by_rep.of(R), head = d.kh * A.rep + R - tok * A.rep;
   T* out = static_cast<T*>(A.o) + (long long)(d.t0 + tok) * A.so_t + head * A.so_h;
   const float inv = 1.f / l;
 #pragma unroll
@@ -1300,6 +1380,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
     for (int z = 0; z < V; z += 2)
       *reinterpret_cast<uint32_t*>(out + e * 32 + lane * V + z) = l == 0.f ? 0u : pack16<T>(acc[e + z] * inv, acc[e + z + 1] * inv);
   if (A.lse && lane == 0) A.lse[(long long)head * A.T + d.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+Divisor divisor(int d) {
+  int k = 31;
+  while ((1ll << (k - 31)) < d) ++k;
+  return {(uint32_t)(((1ull << k) + d - 1) / d), k};
 }
 
 // CTAs of a launch (without a device, as in a size computed on the host alone: a B200's)
@@ -1326,9 +1412,9 @@ bool pool_map(CUtensorMap* map, const cfb_kv_cache& c, void* base, int rows) {
 
 template <typename T, int D, int SRC, int M>
 cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
-  if (allow_smem<attn_kernel<T, D, SRC, M>>((int)Layout<D, SRC>::bytes) != cudaSuccess)
+  if (allow_smem<attn_kernel<T, D, SRC, M>>((int)Layout<D, SRC, M>::bytes) != cudaSuccess)
     return cfb_launch_status("attn_kernel attribute");
-  attn_kernel<T, D, SRC, M><<<grid, threads_of(SRC), Layout<D, SRC>::bytes, st>>>(A, maps[0], maps[1]);
+  attn_kernel<T, D, SRC, M><<<grid, threads_of(SRC, M), Layout<D, SRC, M>::bytes, st>>>(A, maps[0], maps[1]);
   if (const cfb_status s = cfb_launch_status("attn_kernel")) return s;
   const long long rows = std::min((long long)M, (long long)A.T * A.rep);
   // pieces: at least a row tile a kv head and request that has tokens; parts of one: the CTAs over those
@@ -1348,7 +1434,7 @@ cfb_status launch(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStre
 }
 template <typename T, int D, int SRC>
 cfb_status launch_rows(const AttnArgs& A, const CUtensorMap* maps, int grid, cudaStream_t st) {
-  return A.m == kM ? launch<T, D, SRC, kM>(A, maps, grid, st) : launch<T, D, SRC, kFewRows>(A, maps, grid, st);
+  return A.m == kM ? launch<T, D, SRC, kM>(A, maps, grid, st) : launch<T, D, SRC, few_rows(is_e4m3(SRC))>(A, maps, grid, st);
 }
 template <typename T, int D>
 cfb_status launch_source(const AttnArgs& A, int src, const CUtensorMap* maps, int grid, cudaStream_t st) {
@@ -1408,9 +1494,9 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   const int fit = std::gcd(c->page_size, kKeys), box = fit < kKeys ? std::min(fit, 8) : fit;
   const uint32_t row = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) < 128 ? 64 : 128, slabs = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) / row;
   const bool grouped = box == 8;
-  const int rep = H / c->kv_heads, m = (long long)T * rep <= (long long)kFewRows * B ? kFewRows : kM;
+  const int rep = H / c->kv_heads, few = few_rows(c->dtype == DT_E4M3), m = (long long)T * rep <= (long long)few * B ? few : kM;
   const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
-                   T, B, H, causal, rep, m, box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
+                   T, B, H, causal, rep, m, divisor(rep), divisor(c->page_size), box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
                    static_cast<Desc*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};
   CUtensorMap maps[2] = {};
   const bool tma = box >= 8 && pool_map(&maps[0], *c, c->k, box) && pool_map(&maps[1], *c, c->v, box);
