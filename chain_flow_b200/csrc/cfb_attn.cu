@@ -31,12 +31,13 @@ namespace {
 // ---- the split ------------------------------------------------------------------------------------
 // The query rows of one kv head of a request (its n tokens x rep heads, token-major) are cut into
 // tiles of kM = 128 rows, the allowed positions of a tile into units of kKeys = 64. A piece of work
-// is (request, kv head, row tile); the units of all pieces, laid end to end, are dealt to the CTAs in
-// equal contiguous shares, so one long context and a thousand short ones both keep every SM busy. A
-// piece cut by a share's end leaves partial results (unnormalised o, m, l, fp32) in the workspace,
-// which attn_join_kernel adds up in unit order; a share holds at most two such pieces (its first and
-// its last), so the workspace does not depend on the lengths. Shares depend only on the lengths:
-// the same call gives the same bits.
+// is (request, kv head, row tile); the pieces, laid end to end, each its units and a fixed cost long, are dealt
+// to the CTAs in equal contiguous shares, so one long context and a thousand short ones both keep every SM
+// busy (without the cost, a CTA of 7 short pieces took 274000 cycles where one of a single piece took 176000:
+// 48 decodes 150 us against 118). A piece cut by a share's end leaves partial results (unnormalised o, m, l,
+// fp32) in the workspace, which attn_join_kernel adds up in unit order; a share holds at most two such pieces
+// (its first and its last), so the workspace does not depend on the lengths. Shares depend only on the
+// lengths: the same call gives the same bits.
 constexpr int kM = 128, kKeys = 64;
 __host__ __device__ constexpr int few_rows(bool e4m3) { return e4m3 ? 8 : 32; }
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarps = 4;
@@ -55,9 +56,9 @@ __host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
 __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
 // warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V (over e4m3 one: registers) or
 // four that copy rows, and over e4m3 four that widen V and bring the scales
-__host__ __device__ constexpr int load_warps(int src) { return src == TMA16 ? 2 : src == TMA8 ? 1 : 4; }
+__host__ __device__ constexpr int load_warps(int src, int m) { return !is_tma(src) ? 4 : src == TMA8 ? 1 : 2; }
 __host__ __device__ constexpr int code_warps(int src, int m) { return !is_e4m3(src) ? 0 : m == kM ? 4 : kKeys / 32; }
-__host__ __device__ constexpr int threads_of(int src, int m) { return (9 + load_warps(src) + code_warps(src, m)) * 32; }
+__host__ __device__ constexpr int threads_of(int src, int m) { return (9 + load_warps(src, m) + code_warps(src, m)) * 32; }
 
 // division of 0 <= n < 2^31 by a fixed d: with 2^k >= 2^31 d, mul = ceil(2^k / d) < 2^32 is above 2^k / d by
 // less than 1, so (n mul) >> k is floor(n / d)
@@ -84,6 +85,9 @@ struct AttnArgs {
   float* part;                            // part_row
 };
 
+// What a piece costs besides its units (queries, results, a pipeline that fills and drains), in units.
+constexpr int kPieceCost = 8;
+
 struct Desc {                             // a piece that begins in this CTA's share and runs past its end
   int last;                               // the last CTA that holds a part of it; -1: no such piece
   int kh, t0, rows, row0;                 // kv head, first token row of the request, valid rows, first row of the tile
@@ -92,7 +96,7 @@ struct Desc {                             // a piece that begins in this CTA's s
   int extra;
 };
 
-// first unit of CTA `cta`'s share
+// where CTA `cta`'s share begins
 CFB_DEV long long share(long long each, int extra, int cta) { return each * cta + min(cta, extra); }
 
 struct Request { int t0, n, L; bool over; };
@@ -114,7 +118,7 @@ CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
   const int last = A.by_rep.of(min((tile + 1) * A.m, r.n * A.rep) - 1);
   return max(1, (row_limit(A, r, last) + kKeys - 1) / kKeys);
 }
-// A kv head's units of request b (0 past the last), for the warp's 32 requests at once: a lane each where all have
+// A kv head's units of request b, and its pieces' cost (0 past the last), for the warp's 32 requests at once: a lane each where all have
 // one tile, else a request at a time with a lane a tile (one prompt of 1500 tokens has 47).
 __device__ __noinline__ int head_units(const AttnArgs& A, int b) {
   const int lane = threadIdx.x & 31;
@@ -122,7 +126,7 @@ __device__ __noinline__ int head_units(const AttnArgs& A, int b) {
   if (b < A.B) r = request(A, b);
   const int tiles = tiles_of(A, r);
   unsigned longer = __ballot_sync(0xffffffffu, tiles > 1);
-  int u = tiles == 1 ? units_of(A, r, 0) : 0;
+  int u = tiles == 1 ? units_of(A, r, 0) + kPieceCost : 0;
 #pragma unroll 1
   for (; longer; longer &= longer - 1) {
     const int x = __ffs(longer) - 1;
@@ -130,7 +134,7 @@ __device__ __noinline__ int head_units(const AttnArgs& A, int b) {
     const int n = tiles_of(A, y);
     int sum = 0;
 #pragma unroll 1
-    for (int t = lane; t < n; t += 32) sum += units_of(A, y, t);
+    for (int t = lane; t < n; t += 32) sum += units_of(A, y, t) + kPieceCost;
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == x) u = sum;
   }
@@ -141,11 +145,11 @@ __device__ __noinline__ int head_units(const AttnArgs& A, int b) {
 // line, here and below: the kernel's roles run side by side, and their code has to share the instruction
 // cache (inlined everywhere, a quarter of all warp cycles went by without an instruction to issue).
 struct Walk {
-  long long u, end;
+  long long at, end;                      // where the piece begins and the share ends, with the pieces' costs
   int b, kh, tile, tiles, units, first;   // units of the piece; first unit of it in this share
   Request r;
   __device__ __noinline__ void start(const AttnArgs& A, long long from, long long to, int req, long long rest, int per_head) {
-    u = from; end = to; b = req;
+    end = to; b = req;
     r = request(A, b);
     tiles = tiles_of(A, r);
     kh = (int)(rest <= 0x7fffffff ? (unsigned)rest / (unsigned)per_head : rest / per_head);
@@ -154,7 +158,7 @@ struct Walk {
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (tile = 0;; tile += 32) {
-      const int mine = tile + lane < tiles ? units_of(A, r, tile + lane) : 0;
+      const int mine = tile + lane < tiles ? units_of(A, r, tile + lane) + kPieceCost : 0;
       int run = mine;
 #pragma unroll 1
       for (int off = 1; off < 32; off <<= 1) {
@@ -165,18 +169,20 @@ struct Walk {
       if (here) {
         const int x = __ffs(here) - 1;
         tile += x;
-        units = __shfl_sync(0xffffffffu, mine, x);
+        units = __shfl_sync(0xffffffffu, mine, x) - kPieceCost;
         first -= __shfl_sync(0xffffffffu, run - mine, x);
+        at = from - first;
+        first = max(first - kPieceCost, 0);
         break;
       }
       first -= __shfl_sync(0xffffffffu, run, 31);
     }
   }
-  CFB_DEV bool done() const { return u >= end; }
-  CFB_DEV int stop() const { return (int)min((long long)units, first + (end - u)); }   // first unit past this share's part
+  CFB_DEV bool done() const { return at + kPieceCost >= end; }
+  CFB_DEV int stop() const { return (int)min((long long)units, end - at - kPieceCost); }     // first unit past this share's part
   __device__ __noinline__ void next(const AttnArgs& A) {
-    u += stop() - first;
-    if (u >= end) return;
+    at += kPieceCost + units;
+    if (done()) return;
     first = 0;
     if (++tile == tiles) {
       tile = 0;
@@ -497,6 +503,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
+  __shared__ long long sh_total[32];
   __shared__ float sh_m[2][kM];
   __shared__ float2 sh_swap[2 * kM];                           // [group][lane of tensor memory]: its maximum and sum
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -536,43 +543,55 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     prefetch_map(&v_map);
   }
 
-  // Where this CTA's share begins: the running sum of the requests' units, by every warp for itself, a
-  // lane a request.
-  long long total = 0;
-  int per = 0;
+  // Where this CTA's share begins: the running sum of the requests' units, a lane a request. Up to 32 requests
+  // every warp looks at for itself; of more, each warp adds up a stretch, and all then search the one that matters.
+  const int warps = threads_of(SRC, M) / 32, span = (A.B + 32 * warps - 1) / (32 * warps);     // a stretch: span * 32 requests
+  const auto scan = [&](long long x) {                         // inclusive, over the lanes
 #pragma unroll 1
-  for (int b0 = 0; b0 < A.B; b0 += 32) {
-    per = head_units(A, b0 + lane);
-    long long sum = (long long)per * A.c.kv_heads;
-#pragma unroll
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    total += sum;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
+    }
+    return x;
+  };
+  int per = 0;
+  long long run;                                               // units up to and with this lane's request (or stretch)
+  if (A.B <= 32) {
+    per = head_units(A, lane);
+    run = (long long)per * A.c.kv_heads;
+  } else {
+    long long sum = 0;
+#pragma unroll 1
+    for (int c = 0; c < span; ++c) sum += (long long)head_units(A, (warp * span + c) * 32 + lane) * A.c.kv_heads;
+    sum = scan(sum);
+    if (lane == 31) sh_total[warp] = sum;
+    __syncthreads();
+    run = lane < warps ? sh_total[lane] : 0;
   }
+  run = scan(run);
+  const long long total = __shfl_sync(0xffffffffu, run, 31);
   const long long each = total <= 0x7fffffff ? (long long)((unsigned)total / (unsigned)grid) : total / grid;
   const int extra = (int)(total - each * grid);
   const long long from = share(each, extra, cta), to = share(each, extra, cta + 1);
   Walk w;
-  w.u = w.end = 0;
+  w.at = w.end = 0;
   if (from < to) {
+    int b0 = 0;
     long long before = 0;
-#pragma unroll 1
-    for (int b0 = 0;; b0 += 32) {
-      if (A.B > 32) per = head_units(A, b0 + lane);
-      const long long mine = (long long)per * A.c.kv_heads;
-      long long run = mine;                                    // inclusive scan
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, run, off);
-        if (lane >= off) run += y;
+    const auto shift = [&](int x) { return x ? __shfl_sync(0xffffffffu, run, x - 1) : 0; };    // what lies before lane x
+    if (A.B > 32) {
+      const int x = __ffs(__ballot_sync(0xffffffffu, from < run)) - 1;
+      before = shift(x);
+      for (b0 = x * span * 32;; b0 += 32) {
+        per = head_units(A, b0 + lane);
+        run = before + scan((long long)per * A.c.kv_heads);
+        const long long last = __shfl_sync(0xffffffffu, run, 31);
+        if (from < last) break;
+        before = last;
       }
-      const unsigned here = __ballot_sync(0xffffffffu, from < before + run);
-      if (here) {                                              // the first request whose units reach past `from`
-        const int x = __ffs(here) - 1;
-        w.start(A, from, to, b0 + x, from - before - __shfl_sync(0xffffffffu, run - mine, x), __shfl_sync(0xffffffffu, per, x));
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, run, 31);
     }
+    const int x = __ffs(__ballot_sync(0xffffffffu, from < run)) - 1;               // the first whose units reach past `from`
+    w.start(A, from, to, b0 + x, from - (x ? shift(x) : before), __shfl_sync(0xffffffffu, per, x));
   }
   tc_fence_before();
   __syncthreads();
@@ -715,7 +734,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       if (lane == 0) mbar_arrive(&bar.q_ready);
 
       // the next tile's Q (of the same heads and request, the common case), into L2 by the time it is wanted
-      if (w.tile + 1 < w.tiles && valid && w.u + (stop - first) < w.end) {
+      if (w.tile + 1 < w.tiles && valid && w.at + w.units + 2 * kPieceCost < w.end) {
         const int next = R + M, nt = A.by_rep.of(next);
         if (nt < w.r.n) {
           const T* p = static_cast<const T*>(A.q) + (long long)(w.r.t0 + nt) * A.sq_t + (w.kh * A.rep + next - nt * A.rep) * A.sq_h + half * (D / 2);
@@ -1004,7 +1023,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.o_free);
       if (threadIdx.x == 0 && first == 0 && stop < w.units) {  // begins here, ends elsewhere
-        const long long end = w.u + w.units;                   // w.u: its first unit
+        const long long end = w.at + kPieceCost + w.units;
         Desc d;
         d.last = cta + 1;
 #pragma unroll 1
@@ -1064,9 +1083,9 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           if constexpr (!is_tma(SRC)) fence_async_shared();
           tc_fence_after();
           const uint32_t k_at = base + Lay::off_k + st * Lay::kTile;
-#pragma unroll 1
+#pragma unroll (QUANT ? 1 : 4)
           for (int n = 0; n < (WIDEN ? kPieces<T> : 1); ++n)
-#pragma unroll 1
+#pragma unroll (QUANT ? 1 : 4)
             for (int k = 0; k < Lay::kSlabs; ++k) {
               const uint64_t desc = k_major<kRowB>(k_at + k * A.slab, A.group);
               if (WIDEN && D == 256 && n == 2)
@@ -1094,10 +1113,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     bool ok = true;
     const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
     const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
-    if (QUANT && lw >= load_warps(SRC)) {
+    if (QUANT && lw >= load_warps(SRC, M)) {
       // -------- V's codes to 16 bits, and (the first two warps, a lane a position) the scales, looked up a unit
       // early
-      const int cw = lw - load_warps(SRC), ct = cw * 32 + lane;
+      const int cw = lw - load_warps(SRC, M), ct = cw * 32 + lane;
       float2 sc = make_float2(0.f, 1.f);
       const auto look = [&](const Walk& w, int i) {
         sc = make_float2(0.f, 1.f);
@@ -1191,8 +1210,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         for (int i = w.first; i < stop; ++i, ++g) {
           const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
 #pragma unroll
-          for (int z = 0; z < (SRC == TMA16 ? 1 : 2); ++z) {
-            const int kv = SRC == TMA16 ? lw : z;
+          for (int z = 0; z < 2 / load_warps(SRC, M); ++z) {
+            const int kv = load_warps(SRC, M) == 2 ? lw : z;
             if (!(ok = kv ? v_free(g) : k_free())) break;
             const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile + lane * bytes;
             uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
