@@ -329,6 +329,27 @@ CFB_DEV void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 CFB_DEV void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// two fp32 operations in one instruction
+CFB_DEV float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+CFB_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+CFB_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+CFB_DEV float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 CFB_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -770,14 +791,13 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             }
 #pragma unroll
             for (int e = c; e < c + 32 && e < kCols; e += 2) {
+              float2 y = mul2(make_float2(x[e], x[e + 1]), make_float2(rowf, rowf));
               if constexpr (QUANT) {
                 const float4 f = sc[(col0 + e) / 2];
-                x[e] = fmaf(x[e] * rowf, f.x, f.y);
-                x[e + 1] = fmaf(x[e + 1] * rowf, f.z, f.w);
-              } else {
-                x[e] *= c2;
-                x[e + 1] *= c2;
+                y = fma2(y, make_float2(f.x, f.y), make_float2(f.z, f.w));
               }
+              x[e] = y.x;
+              x[e + 1] = y.y;
             }
           }
           if (masked) {
@@ -787,7 +807,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < kCols; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          for (int e = 0; e < kCols; e += 2) top[e / 2 & 3] = max3(top[e / 2 & 3], x[e], x[e + 1]);
           const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
           float now = -INFINITY;                               // the maximum the weights so far are relative to
           if (i > first) {
@@ -817,7 +837,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           l *= m == -INFINITY ? 1.f : exp2_approx(m - now);
           m = now;
           const float mm = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float2 less = make_float2(-mm, -mm);
+          float2 sum[2] = {};
 #pragma unroll
           for (int c = 0; c < kCols; c += 32) {
             uint32_t p[16];
@@ -825,16 +846,18 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             for (int e = 0; e < 32 && e < kCols; e += 4) {
               float y[4];
 #pragma unroll
-              for (int z = 0; z < 4; ++z) y[z] = exp2_approx(x[c + e + z] - mm);
+              for (int z = 0; z < 4; z += 2) {
+                const float2 d = add2(make_float2(x[c + e + z], x[c + e + z + 1]), less);
+                y[z] = exp2_approx(d.x);
+                y[z + 1] = exp2_approx(d.y);
+              }
               if constexpr (QUANT) {
                 const float4 f = sc[kKeys / 2 + (col0 + c + e) / 4];
-                sum[0] = fmaf(y[0], f.x, sum[0]);
-                sum[1] = fmaf(y[1], f.y, sum[1]);
-                sum[2] = fmaf(y[2], f.z, sum[2]);
-                sum[3] = fmaf(y[3], f.w, sum[3]);
+                sum[0] = fma2(make_float2(y[0], y[1]), make_float2(f.x, f.y), sum[0]);
+                sum[1] = fma2(make_float2(y[2], y[3]), make_float2(f.z, f.w), sum[1]);
               } else {
-#pragma unroll
-                for (int z = 0; z < 4; ++z) sum[z] += y[z];
+                sum[0] = add2(make_float2(y[0], y[1]), sum[0]);
+                sum[1] = add2(make_float2(y[2], y[3]), sum[1]);
               }
               if constexpr (PIECES) {
                 p[e / 4] = piece_of<T>(y, lane >> 3);
@@ -861,7 +884,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               tmem_st16(tw + Lay::s_col + s * kKeys + c / 2, p);
             }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
           tc_fence_before();
         } else {
@@ -1140,7 +1163,9 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             // a scale of NaN reaches the row through its score; where the row may not see the position, its
             // weight of 0 meets a finite factor
             uint8_t* const at = sm + Lay::off_scale + ss * kScaleBytes;
-            reinterpret_cast<float2*>(at)[ct] = make_float2(sc.x, log2f(sc.y));
+            float* const two = reinterpret_cast<float*>(at) + (ct >> 1) * 4 + (ct & 1);            // k's of two positions, then log2 v's
+            two[0] = sc.x;
+            two[2] = log2f(sc.y);
             reinterpret_cast<float*>(at + kKeys * 8)[ct] = sc.y > 0.f ? 1.f / sc.y : 1.f;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.sc_full[ss]);
