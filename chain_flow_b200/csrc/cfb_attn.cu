@@ -1329,7 +1329,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 // pieces, as in a step of a few decodes), else 1. A warp takes every WARPS-th part, kBatch of them at a
 // time with all their loads in flight together: the kernel is a chain of memory latencies, so it is
 // made short.
-constexpr int kJoinWarps = 8, kBatch = 8;
+constexpr int kJoinWarps = 8;
 
 template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs A) {
@@ -1341,6 +1341,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
   // the parts: this CTA's second one, then the first one of every later CTA that has a share
   const int last = d.each > 0 ? d.last : min(d.last, d.extra - 1);
   constexpr int E = D / 32, V = E < 4 ? E : 4;                 // elements a lane; of one access
+  constexpr int kBatch = WARPS > 1 ? 8 : 2;                    // parts in flight (rarely more than two or three where a warp has a row)
   float acc[E], l = 0.f, m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
