@@ -147,13 +147,14 @@ __global__ void __launch_bounds__(kStepThreads) gdn_walk_kernel(const cfb_gdn_ar
 // request's chunks with three products a chunk that depend on one another.
 //
 // Precision. The state is fp32 and has to stay so over thousands of chunks, so no product rounds an
-// operand to fewer than 22 bits: k and q are exact in tf32 as they are (their norms are applied
-// afterwards, in fp32), and S, U and T are split into two tf32 terms, x = hi + lo, lo * lo dropped
-// (relative error about 2^-22). Exponents of differences G_i - G_j are of sums kept in 64 bits: in 32,
-// a strong decay's G of a few hundred would cost 1e-5. S is updated by one fp32 fma an element from a
-// product that starts at zero, because sums carried through the tensor cores lose a little towards zero
-// with every step. o is rounded to 16 bits, so its own products take hi terms only over bf16 (11 bits
-// against its 8), and both terms over fp16.
+// operand to fewer than 22 bits. k and q are exact as they are (their norms are applied afterwards, in
+// fp32). Over bf16, S and U meet k as three bf16 pieces, exactly, 16 columns a product (a chunk of one head
+// at 8191 tokens: 1.9 us; the tf32 terms, 8 columns a product, 2.0). Else, S, U and T are split into two
+// tf32 terms, x = hi + lo, lo * lo dropped (relative error about 2^-22): fp16 pieces would need a scale a row
+// and chunk. Exponents of differences G_i - G_j are of sums kept in 64 bits: in 32, a strong decay's G of a
+// few hundred would cost 1e-5. S is updated by one fp32 fma an element from a product that starts at zero,
+// because sums carried through the tensor cores lose a little towards zero with every step. o is rounded to
+// 16 bits, so its own products take hi terms only over bf16 (11 bits against its 8), and both terms over fp16.
 //
 // Why mma.sync and not tcgen05: the scan is a chain over a head's chunks, and what bounds it is the
 // latency of one link, not throughput. With 16 value rows a warp, the state lives in the warp's
@@ -180,6 +181,17 @@ constexpr int kRowHalves = kK + 8;                             // padded row of 
 CFB_DEV void split(float x, float& hi, float& lo) {
   hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
   lo = __uint_as_float((__float_as_uint(x - hi) + 0x1000u) & 0xffffe000u);
+}
+// x = b1 + b2 + b3, bf16 each and exactly so: a piece is the top 16 bits of what is left, 8 of the 24 bits of
+// x's mantissa. Two neighbours' pieces as one register of an m16n8k16 operand.
+CFB_DEV void split3(float x, float y, uint32_t (&p)[3]) {
+  p[0] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+#pragma unroll
+  for (int i = 1; i < 3; ++i) {
+    x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+    p[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  }
 }
 CFB_DEV void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -632,16 +644,43 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
     float R[kBlocks][4] = {}, Rl[kBlocks][4] = {};
     uint32_t kw[2][4];                                         // a block ahead
     ldmatrix4(kw[0], block(at, ks * NJ));
+    if constexpr (!kFine) {
+      // two blocks of 8 columns a product, the accumulators as its first operand as they lie
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      float hi[4], lo[4];
-      operand(S[j], hi, lo);
-      if (j + 1 < NJ) ldmatrix4(kw[(j + 1) & 1], block(at, ks * NJ + j + 1));
+      for (int j = 0; j < NJ; j += 2) {
+        uint32_t p[4][3], now[2][4];
+        split3(S[j][0], S[j][1], p[0]);
+        split3(S[j][2], S[j][3], p[1]);
+        split3(S[j + 1][0], S[j + 1][1], p[2]);
+        split3(S[j + 1][2], S[j + 1][3], p[3]);
+        if (j == 0) ldmatrix4(kw[1], block(at, ks * NJ + 1));
 #pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt) {
-        const float2 k2 = unpack16<T>(kw[j & 1][nt]);
-        mma_tf32(R[nt], hi, k2.x, k2.y);
-        mma_tf32(Rl[nt], lo, k2.x, k2.y);
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) now[z][e] = kw[z][e];
+        if (j + 2 < NJ) {
+          ldmatrix4(kw[0], block(at, ks * NJ + j + 2));
+          ldmatrix4(kw[1], block(at, ks * NJ + j + 3));
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t a[4] = {p[0][i], p[1][i], p[2][i], p[3][i]};
+#pragma unroll
+          for (int nt = 0; nt < kBlocks; ++nt) mma_16<T>(i ? Rl[nt] : R[nt], a, now[0][nt], now[1][nt]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        float hi[4], lo[4];
+        operand(S[j], hi, lo);
+        if (j + 1 < NJ) ldmatrix4(kw[(j + 1) & 1], block(at, ks * NJ + j + 1));
+#pragma unroll
+        for (int nt = 0; nt < kBlocks; ++nt) {
+          const float2 k2 = unpack16<T>(kw[j & 1][nt]);
+          mma_tf32(R[nt], hi, k2.x, k2.y);
+          mma_tf32(Rl[nt], lo, k2.x, k2.y);
+        }
       }
     }
     // both halves need all of S k (two buffers in turn: the next chunk's barrier comes between a value's
@@ -739,7 +778,19 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
 #pragma unroll
     for (int nt = 0; nt < kBlocks; ++nt) {
       U[nt][0] *= eg[nt].x; U[nt][1] *= eg[nt].y; U[nt][2] *= eg[nt].x; U[nt][3] *= eg[nt].y;
-      operand(U[nt], hi[nt], lo[nt]);
+      if constexpr (kFine) operand(U[nt], hi[nt], lo[nt]);
+    }
+    uint32_t up[3][kBlocks / 2][4];                            // U's pieces, 16 tokens an operand
+    if constexpr (!kFine) {
+#pragma unroll
+      for (int nt = 0; nt < kBlocks; ++nt)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          uint32_t p[3];
+          split3(U[nt][2 * z], U[nt][2 * z + 1], p);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) up[i][nt / 2][2 * (nt & 1) + z] = p[i];
+        }
     }
 #pragma unroll
     for (int j = 0; j < NJ; j += 2) {                          // four sums side by side cover a product's latency
@@ -753,14 +804,23 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
         ldmatrix4_t(kt[0], block(at, ks * NJ + j + 2));
         ldmatrix4_t(kt[1], block(at, ks * NJ + j + 3));
       }
+      if constexpr (!kFine) {
 #pragma unroll
-      for (int nt = 0; nt < kBlocks; ++nt)
+        for (int nt = 0; nt < kBlocks; nt += 2)
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const float2 k2 = unpack16<T>(now[z][nt]);
-          mma_tf32(acc[z], hi[nt], k2.x, k2.y);
-          mma_tf32(accl[z], lo[nt], k2.x, k2.y);
-        }
+          for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) mma_16<T>(i ? accl[z] : acc[z], up[i][nt / 2], now[z][nt], now[z][nt + 1]);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < kBlocks; ++nt)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const float2 k2 = unpack16<T>(now[z][nt]);
+            mma_tf32(acc[z], hi[nt], k2.x, k2.y);
+            mma_tf32(accl[z], lo[nt], k2.x, k2.y);
+          }
+      }
 #pragma unroll
       for (int z = 0; z < 2; ++z)
 #pragma unroll
