@@ -8,13 +8,28 @@
 // Over an e4m3 cache k_j = ks_j kc_j and v_j = vs_j vc_j (codes and scales), and
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
-// so the weights stay at most 1, whatever the scales. Scores are formed on the 8-bit tensor path: keys as
-// the codes they are, the query in e4m3 pieces of 4 bits, q = q1 + q2 (+ q3), two over bf16 (8 bits) and
-// three over fp16 (11); a query row is first brought to a largest element of 128 to 256 by a power of two, so
-// that what e4m3's smallest step (2^-9) loses of a small element is 2^-17 of the largest. Value codes are
-// widened to 16 bits (exactly) on their way and meet 16-bit weights. (Both other ways were built: keys
-// widened too spend shared memory's bandwidth, 350 us for 48 decodes of the shape below against 170; weights in
-// pieces spend the conversion unit's, a warp instruction in 16 cycles, 440 us for five prompts.)
+// so the weights stay at most 1 (or a fixed power of two), whatever the scales. Scores are formed on the 8-bit
+// tensor path: keys as the codes they are, the query in e4m3 pieces of 4 bits, q = q1 + q2 (+ q3), two over
+// bf16 (8 bits) and three over fp16 (11); a query row is first brought to a largest element of 128 to 256 by a
+// power of two, so that what e4m3's smallest step (2^-9) loses of a small element is 2^-17 of the largest.
+//
+// Tiles of rows (a row: a query head of a token). 128, a row a lane of tensor memory. Where a request has at
+// most few_rows on average (T rep <= few_rows B), tiles of that many, repeated in all four quarters of the
+// lanes, each of which weighs a quarter of a unit's positions, so that a decode's softmax runs on eight warps:
+//   16-bit: 32 rows (one decode of 9001 positions, 16 heads on 4 of 256: 21 us; with 128-row tiles 26);
+//   e4m3: 8 rows, and in each quarter 8 lanes a piece of the query, so that one product forms all the pieces'
+//   scores; the weights are cut into pieces in the same lanes and meet the values' codes as they are. (48 decodes
+//   of up to 8192 positions, the same heads: 118 us. Over 128-row tiles, with V widened: 250; with the weights
+//   in pieces: 170.)
+// Over 128-row tiles the value codes are widened to 16 bits (exactly) on their way and meet 16-bit weights:
+// there pieces of the weights would keep the conversion unit (a warp instruction in 16 cycles) busy (five
+// prompts of up to 1500 tokens, 32 heads on 8 of 128: 440 us against 235), and keys widened too would spend shared
+// memory's bandwidth.
+//
+// What bounds it: over long prompts the tensor work (a prompt's chunk of 2048 tokens on 16384, 16 heads on 4 of
+// 256: 431 us, 1190 TFLOP/s; a 64-position product is issue-bound, 45 cycles for 32 of work, and D = 256 leaves
+// tensor memory no room for wider ones); over short pieces and decodes what a piece costs besides its units (about
+// 8 units' time) and instruction issue.
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
 #include <algorithm>
@@ -54,11 +69,12 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 enum Source : int { TMA16 = 0, ROWS16 = 1, TMA8 = 2, ROWS8 = 3 };
 __host__ __device__ constexpr bool is_e4m3(int src) { return src >= TMA8; }
 __host__ __device__ constexpr bool is_tma(int src) { return (src & 1) == 0; }
-// warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V (over e4m3 one: registers) or
-// four that copy rows, and over e4m3 four that widen V and bring the scales
-__host__ __device__ constexpr int load_warps(int src, int m) { return !is_tma(src) ? 4 : src == TMA8 ? 1 : 2; }
+// warps 0-7 softmax, 8 products, then two that issue the TMA copies of K and of V (over e4m3 one: registers, and
+// over tiles of few rows a second one took 160 us where one took 151) or four that copy rows, and over e4m3 four
+// that widen V and bring the scales, or two that bring the scales
+__host__ __device__ constexpr int load_warps(int src) { return !is_tma(src) ? 4 : src == TMA8 ? 1 : 2; }
 __host__ __device__ constexpr int code_warps(int src, int m) { return !is_e4m3(src) ? 0 : m == kM ? 4 : kKeys / 32; }
-__host__ __device__ constexpr int threads_of(int src, int m) { return (9 + load_warps(src, m) + code_warps(src, m)) * 32; }
+__host__ __device__ constexpr int threads_of(int src, int m) { return (9 + load_warps(src) + code_warps(src, m)) * 32; }
 
 // division of 0 <= n < 2^31 by a fixed d: with 2^k >= 2^31 d, mul = ceil(2^k / d) < 2^32 is above 2^k / d by
 // less than 1, so (n mul) >> k is floor(n / d)
@@ -118,8 +134,9 @@ CFB_DEV int units_of(const AttnArgs& A, const Request& r, int tile) {
   const int last = A.by_rep.of(min((tile + 1) * A.m, r.n * A.rep) - 1);
   return max(1, (row_limit(A, r, last) + kKeys - 1) / kKeys);
 }
-// A kv head's units of request b, and its pieces' cost (0 past the last), for the warp's 32 requests at once: a lane each where all have
-// one tile, else a request at a time with a lane a tile (one prompt of 1500 tokens has 47).
+// A kv head's units of request b, and its pieces' cost (0 past the last request), for the warp's 32 requests at
+// once: a lane a request where it has one tile, else a request at a time with a lane a tile (a prompt of 1500
+// tokens and 4 heads a kv head has 47; a lane adding those up took 26000 cycles).
 __device__ __noinline__ int head_units(const AttnArgs& A, int b) {
   const int lane = threadIdx.x & 31;
   Request r = {0, 0, 0, false};
@@ -201,8 +218,8 @@ struct Walk {
 // ---- shared and tensor memory ------------------------------------------------------------------------
 // K and V tiles are 128-byte-swizzled: groups of 8 rows of 64 columns (128 B), a row's 16-byte pieces
 // XORed with row & 7, as [slab of 64 columns][group] or, where the pages are no multiple of a unit,
-// [group][slab], so that one TMA box of 8 rows brings all their columns. K is read K-major (the head dim is summed over), V MN-major (the positions are), from the
-// same image. Q lies in tensor memory: as the first operand of S = Q K^T it would be read from
+// [group][slab], so that one TMA box of 8 rows brings all their columns. K is read K-major (the head dim is
+// summed over), V MN-major (the positions are), from the same image. Q lies in tensor memory: as the first operand of S = Q K^T it would be read from
 // shared memory again with every unit, and a 128 x 64 product of 16 reads 4 KB of it in its 32 cycles,
 // the whole shared-memory bandwidth. Tensor memory columns: two units' S (fp32), each overwritten by
 // its P (16-bit), then Q, then O.
@@ -500,15 +517,16 @@ __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------
-// One CTA per SM. The loading warps (Source) fill, per unit, a K and a V tile: pages are found through
-// the page table a unit early, positions past the end are zeros where it matters (V), and e4m3 codes
-// are widened on the way. Warp 8 issues the tensor work: S(i) = Q K(i)^T into one of two fp32 tiles in
-// tensor memory, then O += P(i-1) V(i-1) with P read from tensor memory, so the softmax of a unit runs
-// beside the next unit's product. Warps 0-7 are the softmax, a thread a row, units alternating between
-// two groups: the row's 64 scores come from tensor memory, and the weights go back there in the
-// operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16; their sum is of
-// the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^8 since
-// the last time: weights are then at most 2^8, far inside both types, and most units touch O not at all.
+// One CTA per SM. The loading warps (Source) fill, per unit, a K and a V tile: pages are found through the page
+// table a unit early, positions past the end are zeros where it matters (V). Warp 8 issues the tensor work:
+// S(i) = Q K(i)^T into one of two fp32 tiles in tensor memory, then O += P(i-1) V(i-1) with P read from tensor
+// memory, so the softmax of a unit runs beside the next unit's product. Warps 0-7 are the softmax, a thread a
+// lane, units alternating between two groups: the lane's scores come from tensor memory, and the weights go
+// back there in the operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16, in
+// pieces as much; their sum is of
+// the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^kSlack since
+// the last time: weights are then at most 2^8 (2^8.5 in pieces, at least 2^6.5 at the maximum: e4m3 holds up to
+// 448 and loses 2^-10), far inside the types, and most units touch O not at all.
 template <typename T, int D, int SRC, int M>
 __global__ void __launch_bounds__(threads_of(SRC, M), 1)
 attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -723,28 +741,28 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               }
               tmem_st8(tw + Lay::q_col + half * (D / 8) + c * 8, piece);
             } else {
-            uint32_t piece[kPieces<T>][8];
+              uint32_t piece[kPieces<T>][8];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const QPieces<T> z = query_pieces<T>(y[c][x], up);
+              for (int x = 0; x < 4; ++x) {
+                const QPieces<T> z = query_pieces<T>(y[c][x], up);
+#pragma unroll
+                for (int n = 0; n < kPieces<T>; ++n) {
+                  piece[n][2 * x] = z.w[n][0];
+                  piece[n][2 * x + 1] = z.w[n][1];
+                }
+              }
 #pragma unroll
               for (int n = 0; n < kPieces<T>; ++n) {
-                piece[n][2 * x] = z.w[n][0];
-                piece[n][2 * x + 1] = z.w[n][1];
+                if (D < 256 || n < 2) tmem_st8(tw + Lay::q_col + n * (D / 4) + half * (D / 8) + c * 8, piece[n]);
+                else {
+                  // the third piece of D = 256: 128-byte-swizzled rows in shared memory, one slab a group
+                  const uint32_t at = base + Lay::off_q3 + half * (kM * 128) + r * 128;
+#pragma unroll
+                  for (int z = 0; z < 2; ++z)
+                    st_shared16(at + (((c * 2 + z) ^ (r & 7)) << 4), piece[n][4 * z], piece[n][4 * z + 1], piece[n][4 * z + 2], piece[n][4 * z + 3]);
+                }
               }
             }
-#pragma unroll
-            for (int n = 0; n < kPieces<T>; ++n) {
-              if (D < 256 || n < 2) tmem_st8(tw + Lay::q_col + n * (D / 4) + half * (D / 8) + c * 8, piece[n]);
-              else {
-                // the third piece of D = 256: 128-byte-swizzled rows in shared memory, one slab a group
-                const uint32_t at = base + Lay::off_q3 + half * (kM * 128) + r * 128;
-#pragma unroll
-                for (int z = 0; z < 2; ++z)
-                  st_shared16(at + (((c * 2 + z) ^ (r & 7)) << 4), piece[n][4 * z], piece[n][4 * z + 1], piece[n][4 * z + 2], piece[n][4 * z + 3]);
-              }
-            }
-          }
           }
           if (WIDEN && D == 256 && kPieces<T> == 3) fence_async_shared();
         }
@@ -1136,10 +1154,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     bool ok = true;
     const auto k_free = [&] { return g < kSt || wait(&bar.k_empty[g % kSt], (g / kSt - 1) & 1); };
     const auto v_free = [&](uint32_t u) { return u < kSt || wait(&bar.v_empty[u % kSt], (u / kSt - 1) & 1); };
-    if (QUANT && lw >= load_warps(SRC, M)) {
+    if (QUANT && lw >= load_warps(SRC)) {
       // -------- V's codes to 16 bits, and (the first two warps, a lane a position) the scales, looked up a unit
       // early
-      const int cw = lw - load_warps(SRC, M), ct = cw * 32 + lane;
+      const int cw = lw - load_warps(SRC), ct = cw * 32 + lane;
       float2 sc = make_float2(0.f, 1.f);
       const auto look = [&](const Walk& w, int i) {
         sc = make_float2(0.f, 1.f);
@@ -1172,38 +1190,38 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             if (i + 1 < stop) look(w, i + 1);
           }
           if constexpr (WIDEN) {
-          if (!(ok = wait(&bar.v_full[st], (g / kSt) & 1))) break;
-          const uint8_t* const raw = sm + Lay::off_v + st * Lay::kTile;
+            if (!(ok = wait(&bar.v_full[st], (g / kSt) & 1))) break;
+            const uint8_t* const raw = sm + Lay::off_v + st * Lay::kTile;
 #pragma unroll 1
-          for (int x0 = 0; x0 < kPasses; x0 += kBatch) {
-            uint4 y[kBatch];
+            for (int x0 = 0; x0 < kPasses; x0 += kBatch) {
+              uint4 y[kBatch];
 #pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-              const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
-              constexpr int kSlabP = Lay::kRowB / 16;
-              const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
-              y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
-              if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);     // past the end: whatever the page holds
-            }
-            if (x0 + kBatch >= kPasses) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bar.v_empty[st]);
-            }
-            if (x0 == 0 && g >= 2 && !(ok = wait(&bar.w_empty[ws], ((g >> 1) + 1) & 1))) break;
+              for (int x = 0; x < kBatch; ++x) {
+                const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
+                constexpr int kSlabP = Lay::kRowB / 16;
+                const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
+                y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
+                if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);     // past the end: whatever the page holds
+              }
+              if (x0 + kBatch >= kPasses) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.v_empty[st]);
+              }
+              if (x0 == 0 && g >= 2 && !(ok = wait(&bar.w_empty[ws], ((g >> 1) + 1) & 1))) break;
 #pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-              const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
-              const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
-              const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
-              const int c0 = (p & 3) * 2, odd = p >> 2 & 1;    // (lanes of odd slabs store their halves in the other order: no two on a bank)
-              const uint4 u = odd ? b : a, v = odd ? a : b;
-              st_shared16(row + (((c0 + odd) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
-              st_shared16(row + (((c0 + 1 - odd) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+              for (int x = 0; x < kBatch; ++x) {
+                const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
+                const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
+                const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
+                const int c0 = (p & 3) * 2, odd = p >> 2 & 1;    // (lanes of odd slabs store their halves in the other order: no two on a bank)
+                const uint4 u = odd ? b : a, v = odd ? a : b;
+                st_shared16(row + (((c0 + odd) ^ (r & 7)) << 4), u.x, u.y, u.z, u.w);
+                st_shared16(row + (((c0 + 1 - odd) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
+              }
             }
-          }
-          if (!ok) break;
-          fence_async_shared();
-          mbar_arrive(&bar.w_full[ws]);
+            if (!ok) break;
+            fence_async_shared();
+            mbar_arrive(&bar.w_full[ws]);
           }
         }
         if (!ok) break;
@@ -1235,8 +1253,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         for (int i = w.first; i < stop; ++i, ++g) {
           const unsigned all = __ballot_sync(0xffffffffu, need && page >= 0);
 #pragma unroll
-          for (int z = 0; z < 2 / load_warps(SRC, M); ++z) {
-            const int kv = load_warps(SRC, M) == 2 ? lw : z;
+          for (int z = 0; z < 2 / load_warps(SRC); ++z) {
+            const int kv = load_warps(SRC) == 2 ? lw : z;
             if (!(ok = kv ? v_free(g) : k_free())) break;
             const uint32_t dst = base + (kv ? Lay::off_v : Lay::off_k) + (g % kSt) * Lay::kTile + lane * bytes;
             uint64_t* const full = kv ? &bar.v_full[g % kSt] : &bar.k_full[g % kSt];
