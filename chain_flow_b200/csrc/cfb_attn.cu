@@ -17,9 +17,10 @@
 // most few_rows on average (T rep <= few_rows B), tiles of that many, repeated in all four quarters of the
 // lanes, each of which weighs a quarter of a unit's positions, so that a decode's softmax runs on eight warps:
 //   16-bit: 32 rows (one decode of 9001 positions, 16 heads on 4 of 256: 21 us; with 128-row tiles 26);
-//   e4m3: 8 rows, and in each quarter 8 lanes a piece of the query, so that one product forms all the pieces'
-//   scores; the weights are cut into pieces in the same lanes and meet the values' codes as they are. (48 decodes
-//   of up to 8192 positions, the same heads: 118 us. Over 128-row tiles, with V widened: 250; with the weights
+//   e4m3: 8 rows, and in each quarter 8 lanes for each of four pieces of the query (piece_of), so that one product
+//   forms all their scores; the weights are cut into pieces in the same lanes and meet the values' codes as they
+//   are. (48 decodes
+//   of up to 8192 positions, the same heads: 128 us. Over 128-row tiles, with V widened: 250; with the weights
 //   in pieces: 170.)
 // Over 128-row tiles the value codes are widened to 16 bits (exactly) on their way and meet 16-bit weights:
 // there pieces of the weights would keep the conversion unit (a warp instruction in 16 cycles) busy (five
@@ -442,19 +443,29 @@ __device__ __noinline__ QPieces<T> query_pieces(uint4 q, float up) {
   return p;
 }
 
-// piece n of four values (zero past the last)
-template <typename T>
+// Piece n of four values, |v| < 2^8.6, where every piece has lanes, and so a scale, of its own: v = p0 + p1 / 16 +
+// p2 / 256 + p3 / 4096. With c_n the value rounded to 4 (n + 1) bits, but to no less than 2^(-9 - 4 n), p_n =
+// 16^n (c_n - c_(n-1)) is at most 8 steps of c_n's, 4 bits, in e4m3's range: the conversion takes it as it is.
+// (Rounding: adding and taking off 1.5 times the power of two whose last place is the step.) So a value keeps 16
+// bits, and nothing above 2^-22 is lost: of a row's weights, one of 2^-29 of the largest. (Pieces of one scale
+// lose what is below 2^-10: under a position that takes most of a row's weight, 8000 others can be a tenth of it
+// together and vanish so. They took 118 us where these take 128, at the 48 decodes above.)
 CFB_DEV uint32_t piece_of(float (&v)[4], int n) {
+  const float up = __uint_as_float((127u + 4u * n) << 23), prev = n ? -up : 0.f;               // 16^n
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y = v[i];
-#pragma unroll
-    for (int k = 0; k < kPieces<T> - 1; ++k) {
-      const float lead = __uint_as_float((__float_as_uint(v[i]) + 0x00080000u) & 0xfff00000u);
-      if (k < n) v[i] -= lead;
-      y = k < n ? v[i] : lead;
-    }
-    v[i] = n < kPieces<T> ? (n == kPieces<T> - 1 ? v[i] : y) : 0.f;
+  for (int i = 0; i < 4; i += 2) {
+    float2 m, before;
+    const auto step = [&](float x) {
+      return ((__float_as_uint(fmaxf(fabsf(x), 0x1p-6f)) & 0x7f800000u) | 0x00400000u) + ((20u - 4u * n) << 23);
+    };
+    const uint32_t a = step(v[i]), b = step(v[i + 1]);
+    m = make_float2(__uint_as_float(a), __uint_as_float(b));
+    before = make_float2(__uint_as_float(a + (4u << 23)), __uint_as_float(b + (4u << 23)));
+    const float2 x = make_float2(v[i], v[i + 1]);
+    const float2 c = add2(add2(x, m), make_float2(-m.x, -m.y)), c1 = add2(add2(x, before), make_float2(-before.x, -before.y));
+    const float2 p = fma2(c1, make_float2(prev, prev), mul2(c, make_float2(up, up)));
+    v[i] = p.x;
+    v[i + 1] = p.y;
   }
   return e4m3_of(v);
 }
@@ -462,7 +473,7 @@ template <typename T>
 __device__ __noinline__ uint2 query_piece(uint4 q, float up, int n) {
   const float2 a = unpack16<T>(q.x), b = unpack16<T>(q.y), c = unpack16<T>(q.z), d = unpack16<T>(q.w);
   float v[4] = {a.x * up, a.y * up, b.x * up, b.y * up}, w[4] = {c.x * up, c.y * up, d.x * up, d.y * up};
-  return make_uint2(piece_of<T>(v, n), piece_of<T>(w, n));
+  return make_uint2(piece_of(v, n), piece_of(w, n));
 }
 
 // The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not.
@@ -522,11 +533,10 @@ __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T
 // S(i) = Q K(i)^T into one of two fp32 tiles in tensor memory, then O += P(i-1) V(i-1) with P read from tensor
 // memory, so the softmax of a unit runs beside the next unit's product. Warps 0-7 are the softmax, a thread a
 // lane, units alternating between two groups: the lane's scores come from tensor memory, and the weights go
-// back there in the operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16, in
-// pieces as much; their sum is of
-// the unrounded fp32 values). O is rescaled only when the row's maximum has grown by more than 2^kSlack since
-// the last time: weights are then at most 2^8 (2^8.5 in pieces, at least 2^6.5 at the maximum: e4m3 holds up to
-// 448 and loses 2^-10), far inside the types, and most units touch O not at all.
+// back there in the operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16, 2^-17
+// in pieces; their sum is of the unrounded fp32 values). O is rescaled only when the row's maximum has grown by
+// more than 2^kSlack since the last time: weights are then at most 2^8 (in pieces 2^8.5, and the largest at least
+// 2^6.5), far inside the types, and most units touch O not at all.
 template <typename T, int D, int SRC, int M>
 __global__ void __launch_bounds__(threads_of(SRC, M), 1)
 attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -651,6 +661,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     const uint32_t tw = tmem + ((uint32_t)(pair * 32) << 16);
     const int r = pair * 32 + lane, tr = PIECES ? lane & 7 : SPREAD ? lane : r;    // lane of tensor memory, row of the tile
     const int col0 = SPREAD ? pair * kCols : 0;
+    const float piece_scale = __uint_as_float((127u - 4u * (lane >> 3)) << 23);                  // PIECES: what this lane's pieces are multiplied by
     const float c2 = A.scale * kLog2e;
     uint32_t g0 = 0, swaps = 0, meets = 0;                     // units before this piece; exchanges of the two groups, of all eight warps
     uint8_t* const turn = sm + Lay::off_turn + warp * (32 * kTurnPitch);
@@ -803,6 +814,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             tmem_wait_ld();
             if constexpr (PIECES) {                            // the products of the query's pieces, added up alike in every lane
 #pragma unroll
+              for (int e = 0; e < kCols; ++e) x[e] *= piece_scale;
+#pragma unroll
               for (int e = 0; e < kCols; ++e) x[e] += __shfl_xor_sync(0xffffffffu, x[e], 8);
 #pragma unroll
               for (int e = 0; e < kCols; ++e) x[e] += __shfl_xor_sync(0xffffffffu, x[e], 16);
@@ -878,7 +891,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
                 sum[1] = add2(make_float2(y[2], y[3]), sum[1]);
               }
               if constexpr (PIECES) {
-                p[e / 4] = piece_of<T>(y, lane >> 3);
+                p[e / 4] = piece_of(y, lane >> 3);
               } else {
                 p[e / 2] = pack16<T>(y[0], y[1]);
                 p[e / 2 + 1] = pack16<T>(y[2], y[3]);
@@ -938,6 +951,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             l += y.x == -INFINITY ? y.y : y.y * exp2_approx(y.x - top);
           }
           mine = lane_m == -INFINITY ? 1.f : exp2_approx(lane_m - top);
+          if (PIECES) mine *= piece_scale;
           m = top;
         } else {
           float2 other;
@@ -975,6 +989,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               float o[16];
               tmem_ld16(tw + Lay::o_col + d + x, o);
               tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= mine;
               if constexpr (PIECES) {                          // the products of the weights' pieces
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[e] += __shfl_xor_sync(0xffffffffu, o[e], 8);
@@ -984,7 +1000,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
               if (lane < rows) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  *reinterpret_cast<float4*>(mine4 + x * 4 + e * 16) = make_float4(o[4 * e] * mine, o[4 * e + 1] * mine, o[4 * e + 2] * mine, o[4 * e + 3] * mine);
+                  *reinterpret_cast<float4*>(mine4 + x * 4 + e * 16) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
               }
             }
             if (!(ok = meet())) break;
