@@ -424,19 +424,18 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
 //   8    one lane issues the copies of the chunks to come: K and Q as [64 columns][32 tokens] 128-byte-
 //        swizzled boxes, V as a plain box, T, P and the vectors in one piece. (The same copies by 16-byte
 //        cp.async kept a warp busy for longer than a chunk takes.)
-constexpr int kScanStages = 4, kTiles = 2, kStateWarps = 2 * kTiles, kOutWarps = 2 * kTiles, kScanRows = 16 * kTiles;
-constexpr int kScanThreads = (kStateWarps + kOutWarps + 1) * 32;
 constexpr int kHandThreads = 4 * 32;                           // a tile's two state and two output warps
-template <typename T>
+template <typename T, int TILES>
 struct Scan {
-  static constexpr int kKV = kC * kK * 2, kV = kC * kScanRows * 2, kPrep = Prep<T>::kFloats * 4;
+  static constexpr int kStages = TILES == 2 ? 4 : 3, kWarps = 2 * TILES, kRows = 16 * TILES, kThreads = (2 * kWarps + (TILES == 2 ? 1 : 4)) * 32;
+  static constexpr int kKV = kC * kK * 2, kV = kC * kRows * 2, kPrep = Prep<T>::kFloats * 4;
   static constexpr int off_q = kKV, off_v = 2 * kKV, off_prep = off_v + kV;
-  static constexpr int stage = (off_prep + kPrep + 1023) / 1024 * 1024, off_swap = kScanStages * stage;
+  static constexpr int stage = (off_prep + kPrep + 1023) / 1024 * 1024, off_swap = kStages * stage;
   static constexpr int kSwap = kBlocks * 2 * 32 * 8;           // one warp's partial sums of S k
   // what a tile's output warp reads: S ([16 blocks][lane] of four), U ([4 blocks][lane]), the first tokens lost
-  static constexpr int off_hand = off_swap + 2 * kStateWarps * kSwap, off_u = 16 * 512, off_lost = off_u + kBlocks * 512;
+  static constexpr int off_hand = off_swap + 2 * kWarps * kSwap, off_u = 16 * 512, off_lost = off_u + kBlocks * 512;
   static constexpr int kHand = off_lost + 256;
-  static constexpr int bytes = off_hand + 2 * kTiles * kHand + 1024;
+  static constexpr int bytes = off_hand + 2 * TILES * kHand + 1024;
   static constexpr int tx = 2 * kKV + kV + kPrep;
 };
 CFB_DEV void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory"); }
@@ -451,19 +450,20 @@ CFB_DEV void operand(const float (&s)[4], float (&hi)[4], float (&lo)[4]) {
   split(s[3], hi[3], lo[3]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kScanThreads)
+template <typename T, int TILES>
+__global__ void __launch_bounds__((4 * TILES + (TILES == 2 ? 1 : 4)) * 32, 1)
 gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float* ws, int* err,
                 const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map) {
-  using Lay = Scan<T>;
+  using Lay = Scan<T, TILES>;
+  constexpr int kScanStages = Lay::kStages, kStateWarps = Lay::kWarps, kOutWarps = Lay::kWarps;
   constexpr int NJ = 8;                                        // 8-column blocks of the state a warp holds
   constexpr bool kFine = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kScanStages], empty[kScanStages];
+  __shared__ uint64_t full[kScanStages], empty[kScanStages], freed[TILES][2];
   __shared__ int dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
-  const int hv = blockIdx.y, b = blockIdx.z, h = hv / (g.HV / g.H), v0 = blockIdx.x * kScanRows;
+  const int hv = blockIdx.y, b = blockIdx.z, h = hv / (g.HV / g.H), v0 = blockIdx.x * Lay::kRows;
   const int first = min(max(cu[b], 0), total), end = min(max(cu[b + 1], first), total);
   const int chunks = (end - first + kC - 1) / kC;
   const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -473,6 +473,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kStateWarps + kOutWarps);
     }
+    for (int i = 0; i < 2 * TILES; ++i) mbar_init(&freed[i >> 1][i & 1], 2);
     fence_mbar_init();
     dead = 0;
   }
@@ -485,15 +486,18 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
     if (mbar_test_wait(bar, parity)) return;
     if (*is_dead == 0 && !mbar_wait(bar, parity)) *is_dead = 1;
   };
-  // barriers of a tile: the state warps' exchange; S and U handed over; a hand-over buffer free again
+  // barriers of a tile: the state warps' exchange; S and U handed over (freed: a hand-over buffer free again)
   const int tile = (warp % kStateWarps) / 2;
-  const int swap_bar = 1 + tile * 5, hand_bar = swap_bar + 1, free_bar = swap_bar + 3;       // (+ chunk & 1)
-  const auto hand_at = [&](int c) { return smem + Lay::off_hand + ((c & 1) * kTiles + tile) * Lay::kHand; };
+  const int swap_bar = 1 + tile * 3, hand_bar = swap_bar + 1;        // (+ chunk & 1)
+  const auto hand_at = [&](int c) { return smem + Lay::off_hand + ((c & 1) * TILES + tile) * Lay::kHand; };
   // token `lane`'s row of a K or Q tile, 8-column block x: 128-byte rows of half the columns, 16-byte pieces
   // XORed with token & 7
   const auto block = [&](uint32_t at, int x) { return at + lane * 128 + (x >> 3) * (kC * 128) + (((x & 7) ^ (lane & 7)) << 4); };
 
-  if (warp == kStateWarps + kOutWarps) {
+  // (four tiles: 20 warps of 96 registers at launch, 61440; then 8 of 152, 8 of 72 and 4 of 24, 60416)
+  if (warp >= kStateWarps + kOutWarps) {
+    if (TILES > 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+    if (warp > kStateWarps + kOutWarps) return;
     // ------------------------------------------------------------ copies
     if (lane == 0) {
       prefetch_map(&q_map);
@@ -507,7 +511,9 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
         const uint32_t at = sm + st * Lay::stage;
         mbar_arrive_expect_tx(&full[st], Lay::tx);
         tma_load_4d(at, &k_map, 0, first + c * kC, 0, h, &full[st]);
-        tma_load_3d(at + Lay::off_v, &v_map, v0, first + c * kC, hv, &full[st]);
+#pragma unroll
+        for (int x = 0; x < TILES / 2; ++x)
+          tma_load_3d(at + Lay::off_v + x * kC * 64, &v_map, v0 + x * 32, first + c * kC, hv, &full[st]);
         bulk_g2s(smem + st * Lay::stage + Lay::off_prep, prep + (long long)c * g.HV * kPrepFloats, Lay::kPrep, &full[st]);
         tma_load_4d(at + Lay::off_q, &q_map, 0, first + c * kC, 0, h, &full[st]);
       }
@@ -516,6 +522,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
   }
 
   if (warp >= kStateWarps) {
+    if (TILES > 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ------------------------------------------------------------ outputs: o = e^G scale rq (S q) + P U
     for (int c = 0; c < chunks; ++c) {
       wait(&full[c % kScanStages], (c / kScanStages) & 1);
@@ -548,7 +555,8 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
         const float u[4] = {u4.x, u4.y, u4.z, u4.w};
         operand(u, hi[jb], lo[jb]);
       }
-      bar_arrive(free_bar + (c & 1), kHandThreads);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&freed[tile][c & 1]);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int nt = n0 + x;
@@ -588,6 +596,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
 
   // -------------------------------------------------------------- state: lane (gid, t) holds rows gid and
   // gid + 8, columns 2t and 2t + 1 of every 8-column block
+  if (TILES > 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
   const int ks = warp & 1;
   float S[NJ][4];
   const long long state_at = ((long long)hv * g.V + v0 + tile * 16 + gid) * kK + ks * NJ * 8 + 2 * t;
@@ -608,7 +617,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
   }
   for (int c = 0; c < chunks; ++c) {
     uint8_t* const hand = hand_at(c);
-    if (c >= 2) bar_sync(free_bar + (c & 1), kHandThreads);
+    if (c >= 2) wait(&freed[tile][c & 1], ((c >> 1) - 1) & 1);
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
       reinterpret_cast<float4*>(hand)[(ks * NJ + j) * 32 + lane] = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
@@ -632,7 +641,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
     uint32_t vw[kBlocks / 2][4];
 #pragma unroll
     for (int nt = 0; nt < kBlocks; nt += 2)
-      ldmatrix4_t(vw[nt / 2], at + Lay::off_v + (nt * 8 + (lane & 7) + (lane & 16 ? 8 : 0)) * (kScanRows * 2) + tile * 32 + (lane & 8 ? 16 : 0));
+      ldmatrix4_t(vw[nt / 2], at + Lay::off_v + (tile >> 1) * (kC * 64) + (nt * 8 + (lane & 7) + (lane & 16 ? 8 : 0)) * 64 + (tile & 1) * 32 + (lane & 8 ? 16 : 0));
     float2 bt[kBlocks], be[kBlocks], eg[kBlocks];
     float4 tw[kPairs];
 #pragma unroll
@@ -692,7 +701,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
     // reading and its overwriting)
     {
       using Sums = float2[kBlocks][2][32];
-      uint8_t* const swap = smem + Lay::off_swap + ((c & 1) * kTiles + tile) * 2 * Lay::kSwap;
+      uint8_t* const swap = smem + Lay::off_swap + ((c & 1) * TILES + tile) * 2 * Lay::kSwap;
       Sums& mine = *reinterpret_cast<Sums*>(swap + ks * Lay::kSwap);
       Sums& theirs = *reinterpret_cast<Sums*>(swap + (ks ^ 1) * Lay::kSwap);
 #pragma unroll
@@ -841,8 +850,6 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[c % kScanStages]);
   }
-  // (hand-over buffers that the output warps have freed and nobody will wait for)
-  for (int c = max(chunks, 2); c < chunks + 2; ++c) bar_sync(free_bar + (c & 1), kHandThreads);
   if (*is_dead) {
     if (lane == 0) *err = DEV_TIMEOUT_FULL;
 #pragma unroll
@@ -898,24 +905,37 @@ bool key_map(CUtensorMap* map, const void* base, int64_t stride, int total, int 
 }
 bool value_map(CUtensorMap* map, const void* base, int64_t stride, int total, int heads, int V) {
   const cuuint64_t dims[3] = {(cuuint64_t)V, (cuuint64_t)total, (cuuint64_t)heads}, strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)V * 2};
-  const cuuint32_t box[3] = {kScanRows, kC, 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {32, kC, 1}, step[3] = {1, 1, 1};
   return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, int TILES>
+cfb_status launch_tiles(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, int* err, const CUtensorMap& q,
+                        const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  using Lay = Scan<T, TILES>;
+  if (allow_smem<gdn_scan_kernel<T, TILES>>(Lay::bytes) != cudaSuccess) return cfb_launch_status("gdn_scan_kernel attribute");
+  if constexpr (TILES > 2) {                                   // the registers that setmaxnreg shares out are those of the launch
+    static const bool enough = [] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, gdn_scan_kernel<T, TILES>) == cudaSuccess && a.numRegs >= 96;
+    }();
+    if (!enough) return CFB_ERR_UNSUPPORTED;
+  }
+  const dim3 grid((unsigned)(g.V / Lay::kRows), (unsigned)g.HV, (unsigned)B);
+  gdn_scan_kernel<T, TILES><<<grid, Lay::kThreads, Lay::bytes, st>>>(g, cu, total, ws, err, q, k, v);
+  return cfb_launch_status("gdn_scan_kernel");
+}
 template <typename T>
 cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, int* err, cudaStream_t st) {
-  if (allow_smem<gdn_scan_kernel<T>>(Scan<T>::bytes) != cudaSuccess)
-    return cfb_launch_status("gdn_scan_kernel attribute");
   CUtensorMap q, k, v;
   if (!tensor_map_encoder()) return cfb_launch_status("cuTensorMapEncodeTiled");
   if (!key_map(&q, g.q, g.q_stride, total, g.H) || !key_map(&k, g.k, g.k_stride, total, g.H) ||
       !value_map(&v, g.v, g.v_stride, total, g.HV, g.V))
     return CFB_ERR_INVALID_ARG;
-  const dim3 grid((unsigned)(g.V / kScanRows), (unsigned)g.HV, (unsigned)B);
-  gdn_scan_kernel<T><<<grid, kScanThreads, Scan<T>::bytes, st>>>(g, cu, total, ws, err, q, k, v);
-  return cfb_launch_status("gdn_scan_kernel");
+  const bool four = g.V % 64 == 0 && (long long)g.V / 32 * g.HV * B >= 3ll * device_sms();
+  return four ? launch_tiles<T, 4>(g, cu, total, B, ws, err, q, k, v, st) : launch_tiles<T, 2>(g, cu, total, B, ws, err, q, k, v, st);
 }
 template <typename T>
 cfb_status launch_chunks(const cfb_gdn_args& g, const int32_t* cu, int total, int B, float* ws, int* err, cudaStream_t st) {
