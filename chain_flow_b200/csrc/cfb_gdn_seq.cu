@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kStepThreads) gdn_walk_kernel(const cfb_gdn_ar
 // the other operand is read as pairs of neighbours anyway), is the first operand's layout too: S feeds
 // S k, that feeds T, U feeds the update, without a trip through shared or tensor memory and with one
 // exchange between the two warps of a tile. Measured, 32 value heads of 128: 8191 tokens of one request 520 us
-// (scan 462, prep 58), nine prompts of up to 1500 tokens 521; a chunk 1.8 us, in which each quarter of the SM
+// (scan 462, prep 58), nine prompts of up to 1500 tokens 480; a chunk 1.8 us, in which each quarter of the SM
 // issues 1660 instructions and 165 products of 8.4 cycles in 3300 cycles: no pipe is full, the chain of dependent
 // steps of one state warp a quarter is the time. (Four warps a tile, a quarter of the columns each, repeat
 // U's product twice as often: 700 us. Two CTAs an SM leave 96 registers a thread: 1070.)
@@ -414,15 +414,15 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
   }
 }
 
-// One CTA per (32 value rows, value head, request), two value tiles of 16 rows, nine warps, so that every
-// quarter of the SM has a warp of the first two kinds:
-//   0-3  the state: warp 2 vt + ks holds tile vt's rows and half ks of the columns. A chunk is S k (the two
-//        halves exchange partial sums), U and the update, nothing else;
-//   4-7  the outputs, a chunk behind, warp 4 + 2 vt + x tile vt's of half x of the tokens: S, as it was before
-//        the chunk, and U reach them through shared memory (two buffers), so that S q and P U are off the
-//        chain that bounds the kernel;
-//   8    one lane issues the copies of the chunks to come: K and Q as [64 columns][32 tokens] 128-byte-
-//        swizzled boxes, V as a plain box, T, P and the vectors in one piece. (The same copies by 16-byte
+// One CTA per (16 TILES value rows, value head, request), TILES value tiles of 16 rows, four warps a tile and one that
+// copies, so that every quarter of the SM has warps of the first two kinds:
+//   the state, two warps a tile: each holds the tile's rows and half of the columns. A chunk is S k (the two halves
+//        exchange partial sums), U and the update, nothing else;
+//   the outputs, two warps a tile, a chunk behind, half of the tokens each: S, as it was before the chunk, and U
+//        reach them through shared memory (two buffers), so that S q and P U are off the chain that bounds the
+//        kernel;
+//   the copies: one lane issues those of the chunks to come: K and Q as [64 columns][32 tokens] 128-byte-swizzled
+//        boxes, V as plain boxes of 32 columns, T, P and the vectors in one piece. (The same copies by 16-byte
 //        cp.async kept a warp busy for longer than a chunk takes.)
 constexpr int kHandThreads = 4 * 32;                           // a tile's two state and two output warps
 template <typename T, int TILES>
@@ -452,7 +452,7 @@ CFB_DEV void operand(const float (&s)[4], float (&hi)[4], float (&lo)[4]) {
 
 template <typename T, int TILES>
 __global__ void __launch_bounds__((4 * TILES + (TILES == 2 ? 1 : 4)) * 32, 1)
-gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float* ws, int* err,
+gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const float* ws, int* err,
                 const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map) {
   using Lay = Scan<T, TILES>;
@@ -463,7 +463,23 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, const float*
   __shared__ uint64_t full[kScanStages], empty[kScanStages], freed[TILES][2];
   __shared__ int dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
-  const int hv = blockIdx.y, b = blockIdx.z, h = hv / (g.HV / g.H), v0 = blockIdx.x * Lay::kRows;
+  const int hv = blockIdx.y, h = hv / (g.HV / g.H), v0 = blockIdx.x * Lay::kRows;
+  // The longest requests first, as many as threads can rank (a long one begun last is the launch's tail: nine
+  // prompts of up to 1500 tokens 487 us in the order they came, 480 so).
+  __shared__ int sh_len[Lay::kThreads], sh_b;
+  if (B <= Lay::kThreads) {
+    const int x = threadIdx.x;
+    int n = 0, before = 0;
+    if (x < B) sh_len[x] = n = min(max(cu[x + 1], 0), total) - min(max(cu[x], 0), total);
+    __syncthreads();
+    if (x < B) {
+#pragma unroll 8
+      for (int i = 0; i < B; ++i) before += sh_len[i] > n || (sh_len[i] == n && i < x);
+      if (before == (int)blockIdx.z) sh_b = x;
+    }
+    __syncthreads();
+  }
+  const int b = B <= Lay::kThreads ? sh_b : blockIdx.z;
   const int first = min(max(cu[b], 0), total), end = min(max(cu[b + 1], first), total);
   const int chunks = (end - first + kC - 1) / kC;
   const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -924,7 +940,7 @@ cfb_status launch_tiles(const cfb_gdn_args& g, const int32_t* cu, int total, int
     if (!enough) return CFB_ERR_UNSUPPORTED;
   }
   const dim3 grid((unsigned)(g.V / Lay::kRows), (unsigned)g.HV, (unsigned)B);
-  gdn_scan_kernel<T, TILES><<<grid, Lay::kThreads, Lay::bytes, st>>>(g, cu, total, ws, err, q, k, v);
+  gdn_scan_kernel<T, TILES><<<grid, Lay::kThreads, Lay::bytes, st>>>(g, cu, total, B, ws, err, q, k, v);
   return cfb_launch_status("gdn_scan_kernel");
 }
 template <typename T>
@@ -934,6 +950,8 @@ cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int 
   if (!key_map(&q, g.q, g.q_stride, total, g.H) || !key_map(&k, g.k, g.k_stride, total, g.H) ||
       !value_map(&v, g.v, g.v_stride, total, g.HV, g.V))
     return CFB_ERR_INVALID_ARG;
+  // Four tiles a CTA where even so each SM has one and a half and more: more chains side by side, fewer CTAs (32 value
+  // heads of 128: nine requests 480 us against 518; one request, 64 CTAs on 148 SMs, would leave half of them idle).
   const bool four = g.V % 64 == 0 && (long long)g.V / 32 * g.HV * B >= 3ll * device_sms();
   return four ? launch_tiles<T, 4>(g, cu, total, B, ws, err, q, k, v, st) : launch_tiles<T, 2>(g, cu, total, B, ws, err, q, k, v, st);
 }
