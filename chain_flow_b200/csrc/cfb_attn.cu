@@ -24,7 +24,7 @@
 //   in pieces: 170.)
 // Over 128-row tiles the value codes are widened to 16 bits (exactly) on their way and meet 16-bit weights:
 // there pieces of the weights would keep the conversion unit (a warp instruction in 16 cycles) busy (five
-// prompts of up to 1500 tokens, 32 heads on 8 of 128: 440 us against 235), and keys widened too would spend shared
+// prompts of up to 1500 tokens, 32 heads on 8 of 128: 440 us against 248), and keys widened too would spend shared
 // memory's bandwidth.
 //
 // What bounds it: over long prompts the tensor work (a prompt's chunk of 2048 tokens on 16384, 16 heads on 4 of
@@ -407,6 +407,19 @@ CFB_DEV uint4 widen8(uint32_t lo, uint32_t hi) {
   return make_uint4(two(lo, 0x1404), two(lo, 0x3424), two(hi, 0x1404), two(hi, 0x3424));
 }
 
+// the same where a code may be a NaN (0x7f, 0xff; any_nan: a word of four has one), which widen8 would read as 480
+CFB_DEV uint32_t any_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+template <typename T>
+__device__ __noinline__ uint4 widen8_nan(uint32_t lo, uint32_t hi) {
+  const auto two = [](uint32_t w) {
+    __nv_fp8_e4m3 a, b;
+    a.__x = w & 0xff;
+    b.__x = w >> 8 & 0xff;
+    return pack16<T>((float)a, (float)b);
+  };
+  return make_uint4(two(lo), two(lo >> 16), two(hi), two(hi >> 16));
+}
+
 // Four values as e4m3: the leading piece, and what it leaves. The piece is the value rounded to 4 bits by an
 // integer addition, which the conversion then takes as it is (it rounds only below e4m3's normal range,
 // by at most half its smallest step).
@@ -493,29 +506,37 @@ __device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int*
 }
 
 // One row's o over positions [from, to) of its own, from its m (and, into the output, divided by its sum):
-// the columns [half * D / 2, ...) of it. For 16-bit rows whose product met a value that is not finite.
-template <typename T, int D>
+// the columns [half * D / 2, ...) of it. For rows whose product met a value that is not finite.
+template <typename T, int D, bool QUANT>
 __device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T* q, int from, int to, float m, float inv, int half,
                                        T* out, float* part) {
   constexpr int E = D / 32;
+  using Stored = std::conditional_t<QUANT, __nv_fp8_e4m3, T>;
+  const auto value = [](Stored y) {
+    if constexpr (QUANT) return (float)y;
+    else return to_float(y);
+  };
   const int lane = threadIdx.x & 31;
   float x[E], acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { x[e] = to_float(q[lane * E + e]); acc[e] = 0.f; }
 #pragma unroll 1
   for (int j = from; j < to; ++j) {
-    const long long off = row_offset(A, b, kh, j, nullptr);
+    long long so = 0;
+    const long long off = row_offset(A, b, kh, j, QUANT ? &so : nullptr);
     if (off < 0) continue;                                     // its score is NaN: so is l, and this row is not here
-    const T* k = static_cast<const T*>(A.c.k) + off + lane * E;
-    const T* v = static_cast<const T*>(A.c.v) + off + lane * E;
+    const Stored* k = static_cast<const Stored*>(A.c.k) + off + lane * E;
+    const Stored* v = static_cast<const Stored*>(A.c.v) + off + lane * E;
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(x[e], to_float(k[e]), s);
+    for (int e = 0; e < E; ++e) s = fmaf(x[e], value(k[e]), s);
 #pragma unroll
     for (int z = 16; z; z >>= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
-    const float p = exp2_approx(s * (A.scale * kLog2e) - m);
+    s *= A.scale * kLog2e;
+    if constexpr (QUANT) s = fmaf(s, A.c.k_scale[so], log2f(A.c.v_scale[so]));
+    const float p = exp2_approx(s - m);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_float(v[e]), acc[e]);
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(p, value(v[e]), acc[e]);
   }
   __syncwarp();
   if (lane >> 4 == half) {
@@ -1011,7 +1032,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
                 const float4 v = *reinterpret_cast<const float4*>(from4 + z * (32 * kTurnPitch));
                 y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
               }
-              if constexpr (!QUANT) bad[0] = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, bad[0]))));
+              bad[0] = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, bad[0]))));
               put(y, row_inv, row_l, off, row, d + piece * 4);
             }
             if (!(ok = meet())) break;
@@ -1025,7 +1046,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if constexpr (!QUANT) bad[e] = fmaf(o[4 * e], 0.f, fmaf(o[4 * e + 1], 0.f, fmaf(o[4 * e + 2], 0.f, fmaf(o[4 * e + 3], 0.f, bad[e]))));
+              bad[e] = fmaf(o[4 * e], 0.f, fmaf(o[4 * e + 1], 0.f, fmaf(o[4 * e + 2], 0.f, fmaf(o[4 * e + 3], 0.f, bad[e]))));
               *reinterpret_cast<float4*>(turn_row + e * 16) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
             __syncwarp();
@@ -1048,32 +1069,30 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             A.lse[(long long)head * A.T + w.r.t0 + tok] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
           }
         }
-        if constexpr (!QUANT) {
-          // A value that is not finite at a position that this row may not see has met a weight of 0 in
-          // the product. Only a causal row's last units can hold one; such a row is taken again from
-          // its own positions alone, with m and l as they are.
-          // (SPREAD: a position's weight is 0 in three of a row's lanes, so any such value does this.)
-          const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
-          const int seen = min(lim, stop * kKeys);             // where its positions here end
-          unsigned again = __ballot_sync(0xffffffffu, worst != 0.f);
-          const unsigned take = __ballot_sync(0xffffffffu, valid && l == l && (SPREAD || (A.causal && lim < stop * kKeys)));
-          if constexpr (SPREAD) {                              // from the lanes that added a row up to the row's own
-            const int per_row = rows <= 8 ? 16 : 4, base_row = pair * 32 / per_row;
-            again = __ballot_sync(0xffffffffu, lane >= base_row && lane < base_row + 32 / per_row &&
-                                                   (again >> ((lane - base_row) * per_row & 31) & ((1u << per_row) - 1)) != 0);
-          }
-          again &= take;
+        // A value that is not finite at a position that this row may not see has met a weight of 0 in
+        // the product. Only a causal row's last units can hold one; such a row is taken again from
+        // its own positions alone, with m and l as they are.
+        // (SPREAD: a position's weight is 0 in three of a row's lanes, so any such value does this.)
+        const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
+        const int seen = min(lim, stop * kKeys);             // where its positions here end
+        unsigned again = __ballot_sync(0xffffffffu, worst != 0.f);
+        const unsigned take = __ballot_sync(0xffffffffu, valid && l == l && (SPREAD || (A.causal && lim < stop * kKeys)));
+        if constexpr (SPREAD) {                              // from the lanes that added a row up to the row's own
+          const int per_row = rows <= 8 ? 16 : 4, base_row = pair * 32 / per_row;
+          again = __ballot_sync(0xffffffffu, lane >= base_row && lane < base_row + 32 / per_row &&
+                                                 (again >> ((lane - base_row) * per_row & 31) & ((1u << per_row) - 1)) != 0);
+        }
+        again &= take;
 #pragma unroll 1
-          while (again) {
-            const int src = __ffs(again) - 1;
-            again &= again - 1;
-            const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = A.by_rep.of(RR), hd = w.kh * A.rep + RR - tk * A.rep;
-            const int li = __shfl_sync(0xffffffffu, seen, src);
-            const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
-            row_again<T, D>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
-                            half, whole ? static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h : nullptr,
-                            part_row<D>(A.part, grid, cta, first == 0, row));
-          }
+        while (again) {
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = A.by_rep.of(RR), hd = w.kh * A.rep + RR - tk * A.rep;
+          const int li = __shfl_sync(0xffffffffu, seen, src);
+          const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
+          row_again<T, D, QUANT>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
+                          half, whole ? static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h : nullptr,
+                          part_row<D>(A.part, grid, cta, first == 0, row));
         }
         tc_fence_before();
       }
@@ -1211,6 +1230,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 #pragma unroll 1
             for (int x0 = 0; x0 < kPasses; x0 += kBatch) {
               uint4 y[kBatch];
+              uint32_t nan = 0;
 #pragma unroll
               for (int x = 0; x < kBatch; ++x) {
                 const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
@@ -1218,6 +1238,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
                 const int swz = Lay::kRowB == 128 ? (p % kSlabP) ^ (r & 7) : (p % kSlabP) ^ (r >> 1 & 3);
                 y[x] = *reinterpret_cast<const uint4*>(raw + p / kSlabP * A.slab + (r >> 3) * A.group + (r & 7) * Lay::kRowB + swz * 16);
                 if (i * kKeys + r >= lim) y[x] = make_uint4(0, 0, 0, 0);     // past the end: whatever the page holds
+                nan |= any_nan(y[x].x) | any_nan(y[x].y) | any_nan(y[x].z) | any_nan(y[x].w);
               }
               if (x0 + kBatch >= kPasses) {
                 __syncwarp();
@@ -1227,7 +1248,14 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
 #pragma unroll
               for (int x = 0; x < kBatch; ++x) {
                 const int z = (x0 + x) * 128 + ct, r = z / kRowP, p = z % kRowP;
-                const uint4 a = widen8<T>(y[x].x, y[x].y), b = widen8<T>(y[x].z, y[x].w);
+                uint4 a, b;
+                if (nan == 0) {
+                  a = widen8<T>(y[x].x, y[x].y);
+                  b = widen8<T>(y[x].z, y[x].w);
+                } else {
+                  a = widen8_nan<T>(y[x].x, y[x].y);
+                  b = widen8_nan<T>(y[x].z, y[x].w);
+                }
                 const uint32_t row = base + Lay::off_w + ws * Lay::kWide + (p >> 2) * (kKeys * 128) + r * 128;
                 const int c0 = (p & 3) * 2, odd = p >> 2 & 1;    // (lanes of odd slabs store their halves in the other order: no two on a bank)
                 const uint4 u = odd ? b : a, v = odd ? a : b;
@@ -1563,6 +1591,10 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   if (H % c->kv_heads || H / c->kv_heads > 128) return CFB_ERR_UNSUPPORTED;
   if ((long long)T * (H / c->kv_heads) > 0x7fffffffll - kM || (long long)table_width * c->page_size > 0x7fffffffll - kKeys)
     return CFB_ERR_UNSUPPORTED;
+  // (a request's units are counted in 32 bits)
+  const int rep = H / c->kv_heads, few = few_rows(c->dtype == DT_E4M3), m = (long long)T * rep <= (long long)few * B ? few : kM;
+  if (((long long)T * rep / m + 1) * ((long long)table_width * c->page_size / kKeys + 1 + kPieceCost) > 0x7fffffffll)
+    return CFB_ERR_UNSUPPORTED;
   if (T == 0 || B == 0) return CFB_OK;
   if (!q || !o || !kv_len || !cu_q || (table_width && !page_table) || !ws) return CFB_ERR_INVALID_ARG;
   if (!rows_aligned(q, 2, sq_t, sq_h) || !rows_aligned(o, 2, so_t, so_h)) return CFB_ERR_INVALID_ARG;
@@ -1573,7 +1605,6 @@ extern "C" cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, 
   const int fit = std::gcd(c->page_size, kKeys), box = fit < kKeys ? std::min(fit, 8) : fit;
   const uint32_t row = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) < 128 ? 64 : 128, slabs = c->dim * (c->dtype == DT_E4M3 ? 1 : 2) / row;
   const bool grouped = box == 8;
-  const int rep = H / c->kv_heads, few = few_rows(c->dtype == DT_E4M3), m = (long long)T * rep <= (long long)few * B ? few : kM;
   const AttnArgs A{q, sq_t, sq_h, *c, page_table, table_stride, table_width, kv_len, cu_q, o, so_t, so_h, lse, scale,
                    T, B, H, causal, rep, m, divisor(rep), divisor(c->page_size), box, grouped ? 8 * row : kKeys * row, grouped ? slabs * 8 * row : 8 * row,
                    static_cast<Desc*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + desc_bytes(grid))};

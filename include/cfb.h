@@ -432,7 +432,8 @@ cfb_status cfb_kv_read(const cfb_kv_cache* c, const int64_t* slots, int T, void*
  * e4m3 cache), strides in elements, rows 16-byte aligned; q rows outside every request are not read
  * and their o and lse not written. ws: cfb_paged_attn_workspace(H, c) bytes, 256-byte aligned,
  * for calls ordered on one stream; it needs no initialisation. Supported: H a multiple of kv_heads,
- * H / kv_heads <= 128. */
+ * H / kv_heads <= 128, T H / kv_heads rows x table_width pages of up to 2^31 tiles of 128 rows (8 or 32 where
+ * requests have few) x (64 positions, and 8 more for each tile). */
 size_t cfb_paged_attn_workspace(int H, int kv_heads, int dim);
 cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, const cfb_kv_cache* c,
                           const int32_t* page_table, int64_t table_stride, int table_width,

@@ -13,7 +13,6 @@ _cases = importlib.util.module_from_spec(_spec)
 _spec.loader.exec_module(_cases)
 _case, _want, _check, ROUND, FP32 = _cases._case, _cases._want, _cases._check, _cases.ROUND, _cases.FP32
 
-pytestmark = pytest.mark.gpu
 TYPES = [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True), (torch.float16, True)]
 
 
@@ -28,6 +27,7 @@ def _run(case, H, HKV, D, dtype, causal=True):
     assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, quant", TYPES)
 @pytest.mark.parametrize("H, HKV, D", [(16, 4, 256), (7, 1, 128), (2, 2, 64)])
 @pytest.mark.parametrize("page", [16, 17, 64])
@@ -38,6 +38,7 @@ def test_few_rows(dtype, quant, H, HKV, D, page, causal):
     _run(case, H, HKV, D, dtype, causal)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, quant", TYPES)
 def test_a_longer_request_among_decodes(dtype, quant):
     """20 tokens x 4 heads among 30 decodes: several tiles of few rows."""
@@ -45,6 +46,7 @@ def test_a_longer_request_among_decodes(dtype, quant):
     _run(case, 8, 2, 128, dtype)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("requests", [32, 33, 700])
 @pytest.mark.parametrize("quant", [False, True])
 def test_many_requests(requests, quant):
@@ -54,6 +56,7 @@ def test_many_requests(requests, quant):
     _run(case, 2, 1, 64, torch.float16)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, quant", TYPES)
 @pytest.mark.parametrize("news", [[1], [40]])
 def test_one_position_takes_most_of_the_weight(dtype, quant, news):
@@ -78,6 +81,7 @@ def test_one_position_takes_most_of_the_weight(dtype, quant, news):
     _check(got, want, dtype)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_values_that_are_not_finite(dtype):
     """An infinite value reaches its own column of the rows that see it; a row before it sees nothing of it."""
@@ -100,3 +104,33 @@ def test_values_that_are_not_finite(dtype):
         mask[hit, :, 7] = False
         err, bound = (got[0].double().cpu() - want[0]).abs(), ROUND[dtype] * (want[0].abs() + want[2]) * 1.01 + FP32 * (want[2] + 1)
         assert bool((err[mask] <= bound[mask]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("news", [[2, 1], [40, 1]])
+def test_codes_that_are_not_a_number(dtype, news):
+    """A NaN code in a later token's key and value: rows before it see nothing of it, rows from it on all of it."""
+    from chain_flow_b200.attention import PagedAttention
+    H, HKV, D, L = 4, 2, 128, 300
+    q, c, table, lens, cu = _case(news, [L, 90], H, HKV, D, 16, dtype, True, seed=9)
+    want = _want(q, c, table, lens, cu, True)
+    slot = int(table[0, (L - 1) // 16]), (L - 1) % 16
+    for pool, columns in ((c.v, [7]), (c.k, range(D))):
+        bits = pool.view(torch.uint8)
+        keep = bits[slot[0], :, slot[1]].clone()
+        bits[slot[0], :, slot[1], 7] = 0x7f
+        got = PagedAttention(H, HKV, D)(q, c, table, lens, cu)
+        torch.cuda.synchronize()
+        bits[slot[0], :, slot[1]] = keep
+        last = news[0] - 1
+        assert bool(torch.isnan(got[0][last][:, list(columns)]).all())
+        mask = torch.ones(sum(news), H, D, dtype=torch.bool)
+        mask[last, :, list(columns)] = False
+        err, bound = (got[0].double().cpu() - want[0]).abs(), ROUND[dtype] * (want[0].abs() + want[2]) * 1.01 + FP32 * (want[2] + 1)
+        assert bool((err[mask] <= bound[mask]).all())
+
+
+def test_more_units_than_32_bits_are_refused():
+    assert _cases._call(T=1 << 23, H=4 * 16, width=1 << 22, st=1 << 22) == 2
+    assert _cases._call(T=0, width=1 << 22, st=1 << 22) == 0
