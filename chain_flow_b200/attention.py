@@ -72,8 +72,11 @@ class PagedAttention:
                 or page_table.dim() != 2 or page_table.shape[0] != B or kv_len.dim() != 1 or cu_q.shape != (B + 1,)
                 or any(t.get_device() != dev for t in (query, page_table, kv_len, cu_q))):
             self._refuse(query, cache, page_table, kv_len, cu_q)
-        if page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+        st, width = page_table.stride(), page_table.shape[1]
+        # (rows that share words, as one prefix expanded over several requests, are copied out)
+        if page_table.dtype != torch.int32 or st[1] != 1 or (B > 1 and st[0] < width):
             page_table = page_table.to(torch.int32).contiguous()
+            st = page_table.stride()
         kv_len, cu_q = _lib.int32(kv_len), _lib.int32(cu_q)
         T = shape[0]
         if out is None:
@@ -84,10 +87,10 @@ class PagedAttention:
             lse = torch.empty((self.heads, T), dtype=torch.float32, device=cache.device)
         elif lse.shape != (self.heads, T) or lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous():
             raise _lib.CfbError(f"lse must be contiguous fp32 [{self.heads}, {T}] on the query's device")
-        so, st = out.stride(), page_table.stride()
+        so = out.stride()
         _lib.check(self.lib.cfb_paged_attn(
-            query.data_ptr(), sq[0], sq[1], cache.desc, page_table.data_ptr(), max(st[0], page_table.shape[1]),
-            page_table.shape[1], kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),
+            query.data_ptr(), sq[0], sq[1], cache.desc, page_table.data_ptr(), max(st[0], width),
+            width, kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),
             self.scale if scale is None else scale, T, B, self.heads, causal, dt, self.ws_ptr, self.ws_bytes,
             _lib.stream_ptr()), "cfb_paged_attn")
         return out, lse
