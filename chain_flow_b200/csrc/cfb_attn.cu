@@ -575,7 +575,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   __shared__ int dead;
   __shared__ long long sh_total[32];
   __shared__ float sh_m[2][kM];
-  __shared__ float2 sh_swap[2 * kM];                           // [group][lane of tensor memory]: its maximum and sum
+  __shared__ float2 sh_swap[2][2 * kM];                        // [buffer][group][lane of tensor memory]: its maximum and sum
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -688,12 +688,16 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     uint8_t* const turn = sm + Lay::off_turn + warp * (32 * kTurnPitch);
     uint8_t* const turn_row = turn + lane * kTurnPitch;                              // this lane's row
     uint8_t* const turn_at = turn + (lane >> 2) * kTurnPitch + (lane & 3) * 16;      // its piece of row lane / 4, then every 8th
-    const auto exchange = [&](float2 mine, float2* other) {    // with the row's thread of the other group
-      sh_swap[half * kM + r] = mine;
+    // With the row's thread of the other group. Two buffers in turn: a warp that goes on to the next exchange (the
+    // next piece's queries after this one's sums, with no barrier between) must not overwrite what the other has
+    // yet to read of this one, and cannot get to the one after that before the other has arrived in the next.
+    const auto exchange = [&](float2 mine, float2* other) {
+      float2* const at = sh_swap[swaps & 1];
+      at[half * kM + r] = mine;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.swap[pair]);
       if (!wait(&bar.swap[pair], swaps++ & 1)) return false;
-      *other = sh_swap[(half ^ 1) * kM + r];
+      *other = at[(half ^ 1) * kM + r];
       return true;
     };
     const auto meet = [&] {
@@ -959,16 +963,16 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         // O then meets by `mine`
         float mine = 1.f;
         if constexpr (SPREAD) {
-          sh_swap[half * kM + r] = make_float2(m, l);
+          sh_swap[0][half * kM + r] = make_float2(m, l);
           if (!meet()) break;
           float lane_m = -INFINITY, top = -INFINITY;
 #pragma unroll
-          for (int z = 0; z < kSoftWarps; ++z) top = fmaxf(top, sh_swap[z * 32 + lane].x);
-          lane_m = fmaxf(m, sh_swap[(half ^ 1) * kM + r].x);
+          for (int z = 0; z < kSoftWarps; ++z) top = fmaxf(top, sh_swap[0][z * 32 + lane].x);
+          lane_m = fmaxf(m, sh_swap[0][(half ^ 1) * kM + r].x);
           l = 0.f;
 #pragma unroll
           for (int z = 0; z < kSoftWarps; ++z) {
-            const float2 y = sh_swap[z * 32 + lane];
+            const float2 y = sh_swap[0][z * 32 + lane];
             l += y.x == -INFINITY ? y.y : y.y * exp2_approx(y.x - top);
           }
           mine = lane_m == -INFINITY ? 1.f : exp2_approx(lane_m - top);
