@@ -1282,6 +1282,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
       const uint32_t bytes = box * D * Lay::kElem;
       int page = -1, off = 0;
       bool need = false;
+      uint32_t sent_k = 0, sent_v = 0;                         // units whose copies this warp has issued
       const auto look = [&](const Walk& w, int i) {
         const int j = i * kKeys + lane * box;
         need = lane * box < kKeys && j < row_limit(A, w.r, w.r.n - 1);
@@ -1316,6 +1317,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             if (lane == 0) mbar_arrive_expect_tx(full, __popc(all) * bytes);
             __syncwarp();
             if (need && page >= 0) tma_load_5d(dst, kv ? &v_map : &k_map, 0, off, 0, w.kh, page, full);
+            (kv ? sent_v : sent_k) = g + 1;
           }
           if (!ok) break;
           if (i + 1 < stop) look(w, i + 1);
@@ -1324,6 +1326,13 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
         w.next(A);
         if (!w.done()) look(w, w.first);
       }
+      // A CTA whose products gave up does not wait for these copies: it must not end before they have landed.
+      const auto landed = [&](uint64_t* full, uint32_t sent) {
+#pragma unroll 1
+        for (uint32_t u = sent < kSt ? 0 : sent - kSt; u < sent; ++u) mbar_wait(&full[u % kSt], (u / kSt) & 1);
+      };
+      landed(bar.k_full, sent_k);
+      landed(bar.v_full, sent_v);
     } else {
       // -------- the warps that copy rows. A thread's copies arrive on the stage's barrier by themselves when
       // they land. Stages come free in the order K(g + 1), V(g) (the products are issued S(g - 1),
