@@ -520,7 +520,8 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
       prefetch_map(&k_map);
       prefetch_map(&v_map);
       const float* const prep = ws + ((long long)(first / kC + b) * g.HV + hv) * kPrepFloats;
-      for (int c = 0; c < chunks; ++c) {
+      int c = 0;
+      for (; c < chunks; ++c) {
         const int st = c % kScanStages;
         if (c >= kScanStages) wait(&empty[st], (c / kScanStages - 1) & 1);
         if (*is_dead) break;
@@ -533,6 +534,8 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
         bulk_g2s(smem + st * Lay::stage + Lay::off_prep, prep + (long long)c * g.HV * kPrepFloats, Lay::kPrep, &full[st]);
         tma_load_4d(at + Lay::off_q, &q_map, 0, first + c * kC, 0, h, &full[st]);
       }
+      // a CTA that gave up must not end before these copies have landed
+      for (int x = max(c - kScanStages, 0); x < c; ++x) mbar_wait(&full[x % kScanStages], (x / kScanStages) & 1);
     }
     return;
   }
