@@ -489,15 +489,19 @@ __device__ __noinline__ uint2 query_piece(uint4 q, float up, int n) {
   return make_uint2(piece_of(v, n), piece_of(w, n));
 }
 
-// The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not.
-__device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int* dead) {
+// What the CTA's waits watch besides their barriers: dead, a wait has expired; alive, when mend_rows last got on.
+struct Watch { int dead; unsigned long long alive; };
+
+// The rest of a wait that was not over at once; false if it never was, or another one of the CTA was not. The limit
+// starts anew while rows are mended (loops over a row's positions, which end, but take what they take).
+__device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile Watch* watch) {
   bool ok = true;
   const unsigned long long t0 = globaltimer();
 #pragma unroll 1
   for (unsigned it = 1; !mbar_try_wait(b, parity); ++it)
     if (it % kPollsPerCheck == 0) {
-      if (wait_expired(t0, kWaitBudgetNs)) *dead = 1;
-      if (*dead != 0) {
+      if (wait_expired(max(t0, watch->alive), kWaitBudgetNs)) watch->dead = 1;
+      if (watch->dead != 0) {
         ok = false;
         break;
       }
@@ -505,47 +509,224 @@ __device__ __noinline__ bool wait_on(uint64_t* b, uint32_t parity, volatile int*
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
-// One row's o over positions [from, to) of its own, from its m (and, into the output, divided by its sum):
-// the columns [half * D / 2, ...) of it. For rows whose product met a value that is not finite.
-template <typename T, int D, bool QUANT>
-__device__ __noinline__ void row_again(const AttnArgs& A, int b, int kh, const T* q, int from, int to, float m, float inv, int half,
-                                       T* out, float* part) {
-  constexpr int E = D / 32;
-  using Stored = std::conditional_t<QUANT, __nv_fp8_e4m3, T>;
-  const auto value = [](Stored y) {
-    if constexpr (QUANT) return (float)y;
-    else return to_float(y);
-  };
-  const int lane = threadIdx.x & 31;
-  float x[E], acc[E];
+// N stored elements (e4m3 codes or T) as fp32; their words as one access
+template <int BYTES> struct WordsOf;
+template <> struct WordsOf<1> { using type = uint8_t; };
+template <> struct WordsOf<2> { using type = uint16_t; };
+template <> struct WordsOf<4> { using type = uint32_t; };
+template <> struct WordsOf<8> { using type = uint2; };
+template <> struct WordsOf<16> { using type = uint4; };
+template <typename Stored, int N>
+CFB_DEV void widen_all(const typename WordsOf<N * sizeof(Stored)>::type& words, float (&x)[N]) {
+  const Stored* const y = reinterpret_cast<const Stored*>(&words);
 #pragma unroll
-  for (int e = 0; e < E; ++e) { x[e] = to_float(q[lane * E + e]); acc[e] = 0.f; }
-#pragma unroll 1
-  for (int j = from; j < to; ++j) {
-    long long so = 0;
-    const long long off = row_offset(A, b, kh, j, QUANT ? &so : nullptr);
-    if (off < 0) continue;                                     // its score is NaN: so is l, and this row is not here
-    const Stored* k = static_cast<const Stored*>(A.c.k) + off + lane * E;
-    const Stored* v = static_cast<const Stored*>(A.c.v) + off + lane * E;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(x[e], value(k[e]), s);
-#pragma unroll
-    for (int z = 16; z; z >>= 1) s += __shfl_xor_sync(0xffffffffu, s, z);
-    s *= A.scale * kLog2e;
-    if constexpr (QUANT) s = fmaf(s, A.c.k_scale[so], log2f(A.c.v_scale[so]));
-    const float p = exp2_approx(s - m);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(p, value(v[e]), acc[e]);
+  for (int e = 0; e < N; ++e) {
+    if constexpr (sizeof(Stored) == 1) x[e] = (float)y[e];
+    else x[e] = to_float(y[e]);
   }
-  __syncwarp();
-  if (lane >> 4 == half) {
+}
+template <typename T, bool QUANT> using StoredOf = std::conditional_t<QUANT, __nv_fp8_e4m3, T>;
+
+// Rows whose product met a value that is not finite, among them rows that do not see its position and met it with a
+// weight of 0. A column in which a row sees such values is what they add up to (an infinity, or NaN); the columns
+// [half * D / 2, ...) are put so in the CTA's partial result `which`, or (-1) the output. Returned: the rows that have a column
+// in which they see none but whose product met one, to be taken again. `again`: the warp's rows, a lane each (the
+// tile's row row0 + lane), with `seen`, where a row's positions end, in the lane. The tile's positions: [from, to),
+// of which every row sees those before `hidden`; nothing is wrong where none of the others holds such a value.
+template <typename T, int D, bool QUANT>
+__device__ __noinline__ unsigned put_spoilt(const AttnArgs& A, const Walk& w, int row0, unsigned again, int from, int hidden, int to, int seen,
+                                            int half, int which, volatile Watch* watch) {
+  constexpr int E = D / 64, kAhead = 4;
+  using Stored = StoredOf<T, QUANT>;
+  using Words = typename WordsOf<E * sizeof(Stored)>::type;
+  const int lane = threadIdx.x & 31;
+  int nan[E], up[E], down[E];                                  // of this lane's columns: the first NaN, infinity, negative infinity
+#pragma unroll
+  for (int e = 0; e < E; ++e) nan[e] = up[e] = down[e] = to;
+  const auto look = [&](int a, int z) {
+#pragma unroll 1
+    for (int j0 = a; j0 < z; j0 += 32) {
+      // (no such page: zeros in the product)
+      const long long off = j0 + lane < z ? row_offset(A, w.b, w.kh, j0 + lane, nullptr) : -1;
+#pragma unroll 1
+      for (int c = 0; c < 32 && j0 + c < z; c += kAhead) {
+        Words vw[kAhead];
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+          const long long o = __shfl_sync(0xffffffffu, off, c + x);
+          vw[x] = Words{};
+          if (o >= 0) vw[x] = __ldg(reinterpret_cast<const Words*>(static_cast<const Stored*>(A.c.v) + o + half * (D / 2)) + lane);
+        }
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+          float v[E];
+          widen_all<Stored, E>(vw[x], v);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (v[e] != v[e]) nan[e] = min(nan[e], j0 + c + x);
+            if (v[e] == INFINITY) up[e] = min(up[e], j0 + c + x);
+            if (v[e] == -INFINITY) down[e] = min(down[e], j0 + c + x);
+          }
+        }
+      }
+      if (lane == 0) watch->alive = globaltimer();
+    }
+  };
+  const auto first = [&](int e) { return min(nan[e], min(up[e], down[e])); };
+  look(hidden, to);
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) any |= first(e) < to;
+  if (!__any_sync(0xffffffffu, any)) return 0;
+  look(from, hidden);
+  unsigned rest = 0;
+#pragma unroll 1
+  for (; again; again &= again - 1) {
+    const int src = __ffs(again) - 1, stop = __shfl_sync(0xffffffffu, seen, src);
+    const int R = w.tile * A.m + row0 + src, tok = A.by_rep.of(R), head = w.kh * A.rep + R - tok * A.rep;
+    const int at = half * (D / 2) + lane * E;
+    T* const out = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h + at;
+    float* const part = part_row<D>(A.part, gridDim.x, blockIdx.x, max(which, 0), row0 + src) + at;
+    bool met = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (out) out[lane * E + e] = from_float<T>(acc[e] * inv);
-      else part[lane * E + e] = acc[e];
+      const bool n = nan[e] < stop || (up[e] < stop && down[e] < stop), p = up[e] < stop;
+      if (n || p || down[e] < stop) {
+        const float y = n ? __int_as_float(0x7fc00000) : p ? INFINITY : -INFINITY;
+        if (which < 0) out[e] = from_float<T>(y);
+        else part[e] = y;
+      } else {
+        met |= first(e) < to;
+      }
+    }
+    if (__any_sync(0xffffffffu, met)) rest |= 1u << src;
+  }
+  return rest;
+}
+
+// Rows taken again: o over positions [from, seen) of each row's own, from its m, the columns [half * D / 2, ...) of it,
+// into the CTA's partial result `which` or (-1) divided by its sum into the output; rows as above. Two rows at a time share
+// the keys and values, in few registers (four rows of two positions ahead took 0.28 to 0.8 s where two take 0.46 to 0.8
+// below, but the kernel spilled round the call: 48 decodes 131 us against 125).
+// (148 tiles of 64 to 128 rows over 131072 positions: each spoilt by its last token's value alone, so that all other rows are
+// taken again, 0.46 s, 0.8 at 256 columns; by every value of a column, so that put_spoilt does, 20 to 29 ms; clean, 1.5 to 4.)
+template <typename T, int D, bool QUANT>
+__device__ __noinline__ void rows_again(const AttnArgs& A, const Walk& w, int row0, unsigned again, int from, int seen, float m, float inv,
+                                        int half, int which, volatile Watch* watch) {
+  constexpr int E = D / 32, EV = D / 64, kRows = 2, kAhead = 2;
+  using Stored = StoredOf<T, QUANT>;
+  using KeyWords = typename WordsOf<E * sizeof(Stored)>::type;
+  using ValueWords = typename WordsOf<EV * sizeof(Stored)>::type;
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  while (again) {
+    int src[kRows], to[kRows], stop = 0, n = 0;
+    float x[kRows][E], acc[kRows][EV], top[kRows], over[kRows];
+    T* out[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      src[i] = again ? __ffs(again) - 1 : src[0];              // (rows short of four repeat the first, unwritten)
+      if (again) ++n;
+      again &= again - 1;
+      to[i] = __shfl_sync(0xffffffffu, seen, src[i]);
+      top[i] = __shfl_sync(0xffffffffu, m, src[i]);
+      over[i] = __shfl_sync(0xffffffffu, inv, src[i]);
+      stop = max(stop, to[i]);
+      const int R = w.tile * A.m + row0 + src[i], tok = A.by_rep.of(R), head = w.kh * A.rep + R - tok * A.rep;
+      const T* const q = static_cast<const T*>(A.q) + (long long)(w.r.t0 + tok) * A.sq_t + head * A.sq_h;
+      out[i] = static_cast<T*>(A.o) + (long long)(w.r.t0 + tok) * A.so_t + head * A.so_h;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = to_float(q[lane * E + e]);
+#pragma unroll
+      for (int e = 0; e < EV; ++e) acc[i][e] = 0.f;
+    }
+#pragma unroll 1
+    for (int j0 = from; j0 < stop; j0 += 32) {
+      long long so = 0;                                        // this lane's position; -1: no such page
+      const long long off = j0 + lane < stop ? row_offset(A, w.b, w.kh, j0 + lane, QUANT ? &so : nullptr) : -1;
+      float ks = A.scale * kLog2e, vs = 0.f;
+      if (QUANT && off >= 0) {
+        ks *= __ldg(A.c.k_scale + so);
+        vs = log2f(__ldg(A.c.v_scale + so));
+      }
+#pragma unroll 1
+      for (int c = 0; c < 32 && j0 + c < stop; c += kAhead) {
+        KeyWords kw[kAhead];
+        ValueWords vw[kAhead];
+        bool there[kAhead];
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+          const long long o = __shfl_sync(0xffffffffu, off, c + z);
+          there[z] = o >= 0;
+          kw[z] = KeyWords{};
+          vw[z] = ValueWords{};
+          if (o >= 0) {
+            kw[z] = __ldg(reinterpret_cast<const KeyWords*>(static_cast<const Stored*>(A.c.k) + o) + lane);
+            vw[z] = __ldg(reinterpret_cast<const ValueWords*>(static_cast<const Stored*>(A.c.v) + o + half * (D / 2)) + lane);
+          }
+        }
+        float s[kAhead][kRows];
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+          float k[E];
+          widen_all<Stored, E>(kw[z], k);
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            s[z][i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[z][i] = fmaf(x[i][e], k[e], s[z][i]);
+          }
+        }
+#pragma unroll
+        for (int y = 16; y; y >>= 1)
+#pragma unroll
+          for (int z = 0; z < kAhead; ++z)
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) s[z][i] += __shfl_xor_sync(0xffffffffu, s[z][i], y);
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+          const float f = __shfl_sync(0xffffffffu, ks, c + z), add = __shfl_sync(0xffffffffu, vs, c + z);
+          float v[EV];
+          widen_all<Stored, EV>(vw[z], v);
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            if (!there[z] || j0 + c + z >= to[i]) continue;    // (no such page: the score is NaN, so is l, and the row is not here)
+            const float p = exp2_approx(fmaf(s[z][i], f, add) - top[i]);
+#pragma unroll
+            for (int e = 0; e < EV; ++e) acc[i][e] = fmaf(p, v[e], acc[i][e]);
+          }
+        }
+      }
+      if (lane == 0) watch->alive = globaltimer();
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      if (i >= n) continue;
+      const int at = half * (D / 2) + lane * EV;
+      if (which < 0) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) out[i][at + e] = from_float<T>(acc[i][e] * over[i]);
+      } else {
+        float* const p = part_row<D>(A.part, gridDim.x, blockIdx.x, which, row0 + src[i]);
+#pragma unroll
+        for (int e = 0; e < EV; ++e) p[at + e] = acc[i][e];
+      }
     }
   }
+}
+
+// The rows `again` (a lane each) of a softmax warp whose product met a value that is not finite; m and inv in the lanes.
+template <typename T, int D, bool QUANT>
+__device__ __noinline__ void mend_rows(const AttnArgs& A, const Walk& w, unsigned again, float m, float inv, volatile Watch* watch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = warp >> 2, row0 = A.m == kM ? (warp & 3) * 32 : 0;
+  const int from = w.first * kKeys, stop = w.stop() * kKeys, to = min(row_limit(A, w.r, w.r.n - 1), stop);
+  const int which = w.first == 0 && stop == w.units * kKeys ? -1 : w.first == 0;
+  const int seen = min(row_limit(A, w.r, A.by_rep.of(w.tile * A.m + row0 + lane)), stop);
+  // (tiles of few rows: every value has met weights of 0)
+  const int low = A.m == kM ? __reduce_min_sync(0xffffffffu, again >> lane & 1 ? seen : 0x7fffffff) : 0;
+  again = put_spoilt<T, D, QUANT>(A, w, row0, again, from, max(low, from), to, seen, half, which, watch);
+  if (again) rows_again<T, D, QUANT>(A, w, row0, again, from, seen, m, inv, half, which, watch);
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------
@@ -572,7 +753,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int dead;
+  __shared__ Watch watch;
   __shared__ long long sh_total[32];
   __shared__ float sh_m[2][kM];
   __shared__ float2 sh_swap[2][2 * kM];                        // [buffer][group][lane of tensor memory]: its maximum and sum
@@ -603,7 +784,8 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
     mbar_init(&bar.drain, 1);
     mbar_init(&bar.meet, kSoftWarps);
     fence_mbar_init();
-    dead = 0;
+    watch.dead = 0;
+    watch.alive = 0;
     A.desc[cta].last = -1;
     A.desc[cta].err = 0;
   }
@@ -671,7 +853,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   // A wait that outlasts its limit marks the CTA dead; every role then leaves its loop at its next wait
   // that is not over at once.
   const auto wait = [&](uint64_t* b, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_test_wait(b, parity)) || wait_on(b, parity, &dead);
+    return __all_sync(0xffffffffu, mbar_test_wait(b, parity)) || wait_on(b, parity, &watch);
   };
 
   if (warp < kSoftWarps) {
@@ -1074,11 +1256,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           }
         }
         // A value that is not finite at a position that this row may not see has met a weight of 0 in
-        // the product. Only a causal row's last units can hold one; such a row is taken again from
+        // the product. Only a causal row's last units can hold one: where they do, such a row is taken again from
         // its own positions alone, with m and l as they are.
         // (SPREAD: a position's weight is 0 in three of a row's lanes, so any such value does this.)
         const float worst = (bad[0] + bad[1]) + (bad[2] + bad[3]);
-        const int seen = min(lim, stop * kKeys);             // where its positions here end
         unsigned again = __ballot_sync(0xffffffffu, worst != 0.f);
         const unsigned take = __ballot_sync(0xffffffffu, valid && l == l && (SPREAD || (A.causal && lim < stop * kKeys)));
         if constexpr (SPREAD) {                              // from the lanes that added a row up to the row's own
@@ -1086,18 +1267,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
           again = __ballot_sync(0xffffffffu, lane >= base_row && lane < base_row + 32 / per_row &&
                                                  (again >> ((lane - base_row) * per_row & 31) & ((1u << per_row) - 1)) != 0);
         }
-        again &= take;
-#pragma unroll 1
-        while (again) {
-          const int src = __ffs(again) - 1;
-          again &= again - 1;
-          const int row = SPREAD ? src : pair * 32 + src, RR = w.tile * M + row, tk = A.by_rep.of(RR), hd = w.kh * A.rep + RR - tk * A.rep;
-          const int li = __shfl_sync(0xffffffffu, seen, src);
-          const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
-          row_again<T, D, QUANT>(A, w.b, w.kh, static_cast<const T*>(A.q) + (long long)(w.r.t0 + tk) * A.sq_t + hd * A.sq_h, first * kKeys, li, mr, ir,
-                          half, whole ? static_cast<T*>(A.o) + (long long)(w.r.t0 + tk) * A.so_t + hd * A.so_h : nullptr,
-                          part_row<D>(A.part, grid, cta, first == 0, row));
-        }
+        if (again & take) mend_rows<T, D, QUANT>(A, w, again & take, m, inv, &watch);
         tc_fence_before();
       }
       __syncwarp();
@@ -1391,7 +1561,7 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   }
   tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0 && dead) A.desc[cta].err = DEV_TIMEOUT_FULL;
+  if (threadIdx.x == 0 && watch.dead) A.desc[cta].err = DEV_TIMEOUT_FULL;
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, Lay::cols);
