@@ -374,6 +374,14 @@ CFB_DEV float exp2_approx(float x) {
   return y;
 }
 
+// A value's scale as the weights take it, with its logarithm and its inverse: at least 2^-60, so that a row whose scale
+// is 0 (a slot never written, a row of zeros) keeps its part of the sum, and stays out of o but for 448 2^-60. The sum loses
+// a position only where its weight is less than 2^-66 of another's of scale 1. (Patterns order like integers: what is NaN
+// or negative is larger, and its logarithm is NaN.)
+CFB_DEV float value_scale(float x) {
+  return __uint_as_float(max(__float_as_uint(x + 0.f), __float_as_uint(0x1p-60f)));
+}
+
 // What the key rows of a page outside the pool read: NaN in both 16-bit types.
 __device__ const uint4 kNanRow[1] = {{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}};
 
@@ -647,7 +655,7 @@ __device__ __noinline__ void rows_again(const AttnArgs& A, const Walk& w, int ro
       float ks = A.scale * kLog2e, vs = 0.f;
       if (QUANT && off >= 0) {
         ks *= __ldg(A.c.k_scale + so);
-        vs = log2f(__ldg(A.c.v_scale + so));
+        vs = log2f(value_scale(__ldg(A.c.v_scale + so)));
       }
 #pragma unroll 1
       for (int c = 0; c < 32 && j0 + c < stop; c += kAhead) {
@@ -1392,8 +1400,9 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
             uint8_t* const at = sm + Lay::off_scale + ss * kScaleBytes;
             float* const two = reinterpret_cast<float*>(at) + (ct >> 1) * 4 + (ct & 1);            // k's of two positions, then log2 v's
             two[0] = sc.x;
-            two[2] = log2f(sc.y);
-            reinterpret_cast<float*>(at + kKeys * 8)[ct] = sc.y > 0.f ? 1.f / sc.y : 1.f;
+            const float vs = value_scale(sc.y);
+            two[2] = log2f(vs);
+            reinterpret_cast<float*>(at + kKeys * 8)[ct] = vs > 0.f ? 1.f / vs : 1.f;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.sc_full[ss]);
             if (i + 1 < stop) look(w, i + 1);

@@ -17,7 +17,8 @@ class PagedKVCache:
     """Keys and values of one layer in ``pages`` pages of ``page_size`` slots. A token's flat slot is
     ``page * page_size + offset``. ``dtype``: fp16 or bf16 (rows are kept as they are), or
     ``torch.float8_e4m3fn`` (each row x of a token and kv head as codes and one fp32 scale
-    ``max(max|x|, 2**-24) / 448``; a row with a NaN or an infinity reads back as NaN).
+    ``max(max|x|, 2**-24) / 448``; a row with a NaN or an infinity reads back as NaN). A slot that was never
+    written holds zeros.
 
     Buffers: ``k``, ``v`` [pages, kv_heads, page_size, head_dim], so that a head's rows of a page
     are contiguous; ``k_scale``, ``v_scale`` fp32 [pages, kv_heads, page_size] (e4m3 only).

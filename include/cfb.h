@@ -389,8 +389,9 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * slots, kept as fp16 (dtype 1), bf16 (2) or e4m3 (3). Row (slot, kv head h) of a flat slot =
  * page * page_size + offset is at page * page_stride + h * head_stride + offset * slot_stride
  * elements of k and of v; its fp32 scale (dtype 3 only) at page * scale_page_stride +
- * h * scale_head_stride + offset * scale_slot_stride of k_scale and of v_scale (positive, or NaN
- * for a row that reads as NaN; codes finite). k and v: 16-byte
+ * h * scale_head_stride + offset * scale_slot_stride of k_scale and of v_scale (not negative, or NaN
+ * for a row that reads as NaN; codes finite). Attention takes a value scale below 2^-60 as 2^-60: a row of
+ * scale 0 has its part of the softmax, and adds less than 448 2^-60 to o. k and v: 16-byte
  * aligned, strides multiples of 16 bytes. Supported: dim in {64, 128, 256}. */
 typedef struct cfb_kv_cache {
   void* k;
