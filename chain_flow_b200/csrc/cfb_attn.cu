@@ -8,7 +8,7 @@
 // Over an e4m3 cache k_j = ks_j kc_j and v_j = vs_j vc_j (codes and scales), and
 //   s_j = (scale ks_j) (q_i . kc_j),  w_j = s_j + log vs_j,  m = max w_j,
 //   o_i = sum exp(w_j - m) vc_j / l,  l = sum exp(w_j - m) / vs_j,
-// so the weights stay at most 1 (or a fixed power of two), whatever the scales. Scores are formed on the 8-bit
+// so the weights stay at most a fixed power of two, whatever the scales. Scores are formed on the 8-bit
 // tensor path: keys as the codes they are, the query in e4m3 pieces of 4 bits, q = q1 + q2 (+ q3), two over
 // bf16 (8 bits) and three over fp16 (11); a query row is first brought to a largest element of 128 to 256 by a
 // power of two, so that what e4m3's smallest step (2^-9) loses of a small element is 2^-17 of the largest.
@@ -745,8 +745,8 @@ __device__ __noinline__ void mend_rows(const AttnArgs& A, const Walk& w, unsigne
 // lane, units alternating between two groups: the lane's scores come from tensor memory, and the weights go
 // back there in the operands' type (the one rounding of the weights: unit roundoff 2^-8 bf16, 2^-11 fp16, 2^-17
 // in pieces; their sum is of the unrounded fp32 values). O is rescaled only when the row's maximum has grown by
-// more than 2^kSlack since the last time: weights are then at most 2^8 (in pieces 2^8.5, and the largest at least
-// 2^6.5), far inside the types, and most units touch O not at all.
+// more than 2^kSlack since the last time: weights are then at most 2^8 (fp16: 2^15, and the largest at least 2^7; in
+// pieces 2^8.5 and 2^6.5), inside the types, and most units touch O not at all.
 template <typename T, int D, int SRC, int M>
 __global__ void __launch_bounds__(threads_of(SRC, M), 1)
 attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -755,8 +755,10 @@ attn_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensor
   constexpr bool SPREAD = M < kM;
   constexpr bool PIECES = QUANT && SPREAD, WIDEN = QUANT && !SPREAD;
   constexpr int kCols = SPREAD ? kKeys / 4 : kKeys;            // a unit's columns of a softmax thread
-  // the weights are at most 2^(kLift + kSlack), and o is rescaled only when the maximum has grown by 2^kSlack
-  constexpr float kLift = PIECES ? 6.5f : 0.f, kSlack = PIECES ? 2.f : 8.f;
+  // the weights are at most 2^(kLift + kSlack), and o is rescaled only when the maximum has grown by 2^kSlack. (fp16: at
+  // most 2^15, so that its smallest step, 2^-24, is 2^-31 of the largest or less: at 2^-24, thousands of small weights
+  // under a large one vanished together.)
+  constexpr float kLift = PIECES ? 6.5f : std::is_same<T, __half>::value ? 7.f : 0.f, kSlack = PIECES ? 2.f : 8.f;
   constexpr int kSt = Lay::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bar;
