@@ -887,11 +887,13 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
   }
 }
 
-cfb_status check_gdn(const cfb_gdn_args* g, int B) {
-  if (!g || B < 0) return CFB_ERR_INVALID_ARG;
-  if (!g->A_log || !g->dt_bias || !g->a || !g->b || !g->q || !g->k || !g->v || !g->o || !g->state_in || !g->state_out ||
-      !g->init_slot || !g->out_slot || g->H <= 0 || g->HV <= 0 || g->slots <= 0)
+cfb_status check_gdn(const cfb_gdn_args* g, int T, int B) {
+  if (!g || T < 0 || B < 0) return CFB_ERR_INVALID_ARG;
+  if (!g->A_log || !g->dt_bias || !g->state_in || !g->state_out || !g->init_slot || !g->out_slot || g->H <= 0 || g->HV <= 0 ||
+      g->slots <= 0)
     return CFB_ERR_INVALID_ARG;
+  // (rows of no tokens are read nowhere, and an empty array's address may be null)
+  if (T > 0 && (!g->a || !g->b || !g->q || !g->k || !g->v || !g->o)) return CFB_ERR_INVALID_ARG;
   for (int c : {g->A_log_dtype, g->dt_bias_dtype, g->a_dtype, g->b_dtype})
     if (c < DT_F32 || c > DT_BF16) return CFB_ERR_INVALID_ARG;
   if ((g->dtype != DT_F16 && g->dtype != DT_BF16) || g->K != kK || g->V <= 0 || g->V % 32 || g->HV % g->H ||
@@ -973,7 +975,7 @@ cfb_status launch_chunks(const cfb_gdn_args& g, const int32_t* cu, int total, in
 
 extern "C" cfb_status cfb_gdn_step(const cfb_gdn_args* g, int B, void* stream) {
   if (B == 0 && g) return CFB_OK;
-  if (const cfb_status s = check_gdn(g, B)) return s;
+  if (const cfb_status s = check_gdn(g, B, B)) return s;
   launch_walk(*g, nullptr, B, B, static_cast<cudaStream_t>(stream));
   return cfb_launch_status("gdn_walk_kernel");
 }
@@ -986,8 +988,8 @@ extern "C" size_t cfb_gdn_chunk_workspace(int T, int B, int HV) {
 extern "C" cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, int T, int B, void* ws, size_t ws_bytes,
                                     void* stream) {
   if (B == 0 && g) return CFB_OK;
-  if (const cfb_status s = check_gdn(g, B)) return s;
-  if (T < 0 || !cu || !ws) return CFB_ERR_INVALID_ARG;
+  if (const cfb_status s = check_gdn(g, T, B)) return s;
+  if (!cu || !ws) return CFB_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_gdn_chunk_workspace(T, B, g->HV)) return CFB_ERR_WORKSPACE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int* const err = static_cast<int*>(ws);

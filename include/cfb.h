@@ -451,12 +451,12 @@ cfb_status cfb_paged_attn_error(const void* ws, int* device_error);
  *   S <- S * exp(-exp(A_log[hv]) * softplus(a[t, hv] + dt_bias[hv]))
  *   S <- S + sigmoid(b[t, hv]) * (v[t, hv] - S kn) (x) kn,   o[t, hv] = S qn,
  * and state_out[out_slot[b]] = the last S (negative or >= slots: not kept; a request without tokens
- * copies its state). q, k [T, H, K] and v, o [T, HV, V] of dtype 1 or 2, a and b [T, HV]: inner
- * dims contiguous, the given token strides in elements (q, k, v, o rows 16-byte aligned). State
- * slots fp32 [HV, V, K], state_in and state_out with the same slot_stride in floats and the same
- * number of slots; they may be the same array. The out slots of a call are distinct, and no
- * request reads another's out slot. Other arguments as cfb_tree_gdn_verify. Supported: K == 128, V
- * a multiple of 32, HV a multiple of H.
+ * copies its state; with T == 0 a, b, q, k, v and o may be NULL). q, k [T, H, K] and v, o [T, HV, V]
+ * of dtype 1 or 2, a and b [T, HV]: inner dims contiguous, the given token strides in elements (q, k,
+ * v, o rows 16-byte aligned). State slots fp32 [HV, V, K], state_in and state_out with the same
+ * slot_stride in floats and the same number of slots; they may be the same array. The out slots of a
+ * call are distinct, and no request reads another's out slot. Other arguments as
+ * cfb_tree_gdn_verify. Supported: K == 128, V a multiple of 32, HV a multiple of H.
  * cfb_gdn_step: one token per request (row t = b of B rows). cfb_gdn_chunk: any lengths; ws:
  * cfb_gdn_chunk_workspace(T, B, HV) bytes, 256-byte aligned, for calls ordered on one stream; it
  * needs no initialisation. */
