@@ -28,6 +28,7 @@ class PagedAttention:
         self.ws_bytes = int(self.lib.cfb_paged_attn_workspace(heads, kv_heads, head_dim))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+        self._ran = False
 
     def _refuse(self, query, cache, page_table, kv_len, cu_q):
         for t, n in ((query, "query"), (page_table, "page_table"), (kv_len, "kv_len"), (cu_q, "cu_q")):
@@ -43,10 +44,12 @@ class PagedAttention:
         raise _lib.CfbError("PagedAttention: page_table [B, width], kv_len [B] and cu_q [B + 1] disagree")
 
     def check(self) -> None:
-        """Raises if a device-side wait of the last call expired (its outputs are then invalid). Waits
-        for the GPU."""
+        """Raises if a device-side wait of the last call with rows and requests expired (its outputs are then invalid;
+        without such a call there is nothing to raise). Waits for the GPU."""
         err = C.c_int(0)
         torch.cuda.synchronize(self.device)
+        if not self._ran:                                # the error words are the kernel's to write
+            return
         _lib.check(self.lib.cfb_paged_attn_error(self.ws_ptr, C.byref(err)), "cfb_paged_attn_error")
         if err.value:
             raise _lib.CfbError(f"PagedAttention: device error {err.value} (a bounded wait expired); outputs are invalid")
@@ -93,4 +96,6 @@ class PagedAttention:
             width, kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),
             self.scale if scale is None else scale, T, B, self.heads, causal, dt, self.ws_ptr, self.ws_bytes,
             _lib.stream_ptr()), "cfb_paged_attn")
+        if T and B:
+            self._ran = True
         return out, lse

@@ -250,12 +250,15 @@ class ChunkedGdn:
         self.ws_bytes = int(self.lib.cfb_gdn_chunk_workspace(max_tokens, max_requests, value_heads))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+        self._ran = False
 
     def check(self) -> None:
-        """Raises if a device-side wait of the last call (with tokens) expired (its outputs are then
-        invalid, its states NaN). Waits for the GPU."""
+        """Raises if a device-side wait of the last call with tokens expired (its outputs are then invalid, its
+        states NaN; without such a call there is nothing to raise). Waits for the GPU."""
         err = C.c_int(0)
         torch.cuda.synchronize(self.device)
+        if not self._ran:                                # the error word is the kernels' to write
+            return
         _lib.check(self.lib.cfb_gdn_chunk_error(self.ws_ptr, C.byref(err)), "cfb_gdn_chunk_error")
         if err.value:
             raise _lib.CfbError(f"ChunkedGdn: device error {err.value} (a bounded wait expired); outputs are invalid")
@@ -282,3 +285,5 @@ class ChunkedGdn:
         cu = _lib.int32(cu_seqlens)
         _lib.check(self.lib.cfb_gdn_chunk(args, cu.data_ptr(), T, B, self.ws_ptr, self.ws_bytes,
                                           _lib.stream_ptr()), "cfb_gdn_chunk")
+        if T and B:
+            self._ran = True

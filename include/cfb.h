@@ -441,8 +441,9 @@ cfb_status cfb_paged_attn(const void* q, int64_t sq_t, int64_t sq_h, const cfb_k
                           const int32_t* kv_len, const int32_t* cu_q, void* o, int64_t so_t,
                           int64_t so_h, float* lse, float scale, int T, int B, int H, int causal,
                           int dtype, void* ws, size_t ws_bytes, void* stream);
-/* Synchronous: the device error word of the last cfb_paged_attn call with this workspace: 0 if it
- * completed, else a bounded device-side wait expired and its outputs are invalid. */
+/* Synchronous: the device error word of the last cfb_paged_attn call with T > 0, B > 0 and this workspace
+ * (there has to be one): 0 if it completed, else a bounded device-side wait expired and its outputs are
+ * invalid. */
 cfb_status cfb_paged_attn_error(const void* ws, int* device_error);
 
 /* The gated delta rule of cfb_tree_gdn_verify without a tree: request b's tokens are the rows
@@ -483,8 +484,9 @@ cfb_status cfb_gdn_step(const cfb_gdn_args* g, int B, void* stream);
 size_t cfb_gdn_chunk_workspace(int T, int B, int HV);
 cfb_status cfb_gdn_chunk(const cfb_gdn_args* g, const int32_t* cu, int T, int B, void* ws,
                          size_t ws_bytes, void* stream);
-/* Synchronous: the device error word of the last cfb_gdn_chunk call with T > 0 and this workspace: 0
- * if it completed, else a bounded device-side wait expired; its outputs are invalid (states NaN). */
+/* Synchronous: the device error word of the last cfb_gdn_chunk call with T > 0, B > 0 and this workspace
+ * (there has to be one): 0 if it completed, else a bounded device-side wait expired; its outputs are
+ * invalid (states NaN). */
 cfb_status cfb_gdn_chunk_error(const void* ws, int* device_error);
 
 /* ---- the per-request context ring -------------------------------------------------------------
