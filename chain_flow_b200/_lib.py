@@ -217,6 +217,16 @@ def stream_ptr(stream=None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def stream_of(device: int, what: str) -> int:
+    """The current stream, for a launch over tensors of cuda device ``device``. That has to be the current
+    device: a kernel launched on another would meet addresses that are not its own."""
+    import torch
+    current = torch._C._cuda_getDevice()
+    if device != current:
+        raise CfbError(f"{what}: the tensors are on cuda:{device}, the current device (or the given stream's) is cuda:{current}")
+    return torch._C._cuda_getCurrentRawStream(current)
+
+
 def require_cuda(t, name: str) -> None:
     if not t.is_cuda:
         raise CfbError(f"{name} must be a CUDA tensor: the chain_flow_b200 engine has no CPU path")

@@ -28,7 +28,7 @@ class PagedAttention:
         self.ws_bytes = int(self.lib.cfb_paged_attn_workspace(heads, kv_heads, head_dim))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
-        self._ran = False
+        self._dev, self._ran = self.ws.get_device(), False
 
     def _refuse(self, query, cache, page_table, kv_len, cu_q):
         for t, n in ((query, "query"), (page_table, "page_table"), (kv_len, "kv_len"), (cu_q, "cu_q")):
@@ -37,6 +37,8 @@ class PagedAttention:
                 raise _lib.CfbError(f"{n} is on {t.device}, the cache on {cache.device}")
         if query.dim() != 3 or query.shape[1] != self.heads or query.shape[2] != self.head_dim or query.stride(2) != 1:
             raise _lib.CfbError(f"query: expected [T, {self.heads}, {self.head_dim}] with a contiguous head dim, got {list(query.shape)}")
+        if cache._dev != self._dev:
+            raise _lib.CfbError(f"PagedAttention: the cache is on {cache.device}, this object's workspace on {self.device}")
         if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim:
             raise _lib.CfbError("PagedAttention: the cache has other kv heads or another head dim")
         if query.dtype not in _DT or (cache.k_scale is None and query.dtype != cache.dtype):
@@ -71,7 +73,7 @@ class PagedAttention:
         dt, sq = _DT.get(dtype), query.stride()
         if (len(shape) != 3 or shape[1] != self.heads or shape[2] != self.head_dim or sq[2] != 1 or dt is None
                 or (cache.k_scale is None and dtype != cache.dtype)
-                or cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim
+                or cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim or dev != self._dev
                 or page_table.dim() != 2 or page_table.shape[0] != B or kv_len.dim() != 1 or cu_q.shape != (B + 1,)
                 or any(t.get_device() != dev for t in (query, page_table, kv_len, cu_q))):
             self._refuse(query, cache, page_table, kv_len, cu_q)
@@ -95,7 +97,7 @@ class PagedAttention:
             query.data_ptr(), sq[0], sq[1], cache.desc, page_table.data_ptr(), max(st[0], width),
             width, kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),
             self.scale if scale is None else scale, T, B, self.heads, causal, dt, self.ws_ptr, self.ws_bytes,
-            _lib.stream_ptr()), "cfb_paged_attn")
+            _lib.stream_of(dev, "PagedAttention")), "cfb_paged_attn")
         if T and B:
             self._ran = True
         return out, lse

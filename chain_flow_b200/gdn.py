@@ -233,7 +233,7 @@ def gdn_step(A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, *, sc
     lib = _lib.load()
     B = q.shape[0]
     args, keep = _sequence_args("gdn_step", A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B)
-    _lib.check(lib.cfb_gdn_step(args, B, _lib.stream_ptr()), "cfb_gdn_step")
+    _lib.check(lib.cfb_gdn_step(args, B, _lib.stream_of(q.get_device(), "gdn_step")), "cfb_gdn_step")
 
 
 class ChunkedGdn:
@@ -250,7 +250,7 @@ class ChunkedGdn:
         self.ws_bytes = int(self.lib.cfb_gdn_chunk_workspace(max_tokens, max_requests, value_heads))
         self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=self.device)
         self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
-        self._ran = False
+        self._dev, self._ran = self.ws.get_device(), False
 
     def check(self) -> None:
         """Raises if a device-side wait of the last call with tokens expired (its outputs are then invalid, its
@@ -276,6 +276,8 @@ class ChunkedGdn:
         B = cu_seqlens.numel() - 1
         if cu_seqlens.dim() != 1 or B < 0 or cu_seqlens.get_device() != q.get_device() or q.dim() != 3 or v.dim() != 3:
             raise _lib.CfbError("ChunkedGdn: cu_seqlens must be 1-D [requests + 1] on q's device, q [T, H, K], v [T, HV, V]")
+        if q.get_device() != self._dev:
+            raise _lib.CfbError(f"ChunkedGdn: q is on {q.device}, this object's workspace on {self.device}")
         T, HV = q.shape[0], v.shape[1]
         if T > self.max_tokens or B > self.max_requests or HV > self.value_heads:
             raise _lib.CfbError(f"ChunkedGdn: {T} tokens / {B} requests / {HV} value heads exceed this object's "
@@ -284,6 +286,6 @@ class ChunkedGdn:
                                     out_state, B)
         cu = _lib.int32(cu_seqlens)
         _lib.check(self.lib.cfb_gdn_chunk(args, cu.data_ptr(), T, B, self.ws_ptr, self.ws_bytes,
-                                          _lib.stream_ptr()), "cfb_gdn_chunk")
+                                          _lib.stream_of(self._dev, "ChunkedGdn")), "cfb_gdn_chunk")
         if T and B:
             self._ran = True

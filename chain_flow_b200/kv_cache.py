@@ -110,7 +110,7 @@ class PagedKVCache:
         if dt not in (1, 2) or value.dtype != dtype or (self.k_scale is None and dtype != self.dtype):
             raise _lib.CfbError("PagedKVCache.write: key and value must share fp16 or bf16, the cache's own unless it is e4m3")
         _lib.check(self.lib.cfb_kv_write(self.desc, key.data_ptr(), sk[0], sk[1], value.data_ptr(), sv[0], sv[1], dt,
-                                         slots.data_ptr(), T, _lib.stream_ptr()), "cfb_kv_write")
+                                         slots.data_ptr(), T, _lib.stream_of(self._dev, "PagedKVCache.write")), "cfb_kv_write")
 
     def read(self, slots, dtype=None, stream=None):
         """(key, value) [T, kv_heads, head_dim] of the flat slots [T] in fp32, fp16 or bf16 (default:
@@ -126,5 +126,5 @@ class PagedKVCache:
         T, D = slots.shape[0], self.head_dim
         key, value = torch.empty(2, T, self.kv_heads, D, dtype=dtype, device=self.device).unbind(0)
         _lib.check(self.lib.cfb_kv_read(self.desc, slots.data_ptr(), T, key.data_ptr(), self.kv_heads * D, D, value.data_ptr(),
-                                        self.kv_heads * D, D, _DT[dtype], _lib.stream_ptr()), "cfb_kv_read")
+                                        self.kv_heads * D, D, _DT[dtype], _lib.stream_of(self._dev, "PagedKVCache.read")), "cfb_kv_read")
         return key, value

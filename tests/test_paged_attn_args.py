@@ -35,10 +35,10 @@ def _read_table(monkeypatch, table, B):
             seen.extend(([[x[b * stride + j] for j in range(width)] for b in range(B)], stride, width))
         return 0
 
-    monkeypatch.setattr(_lib, "stream_ptr", lambda stream=None: 0)
+    monkeypatch.setattr(_lib, "stream_of", lambda device, what: 0)
     attn = object.__new__(PagedAttention)
     attn.__dict__.update(lib=SimpleNamespace(cfb_paged_attn=entry), device=torch.device("cpu"), heads=H, kv_heads=HKV, head_dim=D,
-                         scale=0.125, ws_bytes=0, ws_ptr=0)
+                         scale=0.125, ws_bytes=0, ws_ptr=0, _dev=-1)
     cache = SimpleNamespace(_dev=-1, device=torch.device("cpu"), k_scale=None, dtype=torch.float16, kv_heads=HKV, head_dim=D, desc=None)
     attn(torch.zeros(3, H, D, dtype=torch.float16), cache, table, torch.zeros(B, dtype=torch.int32), torch.zeros(B + 1, dtype=torch.int32))
     return seen
