@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kStepThreads) gdn_walk_kernel(const cfb_gdn_ar
 // gdn_prep_kernel forms T = (I + A)^-1 and P of every chunk at once; gdn_scan_kernel then walks a
 // request's chunks with three products a chunk that depend on one another.
 //
-// Precision. The state is fp32 and has to stay so over thousands of chunks, so no product rounds an
+// Precision. The state is fp32 and has to stay so over thousands of chunks, so no product on its way rounds an
 // operand to fewer than 22 bits. k and q are exact as they are (their norms are applied afterwards, in
 // fp32). Over bf16, S and U meet k as three bf16 pieces, exactly, 16 columns a product (a chunk of one head
 // at 8191 tokens: 1.9 us; the tf32 terms, 8 columns a product, 2.0). Else, S, U and T are split into two
@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(kStepThreads) gdn_walk_kernel(const cfb_gdn_ar
 // and chunk. Exponents of differences G_i - G_j are of sums kept in 64 bits: in 32, a strong decay's G of a
 // few hundred would cost 1e-5. S is updated by one fp32 fma an element from a product that starts at zero,
 // because sums carried through the tensor cores lose a little towards zero with every step. o is rounded to
-// 16 bits, so its own products take hi terms only over bf16 (11 bits against its 8), and both terms over fp16.
+// 16 bits and nothing depends on it, so its own products' S, U and P are the exception: over fp16 both terms, over bf16
+// one, rounded to nearest (11 bits against o's 8; cut off, every output came out 2^-10.7 short).
 //
 // Why mma.sync and not tcgen05: the scan is a chain over a head's chunks, and what bounds it is the
 // latency of one link, not throughput. With 16 value rows a warp, the state lives in the warp's
@@ -198,6 +199,9 @@ CFB_DEV void split3(float x, float y, uint32_t (&p)[3]) {
     p[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
   }
 }
+// x rounded to 11 bits (tf32); a NaN may come out as anything
+CFB_DEV float nearest11(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
+CFB_DEV float nearest11_nan(float x) { return x == x ? nearest11(x) : x; }
 CFB_DEV void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(64) gdn_prep_kernel(const cfb_gdn_args g, cons
           split(x, w.x, w.z);
           split(y, w.y, w.w);
           if constexpr (Prep<T>::kP == 4) *reinterpret_cast<float4*>(dst) = w;
-          else *reinterpret_cast<float2*>(dst) = make_float2(w.x, w.y);
+          else *reinterpret_cast<float2*>(dst) = make_float2(nearest11_nan(x), nearest11_nan(y));
         }
       }
     float* const v = out + Prep<T>::kVec;
@@ -448,6 +452,15 @@ CFB_DEV void operand(const float (&s)[4], float (&hi)[4], float (&lo)[4]) {
   split(s[2], hi[1], lo[1]);
   split(s[1], hi[2], lo[2]);
   split(s[3], hi[3], lo[3]);
+}
+// the same in one term, rounded to nearest
+template <bool NAN_KEPT>
+CFB_DEV void operand11(const float (&s)[4], float (&hi)[4]) {
+  const auto near = [](float x) { return NAN_KEPT ? nearest11_nan(x) : nearest11(x); };
+  hi[0] = near(s[0]);
+  hi[1] = near(s[2]);
+  hi[2] = near(s[1]);
+  hi[3] = near(s[3]);
 }
 
 template <typename T, int TILES>
@@ -559,7 +572,8 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
         const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
         uint32_t qw[4];
         ldmatrix4(qw, block(q_at, j));
-        operand(sj, hi[0], lo[0]);
+        if constexpr (kFine) operand(sj, hi[0], lo[0]);
+        else operand11<false>(sj, hi[0]);                      // (a row of S with a NaN in it has lost its first token)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float2 q2 = unpack16<T>(n0 ? qw[2 + x] : qw[x]);
@@ -572,7 +586,8 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
       for (int jb = 0; jb < kBlocks; ++jb) {
         const float4 u4 = reinterpret_cast<const float4*>(hand + Lay::off_u)[jb * 32 + lane];
         const float u[4] = {u4.x, u4.y, u4.z, u4.w};
-        operand(u, hi[jb], lo[jb]);
+        if constexpr (kFine) operand(u, hi[jb], lo[jb]);
+        else operand11<true>(u, hi[jb]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&freed[tile][c & 1]);
