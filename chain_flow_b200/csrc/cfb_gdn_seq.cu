@@ -964,26 +964,22 @@ cfb_status launch_tiles(const cfb_gdn_args& g, const int32_t* cu, int total, int
   return cfb_launch_status("gdn_scan_kernel");
 }
 template <typename T>
-cfb_status launch_scan(const cfb_gdn_args& g, const int32_t* cu, int total, int B, const float* ws, int* err, cudaStream_t st) {
-  CUtensorMap q, k, v;
-  if (!tensor_map_encoder()) return cfb_launch_status("cuTensorMapEncodeTiled");
-  if (!key_map(&q, g.q, g.q_stride, total, g.H) || !key_map(&k, g.k, g.k_stride, total, g.H) ||
-      !value_map(&v, g.v, g.v_stride, total, g.HV, g.V))
-    return CFB_ERR_INVALID_ARG;
-  // Four tiles a CTA where even so each SM has one and a half and more: more chains side by side, fewer CTAs (32 value
-  // heads of 128: nine requests 480 us against 518; one request, 64 CTAs on 148 SMs, would leave half of them idle).
-  const bool four = g.V % 64 == 0 && (long long)g.V / 32 * g.HV * B >= 3ll * device_sms();
-  return four ? launch_tiles<T, 4>(g, cu, total, B, ws, err, q, k, v, st) : launch_tiles<T, 2>(g, cu, total, B, ws, err, q, k, v, st);
-}
-template <typename T>
 cfb_status launch_chunks(const cfb_gdn_args& g, const int32_t* cu, int total, int B, float* ws, int* err, cudaStream_t st) {
   if (total == 0) {                                            // states only
     launch_walk(g, cu, total, B, st);
     return cfb_launch_status("gdn_walk_kernel");
   }
+  CUtensorMap q, k, v;
+  if (!tensor_map_encoder()) return CFB_ERR_CUDA;
+  if (!key_map(&q, g.q, g.q_stride, total, g.H) || !key_map(&k, g.k, g.k_stride, total, g.H) ||
+      !value_map(&v, g.v, g.v_stride, total, g.HV, g.V))
+    return CFB_ERR_INVALID_ARG;
   gdn_prep_kernel<T><<<dim3((unsigned)chunk_slots(total, B), (unsigned)g.HV), 64, 0, st>>>(g, cu, total, B, ws, err);
   if (const cfb_status s = cfb_launch_status("gdn_prep_kernel")) return s;
-  return launch_scan<T>(g, cu, total, B, ws, err, st);
+  // Four tiles a CTA where even so each SM has one and a half and more: more chains side by side, fewer CTAs (32 value
+  // heads of 128: nine requests 480 us against 518; one request, 64 CTAs on 148 SMs, would leave half of them idle).
+  const bool four = g.V % 64 == 0 && (long long)g.V / 32 * g.HV * B >= 3ll * device_sms();
+  return four ? launch_tiles<T, 4>(g, cu, total, B, ws, err, q, k, v, st) : launch_tiles<T, 2>(g, cu, total, B, ws, err, q, k, v, st);
 }
 
 }  // namespace
