@@ -93,6 +93,8 @@ class PagedAttention:
         elif lse.shape != (self.heads, T) or lse.dtype != torch.float32 or lse.get_device() != dev or not lse.is_contiguous():
             raise _lib.CfbError(f"lse must be contiguous fp32 [{self.heads}, {T}] on the query's device")
         so = out.stride()
+        if T == 1:                                       # one token's stride can be any number, as 1 of a transposed column
+            sq, so = (0, sq[1]), (0, so[1])
         _lib.check(self.lib.cfb_paged_attn(
             query.data_ptr(), sq[0], sq[1], cache.desc, page_table.data_ptr(), max(st[0], width),
             width, kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), so[0], so[1], lse.data_ptr(),

@@ -184,9 +184,12 @@ def _refuse_sequence(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, o
 
 
 def _heads_strides(t):
-    """The token stride of a [T, heads, dim] tensor with contiguous heads, else None."""
+    """The token stride of a [T, heads, dim] tensor with contiguous heads, else None. (One token's can be any
+    number, as 1 of a transposed column: what the heads take stands for it.)"""
     st = t.stride()
-    return st[0] if st[2] == 1 and (st[1] == t.shape[2] or t.shape[1] == 1) else None
+    if st[2] != 1 or (st[1] != t.shape[2] and t.shape[1] != 1):
+        return None
+    return st[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B):

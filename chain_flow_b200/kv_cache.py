@@ -105,6 +105,8 @@ class PagedKVCache:
         for t, n, st in ((key, "key", sk), (value, "value", sv)):
             if t.shape != shape or st[2] != 1 or t.get_device() != self._dev:
                 self._refuse_rows(t, n, T)
+        if T == 1:                                       # one token's stride can be any number, as 1 of a transposed column
+            sk, sv = (0, sk[1]), (0, sv[1])
         dtype = key.dtype
         dt = _DT.get(dtype)
         if dt not in (1, 2) or value.dtype != dtype or (self.k_scale is None and dtype != self.dtype):
