@@ -20,17 +20,17 @@
 //   e4m3: 8 rows, and in each quarter 8 lanes for each of four pieces of the query (piece_of), so that one product
 //   forms all their scores; the weights are cut into pieces in the same lanes and meet the values' codes as they
 //   are. (48 decodes
-//   of up to 8192 positions, the same heads: 128 us. Over 128-row tiles, with V widened: 250; with the weights
+//   of up to 8192 positions, the same heads: 126 us. Over 128-row tiles, with V widened: 250; with the weights
 //   in pieces: 170.)
 // Over 128-row tiles the value codes are widened to 16 bits (exactly) on their way and meet 16-bit weights:
 // there pieces of the weights would keep the conversion unit (a warp instruction in 16 cycles) busy (five
-// prompts of up to 1500 tokens, 32 heads on 8 of 128: 440 us against 248), and keys widened too would spend shared
-// memory's bandwidth.
+// prompts of up to 1500 tokens, 32 heads on 8 of 128: 440 us against 248, 253 since), and keys widened too would
+// spend shared memory's bandwidth.
 //
 // What bounds it: over long prompts the tensor work (a prompt's chunk of 2048 tokens on 16384, 16 heads on 4 of
-// 256: 431 us, 1190 TFLOP/s; a 64-position product is issue-bound, 45 cycles for 32 of work, and D = 256 leaves
-// tensor memory no room for wider ones); over short pieces and decodes what a piece costs besides its units (about
-// 8 units' time) and instruction issue.
+// 256: 429 us in a short run, 1200 TFLOP/s, 495 to 500 us and 1040 under the power cap; a 64-position product is
+// issue-bound, 45 cycles for 32 of work, and D = 256 leaves tensor memory no room for wider ones); over short pieces
+// and decodes what a piece costs besides its units (about 8 units' time) and a unit's chain of dependent steps.
 #include <cuda_runtime.h>
 #include <cuda_fp8.h>
 #include <algorithm>

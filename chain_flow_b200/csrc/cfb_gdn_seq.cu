@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(kStepThreads) gdn_walk_kernel(const cfb_gdn_ar
 // registers in the accumulator layout, which, with the summed index permuted (2t, 2t + 1 for t, t + 4;
 // the other operand is read as pairs of neighbours anyway), is the first operand's layout too: S feeds
 // S k, that feeds T, U feeds the update, without a trip through shared or tensor memory and with one
-// exchange between the two warps of a tile. Measured, 32 value heads of 128: 8191 tokens of one request 520 us
-// (scan 462, prep 58), nine prompts of up to 1500 tokens 480; a chunk 1.8 us, in which each quarter of the SM
+// exchange between the two warps of a tile. Measured, 32 value heads of 128: 8191 tokens of one request 515 us
+// (scan 457, prep 58), nine prompts of up to 1500 tokens 480; a chunk 1.8 us, in which each quarter of the SM
 // issues 1660 instructions and 165 products of 8.4 cycles in 3300 cycles: no pipe is full, the chain of dependent
 // steps of one state warp a quarter is the time. (Four warps a tile, a quarter of the columns each, repeat
 // U's product twice as often: 700 us. Two CTAs an SM leave 96 registers a thread: 1070.)
