@@ -507,13 +507,18 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
     dead = 0;
   }
   __syncthreads();
-  // A wait that outlasts its limit marks the CTA dead: from then on nothing waits, the chunks run through
-  // to the end on whatever is there (so that the barriers between warps still meet), and the state is set
-  // to NaN.
+  // A wait that outlasts its limit marks the CTA dead: from then on nothing waits for copies, the chunks run through
+  // to the end on whatever is there, and the state is set to NaN. What a tile's warps wait for from one another they
+  // wait for all the same: the state warps, a hand-over buffer ahead, would else arrive at a barrier twice where
+  // the output warps have not been once, and those would then stay there for good. (Such a wait is for warps that get
+  // on: they wait for copies, 1 s at most and once, and for these warps. Its own limit is well above that.)
   volatile int* const is_dead = &dead;
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_test_wait(bar, parity)) return;
     if (*is_dead == 0 && !mbar_wait(bar, parity)) *is_dead = 1;
+  };
+  const auto wait_freed = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_test_wait(bar, parity) && !mbar_wait(bar, parity, nullptr, 8 * kWaitBudgetNs)) *is_dead = 1;
   };
   // barriers of a tile: the state warps' exchange; S and U handed over (freed: a hand-over buffer free again)
   const int tile = (warp % kStateWarps) / 2;
@@ -651,7 +656,7 @@ gdn_scan_kernel(const cfb_gdn_args g, const int32_t* cu, int total, int B, const
   }
   for (int c = 0; c < chunks; ++c) {
     uint8_t* const hand = hand_at(c);
-    if (c >= 2) wait(&freed[tile][c & 1], ((c >> 1) - 1) & 1);
+    if (c >= 2) wait_freed(&freed[tile][c & 1], ((c >> 1) - 1) & 1);
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
       reinterpret_cast<float4*>(hand)[(ks * NJ + j) * 32 + lane] = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
