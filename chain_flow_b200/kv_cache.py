@@ -38,7 +38,8 @@ class PagedKVCache:
     @classmethod
     def from_tensors(cls, k, v, k_scale=None, v_scale=None) -> "PagedKVCache":
         """A cache over existing buffers [pages, kv_heads, page_size, head_dim] (permuted views of
-        another layout are fine; k and v share strides, and so do their scales)."""
+        another layout are fine; k and v share strides, and so do their scales). Scales are not negative; a row of
+        scale 0 stands for zeros."""
         self = cls.__new__(cls)
         self._bind(k, v, k_scale, v_scale)
         return self
