@@ -183,25 +183,25 @@ def _refuse_sequence(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, o
                         "and out_state must be fp32 with contiguous slots and one slot stride")
 
 
-def _heads_strides(t):
-    """The token stride of a [T, heads, dim] tensor with contiguous heads, else None. (One token's can be any
-    number, as 1 of a transposed column: what the heads take stands for it.)"""
-    st = t.stride()
-    if st[2] != 1 or (st[1] != t.shape[2] and t.shape[1] != 1):
+def _token_stride(st, T, heads, dim):
+    """The token stride of a [T, heads, dim] tensor of strides ``st`` with contiguous heads, else None. (One token's
+    can be any number, as 1 of a transposed column: what the heads take stands for it.)"""
+    if st[2] != 1 or (st[1] != dim and heads != 1):
         return None
-    return st[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return st[0] if T > 1 else heads * dim
 
 
 def _sequence_args(what, A_log, dt_bias, a, b, q, k, v, o, state, init_slot, out_slot, scale, out_state, B):
     """(the packed cfb_gdn_args, the converted index tensors, which the caller keeps until the launch)."""
     out_state = state if out_state is None else out_state
     qs, vs, ss, dev, dt = q.shape, v.shape, state.shape, q.get_device(), q.dtype
-    good = len(qs) == 3 and len(vs) == 3 and len(ss) == 4 and dev >= 0 and dt in _HALVES
+    good = len(qs) == 3 and len(vs) == 3 and len(ss) == 4 and dev >= 0 and dt in _HALVES and k.dim() == 3 and o.dim() == 3
     if good:
         T, H, K = qs
         HV, V = vs[1], vs[2]
         gates = (T, HV)
-        sq, sk, sv, so = _heads_strides(q), _heads_strides(k), _heads_strides(v), _heads_strides(o)
+        sq, sk = _token_stride(q.stride(), T, H, K), _token_stride(k.stride(), T, H, K)
+        sv, so = _token_stride(v.stride(), T, HV, V), _token_stride(o.stride(), T, HV, V)
         sa, sb, s_in, s_out = a.stride(), b.stride(), state.stride(), out_state.stride()
         c_A, c_d, c_a, c_b = (_DTYPE_CODE.get(t.dtype) for t in (A_log, dt_bias, a, b))
         good = (k.shape == qs and vs[0] == T and o.shape == vs and a.shape == gates and b.shape == gates

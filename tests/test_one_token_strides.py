@@ -52,3 +52,13 @@ def test_gated_delta_rule(step):
     d["o"] = _column(torch.zeros(d["v"].shape, device="cuda", dtype=torch.bfloat16))
     cases._run(d, step=step)
     cases._check(d["o"], d["state"], c, cases._oracle(c))
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_rows_without_a_heads_dim_are_refused(step):
+    from chain_flow_b200 import _lib
+    cases = _cases("test_gdn_seq")
+    d = cases._gpu(cases._case([1, 1], 2, 4, 64, torch.float16, seed=7))
+    for n in ("q", "k", "v", "o"):
+        with pytest.raises(_lib.CfbError):
+            cases._run({**d, n: d[n].flatten(1)}, step=step)
