@@ -267,7 +267,7 @@ def prepare(case, seed):
         from chain_flow_b200.kv_cache import PagedKVCache, PagePool
         from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
         if case["op"] == "sample":
-            s["verifier"] = SampledVerifier(len(s["logits"]), case["requests"], s["nodes"], case["vocab"])
+            s["verifier"] = SampledVerifier(len(s["logits"]), case["requests"], s["nodes"])
         elif case["op"] == "reject":
             s["verifier"] = RejectionVerifier(len(s["logits"]), case["requests"], case["drafts"], case["vocab"], draft_ids=s["ids"])
         if "layers" in s:
