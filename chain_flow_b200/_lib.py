@@ -34,6 +34,8 @@ EXPORTED = [
     "cfb_vae_plan_workspace", "cfb_vae_plan_build", "cfb_tree_attn_merge", "cfb_tree_verify_workspace",
     "cfb_tree_verify_greedy", "cfb_tree_gdn_factor", "cfb_kv_write", "cfb_kv_read", "cfb_paged_attn_workspace",
     "cfb_paged_attn", "cfb_paged_attn_error", "cfb_gdn_step", "cfb_gdn_chunk_workspace", "cfb_gdn_chunk", "cfb_gdn_chunk_error",
+    "cfb_verify_workspace", "cfb_tree_verify_sampled", "cfb_chain_verify_rejection", "cfb_kv_keep", "cfb_kv_copy_pages",
+    "cfb_pages_reserve", "cfb_pages_release", "cfb_pages_fork",
 ]
 ABI_VERSION = 5
 XROWS, XFLOATS = 64, 18          # CFB_XROWS, CFB_XFLOATS: the merged-list exchange rows
@@ -170,6 +172,17 @@ def _declare(lib):
     lib.cfb_tree_verify_workspace.restype = sz
     lib.cfb_tree_verify_greedy.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp,
                                            sz, vp, vp]
+    lib.cfb_verify_workspace.argtypes = [i32, i32]
+    lib.cfb_verify_workspace.restype = sz
+    lib.cfb_tree_verify_sampled.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp,
+                                            vp, sz, vp, vp]
+    lib.cfb_chain_verify_rejection.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, i64, i32, i32, vp, vp, vp, i32, vp, i32,
+                                               i32, vp, vp, vp, vp, sz, vp, vp]
+    lib.cfb_kv_keep.argtypes = [vp, i32, vp, i64, i32, vp, vp, i64, vp, i32, i32, vp]
+    lib.cfb_kv_copy_pages.argtypes = [vp, i32, vp, vp, vp, i32, vp]
+    lib.cfb_pages_reserve.argtypes = [vp, i32, i32, vp, i64, i32, vp, vp, vp, i32, vp]
+    lib.cfb_pages_release.argtypes = [vp, i32, i32, vp, i64, i32, vp, vp, i32, vp, vp]
+    lib.cfb_pages_fork.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, vp, vp, vp, i32, vp, i32, vp]
     lib.cfb_kv_write.argtypes = [C.POINTER(KvCache), vp, i64, i64, vp, i64, i64, i32, vp, i32, vp]
     lib.cfb_kv_read.argtypes = [C.POINTER(KvCache), vp, i32, vp, i64, i64, vp, i64, i64, i32, vp]
     lib.cfb_paged_attn_workspace.argtypes = [i32, i32, i32]

@@ -1,6 +1,8 @@
 """The paged key/value cache of a target's full-attention layer, on the sm_100a kernels of
-libcfb.so (cfb_kv.cu): rows are written to slots of pages, quantised as they are written where the
-cache holds e4m3, and read back. ``attention.PagedAttention`` attends over it."""
+libcfb.so (cfb_kv.cu, cfb_pages.cu): rows are written to slots of pages, quantised as they are written
+where the cache holds e4m3, and read back. ``attention.PagedAttention`` attends over it. Over the caches of
+all layers at once, ``keep_path`` moves a step's accepted rows together and ``copy_pages`` copies pages;
+``PagePool`` counts who holds a page: it hands pages out, takes them back and forks a request's."""
 from __future__ import annotations
 
 import ctypes as C
@@ -131,3 +133,177 @@ class PagedKVCache:
         _lib.check(self.lib.cfb_kv_read(self.desc, slots.data_ptr(), T, key.data_ptr(), self.kv_heads * D, D, value.data_ptr(),
                                         self.kv_heads * D, D, _DT[dtype], _lib.stream_of(self._dev, "PagedKVCache.read")), "cfb_kv_read")
         return key, value
+
+
+def _layers(caches, what: str, device=None):
+    """(descriptor array, number, device number) of one cache or a sequence of caches of one geometry."""
+    if isinstance(caches, PagedKVCache):
+        caches = (caches,)
+    dev = caches[0]._dev if len(caches) else device
+    if any(c._dev != dev for c in caches):
+        raise _lib.CfbError(f"{what}: the caches are on several devices")
+    if device is not None and dev != device:
+        raise _lib.CfbError(f"{what}: the caches are on cuda:{dev}, the pages on cuda:{device}")
+    return (C.c_void_p * len(caches))(*[C.addressof(c._desc) for c in caches]), len(caches), dev
+
+
+def _check_layers(caches, what: str) -> None:
+    caches = (caches,) if isinstance(caches, PagedKVCache) else caches
+    first = caches[0]
+    for c in caches[1:]:
+        if (c.k.shape != first.k.shape or c.dtype != first.dtype or c.k.stride() != first.k.stride()
+                or (c.k_scale is not None and c.k_scale.stride() != first.k_scale.stride())):
+            raise _lib.CfbError(f"{what}: the caches differ in shape, dtype or strides")
+
+
+def _index(t, name: str, what: str, dev: int, shape):
+    """t, an integer tensor of `shape` on device dev, as contiguous int32."""
+    if t.get_device() != dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != tuple(shape):
+        _lib.require_cuda(t, name)
+        raise _lib.CfbError(f"{what}: {name} must be integers {list(shape)} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return _lib.int32(t)
+
+
+def keep_path(caches, page_table, base, path, length, stream=None) -> None:
+    """A step's accepted rows moved together, in the caches of all layers (one PagedKVCache or a sequence of one geometry).
+    Request b's tree was written to the positions ``base[b] + node``; its rows ``base[b] + path[b, j]``, j < length[b], go
+    to ``base[b] + j``. ``path`` [B, S] and ``length`` [B] are a verifier's accepted_path and accepted_len (increasing
+    nodes; S <= 1024), page_table [B, width]: integer tensors on the GPU, nothing is read back. Nodes below 0 and
+    positions outside the table or the pool are left out. What lies behind the kept rows is stale: the context ends at
+    ``base + length``."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return keep_path(caches, page_table, base, path, length)
+    desc, n, dev = _layers(caches, "keep_path")
+    if n == 0:
+        return
+    if page_table.dim() != 2 or path.dim() != 2:
+        raise _lib.CfbError("keep_path: page_table [B, width] and path [B, S] must be matrices")
+    (B, width), S = page_table.shape, path.shape[1]
+    page_table = _index(page_table, "page_table", "keep_path", dev, (B, width))
+    base, path = _index(base, "base", "keep_path", dev, (B,)), _index(path, "path", "keep_path", dev, (B, S))
+    length = _index(length, "length", "keep_path", dev, (B,))
+    status = _lib.load().cfb_kv_keep(desc, n, page_table.data_ptr(), width, width, base.data_ptr(), path.data_ptr(), S,
+                                     length.data_ptr(), S, B, _lib.stream_of(dev, "keep_path"))
+    if status:
+        _check_layers(caches, "keep_path")
+        _lib.check(status, "cfb_kv_keep")
+
+
+def copy_pages(caches, src, dst, slots=None, stream=None) -> None:
+    """Pages src [n] of every cache (one PagedKVCache or a sequence of one geometry) copied to pages dst [n]; with ``slots``
+    [n], the first slots[i] slots of them. Pairs with a page outside the pool are left out. The dst of a call are
+    distinct, and none of them is a src."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return copy_pages(caches, src, dst, slots)
+    desc, n, dev = _layers(caches, "copy_pages")
+    if n == 0:
+        return
+    pairs = src.shape[0] if src.dim() == 1 else -1
+    src, dst = _index(src, "src", "copy_pages", dev, (pairs,)), _index(dst, "dst", "copy_pages", dev, (pairs,))
+    slots = None if slots is None else _index(slots, "slots", "copy_pages", dev, (pairs,))
+    status = _lib.load().cfb_kv_copy_pages(desc, n, src.data_ptr(), dst.data_ptr(), None if slots is None else slots.data_ptr(),
+                                           pairs, _lib.stream_of(dev, "copy_pages"))
+    if status:
+        _check_layers(caches, "copy_pages")
+        _lib.check(status, "cfb_kv_copy_pages")
+
+
+class PagePool:
+    """Who holds the pages of a target's caches: ``refs`` int32 [pages] counts the requests that hold a page (0: free).
+    Requests' pages are rows of a page table (int32 [rows, width], as PagedAttention takes it; changed in place), in order
+    of their positions. Every call is a launch or two on the current stream (or ``stream=``) and reads nothing back;
+    calls on a pool are ordered on one stream. Pages handed out are always the lowest free ones, request after request.
+    ``err`` int32 [1] becomes non-zero when a page is given back that nobody holds."""
+
+    def __init__(self, pages: int, page_size: int, device=None):
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if pages <= 0:
+            raise _lib.CfbError("PagePool: pages must be positive")
+        self._bind(torch.zeros(pages, dtype=torch.int32, device=dev), page_size)
+
+    @classmethod
+    def from_refs(cls, refs, page_size: int) -> "PagePool":
+        """A pool over existing counts (int32 [pages], contiguous, on the GPU)."""
+        self = cls.__new__(cls)
+        self._bind(refs, page_size)
+        return self
+
+    def _bind(self, refs, page_size: int) -> None:
+        _lib.require_cuda(refs, "refs")
+        if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous() or not 0 < refs.shape[0] <= 1 << 20:
+            raise _lib.CfbError("PagePool: refs must be contiguous int32 [pages], 1 to 2^20 pages")
+        if page_size <= 0:
+            raise _lib.CfbError("PagePool: page_size must be positive")
+        self.lib = _lib.load()
+        self.refs, self.page_size, self.pages, self._dev = refs, page_size, refs.shape[0], refs.get_device()
+        self.err = torch.zeros(1, dtype=torch.int32, device=refs.device)
+
+    def _table(self, table, what: str):
+        """(address, row stride, width, rows) of a table that is changed in place."""
+        if (table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != self._dev
+                or (table.shape[1] > 1 and table.stride(1) != 1) or (table.shape[0] > 1 and table.stride(0) < table.shape[1])):
+            _lib.require_cuda(table, "table")
+            raise _lib.CfbError(f"{what}: table must be int32 [rows, width] on the pool's device, its rows contiguous and apart")
+        rows, width = table.shape
+        return table.data_ptr(), max(table.stride(0), width), width, rows
+
+    def reserve(self, table, length, target, stream=None):
+        """Pages for the positions [length[b], target[b]) that request b's pages do not cover yet, into its row. Returns
+        granted int32 [B]: 0 where the pool ran out (that request and all later ones that ask get nothing) or a row is too
+        short."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.reserve(table, length, target)
+        at, stride, width, B = self._table(table, "PagePool.reserve")
+        length = _index(length, "length", "PagePool.reserve", self._dev, (B,))
+        target = _index(target, "target", "PagePool.reserve", self._dev, (B,))
+        granted = torch.empty(B, dtype=torch.int32, device=self.refs.device)
+        _lib.check(self.lib.cfb_pages_reserve(self.refs.data_ptr(), self.pages, self.page_size, at, stride, width,
+                                              length.data_ptr(), target.data_ptr(), granted.data_ptr(), B,
+                                              _lib.stream_of(self._dev, "PagePool.reserve")), "cfb_pages_reserve")
+        return granted
+
+    def release(self, table, length, keep=None, stream=None) -> None:
+        """Gives back the pages of request b's positions past keep[b] (all of them without ``keep``) up to length[b]; their
+        entries become -1. A page that others hold stays theirs."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.release(table, length, keep)
+        at, stride, width, B = self._table(table, "PagePool.release")
+        length = _index(length, "length", "PagePool.release", self._dev, (B,))
+        keep = None if keep is None else _index(keep, "keep", "PagePool.release", self._dev, (B,))
+        _lib.check(self.lib.cfb_pages_release(self.refs.data_ptr(), self.pages, self.page_size, at, stride, width,
+                                              length.data_ptr(), None if keep is None else keep.data_ptr(), B,
+                                              self.err.data_ptr(), _lib.stream_of(self._dev, "PagePool.release")),
+                   "cfb_pages_release")
+
+    def fork(self, table, length, parent, child, caches=(), stream=None):
+        """Rows child [n] of the table become copies of rows parent [n]: full pages are shared, the slots of a last page
+        that is not full are copied to a page of the child's own in every cache (one PagedKVCache or a sequence of one
+        geometry, with this pool's pages). ``length`` int32 [rows], contiguous, is changed in place: length[child] =
+        length[parent]. Returns granted int32 [n]: 0 where the pool ran out (that fork and all later ones that need a
+        page) or a row is none of the table's. The children are distinct, hold no pages, and none is a parent."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.fork(table, length, parent, child, caches)
+        at, stride, width, rows = self._table(table, "PagePool.fork")
+        if length.shape != (rows,) or length.dtype != torch.int32 or not length.is_contiguous() or length.get_device() != self._dev:
+            _lib.require_cuda(length, "length")
+            raise _lib.CfbError(f"PagePool.fork: length must be contiguous int32 [{rows}] on the pool's device")
+        n = parent.shape[0] if parent.dim() == 1 else -1
+        parent = _index(parent, "parent", "PagePool.fork", self._dev, (n,))
+        child = _index(child, "child", "PagePool.fork", self._dev, (n,))
+        desc, layers, _ = _layers(caches, "PagePool.fork", self._dev)
+        granted = torch.empty(n, dtype=torch.int32, device=self.refs.device)
+        status = self.lib.cfb_pages_fork(self.refs.data_ptr(), self.pages, self.page_size, at, stride, width, rows,
+                                         length.data_ptr(), parent.data_ptr(), child.data_ptr(), granted.data_ptr(), n, desc,
+                                         layers, _lib.stream_of(self._dev, "PagePool.fork"))
+        if status and layers:
+            _check_layers(caches, "PagePool.fork")
+            first = caches if isinstance(caches, PagedKVCache) else caches[0]
+            if first.page_size != self.page_size or first.pages < self.pages:
+                raise _lib.CfbError("PagePool.fork: the caches have other pages than the pool")
+        _lib.check(status, "cfb_pages_fork")
+        return granted

@@ -4,6 +4,11 @@ kernels of libcfb.so (cfb_tree.cu).
 * ``tree_attn_merge``: the tree-attention fix-up of one full-attention layer (the reference fork's
   ``suffix_merge``, src/chain_flow/patches/vllm-0.25.1-chain-flow-tree.patch:5516-5537; eager form
   ``_tree_suffix_eager`` :529-575 + vLLM's ``merge_attn_states``).
+* ``TreeVerifier``: greedy verification of draft trees.
+* ``SampledVerifier``, ``RejectionVerifier`` (cfb_verify.cu): drafts verified against the target's
+  probabilities at a temperature, from given random numbers; trees (and chains) without draft
+  probabilities, chains with them. The reference's fork leaves requests above temperature 0 to the
+  engine's own sampler (src/chain_flow/vllm_plugin/tree_sampling.py).
 """
 from __future__ import annotations
 
@@ -102,3 +107,152 @@ class TreeVerifier:
             self.accepted_len.data_ptr(), self.row_argmax.data_ptr(), C.c_void_p(self.ws_ptr), self.ws_bytes,
             self.err.data_ptr(), C.c_void_p(_lib.stream_ptr(stream))), "cfb_tree_verify_greedy")
         return self.out_tokens[:B], self.accepted_path[:B], self.accepted_len[:B]
+
+
+class _ProbabilityVerifier:
+    """What SampledVerifier and RejectionVerifier share: their buffers, allocated once for up to ``max_rows`` logits rows
+    and ``max_batch`` requests and reused, so a call allocates nothing (CUDA-graph capturable) and calls of one verifier
+    are ordered on one stream. ``err`` int32 [1] becomes non-zero when a request's offsets do not fit its rows."""
+
+    def __init__(self, max_rows: int, max_batch: int, max_spec_len: int, device=None):
+        self.lib = _lib.load()
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if max_rows <= 0 or max_batch <= 0 or not 0 <= max_spec_len <= 1024:
+            raise _lib.CfbError(f"{type(self).__name__}: max_rows and max_batch must be positive, max_spec_len 0 to 1024")
+        self.max_rows, self.max_batch, self.max_spec = max_rows, max_batch, max_spec_len
+        self.ws_bytes = int(self.lib.cfb_verify_workspace(max_rows, max_batch))
+        self.ws = torch.zeros(self.ws_bytes + 256, dtype=torch.uint8, device=dev)
+        self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+        self._dev = self.ws.get_device()
+        self.out_tokens = torch.empty(max_batch, max_spec_len + 1, dtype=torch.int32, device=dev)
+        self.accepted_len = torch.empty(max_batch, dtype=torch.int32, device=dev)
+        self.logprobs = torch.empty(max_batch, max_spec_len + 1, dtype=torch.float32, device=dev)
+        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def _refuse(self, what, wrong):
+        raise _lib.CfbError(f"{type(self).__name__}: {what} {wrong}")
+
+    def _ints(self, t, name, shape):
+        if t.get_device() != self._dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != shape:
+            _lib.require_cuda(t, name)
+            self._refuse(name, f"must be integers {list(shape)} on cuda:{self._dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+        return _lib.int32(t)
+
+    def _numbers(self, t, name, n):
+        if t.get_device() != self._dev or t.dtype not in (torch.float32, torch.float64) or t.shape != (n,):
+            _lib.require_cuda(t, name)
+            self._refuse(name, f"must be fp32 or fp64 [{n}] on cuda:{self._dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+        return t.contiguous()
+
+    def _common(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, temperature):
+        """The checked arguments that both verifiers take: (logits' dtype code, row stride, B, ...)."""
+        dt = _LOGITS.get(logits.dtype)
+        if logits.get_device() != self._dev or dt is None or logits.dim() != 2 or logits.shape[1] == 0 or (
+                logits.stride(1) != 1 and logits.shape[1] > 1):
+            _lib.require_cuda(logits, "logits")
+            self._refuse("logits", f"must be fp32, fp16 or bf16 rows with a contiguous vocabulary dim on cuda:{self._dev}")
+        rows, V = logits.shape
+        B = cu_num_draft.shape[0] if cu_num_draft.dim() == 1 else -1
+        if rows > self.max_rows or B > self.max_batch:
+            self._refuse(f"{rows} rows / {B} requests", f"exceed this verifier ({self.max_rows} / {self.max_batch})")
+        ld = logits.stride(0) if rows > 1 else V
+        if ld < V:
+            self._refuse("logits", "has rows that share words")
+        cu_d, cu_s = self._ints(cu_num_draft, "cu_num_draft", (B,)), self._ints(cu_num_sampled, "cu_num_sampled", (B,))
+        tokens = self._ints(draft_tokens, "draft_tokens", (draft_tokens.numel(),))
+        if temperature is not None:
+            if temperature.get_device() != self._dev or not temperature.is_floating_point() or temperature.shape != (B,):
+                _lib.require_cuda(temperature, "temperature")
+                self._refuse("temperature", f"must be floating-point [{B}] on cuda:{self._dev}")
+            temperature = temperature.to(torch.float32).contiguous()
+        return dt, ld, rows, V, B, cu_d, cu_s, tokens, temperature
+
+
+_LOGITS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class SampledVerifier(_ProbabilityVerifier):
+    """Verification of draft trees (a chain is a tree) at a temperature, on cfb_tree_verify_sampled. Every row draws a
+    token from the target's softmax(logits / temperature) with its given number; from the root, a request's walk moves to
+    the first child that carries the row's token and ends where none does, with that token as the bonus. The output is
+    distributed as the target's own. Requests of temperature 0 take the argmax, as TreeVerifier."""
+
+    def __init__(self, max_rows: int, max_batch: int, max_spec_len: int, device=None):
+        super().__init__(max_rows, max_batch, max_spec_len, device)
+        self.accepted_path = torch.empty(max_batch, max_spec_len, dtype=torch.int32, device=self.ws.device)
+
+    def __call__(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, parents, uniforms, temperature=None, stream=None):
+        """(output_tokens [B, max_spec + 1], accepted_path [B, max_spec], accepted_len [B]) int32 and logprobs fp32
+        [B, max_spec + 1], views of this verifier's buffers, -1 (logprobs 0) after a request's tokens. logits, offsets,
+        draft_tokens and parents as TreeVerifier takes them; uniforms fp32 or fp64 [rows] in [0, 1), one number a logits
+        row; temperature [B] (None: 1 for all; 0: greedy). logprobs are the output tokens' log probabilities under
+        softmax(logits / temperature) (greedy requests: softmax(logits)). A token of logit -inf is never drawn; a row
+        of nothing else ends its walk with token -1."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self(logits, cu_num_draft, cu_num_sampled, draft_tokens, parents, uniforms, temperature)
+        dt, ld, rows, V, B, cu_d, cu_s, tokens, temp = self._common(logits, cu_num_draft, cu_num_sampled, draft_tokens, temperature)
+        par, u = self._ints(parents, "parents", tuple(tokens.shape)), self._numbers(uniforms, "uniforms", rows)
+        if B and rows:
+            _lib.check(self.lib.cfb_tree_verify_sampled(
+                logits.data_ptr(), ld, rows, V, dt, cu_d.data_ptr(), cu_s.data_ptr(), tokens.data_ptr(), par.data_ptr(),
+                tokens.shape[0], u.data_ptr(), u.element_size(), None if temp is None else temp.data_ptr(), B, self.max_spec,
+                self.out_tokens.data_ptr(), self.accepted_path.data_ptr(), self.accepted_len.data_ptr(), self.logprobs.data_ptr(),
+                self.ws_ptr, self.ws_bytes, self.err.data_ptr(), _lib.stream_of(self._dev, "SampledVerifier")),
+                "cfb_tree_verify_sampled")
+        elif B:
+            self._refuse("logits", "has no rows")
+        return self.out_tokens[:B], self.accepted_path[:B], self.accepted_len[:B], self.logprobs[:B]
+
+
+class RejectionVerifier(_ProbabilityVerifier):
+    """Verification of drafted chains whose draft model gave probabilities, on cfb_chain_verify_rejection. A draft stays if
+    u q < p (its draft and target probability); the first that does not is replaced by a draw from max(p - q, 0), and a
+    chain that stays whole is followed by a draw from its last row. The output is distributed as the target's own.
+
+    ``draft_ids`` [R] (distinct, as a shortlist file's ids): the tokens that the columns of draft_probs stand for; all
+    other tokens have draft probability 0. None: the columns are the vocabulary."""
+
+    def __init__(self, max_rows: int, max_batch: int, max_spec_len: int, vocab_size: int, draft_ids=None, device=None):
+        super().__init__(max_rows, max_batch, max_spec_len, device)
+        self.vocab, self.width, self.index_of = vocab_size, vocab_size, None
+        if draft_ids is not None:
+            ids = draft_ids.to(device=self.ws.device, dtype=torch.int64)
+            if ids.dim() != 1 or ids.numel() == 0 or int(ids.min()) < 0 or int(ids.max()) >= vocab_size or ids.unique().numel() != ids.numel():
+                self._refuse("draft_ids", f"must be distinct token ids [R] below {vocab_size}")
+            self.width = ids.numel()
+            self.index_of = torch.full((vocab_size,), -1, dtype=torch.int32, device=self.ws.device)
+            self.index_of[ids] = torch.arange(self.width, dtype=torch.int32, device=self.ws.device)
+
+    def __call__(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, draft_probs, uniforms, resample, temperature=None,
+                 stream=None):
+        """(output_tokens [B, max_spec + 1], accepted_len [B]) int32 and logprobs fp32 [B, max_spec + 1], as
+        SampledVerifier's. Request b's drafts are the flat rows [cu_num_draft[b - 1], cu_num_draft[b]) of draft_tokens and
+        of draft_probs fp32 [drafts, R] (contiguous rows; what is not a positive number counts as 0); uniforms [drafts]
+        accept them, resample [B] draws, each fp32 or fp64 in [0, 1). A greedy request (temperature 0) keeps the drafts
+        that are its rows' argmax."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self(logits, cu_num_draft, cu_num_sampled, draft_tokens, draft_probs, uniforms, resample, temperature)
+        dt, ld, rows, V, B, cu_d, cu_s, tokens, temp = self._common(logits, cu_num_draft, cu_num_sampled, draft_tokens, temperature)
+        n = tokens.shape[0]
+        if V != self.vocab:
+            self._refuse("logits", f"has {V} columns, this verifier's vocabulary {self.vocab}")
+        if (draft_probs.get_device() != self._dev or draft_probs.dtype != torch.float32 or draft_probs.shape != (n, self.width)
+                or (draft_probs.stride(1) != 1 and self.width > 1) or (n > 1 and draft_probs.stride(0) < self.width)):
+            _lib.require_cuda(draft_probs, "draft_probs")
+            self._refuse("draft_probs", f"must be fp32 [{n}, {self.width}] with contiguous rows on cuda:{self._dev}")
+        u, v = self._numbers(uniforms, "uniforms", n), self._numbers(resample, "resample", B)
+        if u.dtype != v.dtype:
+            u, v = u.double(), v.double()
+        if B and rows:
+            _lib.check(self.lib.cfb_chain_verify_rejection(
+                logits.data_ptr(), ld, rows, V, dt, cu_d.data_ptr(), cu_s.data_ptr(), tokens.data_ptr(), draft_probs.data_ptr(),
+                draft_probs.stride(0) if n > 1 else self.width, n, self.width,
+                None if self.index_of is None else self.index_of.data_ptr(), u.data_ptr(), v.data_ptr(), v.element_size(),
+                None if temp is None else temp.data_ptr(), B, self.max_spec, self.out_tokens.data_ptr(),
+                self.accepted_len.data_ptr(), self.logprobs.data_ptr(), self.ws_ptr, self.ws_bytes, self.err.data_ptr(),
+                _lib.stream_of(self._dev, "RejectionVerifier")), "cfb_chain_verify_rejection")
+        elif B:
+            self._refuse("logits", "has no rows")
+        return self.out_tokens[:B], self.accepted_len[:B], self.logprobs[:B]

@@ -384,6 +384,48 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
                                   int32_t* accepted_len, int32_t* row_argmax, void* ws,
                                   size_t ws_bytes, int* err, void* stream);
 
+/* Verification of drafted tokens against the target's probabilities, from given random numbers. Rows,
+ * offsets, draft_tokens and parents as cfb_tree_verify_greedy; num_drafts: entries of draft_tokens.
+ * With the weights w_i = exp((l_i - max l) / tau) of a logits row l, tau = temperature[r] of its request
+ * (NULL: 1), a number u in [0, 1) draws the first token i with w_0 + .. + w_i > u (w_0 + .. + w_V-1).
+ * -inf weighs nothing; several +inf share the mass; a row that is all -inf has no token: -1, and the
+ * walk ends. Below 2^-126 (0), or NaN, a temperature makes its request greedy: the largest logit, the
+ * first of equals; so does a NaN in a row (the first NaN). Above 2^100 it counts as 2^100. Random
+ * numbers are fp32 or fp64 (uniform_size 4 or 8), taken into [0, 1 - 2^-32] (NaN: 0). Decisions are those
+ * of 64-bit arithmetic.
+ * cfb_tree_verify_sampled: no draft probabilities. Row j draws a token with uniforms[j] (one for each
+ * of num_rows); the walk moves to the first child that carries it, as the greedy one does. The output
+ * is distributed as the target's own, whatever the tree.
+ * cfb_chain_verify_rejection: each request's drafts are a chain, draft i (flat) was drawn from the
+ * probabilities q = draft_probs[i] (fp32 rows of probs_width, row stride ld_probs) over the whole
+ * vocabulary (index_of NULL, probs_width V) or over columns: token x has column index_of[x] < probs_width,
+ * or -1: probability 0 (what is not a positive number counts as 0). With p the row's probabilities, draft
+ * token d stays if uniforms[i] q_d < p_d (uniforms: one for each draft); the first that does not is
+ * replaced by a draw of resample[r] from max(p - q, 0), or p where that is nowhere positive; if all
+ * stay, resample[r] draws the bonus token from the last row. A greedy row keeps d if it is the
+ * argmax. A draft outside the vocabulary is refused.
+ * Outputs as cfb_tree_verify_greedy, and logprobs fp32 [batch, max_spec_len + 1]: the output tokens' log
+ * probabilities under w (of a greedy request: tau = 1), 0 after them.
+ * logits: element-aligned, any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
+ * ZERO before its first use (each launch leaves it so that the next may follow), for calls ordered on
+ * one stream. err as there. Supported: max_spec_len <= 1024, V <= 2^22 - 8, batch <= 65535. */
+size_t cfb_verify_workspace(int num_rows, int batch);
+cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, int num_rows, int V, int dtype,
+                                   const int32_t* cu_num_draft, const int32_t* cu_num_sampled,
+                                   const int32_t* draft_tokens, const int32_t* parents, int num_drafts,
+                                   const void* uniforms, int uniform_size, const float* temperature,
+                                   int batch, int max_spec_len, int32_t* output_tokens,
+                                   int32_t* accepted_path, int32_t* accepted_len, float* logprobs,
+                                   void* ws, size_t ws_bytes, int* err, void* stream);
+cfb_status cfb_chain_verify_rejection(const void* logits, int64_t ld, int num_rows, int V, int dtype,
+                                      const int32_t* cu_num_draft, const int32_t* cu_num_sampled,
+                                      const int32_t* draft_tokens, const float* draft_probs,
+                                      int64_t ld_probs, int num_drafts, int probs_width,
+                                      const int32_t* index_of, const void* uniforms, const void* resample,
+                                      int uniform_size, const float* temperature, int batch,
+                                      int max_spec_len, int32_t* output_tokens, int32_t* accepted_len,
+                                      float* logprobs, void* ws, size_t ws_bytes, int* err, void* stream);
+
 /* ---- the target model's side of a step: paged cache, attention over it, gated delta rule --------
  * The key/value cache of one full-attention layer: rows of `dim` elements in pages of page_size
  * slots, kept as fp16 (dtype 1), bf16 (2) or e4m3 (3). Row (slot, kv head h) of a flat slot =
@@ -418,6 +460,45 @@ cfb_status cfb_kv_write(const cfb_kv_cache* c, const void* key, int64_t sk_t, in
                         const int64_t* slots, int T, void* stream);
 cfb_status cfb_kv_read(const cfb_kv_cache* c, const int64_t* slots, int T, void* key, int64_t sk_t,
                        int64_t sk_h, void* value, int64_t sv_t, int64_t sv_h, int dtype, void* stream);
+
+/* A step's accepted rows moved together, in the caches of all of a target's layers (n_caches pointers to caches of one
+ * geometry: all but the buffers' addresses alike). The nodes of request b's tree lie at the positions base[b] + node of its
+ * pages page_table[b * table_stride + j]; row base[b] + path[b * path_stride + j] of every layer and head moves to
+ * base[b] + j, for j < count[b] (of at most max_len). path: the accepted nodes, increasing (path[j] >= j), as the verifiers'
+ * accepted_path with accepted_len; a negative node, or a position outside the table or the pool, is left out. The
+ * positions from base[b] on are the request's own. All indices int32 on the device. Supported: max_len <= 1024. */
+cfb_status cfb_kv_keep(const cfb_kv_cache* const* caches, int n_caches, const int32_t* page_table,
+                       int64_t table_stride, int table_width, const int32_t* base, const int32_t* path,
+                       int64_t path_stride, const int32_t* count, int max_len, int B, void* stream);
+/* The first slots[i] slots (NULL: all) of page src[i] to page dst[i], for each of `pairs` pairs, in every cache. A pair
+ * with a page outside the pool, or of a page with itself, is left out; the dst of a call are distinct, and none is a src. */
+cfb_status cfb_kv_copy_pages(const cfb_kv_cache* const* caches, int n_caches, const int32_t* src,
+                             const int32_t* dst, const int32_t* slots, int pairs, void* stream);
+
+/* The pages of a pool by their reference counts refs[pages] (int32, on the device; 0: free), and rows of a page table
+ * (int32 [B, table_width], row stride table_stride) that hold a request's pages in order of its positions.
+ * cfb_pages_reserve: request b holds pages for length[b] positions and asks for those of target[b] (not more: nothing is
+ * asked). Requests take the lowest free pages in order (count 1), until one asks for more than are left: it and all
+ * later ones that ask get none. granted[b]: 1, or 0 where a request got none; one that asks for more than a row holds
+ * gets none either, and leaves the others theirs.
+ * cfb_pages_release: the pages of the positions past keep[b] (NULL: 0) up to length[b] lose a reference, their entries
+ * become -1. Entries outside the pool are left out; a page that nobody holds keeps its count and sets *err (may be NULL).
+ * cfb_pages_fork: row child[i] becomes a copy of row parent[i] (both of `rows` rows; a row outside, or its own child: not
+ * granted), length[child[i]] = length[parent[i]]: the full pages are shared (a reference more), and the slots of a last
+ * page that is not full are copied to a page of the child's own (the lowest free, in order of i, granted as above) in each
+ * of the caches (n_caches may be 0: their owner copies). What row child[i] held is not given back; the children of a
+ * call are distinct, and none is a parent.
+ * Calls on a pool are ordered on one stream. Supported: pages <= 2^20. */
+cfb_status cfb_pages_reserve(int32_t* refs, int pages, int page_size, int32_t* table, int64_t table_stride,
+                             int table_width, const int32_t* length, const int32_t* target, int32_t* granted,
+                             int B, void* stream);
+cfb_status cfb_pages_release(int32_t* refs, int pages, int page_size, int32_t* table, int64_t table_stride,
+                             int table_width, const int32_t* length, const int32_t* keep, int B, int* err,
+                             void* stream);
+cfb_status cfb_pages_fork(int32_t* refs, int pages, int page_size, int32_t* table, int64_t table_stride,
+                          int table_width, int rows, int32_t* length, const int32_t* parent,
+                          const int32_t* child, int32_t* granted, int n, const cfb_kv_cache* const* caches,
+                          int n_caches, void* stream);
 
 /* Attention of new tokens over a paged cache, for B requests in one launch. Request b owns the
  * query rows [cu_q[b], cu_q[b + 1]) (int32 [B + 1], non-decreasing, within [0, T]), n of them, and

@@ -24,6 +24,8 @@ from .vae import vae_encode, vae_decode, predict_hidden_vae
 from .tree_attn import tree_attn_merge, attention_over
 from .tree_verify import tree_verify_greedy
 from .paged import kv_quantise, kv_values, paged_attention
+from .verify import tree_verify_sampled, chain_verify_rejection
+from . import pages
 
 __all__ = [
     "FlowConfig", "layer_norm", "mha", "flow_block", "expert_velocity", "integrate",
@@ -32,4 +34,5 @@ __all__ = [
     "tree_gdn_scan", "path_gdn_output", "tree_gdn_verify", "tree_gdn_factor", "ring_write", "ring_gather",
     "vae_encode", "vae_decode", "predict_hidden_vae", "tree_attn_merge", "attention_over", "tree_verify_greedy",
     "gdn_sequence", "kv_quantise", "kv_values", "paged_attention",
+    "tree_verify_sampled", "chain_verify_rejection", "pages",
 ]
