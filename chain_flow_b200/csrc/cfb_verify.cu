@@ -17,11 +17,12 @@
 // totals through distributed shared memory.
 //
 // Error of the pass, with u = 2^-24 and x = (l - max l) c: an element's exponent is off by 3 u |x| (difference, c,
-// product; its unit's base likewise), each of its two exponentials by 4 u, and sums of V weights by 15 u (chains of 8,
-// pairs, the warp) and 5 u where the draw's unit is scanned. Under the weights the mean of |x| is their entropy less
-// log2 of their sum Z relative to the largest: at most log2(V / Z). What decides is C - t = C - u Z: an error that is
-// the same share of every weight cancels in it but for a half. So C - t is off by less than
-//   Z u (3 ln 2 log2(V / Z) + (8 + 15) / 2 + 5).
+// product; its unit's base likewise), each of its two exponentials by 4 u, a unit's sum by 12 u (chains of 4, pairs,
+// the warp). Under the weights the mean of |x| is their entropy less log2 of their sum Z relative to the largest: at
+// most log2(V / Z). What decides is C - t = C - u Z: an error that is the same share of every weight cancels in it but
+// for a half. The sums over CTAs, over a CTA's n units, and inside the draw's unit are fp32 too. So C - t is off by
+// less than
+//   u Z (3 ln 2 log2(V / Z) + (8 + 12) / 2 + 10) + u (mass of the CTA's part) (8 + n / 32) + 18 u (mass of the unit).
 // Rows of 248320 normal logits of deviation 2.5 fall into that band once in ten draws, a language model's less.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -64,6 +65,7 @@ struct VerifyArgs {
 };
 
 enum Kind : int { ROW_MASS = 0, ROW_EMPTY = 1, ROW_NAN = 2 };
+constexpr int kUndecided = 2;                              // RowResult::accept: fp32 did not decide (scaled: the row's largest)
 
 struct Pub { float top; int nan; double sum; };            // a CTA's part of a row
 struct Found { int token, unsure; float logit; int pad; };
@@ -71,10 +73,14 @@ struct Found { int token, unsure; float logit; int pad; };
 struct Shared {
   Pub pub[2];
   Found found[2];
-  double z, r;               // of the whole row: sum of weights, of what is left above q
-  double before, end;        // the running sum before this CTA's part and behind it
-  float top;                 // of the whole row
+  double z;                  // sum of the row's weights
+  double whole;              // sum of what the last pass summed
+  double t;                  // the owner's: its part's threshold, in the scale of its sums
+  float band;                // and how near to it fp32 decides nothing
+  float top;                 // of the row
   int kind;
+  int owner;                 // the CTA whose part has the threshold, or (greedy rows) the first of the largest
+  int last;
 };
 
 CFB_DEV float ex2(float x) {
@@ -178,36 +184,35 @@ template <typename T> CFB_DEV float vector_max(const uint4& v) {
 CFB_DEV float weight(float l, float base, float c) {
   return l == base ? 1.f : isinf(base) ? 0.f : ex2((l - base) * c);
 }
-// 2^y for y <= 0 to 10^-14, denormals kept: the series of 2^r, |r| <= 1/2, cut after r^11 (the first term left out is
-// 6 10^-15), and the power of two in two factors, since one alone does not reach the denormals. Inlined and without a branch,
-// so that several run side by side: the library's function took this pass 4 times as long.
-CFB_DEV double exp2_neg(double y) {
-  y = fmax(y, -1100.);
+// 2^y for the weights in 64 bits, by a whole warp: y = k / 32 + r with |r| <= 1/64, the series of 2^r cut after r^5 (the first
+// term left out is 2 10^-15), 2^(k mod 32 / 32) from the lane that holds it. x: y in fp32; below 2^-1090 it is 0. The
+// library's function branches, which kept several from running side by side: a pass took 4 times as long.
+CFB_DEV double exp2_table(int lane) { return exp2((double)lane * 0.03125); }
+CFB_DEV double exp2_neg(double y, float x, double table) {
+  const bool none = !(x > -1090.f);
+  y = none ? 0. : y;
   const double magic = 6755399441055744.;                  // 1.5 2^52: adding it rounds to a whole number
-  const double shifted = y + magic, r = y - (shifted - magic);
-  const int n = __double2loint(shifted), h = n >> 1;
-  double p = 0x1.e8cac7351bb25p-32;                       // ln2^k / k!
-  p = fma(p, r, 0x1.e4cf5158b8ecap-28);
-  p = fma(p, r, 0x1.b5253d395e7c4p-24);
-  p = fma(p, r, 0x1.62c0223a5c824p-20);
-  p = fma(p, r, 0x1.ffcbfc588b0c7p-17);
-  p = fma(p, r, 0x1.430912f86c787p-13);
-  p = fma(p, r, 0x1.5d87fe78a6731p-10);
+  const double shifted = fma(y, 32., magic), r = fma(shifted - magic, -0.03125, y);
+  const int k = __double2loint(shifted), n = k >> 5;
+  double p = 0x1.5d87fe78a6731p-10;                                           // ln2^k / k!
   p = fma(p, r, 0x1.3b2ab6fba4e77p-7);
   p = fma(p, r, 0x1.c6b08d704a0c0p-5);
   p = fma(p, r, 0x1.ebfbdff82c58fp-3);
   p = fma(p, r, 0x1.62e42fefa39efp-1);
-  p = fma(p, r, 1.);
-  return p * __hiloint2double((1023 + h) << 20, 0) * __hiloint2double((1023 + n - h) << 20, 0);
+  const double t = __shfl_sync(0xffffffffu, table, k & 31);
+  p = fma(p * r, t, t);
+  const int up = max(n, -1020);                            // (denormals in a second step)
+  p = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
+  if (n < -1020) p *= __hiloint2double((1023 + n + 1020) << 20, 0);
+  return none ? 0. : p;
 }
-// the fp32 number as a double, by its bits (conversions are slow): what is 0 becomes 2^-127 and -inf -2^128, which
-// differ from them by nothing that a weight shows
+// the fp32 number as a double, by its bits (conversions are slow): what is 0 becomes 2^-127, and an infinity 2^128
 CFB_DEV double widen(float f) {
   const uint32_t b = __float_as_uint(f);
   return __hiloint2double((int)((b & 0x80000000u) | (((b >> 3) & 0x0fffffffu) + 0x38000000u)), (int)(b << 29));
 }
-CFB_DEV double weight64(float l, float base, double c64) {
-  return l == base ? 1. : isinf(base) ? 0. : exp2_neg(((double)l - (double)base) * c64);
+CFB_DEV double weight64(float l, float base, double c64) {           // of one element
+  return l == base ? 1. : isinf(base) ? 0. : exp2(((double)l - (double)base) * c64);
 }
 // the draft probability of token i (0 outside the row and for what is not a positive number)
 template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
@@ -218,13 +223,21 @@ template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
 
 enum Mode : int { W32 = 0, W64 = 1, R32 = 2, R64 = 3 };    // weights, or what is left of them above q
 template <int MODE> constexpr bool kNarrow = MODE == W32 || MODE == R32;
+// elements of a summed unit, and a lane's of them: in 64 bits, where an element costs much more, smaller ones to scan
+template <int MODE> constexpr int kSpan = kNarrow<MODE> ? kUnit : 256;
 
-// iz: 1 / the row's sum of weights (R32, R64)
-template <int MODE, typename T> CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz) {
-  if constexpr (MODE == W32) return weight(l, base, w.c);
-  else if constexpr (MODE == W64) return weight64(l, base, w.c64);
-  else if constexpr (MODE == R32) return fmaxf(weight(l, base, w.c) * (float)iz - draft_prob(w, i), 0.f);
-  else return fmax(weight64(l, base, w.c64) * iz - (double)draft_prob(w, i), 0.);
+// an element's value, by a whole warp. iz: 1 / the row's sum of weights (R32, R64)
+template <int MODE, typename T> CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, double table) {
+  if constexpr (MODE == W32) {
+    return weight(l, base, w.c);
+  } else if constexpr (MODE == R32) {
+    return fmaxf(weight(l, base, w.c) * (float)iz - draft_prob(w, i), 0.f);
+  } else {
+    const double e = exp2_neg((widen(l) - (double)base) * w.c64, (l - base) * w.c, table);
+    const double v = l == base ? 1. : isinf(base) ? 0. : e;
+    if constexpr (MODE == W64) return v;
+    else return fmax(v * iz - (double)draft_prob(w, i), 0.);
+  }
 }
 
 // The part of a row that a CTA has: units [u0, u1) of it
@@ -235,7 +248,7 @@ template <typename T> CFB_DEV Span span_of(const Row<T>& w, int rank, int ranks)
 }
 
 // every unit's largest and its sum of weights relative to that; a unit's loads are under way while the one before is summed
-template <typename T> CFB_DEV void stats_units(const Row<T>& w, Span s, float* tops, double* sums) {
+template <typename T> CFB_DEV void stats_units(const Row<T>& w, Span s, float* tops, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint4 next[kVectors<T>];
   if (s.u0 + warp < s.u1) load_unit(w, s.u0 + warp, lane, next);
@@ -251,16 +264,17 @@ template <typename T> CFB_DEV void stats_units(const Row<T>& w, Span s, float* t
     float sum = 0.f;
     if (fabsf(top) < INFINITY) {
       const Pair base = pair(-top, -top), c = pair(w.c, w.c);
-      Pair a[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+      Pair a[4] = {pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
       for (int j = 0; j < kVectors<T>; ++j)
 #pragma unroll
         for (int k = 0; k < kE<T> / 2; ++k) {
           const float2 l = pair_of<T>(v[j], k);
           const float2 x = both(mul2(add2(pair(l.x, l.y), base), c));
-          a[k & 1] = add2(a[k & 1], pair(ex2(x.x), ex2(x.y)));
+          const int i = (j * (kE<T> / 2) + k) & 3;
+          a[i] = add2(a[i], pair(ex2(x.x), ex2(x.y)));
         }
-      const float2 t = both(add2(a[0], a[1]));
+      const float2 t = both(add2(add2(a[0], a[1]), add2(a[2], a[3])));
       sum = t.x + t.y;
     } else {                                               // +inf, or nothing but -inf; NaN makes the sum NaN
 #pragma unroll
@@ -296,7 +310,7 @@ template <typename F> CFB_DEV void table_entries(const F* t, int i, int n, int V
 }
 
 // every unit's sum of what is left above q
-template <typename T> CFB_DEV void rest_units(const Row<T>& w, Span s, float base, float iz, double* sums) {
+template <typename T> CFB_DEV void rest_units(const Row<T>& w, Span s, float base, float iz, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int u = s.u0 + warp; u < s.u1; u += kWarps) {
     uint4 v[kVectors<T>];
@@ -325,40 +339,34 @@ template <typename T> CFB_DEV void rest_units(const Row<T>& w, Span s, float bas
     if (lane == 0) sums[u - s.u0] = sum;
   }
 }
-// every unit's sum in 64 bits
-template <int MODE, typename T> CFB_DEV void exact_units(const Row<T>& w, Span s, float base, double iz, double* sums) {
+// every unit's sum in 64 bits: a lane has 8 neighbours of 256
+template <int MODE, typename T>
+CFB_DEV void exact_units(const Row<T>& w, Span s, float base, double iz, double table, double* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const double top = base;
-  for (int u = s.u0 + warp; u < s.u1; u += kWarps) {
+  constexpr int kPer = kUnit / kSpan<MODE>;
+  for (int u = s.u0 * kPer + warp; u < s.u1 * kPer; u += kWarps) {
+    const int i = u * kSpan<MODE> + lane * 8 - w.shift;
     double a[2] = {0., 0.};
-    if (isinf(base) || MODE == R64) {
-#pragma unroll 1
-      for (int k = 0; k < kPerLane; ++k) {
-        const int i = u * kUnit + k * 32 + lane - w.shift;
-        if (i >= 0 && i < w.V) a[0] += value_of<MODE>(w, to_float(w.p[i]), i, base, iz);
-      }
-    } else {
-#pragma unroll 1
-      for (int j = 0; j < kVectors<T>; ++j) {
-        const uint4 v = load_vector(w, first_of(w, u, j, lane));
 #pragma unroll
-        for (int k = 0; k < kE<T> / 2; ++k) {
-          const float2 l = pair_of<T>(v, k);
-          a[0] += exp2_neg((widen(l.x) - top) * w.c64);
-          a[1] += exp2_neg((widen(l.y) - top) * w.c64);
-        }
+    for (int j = 0; j < 8 / kE<T>; ++j) {
+      const uint4 v = load_vector(w, i + j * kE<T>);
+#pragma unroll
+      for (int k = 0; k < kE<T> / 2; ++k) {
+        const float2 l = pair_of<T>(v, k);
+        a[0] += value_of<MODE>(w, l.x, i + j * kE<T> + 2 * k, base, iz, table);
+        a[1] += value_of<MODE>(w, l.y, i + j * kE<T> + 2 * k + 1, base, iz, table);
       }
     }
     const double sum = warp_sum(a[0] + a[1]);
-    if (lane == 0) sums[u - s.u0] = sum;
+    if (lane == 0) sums[u - s.u0 * kPer] = sum;
   }
 }
 
 // Warp 0: the units' sums become running ones
-CFB_DEV double run_up(double* sums, int n, int lane) {
-  double before = 0.;
+template <typename F> CFB_DEV F run_up(F* sums, int n, int lane) {
+  F before = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
-    const double v = warp_scan(i0 + lane < n ? sums[i0 + lane] : 0., lane);
+    const F v = warp_scan(i0 + lane < n ? sums[i0 + lane] : (F)0, lane);
     if (i0 + lane < n) sums[i0 + lane] = before + v;
     before += __shfl_sync(0xffffffffu, v, 31);
   }
@@ -366,14 +374,13 @@ CFB_DEV double run_up(double* sums, int n, int lane) {
   return before;
 }
 
-// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start). A lane takes 32
-// neighbours of the unit that holds it. The fp32 modes sum in fp32 inside the unit: 37 additions in a row at most,
-// another 2^-18 of the unit's mass.
-template <int MODE, typename T>
-CFB_DEV Found find(const Row<T>& w, Span s, const double* sums, double t, float base, double iz, double band) {
-  using F = typename std::conditional<kNarrow<MODE>, float, double>::type;
-  constexpr int kRoll = kNarrow<MODE> ? kPerLane : 1;
-  const int lane = threadIdx.x & 31, n = s.u1 - s.u0;
+// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start): by units, by lanes
+// of neighbours, by a lane's elements. band: for all but the unit's own rounding.
+template <int MODE, typename T, typename F>
+CFB_DEV Found find(const Row<T>& w, Span s, const F* sums, F t, float base, double iz, float band) {
+  constexpr int kPer = kUnit / kSpan<MODE>, kLane = kSpan<MODE> / 32;   // summed units a unit; a lane's elements
+  const int lane = threadIdx.x & 31, n = (s.u1 - s.u0) * kPer;
+  const double table = kNarrow<MODE> ? 0. : exp2_table(lane);
   int u = -1;
   for (int i0 = 0; i0 < n && u < 0; i0 += 32) {
     const unsigned hit = __ballot_sync(0xffffffffu, i0 + lane < n && sums[i0 + lane] > t);
@@ -384,68 +391,60 @@ CFB_DEV Found find(const Row<T>& w, Span s, const double* sums, double t, float 
     unsure = true;
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + lane;
-      const unsigned hit = __ballot_sync(0xffffffffu, i < n && sums[i] > (i ? sums[i - 1] : 0.));
+      const unsigned hit = __ballot_sync(0xffffffffu, i < n && sums[i] > (i ? sums[i - 1] : (F)0));
       if (hit) u = i0 + 31 - __clz(hit);
     }
     if (u < 0) return {-1, 1, 0.f, 0};
   }
-  t -= u ? sums[u - 1] : 0.;
-  const int i0 = (s.u0 + u) * kUnit + lane * kPerLane - w.shift;
-  uint4 v[kVectors<T>];
-  if constexpr (kNarrow<MODE>)
+  const int first = s.u0 * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
+  F a = 0;
 #pragma unroll
-    for (int j = 0; j < kVectors<T>; ++j) v[j] = load_vector(w, i0 + j * kE<T>);
-  const auto logit = [&](int e) {
-    if constexpr (kNarrow<MODE>) {
-      const float2 l = pair_of<T>(v[e / kE<T>], e % kE<T> / 2);
-      return e & 1 ? l.y : l.x;
-    } else {
-      return i0 + e >= 0 && i0 + e < w.V ? to_float(w.p[i0 + e]) : -INFINITY;
+  for (int j = 0; j < kLane / kE<T>; ++j) {
+    const uint4 x = load_vector(w, i0 + j * kE<T>);
+    F v[kE<T>];
+#pragma unroll
+    for (int k = 0; k < kE<T> / 2; ++k) {
+      const float2 l = pair_of<T>(x, k);
+      v[2 * k] = value_of<MODE>(w, l.x, i0 + j * kE<T> + 2 * k, base, iz, table);
+      v[2 * k + 1] = value_of<MODE>(w, l.y, i0 + j * kE<T> + 2 * k + 1, base, iz, table);
     }
-  };
-  F x[kNarrow<MODE> ? kPerLane : 1], a = 0;
-  int last = -1;                                           // this lane's last token with mass
-#pragma unroll kRoll
-  for (int e = 0; e < kPerLane; ++e) {
-    const F y = value_of<MODE>(w, logit(e), i0 + e, base, iz);
-    if constexpr (kNarrow<MODE>) x[e] = y;
-    a += y;
-    if (y > 0) last = e;
+#pragma unroll
+    for (int e = kE<T>; e > 1; e >>= 1)
+#pragma unroll
+      for (int k = 0; k < e / 2; ++k) v[k] = v[2 * k] + v[2 * k + 1];
+    a += v[0];
   }
+  const F before = u ? sums[u - 1] : (F)0, at = t - before, mass = sums[u] - before;
   const F scan = warp_scan(a, lane), up = __shfl_up_sync(0xffffffffu, scan, 1);
-  const unsigned some = __ballot_sync(0xffffffffu, a > 0);
-  unsigned hit = __ballot_sync(0xffffffffu, a > 0 && (double)scan > t);
-  if (!hit) {                                              // as above, inside the unit
+  // where no sum passes, for rounding or after the fallback above: the last that has any
+  unsigned hit = __ballot_sync(0xffffffffu, a > 0 && scan > at);
+  if (!hit) {
+    const unsigned some = __ballot_sync(0xffffffffu, a > 0);
     if (!some) return {-1, 1, 0.f, 0};
     unsure = true;
     hit = 1u << (31 - __clz(some));
   }
-  const int who = __ffs(hit) - 1;
-  int token = -1;
-  float l = 0.f;
-  F run = lane ? up : (F)0, lo = 0, hi = 0;
-  if (lane == who) {
-#pragma unroll kRoll
-    for (int e = 0; e < kPerLane; ++e) {
-      F y;
-      if constexpr (kNarrow<MODE>) y = x[e];
-      else y = value_of<MODE>(w, logit(e), i0 + e, base, iz);
-      if (token < 0 && y > 0 && ((double)(run + y) > t || e == last)) {
-        token = i0 + e;
-        l = logit(e);
-        lo = run;
-        hi = run + y;
-      }
-      run += y;
-    }
+  const int who = __ffs(hit) - 1, i = first + who * kLane + lane;
+  const F head = who ? __shfl_sync(0xffffffffu, up, who) : (F)0;
+  const float l = lane < kLane && i >= 0 && i < w.V ? to_float(w.p[i]) : -INFINITY;
+  const F y = value_of<MODE>(w, l, lane < kLane ? i : -1, base, iz, table), run = head + warp_scan(y, lane);
+  hit = __ballot_sync(0xffffffffu, y > 0 && run > at);
+  if (!hit) {
+    unsure = true;
+    hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, y > 0)));
   }
-  unsure |= !(t - (double)lo >= band && (double)hi - t >= band);
-  return {__shfl_sync(0xffffffffu, token, who), (int)__shfl_sync(0xffffffffu, (int)unsure, who), __shfl_sync(0xffffffffu, l, who), 0};
+  const int e = __ffs(hit) - 1;
+  const F hi = __shfl_sync(0xffffffffu, run, e), lo = e ? __shfl_sync(0xffffffffu, run, max(e - 1, 0)) : head;
+  if constexpr (kNarrow<MODE>) {
+    const float off = band + 18.f * (float)kRound * mass;
+    unsure |= !(at - lo >= off && hi - at >= off);
+  }
+  return {first + who * kLane + e, unsure, __shfl_sync(0xffffffffu, l, e), 0};
 }
 
 // Warp 0: the first element that equals the row's largest (or the first NaN)
 template <typename T>
-CFB_DEV int find_top(const Row<T>& w, Span s, const float* tops, const double* sums, float top, bool nan) {
+CFB_DEV int find_top(const Row<T>& w, Span s, const float* tops, const float* sums, float top, bool nan) {
   const int lane = threadIdx.x & 31, n = s.u1 - s.u0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int k = i0 + lane;
@@ -473,52 +472,70 @@ CFB_DEV int find_top(const Row<T>& w, Span s, const float* tops, const double* s
 template <typename T> struct Team {
   Shared* sh;
   float* tops;
-  double* sums;
+  void* room;                // the units' sums
   int rank, ranks, ph;
 
-  // this CTA's part, handed to the others by the next cluster barrier
-  CFB_DEV void publish(float top, int nan, double sum) {
-    sh->pub[ph] = {top, nan, sum};
-    sh->found[ph] = {-1, 1, 0.f, 0};                       // kept where no part has the threshold
-  }
+  // How far an fp32 sum over the row may be from its side of a threshold, as a share of the row's mass
+  CFB_DEV float band(const Row<T>& w) const { return (float)kRound * (2.08f * __log2f((float)w.V / (float)sh->z) + 20.f); }
 
-  // totals of all CTAs -> the row's, and what lies before this one's part. `scaled`: each relative to its own largest
-  CFB_DEV void exchange(float c, bool scaled, double* whole) {
+  // The CTAs' totals, handed over by the cluster's barrier -> the row's; who has the threshold u of it. SCALED: each
+  // total is relative to its CTA's largest; greedy: the owner is the first that has the row's largest.
+  template <typename F, bool SCALED> CFB_DEV void exchange(const Row<T>& w, double u, bool greedy, bool rest) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
       Pub p{-INFINITY, 0, 0.};
       if (lane < ranks) p = *cluster.map_shared_rank(&sh->pub[ph], lane);
-      if (scaled) {
-        const float top = warp_max(p.top);
-        const bool nan = __any_sync(0xffffffffu, p.nan);
-        if (lane == 0) {
+      F scale = 1;
+      bool nan = false;
+      float top = sh->top;
+      if constexpr (SCALED) {
+        top = warp_max(p.top);
+        nan = __any_sync(0xffffffffu, p.nan);
+        scale = p.top == -INFINITY ? 0.f : weight(p.top, top, w.c);
+      }
+      const F own = (F)p.sum, m = own * scale;
+      F scan = m;
+#pragma unroll
+      for (int off = 1; off < kMaxCluster; off <<= 1) {
+        const F o = __shfl_up_sync(0xffffffffu, scan, off);
+        if (lane >= off) scan += o;
+      }
+      const F whole = __shfl_sync(0xffffffffu, scan, kMaxCluster - 1);
+      // (the sum before, not the one behind less this part's, which would lose small ones)
+      const F up = __shfl_up_sync(0xffffffffu, scan, 1), before = lane ? up : (F)0;
+      const F most = whole * (F)(sizeof(F) == 4 ? 1. - 1.2e-7 : 1. - 2.3e-16), raw = (F)(u * (double)whole), t = raw < most ? raw : most;
+      unsigned hit = __ballot_sync(0xffffffffu, m > 0 && before <= t && t < scan);
+      if (!hit) hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, m > 0) | 1u));
+      if (SCALED && (greedy || nan)) hit = __ballot_sync(0xffffffffu, nan ? p.nan != 0 : p.top == top);
+      if (lane == rank) {
+        sh->t = (double)((t - before) / scale);
+        // (of what is left above q, the error is that of the probabilities, whose whole is 1)
+        if (SCALED || rest) {
+          const float z = SCALED ? (float)whole : (float)sh->z;
+          const float row = (float)kRound * (2.08f * __log2f((float)w.V / z) + 20.f);
+          const int n = ((w.V + kUnit - 1) / kUnit + ranks - 1) / ranks;
+          sh->band = (rest ? row + 24.f * (float)kRound : row * (float)whole / (float)scale) + (float)kRound * (8 + n / 32) * (float)own;
+        }
+      }
+      if (lane == 0) {
+        sh->owner = __ffs(hit) - 1;
+        sh->whole = whole;
+        if (SCALED) {
+          sh->z = whole;
           sh->top = top;
           sh->kind = nan ? ROW_NAN : top == -INFINITY ? ROW_EMPTY : ROW_MASS;
         }
-        p.sum *= p.top == -INFINITY ? 0. : (double)weight(p.top, top, c);
       }
-      double scan = p.sum;
-#pragma unroll
-      for (int off = 1; off < kMaxCluster; off <<= 1) {
-        const double o = __shfl_up_sync(0xffffffffu, scan, off);
-        if (lane >= off) scan += o;
-      }
-      // (the sum before, not the one behind less this part's, which would lose small ones)
-      const double before = __shfl_up_sync(0xffffffffu, scan, 1);
-      if (lane == rank) {
-        sh->before = rank ? before : 0.;
-        sh->end = scan;
-      }
-      if (lane == kMaxCluster - 1) *whole = scan;
     }
     __syncthreads();
   }
 
   // the pass over the row
-  CFB_DEV void stats(const Row<T>& w) {
+  CFB_DEV void stats(const Row<T>& w, double u, bool greedy) {
     const Span s = span_of(w, rank, ranks);
+    float* const sums = static_cast<float*>(room);
     stats_units(w, s, tops, sums);
     __syncthreads();
     ph ^= 1;
@@ -532,148 +549,137 @@ template <typename T> struct Team {
       }
       top = warp_max(top);
       nan = __any_sync(0xffffffffu, nan);
-      double sum = 0.;
+      float sum = 0.f;
       if (!nan) {
-        for (int i = lane; i < n; i += 32) sums[i] *= tops[i] == -INFINITY ? 0. : (double)weight(tops[i], top, w.c);
+        for (int i = lane; i < n; i += 32) sums[i] *= tops[i] == -INFINITY ? 0.f : weight(tops[i], top, w.c);
         __syncwarp();
         sum = run_up(sums, n, lane);
       }
-      if (lane == 0) publish(top, nan, sum);
+      if (lane == 0) sh->pub[ph] = {top, nan, (double)sum};
     }
-    exchange(w.c, true, &sh->z);
+    exchange<float, true>(w, u, greedy, false);
   }
 
-  // a pass that knows the row's largest
-  template <int MODE> CFB_DEV void pass(const Row<T>& w, double* whole) {
+  // a pass that knows the row's largest, and its sum where it needs it
+  template <int MODE> CFB_DEV void pass(const Row<T>& w, double u) {
+    using F = typename std::conditional<kNarrow<MODE>, float, double>::type;
     const Span s = span_of(w, rank, ranks);
-    if constexpr (MODE == R32) rest_units(w, s, sh->top, (float)(1. / sh->z), sums);
-    else exact_units<MODE>(w, s, sh->top, 1. / sh->z, sums);
+    F* const sums = static_cast<F*>(room);
+    if constexpr (MODE == R32) rest_units(w, s, sh->top, 1.f / (float)sh->z, sums);
+    else exact_units<MODE>(w, s, sh->top, MODE == R64 ? 1. / sh->z : 0., exp2_table(threadIdx.x & 31), sums);
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) {
-      const double sum = run_up(sums, s.u1 - s.u0, threadIdx.x);
-      if (threadIdx.x == 0) publish(sh->top, 0, sum);
+      const F sum = run_up(sums, (s.u1 - s.u0) * (kUnit / kSpan<MODE>), (int)threadIdx.x);
+      if (threadIdx.x == 0) sh->pub[ph] = {sh->top, 0, (double)sum};
     }
-    exchange(w.c, false, whole);
+    exchange<F, false>(w, u, false, MODE == R32);
   }
 
-  // Warp 0 of the CTA that found it hands it to all
-  CFB_DEV Found share(bool mine, Found f) {
+  // Warp 0 of the owner: the token of the last pass's threshold
+  template <int MODE> CFB_DEV Found found(const Row<T>& w) const {
+    using F = typename std::conditional<kNarrow<MODE>, float, double>::type;
+    return find<MODE>(w, span_of(w, rank, ranks), static_cast<const F*>(room), (F)sh->t, MODE == W32 ? sh->pub[ph].top : sh->top,
+                      MODE == R32 ? (double)(1.f / (float)sh->z) : MODE == R64 ? 1. / sh->z : 0., sh->band);
+  }
+  CFB_DEV Found found_top(const Row<T>& w) const {
+    const int t = find_top(w, span_of(w, rank, ranks), tops, static_cast<const float*>(room), sh->top, sh->kind == ROW_NAN);
+    return {t, 0, sh->top, 0};
+  }
+
+  // Warp 0 of the owner hands what it found to all
+  CFB_DEV Found share(Found f) {
     cg::cluster_group cluster = cg::this_cluster();
-    if (mine && threadIdx.x < ranks) *cluster.map_shared_rank(&sh->found[ph], (int)threadIdx.x) = f;
+    if (rank == sh->owner && threadIdx.x < ranks) *cluster.map_shared_rank(&sh->found[ph], (int)threadIdx.x) = f;
     cluster.sync();
     return sh->found[ph];
   }
-
-  // the draw of threshold u among the running sums of the last pass, whose whole is `whole`
-  template <int MODE> CFB_DEV Found draw(const Row<T>& w, double u, double whole) {
-    bool mine = false;
+  template <int MODE> CFB_DEV Found draw(const Row<T>& w) {
     Found f{-1, 1, 0.f, 0};
-    if (threadIdx.x < 32) {
-      const Pub own = sh->pub[ph];
-      const double t = fmin(u * whole, whole * (1. - 2.220446049250313e-16));
-      // relative to the base of this CTA's sums
-      const double scale = MODE == W32 ? (own.top == -INFINITY ? 0. : (double)weight(own.top, sh->top, w.c)) : 1.;
-      mine = own.sum * scale > 0. && sh->before <= t && (t < sh->end || last_with_mass(w.c, MODE == W32));
-      // (of what is left above q, the error is that of the probabilities, whose whole is 1)
-      if (mine)
-        f = find<MODE>(w, span_of(w, rank, ranks), sums, (t - sh->before) / scale, MODE == W32 ? own.top : sh->top, 1. / sh->z,
-                       MODE == W32 ? band(w) * whole / scale : MODE == R32 ? band(w) + 24 * kRound : 0.);
-    }
-    return share(mine, f);
-  }
-  // how far a sum may be from its threshold's side, as a share of the row's mass (from what is left above q: and the
-  // probabilities' own rounding)
-  CFB_DEV double band(const Row<T>& w) const { return kRound * (2.08 * (double)__log2f((float)w.V / (float)sh->z) + 17.); }
-  // no later part has any
-  CFB_DEV bool last_with_mass(float c, bool scaled) {
-    for (int r = rank + 1; r < ranks; ++r) {
-      const Pub p = *cg::this_cluster().map_shared_rank(&sh->pub[ph], r);
-      if (p.sum > 0. && (!scaled || weight(p.top, sh->top, c) > 0.f)) return false;
-    }
-    return true;
-  }
-
-  // the first of the row's largest
-  CFB_DEV int top_token(const Row<T>& w, bool nan) {
-    bool mine = false;
-    Found f{-1, 0, 0.f, 0};
-    if (threadIdx.x < 32) {
-      mine = nan ? sh->pub[ph].nan : sh->pub[ph].top == sh->top;
-      for (int r = 0; r < rank && mine; ++r) {
-        const Pub p = *cg::this_cluster().map_shared_rank(&sh->pub[ph], r);
-        mine = !(nan ? p.nan != 0 : p.top == sh->top);
-      }
-      if (mine) f.token = find_top(w, span_of(w, rank, ranks), tops, sums, sh->top, nan);
-    }
-    return share(mine, f).token;
+    if (rank == sh->owner && threadIdx.x < 32) f = found<MODE>(w);
+    return share(f);
   }
 };
 
-// the draw in 64 bits, and the alternation of the exchanged buffers after it. rest: from what is left above q
-struct Exact { Found f; int ph; };
-template <typename T>
-__device__ __noinline__ Exact exact_draw(Team<T> team, Row<T> w, bool rest, double v) {
-  Shared& sh = *team.sh;
-  team.template pass<W64>(w, &sh.z);
-  if (rest) {
-    team.template pass<R64>(w, &sh.r);
-    if (sh.r > 0.) {
-      const Found f = team.template draw<R64>(w, v, sh.r);
-      return {f, team.ph};
-    }
-    team.template pass<W64>(w, &sh.z);                     // nothing above q: the target's own
-  }
-  const Found f = team.template draw<W64>(w, v, sh.z);
-  return {f, team.ph};
-}
-// the sum of the row's weights in 64 bits
-template <typename T> __device__ __noinline__ int exact_sum(Team<T> team, Row<T> w) {
-  team.template pass<W64>(w, &team.sh->z);
-  return team.ph;
-}
+// What a row is asked: drafted: it has a draft with probabilities, `draft`, which u accepts; v draws
+struct Asked { bool greedy, drafted; int draft; double u, v; };
 
-// One row, by a whole cluster; every thread gets the result. drafted: the row has a draft with probabilities, `draft`,
-// which u accepts; v draws.
-template <bool CHAIN, typename T>
-CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, bool greedy, bool drafted, int draft, double u, double v) {
+// The row decided in 64 bits, its largest in sh.top. Every thread of the cluster gets the result (in bit 8 of accept,
+// whether the exchanged buffers have been alternated).
+template <typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
   Shared& sh = *team.sh;
-  const bool in = CHAIN && drafted && draft >= 0 && draft < w.V;       // a draft that is no token is refused
-  const float of_draft = in ? to_float(w.p[draft]) : -INFINITY;
-  const double uq = in ? u * (double)draft_prob(w, draft) : 0.;
-  team.stats(w);
-  const auto scaled = [&](float l) { return l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64; };     // log2
-  if (sh.kind == ROW_EMPTY) return {-1, 0, 0., 1.};
-  if (greedy || sh.kind == ROW_NAN) {
-    const int t = team.top_token(w, sh.kind == ROW_NAN);
-    return {t, drafted && t == draft, sh.kind == ROW_NAN ? (double)NAN : 0., sh.z};
-  }
-  Found f{-1, 1, 0.f, 0};
-  if constexpr (CHAIN) {
-    if (drafted) {
-      if (in) {
-        double p = (double)weight(of_draft, sh.top, w.c) / sh.z;
-        // (every CTA computes the same)
-        if (fabs(uq - p) <= p * (2. * team.band(w) + kRound * (2.08 * fabs(scaled(of_draft)) + 8.))) {
-          team.ph = exact_sum(team, w);
-          p = weight64(of_draft, sh.top, w.c64) / sh.z;
-        }
-        if (uq < p) return {draft, 1, scaled(of_draft), sh.z};
-      }
-      team.template pass<R32>(w, &sh.r);
-      if (sh.r > 2. * team.band(w) + 48 * kRound) f = team.template draw<R32>(w, v, sh.r);
-    } else {
-      f = team.template draw<W32>(w, v, sh.z);
+  const int ph = team.ph;
+  const auto scaled = [&](float l) { return l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64; };
+  const auto result = [&](int token, int accept, float l) {
+    return RowResult{token, accept | (team.ph ^ ph) << 8, scaled(l), sh.z};
+  };
+  const auto sum = [&] {
+    team.template pass<W64>(w, a.v);
+    if (threadIdx.x == 0) sh.z = sh.whole;
+    __syncthreads();
+  };
+  sum();
+  Found f;
+  if (a.drafted) {
+    if (a.draft >= 0 && a.draft < w.V) {
+      const float l = to_float(w.p[a.draft]);
+      if (a.u * (double)draft_prob(w, a.draft) < weight64(l, sh.top, w.c64) / sh.z) return result(a.draft, 1, l);
+    }
+    team.template pass<R64>(w, a.v);
+    if (sh.whole > 0.) {
+      f = team.template draw<R64>(w);
+    } else {                                               // nothing above q: the target's own
+      sum();
+      f = team.template draw<W64>(w);
     }
   } else {
-    f = team.template draw<W32>(w, v, sh.z);
+    f = team.template draw<W64>(w);
   }
+  return result(f.token, 0, f.logit);
+}
+
+// One row, by a whole cluster. LAZY: what fp32 does not decide is left undecided, and the result is valid in warp 0 of
+// the CTA *holder; otherwise every thread gets it.
+template <bool CHAIN, bool LAZY, typename T>
+CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, const Asked& a, int* holder) {
+  Shared& sh = *team.sh;
+  const bool in = CHAIN && a.drafted && a.draft >= 0 && a.draft < w.V;       // a draft that is no token is refused
+  const float of_draft = in ? to_float(w.p[a.draft]) : -INFINITY, q = in ? draft_prob(w, a.draft) : 0.f;
+  team.stats(w, a.v, a.greedy);
+  const auto scaled = [&](float l) { return l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64; };     // log2
+  *holder = 0;
+  if (sh.kind == ROW_EMPTY) return {-1, 0, 0., 1.};
+  Found f{-1, 1, 0.f, 0};
+  const bool plain = a.greedy || sh.kind == ROW_NAN;
+  if (CHAIN && a.drafted && !plain) {
+    if (in) {
+      const float x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) / (float)sh.z, uq = (float)a.u * q;
+      // (every CTA computes the same)
+      const float off = p * (2.f * team.band(w) + (float)kRound * (2.08f * fabsf(x) + 12.f));
+      if (!(fabsf(uq - p) > off)) {
+        if constexpr (LAZY) return {-1, kUndecided, (double)sh.top, 1.};
+        const RowResult r = exact_row(team, w, a);
+        team.ph ^= r.accept >> 8;
+        return {r.token, r.accept & 1, r.scaled, r.mass};
+      }
+      if (uq < p) return {a.draft, 1, scaled(of_draft), sh.z};
+    }
+    team.template pass<R32>(w, a.v);
+  }
+  *holder = sh.owner;
+  if (team.rank == sh.owner && threadIdx.x < 32) {
+    if (plain) f = team.found_top(w);
+    else if (!CHAIN || !a.drafted) f = team.template found<W32>(w);
+    else if (sh.whole > 2. * (team.band(w) + 24 * kRound)) f = team.template found<R32>(w);
+  }
+  if constexpr (!LAZY) f = team.share(f);
   if (f.unsure) {
-    const Exact e = exact_draw(team, w, drafted, v);
-    f = e.f;
-    team.ph = e.ph;
+    if constexpr (LAZY) return {-1, kUndecided, (double)sh.top, 1.};
+    const RowResult r = exact_row(team, w, a);
+    team.ph ^= r.accept >> 8;
+    return {r.token, r.accept & 1, r.scaled, r.mass};
   }
-  return {f.token, 0, scaled(f.logit), sh.z};
+  return {f.token, CHAIN && plain && a.drafted && f.token == a.draft, sh.kind == ROW_NAN ? (double)NAN : scaled(f.logit), sh.z};
 }
 
 CFB_DEV double number_at(const void* p, int size, long long i) {
@@ -681,33 +687,40 @@ CFB_DEV double number_at(const void* p, int size, long long i) {
   return fmin(fmax(u, 0.), 1. - 0x1p-32);                  // (an upper end that sums of 64 bits still resolve)
 }
 
-template <typename T> CFB_DEV Row<T> row_of(const VerifyArgs& A, int row, float temp, bool greedy) {
-  Row<T> w;
-  w.p = static_cast<const T*>(A.logits) + (long long)row * A.ld;
+// row j of request b, and what it is asked
+template <typename T, bool CHAIN>
+CFB_DEV void row_of(const VerifyArgs& A, int b, int d0, int n, int s0, int j, float temp, Row<T>& w, Asked& a) {
+  w.p = static_cast<const T*>(A.logits) + (long long)(s0 + j) * A.ld;
   w.V = A.V;
   w.shift = (int)((reinterpret_cast<uintptr_t>(w.p) & 15) / sizeof(T));
-  const float tau = greedy ? 1.f : fminf(temp, kHighTemp);
-  w.c64 = 1.4426950408889634 / (double)tau;
+  a.greedy = !(temp >= kLowTemp);
+  const float tau = a.greedy ? 1.f : fminf(temp, kHighTemp);
+  w.c64 = tau == 1.f ? 1.4426950408889634 : 1.4426950408889634 / (double)tau;
   w.c = (float)fmin(w.c64, 3.4e38);
   w.q = nullptr;
   w.index_of = A.index_of;
-  return w;
+  a.drafted = CHAIN && j < n;
+  a.draft = a.drafted ? A.draft_tokens[d0 + j] : -1;
+  a.u = a.drafted ? number_at(A.uniforms, A.uniform_size, d0 + j) : 0.;
+  a.v = CHAIN ? number_at(A.resample, A.uniform_size, b) : number_at(A.uniforms, A.uniform_size, s0 + j);
+  if (a.drafted) w.q = A.probs + (long long)(d0 + j) * A.ld_probs;
 }
 
 // FLAT: a cluster a row (grid.y: rows of a request, grid.z: requests), every row at once; the request's last
-// cluster walks. Otherwise a cluster a request (grid.y), which takes the rows of its walk in turn.
-// CHAIN: draft probabilities; a node's only child is the next one.
+// cluster walks, and decides the rows that its walk meets undecided. Otherwise a cluster a request (grid.y), which
+// takes the rows of its walk in turn. CHAIN: draft probabilities; a node's only child is the next one.
 template <typename T, bool CHAIN, bool FLAT>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A, int most) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs A, int most) {
   extern __shared__ double s_dyn[];
   __shared__ Shared sh;
-  __shared__ int s_last;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   // what a walk keeps: the results of its rows (in turn, or FLAT: of all rows), the rows it took, the tree
-  RowResult* const s_row = reinterpret_cast<RowResult*>(s_dyn + most);
+  constexpr int kPer = kUnit / kSpan<W64>;
+  RowResult* const s_row = reinterpret_cast<RowResult*>(s_dyn + kPer * most);
   int* const s_node = reinterpret_cast<int*>(s_row + A.max_spec + 1);
-  int* const s_parent = s_node + A.max_spec + 1;
+  int* const s_next = s_node + A.max_spec + 1;             // FLAT: the child that a row's token leads to
+  int* const s_parent = s_next + A.max_spec + 1;
   int* const s_token = s_parent + A.max_spec;
   Team<T> team{&sh, reinterpret_cast<float*>(s_token + A.max_spec), s_dyn, rank, ranks, 0};
   const int b = FLAT ? blockIdx.z : blockIdx.y;
@@ -718,54 +731,78 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A,
   const bool sane = drafts >= 0 && drafts <= A.max_spec && start >= 0 && start + drafts < A.num_rows && d0 >= 0 &&
                     d0 + drafts <= A.num_drafts;
   const int n = (int)drafts, s0 = (int)start;
-  const bool greedy = !(temp >= kLowTemp);
-  const auto take = [&](int j) {                           // row j of the request
-    Row<T> w = row_of<T>(A, s0 + j, temp, greedy);
-    if constexpr (CHAIN) {
-      const bool drafted = j < n;
-      if (drafted) w.q = A.probs + (long long)(d0 + j) * A.ld_probs;
-      return resolve<true>(team, w, greedy, drafted, drafted ? A.draft_tokens[d0 + j] : -1,
-                           drafted ? number_at(A.uniforms, A.uniform_size, d0 + j) : 0., number_at(A.resample, A.uniform_size, b));
-    } else {
-      return resolve<false>(team, w, greedy, false, -1, 0., number_at(A.uniforms, A.uniform_size, s0 + j));
-    }
-  };
+  Row<T> w;
+  Asked a;
   if constexpr (FLAT) {
     const int j = blockIdx.y;
-    if (sane && j <= n) {
-      const RowResult r = take(j);
-      if (rank == 0 && threadIdx.x == 0) A.rows[s0 + j] = r;
-      cluster.sync();                                      // no CTA ends while another reads its shared memory
+    const bool live = sane && j <= n;
+    int holder = 0;
+    RowResult r{};
+    if (live) {
+      row_of<T, CHAIN>(A, b, d0, n, s0, j, temp, w, a);
+      r = resolve<CHAIN, true>(team, w, a, &holder);
     }
-    if (rank != 0) return;
-    if (threadIdx.x == 0) {
-      __threadfence();
-      const unsigned prev = atomicAdd(A.counter + b, 1u);
-      s_last = prev + 1 == gridDim.y;
-      if (s_last) { __threadfence(); A.counter[b] = 0u; }
+    if (rank == holder && threadIdx.x < 32) {              // count the row in, and tell the cluster if it was the last
+      int last = 0;
+      if (threadIdx.x == 0) {
+        if (live) A.rows[s0 + j] = r;
+        __threadfence();
+        last = atomicAdd(A.counter + b, 1u) + 1 == gridDim.y;
+        if (last) A.counter[b] = 0u;
+      }
+      last = __shfl_sync(0xffffffffu, last, 0);
+      if (threadIdx.x < ranks) *cluster.map_shared_rank(&sh.last, (int)threadIdx.x) = last;
     }
-    __syncthreads();
-    if (!s_last) return;
+    cluster.sync();
+    if (!sh.last) return;
     __threadfence();
-    if (sane)
-      for (int i = threadIdx.x; i <= n; i += kThreads) {
+  }
+  if (sane) {
+    for (int i = threadIdx.x; i <= n; i += kThreads) {
+      if constexpr (FLAT) {
         const RowResult* const r = A.rows + s0 + i;
         const int2 t = __ldcg(reinterpret_cast<const int2*>(r));
         s_row[i] = {t.x, t.y, __ldcg(&r->scaled), __ldcg(&r->mass)};
+        s_next[i] = n;
       }
+      if (!CHAIN && i < n) {
+        s_parent[i] = A.parents[d0 + i];
+        s_token[i] = A.draft_tokens[d0 + i];
+      }
+    }
+    __syncthreads();
+    if constexpr (FLAT && !CHAIN) {
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int up = s_parent[i] + 1;                    // the row that leads to node i
+        if (up >= 0 && up <= n && s_row[up].accept != kUndecided && s_row[up].token >= 0 && s_row[up].token == s_token[i])
+          atomicMin(s_next + up, i);
+      }
+      __syncthreads();
+    }
   }
   int pos = -1;                                            // the last token's place: accepted drafts
   if (sane) {
-    for (int i = threadIdx.x; !CHAIN && i < n; i += kThreads) {
-      s_parent[i] = A.parents[d0 + i];
-      s_token[i] = A.draft_tokens[d0 + i];
-    }
-    __syncthreads();
     int cur = -1;
     for (;;) {                                             // (every thread of every CTA takes the same steps)
       RowResult r;
-      if constexpr (FLAT) r = s_row[cur + 1];
-      else r = take(cur + 1);
+      bool known = FLAT;
+      if constexpr (FLAT) {
+        r = s_row[cur + 1];
+        if (r.accept == kUndecided) {
+          row_of<T, CHAIN>(A, b, d0, n, s0, cur + 1, temp, w, a);
+          if (threadIdx.x == 0) sh.top = (float)r.scaled;
+          __syncthreads();
+          r = exact_row(team, w, a);
+          team.ph ^= r.accept >> 8;
+          r.accept &= 1;
+          if (threadIdx.x == 0) s_row[cur + 1] = r;
+          known = false;
+        }
+      } else {
+        int holder;
+        row_of<T, CHAIN>(A, b, d0, n, s0, cur + 1, temp, w, a);
+        r = resolve<CHAIN, false>(team, w, a, &holder);
+      }
       ++pos;
       if (threadIdx.x == 0) {
         s_node[pos] = cur;
@@ -775,6 +812,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A,
       if (pos < A.max_spec && r.token >= 0) {
         if constexpr (CHAIN) {
           nxt = r.accept && cur + 1 < n ? cur + 1 : -1;
+        } else if (known) {
+          nxt = s_next[cur + 1] < n ? s_next[cur + 1] : -1;
         } else {                                           // the first child of cur that carries the token
           for (int i0 = 0; i0 < n && nxt < 0; i0 += 32) {
             const int i = i0 + (int)(threadIdx.x & 31);
@@ -786,8 +825,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A,
       if (nxt < 0) break;
       cur = nxt;
     }
-    if constexpr (!FLAT) cluster.sync();
-    __syncthreads();
+    cluster.sync();                                        // no CTA ends while another reads its shared memory
   }
   if (rank != 0) return;
   for (int p = threadIdx.x; p <= A.max_spec; p += kThreads) {
@@ -796,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A,
     if (p <= pos) {
       const RowResult r = s_row[FLAT ? s_node[p] + 1 : p];
       token = r.token;
-      if (token >= 0) logp = (float)(r.scaled * 0.6931471805599453 - log(r.mass));
+      if (token >= 0) logp = (float)(r.scaled * 0.6931471805599453) - log1pf((float)(r.mass - 1.));      // (mass >= 1)
     }
     A.out_tokens[(long long)b * (A.max_spec + 1) + p] = token;
     A.out_logp[(long long)b * (A.max_spec + 1) + p] = logp;
@@ -811,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A,
 
 template <typename T, bool CHAIN, bool FLAT>
 cfb_status launch(const VerifyArgs& a, int cluster, cudaStream_t st) {
-  const auto bytes = [](long long units, long long spec) { return (int)(units * 12 + (spec + 1) * 28 + spec * 8); };
+  const auto bytes = [](long long units, long long spec) { return (int)(units * (kUnit / kSpan<W64> * 8 + 4) + (spec + 1) * 32 + spec * 8); };
   const long long units = (a.V + 7 + kUnit - 1) / kUnit, most = (units + cluster - 1) / cluster + 1;
   if (allow_smem<verify_kernel<T, CHAIN, FLAT>>(bytes(kMaxVocab / kUnit + 2, kMaxNodes)) != cudaSuccess)
     return cfb_launch_status("verify_kernel");
