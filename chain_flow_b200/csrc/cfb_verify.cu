@@ -67,16 +67,14 @@ struct VerifyArgs {
 enum Kind : int { ROW_MASS = 0, ROW_EMPTY = 1, ROW_NAN = 2 };
 constexpr int kUndecided = 2;                              // RowResult::accept: fp32 did not decide (scaled: the row's largest)
 
-struct Pub { float top; int nan; double sum; };            // a CTA's part of a row
+struct Pub { float top; int nan; float sum; float pad; double sum64; };      // a CTA's part of a row
 struct Found { int token, unsure; float logit; int pad; };
 
 struct Shared {
   Pub pub[2];
   Found found[2];
-  double z;                  // sum of the row's weights
-  double whole;              // sum of what the last pass summed
-  double t;                  // the owner's: its part's threshold, in the scale of its sums
-  float band;                // and how near to it fp32 decides nothing
+  double z, whole;           // sum of the row's weights; of what the last pass summed
+  double before, end;        // the running sums of the last pass before this CTA's part and behind it
   float top;                 // of the row
   int kind;
   int owner;                 // the CTA whose part has the threshold, or (greedy rows) the first of the largest
@@ -86,6 +84,16 @@ struct Shared {
 CFB_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+CFB_DEV float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+CFB_DEV float reciprocal(float x) {                        // (a division takes 280 cycles)
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 CFB_DEV float warp_max(float v) {                          // NaN counts as nothing
@@ -129,8 +137,10 @@ CFB_DEV Pair mul2(Pair a, Pair b) {
   return p;
 }
 
-// A logits row: element i lies at p[i]. Vectors of 16 bytes start at element -shift, so that they are aligned.
+// A logits row: element i lies at p[i]. Vectors of 16 bytes start at element -shift, so that they are aligned. Units of kUnit
+// elements from there on; this CTA has [u0, u1) of them.
 template <typename T> struct Row {
+  int u0, u1;
   const T* p;
   int V, shift;
   float c;                    // log2(e) / tau
@@ -150,16 +160,24 @@ template <> CFB_DEV float lowest<float>() { return -INFINITY; }
 template <> CFB_DEV __half lowest<__half>() { return __ushort_as_half(0xfc00); }
 template <> CFB_DEV __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
 // elements [i, i + kE) as they lie in memory, -inf outside the row
-template <typename T> CFB_DEV uint4 load_vector(const Row<T>& w, int i) {
-  if (i >= 0 && i + kE<T> <= w.V) return __ldg(reinterpret_cast<const uint4*>(w.p + i));
+template <typename T> __device__ __noinline__ uint4 load_edge(const T* p, int V, int i) {
   union { uint4 v; T e[kE<T>]; } u;
 #pragma unroll
-  for (int e = 0; e < kE<T>; ++e) u.e[e] = i + e >= 0 && i + e < w.V ? w.p[i + e] : lowest<T>();
+  for (int e = 0; e < kE<T>; ++e) u.e[e] = i + e >= 0 && i + e < V ? p[i + e] : lowest<T>();
   return u.v;
 }
-template <typename T> CFB_DEV void load_unit(const Row<T>& w, int unit, int lane, uint4 (&u)[kVectors<T>]) {
+// N vectors, `step` elements apart from element i on, of a unit of `span` elements that starts at `first`
+template <int N, typename T> CFB_DEV void load_vectors(const Row<T>& w, int first, int span, int i, int step, uint4 (&u)[N]) {
+  if (first >= 0 && first + span <= w.V) {
 #pragma unroll
-  for (int j = 0; j < kVectors<T>; ++j) u[j] = load_vector(w, first_of(w, unit, j, lane));
+    for (int j = 0; j < N; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(w.p + i + j * step));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) u[j] = load_edge(w.p, w.V, i + j * step);
+  }
+}
+template <typename T> CFB_DEV void load_unit(const Row<T>& w, int unit, int lane, uint4 (&u)[kVectors<T>]) {
+  load_vectors(w, unit * kUnit - w.shift, kUnit, first_of(w, unit, 0, lane), 32 * kE<T>, u);
 }
 // element pair k (of kE / 2) of a vector
 template <typename T> CFB_DEV float2 pair_of(const uint4& v, int k) {
@@ -180,39 +198,38 @@ template <typename T> CFB_DEV float vector_max(const uint4& v) {
   }
 }
 
-// weights relative to a base: of a largest +inf the tokens that have it share the mass
-CFB_DEV float weight(float l, float base, float c) {
-  return l == base ? 1.f : isinf(base) ? 0.f : ex2((l - base) * c);
-}
-// 2^y for the weights in 64 bits, by a whole warp: y = k / 32 + r with |r| <= 1/64, the series of 2^r cut after r^5 (the first
-// term left out is 2 10^-15), 2^(k mod 32 / 32) from the lane that holds it. x: y in fp32; below 2^-1090 it is 0. The
-// library's function branches, which kept several from running side by side: a pass took 4 times as long.
+// the weight relative to a finite base
+CFB_DEV float weight(float l, float base, float c) { return ex2((l - base) * c); }
+// a sum's scale where a larger base takes over (of a largest +inf only what has it counts)
+CFB_DEV float rescale(float top, float base, float c) { return top == base ? 1.f : top == -INFINITY || base == INFINITY ? 0.f : weight(top, base, c); }
+
+// The weight 2^((l - base) c) in 64 bits, relative to a finite base, by a whole warp: with y = (l - base) c = k / 32 + r, |r| <= 1/64,
+// the series of 2^r cut after r^5 (the first term left out is 2 10^-15), times 2^(k mod 32 / 32) from the lane that holds
+// it. 0 below 2^-1020. The library's function branches, which kept several from running side by side: a pass took 4
+// times as long.
 CFB_DEV double exp2_table(int lane) { return exp2((double)lane * 0.03125); }
-CFB_DEV double exp2_neg(double y, float x, double table) {
-  const bool none = !(x > -1090.f);
-  y = none ? 0. : y;
-  const double magic = 6755399441055744.;                  // 1.5 2^52: adding it rounds to a whole number
-  const double shifted = fma(y, 32., magic), r = fma(shifted - magic, -0.03125, y);
-  const int k = __double2loint(shifted), n = k >> 5;
-  double p = 0x1.5d87fe78a6731p-10;                                           // ln2^k / k!
+// the fp32 number as a double, by its bits (conversions are slow): what is 0 becomes 2^-127, and an infinity 2^128
+template <typename T> CFB_DEV double widen(float f) {
+  const int b = __float_as_int(f);
+  return __hiloint2double(((b >> 3) & 0x8fffffff) + 0x38000000, sizeof(T) == 4 ? b << 29 : 0);
+}
+template <typename T> CFB_DEV double fast_weight64(float l, double base, double c, double table) {
+  const double d = widen<T>(l) - base, magic = 6755399441055744.;        // 1.5 2^52: adding it rounds to a whole number
+  const double y = d * c, shifted = fma(y, 32., magic), r = fma(shifted - magic, -0.03125, y);
+  const int k = __double2loint(shifted);
+  double p = 0x1.5d87fe78a6731p-10;                        // ln2^k / k!
   p = fma(p, r, 0x1.3b2ab6fba4e77p-7);
   p = fma(p, r, 0x1.c6b08d704a0c0p-5);
   p = fma(p, r, 0x1.ebfbdff82c58fp-3);
   p = fma(p, r, 0x1.62e42fefa39efp-1);
-  const double t = __shfl_sync(0xffffffffu, table, k & 31);
+  const double t = __shfl_sync(0xffffffffu, table, k);
   p = fma(p * r, t, t);
-  const int up = max(n, -1020);                            // (denormals in a second step)
-  p = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
-  if (n < -1020) p *= __hiloint2double((1023 + n + 1020) << 20, 0);
-  return none ? 0. : p;
+  p = __hiloint2double(__double2hiint(p) + ((k << 15) & 0xfff00000), __double2loint(p));
+  return y > -1020. ? p : 0.;
 }
-// the fp32 number as a double, by its bits (conversions are slow): what is 0 becomes 2^-127, and an infinity 2^128
-CFB_DEV double widen(float f) {
-  const uint32_t b = __float_as_uint(f);
-  return __hiloint2double((int)((b & 0x80000000u) | (((b >> 3) & 0x0fffffffu) + 0x38000000u)), (int)(b << 29));
-}
-CFB_DEV double weight64(float l, float base, double c64) {           // of one element
-  return l == base ? 1. : isinf(base) ? 0. : exp2(((double)l - (double)base) * c64);
+// by one thread, of any base, to the smallest denormal
+CFB_DEV double weight64(float l, float base, double c) {
+  return l == base ? 1. : isinf(base) ? 0. : exp2(((double)l - (double)base) * c);
 }
 // the draft probability of token i (0 outside the row and for what is not a positive number)
 template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
@@ -226,37 +243,30 @@ template <int MODE> constexpr bool kNarrow = MODE == W32 || MODE == R32;
 // elements of a summed unit, and a lane's of them: in 64 bits, where an element costs much more, smaller ones to scan
 template <int MODE> constexpr int kSpan = kNarrow<MODE> ? kUnit : 256;
 
-// an element's value, by a whole warp. iz: 1 / the row's sum of weights (R32, R64)
-template <int MODE, typename T> CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, double table) {
+// an element's value, by a whole warp. iz: 1 / the row's sum of weights (R32, R64). SLOW (64 bits): any base, denormals kept
+template <int MODE, bool SLOW, typename T>
+CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, double table) {
   if constexpr (MODE == W32) {
     return weight(l, base, w.c);
   } else if constexpr (MODE == R32) {
     return fmaxf(weight(l, base, w.c) * (float)iz - draft_prob(w, i), 0.f);
   } else {
-    const double e = exp2_neg((widen(l) - (double)base) * w.c64, (l - base) * w.c, table);
-    const double v = l == base ? 1. : isinf(base) ? 0. : e;
+    const double v = SLOW ? weight64(l, base, w.c64) : fast_weight64<T>(l, base, w.c64, table);
     if constexpr (MODE == W64) return v;
     else return fmax(v * iz - (double)draft_prob(w, i), 0.);
   }
 }
 
-// The part of a row that a CTA has: units [u0, u1) of it
-struct Span { int u0, u1; };
-template <typename T> CFB_DEV Span span_of(const Row<T>& w, int rank, int ranks) {
-  const int units = (w.V + w.shift + kUnit - 1) / kUnit;
-  return {(int)((long long)units * rank / ranks), (int)((long long)units * (rank + 1) / ranks)};
-}
-
 // every unit's largest and its sum of weights relative to that; a unit's loads are under way while the one before is summed
-template <typename T> CFB_DEV void stats_units(const Row<T>& w, Span s, float* tops, float* sums) {
+template <typename T> CFB_DEV void stats_units(const Row<T>& w, float* tops, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint4 next[kVectors<T>];
-  if (s.u0 + warp < s.u1) load_unit(w, s.u0 + warp, lane, next);
-  for (int u = s.u0 + warp; u < s.u1; u += kWarps) {
+  if (w.u0 + warp < w.u1) load_unit(w, w.u0 + warp, lane, next);
+  for (int u = w.u0 + warp; u < w.u1; u += kWarps) {
     uint4 v[kVectors<T>];
 #pragma unroll
     for (int j = 0; j < kVectors<T>; ++j) v[j] = next[j];
-    if (u + kWarps < s.u1) load_unit(w, u + kWarps, lane, next);
+    if (u + kWarps < w.u1) load_unit(w, u + kWarps, lane, next);
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVectors<T>; ++j) m = fmaxf(m, vector_max<T>(v[j]));
@@ -288,8 +298,8 @@ template <typename T> CFB_DEV void stats_units(const Row<T>& w, Span s, float* t
     }
     sum = warp_sum(sum);
     if (lane == 0) {
-      tops[u - s.u0] = top;
-      sums[u - s.u0] = sum;
+      tops[u - w.u0] = top;
+      sums[u - w.u0] = sum;
     }
   }
 }
@@ -310,9 +320,9 @@ template <typename F> CFB_DEV void table_entries(const F* t, int i, int n, int V
 }
 
 // every unit's sum of what is left above q
-template <typename T> CFB_DEV void rest_units(const Row<T>& w, Span s, float base, float iz, float* sums) {
+template <typename T> CFB_DEV void rest_units(const Row<T>& w, float base, float iz, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int u = s.u0 + warp; u < s.u1; u += kWarps) {
+  for (int u = w.u0 + warp; u < w.u1; u += kWarps) {
     uint4 v[kVectors<T>];
     load_unit(w, u, lane, v);
     float a[2] = {0.f, 0.f};
@@ -336,29 +346,30 @@ template <typename T> CFB_DEV void rest_units(const Row<T>& w, Span s, float bas
       }
     }
     const float sum = warp_sum(a[0] + a[1]);
-    if (lane == 0) sums[u - s.u0] = sum;
+    if (lane == 0) sums[u - w.u0] = sum;
   }
 }
 // every unit's sum in 64 bits: a lane has 8 neighbours of 256
-template <int MODE, typename T>
-CFB_DEV void exact_units(const Row<T>& w, Span s, float base, double iz, double table, double* sums) {
+template <int MODE, bool SLOW, typename T>
+CFB_DEV void exact_units(const Row<T>& w, float base, double iz, double* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kPer = kUnit / kSpan<MODE>;
-  for (int u = s.u0 * kPer + warp; u < s.u1 * kPer; u += kWarps) {
-    const int i = u * kSpan<MODE> + lane * 8 - w.shift;
+  const double table = exp2_table(lane);
+  constexpr int kPer = kUnit / kSpan<MODE>, N = 8 / kE<T>;
+  for (int u = w.u0 * kPer + warp; u < w.u1 * kPer; u += kWarps) {
+    const int first = u * kSpan<MODE> - w.shift, i = first + lane * 8;
+    uint4 v[N];
+    load_vectors(w, first, kSpan<MODE>, i, kE<T>, v);
     double a[2] = {0., 0.};
-#pragma unroll
-    for (int j = 0; j < 8 / kE<T>; ++j) {
-      const uint4 v = load_vector(w, i + j * kE<T>);
-#pragma unroll
+#pragma unroll SLOW ? 1 : N
+    for (int j = 0; j < N; ++j)
+#pragma unroll SLOW ? 1 : kE<T> / 2
       for (int k = 0; k < kE<T> / 2; ++k) {
-        const float2 l = pair_of<T>(v, k);
-        a[0] += value_of<MODE>(w, l.x, i + j * kE<T> + 2 * k, base, iz, table);
-        a[1] += value_of<MODE>(w, l.y, i + j * kE<T> + 2 * k + 1, base, iz, table);
+        const float2 l = pair_of<T>(v[j], k);
+        a[0] += value_of<MODE, SLOW>(w, l.x, i + j * kE<T> + 2 * k, base, iz, table);
+        a[1] += value_of<MODE, SLOW>(w, l.y, i + j * kE<T> + 2 * k + 1, base, iz, table);
       }
-    }
     const double sum = warp_sum(a[0] + a[1]);
-    if (lane == 0) sums[u - s.u0 * kPer] = sum;
+    if (lane == 0) sums[u - w.u0 * kPer] = sum;
   }
 }
 
@@ -376,10 +387,11 @@ template <typename F> CFB_DEV F run_up(F* sums, int n, int lane) {
 
 // Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start): by units, by lanes
 // of neighbours, by a lane's elements. band: for all but the unit's own rounding.
-template <int MODE, typename T, typename F>
-CFB_DEV Found find(const Row<T>& w, Span s, const F* sums, F t, float base, double iz, float band) {
+template <int MODE, bool SLOW, typename T, typename F>
+CFB_DEV Found find(const Row<T>& w, const F* sums, F t, float base, double iz, float band) {
   constexpr int kPer = kUnit / kSpan<MODE>, kLane = kSpan<MODE> / 32;   // summed units a unit; a lane's elements
-  const int lane = threadIdx.x & 31, n = (s.u1 - s.u0) * kPer;
+  constexpr int N = kLane / kE<T>;
+  const int lane = threadIdx.x & 31, n = (w.u1 - w.u0) * kPer;
   const double table = kNarrow<MODE> ? 0. : exp2_table(lane);
   int u = -1;
   for (int i0 = 0; i0 < n && u < 0; i0 += 32) {
@@ -396,23 +408,20 @@ CFB_DEV Found find(const Row<T>& w, Span s, const F* sums, F t, float base, doub
     }
     if (u < 0) return {-1, 1, 0.f, 0};
   }
-  const int first = s.u0 * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
+  const int first = w.u0 * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
+  uint4 x[N];
+  load_vectors(w, first, kSpan<MODE>, i0, kE<T>, x);
   F a = 0;
-#pragma unroll
-  for (int j = 0; j < kLane / kE<T>; ++j) {
-    const uint4 x = load_vector(w, i0 + j * kE<T>);
-    F v[kE<T>];
-#pragma unroll
+#pragma unroll SLOW ? 1 : N
+  for (int j = 0; j < N; ++j) {
+    F v[4] = {0, 0, 0, 0};
+#pragma unroll SLOW ? 1 : kE<T> / 2
     for (int k = 0; k < kE<T> / 2; ++k) {
-      const float2 l = pair_of<T>(x, k);
-      v[2 * k] = value_of<MODE>(w, l.x, i0 + j * kE<T> + 2 * k, base, iz, table);
-      v[2 * k + 1] = value_of<MODE>(w, l.y, i0 + j * kE<T> + 2 * k + 1, base, iz, table);
+      const float2 l = pair_of<T>(x[j], k);
+      v[k] = value_of<MODE, SLOW>(w, l.x, i0 + j * kE<T> + 2 * k, base, iz, table);
+      v[k] += value_of<MODE, SLOW>(w, l.y, i0 + j * kE<T> + 2 * k + 1, base, iz, table);
     }
-#pragma unroll
-    for (int e = kE<T>; e > 1; e >>= 1)
-#pragma unroll
-      for (int k = 0; k < e / 2; ++k) v[k] = v[2 * k] + v[2 * k + 1];
-    a += v[0];
+    a += (v[0] + v[1]) + (v[2] + v[3]);
   }
   const F before = u ? sums[u - 1] : (F)0, at = t - before, mass = sums[u] - before;
   const F scan = warp_scan(a, lane), up = __shfl_up_sync(0xffffffffu, scan, 1);
@@ -427,7 +436,7 @@ CFB_DEV Found find(const Row<T>& w, Span s, const F* sums, F t, float base, doub
   const int who = __ffs(hit) - 1, i = first + who * kLane + lane;
   const F head = who ? __shfl_sync(0xffffffffu, up, who) : (F)0;
   const float l = lane < kLane && i >= 0 && i < w.V ? to_float(w.p[i]) : -INFINITY;
-  const F y = value_of<MODE>(w, l, lane < kLane ? i : -1, base, iz, table), run = head + warp_scan(y, lane);
+  const F y = value_of<MODE, SLOW>(w, l, lane < kLane ? i : -1, base, iz, table), run = head + warp_scan(y, lane);
   hit = __ballot_sync(0xffffffffu, y > 0 && run > at);
   if (!hit) {
     unsure = true;
@@ -444,13 +453,13 @@ CFB_DEV Found find(const Row<T>& w, Span s, const F* sums, F t, float base, doub
 
 // Warp 0: the first element that equals the row's largest (or the first NaN)
 template <typename T>
-CFB_DEV int find_top(const Row<T>& w, Span s, const float* tops, const float* sums, float top, bool nan) {
-  const int lane = threadIdx.x & 31, n = s.u1 - s.u0;
+__device__ __noinline__ int find_top(Row<T> w, const float* tops, const float* sums, float top, bool nan) {
+  const int lane = threadIdx.x & 31, n = w.u1 - w.u0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int k = i0 + lane;
     const unsigned hit = __ballot_sync(0xffffffffu, k < n && (nan ? sums[k] != sums[k] : tops[k] == top));
     if (!hit) continue;
-    const int u = s.u0 + i0 + __ffs(hit) - 1;
+    const int u = w.u0 + i0 + __ffs(hit) - 1;
     uint4 v[kVectors<T>];
     load_unit(w, u, lane, v);
     int best = 0x7fffffff;
@@ -475,27 +484,30 @@ template <typename T> struct Team {
   void* room;                // the units' sums
   int rank, ranks, ph;
 
-  // How far an fp32 sum over the row may be from its side of a threshold, as a share of the row's mass
-  CFB_DEV float band(const Row<T>& w) const { return (float)kRound * (2.08f * __log2f((float)w.V / (float)sh->z) + 20.f); }
+  // How far an fp32 sum over the row may be from its side of a threshold, as a share of the row's mass z
+  CFB_DEV float band(const Row<T>& w, float z) const {
+    return (float)kRound * (2.08f * (lg2((float)w.V) - lg2(z)) + 20.f);
+  }
 
   // The CTAs' totals, handed over by the cluster's barrier -> the row's; who has the threshold u of it. SCALED: each
   // total is relative to its CTA's largest; greedy: the owner is the first that has the row's largest.
-  template <typename F, bool SCALED> CFB_DEV void exchange(const Row<T>& w, double u, bool greedy, bool rest) {
+  template <typename F, bool SCALED> CFB_DEV void exchange(const Row<T>& w, F u, bool greedy) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
-      Pub p{-INFINITY, 0, 0.};
+      Pub p{-INFINITY, 0, 0.f, 0.f, 0.};
       if (lane < ranks) p = *cluster.map_shared_rank(&sh->pub[ph], lane);
-      F scale = 1;
+      F m;
+      if constexpr (sizeof(F) == 8) m = p.sum64;
+      else m = p.sum;
       bool nan = false;
-      float top = sh->top;
+      float top = 0.f;
       if constexpr (SCALED) {
         top = warp_max(p.top);
         nan = __any_sync(0xffffffffu, p.nan);
-        scale = p.top == -INFINITY ? 0.f : weight(p.top, top, w.c);
+        m *= rescale(p.top, top, w.c);
       }
-      const F own = (F)p.sum, m = own * scale;
       F scan = m;
 #pragma unroll
       for (int off = 1; off < kMaxCluster; off <<= 1) {
@@ -505,19 +517,13 @@ template <typename T> struct Team {
       const F whole = __shfl_sync(0xffffffffu, scan, kMaxCluster - 1);
       // (the sum before, not the one behind less this part's, which would lose small ones)
       const F up = __shfl_up_sync(0xffffffffu, scan, 1), before = lane ? up : (F)0;
-      const F most = whole * (F)(sizeof(F) == 4 ? 1. - 1.2e-7 : 1. - 2.3e-16), raw = (F)(u * (double)whole), t = raw < most ? raw : most;
+      const F t = threshold(u, whole);
       unsigned hit = __ballot_sync(0xffffffffu, m > 0 && before <= t && t < scan);
       if (!hit) hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, m > 0) | 1u));
       if (SCALED && (greedy || nan)) hit = __ballot_sync(0xffffffffu, nan ? p.nan != 0 : p.top == top);
       if (lane == rank) {
-        sh->t = (double)((t - before) / scale);
-        // (of what is left above q, the error is that of the probabilities, whose whole is 1)
-        if (SCALED || rest) {
-          const float z = SCALED ? (float)whole : (float)sh->z;
-          const float row = (float)kRound * (2.08f * __log2f((float)w.V / z) + 20.f);
-          const int n = ((w.V + kUnit - 1) / kUnit + ranks - 1) / ranks;
-          sh->band = (rest ? row + 24.f * (float)kRound : row * (float)whole / (float)scale) + (float)kRound * (8 + n / 32) * (float)own;
-        }
+        sh->before = before;
+        sh->end = scan;
       }
       if (lane == 0) {
         sh->owner = __ffs(hit) - 1;
@@ -531,16 +537,17 @@ template <typename T> struct Team {
     }
     __syncthreads();
   }
+  static CFB_DEV float threshold(float u, float whole) { return fminf(u * whole, whole * (1.f - 0x1p-23f)); }
+  static CFB_DEV double threshold(double u, double whole) { return fmin(u * whole, whole * (1. - 0x1p-52)); }
 
   // the pass over the row
   CFB_DEV void stats(const Row<T>& w, double u, bool greedy) {
-    const Span s = span_of(w, rank, ranks);
     float* const sums = static_cast<float*>(room);
-    stats_units(w, s, tops, sums);
+    stats_units(w, tops, sums);
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) {
-      const int lane = threadIdx.x, n = s.u1 - s.u0;
+      const int lane = threadIdx.x, n = w.u1 - w.u0;
       float top = -INFINITY;
       bool nan = false;
       for (int i = lane; i < n; i += 32) {
@@ -549,55 +556,68 @@ template <typename T> struct Team {
       }
       top = warp_max(top);
       nan = __any_sync(0xffffffffu, nan);
-      float sum = 0.f;
-      if (!nan) {
-        for (int i = lane; i < n; i += 32) sums[i] *= tops[i] == -INFINITY ? 0.f : weight(tops[i], top, w.c);
-        __syncwarp();
-        sum = run_up(sums, n, lane);
+      float before = 0.f;                                  // the units' sums become running ones, relative to the CTA's largest
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        const float v = warp_scan(i < n && !nan ? sums[i] * rescale(tops[i], top, w.c) : 0.f, lane);
+        if (i < n && !nan) sums[i] = before + v;
+        before += __shfl_sync(0xffffffffu, v, 31);
       }
-      if (lane == 0) sh->pub[ph] = {top, nan, (double)sum};
+      if (lane == 0) sh->pub[ph] = {top, nan, before, 0.f, 0.};
     }
-    exchange<float, true>(w, u, greedy, false);
+    exchange<float, true>(w, (float)u, greedy);
   }
 
   // a pass that knows the row's largest, and its sum where it needs it
-  template <int MODE> CFB_DEV void pass(const Row<T>& w, double u) {
-    using F = typename std::conditional<kNarrow<MODE>, float, double>::type;
-    const Span s = span_of(w, rank, ranks);
-    F* const sums = static_cast<F*>(room);
-    if constexpr (MODE == R32) rest_units(w, s, sh->top, 1.f / (float)sh->z, sums);
-    else exact_units<MODE>(w, s, sh->top, MODE == R64 ? 1. / sh->z : 0., exp2_table(threadIdx.x & 31), sums);
+  CFB_DEV void rest_pass(const Row<T>& w, double u) {
+    float* const sums = static_cast<float*>(room);
+    rest_units(w, sh->top, reciprocal((float)sh->z), sums);
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) {
-      const F sum = run_up(sums, (s.u1 - s.u0) * (kUnit / kSpan<MODE>), (int)threadIdx.x);
-      if (threadIdx.x == 0) sh->pub[ph] = {sh->top, 0, (double)sum};
+      const float sum = run_up(sums, w.u1 - w.u0, (int)threadIdx.x);
+      if (threadIdx.x == 0) sh->pub[ph].sum = sum;
     }
-    exchange<F, false>(w, u, false, MODE == R32);
+    exchange<float, false>(w, (float)u, false);
+  }
+  template <int MODE, bool SLOW> CFB_DEV void exact_pass(const Row<T>& w, double u) {
+    double* const sums = static_cast<double*>(room);
+    exact_units<MODE, SLOW>(w, sh->top, MODE == R64 ? 1. / sh->z : 0., sums);
+    __syncthreads();
+    ph ^= 1;
+    if (threadIdx.x < 32) {
+      const double sum = run_up(sums, (w.u1 - w.u0) * (kUnit / kSpan<MODE>), (int)threadIdx.x);
+      if (threadIdx.x == 0) sh->pub[ph].sum64 = sum;
+    }
+    exchange<double, false>(w, u, false);
   }
 
   // Warp 0 of the owner: the token of the last pass's threshold
-  template <int MODE> CFB_DEV Found found(const Row<T>& w) const {
-    using F = typename std::conditional<kNarrow<MODE>, float, double>::type;
-    return find<MODE>(w, span_of(w, rank, ranks), static_cast<const F*>(room), (F)sh->t, MODE == W32 ? sh->pub[ph].top : sh->top,
-                      MODE == R32 ? (double)(1.f / (float)sh->z) : MODE == R64 ? 1. / sh->z : 0., sh->band);
+  CFB_DEV Found found(const Row<T>& w, double u) const {
+    const float top = sh->pub[ph].top, scale = rescale(sh->top, top, w.c);        // (1 / what the part's sums were scaled by)
+    const float whole = (float)sh->whole, own = (float)(sh->end - sh->before) * scale;
+    if (isinf(top) || !(scale < INFINITY)) return {-1, 1, 0.f, 0};                 // several of +inf: in 64 bits
+    return find<W32, false>(w, static_cast<const float*>(room), (threshold((float)u, whole) - (float)sh->before) * scale, top, 0.,
+                            band(w, whole) * whole * scale + (float)kRound * (8 + (w.u1 - w.u0) / 32) * own);
   }
-  CFB_DEV Found found_top(const Row<T>& w) const {
-    const int t = find_top(w, span_of(w, rank, ranks), tops, static_cast<const float*>(room), sh->top, sh->kind == ROW_NAN);
-    return {t, 0, sh->top, 0};
+  CFB_DEV Found found_rest(const Row<T>& w, double u) const {
+    // (of what is left above q, the error is that of the probabilities, whose whole is 1)
+    const float whole = (float)sh->whole, z = (float)sh->z, off = band(w, z) + 24 * (float)kRound;
+    if (!(whole > 2.f * off)) return {-1, 1, 0.f, 0};
+    return find<R32, false>(w, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before, sh->top,
+                            (double)reciprocal(z), off + (float)kRound * (8 + (w.u1 - w.u0) / 32) * whole);
+  }
+  template <int MODE, bool SLOW> CFB_DEV Found found64(const Row<T>& w, double u) const {
+    return find<MODE, SLOW>(w, static_cast<const double*>(room), threshold(u, sh->whole) - sh->before, sh->top,
+                            MODE == R64 ? 1. / sh->z : 0., 0.f);
   }
 
   // Warp 0 of the owner hands what it found to all
-  CFB_DEV Found share(Found f) {
+  CFB_DEV Found share(const Found& f) {
     cg::cluster_group cluster = cg::this_cluster();
     if (rank == sh->owner && threadIdx.x < ranks) *cluster.map_shared_rank(&sh->found[ph], (int)threadIdx.x) = f;
     cluster.sync();
     return sh->found[ph];
-  }
-  template <int MODE> CFB_DEV Found draw(const Row<T>& w) {
-    Found f{-1, 1, 0.f, 0};
-    if (rank == sh->owner && threadIdx.x < 32) f = found<MODE>(w);
-    return share(f);
   }
 };
 
@@ -606,36 +626,44 @@ struct Asked { bool greedy, drafted; int draft; double u, v; };
 
 // The row decided in 64 bits, its largest in sh.top. Every thread of the cluster gets the result (in bit 8 of accept,
 // whether the exchanged buffers have been alternated).
-template <typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
+template <bool CHAIN, bool SLOW, typename T> CFB_DEV RowResult exact_steps(Team<T> team, const Row<T>& w, const Asked& a) {
   Shared& sh = *team.sh;
   const int ph = team.ph;
-  const auto scaled = [&](float l) { return l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64; };
   const auto result = [&](int token, int accept, float l) {
-    return RowResult{token, accept | (team.ph ^ ph) << 8, scaled(l), sh.z};
+    const double scaled = l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64;
+    return RowResult{token, accept | (team.ph ^ ph) << 8, scaled, sh.z};
   };
-  const auto sum = [&] {
-    team.template pass<W64>(w, a.v);
+  Found f{-1, 1, 0.f, 0};
+  bool rest = false;
+  for (;;) {
+    team.template exact_pass<W64, SLOW>(w, a.v);
     if (threadIdx.x == 0) sh.z = sh.whole;
     __syncthreads();
-  };
-  sum();
-  Found f;
-  if (a.drafted) {
-    if (a.draft >= 0 && a.draft < w.V) {
-      const float l = to_float(w.p[a.draft]);
-      if (a.u * (double)draft_prob(w, a.draft) < weight64(l, sh.top, w.c64) / sh.z) return result(a.draft, 1, l);
+    if constexpr (CHAIN) {
+      if (a.drafted && !rest) {
+        if (a.draft >= 0 && a.draft < w.V) {
+          const float l = to_float(w.p[a.draft]);
+          if (a.u * (double)draft_prob(w, a.draft) < weight64(l, sh.top, w.c64) / sh.z) return result(a.draft, 1, l);
+        }
+        team.template exact_pass<R64, SLOW>(w, a.v);
+        if (sh.whole > 0.) {
+          if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<R64, SLOW>(w, a.v);
+          break;
+        }
+        rest = true;                                       // nothing above q: the target's own
+        continue;
+      }
     }
-    team.template pass<R64>(w, a.v);
-    if (sh.whole > 0.) {
-      f = team.template draw<R64>(w);
-    } else {                                               // nothing above q: the target's own
-      sum();
-      f = team.template draw<W64>(w);
-    }
-  } else {
-    f = team.template draw<W64>(w);
+    if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<W64, SLOW>(w, a.v);
+    break;
   }
+  f = team.share(f);
   return result(f.token, 0, f.logit);
+}
+template <bool CHAIN, typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
+  // (weights below 2^-1020 count where the threshold is that small, and only there)
+  return isinf(team.sh->top) || a.v < 0x1p-900 || (CHAIN && a.u < 0x1p-900) ? exact_steps<CHAIN, true>(team, w, a)
+                                                                            : exact_steps<CHAIN, false>(team, w, a);
 }
 
 // One row, by a whole cluster. LAZY: what fp32 does not decide is left undecided, and the result is valid in warp 0 of
@@ -651,31 +679,30 @@ CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, const Asked& a, int* h
   if (sh.kind == ROW_EMPTY) return {-1, 0, 0., 1.};
   Found f{-1, 1, 0.f, 0};
   const bool plain = a.greedy || sh.kind == ROW_NAN;
+  bool unsure = false;
   if (CHAIN && a.drafted && !plain) {
     if (in) {
-      const float x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) / (float)sh.z, uq = (float)a.u * q;
+      const float z = (float)sh.z, x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) * reciprocal(z), uq = (float)a.u * q;
       // (every CTA computes the same)
-      const float off = p * (2.f * team.band(w) + (float)kRound * (2.08f * fabsf(x) + 12.f));
-      if (!(fabsf(uq - p) > off)) {
-        if constexpr (LAZY) return {-1, kUndecided, (double)sh.top, 1.};
-        const RowResult r = exact_row(team, w, a);
-        team.ph ^= r.accept >> 8;
-        return {r.token, r.accept & 1, r.scaled, r.mass};
-      }
-      if (uq < p) return {a.draft, 1, scaled(of_draft), sh.z};
+      const float off = p * (2.f * team.band(w, z) + (float)kRound * (2.08f * fabsf(x) + 16.f));
+      unsure = !(fabsf(uq - p) > off);
+      if (!unsure && uq < p) return {a.draft, 1, scaled(of_draft), sh.z};
     }
-    team.template pass<R32>(w, a.v);
+    if (!unsure) team.rest_pass(w, a.v);
   }
-  *holder = sh.owner;
-  if (team.rank == sh.owner && threadIdx.x < 32) {
-    if (plain) f = team.found_top(w);
-    else if (!CHAIN || !a.drafted) f = team.template found<W32>(w);
-    else if (sh.whole > 2. * (team.band(w) + 24 * kRound)) f = team.template found<R32>(w);
+  if (!unsure) {
+    *holder = sh.owner;
+    if (team.rank == sh.owner && threadIdx.x < 32) {
+      if (plain) f = {find_top(w, team.tops, static_cast<const float*>(team.room), sh.top, sh.kind == ROW_NAN), 0, sh.top, 0};
+      else if (!CHAIN || !a.drafted) f = team.found(w, a.v);
+      else f = team.found_rest(w, a.v);
+    }
+    if constexpr (!LAZY) f = team.share(f);
+    unsure = f.unsure;
   }
-  if constexpr (!LAZY) f = team.share(f);
-  if (f.unsure) {
+  if (unsure) {
     if constexpr (LAZY) return {-1, kUndecided, (double)sh.top, 1.};
-    const RowResult r = exact_row(team, w, a);
+    const RowResult r = exact_row<CHAIN>(team, w, a);
     team.ph ^= r.accept >> 8;
     return {r.token, r.accept & 1, r.scaled, r.mass};
   }
@@ -689,10 +716,13 @@ CFB_DEV double number_at(const void* p, int size, long long i) {
 
 // row j of request b, and what it is asked
 template <typename T, bool CHAIN>
-CFB_DEV void row_of(const VerifyArgs& A, int b, int d0, int n, int s0, int j, float temp, Row<T>& w, Asked& a) {
+CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n, int s0, int j, float temp, Row<T>& w, Asked& a) {
   w.p = static_cast<const T*>(A.logits) + (long long)(s0 + j) * A.ld;
   w.V = A.V;
   w.shift = (int)((reinterpret_cast<uintptr_t>(w.p) & 15) / sizeof(T));
+  const int units = (w.V + w.shift + kUnit - 1) / kUnit;
+  w.u0 = min(rank * per, units);
+  w.u1 = min(w.u0 + per, units);
   a.greedy = !(temp >= kLowTemp);
   const float tau = a.greedy ? 1.f : fminf(temp, kHighTemp);
   w.c64 = tau == 1.f ? 1.4426950408889634 : 1.4426950408889634 / (double)tau;
@@ -710,14 +740,14 @@ CFB_DEV void row_of(const VerifyArgs& A, int b, int d0, int n, int s0, int j, fl
 // cluster walks, and decides the rows that its walk meets undecided. Otherwise a cluster a request (grid.y), which
 // takes the rows of its walk in turn. CHAIN: draft probabilities; a node's only child is the next one.
 template <typename T, bool CHAIN, bool FLAT>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs A, int most) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs A, int per) {
   extern __shared__ double s_dyn[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   // what a walk keeps: the results of its rows (in turn, or FLAT: of all rows), the rows it took, the tree
   constexpr int kPer = kUnit / kSpan<W64>;
-  RowResult* const s_row = reinterpret_cast<RowResult*>(s_dyn + kPer * most);
+  RowResult* const s_row = reinterpret_cast<RowResult*>(s_dyn + kPer * per);
   int* const s_node = reinterpret_cast<int*>(s_row + A.max_spec + 1);
   int* const s_next = s_node + A.max_spec + 1;             // FLAT: the child that a row's token leads to
   int* const s_parent = s_next + A.max_spec + 1;
@@ -731,6 +761,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   const bool sane = drafts >= 0 && drafts <= A.max_spec && start >= 0 && start + drafts < A.num_rows && d0 >= 0 &&
                     d0 + drafts <= A.num_drafts;
   const int n = (int)drafts, s0 = (int)start;
+  // a thread's node of the tree, on its way while the rows are taken
+  const bool node = !CHAIN && sane && (int)threadIdx.x < n;
+  const int my_parent = node ? A.parents[d0 + threadIdx.x] : 0, my_token = node ? A.draft_tokens[d0 + threadIdx.x] : 0;
   Row<T> w;
   Asked a;
   if constexpr (FLAT) {
@@ -739,15 +772,14 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     int holder = 0;
     RowResult r{};
     if (live) {
-      row_of<T, CHAIN>(A, b, d0, n, s0, j, temp, w, a);
+      row_of<T, CHAIN>(A, rank, per, b, d0, n, s0, j, temp, w, a);
       r = resolve<CHAIN, true>(team, w, a, &holder);
     }
     if (rank == holder && threadIdx.x < 32) {              // count the row in, and tell the cluster if it was the last
       int last = 0;
       if (threadIdx.x == 0) {
         if (live) A.rows[s0 + j] = r;
-        __threadfence();
-        last = atomicAdd(A.counter + b, 1u) + 1 == gridDim.y;
+        last = atom_add_acqrel(A.counter + b, 1u) + 1 == gridDim.y;
         if (last) A.counter[b] = 0u;
       }
       last = __shfl_sync(0xffffffffu, last, 0);
@@ -755,7 +787,6 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     }
     cluster.sync();
     if (!sh.last) return;
-    __threadfence();
   }
   if (sane) {
     for (int i = threadIdx.x; i <= n; i += kThreads) {
@@ -766,8 +797,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
         s_next[i] = n;
       }
       if (!CHAIN && i < n) {
-        s_parent[i] = A.parents[d0 + i];
-        s_token[i] = A.draft_tokens[d0 + i];
+        s_parent[i] = i < kThreads ? my_parent : A.parents[d0 + i];
+        s_token[i] = i < kThreads ? my_token : A.draft_tokens[d0 + i];
       }
     }
     __syncthreads();
@@ -781,6 +812,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     }
   }
   int pos = -1;                                            // the last token's place: accepted drafts
+  bool remote = !FLAT;                                     // others may be reading this CTA's shared memory
   if (sane) {
     int cur = -1;
     for (;;) {                                             // (every thread of every CTA takes the same steps)
@@ -789,18 +821,19 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       if constexpr (FLAT) {
         r = s_row[cur + 1];
         if (r.accept == kUndecided) {
-          row_of<T, CHAIN>(A, b, d0, n, s0, cur + 1, temp, w, a);
+          row_of<T, CHAIN>(A, rank, per, b, d0, n, s0, cur + 1, temp, w, a);
           if (threadIdx.x == 0) sh.top = (float)r.scaled;
           __syncthreads();
-          r = exact_row(team, w, a);
+          r = exact_row<CHAIN>(team, w, a);
           team.ph ^= r.accept >> 8;
           r.accept &= 1;
           if (threadIdx.x == 0) s_row[cur + 1] = r;
           known = false;
+          remote = true;
         }
       } else {
         int holder;
-        row_of<T, CHAIN>(A, b, d0, n, s0, cur + 1, temp, w, a);
+        row_of<T, CHAIN>(A, rank, per, b, d0, n, s0, cur + 1, temp, w, a);
         r = resolve<CHAIN, false>(team, w, a, &holder);
       }
       ++pos;
@@ -825,7 +858,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       if (nxt < 0) break;
       cur = nxt;
     }
-    cluster.sync();                                        // no CTA ends while another reads its shared memory
+    if (remote) cluster.sync();                            // no CTA ends while another reads its shared memory
+    __syncthreads();
   }
   if (rank != 0) return;
   for (int p = threadIdx.x; p <= A.max_spec; p += kThreads) {
@@ -850,13 +884,13 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
 template <typename T, bool CHAIN, bool FLAT>
 cfb_status launch(const VerifyArgs& a, int cluster, cudaStream_t st) {
   const auto bytes = [](long long units, long long spec) { return (int)(units * (kUnit / kSpan<W64> * 8 + 4) + (spec + 1) * 32 + spec * 8); };
-  const long long units = (a.V + 7 + kUnit - 1) / kUnit, most = (units + cluster - 1) / cluster + 1;
+  const long long units = (a.V + 7 + kUnit - 1) / kUnit, per = (units + cluster - 1) / cluster;
   if (allow_smem<verify_kernel<T, CHAIN, FLAT>>(bytes(kMaxVocab / kUnit + 2, kMaxNodes)) != cudaSuccess)
     return cfb_launch_status("verify_kernel");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = FLAT ? dim3(cluster, a.max_spec + 1, a.batch) : dim3(cluster, a.batch, 1);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = bytes(most, a.max_spec);
+  cfg.dynamicSmemBytes = bytes(per, a.max_spec);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -864,7 +898,7 @@ cfb_status launch(const VerifyArgs& a, int cluster, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, verify_kernel<T, CHAIN, FLAT>, a, (int)most);
+  cudaLaunchKernelEx(&cfg, verify_kernel<T, CHAIN, FLAT>, a, (int)per);
   return cfb_launch_status("verify_kernel");
 }
 
