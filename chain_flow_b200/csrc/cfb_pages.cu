@@ -8,12 +8,15 @@
 // The free pages of a pool are those whose count is 0, and a call takes the lowest of them, request after
 // request, so that its result does not depend on any order of execution. One CTA finds them: it turns the
 // counts into a bit a page in shared memory (32 loads in flight a thread), counts the bits, and then gives
-// every page that is asked for a thread, which looks up its request and its free page by bisection.
+// every page that is asked for a thread, which looks up its request and its free page by bisection. Of a large pool a
+// cluster of 8 CTAs does that, an eighth of the counts and of the pages each.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include "cfb_types.cuh"
 
 using namespace cfb;
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -28,9 +31,6 @@ struct Layers {                              // caches of one geometry
   int size, pieces;                          // bytes an element, log2 of a row's 16-byte pieces
 };
 
-__device__ __forceinline__ long long row_bytes(const Layers& L, long long page, long long off) {
-  return (page * L.c.page_stride + off * L.c.slot_stride) * L.size;
-}
 
 // ---- accepted rows ----------------------------------------------------------------------------------
 struct KeepArgs {
@@ -39,66 +39,77 @@ struct KeepArgs {
   int max_len, heads;                        // heads a CTA
 };
 
-// A CTA: a request (x), a layer's keys or values (y), a group of heads (z). The rows of a batch are all read
-// before the first is written; a later batch reads rows behind every one that was written, since a path's
-// j-th node is not before j.
-__global__ void __launch_bounds__(kThreads) kv_keep_kernel(const __grid_constant__ Layers L, const KeepArgs A) {
-  __shared__ long long s_src[kMaxPath], s_dst[kMaxPath];     // flat slots, or -1
-  const int b = blockIdx.x, n = min(max(A.count[b], 0), A.max_len);
-  if (n == 0) return;
+// A CTA: a request (x), a layer (y), a group of heads (z). The rows of a batch are all read before the first is written; a
+// later batch reads rows behind every one that was written, since a path's j-th node is not before j.
+// Bound by latency: three loads that wait for each other (path, page table, rows), then the stores. Keys and values by one
+// CTA, so that 64 requests of 8 layers are in flight at once.
+__global__ void __launch_bounds__(kThreads, 3) kv_keep_kernel(const __grid_constant__ Layers L, const KeepArgs A) {
+  extern __shared__ longlong4 s_move[];      // of a position: byte offsets of its row, from and to (or -1), and its scales'
+  const int b = blockIdx.x, S = L.c.page_size;
+  const int count = A.count[b];
   const long long base = A.base[b];
-  const auto slot_of = [&](long long pos) -> long long {
-    if (pos < 0 || pos >= (long long)A.width * L.c.page_size) return -1;
-    const int page = A.table[b * A.table_stride + pos / L.c.page_size];
-    return page < 0 || page >= L.c.pages ? -1 : (long long)page * L.c.page_size + pos % L.c.page_size;
-  };
-  for (int j = threadIdx.x; j < n; j += kThreads) {
+  for (int j = threadIdx.x; j < A.max_len; j += kThreads) {
     const int node = A.path[b * A.path_stride + j];
-    const long long src = node < 0 || node == j ? -1 : slot_of(base + node), dst = src < 0 ? -1 : slot_of(base + j);
-    s_src[j] = dst < 0 ? -1 : src;
-    s_dst[j] = dst;
+    const long long from = base + node, to = base + j, end = (long long)A.width * S;
+    longlong4 m = make_longlong4(-1, 0, 0, 0);
+    if (j < count && node >= 0 && node != j && from >= 0 && to >= 0 && from < end && to < end) {
+      const long long fp = from / S, tp = to / S, fo = from - fp * S, to_ = to - tp * S;
+      const int fpage = A.table[b * A.table_stride + fp], tpage = A.table[b * A.table_stride + tp];
+      if (fpage >= 0 && fpage < L.c.pages && tpage >= 0 && tpage < L.c.pages) {
+        m.x = (fpage * L.c.page_stride + fo * L.c.slot_stride) * L.size;
+        m.y = (tpage * L.c.page_stride + to_ * L.c.slot_stride) * L.size;
+        m.z = fpage * L.c.scale_page_stride + fo * L.c.scale_slot_stride;
+        m.w = tpage * L.c.scale_page_stride + to_ * L.c.scale_slot_stride;
+      }
+    }
+    s_move[j] = m;
   }
   __syncthreads();
-  const bool value = blockIdx.y & 1;
-  const auto& at = L.at[blockIdx.y >> 1];
-  char* const rows = value ? at.v : at.k;
-  float* const scales = value ? at.vs : at.ks;
+  const int n = min(count, A.max_len);
+  const auto& at = L.at[blockIdx.y];
   const int h0 = blockIdx.z * A.heads, hn = min(A.heads, L.c.kv_heads - h0);
-  const int wide = hn << L.pieces, batch = kThreads * kHeld / wide;      // pieces a position, positions a batch
+  const int wide = hn << L.pieces, batch = kThreads * kHeld / 2 / wide;    // pieces a position, positions a batch
+  const long long head = L.c.head_stride * L.size;
   for (int j0 = 0; j0 < n; j0 += batch) {
-    const int m = min(batch, n - j0);
+    const int m = min(batch, n - j0), half = m * wide;
     uint4 w[kHeld];
-    float sc[2];
-    const auto piece = [&](int i, long long slot) {
-      const int x = i % wide, h = h0 + (x >> L.pieces), c = x & ((1 << L.pieces) - 1);
-      return reinterpret_cast<uint4*>(rows + row_bytes(L, slot / L.c.page_size, slot % L.c.page_size) +
-                                      h * L.c.head_stride * L.size) + c;
-    };
-    const auto scale = [&](int i, long long slot) {
-      return scales + slot / L.c.page_size * L.c.scale_page_stride + slot % L.c.page_size * L.c.scale_slot_stride +
-             (h0 + i % hn) * L.c.scale_head_stride;
-    };
+    char* to[kHeld];
+    float sc[4];
+    float* scale_to[4];
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-      const int i = k * kThreads + threadIdx.x;
-      if (i < m * wide && s_src[j0 + i / wide] >= 0) w[k] = *piece(i, s_src[j0 + i / wide]);
+      const int i = k * kThreads + threadIdx.x, x = i < half ? i : i - half;
+      to[k] = nullptr;
+      if (i < 2 * half) {
+        const int j = x / wide, y = x - j * wide;
+        const longlong4 v = s_move[j0 + j];
+        if (v.x >= 0) {
+          char* const rows = (i < half ? at.k : at.v) + (h0 + (y >> L.pieces)) * head + ((y & ((1 << L.pieces) - 1)) << 4);
+          w[k] = *reinterpret_cast<const uint4*>(rows + v.x);
+          to[k] = rows + v.y;
+        }
+      }
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = k * kThreads + threadIdx.x;
-      if (scales && i < m * hn && s_src[j0 + i / hn] >= 0) sc[k] = *scale(i, s_src[j0 + i / hn]);
+    for (int k = 0; k < 4; ++k) {
+      const int i = k * kThreads + threadIdx.x, x = i < m * hn ? i : i - m * hn;
+      scale_to[k] = nullptr;
+      if (at.ks && i < 2 * m * hn) {
+        const longlong4 v = s_move[j0 + x / hn];
+        if (v.x >= 0) {
+          float* const scales = (i < m * hn ? at.ks : at.vs) + (h0 + x % hn) * L.c.scale_head_stride;
+          sc[k] = scales[v.z];
+          scale_to[k] = scales + v.w;
+        }
+      }
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int i = k * kThreads + threadIdx.x;
-      if (i < m * wide && s_src[j0 + i / wide] >= 0) *piece(i, s_dst[j0 + i / wide]) = w[k];
-    }
+    for (int k = 0; k < kHeld; ++k)
+      if (to[k]) *reinterpret_cast<uint4*>(to[k]) = w[k];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = k * kThreads + threadIdx.x;
-      if (scales && i < m * hn && s_src[j0 + i / hn] >= 0) *scale(i, s_dst[j0 + i / hn]) = sc[k];
-    }
+    for (int k = 0; k < 4; ++k)
+      if (scale_to[k]) *scale_to[k] = sc[k];
   }
 }
 
@@ -108,8 +119,8 @@ __device__ __forceinline__ void copy_page(const Layers& L, int layer, bool value
   const int pages = L.c.pages, n = min(slots, L.c.page_size);
   if (src < 0 || src >= pages || dst < 0 || dst >= pages || src == dst || n <= 0) return;
   const auto& at = L.at[layer];
-  const char* const from = (value ? at.v : at.k) + row_bytes(L, src, 0);
-  char* const to = (value ? at.v : at.k) + row_bytes(L, dst, 0);
+  const char* const from = (value ? at.v : at.k) + src * L.c.page_stride * L.size;
+  char* const to = (value ? at.v : at.k) + dst * L.c.page_stride * L.size;
   const int total = (L.c.kv_heads * n) << L.pieces;
   for (int i0 = threadIdx.x; i0 < total; i0 += kHeld * kThreads) {
     uint4 w[kHeld];
@@ -155,6 +166,7 @@ __device__ __forceinline__ int pages_for(int positions, int page_size) {
 constexpr int kTake = 1024;                  // threads of the CTA that takes pages, and requests it takes at a time
 constexpr int kGroup = 8;                    // 32-page words a counted group
 constexpr int kMaxPages = 1 << 20;
+constexpr int kLarge = 8192;                 // pages from which on 8 CTAs look for free ones
 
 struct TakeArgs {
   Pool P;
@@ -165,41 +177,78 @@ struct TakeArgs {
 };
 
 // inclusive running sum over the CTA; every thread has to come
-__device__ __forceinline__ long long cta_scan(long long v, long long* s_warp, long long* total) {
+template <typename F> __device__ __forceinline__ F cta_scan(F v, F* s_warp, F* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, v, off);
+    const F o = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= off) v += o;
   }
   __syncthreads();
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    long long x = s_warp[lane];
+  // (every warp sums the warps' totals for itself: no third barrier)
+  F x = s_warp[lane];
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, x, off);
-      if (lane >= off) x += o;
-    }
-    s_warp[lane] = x;
+  for (int off = 1; off < 32; off <<= 1) {
+    const F o = __shfl_up_sync(0xffffffffu, x, off);
+    if (lane >= off) x += o;
   }
-  __syncthreads();
-  *total = s_warp[31];
-  return v + (warp ? s_warp[warp - 1] : 0);
+  *total = __shfl_sync(0xffffffffu, x, 31);
+  const F before = __shfl_sync(0xffffffffu, x, max(warp - 1, 0));
+  return v + (warp ? before : (F)0);
+}
+// the position of the n-th set bit (n < number of bits)
+__device__ __forceinline__ int nth_bit(uint32_t bits, int n) {
+  int at = 0;
+#pragma unroll
+  for (int half = 16; half; half >>= 1) {
+    const int c = __popc(bits & ((1u << half) - 1));
+    if (n >= c) {
+      n -= c;
+      at += half;
+      bits >>= half;
+    }
+  }
+  return at;
 }
 
 // FORK: request i is the fork of row parent[i] into row child[i], which needs a page for what its last one holds.
 template <bool FORK>
 __global__ void __launch_bounds__(kTake) pages_take_kernel(const TakeArgs A) {
+  if constexpr (FORK) asm volatile("griddepcontrol.launch_dependents;");      // pages_fork_kernel, which waits
   extern __shared__ uint32_t s_free[];       // a bit a page; then the free pages up to each group of words
-  __shared__ long long s_warp[32], s_start[kTake];         // s_start: pages asked for up to a request, in order
+  __shared__ long long s_warp[32];
+  __shared__ int s_sum[32];
+  __shared__ int s_start[kTake];                           // pages asked for up to a request, in order (up to 2^30)
   __shared__ int s_first[kTake];                           // where a request's pages go in its row, or -1
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   const Pool& P = A.P;
   const int words = (P.pages + 31) / 32, groups = (words + kGroup - 1) / kGroup;
   int* const s_count = reinterpret_cast<int*>(s_free + groups * kGroup);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int w0 = warp * 32; w0 < groups * kGroup; w0 += kTake) {
+  // the first requests' needs are on their way while the counts are read
+  const auto need_of = [&](int b, int* first) {            // -1: it cannot be granted
+    *first = 0;
+    if (b >= A.n) return 0;
+    if constexpr (FORK) {
+      const int from = A.parent[b], to = A.child[b];
+      if (from < 0 || from >= P.rows || to < 0 || to >= P.rows || from == to) return -1;
+      const int len = max(A.length[from], 0), need = len % P.page_size ? 1 : 0;
+      *first = len / P.page_size;
+      return *first + need <= P.width ? need : -1;
+    } else {
+      *first = pages_for(A.length[b], P.page_size);
+      const int upto = pages_for(A.target[b], P.page_size), need = max(upto - *first, 0);
+      return need == 0 || upto <= P.width ? need : -1;
+    }
+  };
+  int first, need = need_of(threadIdx.x, &first);
+  // a CTA's share of the words, in whole 32s
+  const int share = ((groups * kGroup + ranks - 1) / ranks + 31) / 32 * 32;
+  const int share0 = rank * share, share1 = min(share0 + share, groups * kGroup);
+  for (int w0 = share0 + warp * 32; w0 < share1; w0 += kTake) {
     int r[32];
     uint32_t mine = 0;
 #pragma unroll
@@ -212,69 +261,57 @@ __global__ void __launch_bounds__(kTake) pages_take_kernel(const TakeArgs A) {
       const uint32_t bits = __ballot_sync(0xffffffffu, r[k] == 0);
       if (lane == k) mine = bits;
     }
-    if (w0 + lane < groups * kGroup) s_free[w0 + lane] = mine;
+    if (w0 + lane < share1) s_free[w0 + lane] = mine;
+  }
+  if (ranks > 1) {                           // every CTA needs all of them; none writes a count before all are read
+    cluster.sync();
+    for (int w = threadIdx.x; w < groups * kGroup; w += kTake)
+      if (w / share != rank) s_free[w] = cluster.map_shared_rank(s_free, w / share)[w];
+    cluster.sync();
   }
   __syncthreads();
-  long long free = 0;
+  int free = 0;
   for (int g0 = 0; g0 < groups; g0 += kTake) {
     int c = 0;
     const int g = g0 + threadIdx.x;
     if (g < groups)
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) c += __popc(s_free[g * kGroup + k]);
-    long long total;
-    const long long up = cta_scan(c, s_warp, &total);
-    if (g < groups) s_count[g] = (int)(free + up);
+    int total;
+    const int up = cta_scan(c, s_sum, &total);
+    if (g < groups) s_count[g] = free + up;
     free += total;
   }
   long long asked = 0;                       // by the requests before
   for (int b0 = 0; b0 < A.n; b0 += kTake) {
     const int b = b0 + threadIdx.x;
-    int need = 0, first = 0;
-    bool fits = false;
-    if (b < A.n) {
-      if constexpr (FORK) {
-        const int from = A.parent[b], to = A.child[b];
-        if (from >= 0 && from < P.rows && to >= 0 && to < P.rows && from != to) {
-          const int len = max(A.length[from], 0);
-          first = len / P.page_size;
-          need = len % P.page_size ? 1 : 0;
-          fits = first + need <= P.width;
-        }
-      } else {
-        first = pages_for(A.length[b], P.page_size);
-        const int upto = pages_for(A.target[b], P.page_size);
-        need = max(upto - first, 0);
-        fits = need == 0 || upto <= P.width;
-      }
-      if (!fits) need = 0;
-    }
+    if (b0) need = need_of(b, &first);
     long long total;
-    const long long up = asked + cta_scan(need, s_warp, &total);
-    const bool ok = fits && (need == 0 || up <= free);
-    if (b < A.n) A.granted[b] = ok;
-    s_start[threadIdx.x] = up;
+    const long long up = asked + cta_scan((long long)max(need, 0), s_warp, &total);
+    const bool ok = need >= 0 && (need == 0 || up <= free);
+    if (b < A.n && rank == 0) A.granted[b] = ok;
+    s_start[threadIdx.x] = (int)min(up, 1ll << 30);
     s_first[threadIdx.x] = ok ? first : -1;
     __syncthreads();
-    const long long end = min(asked + total, free);
-    for (long long r = asked + threadIdx.x; r < end; r += kTake) {
+    const int end = (int)min(asked + total, (long long)free);
+    for (long long at = asked + rank * kTake + threadIdx.x; at < end; at += ranks * kTake) {
+      const int r = (int)at;
       int lo = 0, hi = kTake - 1;            // the first request with s_start > r
-      while (lo < hi) {
+#pragma unroll
+      for (int step = 0; step < 10; ++step) {
         const int mid = (lo + hi) >> 1;
         if (s_start[mid] > r) hi = mid; else lo = mid + 1;
       }
       if (s_first[lo] < 0) continue;
-      const long long before = lo ? s_start[lo - 1] : asked;
+      const int before = lo ? s_start[lo - 1] : (int)asked;
       int g = 0, gh = groups - 1;            // the group that holds free page r
       while (g < gh) {
         const int mid = (g + gh) >> 1;
         if (s_count[mid] > r) gh = mid; else g = mid + 1;
       }
-      int at = (int)(r - (g ? s_count[g - 1] : 0)), w = g * kGroup;
-      for (int c; at >= (c = __popc(s_free[w])); ++w) at -= c;
-      uint32_t bits = s_free[w];
-      for (; at; --at) bits &= bits - 1;
-      const int page = w * 32 + __ffs(bits) - 1;
+      int left = r - (g ? s_count[g - 1] : 0), w = g * kGroup;
+      for (int c; left >= (c = __popc(s_free[w])); ++w) left -= c;
+      const int page = w * 32 + nth_bit(s_free[w], left);
       const int row = FORK ? A.child[b0 + lo] : b0 + lo;
       P.table[row * P.stride + s_first[lo] + (r - before)] = page;
       P.refs[page] = 1;
@@ -307,6 +344,7 @@ __global__ void __launch_bounds__(kThreads) pages_fork_kernel(const __grid_const
                                                               const int32_t* parent, const int32_t* child,
                                                               const int32_t* granted, int lead) {
   const int i = blockIdx.x, y = (int)blockIdx.y - lead;
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // launched early: for pages_take_kernel's results
   if (!granted[i]) return;
   const int from = parent[i], to = child[i], len = max(length[from], 0), full = len / P.page_size;
   const int32_t* const src = P.table + from * P.stride;
@@ -355,7 +393,18 @@ cfb_status check_pool(const int32_t* refs, int pages, int page_size, const int32
 template <bool FORK> cfb_status launch_take(const TakeArgs& a, cudaStream_t st) {
   const auto bytes = [](int pages) { return ((pages + 31) / 32 + kGroup - 1) / kGroup * (kGroup + 1) * 4; };
   if (allow_smem<pages_take_kernel<FORK>>(bytes(kMaxPages)) != cudaSuccess) return cfb_launch_status("pages_take_kernel");
-  pages_take_kernel<FORK><<<1, kTake, bytes(a.P.pages), st>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(a.P.pages >= kLarge ? 8 : 1);
+  cfg.blockDim = dim3(kTake);
+  cfg.dynamicSmemBytes = bytes(a.P.pages);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cfg.gridDim.x;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, pages_take_kernel<FORK>, a);
   return cfb_launch_status("pages_take_kernel");
 }
 
@@ -375,9 +424,9 @@ extern "C" cfb_status cfb_kv_keep(const cfb_kv_cache* const* caches, int n_cache
     const Layers L = layers_of(caches + i, n);
     a.heads = kThreads >> L.pieces;                        // up to kThreads pieces a position
     if (a.heads > L.c.kv_heads) a.heads = L.c.kv_heads;
-    const dim3 grid(B, 2 * n, (L.c.kv_heads + a.heads - 1) / a.heads);
+    const dim3 grid(B, n, (L.c.kv_heads + a.heads - 1) / a.heads);
     if (grid.z > 65535) return CFB_ERR_UNSUPPORTED;
-    kv_keep_kernel<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(L, a);
+    kv_keep_kernel<<<grid, kThreads, max_len * sizeof(longlong4), static_cast<cudaStream_t>(stream)>>>(L, a);
     if (const cfb_status s = cfb_launch_status("kv_keep_kernel")) return s;
   }
   return CFB_OK;
@@ -437,8 +486,16 @@ extern "C" cfb_status cfb_pages_fork(int32_t* refs, int pages, int page_size, in
   for (int i = 0; i == 0 || i < n_caches; i += kLayers) {
     const int m = n_caches - i < kLayers ? n_caches - i : kLayers, lead = i == 0;
     const Layers L = m > 0 ? layers_of(caches + i, m) : Layers{};
-    pages_fork_kernel<<<dim3(n, lead + 2 * m), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(L, a.P, length, parent, child,
-                                                                                               granted, lead);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(n, lead + 2 * m);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, pages_fork_kernel, L, a.P, length, parent, child, static_cast<const int32_t*>(granted), lead);
     if (const cfb_status s = cfb_launch_status("pages_fork_kernel")) return s;
   }
   return CFB_OK;

@@ -6,6 +6,7 @@ all layers at once, ``keep_path`` moves a step's accepted rows together and ``co
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -80,6 +81,7 @@ class PagedKVCache:
             k.stride(0), k.stride(1), k.stride(2), *ss, self.pages, self.page_size, self.kv_heads, self.head_dim,
             _DT[k.dtype])
         self.desc = C.byref(self._desc)
+        self._at = C.addressof(self._desc)
 
     def _slots(self, slots):
         if slots.dim() != 1 or slots.is_floating_point() or slots.get_device() != self._dev:
@@ -136,15 +138,17 @@ class PagedKVCache:
 
 
 def _layers(caches, what: str, device=None):
-    """(descriptor array, number, device number) of one cache or a sequence of caches of one geometry."""
+    """(packed descriptor addresses, number, device number) of one cache or a sequence of caches of one geometry."""
     if isinstance(caches, PagedKVCache):
         caches = (caches,)
-    dev = caches[0]._dev if len(caches) else device
-    if any(c._dev != dev for c in caches):
-        raise _lib.CfbError(f"{what}: the caches are on several devices")
+    n = len(caches)
+    dev = caches[0]._dev if n else device
+    for c in caches:
+        if c._dev != dev:
+            raise _lib.CfbError(f"{what}: the caches are on several devices")
     if device is not None and dev != device:
         raise _lib.CfbError(f"{what}: the caches are on cuda:{dev}, the pages on cuda:{device}")
-    return (C.c_void_p * len(caches))(*[C.addressof(c._desc) for c in caches]), len(caches), dev
+    return struct.pack("%dP" % n, *[c._at for c in caches]), n, dev
 
 
 def _check_layers(caches, what: str) -> None:
@@ -158,6 +162,8 @@ def _check_layers(caches, what: str) -> None:
 
 def _index(t, name: str, what: str, dev: int, shape):
     """t, an integer tensor of `shape` on device dev, as contiguous int32."""
+    if t.dtype is torch.int32 and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t
     if t.get_device() != dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != tuple(shape):
         _lib.require_cuda(t, name)
         raise _lib.CfbError(f"{what}: {name} must be integers {list(shape)} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
@@ -242,12 +248,12 @@ class PagePool:
 
     def _table(self, table, what: str):
         """(address, row stride, width, rows) of a table that is changed in place."""
-        if (table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != self._dev
-                or (table.shape[1] > 1 and table.stride(1) != 1) or (table.shape[0] > 1 and table.stride(0) < table.shape[1])):
+        shape, st = table.shape, table.stride()
+        if (len(shape) != 2 or table.dtype is not torch.int32 or table.get_device() != self._dev
+                or (shape[1] > 1 and st[1] != 1) or (shape[0] > 1 and st[0] < shape[1])):
             _lib.require_cuda(table, "table")
             raise _lib.CfbError(f"{what}: table must be int32 [rows, width] on the pool's device, its rows contiguous and apart")
-        rows, width = table.shape
-        return table.data_ptr(), max(table.stride(0), width), width, rows
+        return table.data_ptr(), max(st[0], shape[1]), shape[1], shape[0]
 
     def reserve(self, table, length, target, stream=None):
         """Pages for the positions [length[b], target[b]) that request b's pages do not cover yet, into its row. Returns

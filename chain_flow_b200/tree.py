@@ -128,11 +128,20 @@ class _ProbabilityVerifier:
         self.accepted_len = torch.empty(max_batch, dtype=torch.int32, device=dev)
         self.logprobs = torch.empty(max_batch, max_spec_len + 1, dtype=torch.float32, device=dev)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._views = {}                                 # of the buffers, by the number of requests: a slice takes a microsecond
+
+    def _outputs(self, B):
+        views = self._views.get(B)
+        if views is None:
+            views = self._views[B] = tuple(t[:B] for t in self._buffers())
+        return views
 
     def _refuse(self, what, wrong):
         raise _lib.CfbError(f"{type(self).__name__}: {what} {wrong}")
 
     def _ints(self, t, name, shape):
+        if t.dtype is torch.int32 and t.shape == shape and t.get_device() == self._dev and t.is_contiguous():
+            return t
         if t.get_device() != self._dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != shape:
             _lib.require_cuda(t, name)
             self._refuse(name, f"must be integers {list(shape)} on cuda:{self._dev}, got {t.dtype} {list(t.shape)} on {t.device}")
@@ -146,16 +155,15 @@ class _ProbabilityVerifier:
 
     def _common(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, temperature):
         """The checked arguments that both verifiers take: (logits' dtype code, row stride, B, ...)."""
-        dt = _LOGITS.get(logits.dtype)
-        if logits.get_device() != self._dev or dt is None or logits.dim() != 2 or logits.shape[1] == 0 or (
-                logits.stride(1) != 1 and logits.shape[1] > 1):
+        dt, shape, st = _LOGITS.get(logits.dtype), logits.shape, logits.stride()
+        if logits.get_device() != self._dev or dt is None or len(shape) != 2 or shape[1] == 0 or (st[1] != 1 and shape[1] > 1):
             _lib.require_cuda(logits, "logits")
             self._refuse("logits", f"must be fp32, fp16 or bf16 rows with a contiguous vocabulary dim on cuda:{self._dev}")
-        rows, V = logits.shape
+        rows, V = shape
         B = cu_num_draft.shape[0] if cu_num_draft.dim() == 1 else -1
         if rows > self.max_rows or B > self.max_batch:
             self._refuse(f"{rows} rows / {B} requests", f"exceed this verifier ({self.max_rows} / {self.max_batch})")
-        ld = logits.stride(0) if rows > 1 else V
+        ld = st[0] if rows > 1 else V
         if ld < V:
             self._refuse("logits", "has rows that share words")
         cu_d, cu_s = self._ints(cu_num_draft, "cu_num_draft", (B,)), self._ints(cu_num_sampled, "cu_num_sampled", (B,))
@@ -164,7 +172,8 @@ class _ProbabilityVerifier:
             if temperature.get_device() != self._dev or not temperature.is_floating_point() or temperature.shape != (B,):
                 _lib.require_cuda(temperature, "temperature")
                 self._refuse("temperature", f"must be floating-point [{B}] on cuda:{self._dev}")
-            temperature = temperature.to(torch.float32).contiguous()
+            if temperature.dtype is not torch.float32 or not temperature.is_contiguous():
+                temperature = temperature.to(torch.float32).contiguous()
         return dt, ld, rows, V, B, cu_d, cu_s, tokens, temperature
 
 
@@ -180,6 +189,10 @@ class SampledVerifier(_ProbabilityVerifier):
     def __init__(self, max_rows: int, max_batch: int, max_spec_len: int, device=None):
         super().__init__(max_rows, max_batch, max_spec_len, device)
         self.accepted_path = torch.empty(max_batch, max_spec_len, dtype=torch.int32, device=self.ws.device)
+        self._ptrs = tuple(t.data_ptr() for t in self._buffers()) + (self.ws_ptr, self.ws_bytes, self.err.data_ptr())
+
+    def _buffers(self):
+        return self.out_tokens, self.accepted_path, self.accepted_len, self.logprobs
 
     def __call__(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, parents, uniforms, temperature=None, stream=None):
         """(output_tokens [B, max_spec + 1], accepted_path [B, max_spec], accepted_len [B]) int32 and logprobs fp32
@@ -197,12 +210,10 @@ class SampledVerifier(_ProbabilityVerifier):
             _lib.check(self.lib.cfb_tree_verify_sampled(
                 logits.data_ptr(), ld, rows, V, dt, cu_d.data_ptr(), cu_s.data_ptr(), tokens.data_ptr(), par.data_ptr(),
                 tokens.shape[0], u.data_ptr(), u.element_size(), None if temp is None else temp.data_ptr(), B, self.max_spec,
-                self.out_tokens.data_ptr(), self.accepted_path.data_ptr(), self.accepted_len.data_ptr(), self.logprobs.data_ptr(),
-                self.ws_ptr, self.ws_bytes, self.err.data_ptr(), _lib.stream_of(self._dev, "SampledVerifier")),
-                "cfb_tree_verify_sampled")
+                *self._ptrs, _lib.stream_of(self._dev, "SampledVerifier")), "cfb_tree_verify_sampled")
         elif B:
             self._refuse("logits", "has no rows")
-        return self.out_tokens[:B], self.accepted_path[:B], self.accepted_len[:B], self.logprobs[:B]
+        return self._outputs(B)
 
 
 class RejectionVerifier(_ProbabilityVerifier):
@@ -223,6 +234,10 @@ class RejectionVerifier(_ProbabilityVerifier):
             self.width = ids.numel()
             self.index_of = torch.full((vocab_size,), -1, dtype=torch.int32, device=self.ws.device)
             self.index_of[ids] = torch.arange(self.width, dtype=torch.int32, device=self.ws.device)
+        self._ptrs = tuple(t.data_ptr() for t in self._buffers()) + (self.ws_ptr, self.ws_bytes, self.err.data_ptr())
+
+    def _buffers(self):
+        return self.out_tokens, self.accepted_len, self.logprobs
 
     def __call__(self, logits, cu_num_draft, cu_num_sampled, draft_tokens, draft_probs, uniforms, resample, temperature=None,
                  stream=None):
@@ -250,9 +265,8 @@ class RejectionVerifier(_ProbabilityVerifier):
                 logits.data_ptr(), ld, rows, V, dt, cu_d.data_ptr(), cu_s.data_ptr(), tokens.data_ptr(), draft_probs.data_ptr(),
                 draft_probs.stride(0) if n > 1 else self.width, n, self.width,
                 None if self.index_of is None else self.index_of.data_ptr(), u.data_ptr(), v.data_ptr(), v.element_size(),
-                None if temp is None else temp.data_ptr(), B, self.max_spec, self.out_tokens.data_ptr(),
-                self.accepted_len.data_ptr(), self.logprobs.data_ptr(), self.ws_ptr, self.ws_bytes, self.err.data_ptr(),
+                None if temp is None else temp.data_ptr(), B, self.max_spec, *self._ptrs,
                 _lib.stream_of(self._dev, "RejectionVerifier")), "cfb_chain_verify_rejection")
         elif B:
             self._refuse("logits", "has no rows")
-        return self.out_tokens[:B], self.accepted_len[:B], self.logprobs[:B]
+        return self._outputs(B)
