@@ -11,19 +11,19 @@
 // so that happens to one row in thousands; rows that are flat over a whole vocabulary pay it always.
 //
 // One pass over the row: a warp takes 1024 elements in registers, their largest, their weights relative
-// to it and the weights' sum, which stay in shared memory (no running rescale: the sums of all such
-// units are brought to one base at the end, in 64 bits). The draw then lies in one unit, which is read again
-// (from L2) and scanned by one warp. A row is shared by a cluster of CTAs, which exchange their
-// totals through distributed shared memory.
+// to it and the weights' sum, which stay in shared memory (no running rescale of elements: such units' sums are brought
+// to one base). A row is shared by a cluster of CTAs, a CTA's part by its warps, each with neighbouring units; CTAs
+// exchange their totals through distributed shared memory. The draw then descends: CTA, warp, unit, a lane's neighbours,
+// element; only its unit is read again (from L2).
 //
 // Error of the pass, with u = 2^-24 and x = (l - max l) c: an element's exponent is off by 3 u |x| (difference, c,
-// product; its unit's base likewise), each of its two exponentials by 4 u, a unit's sum by 12 u (chains of 4, pairs,
-// the warp). Under the weights the mean of |x| is their entropy less log2 of their sum Z relative to the largest: at
-// most log2(V / Z). What decides is C - t = C - u Z: an error that is the same share of every weight cancels in it but
-// for a half. The sums over CTAs, over a CTA's n units, and inside the draw's unit are fp32 too. So C - t is off by
-// less than
-//   u Z (3 ln 2 log2(V / Z) + (8 + 12) / 2 + 10) + u (mass of the CTA's part) (8 + n / 32) + 18 u (mass of the unit).
-// Rows of 248320 normal logits of deviation 2.5 fall into that band once in ten draws, a language model's less.
+// product; its unit's base likewise), its exponential and those of two changes of base by 4 u each, a unit's sum by 12 u
+// (chains of 4, pairs, the warp), a warp's sum of q units by 2 q u. Under the weights the mean of |x| is their entropy less
+// log2 of their sum Z relative to the largest: at most log2(V / Z). What decides is C - t = C - u Z: an error that is
+// the same share of every weight cancels in it but for a half. The sums over CTAs, a CTA's warps and units, and
+// inside the draw's unit are fp32 too. So C - t is off by less than
+//   u Z (3 ln 2 log2(V / Z) + (12 + 12 + 2 q) / 2 + 10) + u (mass of the CTA's part) (12 + 2 q) + 18 u (mass of the unit).
+// Rows of 248320 normal logits of deviation 2.5 fall into that band once in eight draws, a language model's less.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <cmath>
@@ -65,7 +65,9 @@ struct VerifyArgs {
 };
 
 enum Kind : int { ROW_MASS = 0, ROW_EMPTY = 1, ROW_NAN = 2 };
-constexpr int kUndecided = 2;                              // RowResult::accept: fp32 did not decide (scaled: the row's largest)
+// RowResult::accept, left for the walk (scaled: the row's largest, mass: the sum of its weights): fp32 did not decide; a draft
+// that is refused, so that something else is to be drawn
+constexpr int kUndecided = 2, kRefused = 3;
 
 struct Pub { float top; int nan; float sum; float pad; double sum64; };      // a CTA's part of a row
 struct Found { int token, unsure; float logit; int pad; };
@@ -75,6 +77,8 @@ struct Shared {
   Found found[2];
   double z, whole;           // sum of the row's weights; of what the last pass summed
   double before, end;        // the running sums of the last pass before this CTA's part and behind it
+  float warp_top[kWarps], warp_sum[kWarps];                // of a warp's units (the sum relative to its largest)
+  double warp_sum64[kWarps];
   float top;                 // of the row
   int kind;
   int owner;                 // the CTA whose part has the threshold, or (greedy rows) the first of the largest
@@ -138,14 +142,14 @@ CFB_DEV Pair mul2(Pair a, Pair b) {
 }
 
 // A logits row: element i lies at p[i]. Vectors of 16 bytes start at element -shift, so that they are aligned. Units of kUnit
-// elements from there on; this CTA has [u0, u1) of them.
+// elements from there on; this CTA has [u0, u1) of them, and each of its warps `each` neighbours.
 template <typename T> struct Row {
-  int u0, u1;
+  int u0, u1, each;
   const T* p;
   int V, shift;
   float c;                    // log2(e) / tau
   double c64;
-  const float* q;             // draft probabilities of the row, or null
+  const float* probs;         // draft probabilities of the row, or null
   const int32_t* index_of;
 };
 template <typename T> constexpr int kE = 16 / (int)sizeof(T);          // elements a vector
@@ -203,29 +207,37 @@ CFB_DEV float weight(float l, float base, float c) { return ex2((l - base) * c);
 // a sum's scale where a larger base takes over (of a largest +inf only what has it counts)
 CFB_DEV float rescale(float top, float base, float c) { return top == base ? 1.f : top == -INFINITY || base == INFINITY ? 0.f : weight(top, base, c); }
 
-// The weight 2^((l - base) c) in 64 bits, relative to a finite base, by a whole warp: with y = (l - base) c = k / 32 + r, |r| <= 1/64,
-// the series of 2^r cut after r^5 (the first term left out is 2 10^-15), times 2^(k mod 32 / 32) from the lane that holds
-// it. 0 below 2^-1020. The library's function branches, which kept several from running side by side: a pass took 4
-// times as long.
+// The weight 2^((l - base) c) in 64 bits, relative to a finite base, by a whole warp: with 32 (l - base) c = k + r, |r| <= 1/2,
+// the series of 2^(r / 32) cut after r^5 (the first term left out is 2 10^-15), times 2^(k mod 32 / 32) from the lane that
+// holds it. Nothing is below 2^-1000 (CUT: is 0). Eleven 64-bit operations, N elements side by side; the library's
+// function branches, which kept several from running side by side: a pass took 4 times as long.
+CFB_DEV float lowest_logit(float base, float c) { return base - 1000.f * reciprocal(c); }
 CFB_DEV double exp2_table(int lane) { return exp2((double)lane * 0.03125); }
-// the fp32 number as a double, by its bits (conversions are slow): what is 0 becomes 2^-127, and an infinity 2^128
-template <typename T> CFB_DEV double widen(float f) {
-  const int b = __float_as_int(f);
-  return __hiloint2double(((b >> 3) & 0x8fffffff) + 0x38000000, sizeof(T) == 4 ? b << 29 : 0);
-}
-template <typename T> CFB_DEV double fast_weight64(float l, double base, double c, double table) {
-  const double d = widen<T>(l) - base, magic = 6755399441055744.;        // 1.5 2^52: adding it rounds to a whole number
-  const double y = d * c, shifted = fma(y, 32., magic), r = fma(shifted - magic, -0.03125, y);
-  const int k = __double2loint(shifted);
-  double p = 0x1.5d87fe78a6731p-10;                        // ln2^k / k!
-  p = fma(p, r, 0x1.3b2ab6fba4e77p-7);
-  p = fma(p, r, 0x1.c6b08d704a0c0p-5);
-  p = fma(p, r, 0x1.ebfbdff82c58fp-3);
-  p = fma(p, r, 0x1.62e42fefa39efp-1);
-  const double t = __shfl_sync(0xffffffffu, table, k);
-  p = fma(p * r, t, t);
-  p = __hiloint2double(__double2hiint(p) + ((k << 15) & 0xfff00000), __double2loint(p));
-  return y > -1020. ? p : 0.;
+template <bool CUT, int N> CFB_DEV void fast_weights64(const float* l, float base, float c, double c32, double table, double* out) {
+  const double magic = 6755399441055744.;                  // 1.5 2^52: adding it rounds to a whole number
+  const float low = lowest_logit(base, c);
+  double r[N], p[N];
+  int k[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double d = (double)fmaxf(l[i], low) - (double)base, shifted = fma(d, c32, magic);
+    k[i] = __double2loint(shifted);
+    r[i] = fma(d, c32, magic - shifted);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {                            // (ln2 / 32)^k / k!
+    p[i] = fma(0x1.5d87fe78a6731p-35, r[i], 0x1.3b2ab6fba4e77p-27);
+    p[i] = fma(p[i], r[i], 0x1.c6b08d704a0c0p-20);
+    p[i] = fma(p[i], r[i], 0x1.ebfbdff82c58fp-13);
+    p[i] = fma(p[i], r[i], 0x1.62e42fefa39efp-6) * r[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double t = __shfl_sync(0xffffffffu, table, k[i]);
+    p[i] = fma(p[i], t, t);
+    p[i] = __hiloint2double(__double2hiint(p[i]) + ((k[i] << 15) & 0xfff00000), __double2loint(p[i]));
+    out[i] = CUT && l[i] <= low ? 0. : p[i];
+  }
 }
 // by one thread, of any base, to the smallest denormal
 CFB_DEV double weight64(float l, float base, double c) {
@@ -235,7 +247,7 @@ CFB_DEV double weight64(float l, float base, double c) {
 template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
   if (i < 0 || i >= w.V) return 0.f;
   const int at = w.index_of ? __ldg(w.index_of + i) : i;
-  return at >= 0 ? fmaxf(__ldg(w.q + at), 0.f) : 0.f;
+  return at >= 0 ? fmaxf(__ldg(w.probs + at), 0.f) : 0.f;
 }
 
 enum Mode : int { W32 = 0, W64 = 1, R32 = 2, R64 = 3 };    // weights, or what is left of them above q
@@ -251,22 +263,26 @@ CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, do
   } else if constexpr (MODE == R32) {
     return fmaxf(weight(l, base, w.c) * (float)iz - draft_prob(w, i), 0.f);
   } else {
-    const double v = SLOW ? weight64(l, base, w.c64) : fast_weight64<T>(l, base, w.c64, table);
+    double v;
+    if constexpr (SLOW) v = weight64(l, base, w.c64);
+    else fast_weights64<true, 1>(&l, base, w.c, 32. * w.c64, table, &v);
     if constexpr (MODE == W64) return v;
     else return fmax(v * iz - (double)draft_prob(w, i), 0.);
   }
 }
 
 // every unit's largest and its sum of weights relative to that; a unit's loads are under way while the one before is summed
-template <typename T> CFB_DEV void stats_units(const Row<T>& w, float* tops, float* sums) {
+template <typename T> CFB_DEV void stats_units(const Row<T>& w, Shared* sh, float* tops, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = w.u0 + warp * w.each, end = min(first + w.each, w.u1);
   uint4 next[kVectors<T>];
-  if (w.u0 + warp < w.u1) load_unit(w, w.u0 + warp, lane, next);
-  for (int u = w.u0 + warp; u < w.u1; u += kWarps) {
+  float most = -INFINITY, total = 0.f;
+  if (first < end) load_unit(w, first, lane, next);
+  for (int u = first; u < end; ++u) {
     uint4 v[kVectors<T>];
 #pragma unroll
     for (int j = 0; j < kVectors<T>; ++j) v[j] = next[j];
-    if (u + kWarps < w.u1) load_unit(w, u + kWarps, lane, next);
+    if (u + 1 < end) load_unit(w, u + 1, lane, next);
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVectors<T>; ++j) m = fmaxf(m, vector_max<T>(v[j]));
@@ -297,10 +313,17 @@ template <typename T> CFB_DEV void stats_units(const Row<T>& w, float* tops, flo
         }
     }
     sum = warp_sum(sum);
+    const float base = fmaxf(most, top);
+    total = total * rescale(most, base, w.c) + sum * rescale(top, base, w.c);
+    most = base;
     if (lane == 0) {
       tops[u - w.u0] = top;
       sums[u - w.u0] = sum;
     }
+  }
+  if (lane == 0) {
+    sh->warp_top[warp] = most;
+    sh->warp_sum[warp] = total;
   }
 }
 
@@ -319,96 +342,156 @@ template <typename F> CFB_DEV void table_entries(const F* t, int i, int n, int V
   }
 }
 
+// the draft probabilities of n tokens from i on
+template <typename T> CFB_DEV void draft_probs(const Row<T>& w, int i, int n, float (&q)[8]) {
+  if (w.index_of) {
+    int at[8];
+    table_entries(w.index_of, i, n, w.V, at, -1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) q[e] = at[e] >= 0 ? __ldg(w.probs + at[e]) : 0.f;
+  } else {
+    table_entries(w.probs, i, n, w.V, q, 0.f);
+  }
+}
+
 // every unit's sum of what is left above q
-template <typename T> CFB_DEV void rest_units(const Row<T>& w, float base, float iz, float* sums) {
+template <typename T> CFB_DEV void rest_units(const Row<T>& w, Shared* sh, float base, float iz, float* sums) {
+  constexpr int N = 16 / kE<T>;                            // vectors whose loads are in flight together
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int u = w.u0 + warp; u < w.u1; u += kWarps) {
-    uint4 v[kVectors<T>];
-    load_unit(w, u, lane, v);
+  const int begin = w.u0 + warp * w.each, end = min(begin + w.each, w.u1);
+  float total = 0.f;
+  for (int u = begin; u < end; ++u) {
     float a[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int j0 = 0; j0 < kVectors<T>; j0 += N) {
+      const int i = first_of(w, u, j0, lane);
+      uint4 v[N];
+      float q[N][8];
+      load_vectors(w, u * kUnit - w.shift, kUnit, i, 32 * kE<T>, v);
 #pragma unroll
-    for (int j = 0; j < kVectors<T>; ++j) {
-      const int i = first_of(w, u, j, lane);
-      float q[8];
-      if (w.index_of) {
-        int at[8];
-        table_entries(w.index_of, i, kE<T>, w.V, at, -1);
+      for (int j = 0; j < N; ++j) draft_probs(w, i + j * 32 * kE<T>, kE<T>, q[j]);
 #pragma unroll
-        for (int e = 0; e < kE<T>; ++e) q[e] = at[e] >= 0 ? __ldg(w.q + at[e]) : 0.f;
-      } else {
-        table_entries(w.q, i, kE<T>, w.V, q, 0.f);
-      }
+      for (int j = 0; j < N; ++j)
 #pragma unroll
-      for (int k = 0; k < kE<T> / 2; ++k) {
-        const float2 l = pair_of<T>(v[j], k);
-        a[0] += fmaxf(weight(l.x, base, w.c) * iz - fmaxf(q[2 * k], 0.f), 0.f);
-        a[1] += fmaxf(weight(l.y, base, w.c) * iz - fmaxf(q[2 * k + 1], 0.f), 0.f);
-      }
+        for (int k = 0; k < kE<T> / 2; ++k) {
+          const float2 l = pair_of<T>(v[j], k);
+          a[0] += fmaxf(weight(l.x, base, w.c) * iz - fmaxf(q[j][2 * k], 0.f), 0.f);
+          a[1] += fmaxf(weight(l.y, base, w.c) * iz - fmaxf(q[j][2 * k + 1], 0.f), 0.f);
+        }
     }
     const float sum = warp_sum(a[0] + a[1]);
+    total += sum;
     if (lane == 0) sums[u - w.u0] = sum;
   }
+  if (lane == 0) sh->warp_sum[warp] = total;
 }
 // every unit's sum in 64 bits: a lane has 8 neighbours of 256
 template <int MODE, bool SLOW, typename T>
-CFB_DEV void exact_units(const Row<T>& w, float base, double iz, double* sums) {
+CFB_DEV void exact_units(const Row<T>& w, Shared* sh, float base, double iz, double* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double table = exp2_table(lane);
   constexpr int kPer = kUnit / kSpan<MODE>, N = 8 / kE<T>;
-  for (int u = w.u0 * kPer + warp; u < w.u1 * kPer; u += kWarps) {
+  const int begin = (w.u0 + warp * w.each) * kPer, end = min(begin + w.each * kPer, w.u1 * kPer);
+  double total = 0.;
+  uint4 next[N];
+  float qnext[8];
+  const auto fetch = [&](int u) {
     const int first = u * kSpan<MODE> - w.shift, i = first + lane * 8;
+    load_vectors(w, first, kSpan<MODE>, i, kE<T>, next);
+    if constexpr (MODE == R64) draft_probs(w, i, 8, qnext);
+  };
+  if (begin < end) fetch(begin);
+  for (int u = begin; u < end; ++u) {
     uint4 v[N];
-    load_vectors(w, first, kSpan<MODE>, i, kE<T>, v);
-    double a[2] = {0., 0.};
-#pragma unroll SLOW ? 1 : N
-    for (int j = 0; j < N; ++j)
-#pragma unroll SLOW ? 1 : kE<T> / 2
-      for (int k = 0; k < kE<T> / 2; ++k) {
-        const float2 l = pair_of<T>(v[j], k);
-        a[0] += value_of<MODE, SLOW>(w, l.x, i + j * kE<T> + 2 * k, base, iz, table);
-        a[1] += value_of<MODE, SLOW>(w, l.y, i + j * kE<T> + 2 * k + 1, base, iz, table);
+    float q[8], l[8];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = next[j];
+    if constexpr (MODE == R64)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = qnext[e];
+    if (u + 1 < end) fetch(u + 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = pair_of<T>(v[e / (kE<T> / 2)], e % (kE<T> / 2));
+      l[2 * e] = x.x;
+      l[2 * e + 1] = x.y;
+    }
+    double a = 0.;
+    if constexpr (SLOW) {
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        const double x = weight64(l[e], base, w.c64);
+        a += MODE == R64 ? fmax(x * iz - (double)fmaxf(q[e], 0.f), 0.) : x;
       }
-    const double sum = warp_sum(a[0] + a[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        double x[4];
+        fast_weights64<MODE == R64, 4>(l + e, base, w.c, 32. * w.c64, table, x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a += MODE == R64 ? fmax(x[k] * iz - (double)fmaxf(q[e + k], 0.f), 0.) : x[k];
+      }
+    }
+    const double sum = warp_sum(a);
+    total += sum;
     if (lane == 0) sums[u - w.u0 * kPer] = sum;
   }
+  if (lane == 0) sh->warp_sum64[warp] = total;
 }
 
-// Warp 0: the units' sums become running ones
-template <typename F> CFB_DEV F run_up(F* sums, int n, int lane) {
-  F before = 0;
+// Of n values, by a warp: the first whose running sum passes *t, which becomes what is left of it; where none does, for
+// rounding, the last that is positive (unsure), or -1
+template <typename F, typename G> CFB_DEV int pick(int n, G value, F* t, bool* unsure) {
+  const int lane = threadIdx.x & 31;
+  F before = 0, before_last = 0;
+  int last = -1;
   for (int i0 = 0; i0 < n; i0 += 32) {
-    const F v = warp_scan(i0 + lane < n ? sums[i0 + lane] : (F)0, lane);
-    if (i0 + lane < n) sums[i0 + lane] = before + v;
-    before += __shfl_sync(0xffffffffu, v, 31);
+    const F v = i0 + lane < n ? value(i0 + lane) : (F)0, scan = before + warp_scan(v, lane);
+    const F up = __shfl_up_sync(0xffffffffu, scan, 1), head = lane ? up : before;
+    const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && scan > *t), some = __ballot_sync(0xffffffffu, v > 0);
+    if (hit) {
+      const int e = __ffs(hit) - 1;
+      *t -= __shfl_sync(0xffffffffu, head, e);
+      return i0 + e;
+    }
+    if (some) {
+      const int e = 31 - __clz(some);
+      last = i0 + e;
+      before_last = __shfl_sync(0xffffffffu, head, e);
+    }
+    before = __shfl_sync(0xffffffffu, scan, 31);
   }
-  __syncwarp();
-  return before;
+  *unsure = true;
+  *t -= before_last;
+  return last;
 }
 
-// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start): by units, by lanes
-// of neighbours, by a lane's elements. band: for all but the unit's own rounding.
+// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start). band: for all but
+// the unit's own rounding.
 template <int MODE, bool SLOW, typename T, typename F>
-CFB_DEV Found find(const Row<T>& w, const F* sums, F t, float base, double iz, float band) {
+CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F* sums, F t, double iz, float band) {
   constexpr int kPer = kUnit / kSpan<MODE>, kLane = kSpan<MODE> / 32;   // summed units a unit; a lane's elements
   constexpr int N = kLane / kE<T>;
-  const int lane = threadIdx.x & 31, n = (w.u1 - w.u0) * kPer;
+  const int lane = threadIdx.x & 31;
   const double table = kNarrow<MODE> ? 0. : exp2_table(lane);
-  int u = -1;
-  for (int i0 = 0; i0 < n && u < 0; i0 += 32) {
-    const unsigned hit = __ballot_sync(0xffffffffu, i0 + lane < n && sums[i0 + lane] > t);
-    if (hit) u = i0 + __ffs(hit) - 1;
-  }
+  const float base = sh->top;
   bool unsure = false;
-  if (u < 0) {                                             // rounding put the threshold past the end: the last unit with mass
-    unsure = true;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned hit = __ballot_sync(0xffffffffu, i < n && sums[i] > (i ? sums[i - 1] : (F)0));
-      if (hit) u = i0 + 31 - __clz(hit);
-    }
-    if (u < 0) return {-1, 1, 0.f, 0};
-  }
-  const int first = w.u0 * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
+  const int part = pick<F>(kWarps, [&](int i) -> F {
+    if constexpr (MODE == W32) return sh->warp_sum[i] * rescale(sh->warp_top[i], base, w.c);
+    else if constexpr (MODE == R32) return sh->warp_sum[i];
+    else return sh->warp_sum64[i];
+  }, &t, &unsure);
+  if (part < 0) return {-1, 1, 0.f, 0};
+  const int begin = part * w.each, n = (min(begin + w.each, w.u1 - w.u0) - begin) * kPer;
+  const auto unit_sum = [&](int i) -> F {
+    if constexpr (MODE == W32) return sums[begin + i] * rescale(tops[begin + i], base, w.c);
+    else return sums[begin * kPer + i];
+  };
+  const int u = pick<F>(n, unit_sum, &t, &unsure);
+  if (u < 0) return {-1, 1, 0.f, 0};
+  const F mass = unit_sum(u);
+  const int first = (w.u0 + begin) * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
   uint4 x[N];
   load_vectors(w, first, kSpan<MODE>, i0, kE<T>, x);
   F a = 0;
@@ -423,30 +506,16 @@ CFB_DEV Found find(const Row<T>& w, const F* sums, F t, float base, double iz, f
     }
     a += (v[0] + v[1]) + (v[2] + v[3]);
   }
-  const F before = u ? sums[u - 1] : (F)0, at = t - before, mass = sums[u] - before;
-  const F scan = warp_scan(a, lane), up = __shfl_up_sync(0xffffffffu, scan, 1);
-  // where no sum passes, for rounding or after the fallback above: the last that has any
-  unsigned hit = __ballot_sync(0xffffffffu, a > 0 && scan > at);
-  if (!hit) {
-    const unsigned some = __ballot_sync(0xffffffffu, a > 0);
-    if (!some) return {-1, 1, 0.f, 0};
-    unsure = true;
-    hit = 1u << (31 - __clz(some));
-  }
-  const int who = __ffs(hit) - 1, i = first + who * kLane + lane;
-  const F head = who ? __shfl_sync(0xffffffffu, up, who) : (F)0;
+  const int who = pick<F>(32, [&](int) { return a; }, &t, &unsure);
+  if (who < 0) return {-1, 1, 0.f, 0};
+  const int i = first + who * kLane + lane;
   const float l = lane < kLane && i >= 0 && i < w.V ? to_float(w.p[i]) : -INFINITY;
-  const F y = value_of<MODE, SLOW>(w, l, lane < kLane ? i : -1, base, iz, table), run = head + warp_scan(y, lane);
-  hit = __ballot_sync(0xffffffffu, y > 0 && run > at);
-  if (!hit) {
-    unsure = true;
-    hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, y > 0)));
-  }
-  const int e = __ffs(hit) - 1;
-  const F hi = __shfl_sync(0xffffffffu, run, e), lo = e ? __shfl_sync(0xffffffffu, run, max(e - 1, 0)) : head;
+  const F y = value_of<MODE, SLOW>(w, l, lane < kLane ? i : -1, base, iz, table);
+  const int e = pick<F>(32, [&](int) { return y; }, &t, &unsure);
+  if (e < 0) return {-1, 1, 0.f, 0};
   if constexpr (kNarrow<MODE>) {
     const float off = band + 18.f * (float)kRound * mass;
-    unsure |= !(at - lo >= off && hi - at >= off);
+    unsure |= !(t >= off && __shfl_sync(0xffffffffu, y, e) - t >= off);
   }
   return {first + who * kLane + e, unsure, __shfl_sync(0xffffffffu, l, e), 0};
 }
@@ -477,6 +546,12 @@ __device__ __noinline__ int find_top(Row<T> w, const float* tops, const float* s
   return -1;
 }
 
+// (the numbers as they lie in memory: what uses them comes after the pass, and so does the wait for them)
+CFB_DEV double number(uint2 raw, int size) {
+  const double u = size == 4 ? (double)__uint_as_float(raw.x) : __hiloint2double((int)raw.y, (int)raw.x);
+  return fmin(fmax(u, 0.), 1. - 0x1p-32);                  // (an upper end that sums of 64 bits still resolve)
+}
+
 // What a cluster finds of a row. `ph` alternates the exchanged buffers.
 template <typename T> struct Team {
   Shared* sh;
@@ -486,7 +561,7 @@ template <typename T> struct Team {
 
   // How far an fp32 sum over the row may be from its side of a threshold, as a share of the row's mass z
   CFB_DEV float band(const Row<T>& w, float z) const {
-    return (float)kRound * (2.08f * (lg2((float)w.V) - lg2(z)) + 20.f);
+    return (float)kRound * (2.08f * (lg2((float)w.V) - lg2(z)) + 22.f + (float)w.each);
   }
 
   // The CTAs' totals, handed over by the cluster's barrier -> the row's; who has the threshold u of it. SCALED: each
@@ -540,75 +615,71 @@ template <typename T> struct Team {
   static CFB_DEV float threshold(float u, float whole) { return fminf(u * whole, whole * (1.f - 0x1p-23f)); }
   static CFB_DEV double threshold(double u, double whole) { return fmin(u * whole, whole * (1. - 0x1p-52)); }
 
+  // Warp 0: the warps' sums handed over
+  template <typename F> CFB_DEV void hand_over() {
+    const int lane = threadIdx.x;
+    F v = 0;
+    if (lane < kWarps) {
+      if constexpr (sizeof(F) == 8) v = sh->warp_sum64[lane];
+      else v = sh->warp_sum[lane];
+    }
+    v = warp_sum(v);
+    if (lane == 0) {
+      if constexpr (sizeof(F) == 8) sh->pub[ph].sum64 = v;
+      else sh->pub[ph].sum = v;
+    }
+  }
+
   // the pass over the row
-  CFB_DEV void stats(const Row<T>& w, double u, bool greedy) {
-    float* const sums = static_cast<float*>(room);
-    stats_units(w, tops, sums);
+  CFB_DEV void stats(const Row<T>& w, uint2 raw, int size, bool greedy) {
+    stats_units(w, sh, tops, static_cast<float*>(room));
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) {
-      const int lane = threadIdx.x, n = w.u1 - w.u0;
-      float top = -INFINITY;
-      bool nan = false;
-      for (int i = lane; i < n; i += 32) {
-        top = fmaxf(top, tops[i]);
-        nan |= sums[i] != sums[i];
-      }
-      top = warp_max(top);
-      nan = __any_sync(0xffffffffu, nan);
-      float before = 0.f;                                  // the units' sums become running ones, relative to the CTA's largest
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        const float v = warp_scan(i < n && !nan ? sums[i] * rescale(tops[i], top, w.c) : 0.f, lane);
-        if (i < n && !nan) sums[i] = before + v;
-        before += __shfl_sync(0xffffffffu, v, 31);
-      }
-      if (lane == 0) sh->pub[ph] = {top, nan, before, 0.f, 0.};
+      const int lane = threadIdx.x;
+      const float mine = lane < kWarps ? sh->warp_top[lane] : -INFINITY, sum = lane < kWarps ? sh->warp_sum[lane] : 0.f;
+      const float top = warp_max(mine);
+      const bool nan = __any_sync(0xffffffffu, sum != sum);
+      const float total = warp_sum(sum * rescale(mine, top, w.c));
+      if (lane == 0) sh->pub[ph] = {top, nan, nan ? 0.f : total, 0.f, 0.};
     }
-    exchange<float, true>(w, (float)u, greedy);
+    exchange<float, true>(w, (float)number(raw, size), greedy);
   }
 
   // a pass that knows the row's largest, and its sum where it needs it
   CFB_DEV void rest_pass(const Row<T>& w, double u) {
-    float* const sums = static_cast<float*>(room);
-    rest_units(w, sh->top, reciprocal((float)sh->z), sums);
+    rest_units(w, sh, sh->top, reciprocal((float)sh->z), static_cast<float*>(room));
     __syncthreads();
     ph ^= 1;
-    if (threadIdx.x < 32) {
-      const float sum = run_up(sums, w.u1 - w.u0, (int)threadIdx.x);
-      if (threadIdx.x == 0) sh->pub[ph].sum = sum;
-    }
+    if (threadIdx.x < 32) hand_over<float>();
     exchange<float, false>(w, (float)u, false);
   }
   template <int MODE, bool SLOW> CFB_DEV void exact_pass(const Row<T>& w, double u) {
-    double* const sums = static_cast<double*>(room);
-    exact_units<MODE, SLOW>(w, sh->top, MODE == R64 ? 1. / sh->z : 0., sums);
+    exact_units<MODE, SLOW>(w, sh, sh->top, MODE == R64 ? 1. / sh->z : 0., static_cast<double*>(room));
     __syncthreads();
     ph ^= 1;
-    if (threadIdx.x < 32) {
-      const double sum = run_up(sums, (w.u1 - w.u0) * (kUnit / kSpan<MODE>), (int)threadIdx.x);
-      if (threadIdx.x == 0) sh->pub[ph].sum64 = sum;
-    }
+    if (threadIdx.x < 32) hand_over<double>();
     exchange<double, false>(w, u, false);
   }
 
   // Warp 0 of the owner: the token of the last pass's threshold
   CFB_DEV Found found(const Row<T>& w, double u) const {
-    const float top = sh->pub[ph].top, scale = rescale(sh->top, top, w.c);        // (1 / what the part's sums were scaled by)
-    const float whole = (float)sh->whole, own = (float)(sh->end - sh->before) * scale;
-    if (isinf(top) || !(scale < INFINITY)) return {-1, 1, 0.f, 0};                 // several of +inf: in 64 bits
-    return find<W32, false>(w, static_cast<const float*>(room), (threshold((float)u, whole) - (float)sh->before) * scale, top, 0.,
-                            band(w, whole) * whole * scale + (float)kRound * (8 + (w.u1 - w.u0) / 32) * own);
+    if (isinf(sh->top)) return {-1, 1, 0.f, 0};            // several of +inf: in 64 bits
+    const float whole = (float)sh->whole;
+    return find<W32, false>(w, sh, tops, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before, 0.,
+                            band(w, whole) * whole + (float)kRound * (12 + 2 * w.each) * (float)(sh->end - sh->before));
   }
+  // (from what is left above q, R: every p is off by its exponent's error and 6 u, and all of them by 1 / Z's, of which
+  // C - u R keeps the share that q has where p is larger, at most 1 - R; sums of R by chains of 16, pairs and the warp)
   CFB_DEV Found found_rest(const Row<T>& w, double u) const {
-    // (of what is left above q, the error is that of the probabilities, whose whole is 1)
-    const float whole = (float)sh->whole, z = (float)sh->z, off = band(w, z) + 24 * (float)kRound;
+    const float whole = (float)sh->whole, z = (float)sh->z, mean = 2.08f * (lg2((float)w.V) - lg2(z)), other = fmaxf(1.f - whole, 0.f);
+    const float off = (float)kRound * (mean * (1.f + other) + 6.f + (40 + 2 * w.each) * other + (36 + 2 * w.each) * whole);
     if (!(whole > 2.f * off)) return {-1, 1, 0.f, 0};
-    return find<R32, false>(w, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before, sh->top,
-                            (double)reciprocal(z), off + (float)kRound * (8 + (w.u1 - w.u0) / 32) * whole);
+    return find<R32, false>(w, sh, tops, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before,
+                            (double)reciprocal(z), off);
   }
   template <int MODE, bool SLOW> CFB_DEV Found found64(const Row<T>& w, double u) const {
-    return find<MODE, SLOW>(w, static_cast<const double*>(room), threshold(u, sh->whole) - sh->before, sh->top,
+    return find<MODE, SLOW>(w, sh, tops, static_cast<const double*>(room), threshold(u, sh->whole) - sh->before,
                             MODE == R64 ? 1. / sh->z : 0., 0.f);
   }
 
@@ -622,11 +693,11 @@ template <typename T> struct Team {
 };
 
 // What a row is asked: drafted: it has a draft with probabilities, `draft`, which u accepts; v draws
-struct Asked { bool greedy, drafted; int draft; double u, v; };
-
+struct Asked { bool greedy, drafted; int draft, size; uint2 raw_u, raw_v; };
 // The row decided in 64 bits, its largest in sh.top. Every thread of the cluster gets the result (in bit 8 of accept,
 // whether the exchanged buffers have been alternated).
-template <bool CHAIN, bool SLOW, typename T> CFB_DEV RowResult exact_steps(Team<T> team, const Row<T>& w, const Asked& a) {
+template <bool CHAIN, bool SLOW, typename T>
+CFB_DEV RowResult exact_steps(Team<T> team, const Row<T>& w, const Asked& a, double u, double v) {
   Shared& sh = *team.sh;
   const int ph = team.ph;
   const auto result = [&](int token, int accept, float l) {
@@ -636,25 +707,25 @@ template <bool CHAIN, bool SLOW, typename T> CFB_DEV RowResult exact_steps(Team<
   Found f{-1, 1, 0.f, 0};
   bool rest = false;
   for (;;) {
-    team.template exact_pass<W64, SLOW>(w, a.v);
+    team.template exact_pass<W64, SLOW>(w, v);
     if (threadIdx.x == 0) sh.z = sh.whole;
     __syncthreads();
     if constexpr (CHAIN) {
       if (a.drafted && !rest) {
         if (a.draft >= 0 && a.draft < w.V) {
           const float l = to_float(w.p[a.draft]);
-          if (a.u * (double)draft_prob(w, a.draft) < weight64(l, sh.top, w.c64) / sh.z) return result(a.draft, 1, l);
+          if (u * (double)draft_prob(w, a.draft) < weight64(l, sh.top, w.c64) / sh.z) return result(a.draft, 1, l);
         }
-        team.template exact_pass<R64, SLOW>(w, a.v);
+        team.template exact_pass<R64, SLOW>(w, v);
         if (sh.whole > 0.) {
-          if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<R64, SLOW>(w, a.v);
+          if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<R64, SLOW>(w, v);
           break;
         }
         rest = true;                                       // nothing above q: the target's own
         continue;
       }
     }
-    if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<W64, SLOW>(w, a.v);
+    if (team.rank == sh.owner && threadIdx.x < 32) f = team.template found64<W64, SLOW>(w, v);
     break;
   }
   f = team.share(f);
@@ -662,56 +733,79 @@ template <bool CHAIN, bool SLOW, typename T> CFB_DEV RowResult exact_steps(Team<
 }
 template <bool CHAIN, typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
   // (weights below 2^-1020 count where the threshold is that small, and only there)
-  return isinf(team.sh->top) || a.v < 0x1p-900 || (CHAIN && a.u < 0x1p-900) ? exact_steps<CHAIN, true>(team, w, a)
-                                                                            : exact_steps<CHAIN, false>(team, w, a);
+  const double u = number(a.raw_u, a.size), v = number(a.raw_v, a.size);
+  const float top = team.sh->top, depth = (top - lowest_logit(top, w.c)) * w.c;       // (fp32 may not hold such a logit)
+  return isinf(top) || !(depth > 990.f && depth < 1010.f) || v < 0x1p-900 ? exact_steps<CHAIN, true>(team, w, a, u, v)
+                                                                          : exact_steps<CHAIN, false>(team, w, a, u, v);
 }
 
-// One row, by a whole cluster. LAZY: what fp32 does not decide is left undecided, and the result is valid in warp 0 of
-// the CTA *holder; otherwise every thread gets it.
+// What replaces a refused draft, the row's largest and the sum of its weights in sh. Every thread of the cluster gets it.
+template <typename T> __device__ __noinline__ RowResult other_token(Team<T> team, Row<T> w, Asked a) {
+  Shared& sh = *team.sh;
+  const int ph = team.ph;
+  const double v = number(a.raw_v, a.size);
+  team.rest_pass(w, v);
+  Found f{-1, 1, 0.f, 0};
+  if (team.rank == sh.owner && threadIdx.x < 32) f = team.found_rest(w, v);
+  f = team.share(f);
+  if (f.unsure) {
+    RowResult r = exact_row<true>(team, w, a);
+    r.accept ^= (team.ph ^ ph) << 8;
+    return r;
+  }
+  const double scaled = f.logit == sh.top ? 0. : ((double)f.logit - (double)sh.top) * w.c64;
+  return {f.token, (team.ph ^ ph) << 8, scaled, sh.z};
+}
+
+// One row, by a whole cluster. LAZY: what fp32 does not decide, and what replaces a refused draft, is left for the walk, and
+// the result is valid in warp 0 of the CTA *holder; otherwise every thread gets it.
 template <bool CHAIN, bool LAZY, typename T>
 CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, const Asked& a, int* holder) {
   Shared& sh = *team.sh;
   const bool in = CHAIN && a.drafted && a.draft >= 0 && a.draft < w.V;       // a draft that is no token is refused
   const float of_draft = in ? to_float(w.p[a.draft]) : -INFINITY, q = in ? draft_prob(w, a.draft) : 0.f;
-  team.stats(w, a.v, a.greedy);
+  team.stats(w, a.raw_v, a.size, a.greedy);
   const auto scaled = [&](float l) { return l == sh.top ? 0. : ((double)l - (double)sh.top) * w.c64; };     // log2
+  const auto later = [&](int what) { return RowResult{-1, what, (double)sh.top, sh.z}; };
+  const auto taken = [&](RowResult r) {
+    team.ph ^= r.accept >> 8;
+    r.accept &= 1;
+    return r;
+  };
   *holder = 0;
   if (sh.kind == ROW_EMPTY) return {-1, 0, 0., 1.};
-  Found f{-1, 1, 0.f, 0};
   const bool plain = a.greedy || sh.kind == ROW_NAN;
-  bool unsure = false;
   if (CHAIN && a.drafted && !plain) {
     if (in) {
-      const float z = (float)sh.z, x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) * reciprocal(z), uq = (float)a.u * q;
+      const float z = (float)sh.z, x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) * reciprocal(z);
+      const float uq = (float)number(a.raw_u, a.size) * q;
       // (every CTA computes the same)
       const float off = p * (2.f * team.band(w, z) + (float)kRound * (2.08f * fabsf(x) + 16.f));
-      unsure = !(fabsf(uq - p) > off);
-      if (!unsure && uq < p) return {a.draft, 1, scaled(of_draft), sh.z};
+      if (!(fabsf(uq - p) > off)) {
+        if constexpr (LAZY) return later(kUndecided);
+        else return taken(exact_row<CHAIN>(team, w, a));
+      }
+      if (uq < p) return {a.draft, 1, scaled(of_draft), sh.z};
     }
-    if (!unsure) team.rest_pass(w, a.v);
+    if constexpr (LAZY) return later(kRefused);
+    else return taken(other_token(team, w, a));
   }
-  if (!unsure) {
-    *holder = sh.owner;
-    if (team.rank == sh.owner && threadIdx.x < 32) {
-      if (plain) f = {find_top(w, team.tops, static_cast<const float*>(team.room), sh.top, sh.kind == ROW_NAN), 0, sh.top, 0};
-      else if (!CHAIN || !a.drafted) f = team.found(w, a.v);
-      else f = team.found_rest(w, a.v);
-    }
-    if constexpr (!LAZY) f = team.share(f);
-    unsure = f.unsure;
+  *holder = sh.owner;
+  Found f{-1, 1, 0.f, 0};
+  if (team.rank == sh.owner && threadIdx.x < 32) {
+    if (plain) f = {find_top(w, team.tops, static_cast<const float*>(team.room), sh.top, sh.kind == ROW_NAN), 0, sh.top, 0};
+    else f = team.found(w, number(a.raw_v, a.size));
   }
-  if (unsure) {
-    if constexpr (LAZY) return {-1, kUndecided, (double)sh.top, 1.};
-    const RowResult r = exact_row<CHAIN>(team, w, a);
-    team.ph ^= r.accept >> 8;
-    return {r.token, r.accept & 1, r.scaled, r.mass};
+  if constexpr (!LAZY) f = team.share(f);
+  if (f.unsure) {
+    if constexpr (LAZY) return later(kUndecided);
+    else return taken(exact_row<CHAIN>(team, w, a));
   }
   return {f.token, CHAIN && plain && a.drafted && f.token == a.draft, sh.kind == ROW_NAN ? (double)NAN : scaled(f.logit), sh.z};
 }
 
-CFB_DEV double number_at(const void* p, int size, long long i) {
-  const double u = size == 4 ? (double)static_cast<const float*>(p)[i] : static_cast<const double*>(p)[i];
-  return fmin(fmax(u, 0.), 1. - 0x1p-32);                  // (an upper end that sums of 64 bits still resolve)
+CFB_DEV uint2 number_at(const void* p, int size, long long i) {
+  return size == 4 ? make_uint2(__ldg(static_cast<const uint32_t*>(p) + i), 0) : __ldg(static_cast<const uint2*>(p) + i);
 }
 
 // row j of request b, and what it is asked
@@ -723,21 +817,23 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
   const int units = (w.V + w.shift + kUnit - 1) / kUnit;
   w.u0 = min(rank * per, units);
   w.u1 = min(w.u0 + per, units);
+  w.each = (per + kWarps - 1) / kWarps;
   a.greedy = !(temp >= kLowTemp);
   const float tau = a.greedy ? 1.f : fminf(temp, kHighTemp);
   w.c64 = tau == 1.f ? 1.4426950408889634 : 1.4426950408889634 / (double)tau;
-  w.c = (float)fmin(w.c64, 3.4e38);
-  w.q = nullptr;
+  w.c = fminf((float)w.c64, 3.4e38f);
+  w.probs = nullptr;
   w.index_of = A.index_of;
   a.drafted = CHAIN && j < n;
   a.draft = a.drafted ? A.draft_tokens[d0 + j] : -1;
-  a.u = a.drafted ? number_at(A.uniforms, A.uniform_size, d0 + j) : 0.;
-  a.v = CHAIN ? number_at(A.resample, A.uniform_size, b) : number_at(A.uniforms, A.uniform_size, s0 + j);
-  if (a.drafted) w.q = A.probs + (long long)(d0 + j) * A.ld_probs;
+  a.size = A.uniform_size;
+  a.raw_u = a.drafted ? number_at(A.uniforms, A.uniform_size, d0 + j) : make_uint2(0, 0);
+  a.raw_v = CHAIN ? number_at(A.resample, A.uniform_size, b) : number_at(A.uniforms, A.uniform_size, s0 + j);
+  if (a.drafted) w.probs = A.probs + (long long)(d0 + j) * A.ld_probs;
 }
 
 // FLAT: a cluster a row (grid.y: rows of a request, grid.z: requests), every row at once; the request's last
-// cluster walks, and decides the rows that its walk meets undecided. Otherwise a cluster a request (grid.y), which
+// cluster walks, and takes again what was left for the walk where it comes by. Otherwise a cluster a request (grid.y), which
 // takes the rows of its walk in turn. CHAIN: draft probabilities; a node's only child is the next one.
 template <typename T, bool CHAIN, bool FLAT>
 __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs A, int per) {
@@ -805,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
     if constexpr (FLAT && !CHAIN) {
       for (int i = threadIdx.x; i < n; i += kThreads) {
         const int up = s_parent[i] + 1;                    // the row that leads to node i
-        if (up >= 0 && up <= n && s_row[up].accept != kUndecided && s_row[up].token >= 0 && s_row[up].token == s_token[i])
+        if (up >= 0 && up <= n && s_row[up].accept < kUndecided && s_row[up].token >= 0 && s_row[up].token == s_token[i])
           atomicMin(s_next + up, i);
       }
       __syncthreads();
@@ -820,11 +916,15 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
       bool known = FLAT;
       if constexpr (FLAT) {
         r = s_row[cur + 1];
-        if (r.accept == kUndecided) {
+        if (r.accept >= kUndecided) {
           row_of<T, CHAIN>(A, rank, per, b, d0, n, s0, cur + 1, temp, w, a);
-          if (threadIdx.x == 0) sh.top = (float)r.scaled;
+          if (threadIdx.x == 0) {
+            sh.top = (float)r.scaled;
+            sh.z = r.mass;
+          }
           __syncthreads();
-          r = exact_row<CHAIN>(team, w, a);
+          if constexpr (CHAIN) r = r.accept == kRefused ? other_token(team, w, a) : exact_row<true>(team, w, a);
+          else r = exact_row<false>(team, w, a);
           team.ph ^= r.accept >> 8;
           r.accept &= 1;
           if (threadIdx.x == 0) s_row[cur + 1] = r;
@@ -881,12 +981,44 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   }
 }
 
+// clusters of a size that the current device holds at a time, asked of the runtime once a device
+template <typename T, bool CHAIN, bool FLAT> int resident(int cluster) {
+  static std::atomic<int> known[64][kMaxCluster + 1];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 64 && (n = known[dev][cluster].load(std::memory_order_relaxed)) > 0) return n;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = 16384;                            // (a large vocabulary's or tree's share of an SM)
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, verify_kernel<T, CHAIN, FLAT>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (n > 0 && dev < 64) known[dev][cluster].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <typename T, bool CHAIN, bool FLAT>
-cfb_status launch(const VerifyArgs& a, int cluster, cudaStream_t st) {
+cfb_status launch(const VerifyArgs& a, cudaStream_t st) {
   const auto bytes = [](long long units, long long spec) { return (int)(units * (kUnit / kSpan<W64> * 8 + 4) + (spec + 1) * 32 + spec * 8); };
-  const long long units = (a.V + 7 + kUnit - 1) / kUnit, per = (units + cluster - 1) / cluster;
   if (allow_smem<verify_kernel<T, CHAIN, FLAT>>(bytes(kMaxVocab / kUnit + 2, kMaxNodes)) != cudaSuccess)
     return cfb_launch_status("verify_kernel");
+  const long long units = (a.V + 7 + kUnit - 1) / kUnit;
+  // as large clusters as are resident together (a cluster that waits for another's end doubles the time)
+  const long long teams = FLAT ? a.num_rows : a.batch;
+  int cluster = kMaxCluster;
+  while (cluster > 1 && (cluster > units || teams > resident<T, CHAIN, FLAT>(cluster))) --cluster;
+  const long long per = (units + cluster - 1) / cluster;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = FLAT ? dim3(cluster, a.max_spec + 1, a.batch) : dim3(cluster, a.batch, 1);
   cfg.blockDim = dim3(kThreads);
@@ -903,16 +1035,13 @@ cfb_status launch(const VerifyArgs& a, int cluster, cudaStream_t st) {
 }
 
 template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaStream_t st) {
-  const int sms = device_sms() > 0 ? device_sms() : 148;
-  const long long row = (long long)a.V * (dtype == DT_F32 ? 4 : 2);
-  const bool flat = row * a.num_rows <= (64ll << 20);
-  // clusters of as many CTAs as the rows at hand leave SMs for
-  const long long teams = flat ? a.num_rows : a.batch;
-  int cluster = kMaxCluster;
-  while (cluster > 1 && teams * cluster > 2 * sms) cluster >>= 1;
+  // All rows at once take the GPU's whole width, but read what no walk reaches, and with more rows there are fewer CTAs
+  // for the ones that it takes again. Measured, walk against all rows, V = 248320, us: 6 rows (one chain) 22 / 16, 48 rows
+  // (8 chains) 56 / 37, 41 rows (one tree) 24 / 24, 82 (two trees) 30 / 44, 192 (32 chains) 71 / 137.
+  const bool flat = (long long)a.V * a.num_rows <= 12ll << 20;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    return flat ? launch<T, CHAIN, true>(a, cluster, st) : launch<T, CHAIN, false>(a, cluster, st);
+    return flat ? launch<T, CHAIN, true>(a, st) : launch<T, CHAIN, false>(a, st);
   };
   if (dtype == DT_F32) return go(float{});
   if (dtype == DT_F16) return go(__half{});
