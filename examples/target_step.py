@@ -3,6 +3,10 @@ with random projections: prompts into the paged cache and the recurrent states, 
 against both, the accepted path committed, a plain decode.
 
     PYTHONPATH=. python examples/target_step.py [--cache e4m3|fp16] [--prompts 700,33,1]
+
+With ``--temperature`` the steps are sampled (SampledTarget): pages come from a pool, each prompt's pages are
+forked to several samples, the trees are verified against the target's probabilities from given random numbers, and
+the accepted rows are moved together in the cache; nothing is read back between the steps.
 """
 from __future__ import annotations
 
@@ -12,8 +16,8 @@ import torch
 
 from chain_flow_b200.attention import PagedAttention
 from chain_flow_b200.gdn import ChunkedGdn, ancestor_chains, gdn_step, gdn_verify, make_tree
-from chain_flow_b200.kv_cache import PagedKVCache
-from chain_flow_b200.tree import ancestor_mask, tree_attn_merge
+from chain_flow_b200.kv_cache import PagedKVCache, PagePool, keep_path
+from chain_flow_b200.tree import SampledVerifier, ancestor_mask, tree_attn_merge
 
 HEADS, KV_HEADS, HEAD_DIM = 16, 4, 256           # the attention layer
 KEY_HEADS, VALUE_HEADS, KEY_DIM, VALUE_DIM = 16, 32, 128, 128    # the gated-delta layer
@@ -95,6 +99,51 @@ class TargetLayers:
         return attn, o
 
 
+class SampledTarget(TargetLayers):
+    """The same layers with pages from a pool, sampled verification and samples that share a prompt's pages. A tree's
+    nodes are in the cache while they are verified, node i at position kv_len + i."""
+
+    def __init__(self, requests: int, max_len: int, nodes: int, dtype=torch.float16, cache_dtype=torch.float8_e4m3fn, seed: int = 0):
+        super().__init__(requests, max_len, nodes, dtype, cache_dtype, seed)
+        self.pool = PagePool(self.cache.pages, PAGE)
+        self.table = torch.full_like(self.table, -1)
+        self.verifier = SampledVerifier(requests * (nodes + 1), requests, nodes)
+        self.granted = []                                # per call: 0 where the pool had no pages left
+
+    def prompt(self, x, news):
+        self.granted.append(self.pool.reserve(self.table, self.kv_len, torch.tensor(news, device="cuda")))
+        return super().prompt(x, news)
+
+    def fork(self, parent, child):
+        """Requests ``child`` (without a context) become copies of requests ``parent``: one prompt, several samples."""
+        self.granted.append(self.pool.fork(self.table, self.kv_len, parent, child, self.cache))
+        self.state[child.long()] = self.state[parent.long()]
+
+    def sampled_step(self, x, parents, tokens, logits, uniforms, temperature=None):
+        """A tree of N nodes a request that carry ``tokens`` [S, N]; logits [S * (N + 1), V] of the committed token's row
+        and the nodes', request after request, and a random number for each. Returns both layers' outputs and the
+        verifier's (tokens, path, length, log probabilities); the accepted nodes have joined the contexts."""
+        S, N = parents.shape
+        self.granted.append(self.pool.reserve(self.table, self.kv_len, self.kv_len + N))
+        request, node = self.slot.long().repeat_interleave(N), torch.arange(N, device="cuda").repeat(S)
+        self.cache.write(x["k"], x["v"], self.slots_of(request, self.kv_len[request] + node))
+        attn, o = self.verify(x, parents)
+        drafts = torch.arange(1, S + 1, device="cuda", dtype=torch.int32)
+        out = self.verifier(logits, drafts * N, drafts * (N + 1), tokens.reshape(-1), parents.reshape(-1), uniforms, temperature)
+        path, length = out[1], out[2]
+        keep_path(self.cache, self.table, self.kv_len, path, length)
+        last = path.gather(1, (length.long() - 1).clamp_min(0)[:, None])[:, 0]
+        self.state[:S] = self.state[torch.where(length > 0, S + self.slot * N + last, self.slot).long()]
+        end = self.kv_len + N
+        self.kv_len = self.kv_len + length
+        self.pool.release(self.table, end, self.kv_len)  # the refused nodes' pages
+        return attn, o, out
+
+    def decode(self, x):
+        self.granted.append(self.pool.reserve(self.table, self.kv_len, self.kv_len + 1))
+        return super().decode(x)
+
+
 def projections(tokens: int, dtype=torch.float16, seed: int = 0):
     """What the two layers' projections would give for ``tokens`` tokens."""
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -109,8 +158,12 @@ def main():
     p.add_argument("--cache", choices=("e4m3", "fp16"), default="e4m3")
     p.add_argument("--prompts", default="700,33,1")
     p.add_argument("--nodes", type=int, default=12)
+    p.add_argument("--temperature", type=float, help="sampled steps at this temperature")
+    p.add_argument("--samples", type=int, default=2, help="samples of each prompt (with --temperature)")
     a = p.parse_args()
     news = [int(n) for n in a.prompts.split(",")]
+    if a.temperature is not None:
+        return sampled(a, news)
     layers = TargetLayers(len(news), max(news) + a.nodes + 1, a.nodes,
                           cache_dtype=torch.float8_e4m3fn if a.cache == "e4m3" else torch.float16)
     out = layers.prompt(projections(sum(news), seed=1), news)
@@ -130,6 +183,32 @@ def main():
     layers.attention.check()
     layers.chunks.check()
     print("accepted", paths, "decoded", *(tuple(t.shape) for t in out), "contexts", layers.kv_len.tolist())
+
+
+def sampled(a, news, vocab: int = 1000, steps: int = 3):
+    """Samples of each prompt: the prompts' pages forked, a few sampled steps, a decode."""
+    P, S = len(news), len(news) * a.samples
+    layers = SampledTarget(S, max(news) + steps * a.nodes + 1, a.nodes,
+                           cache_dtype=torch.float8_e4m3fn if a.cache == "e4m3" else torch.float16)
+    layers.prompt(projections(sum(news), seed=1), news + [0] * (S - P))
+    child = torch.arange(P, S, device="cuda")
+    layers.fork(child % P, child)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for step in range(steps):
+        parents = torch.stack([make_tree(a.nodes, 4, 3, seed=step * S + b)[0] for b in range(S)]).cuda()
+        logits = 3 * torch.randn(S * (a.nodes + 1), vocab, device="cuda", generator=g)
+        # drafts that their parents' rows favour, as a drafter's are
+        rows = logits.view(S, a.nodes + 1, vocab).topk(3, dim=2).indices.gather(1, (parents + 1)[..., None].expand(-1, -1, 3))
+        tokens = rows.gather(2, (torch.arange(a.nodes, device="cuda") % 3).expand(S, -1)[..., None])[..., 0]
+        uniforms = torch.rand(S * (a.nodes + 1), device="cuda", generator=g)
+        _, _, out = layers.sampled_step(projections(S * a.nodes, seed=2 + step), parents, tokens, logits, uniforms,
+                                        torch.full((S,), a.temperature, device="cuda"))
+        print("step", step, "accepted", out[2].tolist(), "tokens", [[t for t in row if t >= 0] for row in out[0].tolist()])
+    out = layers.decode(projections(S, seed=9))
+    layers.attention.check()
+    layers.chunks.check()
+    print("decoded", *(tuple(t.shape) for t in out), "contexts", layers.kv_len.tolist(), "pages held", int((layers.pool.refs > 0).sum()),
+          "all granted", all(bool(t.all()) for t in layers.granted))
 
 
 if __name__ == "__main__":
