@@ -53,7 +53,7 @@ struct VerifyArgs {
   const void* logits; long long ld; int V, num_rows;
   const int32_t* cu_draft; const int32_t* cu_sampled;      // [batch]
   const int32_t* draft_tokens; const int32_t* parents;     // parents: trees only
-  const float* probs; long long ld_probs;                  // draft probabilities [drafts, probs_width]
+  const float* probs; long long ld_probs; int probs_width; // draft probabilities [drafts, probs_width]
   const int32_t* index_of;                                 // [V] column of a token, or -1; NULL: the token itself
   const void* uniforms; const void* resample; int uniform_size;   // 4 or 8 bytes
   const float* temperature;
@@ -151,6 +151,7 @@ template <typename T> struct Row {
   double c64;
   const float* probs;         // draft probabilities of the row, or null
   const int32_t* index_of;
+  int width;                  // columns that index_of may name
 };
 template <typename T> constexpr int kE = 16 / (int)sizeof(T);          // elements a vector
 template <typename T> constexpr int kVectors = kPerLane / kE<T>;       // vectors of a unit a lane
@@ -247,7 +248,7 @@ CFB_DEV double weight64(float l, float base, double c) {
 template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
   if (i < 0 || i >= w.V) return 0.f;
   const int at = w.index_of ? __ldg(w.index_of + i) : i;
-  return at >= 0 ? fmaxf(__ldg(w.probs + at), 0.f) : 0.f;
+  return (unsigned)at < (unsigned)w.width ? fmaxf(__ldg(w.probs + at), 0.f) : 0.f;
 }
 
 enum Mode : int { W32 = 0, W64 = 1, R32 = 2, R64 = 3 };    // weights, or what is left of them above q
@@ -349,7 +350,7 @@ template <typename T> CFB_DEV void draft_probs(const Row<T>& w, int i, int n, fl
     table_entries(w.index_of, i, n, w.V, at, -1);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) q[e] = at[e] >= 0 ? __ldg(w.probs + at[e]) : 0.f;
+      if (e < n) q[e] = (unsigned)at[e] < (unsigned)w.width ? __ldg(w.probs + at[e]) : 0.f;
   } else {
     table_entries(w.probs, i, n, w.V, q, 0.f);
   }
@@ -824,6 +825,7 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
   w.c = fminf((float)w.c64, 3.4e38f);
   w.probs = nullptr;
   w.index_of = A.index_of;
+  w.width = A.index_of ? A.probs_width : A.V;
   a.drafted = CHAIN && j < n;
   a.draft = a.drafted ? A.draft_tokens[d0 + j] : -1;
   a.size = A.uniform_size;
@@ -852,9 +854,10 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   const int b = FLAT ? blockIdx.z : blockIdx.y;
   const int d0 = b ? A.cu_draft[b - 1] : 0;
   const long long drafts = (long long)A.cu_draft[b] - d0, start = A.cu_sampled[b] - (drafts + 1);
+  const int before = b ? A.cu_sampled[b - 1] : 0;
   const float temp = A.temperature ? A.temperature[b] : 1.f;
-  // offsets that do not describe rows of this logits matrix (or drafts) are never dereferenced
-  const bool sane = drafts >= 0 && drafts <= A.max_spec && start >= 0 && start + drafts < A.num_rows && d0 >= 0 &&
+  // offsets that do not describe rows of this logits matrix (or drafts), of this request alone, are never dereferenced
+  const bool sane = drafts >= 0 && drafts <= A.max_spec && start >= max(before, 0) && start + drafts < A.num_rows && d0 >= 0 &&
                     d0 + drafts <= A.num_drafts;
   const int n = (int)drafts, s0 = (int)start;
   // a thread's node of the tree, on its way while the rows are taken
@@ -1038,7 +1041,8 @@ template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaS
   // All rows at once take the GPU's whole width, but read what no walk reaches, and with more rows there are fewer CTAs
   // for the ones that it takes again. Measured, walk against all rows, V = 248320, us: 6 rows (one chain) 22 / 16, 48 rows
   // (8 chains) 56 / 37, 41 rows (one tree) 24 / 24, 82 (two trees) 30 / 44, 192 (32 chains) 71 / 137.
-  const bool flat = (long long)a.V * a.num_rows <= 12ll << 20;
+  // (and a cluster goes to every row that a request may have: many that have none would cost more than they save)
+  const bool flat = (long long)a.V * a.num_rows <= 12ll << 20 && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
   const auto go = [&](auto t) {
     using T = decltype(t);
     return flat ? launch<T, CHAIN, true>(a, st) : launch<T, CHAIN, false>(a, st);
@@ -1113,6 +1117,7 @@ extern "C" cfb_status cfb_chain_verify_rejection(const void* logits, int64_t ld,
   if (!index_of && probs_width != V) return CFB_ERR_INVALID_ARG;
   a.probs = draft_probs;
   a.ld_probs = ld_probs;
+  a.probs_width = probs_width;
   a.index_of = index_of;
   a.resample = resample;
   return launch_as<true>(a, dtype, static_cast<cudaStream_t>(stream));

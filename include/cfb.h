@@ -398,8 +398,8 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * is distributed as the target's own, whatever the tree.
  * cfb_chain_verify_rejection: each request's drafts are a chain, draft i (flat) was drawn from the
  * probabilities q = draft_probs[i] (fp32 rows of probs_width, row stride ld_probs) over the whole
- * vocabulary (index_of NULL, probs_width V) or over columns: token x has column index_of[x] < probs_width,
- * or -1: probability 0 (what is not a positive number counts as 0). With p the row's probabilities, draft
+ * vocabulary (index_of NULL, probs_width V) or over columns: token x has column index_of[x], or (-1, or
+ * probs_width and more) probability 0 (what is not a positive number counts as 0). With p the row's probabilities, draft
  * token d stays if uniforms[i] q_d < p_d (uniforms: one for each draft); the first that does not is
  * replaced by a draw of resample[r] from max(p - q, 0), or p where that is nowhere positive; if all
  * stay, resample[r] draws the bonus token from the last row. A greedy row keeps d if it is the

@@ -290,7 +290,7 @@ def test_offsets_that_fit_nothing(big):
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
     u = torch.rand(rows, device="cuda")
     for cu_d, cu_s in ((i32(2, 4), i32(3, rows + 3)), (i32(2, 9), i32(3, 6)), (i32(2, 1), i32(3, 6)), (i32(2, 4), i32(3, 1)),
-                       (i32(2, -1 << 31), i32(3, 6))):
+                       (i32(2, -1 << 31), i32(3, 6)), (i32(2, 4), i32(3, 5))):          # (the last: another request's row)
         ver = SampledVerifier(rows, 2, 3)
         out, path, count, logp = ver(logits, cu_d, cu_s, tok, par, u)
         assert int(ver.err.item()) == 7 and out[1].tolist() == [-1] * 4 and path[1].tolist() == [-1] * 3 and int(count[1]) == 0
@@ -485,3 +485,49 @@ def test_capture_streams_and_refusals(monkeypatch):
         ver(*dev)
     with pytest.raises(_lib.CfbError, match="current device"):
         rej(lg, cu_d, cu_s, tok, q, u[:9], u[:3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [777, 4096, 40001])
+def test_rows_that_are_odd_in_16_bits(dtype, V):
+    from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
+    g = torch.Generator().manual_seed(V)
+    info, inf = torch.finfo(dtype), math.inf
+    rows = []
+    for change in (lambda r: None, lambda r: r.fill_(info.min), lambda r: r.fill_(-inf), lambda r: r[5:].fill_(info.min),
+                   lambda r: (r.fill_(-inf), r[V - 1:].fill_(-3.0)), lambda r: r[[1, V - 2]].fill_(inf), lambda r: r.__setitem__(torch.tensor([1, V - 2]), inf),
+                   lambda r: r.__setitem__(700, math.nan), lambda r: (r.fill_(info.min), r.__setitem__(V // 2, info.max)), lambda r: r.fill_(0),
+                   lambda r: r.fill_(info.max), lambda r: r.mul_(100)):
+        row = (torch.randn(V, generator=g) * 3).to(dtype)
+        change(row)
+        rows += [row] * 4
+    n = len(rows)
+    logits, u = torch.stack(rows), torch.rand(n, generator=g, dtype=torch.float64)
+    temp = torch.tensor([1.0, 0.0, 0.2, 3.0] * (n // 4))
+    flat = (torch.zeros(n, dtype=torch.int32), torch.arange(1, n + 1, dtype=torch.int32), torch.empty(0, dtype=torch.int32),
+            torch.empty(0, dtype=torch.int32))
+    _check(_sampled(SampledVerifier(n, n, 0), logits, flat, u, temp), oracle.tree_verify_sampled(logits, *flat, u, temp, 0))
+    both = torch.stack([r for row in rows for r in (row, rows[0])])
+    tok = torch.randint(V, (n,), generator=g, dtype=torch.int32)
+    tok[::3] = both[::2].float().nan_to_num(0).argmax(1).int()[::3]
+    q = torch.softmax(torch.randn(n, V, generator=g) * 3, 1)
+    flat = (torch.arange(1, n + 1).int(), (2 * torch.arange(1, n + 1)).int(), tok)
+    args = (both, *flat, q, u, torch.rand(n, generator=g, dtype=torch.float64), temp)
+    ver = RejectionVerifier(2 * n, n, 1, V)
+    _check(_rejected(ver, both, flat, *args[4:]), oracle.chain_verify_rejection(*args, 1))
+
+
+@pytest.mark.gpu
+def test_verifiers_far_larger_than_their_calls():
+    """A verifier for 1024 drafts and many requests, given few; lists that name columns outside the draft probabilities."""
+    from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
+    logits, flat, u = _case([3, 0, 7], 2000, torch.float32, 5)
+    ver = SampledVerifier(4000, 900, 1024)
+    _check(_sampled(ver, logits, flat, u), oracle.tree_verify_sampled(logits, *flat, u, None, 1024))
+    V = 600
+    logits, flat, probs, u, v = _chains([4, 2], V, torch.float16, 3)
+    ver = RejectionVerifier(50, 9, 64, V, draft_ids=torch.arange(V))
+    ver.index_of[::2] = 1 << 30                          # as a C caller's list may be wrong: read as probability 0
+    probs[:, ::2] = 0
+    _check(_rejected(ver, logits, flat, probs, u, v), oracle.chain_verify_rejection(logits, *flat, probs, u, v, None, 64))
