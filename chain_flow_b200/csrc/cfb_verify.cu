@@ -35,11 +35,14 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
+// Small CTAs, several an SM, in large clusters: their serial steps cover one another (a batch of 64 trees 80 us with 2 CTAs of
+// 512 threads an SM, 71 with 4 of 256). Chains, whose steps hold more, take 80 registers a thread and 3 CTAs an SM (48
+// chains 104 us; with 4 CTAs 116), trees 64 and 4 (64 trees 71; with 3 CTAs 78).
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPerLane = 32;                 // elements of a unit in a lane's registers
 constexpr int kUnit = 32 * kPerLane;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kMaxVocab = 1 << 22;
 constexpr int kMaxNodes = 1024;              // draft nodes per request (max_spec_len)
 constexpr double kRound = 1.0 / 16777216;    // 2^-24
@@ -272,18 +275,15 @@ CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, do
   }
 }
 
-// every unit's largest and its sum of weights relative to that; a unit's loads are under way while the one before is summed
+// every unit's largest and its sum of weights relative to that. (Other warps cover a unit's loads: the next unit's under way in
+// registers cost a batch of chains 145 us against 129.)
 template <typename T> CFB_DEV void stats_units(const Row<T>& w, Shared* sh, float* tops, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = w.u0 + warp * w.each, end = min(first + w.each, w.u1);
-  uint4 next[kVectors<T>];
   float most = -INFINITY, total = 0.f;
-  if (first < end) load_unit(w, first, lane, next);
   for (int u = first; u < end; ++u) {
     uint4 v[kVectors<T>];
-#pragma unroll
-    for (int j = 0; j < kVectors<T>; ++j) v[j] = next[j];
-    if (u + 1 < end) load_unit(w, u + 1, lane, next);
+    load_unit(w, u, lane, v);
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVectors<T>; ++j) m = fmaxf(m, vector_max<T>(v[j]));
@@ -838,7 +838,7 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
 // cluster walks, and takes again what was left for the walk where it comes by. Otherwise a cluster a request (grid.y), which
 // takes the rows of its walk in turn. CHAIN: draft probabilities; a node's only child is the next one.
 template <typename T, bool CHAIN, bool FLAT>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs A, int per) {
+__global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const __grid_constant__ VerifyArgs A, int per) {
   extern __shared__ double s_dyn[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -984,6 +984,16 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const __grid_consta
   }
 }
 
+// clusters of more than 8 CTAs allowed, once a device
+template <typename T, bool CHAIN, bool FLAT> cudaError_t allow_clusters() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T, CHAIN, FLAT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
 // clusters of a size that the current device holds at a time, asked of the runtime once a device
 template <typename T, bool CHAIN, bool FLAT> int resident(int cluster) {
   static std::atomic<int> known[64][kMaxCluster + 1];
@@ -1014,7 +1024,8 @@ template <typename T, bool CHAIN, bool FLAT> int resident(int cluster) {
 template <typename T, bool CHAIN, bool FLAT>
 cfb_status launch(const VerifyArgs& a, cudaStream_t st) {
   const auto bytes = [](long long units, long long spec) { return (int)(units * (kUnit / kSpan<W64> * 8 + 4) + (spec + 1) * 32 + spec * 8); };
-  if (allow_smem<verify_kernel<T, CHAIN, FLAT>>(bytes(kMaxVocab / kUnit + 2, kMaxNodes)) != cudaSuccess)
+  if (allow_smem<verify_kernel<T, CHAIN, FLAT>>(bytes(kMaxVocab / kUnit + 2, kMaxNodes)) != cudaSuccess ||
+      allow_clusters<T, CHAIN, FLAT>() != cudaSuccess)
     return cfb_launch_status("verify_kernel");
   const long long units = (a.V + 7 + kUnit - 1) / kUnit;
   // as large clusters as are resident together (a cluster that waits for another's end doubles the time)
@@ -1039,10 +1050,11 @@ cfb_status launch(const VerifyArgs& a, cudaStream_t st) {
 
 template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaStream_t st) {
   // All rows at once take the GPU's whole width, but read what no walk reaches, and with more rows there are fewer CTAs
-  // for the ones that it takes again. Measured, walk against all rows, V = 248320, us: 6 rows (one chain) 22 / 16, 48 rows
-  // (8 chains) 56 / 37, 41 rows (one tree) 24 / 24, 82 (two trees) 30 / 44, 192 (32 chains) 71 / 137.
+  // for what the walk takes again. Measured, walk against all rows, us. Trees, V = 248320: 6 rows (one chain) 18 / 13, 41 (one
+  // tree) 20 / 21, 48 (8 chains) 45 / 34, 82 (two trees) 24 / 35; V = 32003: 384 (64 chains) 65 / 40, 656 (16 trees)
+  // 39 / 47. Chains with draft probabilities, V = 248320: 6 rows 25 / 17, 24 54 / 54, 48 56 / 72; V = 32003: 96 48 / 42, 288 65 / 81.
   // (and a cluster goes to every row that a request may have: many that have none would cost more than they save)
-  const bool flat = (long long)a.V * a.num_rows <= 12ll << 20 && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
+  const bool flat = (long long)a.V * a.num_rows <= (CHAIN ? 5ll : 12ll) << 20 && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
   const auto go = [&](auto t) {
     using T = decltype(t);
     return flat ? launch<T, CHAIN, true>(a, st) : launch<T, CHAIN, false>(a, st);
