@@ -45,6 +45,9 @@ constexpr int kUnit = 32 * kPerLane;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxVocab = 1 << 22;
 constexpr int kMaxNodes = 1024;              // draft nodes per request (max_spec_len)
+constexpr int kMaxBatch = 65535;
+// the workspace: a counter for every request that a call may have, so that no call's rows lie where another's counters do
+constexpr size_t kCounters = (kMaxBatch + 1) * sizeof(unsigned);
 constexpr double kRound = 1.0 / 16777216;    // 2^-24
 constexpr float kLowTemp = 1.17549435e-38f;  // 2^-126: below it (or NaN) a request is greedy
 constexpr float kHighTemp = 1.26765060e30f;  // 2^100
@@ -1073,7 +1076,7 @@ cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_ro
   if (!logits || !cu_draft || !cu_sampled || !out_tokens || !out_len || !out_logp || !ws) return CFB_ERR_INVALID_ARG;
   if (num_drafts < 0 || (num_drafts > 0 && !draft_tokens)) return CFB_ERR_INVALID_ARG;
   if (dtype < DT_F32 || dtype > DT_BF16 || (uniform_size != 4 && uniform_size != 8)) return CFB_ERR_UNSUPPORTED;
-  if (max_spec > kMaxNodes || V > kMaxVocab - 8 || batch > 65535) return CFB_ERR_UNSUPPORTED;
+  if (max_spec > kMaxNodes || V > kMaxVocab - 8 || batch > kMaxBatch) return CFB_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return CFB_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_verify_workspace(num_rows, batch)) return CFB_ERR_WORKSPACE;
   a.logits = logits; a.ld = ld; a.V = V; a.num_rows = num_rows;
@@ -1082,7 +1085,7 @@ cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_ro
   a.num_drafts = num_drafts; a.batch = batch; a.max_spec = max_spec;
   a.out_tokens = out_tokens; a.out_len = out_len; a.out_logp = out_logp;
   a.counter = static_cast<unsigned*>(ws);
-  a.rows = reinterpret_cast<RowResult*>(static_cast<char*>(ws) + ((size_t)batch * 4 + 255) / 256 * 256);
+  a.rows = reinterpret_cast<RowResult*>(static_cast<char*>(ws) + kCounters);
   a.err = err;
   return CFB_OK;
 }
@@ -1091,7 +1094,7 @@ cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_ro
 
 extern "C" size_t cfb_verify_workspace(int num_rows, int batch) {
   if (num_rows <= 0 || batch <= 0) return 0;
-  return ((size_t)batch * 4 + 255) / 256 * 256 + (size_t)num_rows * sizeof(RowResult);
+  return kCounters + (size_t)num_rows * sizeof(RowResult);
 }
 
 extern "C" cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, int num_rows, int V, int dtype,

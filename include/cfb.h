@@ -407,8 +407,8 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * Outputs as cfb_tree_verify_greedy, and logprobs fp32 [batch, max_spec_len + 1]: the output tokens' log
  * probabilities under w (of a greedy request: tau = 1), 0 after them.
  * logits: element-aligned, any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
- * ZERO before its first use (each launch leaves it so that the next may follow), for calls ordered on
- * one stream. err as there. Supported: max_spec_len <= 1024, V <= 2^20 - 8, batch <= 65535. */
+ * ZERO before its first use (each launch leaves it so that the next, of any size, may follow), for calls ordered on
+ * one stream. err as there. Supported: max_spec_len <= 1024, V <= 2^22 - 8, batch <= 65535. */
 size_t cfb_verify_workspace(int num_rows, int batch);
 cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, int num_rows, int V, int dtype,
                                    const int32_t* cu_num_draft, const int32_t* cu_num_sampled,

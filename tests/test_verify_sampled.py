@@ -531,3 +531,34 @@ def test_verifiers_far_larger_than_their_calls():
     ver.index_of[::2] = 1 << 30                          # as a C caller's list may be wrong: read as probability 0
     probs[:, ::2] = 0
     _check(_rejected(ver, logits, flat, probs, u, v), oracle.chain_verify_rejection(logits, *flat, probs, u, v, None, 64))
+
+
+@pytest.mark.gpu
+def test_calls_of_other_sizes_on_one_verifier():
+    """Few requests of many rows, then many of few: nothing of one call is left for the next."""
+    from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
+    tree, chain = SampledVerifier(300, 150, 8), RejectionVerifier(300, 150, 8, 500)
+    for turn, sizes in enumerate([[8] * 12, [1] * 150, [8] * 30, [0, 1] * 70, [2]]):
+        logits, flat, u = _case(sizes, 500, torch.bfloat16, turn)
+        _check(_sampled(tree, logits, flat, u), oracle.tree_verify_sampled(logits, *flat, u, None, 8))
+        logits, flat, probs, u, v = _chains(sizes, 500, torch.bfloat16, turn)
+        _check(_rejected(chain, logits, flat, probs, u, v), oracle.chain_verify_rejection(logits, *flat, probs, u, v, None, 8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [(1 << 20) + 3, (1 << 22) - 8])
+def test_the_largest_vocabularies(V):
+    from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
+    sizes = [1, 2]
+    logits, flat, u = _case(sizes, V, torch.float16, 4)
+    ver = SampledVerifier(5, 2, 2)
+    _check(_sampled(ver, logits, flat, u), oracle.tree_verify_sampled(logits, *flat, u, None, 2))
+    logits, flat, probs, u, v = _chains(sizes, V, torch.float16, 4)
+    ver = RejectionVerifier(5, 2, 2, V)
+    _check(_rejected(ver, logits, flat, probs, u, v), oracle.chain_verify_rejection(logits, *flat, probs, u, v, None, 2))
+    # 160 requests, a CTA each: the whole vocabulary's sums in one
+    logits = (torch.randn(4, V, generator=torch.Generator().manual_seed(6)) * 2.5).half().cuda().repeat(40, 1)
+    flat, u = (torch.zeros(160).int(), torch.arange(1, 161).int(), torch.zeros(0).int(), torch.zeros(0).int()), torch.rand(160)
+    got = _sampled(SampledVerifier(160, 160, 0), logits, flat, u)
+    want = oracle.tree_verify_sampled(logits[:4].cpu(), flat[0][:4], flat[1][:4], *flat[2:], u[:4], None, 0)
+    assert torch.equal(got[0][:4].cpu().long(), want[0]) and bool((got[0] >= 0).all())
