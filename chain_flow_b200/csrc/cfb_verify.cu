@@ -924,6 +924,7 @@ __global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const _
         r = s_row[cur + 1];
         if (r.accept >= kUndecided) {
           row_of<T, CHAIN>(A, rank, per, b, d0, n, s0, cur + 1, temp, w, a);
+          __syncthreads();                                   // (warps may still be deciding the row before from them)
           if (threadIdx.x == 0) {
             sh.top = (float)r.scaled;
             sh.z = r.mass;
@@ -1069,8 +1070,8 @@ template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaS
 
 // what both entry points check, and their common arguments
 cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_rows, int V, int dtype, const int32_t* cu_draft,
-                       const int32_t* cu_sampled, const int32_t* draft_tokens, const void* uniforms, int uniform_size,
-                       const float* temperature, int num_drafts, int batch, int max_spec, int32_t* out_tokens, int32_t* out_len,
+                       const int32_t* cu_sampled, const int32_t* draft_tokens, const void* uniforms, const void* resample,
+                       int uniform_size, const float* temperature, int num_drafts, int batch, int max_spec, int32_t* out_tokens, int32_t* out_len,
                        float* out_logp, void* ws, size_t ws_bytes, int* err) {
   if (num_rows <= 0 || V <= 0 || batch <= 0 || max_spec < 0 || ld < V) return CFB_ERR_INVALID_ARG;
   if (!logits || !cu_draft || !cu_sampled || !out_tokens || !out_len || !out_logp || !ws) return CFB_ERR_INVALID_ARG;
@@ -1078,10 +1079,11 @@ cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_ro
   if (dtype < DT_F32 || dtype > DT_BF16 || (uniform_size != 4 && uniform_size != 8)) return CFB_ERR_UNSUPPORTED;
   if (max_spec > kMaxNodes || V > kMaxVocab - 8 || batch > kMaxBatch) return CFB_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return CFB_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(uniforms) | reinterpret_cast<uintptr_t>(resample)) % uniform_size) return CFB_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(ws) & 255) || ws_bytes < cfb_verify_workspace(num_rows, batch)) return CFB_ERR_WORKSPACE;
   a.logits = logits; a.ld = ld; a.V = V; a.num_rows = num_rows;
   a.cu_draft = cu_draft; a.cu_sampled = cu_sampled; a.draft_tokens = draft_tokens;
-  a.uniforms = uniforms; a.uniform_size = uniform_size; a.temperature = temperature;
+  a.uniforms = uniforms; a.resample = resample; a.uniform_size = uniform_size; a.temperature = temperature;
   a.num_drafts = num_drafts; a.batch = batch; a.max_spec = max_spec;
   a.out_tokens = out_tokens; a.out_len = out_len; a.out_logp = out_logp;
   a.counter = static_cast<unsigned*>(ws);
@@ -1106,7 +1108,7 @@ extern "C" cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, in
                                               float* logprobs, void* ws, size_t ws_bytes, int* err, void* stream) {
   VerifyArgs a{};
   if (const cfb_status s = common_args(a, logits, ld, num_rows, V, dtype, cu_num_draft, cu_num_sampled, draft_tokens, uniforms,
-                                       uniform_size, temperature, num_drafts, batch, max_spec_len, output_tokens, accepted_len,
+                                       nullptr, uniform_size, temperature, num_drafts, batch, max_spec_len, output_tokens, accepted_len,
                                        logprobs, ws, ws_bytes, err))
     return s;
   if (!uniforms || (num_drafts > 0 && !parents) || (max_spec_len > 0 && !accepted_path)) return CFB_ERR_INVALID_ARG;
@@ -1125,7 +1127,7 @@ extern "C" cfb_status cfb_chain_verify_rejection(const void* logits, int64_t ld,
                                                  size_t ws_bytes, int* err, void* stream) {
   VerifyArgs a{};
   if (const cfb_status s = common_args(a, logits, ld, num_rows, V, dtype, cu_num_draft, cu_num_sampled, draft_tokens, uniforms,
-                                       uniform_size, temperature, num_drafts, batch, max_spec_len, output_tokens, accepted_len,
+                                       resample, uniform_size, temperature, num_drafts, batch, max_spec_len, output_tokens, accepted_len,
                                        logprobs, ws, ws_bytes, err))
     return s;
   if (probs_width <= 0 || ld_probs < probs_width || !resample || (num_drafts > 0 && (!draft_probs || !uniforms))) return CFB_ERR_INVALID_ARG;
@@ -1134,6 +1136,5 @@ extern "C" cfb_status cfb_chain_verify_rejection(const void* logits, int64_t ld,
   a.ld_probs = ld_probs;
   a.probs_width = probs_width;
   a.index_of = index_of;
-  a.resample = resample;
   return launch_as<true>(a, dtype, static_cast<cudaStream_t>(stream));
 }

@@ -273,7 +273,8 @@ class PagePool:
 
     def release(self, table, length, keep=None, stream=None) -> None:
         """Gives back the pages of request b's positions past keep[b] (all of them without ``keep``) up to length[b]; their
-        entries become -1. A page that others hold stays theirs."""
+        entries become -1. A page that others hold stays theirs; a kept last page that they hold too stays shared, so a
+        request that cuts back into what it shares forks (to a row of its own) before it writes there."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.release(table, length, keep)

@@ -406,7 +406,7 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * argmax. A draft outside the vocabulary is refused.
  * Outputs as cfb_tree_verify_greedy, and logprobs fp32 [batch, max_spec_len + 1]: the output tokens' log
  * probabilities under w (of a greedy request: tau = 1), 0 after them.
- * logits: element-aligned, any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
+ * logits and the random numbers: element-aligned; any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
  * ZERO before its first use (each launch leaves it so that the next, of any size, may follow), for calls ordered on
  * one stream. err as there. Supported: max_spec_len <= 1024, V <= 2^22 - 8, batch <= 65535. */
 size_t cfb_verify_workspace(int num_rows, int batch);
@@ -483,6 +483,7 @@ cfb_status cfb_kv_copy_pages(const cfb_kv_cache* const* caches, int n_caches, co
  * gets none either, and leaves the others theirs.
  * cfb_pages_release: the pages of the positions past keep[b] (NULL: 0) up to length[b] lose a reference, their entries
  * become -1. Entries outside the pool are left out; a page that nobody holds keeps its count and sets *err (may be NULL).
+ * (A kept last page that others hold too stays shared: who cuts back into a forked prefix forks before it writes there.)
  * cfb_pages_fork: row child[i] becomes a copy of row parent[i] (both of `rows` rows; a row outside, or its own child: not
  * granted), length[child[i]] = length[parent[i]]: the full pages are shared (a reference more), and the slots of a last
  * page that is not full are copied to a page of the child's own (the lowest free, in order of i, granted as above) in each

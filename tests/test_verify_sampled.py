@@ -562,3 +562,10 @@ def test_the_largest_vocabularies(V):
     got = _sampled(SampledVerifier(160, 160, 0), logits, flat, u)
     want = oracle.tree_verify_sampled(logits[:4].cpu(), flat[0][:4], flat[1][:4], *flat[2:], u[:4], None, 0)
     assert torch.equal(got[0][:4].cpu().long(), want[0]) and bool((got[0] >= 0).all())
+
+
+def test_random_numbers_at_an_address_that_is_no_elements():
+    lib = _lib.load()
+    assert _tree_call(lib, u=FAKE + 4, size=8) == 1 and _tree_call(lib, u=FAKE + 2) == 1
+    for change in (dict(u=FAKE + 4, size=8), dict(v=FAKE + 4, size=8), dict(v=FAKE + 1)):
+        assert _chain_call(lib, **change) == 1, change
