@@ -6,7 +6,7 @@
 // number u in [0, 1) draws the first token i with w_0 + .. + w_i > u sum w. A refused draft draws from
 // r_i = max(w_i / sum w - q_i, 0) instead. Which token that is, is a whole number, so it has to be the
 // one that exact arithmetic gives, although the pass over the row is fp32: the pass carries a bound of
-// its error (kBand), and where a sum comes nearer to its threshold than that, the row is taken again in
+// its error, and where a sum comes nearer to its threshold than that, the row is taken again in
 // 64 bits. A language model's row at temperature 1 has a token of some hundredths where the draw falls,
 // so that happens to one row in thousands; rows that are flat over a whole vocabulary pay it always.
 //
@@ -16,14 +16,15 @@
 // exchange their totals through distributed shared memory. The draw then descends: CTA, warp, unit, a lane's neighbours,
 // element; only its unit is read again (from L2).
 //
-// Error of the pass, with u = 2^-24 and x = (l - max l) c: an element's exponent is off by 3 u |x| (difference, c,
-// product; its unit's base likewise), its exponential and those of two changes of base by 4 u each, a unit's sum by 12 u
-// (chains of 4, pairs, the warp), a warp's sum of q units by 2 q u. Under the weights the mean of |x| is their entropy less
-// log2 of their sum Z relative to the largest: at most log2(V / Z). What decides is C - t = C - u Z: an error that is
-// the same share of every weight cancels in it but for a half. The sums over CTAs, a CTA's warps and units, and
-// inside the draw's unit are fp32 too. So C - t is off by less than
-//   u Z (3 ln 2 log2(V / Z) + (12 + 12 + 2 q) / 2 + 10) + u (mass of the CTA's part) (12 + 2 q) + 18 u (mass of the unit).
-// Rows of 248320 normal logits of deviation 2.5 fall into that band once in eight draws, a language model's less.
+// Error of the pass, with u = 2^-24 and x = (l - max l) c, in relative terms: an element's exponent is off by
+// (2 + d) u |x| (difference, product, and d u of c itself), on its way to the row's largest that counts once; the exponential and
+// the three changes of base (unit, warp, CTA, row) by 4 u each, their products by u; a unit's sum by 11 u (chains of 4,
+// pairs, the warp), a warp's sum of q units by (5 + q / 32) u; the sums over warps and CTAs are 64 bits. Under the weights the mean of
+// |x| is their entropy less log2 of their sum Z relative to the largest: at most log2(V / Z). What decides is
+// C - t = C - v Z: of an error that every weight has in both, at most half remains, since 2 v (1 - v) <= 1 / 2. Where C comes from other
+// sums than Z does, their errors count in full: the sum over the CTA's warps (6 u of its part), over the warp's units (their
+// changes of base and two sums, (35 + q / 16) u of the warp's mass), inside the unit (18 u of its mass). So C - t is off by less than
+//   u Z (ln 2 (2 + d) log2(V / Z) + (16 + 3 + 11 + 5 + q / 32) / 2 + 2) + u (6 part + (35 + q / 16) warp + 18 unit).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <cmath>
@@ -75,7 +76,7 @@ enum Kind : int { ROW_MASS = 0, ROW_EMPTY = 1, ROW_NAN = 2 };
 // that is refused, so that something else is to be drawn
 constexpr int kUndecided = 2, kRefused = 3;
 
-struct Pub { float top; int nan; float sum; float pad; double sum64; };      // a CTA's part of a row
+struct Pub { float top; int nan; double sum; };      // a CTA's part of a row
 struct Found { int token, unsure; float logit; int pad; };
 
 struct Shared {
@@ -283,7 +284,7 @@ CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, do
 template <typename T> CFB_DEV void stats_units(const Row<T>& w, Shared* sh, float* tops, float* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = w.u0 + warp * w.each, end = min(first + w.each, w.u1);
-  float most = -INFINITY, total = 0.f;
+  float most = -INFINITY;
   for (int u = first; u < end; ++u) {
     uint4 v[kVectors<T>];
     load_unit(w, u, lane, v);
@@ -317,14 +318,16 @@ template <typename T> CFB_DEV void stats_units(const Row<T>& w, Shared* sh, floa
         }
     }
     sum = warp_sum(sum);
-    const float base = fmaxf(most, top);
-    total = total * rescale(most, base, w.c) + sum * rescale(top, base, w.c);
-    most = base;
+    most = fmaxf(most, top);
     if (lane == 0) {
       tops[u - w.u0] = top;
       sums[u - w.u0] = sum;
     }
   }
+  __syncwarp();
+  float total = 0.f;
+  for (int u = first + lane; u < end; u += 32) total += sums[u - w.u0] * rescale(tops[u - w.u0], most, w.c);
+  total = warp_sum(total);
   if (lane == 0) {
     sh->warp_top[warp] = most;
     sh->warp_sum[warp] = total;
@@ -471,21 +474,22 @@ template <typename F, typename G> CFB_DEV int pick(int n, G value, F* t, bool* u
   return last;
 }
 
-// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start). band: for all but
-// the unit's own rounding.
+// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start). W32: warps' sums
+// are relative to part_top. band: for all but what the warp and the unit add.
 template <int MODE, bool SLOW, typename T, typename F>
-CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F* sums, F t, double iz, float band) {
+CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F* sums, F t, double iz, float part_top, float band) {
   constexpr int kPer = kUnit / kSpan<MODE>, kLane = kSpan<MODE> / 32;   // summed units a unit; a lane's elements
   constexpr int N = kLane / kE<T>;
   const int lane = threadIdx.x & 31;
   const double table = kNarrow<MODE> ? 0. : exp2_table(lane);
   const float base = sh->top;
   bool unsure = false;
-  const int part = pick<F>(kWarps, [&](int i) -> F {
-    if constexpr (MODE == W32) return sh->warp_sum[i] * rescale(sh->warp_top[i], base, w.c);
+  const auto warp_mass = [&](int i) -> F {
+    if constexpr (MODE == W32) return sh->warp_sum[i] * rescale(part_top, base, w.c);
     else if constexpr (MODE == R32) return sh->warp_sum[i];
     else return sh->warp_sum64[i];
-  }, &t, &unsure);
+  };
+  const int part = pick<F>(kWarps, warp_mass, &t, &unsure);
   if (part < 0) return {-1, 1, 0.f, 0};
   const int begin = part * w.each, n = (min(begin + w.each, w.u1 - w.u0) - begin) * kPer;
   const auto unit_sum = [&](int i) -> F {
@@ -518,7 +522,8 @@ CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F
   const int e = pick<F>(32, [&](int) { return y; }, &t, &unsure);
   if (e < 0) return {-1, 1, 0.f, 0};
   if constexpr (kNarrow<MODE>) {
-    const float off = band + 18.f * (float)kRound * mass;
+    float off = band + 18.f * (float)kRound * mass;
+    if constexpr (MODE == W32) off += (float)kRound * (36.f + 0.07f * (float)w.each) * warp_mass(part);
     unsure |= !(t >= off && __shfl_sync(0xffffffffu, y, e) - t >= off);
   }
   return {first + who * kLane + e, unsure, __shfl_sync(0xffffffffu, l, e), 0};
@@ -563,40 +568,41 @@ template <typename T> struct Team {
   void* room;                // the units' sums
   int rank, ranks, ph;
 
-  // How far an fp32 sum over the row may be from its side of a threshold, as a share of the row's mass z
-  CFB_DEV float band(const Row<T>& w, float z) const {
-    return (float)kRound * (2.08f * (lg2((float)w.V) - lg2(z)) + 22.f + (float)w.each);
+  // The mean error of the exponents, and how far an fp32 sum over the row may be from its side of a threshold, as a share
+  // of the row's mass z, in u
+  CFB_DEV float mean_off(const Row<T>& w, float z) const {
+    const float d = fabsf((float)(w.c64 - (double)w.c)) * reciprocal(w.c) * 16777216.f;
+    return 0.6932f * (2.001f + d) * (lg2((float)w.V) - lg2(z));
   }
+  CFB_DEV float band(const Row<T>& w, float z) const { return mean_off(w, z) + 20.f + (float)w.each * 0.02f; }
 
   // The CTAs' totals, handed over by the cluster's barrier -> the row's; who has the threshold u of it. SCALED: each
   // total is relative to its CTA's largest; greedy: the owner is the first that has the row's largest.
-  template <typename F, bool SCALED> CFB_DEV void exchange(const Row<T>& w, F u, bool greedy) {
+  template <bool SCALED> CFB_DEV void exchange(const Row<T>& w, double u, bool greedy) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
-      Pub p{-INFINITY, 0, 0.f, 0.f, 0.};
+      Pub p{-INFINITY, 0, 0.};
       if (lane < ranks) p = *cluster.map_shared_rank(&sh->pub[ph], lane);
-      F m;
-      if constexpr (sizeof(F) == 8) m = p.sum64;
-      else m = p.sum;
+      double m = p.sum;
       bool nan = false;
       float top = 0.f;
       if constexpr (SCALED) {
         top = warp_max(p.top);
         nan = __any_sync(0xffffffffu, p.nan);
-        m *= rescale(p.top, top, w.c);
+        m *= (double)rescale(p.top, top, w.c);
       }
-      F scan = m;
+      double scan = m;
 #pragma unroll
       for (int off = 1; off < kMaxCluster; off <<= 1) {
-        const F o = __shfl_up_sync(0xffffffffu, scan, off);
+        const double o = __shfl_up_sync(0xffffffffu, scan, off);
         if (lane >= off) scan += o;
       }
-      const F whole = __shfl_sync(0xffffffffu, scan, kMaxCluster - 1);
+      const double whole = __shfl_sync(0xffffffffu, scan, kMaxCluster - 1);
       // (the sum before, not the one behind less this part's, which would lose small ones)
-      const F up = __shfl_up_sync(0xffffffffu, scan, 1), before = lane ? up : (F)0;
-      const F t = threshold(u, whole);
+      const double up = __shfl_up_sync(0xffffffffu, scan, 1), before = lane ? up : 0.;
+      const double t = threshold(u, whole);
       unsigned hit = __ballot_sync(0xffffffffu, m > 0 && before <= t && t < scan);
       if (!hit) hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, m > 0) | 1u));
       if (SCALED && (greedy || nan)) hit = __ballot_sync(0xffffffffu, nan ? p.nan != 0 : p.top == top);
@@ -616,22 +622,23 @@ template <typename T> struct Team {
     }
     __syncthreads();
   }
-  static CFB_DEV float threshold(float u, float whole) { return fminf(u * whole, whole * (1.f - 0x1p-23f)); }
   static CFB_DEV double threshold(double u, double whole) { return fmin(u * whole, whole * (1. - 0x1p-52)); }
 
   // Warp 0: the warps' sums handed over
+  static CFB_DEV double warps_sum(double v) {
+#pragma unroll
+    for (int off = kWarps / 2; off; off >>= 1) v += __shfl_down_sync(0xffffffffu, v, off);
+    return v;
+  }
   template <typename F> CFB_DEV void hand_over() {
     const int lane = threadIdx.x;
-    F v = 0;
+    double v = 0.;
     if (lane < kWarps) {
       if constexpr (sizeof(F) == 8) v = sh->warp_sum64[lane];
-      else v = sh->warp_sum[lane];
+      else v = (double)sh->warp_sum[lane];
     }
-    v = warp_sum(v);
-    if (lane == 0) {
-      if constexpr (sizeof(F) == 8) sh->pub[ph].sum64 = v;
-      else sh->pub[ph].sum = v;
-    }
+    v = warps_sum(v);
+    if (lane == 0) sh->pub[ph].sum = v;
   }
 
   // the pass over the row
@@ -642,12 +649,13 @@ template <typename T> struct Team {
     if (threadIdx.x < 32) {
       const int lane = threadIdx.x;
       const float mine = lane < kWarps ? sh->warp_top[lane] : -INFINITY, sum = lane < kWarps ? sh->warp_sum[lane] : 0.f;
-      const float top = warp_max(mine);
+      const float top = warp_max(mine), scaled = sum * rescale(mine, top, w.c);
       const bool nan = __any_sync(0xffffffffu, sum != sum);
-      const float total = warp_sum(sum * rescale(mine, top, w.c));
-      if (lane == 0) sh->pub[ph] = {top, nan, nan ? 0.f : total, 0.f, 0.};
+      const double total = warps_sum((double)scaled);
+      if (lane < kWarps) sh->warp_sum[lane] = scaled;      // (relative to the CTA's largest from here on)
+      if (lane == 0) sh->pub[ph] = {top, nan, nan ? 0. : total};
     }
-    exchange<float, true>(w, (float)number(raw, size), greedy);
+    exchange<true>(w, number(raw, size), greedy);
   }
 
   // a pass that knows the row's largest, and its sum where it needs it
@@ -656,35 +664,36 @@ template <typename T> struct Team {
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) hand_over<float>();
-    exchange<float, false>(w, (float)u, false);
+    exchange<false>(w, u, false);
   }
   template <int MODE, bool SLOW> CFB_DEV void exact_pass(const Row<T>& w, double u) {
     exact_units<MODE, SLOW>(w, sh, sh->top, MODE == R64 ? 1. / sh->z : 0., static_cast<double*>(room));
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) hand_over<double>();
-    exchange<double, false>(w, u, false);
+    exchange<false>(w, u, false);
   }
 
   // Warp 0 of the owner: the token of the last pass's threshold
   CFB_DEV Found found(const Row<T>& w, double u) const {
     if (isinf(sh->top)) return {-1, 1, 0.f, 0};            // several of +inf: in 64 bits
     const float whole = (float)sh->whole;
-    return find<W32, false>(w, sh, tops, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before, 0.,
-                            band(w, whole) * whole + (float)kRound * (12 + 2 * w.each) * (float)(sh->end - sh->before));
+    return find<W32, false>(w, sh, tops, static_cast<const float*>(room), (float)(threshold(u, sh->whole) - sh->before), 0.,
+                            sh->pub[ph].top, (float)kRound * (band(w, whole) * whole + 6.f * (float)(sh->end - sh->before)));
   }
   // (from what is left above q, R: every p is off by its exponent's error and 6 u, and all of them by 1 / Z's, of which
-  // C - u R keeps the share that q has where p is larger, at most 1 - R; sums of R by chains of 16, pairs and the warp)
+  // C - v R keeps the share that q has where p is larger, at most 1 - R; a unit's sum is off by 23 u (chains of 16, pairs, the
+  // warp), a warp's by q u, of which half remains, the sum over warps by 4 u, the one over units by (5 + q / 6) u, and by q u, since it is another)
   CFB_DEV Found found_rest(const Row<T>& w, double u) const {
-    const float whole = (float)sh->whole, z = (float)sh->z, mean = 2.08f * (lg2((float)w.V) - lg2(z)), other = fmaxf(1.f - whole, 0.f);
-    const float off = (float)kRound * (mean * (1.f + other) + 6.f + (40 + 2 * w.each) * other + (36 + 2 * w.each) * whole);
+    const float whole = (float)sh->whole, z = (float)sh->z, mean = mean_off(w, z), other = fmaxf(1.f - whole, 0.f), q = (float)w.each;
+    const float off = (float)kRound * (mean * (1.f + other) + 6.f + (39.f + 0.04f * q) * other + (22.f + 2.f * q) * whole);
     if (!(whole > 2.f * off)) return {-1, 1, 0.f, 0};
-    return find<R32, false>(w, sh, tops, static_cast<const float*>(room), threshold((float)u, whole) - (float)sh->before,
-                            (double)reciprocal(z), off);
+    return find<R32, false>(w, sh, tops, static_cast<const float*>(room), (float)(threshold(u, sh->whole) - sh->before),
+                            (double)reciprocal(z), 0.f, off);
   }
   template <int MODE, bool SLOW> CFB_DEV Found found64(const Row<T>& w, double u) const {
     return find<MODE, SLOW>(w, sh, tops, static_cast<const double*>(room), threshold(u, sh->whole) - sh->before,
-                            MODE == R64 ? 1. / sh->z : 0., 0.f);
+                            MODE == R64 ? 1. / sh->z : 0., 0.f, 0.f);
   }
 
   // Warp 0 of the owner hands what it found to all
@@ -784,7 +793,7 @@ CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, const Asked& a, int* h
       const float z = (float)sh.z, x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) * reciprocal(z);
       const float uq = (float)number(a.raw_u, a.size) * q;
       // (every CTA computes the same)
-      const float off = p * (2.f * team.band(w, z) + (float)kRound * (2.08f * fabsf(x) + 16.f));
+      const float off = p * (float)kRound * (2.f * team.band(w, z) + 2.08f * fabsf(x) + 16.f);
       if (!(fabsf(uq - p) > off)) {
         if constexpr (LAZY) return later(kUndecided);
         else return taken(exact_row<CHAIN>(team, w, a));
