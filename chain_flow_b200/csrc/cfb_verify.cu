@@ -393,57 +393,74 @@ template <typename T> CFB_DEV void rest_units(const Row<T>& w, Shared* sh, float
   }
   if (lane == 0) sh->warp_sum[warp] = total;
 }
-// every unit's sum in 64 bits: a lane has 8 neighbours of 256
+
+// every unit's sum in 64 bits, by quarters: a lane has 8 neighbours of 256. (A unit's loads together and its four sums
+// reduced side by side: chains of a batch 104 -> 100 us.)
 template <int MODE, bool SLOW, typename T>
 CFB_DEV void exact_units(const Row<T>& w, Shared* sh, float base, double iz, double* sums) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double table = exp2_table(lane);
   constexpr int kPer = kUnit / kSpan<MODE>, N = 8 / kE<T>;
+  static_assert(kPer == 4);
   const int begin = (w.u0 + warp * w.each) * kPer, end = min(begin + w.each * kPer, w.u1 * kPer);
   double total = 0.;
-  uint4 next[N];
-  float qnext[8];
-  const auto fetch = [&](int u) {
+  for (int u = begin; u < end; u += kPer) {
     const int first = u * kSpan<MODE> - w.shift, i = first + lane * 8;
-    load_vectors(w, first, kSpan<MODE>, i, kE<T>, next);
-    if constexpr (MODE == R64) draft_probs(w, i, 8, qnext);
-  };
-  if (begin < end) fetch(begin);
-  for (int u = begin; u < end; ++u) {
-    uint4 v[N];
-    float q[8], l[8];
+    uint4 v[kPer * N];
+    if (first >= 0 && first + kUnit <= w.V) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = next[j];
-    if constexpr (MODE == R64)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = qnext[e];
-    if (u + 1 < end) fetch(u + 1);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 x = pair_of<T>(v[e / (kE<T> / 2)], e % (kE<T> / 2));
-      l[2 * e] = x.x;
-      l[2 * e + 1] = x.y;
-    }
-    double a = 0.;
-    if constexpr (SLOW) {
-#pragma unroll 1
-      for (int e = 0; e < 8; ++e) {
-        const double x = weight64(l[e], base, w.c64);
-        a += MODE == R64 ? fmax(x * iz - (double)fmaxf(q[e], 0.f), 0.) : x;
-      }
+      for (int k = 0; k < kPer * N; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(w.p + i + k / N * kSpan<MODE> + k % N * kE<T>));
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        double x[4];
-        fast_weights64<MODE == R64, 4>(l + e, base, w.c, 32. * w.c64, table, x);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a += MODE == R64 ? fmax(x[k] * iz - (double)fmaxf(q[e + k], 0.f), 0.) : x[k];
-      }
+      for (int k = 0; k < kPer * N; ++k) v[k] = load_edge(w.p, w.V, i + k / N * kSpan<MODE> + k % N * kE<T>);
     }
-    const double sum = warp_sum(a);
+    float qnext[8];
+    if constexpr (MODE == R64) draft_probs(w, i, 8, qnext);
+    double part[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      float q[8], l[8];
+      if constexpr (MODE == R64) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = qnext[e];
+        if (k + 1 < kPer) draft_probs(w, i + (k + 1) * kSpan<MODE>, 8, qnext);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = pair_of<T>(v[k * N + e / (kE<T> / 2)], e % (kE<T> / 2));
+        l[2 * e] = x.x;
+        l[2 * e + 1] = x.y;
+      }
+      double a = 0.;
+      if constexpr (SLOW) {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const double x = weight64(l[e], base, w.c64);
+          a += MODE == R64 ? fmax(x * iz - (double)fmaxf(q[e], 0.f), 0.) : x;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          double x[4];
+          fast_weights64<MODE == R64, 4>(l + e, base, w.c, 32. * w.c64, table, x);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) a += MODE == R64 ? fmax(x[n] * iz - (double)fmaxf(q[e + n], 0.f), 0.) : x[n];
+        }
+      }
+      part[k] = a;
+    }
+    // the four sums over the warp: of sum i + 2 j the lanes of the low bits i, j
+    const bool odd = lane & 1, high = lane & 2;
+    const double x = (odd ? part[1] : part[0]) + __shfl_xor_sync(0xffffffffu, odd ? part[0] : part[1], 1);
+    const double y = (odd ? part[3] : part[2]) + __shfl_xor_sync(0xffffffffu, odd ? part[2] : part[3], 1);
+    double sum = (high ? y : x) + __shfl_xor_sync(0xffffffffu, high ? x : y, 2);
+#pragma unroll
+    for (int off = 4; off < 32; off *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     total += sum;
-    if (lane == 0) sums[u - w.u0 * kPer] = sum;
+    if (lane < kPer) sums[u - w.u0 * kPer + lane] = sum;
   }
+  total += __shfl_xor_sync(0xffffffffu, total, 1);
+  total += __shfl_xor_sync(0xffffffffu, total, 2);
   if (lane == 0) sh->warp_sum64[warp] = total;
 }
 
