@@ -36,9 +36,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-// Small CTAs, several an SM, in large clusters: their serial steps cover one another (a batch of 64 trees 80 us with 2 CTAs of
-// 512 threads an SM, 71 with 4 of 256). Chains, whose steps hold more, take 80 registers a thread and 3 CTAs an SM (48
-// chains 104 us; with 4 CTAs 116), trees 64 and 4 (64 trees 71; with 3 CTAs 78).
+// Small CTAs, several an SM, in large clusters: their serial steps cover one another (a batch of 64 trees took 80 us with 2
+// CTAs of 512 threads an SM, 71 with 4 of 256). Chains, whose steps hold more, take 80 registers a thread and 3 CTAs an SM
+// (48 chains 100 us; with 4 CTAs 105), trees 64 and 4 (64 trees 69; with 3 CTAs 78).
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kPerLane = 32;                 // elements of a unit in a lane's registers
@@ -1079,12 +1079,14 @@ cfb_status launch(const VerifyArgs& a, cudaStream_t st) {
 }
 
 template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaStream_t st) {
-  // All rows at once take the GPU's whole width, but read what no walk reaches, and with more rows there are fewer CTAs
-  // for what the walk takes again. Measured, walk against all rows, us. Trees, V = 248320: 6 rows (one chain) 18 / 13, 41 (one
-  // tree) 20 / 21, 48 (8 chains) 45 / 34, 82 (two trees) 24 / 35; V = 32003: 384 (64 chains) 65 / 40, 656 (16 trees)
-  // 39 / 47. Chains with draft probabilities, V = 248320: 6 rows 25 / 17, 24 54 / 54, 48 56 / 72; V = 32003: 96 48 / 42, 288 65 / 81.
+  // All rows at once take the GPU's whole width, but read what no walk reaches, the more so the more rows a request has, and
+  // with more rows there are fewer CTAs for what the walk takes again. Measured, all rows at once / walk, us. Without draft probabilities,
+  // 6 rows a request, V = 248320: 1 request 14 / 18, 8 33 / 46, 16 49 / 55, 64 160 / 80; V = 32003: 64 40 / 60. 41 rows a request,
+  // V = 248320: 1 request 22 / 23 (eight draws of it), 2 35 / 24; V = 32003: 1 17 / 18, 4 25 / 30, 16 47 / 38; V = 5000: 16 20 / 29. With draft probabilities,
+  // 6 rows, V = 248320: 1 request 17 / 24, 2 34 / 34, 4 53 / 51, 8 68 / 54; V = 32003: 16 41 / 46, 48 78 / 61.
   // (and a cluster goes to every row that a request may have: many that have none would cost more than they save)
-  const bool flat = (long long)a.V * a.num_rows <= (CHAIN ? 5ll : 12ll) << 20 && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
+  const long long most = (CHAIN ? 5ll : a.num_rows <= 16ll * a.batch ? 24ll : 12ll) << 20;      // elements
+  const bool flat = (long long)a.V * a.num_rows <= most && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
   const auto go = [&](auto t) {
     using T = decltype(t);
     return flat ? launch<T, CHAIN, true>(a, st) : launch<T, CHAIN, false>(a, st);
