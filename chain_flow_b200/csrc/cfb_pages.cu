@@ -32,7 +32,6 @@ struct Layers {                              // caches of one geometry
   int size, pieces;                          // bytes an element, log2 of a row's 16-byte pieces
 };
 
-
 // The pool's kernels follow one another in a stream (given back, taken, forked): each is launched while the one before
 // still runs and waits for its end before it reads anything, which hides part of a launch (a scheduler's step of two kernels 13.8 -> 12.3 us).
 __device__ __forceinline__ void after_the_kernel_before() {
@@ -68,7 +67,8 @@ struct KeepArgs {
 // A CTA: a request (x), a layer (y), a group of heads (z). The rows of a batch are all read before the first is written; a
 // later batch reads rows behind every one that was written, since a path's j-th node is not before j.
 // Bound by latency: three loads that wait for each other (path, page table, rows), then the stores. Keys and values by one
-// CTA, so that 64 requests of 8 layers are in flight at once.
+// CTA, so that 64 requests of 8 layers are in flight at once. Measured, 8 layers of 4 heads of 256, up to 5 rows a request: one
+// request, bf16, 5 us; 64, e4m3, 7 (bytes: 0.8).
 __global__ void __launch_bounds__(kThreads, 3) kv_keep_kernel(const __grid_constant__ Layers L, const KeepArgs A) {
   extern __shared__ longlong4 s_move[];      // of a position: byte offsets of its row, from and to (or -1), and its scales'
   const int b = blockIdx.x, S = L.c.page_size;
@@ -174,7 +174,8 @@ __device__ __forceinline__ void copy_page(const Layers& L, int layer, bool value
   }
 }
 
-// A CTA: a pair of pages (x), a layer's keys or values (y)
+// A CTA: a pair of pages (x), a layer's keys or values (y). Bound by HBM: 1.07 GB read and written in 165 us, 6.5 TB/s, as
+// a plain copy's rate.
 __global__ void __launch_bounds__(kThreads, 5) kv_copy_pages_kernel(const __grid_constant__ Layers L, const int32_t* src,
                                                                  const int32_t* dst, const int32_t* slots) {
   copy_page(L, blockIdx.y >> 1, blockIdx.y & 1, src[blockIdx.x], dst[blockIdx.x], slots ? slots[blockIdx.x] : L.c.page_size);
@@ -240,6 +241,8 @@ __device__ __forceinline__ int nth_bit(uint32_t bits, int n) {
 }
 
 // FORK: request i is the fork of row parent[i] into row child[i], which needs a page for what its last one holds.
+// Bound by latency: the counts' loads, a barrier or two a running sum, a bisection a page that is asked for. Measured: 256
+// requests of a pool of 65536 pages, the release before it included, 12.4 us (bytes: 0.07); one CTA for all of it took 34 with it.
 template <bool FORK>
 __global__ void __launch_bounds__(kTake) pages_take_kernel(const TakeArgs A) {
   after_the_kernel_before();
@@ -366,7 +369,8 @@ __global__ void __launch_bounds__(kThreads) pages_release_kernel(const Pool P, c
 }
 
 // After pages_take_kernel<true>. A CTA: a fork (x); its row and counts (the first `lead` y, 0 or 1), or its last page in
-// a layer's keys or values.
+// a layer's keys or values. Measured, both kernels: 8 forks of 9001 positions, a page in 8 layers each, 13.4 us (bytes: 0.7); 64
+// of 1500, pages of 48 slots in e4m3, 22.6 (7.9).
 __global__ void __launch_bounds__(kThreads, 5) pages_fork_kernel(const __grid_constant__ Layers L, const Pool P, int32_t* length,
                                                               const int32_t* parent, const int32_t* child,
                                                               const int32_t* granted, int lead) {

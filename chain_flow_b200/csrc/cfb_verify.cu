@@ -863,6 +863,11 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
   if (a.drafted) w.probs = A.probs + (long long)(d0 + j) * A.ld_probs;
 }
 
+// Bound by latency, not by a pipe (64 trees of 41 bf16 rows over 248320 tokens: SM 25 %, DRAM 19 %; a warp waits longest at
+// barriers, for another CTA's totals or warp 0's descent): the rows of a walk come one after another, about 9500
+// cycles each, and one that goes through 64 bits takes 16000 to 80000 more. Measured at V = 248320: one chain of 5 drafts 13
+// us, one tree of 40 22, 64 trees 69 (the visited rows' bytes: 14), one chain with draft probabilities 33, 48 of them 100 (17);
+// without the rows in 64 bits 12, 17, 54, 27 and 63.
 // FLAT: a cluster a row (grid.y: rows of a request, grid.z: requests), every row at once; the request's last
 // cluster walks, and takes again what was left for the walk where it comes by. Otherwise a cluster a request (grid.y), which
 // takes the rows of its walk in turn. CHAIN: draft probabilities; a node's only child is the next one.
