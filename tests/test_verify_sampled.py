@@ -569,3 +569,37 @@ def test_random_numbers_at_an_address_that_is_no_elements():
     assert _tree_call(lib, u=FAKE + 4, size=8) == 1 and _tree_call(lib, u=FAKE + 2) == 1
     for change in (dict(u=FAKE + 4, size=8), dict(v=FAKE + 4, size=8), dict(v=FAKE + 1)):
         assert _chain_call(lib, **change) == 1, change
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V, n", [(30011, 120), (140001, 190)])
+def test_rows_that_rise_and_fall_next_to_a_border(V, n):
+    """Rows whose largest element changes all along (every unit's sums change their base), at temperatures that fp32 holds
+    badly, with numbers from 10^-12 to 10^-4 beside a border: around and below what an fp32 sum is off by."""
+    from chain_flow_b200.tree import RejectionVerifier, SampledVerifier
+    g = torch.Generator().manual_seed(7)
+    i = torch.arange(V, dtype=torch.float64)
+    shapes = [12 * i / V, 12 - 12 * i / V, 6 + 6 * torch.sin(i / 900), (i % 1024) / 90, 10 - 300 * (i / V - 0.5) ** 2, 0 * i]
+    temps = [1.0, 0.7, 1.3, 1 / 3, 2.1]
+    logits = torch.stack([shapes[r % 6] + 0.3 * torch.randn(V, generator=g) for r in range(n)]).float()
+    temp = torch.tensor([temps[r // 6 % 5] for r in range(n)])
+    u, off = torch.zeros(n, dtype=torch.float64), [1e-12, 1e-9, 3e-8, 3e-7, 1e-6, 3e-6, 1e-5, 1e-4]
+    q, v = torch.zeros(n, V), torch.zeros(n, dtype=torch.float64)
+    for r in range(n):
+        p = torch.softmax(logits[r].double() / temp[r].double(), 0)
+        c = torch.cumsum(p, 0)
+        t = int(torch.searchsorted(c, torch.rand(1, generator=g, dtype=torch.float64)).clamp(max=V - 2))
+        side = off[int(torch.randint(8, (1,), generator=g))] * (1 if torch.rand(1, generator=g) < 0.5 else -1)
+        u[r] = c[t] / c[-1] + side
+        q[r] = torch.softmax(logits[r].double() / temp[r].double() + 0.5 * torch.randn(V, generator=g), 0).float()
+        c = torch.cumsum((p - q[r].double()).clamp_min(0), 0)
+        t = int(torch.searchsorted(c, c[-1] * torch.rand(1, generator=g, dtype=torch.float64)).clamp(max=V - 2))
+        v[r] = c[t] / c[-1] + side
+    none, ends = torch.zeros(0, dtype=torch.int32), torch.arange(1, n + 1, dtype=torch.int32)
+    flat = (torch.zeros(n, dtype=torch.int32), ends, none, none)
+    _check(_sampled(SampledVerifier(n, n, 0), logits, flat, u, temp), oracle.tree_verify_sampled(logits, *flat, u, temp, 0))
+    m = n // 2                                           # a draft of each, refused: the draw is from what is left
+    chain = (ends[:m], 2 * ends[:m], torch.full((m,), -1, dtype=torch.int32))
+    rows = logits[:m].repeat_interleave(2, 0)
+    args = (rows, *chain, q[:m], torch.zeros(m), v[:m], temp[:m])
+    _check(_rejected(RejectionVerifier(2 * m, m, 1, V), rows, chain, *args[4:]), oracle.chain_verify_rejection(*args, 1))
