@@ -251,6 +251,8 @@ template <bool CUT, int N> CFB_DEV void fast_weights64(const float* l, float bas
 CFB_DEV double weight64(float l, float base, double c) {
   return l == base ? 1. : isinf(base) ? 0. : exp2(((double)l - (double)base) * c);
 }
+// (by the sign: the library's maximum looks for NaN, which there is none of)
+CFB_DEV double positive(double r) { return __double2hiint(r) < 0 ? 0. : r; }
 // the draft probability of token i (0 outside the row and for what is not a positive number)
 template <typename T> CFB_DEV float draft_prob(const Row<T>& w, int i) {
   if (i < 0 || i >= w.V) return 0.f;
@@ -275,7 +277,7 @@ CFB_DEV auto value_of(const Row<T>& w, float l, int i, float base, double iz, do
     if constexpr (SLOW) v = weight64(l, base, w.c64);
     else fast_weights64<true, 1>(&l, base, w.c, 32. * w.c64, table, &v);
     if constexpr (MODE == W64) return v;
-    else return fmax(v * iz - (double)draft_prob(w, i), 0.);
+    else return positive(v * iz - (double)draft_prob(w, i));
   }
 }
 
@@ -436,7 +438,7 @@ CFB_DEV void exact_units(const Row<T>& w, Shared* sh, float base, double iz, dou
 #pragma unroll 1
         for (int e = 0; e < 8; ++e) {
           const double x = weight64(l[e], base, w.c64);
-          a += MODE == R64 ? fmax(x * iz - (double)fmaxf(q[e], 0.f), 0.) : x;
+          a += MODE == R64 ? positive(x * iz - (double)fmaxf(q[e], 0.f)) : x;
         }
       } else {
 #pragma unroll
@@ -444,7 +446,7 @@ CFB_DEV void exact_units(const Row<T>& w, Shared* sh, float base, double iz, dou
           double x[4];
           fast_weights64<MODE == R64, 4>(l + e, base, w.c, 32. * w.c64, table, x);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) a += MODE == R64 ? fmax(x[n] * iz - (double)fmaxf(q[e + n], 0.f), 0.) : x[n];
+          for (int n = 0; n < 4; ++n) a += MODE == R64 ? positive(x[n] * iz - (double)fmaxf(q[e + n], 0.f)) : x[n];
         }
       }
       part[k] = a;
@@ -866,7 +868,7 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
 // Bound by latency, not by a pipe (64 trees of 41 bf16 rows over 248320 tokens: SM 25 %, DRAM 19 %; a warp waits longest at
 // barriers, for another CTA's totals or warp 0's descent): the rows of a walk come one after another, about 9500
 // cycles each, and one that goes through 64 bits takes 16000 to 80000 more. Measured at V = 248320: one chain of 5 drafts 13
-// us, one tree of 40 22, 64 trees 69 (the visited rows' bytes: 14), one chain with draft probabilities 33, 48 of them 100 (17);
+// us, one tree of 40 22, 64 trees 69 (the visited rows' bytes: 14), one chain with draft probabilities 33, 48 of them 98 (17);
 // without the rows in 64 bits 12, 17, 54, 27 and 63.
 // FLAT: a cluster a row (grid.y: rows of a request, grid.z: requests), every row at once; the request's last
 // cluster walks, and takes again what was left for the walk where it comes by. Otherwise a cluster a request (grid.y), which
