@@ -7,8 +7,9 @@
 // r_i = max(w_i / sum w - q_i, 0) instead. Which token that is, is a whole number, so it has to be the
 // one that exact arithmetic gives, although the pass over the row is fp32: the pass carries a bound of
 // its error, and where a sum comes nearer to its threshold than that, the row is taken again in
-// 64 bits. A language model's row at temperature 1 has a token of some hundredths where the draw falls,
-// so that happens to one row in thousands; rows that are flat over a whole vocabulary pay it always.
+// 64 bits. That happens the more, the more of a row's mass lies in tokens as small as the bound: to one in eight rows of
+// 248320 normal logits of deviation 2.5 (one in three draws from what is left above q there), seldom where a few tokens
+// hold most, always where a row is flat over a vocabulary.
 //
 // One pass over the row: a warp takes 1024 elements in registers, their largest, their weights relative
 // to it and the weights' sum, which stay in shared memory (no running rescale of elements: such units' sums are brought
@@ -764,7 +765,7 @@ CFB_DEV RowResult exact_steps(Team<T> team, const Row<T>& w, const Asked& a, dou
   return result(f.token, 0, f.logit);
 }
 template <bool CHAIN, typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
-  // (weights below 2^-1020 count where the threshold is that small, and only there)
+  // (weights below 2^-1000, which the fast ones cut, count where the threshold is that small, and only there)
   const double u = number(a.raw_u, a.size), v = number(a.raw_v, a.size);
   const float top = team.sh->top, depth = (top - lowest_logit(top, w.c)) * w.c;       // (fp32 may not hold such a logit)
   return isinf(top) || !(depth > 990.f && depth < 1010.f) || v < 0x1p-900 ? exact_steps<CHAIN, true>(team, w, a, u, v)
