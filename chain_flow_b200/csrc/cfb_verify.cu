@@ -265,6 +265,9 @@ enum Mode : int { W32 = 0, W64 = 1, R32 = 2, R64 = 3 };    // weights, or what i
 template <int MODE> constexpr bool kNarrow = MODE == W32 || MODE == R32;
 // elements of a summed unit, and a lane's of them: in 64 bits, where an element costs much more, smaller ones to scan
 template <int MODE> constexpr int kSpan = kNarrow<MODE> ? kUnit : 256;
+// Sums up to this are no mass: masked tokens count as 2^-1000 each in the fast sums of weights (without the cut a batch of
+// trees takes 1 us less), and the search, which cuts them, would find nothing among them.
+template <int MODE, bool SLOW> constexpr double kNothing = MODE == W64 && !SLOW ? 0x1p-960 : 0.;
 
 // an element's value, by a whole warp. iz: 1 / the row's sum of weights (R32, R64). SLOW (64 bits): any base, denormals kept
 template <int MODE, bool SLOW, typename T>
@@ -467,37 +470,40 @@ CFB_DEV void exact_units(const Row<T>& w, Shared* sh, float base, double iz, dou
   if (lane == 0) sh->warp_sum64[warp] = total;
 }
 
-// Of n values, by a warp: the first whose running sum passes *t, which becomes what is left of it; where none does, for
-// rounding, the last that is positive (unsure), or -1
-template <typename F, typename G> CFB_DEV int pick(int n, G value, F* t, bool* unsure) {
+// Of n values, by a warp: the first above `floor` whose running sum, from *head on, passes t; where none does, for rounding, the
+// last above it (unsure), or -1. *head becomes the running sum in front of it
+template <typename F, typename G> CFB_DEV int pick(int n, G value, F* head, F t, F floor, bool* unsure) {
   const int lane = threadIdx.x & 31;
-  F before = 0, before_last = 0;
+  F before = *head, before_last = before;
   int last = -1;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const F v = i0 + lane < n ? value(i0 + lane) : (F)0, scan = before + warp_scan(v, lane);
-    const F up = __shfl_up_sync(0xffffffffu, scan, 1), head = lane ? up : before;
-    const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && scan > *t), some = __ballot_sync(0xffffffffu, v > 0);
+    const F up = __shfl_up_sync(0xffffffffu, scan, 1), front = lane ? up : before;
+    const unsigned hit = __ballot_sync(0xffffffffu, v > floor && scan > t), some = __ballot_sync(0xffffffffu, v > floor);
     if (hit) {
       const int e = __ffs(hit) - 1;
-      *t -= __shfl_sync(0xffffffffu, head, e);
+      *head = __shfl_sync(0xffffffffu, front, e);
       return i0 + e;
     }
     if (some) {
       const int e = 31 - __clz(some);
       last = i0 + e;
-      before_last = __shfl_sync(0xffffffffu, head, e);
+      before_last = __shfl_sync(0xffffffffu, front, e);
     }
     before = __shfl_sync(0xffffffffu, scan, 31);
   }
   *unsure = true;
-  *t -= before_last;
+  *head = before_last;
   return last;
 }
 
-// Warp 0: the first token of this CTA's part whose running sum passes t (relative to the part's start). W32: warps' sums
-// are relative to part_top. band: for all but what the warp and the unit add.
+// Warp 0: the first token of this CTA's part whose running sum passes the threshold t. In 64 bits that is the sum over the whole row,
+// `head` in front of the part, carried down as it is: where it comes to exactly t at a border, what has next to no mass
+// behind the border leaves it at t, as in one sum over the row, while against a rest of 0 it would pass. In fp32 (which is not
+// decided near a border) t is relative to the part's start, then to each step's. W32: warps' sums are relative to
+// part_top. band: for all but what the warp and the unit add.
 template <int MODE, bool SLOW, typename T, typename F>
-CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F* sums, F t, double iz, float part_top, float band) {
+CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F* sums, F head, F t, double iz, float part_top, float band) {
   constexpr int kPer = kUnit / kSpan<MODE>, kLane = kSpan<MODE> / 32;   // summed units a unit; a lane's elements
   constexpr int N = kLane / kE<T>;
   const int lane = threadIdx.x & 31;
@@ -509,14 +515,22 @@ CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F
     else if constexpr (MODE == R32) return sh->warp_sum[i];
     else return sh->warp_sum64[i];
   };
-  const int part = pick<F>(kWarps, warp_mass, &t, &unsure);
+  const auto step = [&](int n, auto value) {
+    const int i = pick<F>(n, value, &head, t, (F)kNothing<MODE, SLOW>, &unsure);
+    if constexpr (kNarrow<MODE>) {
+      t -= head;
+      head = 0;
+    }
+    return i;
+  };
+  const int part = step(kWarps, warp_mass);
   if (part < 0) return {-1, 1, 0.f, 0};
   const int begin = part * w.each, n = (min(begin + w.each, w.u1 - w.u0) - begin) * kPer;
   const auto unit_sum = [&](int i) -> F {
     if constexpr (MODE == W32) return sums[begin + i] * rescale(tops[begin + i], base, w.c);
     else return sums[begin * kPer + i];
   };
-  const int u = pick<F>(n, unit_sum, &t, &unsure);
+  const int u = step(n, unit_sum);
   if (u < 0) return {-1, 1, 0.f, 0};
   const F mass = unit_sum(u);
   const int first = (w.u0 + begin) * kUnit + u * kSpan<MODE> - w.shift, i0 = first + lane * kLane;
@@ -534,12 +548,12 @@ CFB_DEV Found find(const Row<T>& w, const Shared* sh, const float* tops, const F
     }
     a += (v[0] + v[1]) + (v[2] + v[3]);
   }
-  const int who = pick<F>(32, [&](int) { return a; }, &t, &unsure);
+  const int who = step(32, [&](int) { return a; });
   if (who < 0) return {-1, 1, 0.f, 0};
   const int i = first + who * kLane + lane;
   const float l = lane < kLane && i >= 0 && i < w.V ? to_float(w.p[i]) : -INFINITY;
   const F y = value_of<MODE, SLOW>(w, l, lane < kLane ? i : -1, base, iz, table);
-  const int e = pick<F>(32, [&](int) { return y; }, &t, &unsure);
+  const int e = step(32, [&](int) { return y; });
   if (e < 0) return {-1, 1, 0.f, 0};
   if constexpr (kNarrow<MODE>) {
     float off = band + 18.f * (float)kRound * mass;
@@ -597,8 +611,8 @@ template <typename T> struct Team {
   CFB_DEV float band(const Row<T>& w, float z) const { return mean_off(w, z) + 20.f + (float)w.each * 0.02f; }
 
   // The CTAs' totals, handed over by the cluster's barrier -> the row's; who has the threshold u of it. SCALED: each
-  // total is relative to its CTA's largest; greedy: the owner is the first that has the row's largest.
-  template <bool SCALED> CFB_DEV void exchange(const Row<T>& w, double u, bool greedy) {
+  // total is relative to its CTA's largest; greedy: the owner is the first that has the row's largest. floor: as in pick.
+  template <bool SCALED> CFB_DEV void exchange(const Row<T>& w, double u, bool greedy, double floor) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (threadIdx.x < 32) {
@@ -623,8 +637,9 @@ template <typename T> struct Team {
       // (the sum before, not the one behind less this part's, which would lose small ones)
       const double up = __shfl_up_sync(0xffffffffu, scan, 1), before = lane ? up : 0.;
       const double t = threshold(u, whole);
-      unsigned hit = __ballot_sync(0xffffffffu, m > 0 && before <= t && t < scan);
-      if (!hit) hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, m > 0) | 1u));
+      // (not by `before`: the sums of two lanes may round apart, and t fall between one's end and the next one's start)
+      unsigned hit = __ballot_sync(0xffffffffu, m > floor && t < scan);
+      if (!hit) hit = 1u << (31 - __clz(__ballot_sync(0xffffffffu, m > floor) | 1u));
       if (SCALED && (greedy || nan)) hit = __ballot_sync(0xffffffffu, nan ? p.nan != 0 : p.top == top);
       if (lane == rank) {
         sh->before = before;
@@ -675,7 +690,7 @@ template <typename T> struct Team {
       if (lane < kWarps) sh->warp_sum[lane] = scaled;      // (relative to the CTA's largest from here on)
       if (lane == 0) sh->pub[ph] = {top, nan, nan ? 0. : total};
     }
-    exchange<true>(w, number(raw, size), greedy);
+    exchange<true>(w, number(raw, size), greedy, 0.);
   }
 
   // a pass that knows the row's largest, and its sum where it needs it
@@ -684,21 +699,21 @@ template <typename T> struct Team {
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) hand_over<float>();
-    exchange<false>(w, u, false);
+    exchange<false>(w, u, false, 0.);
   }
   template <int MODE, bool SLOW> CFB_DEV void exact_pass(const Row<T>& w, double u) {
     exact_units<MODE, SLOW>(w, sh, sh->top, MODE == R64 ? 1. / sh->z : 0., static_cast<double*>(room));
     __syncthreads();
     ph ^= 1;
     if (threadIdx.x < 32) hand_over<double>();
-    exchange<false>(w, u, false);
+    exchange<false>(w, u, false, kNothing<MODE, SLOW>);
   }
 
   // Warp 0 of the owner: the token of the last pass's threshold
   CFB_DEV Found found(const Row<T>& w, double u) const {
     if (isinf(sh->top)) return {-1, 1, 0.f, 0};            // several of +inf: in 64 bits
     const float whole = (float)sh->whole;
-    return find<W32, false>(w, sh, tops, static_cast<const float*>(room), (float)(threshold(u, sh->whole) - sh->before), 0.,
+    return find<W32, false>(w, sh, tops, static_cast<const float*>(room), 0.f, (float)(threshold(u, sh->whole) - sh->before), 0.,
                             sh->pub[ph].top, (float)kRound * (band(w, whole) * whole + 6.f * (float)(sh->end - sh->before)));
   }
   // (from what is left above q, R: every p is off by its exponent's error and 6 u, and all of them by 1 / Z's, of which
@@ -708,11 +723,11 @@ template <typename T> struct Team {
     const float whole = (float)sh->whole, z = (float)sh->z, mean = mean_off(w, z), other = fmaxf(1.f - whole, 0.f), q = (float)w.each;
     const float off = (float)kRound * (mean * (1.f + other) + 6.f + (39.f + 0.04f * q) * other + (22.f + 2.f * q) * whole);
     if (!(whole > 2.f * off)) return {-1, 1, 0.f, 0};
-    return find<R32, false>(w, sh, tops, static_cast<const float*>(room), (float)(threshold(u, sh->whole) - sh->before),
+    return find<R32, false>(w, sh, tops, static_cast<const float*>(room), 0.f, (float)(threshold(u, sh->whole) - sh->before),
                             (double)reciprocal(z), 0.f, off);
   }
   template <int MODE, bool SLOW> CFB_DEV Found found64(const Row<T>& w, double u) const {
-    return find<MODE, SLOW>(w, sh, tops, static_cast<const double*>(room), threshold(u, sh->whole) - sh->before,
+    return find<MODE, SLOW>(w, sh, tops, static_cast<const double*>(room), sh->before, threshold(u, sh->whole),
                             MODE == R64 ? 1. / sh->z : 0., 0.f, 0.f);
   }
 
@@ -765,7 +780,8 @@ CFB_DEV RowResult exact_steps(Team<T> team, const Row<T>& w, const Asked& a, dou
   return result(f.token, 0, f.logit);
 }
 template <bool CHAIN, typename T> __device__ __noinline__ RowResult exact_row(Team<T> team, Row<T> w, Asked a) {
-  // (weights below 2^-1000, which the fast ones cut, count where the threshold is that small, and only there)
+  // (weights below 2^-1000, which the fast ones cut, count where the threshold is that small, and only there: all of a row's
+  // together are below 2^-78 of a threshold of 2^-900)
   const double u = number(a.raw_u, a.size), v = number(a.raw_v, a.size);
   const float top = team.sh->top, depth = (top - lowest_logit(top, w.c)) * w.c;       // (fp32 may not hold such a logit)
   return isinf(top) || !(depth > 990.f && depth < 1010.f) || v < 0x1p-900 ? exact_steps<CHAIN, true>(team, w, a, u, v)
