@@ -827,9 +827,9 @@ CFB_DEV RowResult resolve(Team<T>& team, const Row<T>& w, const Asked& a, int* h
   if (CHAIN && a.drafted && !plain) {
     if (in) {
       const float z = (float)sh.z, x = (of_draft - sh.top) * w.c, p = weight(of_draft, sh.top, w.c) * reciprocal(z);
-      const float uq = (float)number(a.raw_u, a.size) * q;
-      // (every CTA computes the same)
-      const float off = p * (float)kRound * (2.f * team.band(w, z) + 2.08f * fabsf(x) + 16.f);
+      const float uq = (float)(number(a.raw_u, a.size) * (double)q);         // (u alone may be below fp32's range)
+      // (every CTA computes the same) Weights below 2^-126 are flushed to 0, and uq and p rounded to 2^-149 there: 2^-124 for it
+      const float off = p * (float)kRound * (2.f * team.band(w, z) + 2.08f * fabsf(x) + 16.f) + 0x1p-124f;
       if (!(fabsf(uq - p) > off)) {
         if constexpr (LAZY) return later(kUndecided);
         else return taken(exact_row<CHAIN>(team, w, a));
