@@ -67,7 +67,7 @@ struct VerifyArgs {
   const float* temperature;
   int batch, max_spec, num_drafts;
   int32_t* out_tokens; int32_t* out_path; int32_t* out_len; float* out_logp;
-  RowResult* rows;                                         // [num_rows]
+  RowResult* rows;                                         // [batch, max_spec + 1], where all rows are taken at once
   unsigned* counter;                                       // [batch]
   int* err;
 };
@@ -909,10 +909,13 @@ __global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const _
   const long long drafts = (long long)A.cu_draft[b] - d0, start = A.cu_sampled[b] - (drafts + 1);
   const int before = b ? A.cu_sampled[b - 1] : 0;
   const float temp = A.temperature ? A.temperature[b] : 1.f;
-  // offsets that do not describe rows of this logits matrix (or drafts), of this request alone, are never dereferenced
+  // Offsets that do not describe rows of this logits matrix (or drafts), or rows before the end of the last request's, are never
+  // dereferenced. (Whether they fall on those of a request further back would take a look at all of them: such a request
+  // reads what is another's, and writes to places of its own.)
   const bool sane = drafts >= 0 && drafts <= A.max_spec && start >= max(before, 0) && start + drafts < A.num_rows && d0 >= 0 &&
                     d0 + drafts <= A.num_drafts;
   const int n = (int)drafts, s0 = (int)start;
+  RowResult* const rows = A.rows + (long long)b * (A.max_spec + 1);
   // a thread's node of the tree, on its way while the rows are taken
   const bool node = !CHAIN && sane && (int)threadIdx.x < n;
   const int my_parent = node ? A.parents[d0 + threadIdx.x] : 0, my_token = node ? A.draft_tokens[d0 + threadIdx.x] : 0;
@@ -930,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const _
     if (rank == holder && threadIdx.x < 32) {              // count the row in, and tell the cluster if it was the last
       int last = 0;
       if (threadIdx.x == 0) {
-        if (live) A.rows[s0 + j] = r;
+        if (live) rows[j] = r;
         last = atom_add_acqrel(A.counter + b, 1u) + 1 == gridDim.y;
         if (last) A.counter[b] = 0u;
       }
@@ -943,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const _
   if (sane) {
     for (int i = threadIdx.x; i <= n; i += kThreads) {
       if constexpr (FLAT) {
-        const RowResult* const r = A.rows + s0 + i;
+        const RowResult* const r = rows + i;
         const int2 t = __ldcg(reinterpret_cast<const int2*>(r));
         s_row[i] = {t.x, t.y, __ldcg(&r->scaled), __ldcg(&r->mass)};
         s_next[i] = n;
@@ -1102,6 +1105,9 @@ cfb_status launch(const VerifyArgs& a, cudaStream_t st) {
   return cfb_launch_status("verify_kernel");
 }
 
+// rows' results that the workspace of a call over num_rows rows holds
+long long most_results(int num_rows) { return 4ll * num_rows + 256; }
+
 template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaStream_t st) {
   // All rows at once take the GPU's whole width, but read what no walk reaches, the more so the more rows a request has, and
   // with more rows there are fewer CTAs for what the walk takes again. Measured, all rows at once / walk, us. Without draft probabilities,
@@ -1110,7 +1116,7 @@ template <bool CHAIN> cfb_status launch_as(const VerifyArgs& a, int dtype, cudaS
   // 6 rows, V = 248320: 1 request 17 / 24, 2 34 / 34, 4 53 / 51, 8 68 / 54; V = 32003: 16 41 / 46, 48 78 / 61.
   // (and a cluster goes to every row that a request may have: many that have none would cost more than they save)
   const long long most = (CHAIN ? 5ll : a.num_rows <= 16ll * a.batch ? 24ll : 12ll) << 20;      // elements
-  const bool flat = (long long)a.V * a.num_rows <= most && (a.max_spec + 1ll) * a.batch <= 4ll * a.num_rows + 256;
+  const bool flat = (long long)a.V * a.num_rows <= most && (a.max_spec + 1ll) * a.batch <= most_results(a.num_rows);
   const auto go = [&](auto t) {
     using T = decltype(t);
     return flat ? launch<T, CHAIN, true>(a, st) : launch<T, CHAIN, false>(a, st);
@@ -1148,7 +1154,7 @@ cfb_status common_args(VerifyArgs& a, const void* logits, int64_t ld, int num_ro
 
 extern "C" size_t cfb_verify_workspace(int num_rows, int batch) {
   if (num_rows <= 0 || batch <= 0) return 0;
-  return kCounters + (size_t)num_rows * sizeof(RowResult);
+  return kCounters + (size_t)most_results(num_rows) * sizeof(RowResult);
 }
 
 extern "C" cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, int num_rows, int V, int dtype,

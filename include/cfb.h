@@ -408,7 +408,9 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * probabilities under w (of a greedy request: tau = 1), 0 after them.
  * logits and the random numbers: element-aligned; any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
  * ZERO before its first use (each launch leaves it so that the next, of any size, may follow), for calls ordered on
- * one stream. err as there. Supported: max_spec_len <= 1024, V <= 2^22 - 8, batch <= 65535. */
+ * one stream. err as there; a request that starts before the end of the one before it emits nothing either. Offsets that
+ * fall back further (rows or drafts of requests before that) are not looked for: what they name within the arrays is
+ * read, and only that request's output depends on it. Supported: max_spec_len <= 1024, V <= 2^22 - 8, batch <= 65535. */
 size_t cfb_verify_workspace(int num_rows, int batch);
 cfb_status cfb_tree_verify_sampled(const void* logits, int64_t ld, int num_rows, int V, int dtype,
                                    const int32_t* cu_num_draft, const int32_t* cu_num_sampled,
