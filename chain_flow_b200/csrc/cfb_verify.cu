@@ -1028,7 +1028,8 @@ __global__ void __launch_bounds__(kThreads, CHAIN ? 3 : 4) verify_kernel(const _
     if (p <= pos) {
       const RowResult r = s_row[FLAT ? s_node[p] + 1 : p];
       token = r.token;
-      if (token >= 0) logp = (float)(r.scaled * 0.6931471805599453) - log1pf((float)(r.mass - 1.));      // (mass >= 1)
+      // formed in 64 bits and rounded once; the mass is the first pass's sum where the row was not taken again
+      if (token >= 0) logp = (float)(r.scaled * 0.6931471805599453 - log(r.mass));
     }
     A.out_tokens[(long long)b * (A.max_spec + 1) + p] = token;
     A.out_logp[(long long)b * (A.max_spec + 1) + p] = logp;

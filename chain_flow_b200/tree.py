@@ -199,8 +199,8 @@ class SampledVerifier(_ProbabilityVerifier):
         [B, max_spec + 1], views of this verifier's buffers, -1 (logprobs 0) after a request's tokens. logits, offsets,
         draft_tokens and parents as TreeVerifier takes them; uniforms fp32 or fp64 [rows] in [0, 1), one number a logits
         row; temperature [B] (None: 1 for all; 0: greedy). logprobs are the output tokens' log probabilities under
-        softmax(logits / temperature) (greedy requests: softmax(logits)). A token of logit -inf is never drawn; a row
-        of nothing else ends its walk with token -1."""
+        softmax(logits / temperature) (greedy requests: softmax(logits)), off by less than 2^-17 and a rounding to fp32. A
+        token of logit -inf is never drawn; a row of nothing else ends its walk with token -1."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self(logits, cu_num_draft, cu_num_sampled, draft_tokens, parents, uniforms, temperature)

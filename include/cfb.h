@@ -405,7 +405,8 @@ cfb_status cfb_tree_verify_greedy(const void* logits, int64_t ld, int num_rows, 
  * stay, resample[r] draws the bonus token from the last row. A greedy row keeps d if it is the
  * argmax. A draft outside the vocabulary is refused.
  * Outputs as cfb_tree_verify_greedy, and logprobs fp32 [batch, max_spec_len + 1]: the output tokens' log
- * probabilities under w (of a greedy request: tau = 1), 0 after them.
+ * probabilities under w (of a greedy request: tau = 1), 0 after them; formed in 64 bits and rounded once, from a
+ * sum of weights that is off by less than 2^-17 of itself (fp32 weights, where the decision needed no others).
  * logits and the random numbers: element-aligned; any ld >= V. ws: cfb_verify_workspace(num_rows, batch) bytes, 256-byte aligned,
  * ZERO before its first use (each launch leaves it so that the next, of any size, may follow), for calls ordered on
  * one stream. err as there; a request that starts before the end of the one before it emits nothing either. Offsets that
