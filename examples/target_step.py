@@ -100,8 +100,9 @@ class TargetLayers:
 
 
 class SampledTarget(TargetLayers):
-    """The same layers with pages from a pool, sampled verification and samples that share a prompt's pages. A tree's
-    nodes are in the cache while they are verified, node i at position kv_len + i."""
+    """The same layers with pages from a pool, sampled verification and samples that share a prompt's pages. A step
+    begins with the token that the last one ended with (its bonus token; after a prompt, the one drawn from its last row):
+    that joins the context, and the tree hangs below it, node i at the position behind it + i while the nodes are verified."""
 
     def __init__(self, requests: int, max_len: int, nodes: int, dtype=torch.float16, cache_dtype=torch.float8_e4m3fn, seed: int = 0):
         super().__init__(requests, max_len, nodes, dtype, cache_dtype, seed)
@@ -119,10 +120,14 @@ class SampledTarget(TargetLayers):
         self.granted.append(self.pool.fork(self.table, self.kv_len, parent, child, self.cache))
         self.state[child.long()] = self.state[parent.long()]
 
-    def sampled_step(self, x, parents, tokens, logits, uniforms, temperature=None):
+    def sampled_step(self, x, parents, tokens, logits, uniforms, temperature=None, committed=None):
         """A tree of N nodes a request that carry ``tokens`` [S, N]; logits [S * (N + 1), V] of the committed token's row
-        and the nodes', request after request, and a random number for each. Returns both layers' outputs and the
-        verifier's (tokens, path, length, log probabilities); the accepted nodes have joined the contexts."""
+        and the nodes', request after request, and a random number for each. ``committed``: the committed tokens'
+        projections (S tokens), which join the contexts and states first (None: they have joined already, by a decode).
+        Returns both layers' outputs of the nodes and the verifier's (tokens, path, length, log probabilities); the accepted
+        nodes have joined the contexts. The last token of a request is the next step's committed one."""
+        if committed is not None:
+            self.decode(committed)
         S, N = parents.shape
         self.granted.append(self.pool.reserve(self.table, self.kv_len, self.kv_len + N))
         request, node = self.slot.long().repeat_interleave(N), torch.arange(N, device="cuda").repeat(S)
@@ -188,7 +193,7 @@ def main():
 def sampled(a, news, vocab: int = 1000, steps: int = 3):
     """Samples of each prompt: the prompts' pages forked, a few sampled steps, a decode."""
     P, S = len(news), len(news) * a.samples
-    layers = SampledTarget(S, max(news) + steps * a.nodes + 1, a.nodes,
+    layers = SampledTarget(S, max(news) + steps * (a.nodes + 1) + 1, a.nodes,
                            cache_dtype=torch.float8_e4m3fn if a.cache == "e4m3" else torch.float16)
     layers.prompt(projections(sum(news), seed=1), news + [0] * (S - P))
     child = torch.arange(P, S, device="cuda")
@@ -202,9 +207,9 @@ def sampled(a, news, vocab: int = 1000, steps: int = 3):
         tokens = rows.gather(2, (torch.arange(a.nodes, device="cuda") % 3).expand(S, -1)[..., None])[..., 0]
         uniforms = torch.rand(S * (a.nodes + 1), device="cuda", generator=g)
         _, _, out = layers.sampled_step(projections(S * a.nodes, seed=2 + step), parents, tokens, logits, uniforms,
-                                        torch.full((S,), a.temperature, device="cuda"))
+                                        torch.full((S,), a.temperature, device="cuda"), projections(S, seed=20 + step))
         print("step", step, "accepted", out[2].tolist(), "tokens", [[t for t in row if t >= 0] for row in out[0].tolist()])
-    out = layers.decode(projections(S, seed=9))
+    out = layers.decode(projections(S, seed=9))      # the last step's bonus tokens
     layers.attention.check()
     layers.chunks.check()
     print("decoded", *(tuple(t.shape) for t in out), "contexts", layers.kv_len.tolist(), "pages held", int((layers.pool.refs > 0).sum()),
