@@ -249,3 +249,10 @@ def int32(t):
     """t as a contiguous int32 tensor (itself if it is one)."""
     import torch
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def int32_indices(t):
+    """t as a contiguous int32 tensor; what 32 bits do not hold becomes their largest or smallest number, which is outside every
+    range of tokens, pages and positions (to(int32) keeps the low bits, which may name one)."""
+    import torch
+    return int32(t.clamp(-1 << 31, (1 << 31) - 1) if t.dtype == torch.int64 else t)

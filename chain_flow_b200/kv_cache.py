@@ -167,7 +167,7 @@ def _index(t, name: str, what: str, dev: int, shape):
     if t.get_device() != dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != tuple(shape):
         _lib.require_cuda(t, name)
         raise _lib.CfbError(f"{what}: {name} must be integers {list(shape)} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
-    return _lib.int32(t)
+    return _lib.int32_indices(t)
 
 
 def keep_path(caches, page_table, base, path, length, stream=None) -> None:

@@ -145,7 +145,7 @@ class _ProbabilityVerifier:
         if t.get_device() != self._dev or t.is_floating_point() or t.dtype == torch.bool or tuple(t.shape) != shape:
             _lib.require_cuda(t, name)
             self._refuse(name, f"must be integers {list(shape)} on cuda:{self._dev}, got {t.dtype} {list(t.shape)} on {t.device}")
-        return _lib.int32(t)
+        return _lib.int32_indices(t)
 
     def _numbers(self, t, name, n):
         if t.get_device() != self._dev or t.dtype not in (torch.float32, torch.float64) or t.shape != (n,):
