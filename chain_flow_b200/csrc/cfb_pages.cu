@@ -435,6 +435,9 @@ extern "C" cfb_status cfb_kv_keep(const cfb_kv_cache* const* caches, int n_cache
                                   const int32_t* count, int max_len, int B, void* stream) {
   if (const cfb_status s = check_layers(caches, n_caches)) return s;
   if (B < 0 || max_len < 0 || table_width < 0 || table_stride < table_width || path_stride < max_len) return CFB_ERR_INVALID_ARG;
+  for (int i = 0; i < n_caches; ++i)                       // (moved twice at once, rows would be read behind the first move's writes)
+    for (int j = 0; j < i; ++j)
+      if (caches[i]->k == caches[j]->k || caches[i]->v == caches[j]->v) return CFB_ERR_INVALID_ARG;
   if (B == 0 || n_caches == 0 || max_len == 0 || table_width == 0) return CFB_OK;
   if (!page_table || !base || !path || !count) return CFB_ERR_INVALID_ARG;
   if (max_len > kMaxPath) return CFB_ERR_UNSUPPORTED;

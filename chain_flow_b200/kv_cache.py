@@ -193,6 +193,8 @@ def keep_path(caches, page_table, base, path, length, stream=None) -> None:
                                      length.data_ptr(), S, B, _lib.stream_of(dev, "keep_path"))
     if status:
         _check_layers(caches, "keep_path")
+        if n > 1 and any(len({t.data_ptr() for t in ts}) < n for ts in ([c.k for c in caches], [c.v for c in caches])):
+            raise _lib.CfbError("keep_path: a cache is given twice")
         _lib.check(status, "cfb_kv_keep")
 
 

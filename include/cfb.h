@@ -464,7 +464,7 @@ cfb_status cfb_kv_write(const cfb_kv_cache* c, const void* key, int64_t sk_t, in
 cfb_status cfb_kv_read(const cfb_kv_cache* c, const int64_t* slots, int T, void* key, int64_t sk_t,
                        int64_t sk_h, void* value, int64_t sv_t, int64_t sv_h, int dtype, void* stream);
 
-/* A step's accepted rows moved together, in the caches of all of a target's layers (n_caches pointers to caches of one
+/* A step's accepted rows moved together, in the caches of all of a target's layers (n_caches pointers to distinct caches of one
  * geometry: all but the buffers' addresses alike). The nodes of request b's tree lie at the positions base[b] + node of its
  * pages page_table[b * table_stride + j]; row base[b] + path[b * path_stride + j] of every layer and head moves to
  * base[b] + j, for j < count[b] (of at most max_len). path: the accepted nodes, increasing (path[j] >= j), as the verifiers'

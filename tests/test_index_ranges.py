@@ -63,3 +63,29 @@ def test_other_integer_types_are_taken():
         assert pool.reserve(table, _i32([0, 0]).to(dt), _i32([17, 3]).to(dt)).tolist() == [1, 1]
         assert table.tolist() == [[0, 1, -1], [2, -1, -1]]
         pool.release(table, _i32([17, 3]).to(dt))
+
+
+def test_a_cache_given_twice():
+    """Its rows would be moved twice at once."""
+    from chain_flow_b200 import _lib
+    from test_cache_pages import FAKE, _array, _cache
+    lib = _lib.load()
+    a, b, c = _cache(), _cache(k=FAKE + 16 * 4096, v=FAKE + 16 * 4096), _cache(k=FAKE + 32 * 4096)
+    call = lambda *x: lib.cfb_kv_keep(_array(*x), len(x), FAKE, 4, 4, FAKE, FAKE, 5, FAKE, 5, 0, None)  # noqa: E731
+    assert call(a) == 0 and call(a, b) == 0 and call(a, a) == 1 and call(a, b, a) == 1 and call(a, b, c) == 1      # (c: a's values)
+
+
+@pytest.mark.gpu
+def test_a_cache_given_twice_in_python():
+    from chain_flow_b200 import _lib
+    from chain_flow_b200.kv_cache import copy_pages, keep_path
+    caches = _caches(2, 6, 16, 2, 64, torch.float16)
+    want = _pools(caches)
+    for twice in (caches + caches[:1], [caches[1]] * 2):
+        with pytest.raises(_lib.CfbError, match="twice"):
+            keep_path(twice, _i32([[0, 1]]), _i32([0]), _i32([[3, 5]]), _i32([2]))
+    _same(caches, want)
+    copy_pages(caches + caches[:1], _i32([0]), _i32([4]))                          # the same bytes twice
+    for t in want:
+        t[4] = t[0]
+    _same(caches, want)
