@@ -146,3 +146,22 @@ def test_parts_whose_sums_round_apart():
     assert float(torch.exp(logits[0, 5].double())) < 2.0 ** -53
     got = _sampled(SampledVerifier(1, 1, 0), logits, _alone(1), torch.tensor([0.25]))
     assert int(got[0][0, 0]) in at[:2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("walk", [False, True])
+@pytest.mark.parametrize("n", [3, 7, 100, 999])
+def test_borders_that_are_no_dyadic_numbers(n, walk):
+    """k / n rounded to 64 bits, and its neighbours: u times the (exact) sum is rounded as the definition rounds it."""
+    from chain_flow_b200.tree import SampledVerifier
+    V = 20011
+    g = torch.Generator().manual_seed(n)
+    ks = (torch.arange(n) if n < 20 else torch.randint(n, (20,), generator=g)).tolist()
+    u = torch.tensor([x for k in ks for x in (k / n, math.nextafter(k / n, 1), max(math.nextafter(k / n, 0), 0))], dtype=torch.float64)
+    for mask, top in ((-math.inf, 3.0), (torch.finfo(torch.float16).min, -2.0)):
+        logits = torch.full((len(u), V), mask, dtype=torch.float16)
+        for row in logits:
+            row[_survivors(V, n, "anywhere", g)] = top
+        flat = _alone(len(u))
+        ver = SampledVerifier(len(u), len(u), WALK if walk else 0)
+        _check(_sampled(ver, logits, flat, u), oracle.tree_verify_sampled(logits, *flat, u, None, ver.max_spec))
