@@ -883,9 +883,11 @@ CFB_DEV void row_of(const VerifyArgs& A, int rank, int per, int b, int d0, int n
 }
 
 // Bound by latency, not by a pipe (64 trees of 41 bf16 rows over 248320 tokens: SM 25 %, DRAM 19 %; a warp waits longest at
-// barriers, for another CTA's totals or warp 0's descent): the rows of a walk come one after another, about 9500
-// cycles each, and one that goes through 64 bits takes 16000 to 80000 more. Measured at V = 248320: one chain of 5 drafts 13
-// us, one tree of 40 22, 64 trees 69 (the visited rows' bytes: 14), one chain with draft probabilities 33, 48 of them 98 (17);
+// barriers, for another CTA's totals or warp 0's descent): the rows of a walk come one after another. Cycles of a row, in a
+// walk alone on the GPU / among 64 trees: units 3500 / 8900, reduction 600 / 1300, exchange 1900 / 3000, descent 3400 / 3700,
+// handing over 900 / 1000; together 10400 / 17900, five of which are the deepest walk. A row that goes through 64 bits
+// takes 17000 / 31500 more (with draft probabilities up to 80000). Measured at V = 248320: one chain of 5 drafts 13
+// us, one tree of 40 22, 64 trees 68 (the visited rows' bytes: 14), one chain with draft probabilities 33, 48 of them 98 (17);
 // without the rows in 64 bits 12, 17, 54, 27 and 63.
 // FLAT: a cluster a row (grid.y: rows of a request, grid.z: requests), every row at once; the request's last
 // cluster walks, and takes again what was left for the walk where it comes by. Otherwise a cluster a request (grid.y), which
